@@ -87,6 +87,8 @@ _SIGNATURES = {
     "jb_activate": "ppilip", "jb_tanh_norm": "ppppffippfpipiiplplp",
     "jb_latent_heads": "piiiiiipppiiiipfpppip", "jb_latent_queries": "piiiiiiippppiiipfppip", "jb_latent_values": "pppippiipiiiiiip",
     "jb_latent_down": "piipfpiippiiippppplip",
+    "jb_step_tables": "ppppppppppppppppppiiiiiiiip", "jb_attention_prefix": "ppppipipipppiiiiiifp",
+    "jb_verify_drafts": "pppppppppppiiiifp",
     "jb_gather_rows": "ppiipppiiip", "jb_latent_attention": "ppppppppiiiiiiifiipp", "jb_attention_tc_matrix": "ppppppiiiiiiiifpipp",
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "u": ctypes.c_ulonglong,
@@ -2400,3 +2402,109 @@ def latent_attention(q: torch.Tensor, pages: torch.Tensor, out: Optional[torch.T
         n_seqs, max_q_len, heads, stored, n, page_size, block_table.shape[1], float(scale), int(n_splits), blocks,
         _ptr(kernel_status(q.device)), _stream()), "latent_attention")
     return (part_o, part_ml, n_splits) if n_splits > 1 else None
+
+
+# -- a step of sequences that share a prefix, with drafted tokens -------------------------------------------------------
+def step_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, rows: torch.Tensor, old_table: torch.Tensor, old_held: torch.Tensor,
+                prefix_pages: torch.Tensor, old_free: torch.Tensor, old_n_free: torch.Tensor, *, q_start: torch.Tensor,
+                kv_len: torch.Tensor, positions: torch.Tensor, token_seq: torch.Tensor, dest_rows: torch.Tensor, table: torch.Tensor,
+                held: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor, missing: torch.Tensor, page_size: int) -> None:
+    """The index arrays of a step on the device, from request lengths; all int32, in one launch.
+
+    Request b has lengths[b] tokens in the cache and brings new_tokens[b] more.  It goes on with the pages that row rows[b] of the
+    last step's `old_table` lists (its first old_held[row] entries), or begins (rows[b] = -1) with the shared `prefix_pages`, which
+    stand in front of every row and are never given back.  Two requests do not go on with the same row.  A row nobody goes on
+    with gives its own pages back: they follow the free pages old_free[:old_n_free], row after row.  Requests take the pages they
+    lack from the front of that list, in order; free_pages[:n_free] is what is left of it.
+
+    Made besides: q_start [B + 1] and kv_len [B]; table [B, width] (-1 where a row holds nothing), held [B]; for every place of
+    the token arrays (as many as a step is laid out for) its position, request and cache row page * page_size + row, -1 in the
+    places behind the last token.  `missing`: pages that neither the free list nor the table's width could give; where it is not
+    zero the cache rows of tokens without a page are -1, and the step must not run.  Outputs are tensors of their own, not inputs."""
+    B, (B0, W0), (_, W) = lengths.shape[0], old_table.shape, table.shape
+    T, N, P = positions.shape[0], old_free.shape[0], prefix_pages.shape[0]
+    for t, name, shape in ((lengths, "lengths", (B,)), (new_tokens, "new tokens", (B,)), (rows, "rows", (B,)), (old_table, "table", (B0, W0)),
+                           (old_held, "held pages", (B0,)), (prefix_pages, "prefix pages", (P,)), (old_free, "free pages", (N,)),
+                           (old_n_free, "number of free pages", (1,)), (q_start, "q_start", (B + 1,)), (kv_len, "kv_len", (B,)),
+                           (positions, "positions", (T,)), (token_seq, "token sequences", (T,)), (dest_rows, "cache rows", (T,)),
+                           (table, "new table", (B, W)), (held, "new held pages", (B,)), (free_pages, "new free pages", (N,)),
+                           (n_free, "new number of free pages", (1,)), (missing, "missing pages", (1,))):
+        _need(t, "step_tables " + name, torch.int32, shape)
+    if W < W0 or P > W:
+        raise KernelError(f"step_tables: a table of {W} pages a row cannot take over rows of {W0} behind {P} shared pages")
+    if any(a.numel() and a.data_ptr() == b.data_ptr() for a, b in ((table, old_table), (free_pages, old_free), (held, old_held),
+                                                                   (n_free, old_n_free), (kv_len, lengths))):
+        raise KernelError("step_tables: the new table and lists cannot lie where the old ones do")
+    _check(_lib("step_tables").jb_step_tables(
+        _ptr(lengths), _ptr(new_tokens), _ptr(rows), _ptr(old_table), _ptr(old_held), _ptr(prefix_pages), _ptr(old_free),
+        _ptr(old_n_free), _ptr(q_start), _ptr(kv_len), _ptr(positions), _ptr(token_seq), _ptr(dest_rows), _ptr(table), _ptr(held),
+        _ptr(free_pages), _ptr(n_free), _ptr(missing), B, B0, T, W0, W, P, N, int(page_size), _stream()), "step_tables")
+
+
+def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, prefix_pages: torch.Tensor,
+                     prefix_len: int, block_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, positions: torch.Tensor,
+                     nh: int, nkv: int, hd: int, page_size: int, scale: float, workspace, max_q_len: int, max_kv_len: int) -> None:
+    """Causal attention of a step's new tokens when all its sequences begin with the same `prefix_len` tokens, whose keys and
+    values lie once in the cache, in `prefix_pages`.  kv_len [n_seqs] counts the prefix too; the key of position prefix_len + i of a
+    sequence is row i % page_size of page block_table[sequence, i // page_size] (a table of whole rows, shared pages in front,
+    is handed over as table[:, shared:]).  q and out: [T, nh hd], float32 or bfloat16 as the cache; positions [T].  Rows behind
+    q_start[n_seqs] are left as they are.  max_q_len, max_kv_len: at least the longest of the step."""
+    T, n_seqs, prefix_len = q.shape[0], kv_len.shape[0], int(prefix_len)
+    _need(q, "attention q", None, (T, nh * hd))
+    _need(out, "attention out", q.dtype, (T, nh * hd))
+    _need(prefix_pages, "prefix pages", torch.int32)
+    _need(q_start, "q_start", torch.int32, (n_seqs + 1,))
+    _need(kv_len, "kv_len", torch.int32, (n_seqs,))
+    _need(positions, "positions", torch.int32, (T,))
+    if _checks[0]:
+        for t, name in ((k_cache, "k cache"), (v_cache, "v cache")):
+            _need(t, name, q.dtype)
+            if t.dim() != 4 or tuple(t.shape[1:]) != (nkv, page_size, hd) or t.shape[0] != k_cache.shape[0]:
+                raise KernelError(f"attention_prefix: cache shape {tuple(t.shape)} is not [pages, {nkv}, {page_size}, {hd}]")
+        if not block_table.is_cuda or block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n_seqs:
+            raise KernelError(f"attention_prefix: the block table must be int32 [{n_seqs}, pages] on the device")
+        if block_table.shape[1] > 1 and block_table.stride(1) != 1:
+            raise KernelError("attention_prefix: a row of the block table must lie in one piece")
+    if prefix_len < 0 or prefix_pages.shape[0] * page_size < prefix_len:
+        raise KernelError(f"attention_prefix: {prefix_pages.shape[0]} pages do not hold a prefix of {prefix_len} tokens")
+    if max_q_len < 0 or block_table.shape[1] * page_size < max_kv_len - prefix_len:
+        raise KernelError(f"attention_prefix: {block_table.shape[1]} pages a sequence do not hold {max_kv_len} tokens behind {prefix_len}")
+    _check(_lib("prefix_attention").jb_attention_prefix(
+        _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), dtype_code(q.dtype), _ptr(prefix_pages), prefix_len, _ptr(block_table),
+        block_table.stride(0), _ptr(q_start), _ptr(kv_len), _ptr(positions), T, n_seqs, nh, nkv, hd, page_size, float(scale), _stream()),
+        "attention_prefix")
+
+
+def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, accepted: torch.Tensor,
+                  out_tokens: torch.Tensor, logprobs: torch.Tensor, kept: torch.Tensor, temperature: float, u_accept: torch.Tensor,
+                  u_draw: torch.Tensor, draft_probs: Optional[torch.Tensor], workspace) -> None:
+    """Drafted tokens against the target's logits.  Sequence b brought rows q_start[b] .. q_start[b + 1] - 1 of the step: the token it
+    ended with and its drafts; logits [T, V] (float32), tokens [T].  With p the softmax of the row before at `temperature` and q the
+    drafting model's probabilities draft_probs[t] (float32 [T, V]; None: the drafts were looked up, q is 1), the draft of row t is
+    accepted while u_accept[t] q(d) < p(d).  The row of the first refusal, or the last, gives one more token: the lowest v whose
+    cumulative weight passes u_draw[b] of all, the weights being max(p - q, 0) after a refusal (p without the draft where q is 1; p
+    if nothing is left), else p.  Temperature 0: drafts must be the argmax, the token is the argmax (lowest index).  Logits of
+    -inf, or that are not numbers, have no weight; a draft outside the vocabulary is refused.
+
+    Out: accepted [B]; out_tokens [B, width], the accepted drafts and the token after them, -1 behind; logprobs [B, width], their
+    log-probabilities under the target (at temperature 1 if it is 0), 0 behind; kept [B], the cached tokens that stay: kv_len less
+    the refused drafts.  A sequence without rows gets -1 and keeps kv_len.  Drafts past `width` - 1 are refused."""
+    T, V = logits.shape
+    B, width = accepted.shape[0], out_tokens.shape[1]
+    _need(logits, "verify logits", torch.float32)
+    _need(tokens, "verify tokens", torch.int32, (T,))
+    _need(q_start, "q_start", torch.int32, (B + 1,))
+    _need(kv_len, "kv_len", torch.int32, (B,))
+    _need(accepted, "accepted drafts", torch.int32)
+    _need(out_tokens, "verified tokens", torch.int32, (B, width))
+    _need(logprobs, "log-probabilities", torch.float32, (B, width))
+    _need(kept, "kept tokens", torch.int32, (B,))
+    _need(u_accept, "numbers of the tests", torch.float32, (T,))
+    _need(u_draw, "numbers of the draws", torch.float32, (B,))
+    if draft_probs is not None:
+        _need(draft_probs, "draft probabilities", torch.float32, (T, V))
+    if not 0.0 <= temperature < float("inf"):
+        raise KernelError(f"verify_drafts: temperature {temperature}")
+    _check(_lib("verify").jb_verify_drafts(
+        _ptr(logits), _ptr(tokens), _ptr(q_start), _ptr(kv_len), _ptr(u_accept), _ptr(u_draw), _ptr(draft_probs), _ptr(accepted),
+        _ptr(out_tokens), _ptr(logprobs), _ptr(kept), T, B, V, width, float(temperature), _stream()), "verify_drafts")
