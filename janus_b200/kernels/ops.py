@@ -87,7 +87,8 @@ _SIGNATURES = {
     "jb_activate": "ppilip", "jb_tanh_norm": "ppppffippfpipiiplplp",
     "jb_latent_heads": "piiiiiipppiiiipfpppip", "jb_latent_queries": "piiiiiiippppiiipfppip", "jb_latent_values": "pppippiipiiiiiip",
     "jb_latent_down": "piipfpiippiiippppplip",
-    "jb_step_tables": "ppppppppppppppppppiiiiiiiip", "jb_attention_prefix": "ppppipipipppiiiiiifp",
+    "jb_step_tables": "ppppppppppppppppppiiiiiiiip", "jb_attention_prefix_f32": "pppppipiipppiiiiiifp",
+    "jb_attention_prefix_bf16": "pppppppipiipppiiiiiiifiiiipp",
     "jb_verify_drafts": "pppppppppppiiiifp",
     "jb_gather_rows": "ppiipppiiip", "jb_latent_attention": "ppppppppiiiiiiifiipp", "jb_attention_tc_matrix": "ppppppiiiiiiiifpipp",
 }
@@ -2469,10 +2470,39 @@ def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise KernelError(f"attention_prefix: {prefix_pages.shape[0]} pages do not hold a prefix of {prefix_len} tokens")
     if max_q_len < 0 or block_table.shape[1] * page_size < max_kv_len - prefix_len:
         raise KernelError(f"attention_prefix: {block_table.shape[1]} pages a sequence do not hold {max_kv_len} tokens behind {prefix_len}")
-    _check(_lib("prefix_attention").jb_attention_prefix(
-        _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), dtype_code(q.dtype), _ptr(prefix_pages), prefix_len, _ptr(block_table),
-        block_table.stride(0), _ptr(q_start), _ptr(kv_len), _ptr(positions), T, n_seqs, nh, nkv, hd, page_size, float(scale), _stream()),
-        "attention_prefix")
+    lib, step = _lib("prefix_attention"), (_ptr(prefix_pages), prefix_len, _ptr(block_table), block_table.stride(0), block_table.shape[1],
+                                           _ptr(q_start), _ptr(kv_len), _ptr(positions), T)
+    if q.dtype == torch.float32:
+        _check(lib.jb_attention_prefix_f32(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), *step, n_seqs, nh, nkv, hd, page_size,
+                                           float(scale), _stream()), "attention_prefix")
+        return
+    tiles, splits, own_slots = attention_prefix_plan(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv, hd)
+    slots = splits + own_slots if own_slots > 1 else splits
+    part_o = part_ml = None
+    if slots:
+        part_o = workspace.get("prefix_part_o", (slots * T * nh * hd,), torch.float32)
+        part_ml = workspace.get("prefix_part_ml", (slots * T * nh * 2,), torch.float32)
+    kernels = 1 if splits == 0 and prefix_len else (splits > 0) + 1 + (own_slots > 1)
+    _check(lib.jb_attention_prefix_bf16(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(part_o), _ptr(part_ml), *step,
+                                        k_cache.shape[0], n_seqs, nh, nkv, hd, page_size, float(scale), int(max_q_len), tiles, splits,
+                                        own_slots, _ptr(kernel_status(q.device)), _stream()), "attention_prefix", kernels=kernels)
+
+
+@functools.lru_cache(maxsize=4096)
+def attention_prefix_plan(T: int, n_seqs: int, max_q_len: int, prefix_len: int, max_own: int, nh: int, nkv: int, hd: int):
+    """(row tiles a CTA, ranges of the prefix, ranges of a sequence's own keys) of a bfloat16 `attention_prefix`; no ranges of the
+    prefix: tiles of one sequence each walk all their keys."""
+    group, sms = nh // nkv, SM_COUNT_TARGET // 2
+    rows = 128 // group                                    # tokens of a tile
+    pages = max(1, (max_own + 63) // 64)
+    tiles = 2 if hd <= 128 and min(T, max_q_len if T * group >= 64 * n_seqs else T) > rows else 1
+    if prefix_len and T * group >= 64 * n_seqs:
+        return tiles, 0, 1
+    blocks = (prefix_len + 127) // 128
+    splits = min(blocks, max(1, sms // (nkv * ((T + tiles * rows - 1) // (tiles * rows))))) if prefix_len else 0
+    ctas = n_seqs * nkv * ((max_q_len * group + 15) // 16)
+    own_slots = min(32, max(1, pages // 2), max(1, 2 * sms // max(1, ctas)))
+    return tiles, splits, own_slots
 
 
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, accepted: torch.Tensor,
