@@ -9,89 +9,11 @@
 // are float32.  Steps whose sequences bring many tokens fill tiles by themselves: there a tile walks the prefix and then its own
 // pages and nothing is joined (`prefix_tc_kernel<WHOLE>`).
 #include <cuda.h>
-#include <math_constants.h>
-#include <stdio.h>
-#include <stdlib.h>
 
+#include "prefix_attention.cuh"
 #include "tc_common.cuh"
 
 namespace {
-
-typedef __nv_bfloat16 bf16;
-
-constexpr int PAGE = 64;
-constexpr float LOG2E = 1.4426950408889634f;
-
-// What every kernel of a call knows.
-struct Step {
-  const int* prefix_pages;
-  const int* table;       // [n_seqs] rows of ld_table pages
-  const int* q_start;
-  const int* kv_len;
-  const int* positions;
-  int prefix_len, ld_table, width, T, n_seqs, nh, nkv, hd;
-  float scale_log2;
-};
-
-// ---------------------------------------------------------------------------
-// One (token, query head) by one warp, a lane with every 32nd number of the head: keys one after another, nothing but the
-// keys that the token sees.  The float32 engine's form, and where a tiled kernel's result is not finite: a masked key weighs 0
-// there, and 0 times what is not a number in a masked value's place would show.
-// ---------------------------------------------------------------------------
-template <typename E>
-__device__ __noinline__ void one_row(const E* __restrict__ q, const E* __restrict__ k_cache, const E* __restrict__ v_cache,
-                                     E* __restrict__ out, const Step& s, int seq, int t, int h) {
-  const int lane = threadIdx.x & 31;
-  const int kvh = h / (s.nh / s.nkv), last = min(min(s.positions[t], s.kv_len[seq] - 1), s.prefix_len + s.width * PAGE - 1);
-  float qr[8], o[8], m = -CUDART_INF_F, l = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    qr[i] = d < s.hd ? jb::to_f32(q[((size_t)t * s.nh + h) * s.hd + d]) * s.scale_log2 : 0.0f;
-    o[i] = 0.0f;
-  }
-  for (int p = 0; p <= last; ++p) {
-    const int i0 = p < s.prefix_len ? p : p - s.prefix_len;
-    const int page = p < s.prefix_len ? s.prefix_pages[i0 / PAGE] : s.table[(size_t)seq * s.ld_table + i0 / PAGE];
-    const size_t row = (((size_t)max(page, 0) * s.nkv + kvh) * PAGE + i0 % PAGE) * s.hd;
-    float x = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < s.hd) x = fmaf(qr[i], jb::to_f32(k_cache[row + lane + 32 * i]), x);
-    x = jb::warp_sum(x);
-    const float m_new = fmaxf(m, x), ref = m_new == -CUDART_INF_F ? 0.0f : m_new;
-    const float corr = exp2f(m - ref), w = exp2f(x - ref);
-    m = m_new;
-    l = l * corr + w;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < s.hd) o[i] = o[i] * corr + w * jb::to_f32(v_cache[row + lane + 32 * i]);
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (lane + 32 * i < s.hd) out[((size_t)t * s.nh + h) * s.hd + lane + 32 * i] = jb::from_f32<E>(o[i] * inv);
-}
-
-__device__ __forceinline__ int sequence_of(const Step& s, int t) {
-  int lo = 0, hi = s.n_seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (s.q_start[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
-__global__ void __launch_bounds__(128) rows_f32_kernel(const float* __restrict__ q, const float* __restrict__ k_cache,
-                                                       const float* __restrict__ v_cache, float* __restrict__ out, const Step s) {
-  jb::pdl_launch_dependents();
-  jb::pdl_wait();
-  const int warp = blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int t = warp / s.nh, h = warp % s.nh;
-  if (t >= s.T || t >= s.q_start[s.n_seqs]) return;
-  one_row(q, k_cache, v_cache, out, s, sequence_of(s, t), t, h);
-}
 
 // ---------------------------------------------------------------------------
 // bfloat16: tiles of 128 (token, query head of one kv head) rows on the tcgen05 tensor cores.
@@ -150,10 +72,6 @@ __device__ __forceinline__ float fast_exp2(float x) {
 __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t lead, uint32_t stride) {
   return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)((lead >> 4) & 0x3FFF) << 16 | (uint64_t)((stride >> 4) & 0x3FFF) << 32 |
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -648,80 +566,8 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const bf16* __restrict
   if (threadIdx.x < 16) not_finite[threadIdx.x] = 0;
   __syncthreads();
   if (prefix_slots > 0) jb::pdl_wait();   // the prefix's partial results are there
-  const int quads = hd / 4;
-  for (int idx = threadIdx.x; idx < n_rows * quads; idx += OWN_THREADS) {
-    const int row = idx / quads, d = idx % quads * 4, rr = row0 + row;
-    const size_t place = (size_t)(start + rr / G) * s.nh + kvh * G + rr % G, all = (size_t)s.T * s.nh;
-    float top = -CUDART_INF_F;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, red_ml[2 * (w * 16 + row)]);
-    if (own_slots == 1)
-      for (int i = 0; i < prefix_slots; ++i) top = fmaxf(top, part_ml[i * all + place].x);
-    const float ref = top == -CUDART_INF_F ? 0.0f : top;
-    float sum = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    auto add = [&](float f, float li, const float4 v) {
-      sum = fmaf(f, li, sum);
-      acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
-    };
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int at = w * 16 + row;
-      add(exp2f(red_ml[2 * at] - ref), red_ml[2 * at + 1], *reinterpret_cast<const float4*>(red_o + at * C::RED_LD + d));
-    }
-    if (own_slots > 1) {
-      const size_t item = (prefix_slots + split) * all + place;
-      *reinterpret_cast<float4*>(part_o + item * hd + d) = acc;
-      if (d == 0) part_ml[item] = make_float2(top, sum);
-      continue;
-    }
-    for (int i = 0; i < prefix_slots; ++i) {
-      const size_t item = i * all + place;
-      const float2 ml = part_ml[item];
-      add(exp2f(ml.x - ref), ml.y, *reinterpret_cast<const float4*>(part_o + item * hd + d));
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-    *reinterpret_cast<uint2*>(out + place * hd + d) = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
-    if (!(isfinite(acc.x) && isfinite(acc.y) && isfinite(acc.z) && isfinite(acc.w))) not_finite[row] = 1;
-  }
-  if (own_slots > 1) return;
-  __syncthreads();
-  for (int row = warp; row < n_rows; row += 4)
-    if (not_finite[row]) one_row(q, k_cache, v_cache, out, s, seq, start + (row0 + row) / G, kvh * G + (row0 + row) % G);
-}
-
-// One warp a (token, query head): all partial results joined in the order of their slots.
-__global__ void __launch_bounds__(128) join_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_cache,
-                                                   const bf16* __restrict__ v_cache, bf16* __restrict__ out,
-                                                   const float* __restrict__ part_o, const float2* __restrict__ part_ml, const Step s,
-                                                   int slots) {
-  jb::pdl_launch_dependents();
-  jb::pdl_wait();
-  const int item = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int t = item / s.nh, h = item % s.nh;
-  if (t >= min(s.T, s.q_start[s.n_seqs])) return;
-  const size_t all = (size_t)s.T * s.nh;
-  float top = -CUDART_INF_F;
-  for (int i = 0; i < slots; ++i) top = fmaxf(top, part_ml[i * all + item].x);
-  const float ref = top == -CUDART_INF_F ? 0.0f : top;
-  bool finite = true;
-  for (int d = lane * 4; d < s.hd; d += 128) {
-    float sum = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i = 0; i < slots; ++i) {
-      const float2 ml = part_ml[i * all + item];
-      const float f = exp2f(ml.x - ref);
-      const float4 v = *reinterpret_cast<const float4*>(part_o + (i * all + item) * s.hd + d);
-      sum = fmaf(f, ml.y, sum);
-      acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-    *reinterpret_cast<uint2*>(out + (size_t)item * s.hd + d) = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
-    finite = finite && isfinite(acc.x) && isfinite(acc.y) && isfinite(acc.z) && isfinite(acc.w);
-  }
-  if (__any_sync(0xffffffffu, !finite)) one_row(q, k_cache, v_cache, out, s, sequence_of(s, t), t, h);
+  finish_rows<bf16, 4, 16, OWN_THREADS>(q, k_cache, v_cache, out, part_o, part_ml, s, red_o, red_ml, C::RED_LD, not_finite, max(n_rows, 0),
+                                        row0, start, seq, kvh, prefix_slots, own_slots, split);
 }
 
 // ---------------------------------------------------------------------------
@@ -786,20 +632,6 @@ cudaError_t own_go(dim3 grid, cudaStream_t stream, const bf16* q, const bf16* k,
 
 }  // namespace
 
-// float32: q, out [T, nh hd], caches [n_pages, nkv, 64, hd] float32.
-JB_EXPORT int jb_attention_prefix_f32(const void* q, const void* k_cache, const void* v_cache, void* out, const int* prefix_pages,
-                                      int prefix_len, const int* block_table, int ld_table, int width, const int* q_start, const int* kv_len,
-                                      const int* positions, int T, int n_seqs, int nh, int nkv, int hd, int page_size, float scale,
-                                      cudaStream_t stream) {
-  if (T <= 0 || n_seqs <= 0) return 0;
-  JB_REFUSE(page_size != PAGE, "attention_prefix: page size %d (need %d)", page_size, PAGE);
-  JB_REFUSE(nkv <= 0 || nh % nkv != 0, "attention_prefix: %d heads are not a multiple of %d kv heads", nh, nkv);
-  JB_REFUSE(hd <= 0 || hd > 256, "attention_prefix: head size %d", hd);
-  const Step s{prefix_pages, block_table, q_start, kv_len, positions, prefix_len, ld_table, width, T, n_seqs, nh, nkv, hd, scale * LOG2E};
-  jb::Launch cfg(dim3((unsigned)(((long long)T * nh + 3) / 4)), dim3(128), 0, stream);
-  return (int)cudaLaunchKernelEx(&cfg.c, rows_f32_kernel, (const float*)q, (const float*)k_cache, (const float*)v_cache, (float*)out, s);
-}
-
 // bfloat16.  splits = 0: tiles of one sequence each walk all their keys (WHOLE).  Else the prefix's keys in `splits` ranges for all
 // rows together and the own keys in `own_slots` ranges a sequence; part_o [splits (+ own_slots if > 1)][T][nh][hd] float32 and
 // part_ml [..][T][nh][2] are scratch.  tiles: row tiles a CTA, 1 or 2.
@@ -856,7 +688,7 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
   if (e != cudaSuccess) return (int)e;
   if (own_slots > 1) {
     jb::Launch cfg(dim3((unsigned)(((long long)T * nh + 3) / 4)), dim3(128), 0, stream);
-    e = cudaLaunchKernelEx(&cfg.c, join_kernel, qb, kb, vb, ob, (const float*)part_o, (const float2*)ml, s, splits + own_slots);
+    e = cudaLaunchKernelEx(&cfg.c, join_kernel<bf16>, qb, kb, vb, ob, (const float*)part_o, (const float2*)ml, s, splits + own_slots);
   }
   return (int)e;
 }

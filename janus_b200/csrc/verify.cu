@@ -6,6 +6,13 @@
 //   the row of the first refusal (or the last row) gives one more token: the lowest v whose cumulative weight C_v passes
 //   u C, the weights being max(w / S - q, 0) after a refusal (w without d where drafts were looked up), else w.
 // T = 0: a draft is accepted if it is the row's argmax (the lowest index of the largest), the token is the argmax.
+//
+// Two launches, both bound by how fast rows come from memory.  `stats_kernel` reads every row once, in chunks of 8,192 logits that
+// its threads hold in registers: a chunk's maximum, the sum of its weights against that maximum, its argmax.  `decide_kernel` has
+// a cluster of up to 8 blocks a request: every block makes the request's decisions from the chunks' results (a few hundred numbers);
+// where drafts of a drafting model were refused the blocks share out the pass over the row's weights and the draft's
+// probabilities and tell one another the chunks' sums through distributed shared memory.  The chunk in which the drawn number falls
+// is then read once more by the block that has it.  All sums are float32 in a fixed order.
 #include <math_constants.h>
 #include <stdio.h>
 
@@ -13,149 +20,372 @@
 
 namespace {
 
-constexpr int THREADS = 1024;
+constexpr int CHUNK = 8192;
+constexpr int STATS_THREADS = 256, STATS_PER = CHUNK / STATS_THREADS;     // 32 logits a thread
+constexpr int THREADS = 512, WARPS = THREADS / 32, PIECE = CHUNK / WARPS;   // a warp has 512 neighbouring logits of a chunk
+constexpr int MAX_CLUSTER = 8;
+constexpr float LOG2E = 1.4426950408889634f;
 
-struct Row {
+// The weight of x against a maximum; heat_log2 = log2(e) / T.  -inf, and what is not a number, weighs nothing.
+__device__ __forceinline__ float weight(float x, float top, float heat_log2) {
+  if (!(x > -CUDART_INF_F)) return 0.0f;
+  return x == top ? 1.0f : exp2f((x - top) * heat_log2);
+}
+
+struct Chunk {
   float top, sum;
   int arg;
 };
 
-__device__ __forceinline__ float weight(float x, float top, float inv_heat) {
-  if (!(x > -CUDART_INF_F)) return 0.0f;   // -inf, and what is not a number
-  return x == top ? 1.0f : expf((x - top) * inv_heat);
+// (the larger value, of equal ones the lower index)
+__device__ __forceinline__ void keep_first(float& top, int& arg, float t, int i) {
+  if (t > top || (t == top && i < arg)) top = t, arg = i;
 }
 
-__device__ Row row_stats(const float* x, int V, float inv_heat, float* scratch, int* scratch_i) {
+template <bool VECTORS>
+__global__ void __launch_bounds__(STATS_THREADS) stats_kernel(const float* __restrict__ logits, Chunk* __restrict__ stats, int V,
+                                                              int chunks, float heat_log2) {
+  __shared__ float s_top[STATS_THREADS / 32], s_sum[STATS_THREADS / 32];
+  __shared__ int s_arg[STATS_THREADS / 32];
+  jb::pdl_wait();
+  jb::pdl_launch_dependents();
+  const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks, v0 = chunk * CHUNK, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float* x = logits + (size_t)row * V + v0;
+  const int n = min(CHUNK, V - v0);
+  float v[STATS_PER];
   float top = -CUDART_INF_F;
   int arg = 0x7fffffff;
-  for (int v = threadIdx.x; v < V; v += THREADS)
-    if (x[v] > top) {
-      top = x[v];
-      arg = v;
+  if constexpr (VECTORS) {
+#pragma unroll
+    for (int i = 0; i < STATS_PER / 4; ++i) {
+      const int at = (tid + STATS_THREADS * i) * 4;
+      float4 t = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+      if (at < n) t = __ldcs(reinterpret_cast<const float4*>(x + at));
+      v[4 * i] = t.x, v[4 * i + 1] = t.y, v[4 * i + 2] = t.z, v[4 * i + 3] = t.w;
     }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  } else {
+#pragma unroll
+    for (int i = 0; i < STATS_PER; ++i) {
+      const int at = tid + STATS_THREADS * i;
+      v[i] = at < n ? __ldcs(x + at) : -CUDART_INF_F;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < STATS_PER; ++i)   // a thread's indices rise
+    if (v[i] > top) top = v[i], arg = v0 + (VECTORS ? (tid + STATS_THREADS * (i / 4)) * 4 + i % 4 : tid + STATS_THREADS * i);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float t = __shfl_xor_sync(0xffffffffu, top, o);
     const int i = __shfl_xor_sync(0xffffffffu, arg, o);
-    if (t > top || (t == top && i < arg)) top = t, arg = i;
+    keep_first(top, arg, t, i);
   }
+  if (lane == 0) s_top[warp] = top, s_arg[warp] = arg;
   __syncthreads();
-  if (lane == 0) scratch[warp] = top, scratch_i[warp] = arg;
+  top = s_top[0], arg = s_arg[0];
+#pragma unroll
+  for (int w = 1; w < STATS_THREADS / 32; ++w) keep_first(top, arg, s_top[w], s_arg[w]);
+  float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < STATS_PER; ++i) part[i & 3] += weight(v[i], top, heat_log2);
+  const float sum = jb::warp_sum((part[0] + part[1]) + (part[2] + part[3]));
+  if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
-  top = scratch[0], arg = scratch_i[0];
-  for (int w = 1; w < THREADS / 32; ++w)
-    if (scratch[w] > top || (scratch[w] == top && scratch_i[w] < arg)) top = scratch[w], arg = scratch_i[w];
-  float sum = 0.0f;
-  for (int v = threadIdx.x; v < V; v += THREADS) sum += weight(x[v], top, inv_heat);
-  __syncthreads();
-  sum = jb::block_sum(sum, scratch);
-  return Row{top, sum, arg == 0x7fffffff ? 0 : arg};
+  if (tid == 0) {
+    float all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < STATS_THREADS / 32; ++w) all += s_sum[w];
+    stats[blockIdx.x] = Chunk{top, all, arg};
+  }
 }
 
-__global__ void __launch_bounds__(THREADS) verify_kernel(const float* __restrict__ logits, const int* __restrict__ tokens,
-                                                         const int* __restrict__ q_start, const int* __restrict__ kv_len,
-                                                         const float* __restrict__ u_accept, const float* __restrict__ u_draw,
-                                                         const float* __restrict__ probs, int* __restrict__ accepted_out,
-                                                         int* __restrict__ out, float* __restrict__ logprobs,
-                                                         int* __restrict__ kept, int V, int width, int T, float heat) {
-  __shared__ float scratch[40];
-  __shared__ int scratch_i[32];
-  __shared__ float s_sum[THREADS];
+__device__ __forceinline__ int cluster_rank() {
+  int r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ int cluster_size() {
+  int n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The place of a variable of this block in the shared memory of block `rank` of the cluster
+__device__ __forceinline__ uint32_t in_block(const void* p, int rank) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ void store_remote(uint32_t at, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+__device__ __forceinline__ float warp_inclusive(float v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float t = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += t;
+  }
+  return v;
+}
+
+// What a token weighs in the draw: w (KEPT), w without token d (LOOKED_UP), what of p is more than q (REFUSED).
+enum Form { KEPT, LOOKED_UP, REFUSED };
+struct Draw {
+  const float* x;
+  const float* q;
+  float top, inv_sum, heat_log2;
+  int d, V;
+  Form form;
+  __device__ __forceinline__ float mass(int v, float xv, float qv) const {
+    const float w = weight(xv, top, heat_log2);
+    if (form == KEPT) return w;
+    return form == LOOKED_UP ? (v == d ? 0.0f : w) : fmaxf(fmaf(w, inv_sum, -qv), 0.0f);
+  }
+  // the masses of four neighbouring tokens
+  __device__ __forceinline__ void four(int v0, bool vectors, float* out) const {
+    float xv[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F}, qv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (vectors) {
+      if (v0 < V) {
+        *reinterpret_cast<float4*>(xv) = *reinterpret_cast<const float4*>(x + v0);
+        if (form == REFUSED) *reinterpret_cast<float4*>(qv) = __ldcs(reinterpret_cast<const float4*>(q + v0));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (v0 + i < V) {
+          xv[i] = x[v0 + i];
+          if (form == REFUSED) qv[i] = q[v0 + i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = mass(v0 + i, xv[i], qv[i]);
+  }
+};
+
+// A chunk's masses, 16 a thread (warp w has PIECE neighbouring tokens, in four runs of four a lane), and the warp's sum: the sums
+// of runs in order.  run_end[k]: the warp's sum up to and with run k.
+__device__ __forceinline__ float warp_masses(const Draw& draw, int chunk, bool vectors, float (&w)[16], float (&run_end)[4]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) draw.four(chunk * CHUNK + warp * PIECE + k * 128 + lane * 4, vectors, w + 4 * k);
+  float run = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    run += __shfl_sync(0xffffffffu, warp_inclusive(((w[4 * k] + w[4 * k + 1]) + w[4 * k + 2]) + w[4 * k + 3]), 31);
+    run_end[k] = run;
+  }
+  return run;
+}
+
+__global__ void __launch_bounds__(THREADS) decide_kernel(const float* __restrict__ logits, const Chunk* __restrict__ stats,
+                                                         const int* __restrict__ tokens, const int* __restrict__ q_start,
+                                                         const int* __restrict__ kv_len, const float* __restrict__ u_accept,
+                                                         const float* __restrict__ u_draw, const float* __restrict__ probs,
+                                                         int* __restrict__ accepted_out, int* __restrict__ out,
+                                                         float* __restrict__ logprobs, int* __restrict__ kept, int V, int chunks, int width,
+                                                         int T, float heat, float heat_log2, int vectors) {
+  extern __shared__ float dyn[];
+  float* chunk_sum = dyn;                                   // [chunks] masses of the drawn row's chunks
+  float* row_top = chunk_sum + chunks;                      // [width] of the request's rows
+  float* row_sum = row_top + width;                         // [width]
+  int* row_arg = reinterpret_cast<int*>(row_sum + width);   // [width]
+  int* row_yes = row_arg + width;                           // [width] the draft behind the row is accepted
+  __shared__ float s_warp[WARPS];
   __shared__ int s_token;
-  const int b = blockIdx.x, tid = threadIdx.x;
+  const int size = cluster_size(), rank = cluster_rank(), b = blockIdx.x / size;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  jb::pdl_wait();
+  jb::pdl_launch_dependents();
   const int lo = min(max(q_start[b], 0), T), hi = min(max(q_start[b + 1], lo), T), rows = min(hi - lo, width);
-  const float inv_heat = heat > 0.0f ? 1.0f / heat : 1.0f;
   int* my = out + (size_t)b * width;
   float* lp = logprobs + (size_t)b * width;
-  if (rows == 0) {
-    for (int k = tid; k < width; k += THREADS) my[k] = -1, lp[k] = 0.0f;
-    if (tid == 0) accepted_out[b] = 0, kept[b] = kv_len[b];
+  if (rows == 0) {   // (the whole cluster)
+    if (rank == 0) {
+      for (int k = tid; k < width; k += THREADS) my[k] = -1, lp[k] = 0.0f;
+      if (tid == 0) accepted_out[b] = 0, kept[b] = kv_len[b];
+    }
     return;
   }
-  int accepted = 0;
-  Row r;
-  for (;; ++accepted) {
-    const float* x = logits + (size_t)(lo + accepted) * V;
-    r = row_stats(x, V, inv_heat, scratch, scratch_i);
-    if (accepted == rows - 1) break;
-    const int t = lo + accepted + 1, d = tokens[t];
-    bool yes = d >= 0 && d < V;
-    if (yes) {
-      if (heat > 0.0f) {
-        const float q = probs ? probs[(size_t)t * V + d] : 1.0f;
-        yes = u_accept[t] * q * r.sum < weight(x[d], r.top, inv_heat);
-      } else {
-        yes = d == r.arg;
-      }
+  // ---- a warp a row: its maximum and sum from its chunks', and the test of the draft behind it ----
+  for (int r = warp; r < rows; r += WARPS) {
+    const Chunk* c = stats + (size_t)(lo + r) * chunks;
+    float top = -CUDART_INF_F, sum = 0.0f;
+    int arg = 0x7fffffff;
+    for (int i = lane; i < chunks; i += 32) keep_first(top, arg, c[i].top, c[i].arg);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float t = __shfl_xor_sync(0xffffffffu, top, o);
+      const int i = __shfl_xor_sync(0xffffffffu, arg, o);
+      keep_first(top, arg, t, i);
     }
-    if (!yes) break;
-    if (tid == 0) my[accepted] = d, lp[accepted] = (x[d] - r.top) * inv_heat - logf(r.sum);
-  }
-  const float* x = logits + (size_t)(lo + accepted) * V;
-  int token = r.arg;
-  if (heat > 0.0f) {
-    const bool refused = accepted < rows - 1;
-    const int d = refused ? tokens[lo + accepted + 1] : -1;
-    const float* q = refused && probs ? probs + (size_t)(lo + accepted + 1) * V : nullptr;
-    const int per = (V + THREADS - 1) / THREADS, v0 = min(tid * per, V), v1 = min(v0 + per, V);
-    for (int form = refused ? 0 : 1; form < 2; ++form) {
-      auto mass = [&](int v) {
-        const float w = weight(x[v], r.top, inv_heat);
-        if (form == 1) return w;
-        return q ? fmaxf(w / r.sum - q[v], 0.0f) : v == d ? 0.0f : w;
-      };
-      float mine = 0.0f;
-      for (int v = v0; v < v1; ++v) mine += mass(v);
-      s_sum[tid] = mine;
-      __syncthreads();
-      if (tid == 0) {
-        float run = 0.0f;
-        int last = -1;
-        for (int i = 0; i < THREADS; ++i) {
-          if (s_sum[i] > 0.0f) last = i;
-          run += s_sum[i];
-        }
-        const float target = u_draw[b] * run;
-        float before = 0.0f;
-        int i = 0;
-        while (i < last && !(target < before + s_sum[i])) before += s_sum[i++];
-        s_token = -1;
-        if (last >= 0) {
-          const int a = min(i * per, V), e = min(a + per, V);
-          for (int v = a; v < e; ++v) {
-            const float w = mass(v);
-            if (w > 0.0f) {
-              before += w;
-              s_token = v;
-              if (target < before) break;
-            }
+    for (int i = lane; i < chunks; i += 32) sum = fmaf(c[i].sum, weight(c[i].top, top, heat_log2), sum);
+    sum = jb::warp_sum(sum);
+    if (arg == 0x7fffffff) arg = 0;
+    if (lane == 0) {
+      bool yes = false;
+      if (r + 1 < rows) {
+        const int t = lo + r + 1, d = tokens[t];
+        if (d >= 0 && d < V) {
+          if (heat > 0.0f) {
+            const float q = probs ? probs[(size_t)t * V + d] : 1.0f;
+            yes = u_accept[t] * q * sum < weight(logits[(size_t)(lo + r) * V + d], top, heat_log2);
+          } else {
+            yes = d == arg;
           }
         }
       }
-      __syncthreads();
-      if (s_token >= 0) token = s_token;
-      if (s_token >= 0) break;
+      row_top[r] = top, row_sum[r] = sum, row_arg[r] = arg, row_yes[r] = yes;
     }
   }
-  for (int k = accepted + 1 + tid; k < width; k += THREADS) my[k] = -1, lp[k] = 0.0f;
-  if (tid == 0) {
-    my[accepted] = token;
-    lp[accepted] = (x[token] - r.top) * inv_heat - logf(r.sum);
-    accepted_out[b] = accepted;
-    kept[b] = kv_len[b] - (hi - lo - 1) + accepted;
+  if (tid == 0) s_token = -1;
+  __syncthreads();
+  int accepted = 0;
+  while (accepted < rows - 1 && row_yes[accepted]) ++accepted;
+  // ---- one more token, from row `accepted` ----
+  int token = row_arg[accepted], writer = 0;
+  if (heat > 0.0f) {
+    const bool refused = accepted < rows - 1;
+    const int next = lo + accepted + 1, d = refused ? tokens[next] : -1;
+    const Chunk* c = stats + (size_t)(lo + accepted) * chunks;
+    Draw draw{logits + (size_t)(lo + accepted) * V, probs ? probs + (size_t)min(next, T - 1) * V : nullptr, row_top[accepted],
+              1.0f / row_sum[accepted], heat_log2, d, V, !refused ? KEPT : probs ? REFUSED : LOOKED_UP};
+    const int c_begin = (int)((long long)rank * chunks / size), c_end = (int)((long long)(rank + 1) * chunks / size);
+    const int d_chunk = draw.form == LOOKED_UP && d >= 0 && d < V ? d / CHUNK : -1;   // its sum is made anew, without d
+    float w[16], run_end[4];
+    auto chunk_mass = [&](int i) {   // by the whole block
+      const float mine = warp_masses(draw, i, vectors, w, run_end);
+      if (lane == 0) s_warp[warp] = mine;
+      __syncthreads();
+      float all = 0.0f;
+#pragma unroll
+      for (int v = 0; v < WARPS; ++v) all += s_warp[v];
+      __syncthreads();
+      return all;
+    };
+    // the chunks' masses, known to every block
+    if (draw.form == REFUSED) {
+      cluster_sync();   // every block is there to be written to
+      for (int i = c_begin; i < c_end; ++i) {
+        const float all = chunk_mass(i);
+        for (int r = tid; r < size; r += THREADS) store_remote(in_block(chunk_sum + i, r), all);
+      }
+      cluster_sync();
+    }
+    float total = 0.0f;
+    for (int form = 0; form < 2; ++form) {
+      if (form == 1 || draw.form != REFUSED) {
+        const float again = d_chunk >= 0 && draw.form == LOOKED_UP ? chunk_mass(d_chunk) : 0.0f;
+        for (int i = tid; i < chunks; i += THREADS)
+          chunk_sum[i] = i == d_chunk && draw.form == LOOKED_UP ? again : c[i].sum * weight(c[i].top, draw.top, heat_log2);
+      }
+      __syncthreads();
+      total = 0.0f;
+      for (int i = 0; i < chunks; ++i) total += chunk_sum[i];
+      if (total > 0.0f || draw.form == KEPT) break;
+      draw.form = KEPT;   // nothing is left: from the row itself
+      __syncthreads();
+    }
+    // the chunk where the drawn number falls (the last one with any mass, should rounding let none pass)
+    const float target = u_draw[b] * total;
+    float before = 0.0f, run = 0.0f;
+    int pick = -1;
+    for (int i = 0; i < chunks; ++i) {
+      const float m = chunk_sum[i];
+      if (m > 0.0f) {
+        pick = i, before = run;
+        if (target < run + m) break;
+      }
+      run += m;
+    }
+    if (pick >= 0) {
+      writer = 0;
+      while (!(pick < (int)((long long)(writer + 1) * chunks / size))) ++writer;
+    }
+    if (pick >= 0 && rank == writer) {
+      const float mine = warp_masses(draw, pick, vectors, w, run_end);
+      if (lane == 0) s_warp[warp] = mine;
+      __syncthreads();
+      // the first warp whose running sum passes the target, or the last one with any mass
+      int owner = -1;
+      float start = before, at = before;
+      for (int v = 0; v < WARPS; ++v) {
+        const float m = s_warp[v];
+        if (m > 0.0f) {
+          owner = v, start = at;
+          if (target < at + m) break;
+        }
+        at += m;
+      }
+      if (warp == owner) {
+        int hit = 0x7fffffff, last = -1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float four = ((w[4 * k] + w[4 * k + 1]) + w[4 * k + 2]) + w[4 * k + 3];
+          float sum = start + (k > 0 ? run_end[k > 0 ? k - 1 : 0] : 0.0f) + (warp_inclusive(four) - four);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int v = pick * CHUNK + warp * PIECE + k * 128 + lane * 4 + i;
+            if (w[4 * k + i] > 0.0f) {
+              sum += w[4 * k + i];
+              last = v;
+              if (target < sum) hit = min(hit, v);
+            }
+          }
+        }
+        hit = __reduce_min_sync(0xffffffffu, hit);
+        last = __reduce_max_sync(0xffffffffu, last);
+        if (lane == 0) s_token = hit != 0x7fffffff ? hit : last;
+      }
+      __syncthreads();
+      if (s_token >= 0) token = s_token;
+    }
+  }
+  if (rank == writer) {
+    for (int k = tid; k < width; k += THREADS) {
+      int v = -1;
+      float p = 0.0f;
+      if (k <= accepted) {
+        v = k < accepted ? tokens[lo + k + 1] : token;
+        const float x = logits[(size_t)(lo + k) * V + v], gap = x == row_top[k] ? 0.0f : x - row_top[k];
+        p = row_sum[k] > 0.0f ? gap * (heat > 0.0f ? 1.0f / heat : 1.0f) - logf(row_sum[k]) : -CUDART_INF_F;
+      }
+      my[k] = v, lp[k] = p;
+    }
+    if (tid == 0) accepted_out[b] = accepted, kept[b] = kv_len[b] - (hi - lo - 1) + accepted;
   }
 }
 
 }  // namespace
 
+// stats: scratch of 3 floats a row and chunk of 8,192 logits.  The launch of decide_kernel is by clusters.
 JB_EXPORT int jb_verify_drafts(const float* logits, const int* tokens, const int* q_start, const int* kv_len, const float* u_accept,
-                               const float* u_draw, const float* probs, int* accepted, int* out, float* logprobs, int* kept, int T,
-                               int B, int V, int width, float heat, cudaStream_t stream) {
+                               const float* u_draw, const float* probs, int* accepted, int* out, float* logprobs, int* kept, void* stats,
+                               int T, int B, int V, int width, float heat, cudaStream_t stream) {
   if (B <= 0) return 0;
   JB_REFUSE(V <= 0 || width <= 0 || T < 0, "verify_drafts: %d rows of %d logits, %d tokens a request", T, V, width);
-  verify_kernel<<<B, THREADS, 0, stream>>>(logits, tokens, q_start, kv_len, u_accept, u_draw, probs, accepted, out, logprobs, kept, V,
-                                           width, T, heat);
-  JB_CHECK_LAUNCH();
-  return 0;
+  const int chunks = (V + CHUNK - 1) / CHUNK;
+  const size_t smem = ((size_t)chunks + 4 * (size_t)width) * sizeof(float);
+  JB_REFUSE(smem > 48 * 1024, "verify_drafts: %d tokens a request over a vocabulary of %d", width, V);
+  JB_REFUSE((long long)T * chunks > 0x7fffffffll || (long long)B * MAX_CLUSTER > 0x7fffffffll, "verify_drafts: %d rows of %d logits", T, V);
+  const float heat_log2 = heat > 0.0f ? LOG2E / heat : LOG2E;
+  const bool vectors = V % 4 == 0 && (((uintptr_t)logits | (uintptr_t)probs) & 15) == 0;
+  cudaError_t e = cudaSuccess;
+  if (T > 0) {
+    jb::Launch cfg(dim3(T * chunks), dim3(STATS_THREADS), 0, stream);
+    e = cudaLaunchKernelEx(&cfg.c, vectors ? stats_kernel<true> : stats_kernel<false>, logits, (Chunk*)stats, V, chunks, heat_log2);
+    if (e != cudaSuccess) return (int)e;
+  }
+  const int size = chunks < MAX_CLUSTER ? chunks : MAX_CLUSTER;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(B * size), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  cfg.attrs = attr, cfg.numAttrs = jb::pdl_enabled() ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, decide_kernel, logits, (const Chunk*)stats, tokens, q_start, kv_len, u_accept, u_draw, probs, accepted,
+                                 out, logprobs, kept, V, chunks, width, T, heat, heat_log2, (int)vectors);
 }

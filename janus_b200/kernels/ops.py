@@ -87,9 +87,9 @@ _SIGNATURES = {
     "jb_activate": "ppilip", "jb_tanh_norm": "ppppffippfpipiiplplp",
     "jb_latent_heads": "piiiiiipppiiiipfpppip", "jb_latent_queries": "piiiiiiippppiiipfppip", "jb_latent_values": "pppippiipiiiiiip",
     "jb_latent_down": "piipfpiippiiippppplip",
-    "jb_step_tables": "ppppppppppppppppppiiiiiiiip", "jb_attention_prefix_f32": "pppppipiipppiiiiiifp",
+    "jb_step_tables": "ppppppppppppppppppiiiiiiiip", "jb_attention_prefix_f32": "pppppppipiipppiiiiiifiiiiip",
     "jb_attention_prefix_bf16": "pppppppipiipppiiiiiiifiiiipp",
-    "jb_verify_drafts": "pppppppppppiiiifp",
+    "jb_verify_drafts": "ppppppppppppiiiifp",
     "jb_gather_rows": "ppiipppiiip", "jb_latent_attention": "ppppppppiiiiiiifiipp", "jb_attention_tc_matrix": "ppppppiiiiiiiifpipp",
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "u": ctypes.c_ulonglong,
@@ -2470,20 +2470,25 @@ def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise KernelError(f"attention_prefix: {prefix_pages.shape[0]} pages do not hold a prefix of {prefix_len} tokens")
     if max_q_len < 0 or block_table.shape[1] * page_size < max_kv_len - prefix_len:
         raise KernelError(f"attention_prefix: {block_table.shape[1]} pages a sequence do not hold {max_kv_len} tokens behind {prefix_len}")
-    lib, step = _lib("prefix_attention"), (_ptr(prefix_pages), prefix_len, _ptr(block_table), block_table.stride(0), block_table.shape[1],
-                                           _ptr(q_start), _ptr(kv_len), _ptr(positions), T)
+    step = (_ptr(prefix_pages), prefix_len, _ptr(block_table), block_table.stride(0), block_table.shape[1],
+            _ptr(q_start), _ptr(kv_len), _ptr(positions), T)
     if q.dtype == torch.float32:
-        _check(lib.jb_attention_prefix_f32(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), *step, n_seqs, nh, nkv, hd, page_size,
-                                           float(scale), _stream()), "attention_prefix")
-        return
-    tiles, splits, own_slots = attention_prefix_plan(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv, hd)
+        rows, own_rows, splits, own_slots = attention_prefix_plan_f32(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv)
+    else:
+        tiles, splits, own_slots = attention_prefix_plan(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv, hd)
     slots = splits + own_slots if own_slots > 1 else splits
     part_o = part_ml = None
     if slots:
         part_o = workspace.get("prefix_part_o", (slots * T * nh * hd,), torch.float32)
         part_ml = workspace.get("prefix_part_ml", (slots * T * nh * 2,), torch.float32)
+    if q.dtype == torch.float32:
+        _check(_lib("prefix_attention_f32").jb_attention_prefix_f32(
+            _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(part_o), _ptr(part_ml), *step, n_seqs, nh, nkv, hd, page_size,
+            float(scale), int(max_q_len), rows, own_rows, splits, own_slots, _stream()), "attention_prefix",
+            kernels=1 if hd % 4 else (splits > 0) + 1 + (own_slots > 1))
+        return
     kernels = 1 if splits == 0 and prefix_len else (splits > 0) + 1 + (own_slots > 1)
-    _check(lib.jb_attention_prefix_bf16(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(part_o), _ptr(part_ml), *step,
+    _check(_lib("prefix_attention").jb_attention_prefix_bf16(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(part_o), _ptr(part_ml), *step,
                                         k_cache.shape[0], n_seqs, nh, nkv, hd, page_size, float(scale), int(max_q_len), tiles, splits,
                                         own_slots, _ptr(kernel_status(q.device)), _stream()), "attention_prefix", kernels=kernels)
 
@@ -2503,6 +2508,18 @@ def attention_prefix_plan(T: int, n_seqs: int, max_q_len: int, prefix_len: int, 
     ctas = n_seqs * nkv * ((max_q_len * group + 15) // 16)
     own_slots = min(32, max(1, pages // 2), max(1, 2 * sms // max(1, ctas)))
     return tiles, splits, own_slots
+
+
+@functools.lru_cache(maxsize=4096)
+def attention_prefix_plan_f32(T: int, n_seqs: int, max_q_len: int, prefix_len: int, max_own: int, nh: int, nkv: int):
+    """(rows of a block over the prefix, over own keys, ranges of the prefix, ranges of a sequence's own keys) of a float32
+    `attention_prefix`."""
+    group, sms = nh // nkv, SM_COUNT_TARGET // 2
+    rows, own_rows = (16 if n * group <= 32 else 64 for n in (T, max_q_len))
+    pages = (prefix_len + 63) // 64
+    splits = min(pages, max(1, sms // (nkv * ((T * group + rows - 1) // rows)))) if prefix_len else 0
+    ctas = n_seqs * nkv * ((max_q_len * group + own_rows - 1) // own_rows)
+    return rows, own_rows, splits, min(32, max(1, (max_own + 127) // 128), max(1, 2 * sms // max(1, ctas)))
 
 
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, accepted: torch.Tensor,
@@ -2535,6 +2552,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Ten
         _need(draft_probs, "draft probabilities", torch.float32, (T, V))
     if not 0.0 <= temperature < float("inf"):
         raise KernelError(f"verify_drafts: temperature {temperature}")
+    stats = workspace.get("verify_stats", (T * ((V + 8191) // 8192) * 3,), torch.float32)
     _check(_lib("verify").jb_verify_drafts(
         _ptr(logits), _ptr(tokens), _ptr(q_start), _ptr(kv_len), _ptr(u_accept), _ptr(u_draw), _ptr(draft_probs), _ptr(accepted),
-        _ptr(out_tokens), _ptr(logprobs), _ptr(kept), T, B, V, width, float(temperature), _stream()), "verify_drafts")
+        _ptr(out_tokens), _ptr(logprobs), _ptr(kept), _ptr(stats), T, B, V, width, float(temperature), _stream()), "verify_drafts", kernels=2)
