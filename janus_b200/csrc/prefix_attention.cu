@@ -5,8 +5,8 @@
 // A softmax over a union of key sets joins from the sets' (maximum m, sum l, weighted values O):
 //   m = max m_i,  l = sum 2^(m_i - m) l_i,  O = sum 2^(m_i - m) O_i   (scores in units of log2).
 // So the prefix is attended once for all: the rows of ALL sequences' tokens make tiles of 128 for the tensor cores, which walk
-// the prefix's keys in ranges (`prefix_tc_kernel<SPLIT>`), while `own_kernel` walks each sequence's own pages; partial results
-// are float32.  Steps whose sequences bring many tokens fill tiles by themselves: there a tile walks the prefix and then its own
+// the prefix's keys in ranges (`prefix_tc_kernel<SHARED>`), and each sequence's own pages are walked (`own_kernel`, or tiles again
+// where a sequence brings many tokens, `<OWN>`) and joined with the float32 partial results.  Steps whose sequences bring many tokens fill tiles by themselves: there a tile walks the prefix and then its own
 // pages and nothing is joined (`prefix_tc_kernel<WHOLE>`).
 #include <cuda.h>
 
@@ -19,11 +19,12 @@ namespace {
 // bfloat16: tiles of 128 (token, query head of one kv head) rows on the tcgen05 tensor cores.
 //   warp 0     TMA producer: the Q tiles, then blocks of KB keys and values (128-byte swizzle), each in a ring of two
 //   warp 1     one lane issues the products: S = Q K^T into tensor memory, O += P V with P from tensor memory
-//   warps 2..  one thread a row: softmax in float32 against a reference maximum that is raised (and O rescaled) only when a
-//              row's maximum has grown by 2^8; P, in bfloat16 as the tensor core takes it, over the first half of S
+//   warps 2..  two threads a row, each with half of a block's keys: softmax in float32 against a reference maximum that is raised
+//              (and O rescaled) only when a row's maximum has grown by 2^8; P, in bfloat16 as the tensor core takes it, over the
+//              first half of S.  (With one thread a row the softmax took twice as long as the products it has to hide behind.)
 // Two tiles a CTA take turns on the tensor core (NT = 2); a single tile has two S buffers and works a block ahead.
-// SPLIT: the rows are the step's tokens whatever sequence they belong to, the keys a range of the prefix's blocks; what is
-// written is the partial result.  WHOLE: the rows are one sequence's, the keys all that they see.
+// SHARED walks an even share of a list of (tile, kv head, key block): a tile's blocks end in one block and go on in the next,
+// which leaves a partial result of its own, and no multiprocessor waits for another's last wave.
 // ---------------------------------------------------------------------------
 constexpr int BM = 128;
 constexpr float RESCALE_LOG2 = 8.0f;
@@ -112,34 +113,64 @@ template <int HDC, int NT, int KB>
 struct Tc {
   static constexpr int SLABS = HDC / 64;                       // 64-number slabs of a row
   static constexpr int Q_BYTES = SLABS * BM * 128, KV_BYTES = SLABS * KB * 128;
-  static constexpr int BARS = 1 + 8 + 2 * 2 + 2 * NT;          // q_full; k, v full and empty x 2; s_full, p_full x 2; o_full, o_done
-  static constexpr int SMEM = NT * Q_BYTES + 4 * KV_BYTES + BARS * 8 + 16 + 1024;
-  static constexpr int THREADS = 64 + NT * 128;
+  static constexpr int BARS = 1 + 8 + 2 * 2 + 3 * NT;          // q_full; k, v full and empty x 2; s_full, p_full x 2; o_full, o_done, o_free
+  static constexpr int SWAP = NT * 2 * BM;                     // floats: what the two halves of a row tell each other
+  static constexpr int SMEM = NT * Q_BYTES + 4 * KV_BYTES + SWAP * 4 + NT * 4 * 4 + BARS * 8 + 16;
+  static constexpr int THREADS = 64 + NT * 256;
   static constexpr int COLS = 2 * KB + NT * HDC <= 256 ? 256 : 512;
   static_assert(2 * KB + NT * HDC <= 512 && SMEM <= 232448, "tensor and shared memory of one CTA");
 };
+// A barrier of two warps that tells both whether any of their threads says `yes`.
+__device__ __forceinline__ bool pair_any(int barrier, bool yes) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, %2, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"((uint32_t)yes), "r"(barrier)
+      : "memory");
+  return any != 0u;
+}
+__device__ __forceinline__ void pair_sync(int barrier) { asm volatile("bar.sync %0, 64;" ::"r"(barrier) : "memory"); }
 
-enum Form { SPLIT, WHOLE };
+// SHARED: the step's tokens over the prefix, results left as parts.  WHOLE: one sequence's tokens over all that they see.  OWN: one
+// sequence's tokens over its own keys, joined with the parts over the prefix.
+enum Form { SHARED, WHOLE, OWN };
 
-// part_o: [slot][token][head][hd] float32, not normalised; part_ml: [slot][token][head] (maximum in log2 units, sum)
+__device__ __forceinline__ void store8(float* p, const uint32_t* r) {   // a whole 32-byte sector of a row
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+               "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void load8(const float* p, float* r) {
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
+               : "l"(p)
+               : "memory");
+}
+
 template <int HDC, int NT, int KB, Form FORM>
 __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
     const bf16* __restrict__ q, const bf16* __restrict__ k_cache, const bf16* __restrict__ v_cache, bf16* __restrict__ out,
-    float* __restrict__ part_o, float2* __restrict__ part_ml, const Step s, int n_splits, int* __restrict__ status) {
+    float* __restrict__ part_o, float2* __restrict__ part_ml, const Step s, const Slots parts, int* __restrict__ status) {
   typedef Tc<HDC, NT, KB> C;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];            // (no static shared memory: it begins where it is declared to)
   const uint32_t q_s = jb::smem_u32(smem), k_s = q_s + NT * C::Q_BYTES, v_s = k_s + 2 * C::KV_BYTES;
-  uint64_t* bars = (uint64_t*)(smem + NT * C::Q_BYTES + 4 * C::KV_BYTES);
+  float* swap = (float*)(smem + NT * C::Q_BYTES + 4 * C::KV_BYTES);   // [tile][half][row]
+  int* gave_up = (int*)(swap + C::SWAP);                       // [tile][quarter]: one of the two warps has
+  uint64_t* bars = (uint64_t*)(gave_up + NT * 4);
   uint32_t* tmem_slot = (uint32_t*)(bars + C::BARS);
   const uint32_t bar0 = jb::smem_u32(bars);
   const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 24, v_full = bar0 + 40, v_empty = bar0 + 56;
   // an S buffer belongs to a tile (NT = 2), or to the even or odd blocks of the one tile
   auto s_full = [&](int b) { return bar0 + 72 + 16 * b; };
   auto p_full = [&](int b) { return bar0 + 80 + 16 * b; };
-  auto o_full = [&](int w) { return bar0 + 104 + 16 * w; };
-  auto o_done = [&](int w) { return bar0 + 112 + 16 * w; };
+  auto o_full = [&](int w) { return bar0 + 104 + 24 * w; };   // a block's product has landed in O
+  auto o_done = [&](int w) { return bar0 + 112 + 24 * w; };   // ... the last block's of a segment
+  auto o_free = [&](int w) { return bar0 + 120 + 24 * w; };   // O has been read and may be begun anew
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     jb::mbar_init(q_full, 1);
@@ -149,86 +180,106 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
       jb::mbar_init(v_full + 8 * i, 1);
       jb::mbar_init(v_empty + 8 * i, 1);
       jb::mbar_init(s_full(i), 1);
-      jb::mbar_init(p_full(i), 128);
+      jb::mbar_init(p_full(i), 256);
     }
     for (int w = 0; w < NT; ++w) {
       jb::mbar_init(o_full(w), 1);
       jb::mbar_init(o_done(w), 1);
+      jb::mbar_init(o_free(w), 256);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x < NT * 4) gave_up[threadIdx.x] = 0;
   if (warp == 1) jb::tmem_alloc<C::COLS>(jb::smem_u32(tmem_slot));
   jb::tc_fence_before();
   __syncthreads();
   jb::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  jb::pdl_wait();
+  if (FORM != OWN || parts.most == 0) jb::pdl_wait();
   // (after the wait: a kernel that starts early may read what the launch before this one wrote)
   jb::pdl_launch_dependents();
 
-  // ---- which rows, which keys ----
-  const int G = s.nh / s.nkv, tpt = BM / G, kvh = blockIdx.x;
-  int tok0, n_tok, seq = 0, first_pos = 0;                     // first token, tokens of all tiles
-  int block0 = 0, n_shared, n_own = 0;                         // first block of the prefix, its blocks, own blocks
-  const int total = min(s.T, max(s.q_start[s.n_seqs], 0));
-  if constexpr (FORM == SPLIT) {
-    tok0 = blockIdx.y * NT * tpt;
-    n_tok = min(NT * tpt, total - tok0);
-    const int blocks = (s.prefix_len + KB - 1) / KB;
-    block0 = (int)((long long)blockIdx.z * blocks / n_splits);
-    n_shared = (int)((long long)(blockIdx.z + 1) * blocks / n_splits) - block0;
-  } else {
-    seq = blockIdx.z;
-    const int start = s.q_start[seq], q_len = s.q_start[seq + 1] - start, tile = gridDim.y - 1 - blockIdx.y;
-    tok0 = start + tile * NT * tpt;
-    n_tok = min(NT * tpt, q_len - tile * NT * tpt);
-    first_pos = s.kv_len[seq] - q_len + tile * NT * tpt;
-    const int see = first_pos + n_tok;                         // keys that the last token sees
-    n_shared = (min(see, s.prefix_len) + KB - 1) / KB;
-    n_own = (min(max(see - s.prefix_len, 0), s.width * PAGE) + KB - 1) / KB;
-  }
-  const int nb = n_tok > 0 ? n_shared + n_own : 0;
+  // ---- which rows, which keys: a list of segments, each one tile (or two) over a range of key blocks ----
+  const int G = s.nh / s.nkv, tpt = BM / G;
+  const int total_tokens = min(s.T, max(s.q_start[s.n_seqs], 0));
+  struct Segment {
+    int tok0, n_tok, kvh, block0, n_shared, nb;   // first token, tokens of all tiles; first block of the prefix, its blocks, all blocks
+    int slot;
+  };
+  int seq = 0, seq_start = 0, seq_pos = 0;        // SHARED: not used
+  const int flat_begin = FORM == SHARED ? range_start(parts, blockIdx.x) : 0, flat_end = FORM == SHARED ? range_start(parts, blockIdx.x + 1) : 1;
+  if constexpr (FORM != SHARED) seq = blockIdx.z, seq_start = s.q_start[seq], seq_pos = s.kv_len[seq] - (s.q_start[seq + 1] - seq_start);
+  // the segment that begins at place `at` of the list; steps `at` on to the next
+  auto segment = [&](int& at) {
+    Segment g;
+    if constexpr (FORM == SHARED) {
+      const int item = at / parts.blocks;
+      g.block0 = at - item * parts.blocks;
+      g.nb = g.n_shared = min(parts.blocks - g.block0, flat_end - at);
+      g.kvh = item % s.nkv, g.tok0 = item / s.nkv * NT * tpt;
+      g.n_tok = min(NT * tpt, total_tokens - g.tok0);
+      g.slot = blockIdx.x - (g.block0 == 0 ? blockIdx.x : range_of(parts, item * parts.blocks));
+      at += g.nb;
+    } else {
+      const int q_len = s.q_start[seq + 1] - seq_start, first = (gridDim.y - 1 - blockIdx.y) * NT * tpt;
+      g.kvh = blockIdx.x, g.tok0 = seq_start + first, g.n_tok = min(NT * tpt, q_len - first), g.block0 = 0, g.slot = 0;
+      const int see = seq_pos + first + g.n_tok;             // keys that the last token sees
+      g.n_shared = FORM == WHOLE ? (max(min(see, s.prefix_len), 0) + KB - 1) / KB : 0;
+      g.nb = g.n_tok > 0 ? g.n_shared + (min(max(see - s.prefix_len, 0), s.width * PAGE) + KB - 1) / KB : 0;
+      ++at;
+    }
+    return g;
+  };
   const int nslab = (s.hd + 63) / 64;
 
-  if (nb > 0 && warp == 0) {
+  if (warp == 0) {
     if (lane == 0) {
-      jb::mbar_expect_tx(q_full, NT * nslab * tpt * G * 128);   // a box holds tpt tokens x G heads
-      for (int w = 0; w < NT; ++w)
-        for (int h = 0; h < nslab; ++h) tma_load_4d(q_s + w * C::Q_BYTES + h * BM * 128, &map_q, q_full, h * 64, 0, kvh, tok0 + w * tpt);
-      const int last_shared = (s.prefix_len - 1) / PAGE;
-      const int last_own = FORM == WHOLE ? min((first_pos + n_tok - s.prefix_len - 1) / PAGE, s.width - 1) : 0;
-      for (int j = 0; j < nb; ++j) {
-        const int st = j & 1;
-        int row0[KB / PAGE];
+      const int last_shared = max((s.prefix_len - 1) / PAGE, 0);
+      bool ok = true;
+      int it = 0;                                             // blocks since the kernel's begin
+      for (int at = flat_begin; at < flat_end && ok;) {
+        const Segment g = segment(at);
+        if (g.nb == 0) break;
+        // every product with the queries before these is done when the last block's keys are free
+        if (it > 0) ok = jb::mbar_wait(k_empty + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, status, 41);
+        if (!ok) break;
+        jb::mbar_expect_tx(q_full, NT * nslab * tpt * G * 128);   // a box holds tpt tokens x G heads
+        for (int w = 0; w < NT; ++w)
+          for (int h = 0; h < nslab; ++h)
+            tma_load_4d(q_s + w * C::Q_BYTES + h * BM * 128, &map_q, q_full, h * 64, 0, g.kvh, g.tok0 + w * tpt);
+        const int last_own = FORM != SHARED ? max(min((seq_pos + g.tok0 - seq_start + g.n_tok - s.prefix_len - 1) / PAGE, s.width - 1), 0) : 0;
+        for (int j = 0; j < g.nb; ++j, ++it) {
+          const int st = it & 1;
+          int row0[KB / PAGE];
 #pragma unroll
-        for (int half = 0; half < KB / PAGE; ++half) {   // a block's second page may lie behind the last: those keys are masked
-          int page;
-          if (j < n_shared) page = s.prefix_pages[min((block0 + j) * (KB / PAGE) + half, last_shared)];
-          else page = s.table[(size_t)seq * s.ld_table + min((j - n_shared) * (KB / PAGE) + half, last_own)];
-          row0[half] = (max(page, 0) * s.nkv + kvh) * PAGE;
+          for (int half = 0; half < KB / PAGE; ++half) {   // a block's second page may lie behind the last: those keys are masked
+            int page;
+            if (FORM == SHARED || j < g.n_shared) page = s.prefix_pages[min((g.block0 + j) * (KB / PAGE) + half, last_shared)];
+            else page = s.table[(size_t)seq * s.ld_table + min((j - g.n_shared) * (KB / PAGE) + half, last_own)];
+            row0[half] = (max(page, 0) * s.nkv + g.kvh) * PAGE;
+          }
+          if (it >= 2 && !(ok = jb::mbar_wait(k_empty + 8 * st, ((it >> 1) - 1) & 1, status, 41))) break;
+          jb::mbar_expect_tx(k_full + 8 * st, nslab * KB * 128);
+#pragma unroll
+          for (int half = 0; half < KB / PAGE; ++half)
+            for (int h = 0; h < nslab; ++h)
+              jb::tma_load_2d(k_s + st * C::KV_BYTES + h * KB * 128 + half * PAGE * 128, &map_k, k_full + 8 * st, h * 64, row0[half]);
+          if (it >= 2 && !(ok = jb::mbar_wait(v_empty + 8 * st, ((it >> 1) - 1) & 1, status, 41))) break;
+          jb::mbar_expect_tx(v_full + 8 * st, nslab * KB * 128);
+#pragma unroll
+          for (int half = 0; half < KB / PAGE; ++half)
+            for (int h = 0; h < nslab; ++h)
+              jb::tma_load_2d(v_s + st * C::KV_BYTES + h * KB * 128 + half * PAGE * 128, &map_v, v_full + 8 * st, h * 64, row0[half]);
         }
-        if (j >= 2 && !jb::mbar_wait(k_empty + 8 * st, ((j >> 1) - 1) & 1, status, 41)) break;
-        jb::mbar_expect_tx(k_full + 8 * st, nslab * KB * 128);
-#pragma unroll
-        for (int half = 0; half < KB / PAGE; ++half)
-          for (int h = 0; h < nslab; ++h)
-            jb::tma_load_2d(k_s + st * C::KV_BYTES + h * KB * 128 + half * PAGE * 128, &map_k, k_full + 8 * st, h * 64, row0[half]);
-        if (j >= 2 && !jb::mbar_wait(v_empty + 8 * st, ((j >> 1) - 1) & 1, status, 41)) break;
-        jb::mbar_expect_tx(v_full + 8 * st, nslab * KB * 128);
-#pragma unroll
-        for (int half = 0; half < KB / PAGE; ++half)
-          for (int h = 0; h < nslab; ++h)
-            jb::tma_load_2d(v_s + st * C::KV_BYTES + h * KB * 128 + half * PAGE * 128, &map_v, v_full + 8 * st, h * 64, row0[half]);
       }
     }
-  } else if (nb > 0 && warp == 1) {
+  } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t idesc_s = jb::instr_desc_bf16(KB);
       const uint32_t idesc_o = jb::instr_desc_bf16((s.hd + 15) & ~15) | (1u << 16);   // values: MN-major
-      bool ok = jb::mbar_wait(q_full, 0, status, 42);
-      auto issue_s = [&](int w, int j) -> bool {
-        const int st = j & 1, b = NT == 2 ? w : j & 1;
-        if (!jb::mbar_wait(k_full + 8 * st, (j >> 1) & 1, status, 42)) return false;
+      auto issue_s = [&](int w, int it) -> bool {
+        const int st = it & 1, b = NT == 2 ? w : it & 1;
+        if (!jb::mbar_wait(k_full + 8 * st, (it >> 1) & 1, status, 42)) return false;
         jb::tc_fence_after();
 #pragma unroll
         for (int h = 0; h < C::SLABS; ++h) {
@@ -242,14 +293,25 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
         if (w == NT - 1) jb::umma_commit(k_empty + 8 * st);
         return true;
       };
+      int at = flat_begin;
+      Segment g = segment(at);
+      int n = 0, j = 0, turn = 0;                              // blocks of the segment, the next one of them, segments so far
+      bool ok = g.nb > 0 && jb::mbar_wait(q_full, 0, status, 42);
+      n = g.nb;
       for (int w = 0; w < NT && ok; ++w) ok = issue_s(w, 0);
-      for (int j = 0; j < nb && ok; ++j) {
-        const int st = j & 1;
-        if (NT == 1 && j + 1 < nb) ok = issue_s(0, j + 1);
+      for (int it = 0; ok; ++it) {
+        const int st = it & 1;
+        const bool last = j == n - 1, more = !last || at < flat_end;
+        bool fresh_q = last && more;                           // the next block is the first of another segment
+        if (NT == 1 && more) {
+          if (fresh_q) ok = jb::mbar_wait(q_full, (turn + 1) & 1, status, 42);
+          ok = ok && issue_s(0, it + 1);
+        }
         for (int w = 0; w < NT && ok; ++w) {
-          const int b = NT == 2 ? w : j & 1;
-          ok = jb::mbar_wait(p_full(b), (NT == 2 ? j : j >> 1) & 1, status, 42);
-          if (ok && w == 0) ok = jb::mbar_wait(v_full + 8 * st, (j >> 1) & 1, status, 42);
+          const int b = NT == 2 ? w : it & 1;
+          ok = jb::mbar_wait(p_full(b), (NT == 2 ? it : it >> 1) & 1, status, 42);
+          if (ok && w == 0) ok = jb::mbar_wait(v_full + 8 * st, (it >> 1) & 1, status, 42);
+          if (ok && j == 0 && turn > 0) ok = jb::mbar_wait(o_free(w), (turn - 1) & 1, status, 42);
           if (!ok) break;
           jb::tc_fence_after();
 #pragma unroll
@@ -257,114 +319,180 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
             umma_ts(tmem + 2 * KB + w * HDC, tmem + b * KB + ks * 8, desc_mn_sw128(v_s + st * C::KV_BYTES + ks * 2048, KB * 128, 1024),
                     idesc_o, (j | ks) ? 1u : 0u);
           jb::umma_commit(o_full(w));
-          if (j == nb - 1) jb::umma_commit(o_done(w));
+          if (last) jb::umma_commit(o_done(w));
           if (w == NT - 1) jb::umma_commit(v_empty + 8 * st);
-          if (NT == 2 && j + 1 < nb) ok = issue_s(w, j + 1);
-        }
-      }
-    }
-  } else if (n_tok > 0 && warp >= 2) {
-    const int w = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-    const int tl = w * tpt + row / G, token = tok0 + tl, head = kvh * G + row % G;
-    const bool valid = row < tpt * G && tl < n_tok;
-    int see_shared = 0, see_own = 0;                           // keys that the row sees
-    if (valid) {
-      const int see = (FORM == SPLIT ? s.positions[token] : first_pos + tl) + 1;
-      see_shared = min(see, s.prefix_len);
-      see_own = see - s.prefix_len;
-    }
-    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16), o_col = 2 * KB + w * HDC;
-    float m_ref = -CUDART_INF_F, l = 0.0f;
-    bool ok = true;
-    for (int j = 0; j < nb && ok; ++j) {
-      const int b = NT == 2 ? w : j & 1;
-      ok = jb::mbar_wait(s_full(b), (NT == 2 ? j : j >> 1) & 1, status, 43);
-      if (!ok) break;
-      jb::tc_fence_after();
-      uint32_t sr[KB];
-#pragma unroll
-      for (int c0 = 0; c0 < KB; c0 += 16) tmem_ld16(lane_addr + b * KB + c0, sr + c0);
-      jb::tmem_ld_wait();
-      const int see = j < n_shared ? see_shared - (block0 + j) * KB : see_own - (j - n_shared) * KB;
-      if (see < KB) {
-#pragma unroll
-        for (int c = 0; c < KB; ++c)
-          if (c >= see) sr[c] = 0xff800000u;   // -inf
-      }
-      const float mx = row_max<KB>(sr) * s.scale_log2;
-      // loads and stores of tensor memory are warp-wide: a warp rescales together if any of its rows has to
-      const bool grow = mx > m_ref + RESCALE_LOG2 || (m_ref == -CUDART_INF_F && mx > -CUDART_INF_F);
-      if (__any_sync(0xffffffffu, grow)) {
-        const float m_new = fmaxf(m_ref, mx);
-        if (j > 0) {
-          ok = jb::mbar_wait(o_full(w), (j - 1) & 1, status, 43);
-          if (!ok) break;
-          jb::tc_fence_after();
-          const float corr = m_new == -CUDART_INF_F ? 1.0f : exp2f(m_ref - m_new);
-#pragma unroll
-          for (int c0 = 0; c0 < HDC; c0 += 16) {
-            if (c0 >= s.hd) break;
-            uint32_t r[16];
-            tmem_ld16(lane_addr + o_col + c0, r);
-            jb::tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
-            tmem_st16(lane_addr + o_col + c0, r);
+          if (NT == 2 && more) {
+            if (fresh_q) ok = jb::mbar_wait(q_full, (turn + 1) & 1, status, 42), fresh_q = false;
+            ok = ok && issue_s(w, it + 1);
           }
-          tmem_st_wait();
-          l *= corr;
         }
-        m_ref = m_new;
+        if (!more) break;
+        ++j;
+        if (last) {
+          g = segment(at);
+          n = g.nb, j = 0, ++turn;
+        }
       }
-      l += exp_pack_sum<KB>(sr, s.scale_log2, m_ref == -CUDART_INF_F ? 0.0f : -m_ref);
-#pragma unroll
-      for (int c0 = 0; c0 < KB / 2; c0 += 16) tmem_st16(lane_addr + b * KB + c0, sr + c0);
-      tmem_st_wait();
-      jb::tc_fence_before();
-      jb::mbar_arrive(p_full(b));
     }
-    if (ok && nb > 0) ok = jb::mbar_wait(o_done(w), 0, status, 43);
-    if (ok) {
-      jb::tc_fence_after();
-      const size_t place = (size_t)token * s.nh + head;
-      if constexpr (FORM == SPLIT) {
-        const size_t item = (size_t)blockIdx.z * s.T * s.nh + place;
-        if (valid) part_ml[item] = make_float2(m_ref, l);
+  } else {
+    // two warps have the same 32 rows, each half of a block's keys (and of O's columns)
+    const int w = (warp - 2) >> 3, quarter = warp & 3, half = (warp - 2) >> 2 & 1, row = quarter * 32 + lane, pair = 1 + w * 4 + quarter;
+    constexpr int KH = KB / 2, DH = HDC / 2;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16), o_col = 2 * KB + w * HDC;
+    float* mine = swap + (w * 2 + half) * BM + row;
+    const float* other = swap + (w * 2 + (half ^ 1)) * BM + row;
+    // The two say to each other that a row's maximum has grown, or that a wait has run out: then both leave, behind a barrier that
+    // they share.  (A value is read before its place is written again: the writer has passed another barrier with the reader.)
+    int* stop = gave_up + w * 4 + quarter;
+    bool ok = true, both = true;
+    int it = 0, turn = 0;
+    auto meet = [&](float value) {
+      *mine = value;
+      if (!ok) *stop = 1;
+      pair_sync(pair);
+      both = *(volatile int*)stop == 0;
+      return *other;
+    };
+    for (int at = flat_begin; at < flat_end && both; ++turn) {
+      const Segment g = segment(at);
+      if (g.n_tok <= 0 && FORM != SHARED) break;
+      const int tl = w * tpt + row / G, token = g.tok0 + tl, head = g.kvh * G + row % G;
+      const bool valid = row < tpt * G && tl < g.n_tok;        // rows past tpt * G belong to no token
+      int see_shared = 0, see_own = 0;                         // keys that the row sees, counted from its half's first
+      if (valid) {
+        const int see = (FORM == SHARED ? s.positions[token] : seq_pos + token - seq_start) + 1;
+        see_shared = min(see, s.prefix_len) - g.block0 * KB - half * KH;
+        see_own = see - s.prefix_len - half * KH;
+      }
+      float m_ref = -CUDART_INF_F, l = 0.0f;
+      for (int j = 0; j < g.nb; ++j, ++it) {
+        const int b = NT == 2 ? w : it & 1;
+        const uint32_t s_at = lane_addr + b * KB;
+        ok = __all_sync(0xffffffffu, ok && jb::mbar_wait(s_full(b), (NT == 2 ? it : it >> 1) & 1, status, 43));
+        jb::tc_fence_after();
+        uint32_t sr[KH];
 #pragma unroll
-        for (int c0 = 0; c0 < HDC; c0 += 16) {
+        for (int c0 = 0; c0 < KH; c0 += 16) tmem_ld16(s_at + half * KH + c0, sr + c0);
+        jb::tmem_ld_wait();
+        const int see = j < g.n_shared ? see_shared - j * KB : see_own - (j - g.n_shared) * KB;
+        if (see < KH) {
+#pragma unroll
+          for (int c = 0; c < KH; ++c)
+            if (c >= see) sr[c] = 0xff800000u;   // -inf
+        }
+        float mx = row_max<KH>(sr) * s.scale_log2;
+        // behind this barrier both halves have their scores, and P may go where scores lie.  Loads and stores of tensor memory
+        // are warp-wide: the two warps rescale together if any of their rows has to
+        const bool grow = mx > m_ref + RESCALE_LOG2 || (m_ref == -CUDART_INF_F && mx > -CUDART_INF_F);
+        jb::tc_fence_before();
+        const bool any = pair_any(pair, grow || !ok);
+        jb::tc_fence_after();
+        if (any) {
+          mx = fmaxf(mx, meet(mx));   // the row's, over both halves
+          if (!both) break;
+          const float m_new = fmaxf(m_ref, mx);
+          if (j > 0) {
+            ok = __all_sync(0xffffffffu, jb::mbar_wait(o_full(w), (it - 1) & 1, status, 43));
+            if (!ok) continue;
+            jb::tc_fence_after();
+            const float corr = m_new == -CUDART_INF_F ? 1.0f : exp2f(m_ref - m_new);
+#pragma unroll
+            for (int c0 = 0; c0 < DH; c0 += 16) {
+              if (half * DH + c0 >= s.hd) break;
+              uint32_t r[16];
+              tmem_ld16(lane_addr + o_col + half * DH + c0, r);
+              jb::tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
+              tmem_st16(lane_addr + o_col + half * DH + c0, r);
+            }
+            tmem_st_wait();
+            l *= corr;
+          }
+          m_ref = m_new;
+        }
+        l += exp_pack_sum<KH>(sr, s.scale_log2, m_ref == -CUDART_INF_F ? 0.0f : -m_ref);
+#pragma unroll
+        for (int c0 = 0; c0 < KH / 2; c0 += 16) tmem_st16(s_at + half * (KH / 2) + c0, sr + c0);
+        tmem_st_wait();
+        jb::tc_fence_before();
+        jb::mbar_arrive(p_full(b));
+      }
+      if (!both) break;
+      if (ok && g.nb > 0) ok = __all_sync(0xffffffffu, jb::mbar_wait(o_done(w), turn & 1, status, 43));
+      const float theirs = meet(l);   // the row's sum over both halves
+      if (!both) break;
+      l = half == 0 ? l + theirs : theirs + l;
+      pair_sync(pair);                // (the place is read before it is written again)
+      jb::tc_fence_after();
+      const size_t place = (size_t)token * s.nh + head, all = (size_t)s.T * s.nh;
+      if constexpr (FORM == SHARED) {
+        const size_t item = g.slot * all + place;
+        if (valid && half == 0) part_ml[item] = make_float2(m_ref, l);
+#pragma unroll
+        for (int c1 = 0; c1 < DH; c1 += 16) {
+          const int c0 = half * DH + c1;
           if (c0 >= s.hd) break;
           uint32_t r[16];
           tmem_ld16(lane_addr + o_col + c0, r);   // warp-wide: rows without a token load too and store nothing
           jb::tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            if (valid && c0 + i < s.hd)
-              *reinterpret_cast<uint4*>(part_o + item * s.hd + c0 + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+          if (valid) store8(part_o + item * s.hd + c0, r);
+          if (valid && c0 + 8 < s.hd) store8(part_o + item * s.hd + c0 + 8, r + 8);
         }
+        jb::tc_fence_before();
+        jb::mbar_arrive(o_free(w));
       } else {
+        // the parts over the prefix weigh in (OWN); few, or the steps of many tokens that come here would not cut the prefix
+        const int slots = FORM == OWN && valid ? slots_of(parts, s, token, g.kvh) : 0;
+        if (FORM == OWN && parts.most > 0) jb::pdl_wait();
+        float top = m_ref;
+        for (int i = 0; i < slots; ++i) top = fmaxf(top, part_ml[i * all + place].x);
+        const float ref = top == -CUDART_INF_F ? 0.0f : top, own_weight = exp2f(m_ref - ref);
+        l *= own_weight;
+        for (int i = 0; i < slots; ++i) {
+          const float2 ml = part_ml[i * all + place];
+          l = fmaf(exp2f(ml.x - ref), ml.y, l);
+        }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         bool finite = true;
 #pragma unroll
-        for (int c0 = 0; c0 < HDC; c0 += 16) {
+        for (int c1 = 0; c1 < DH; c1 += 16) {
+          const int c0 = half * DH + c1;
           if (c0 >= s.hd) break;
           uint32_t r[16];
-          if (nb > 0) {
+          if (g.nb > 0) {
             tmem_ld16(lane_addr + o_col + c0, r);
             jb::tmem_ld_wait();
+          }
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = g.nb > 0 ? __uint_as_float(r[i]) * own_weight : 0.0f;
+          if constexpr (FORM == OWN) {
+            for (int i = 0; i < slots; ++i) {
+              const float f = exp2f(part_ml[i * all + place].x - ref);
+              float more[16];
+              load8(part_o + (i * all + place) * s.hd + c0, more);
+              if (c0 + 8 < s.hd) load8(part_o + (i * all + place) * s.hd + c0 + 8, more + 8);
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (e < 8 || c0 + 8 < s.hd) v[e] = fmaf(f, more[e], v[e]);
+            }
           }
           uint32_t p[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float a = nb > 0 ? __uint_as_float(r[2 * i]) * inv : 0.0f, c = nb > 0 ? __uint_as_float(r[2 * i + 1]) * inv : 0.0f;
-            finite = finite && (c0 + 2 * i >= s.hd || (isfinite(a) && isfinite(c)));
-            p[i] = pack_bf16(a, c);
+            const float x = v[2 * i] * inv, y = v[2 * i + 1] * inv;
+            finite = finite && (c0 + 2 * i >= s.hd || (isfinite(x) && isfinite(y)));
+            p[i] = pack_bf16(x, y);
           }
           if (valid) {
             *reinterpret_cast<uint4*>(out + place * s.hd + c0) = make_uint4(p[0], p[1], p[2], p[3]);
             if (c0 + 8 < s.hd) *reinterpret_cast<uint4*>(out + place * s.hd + c0 + 8) = make_uint4(p[4], p[5], p[6], p[7]);
           }
         }
-        unsigned again = __ballot_sync(0xffffffffu, valid && !finite);
+        // a row that is not finite is made once more by itself, by its first half's warp, when both halves have written
+        finite = meet(finite ? 0.0f : 1.0f) == 0.0f && finite;
+        unsigned again = half == 0 ? __ballot_sync(0xffffffffu, valid && !finite) : 0u;
         while (again) {
           const int l0 = __ffs(again) - 1;
           again &= again - 1;
@@ -375,6 +503,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
     }
     jb::tc_fence_before();
   }
+  if (FORM == OWN && parts.most > 0) jb::pdl_wait();   // (every thread, before the kernel ends)
   __syncthreads();
   if (warp == 1) {
     jb::tc_fence_after();
@@ -383,26 +512,23 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// bfloat16: each sequence's own pages, by warp-level products.  A CTA has 16 (token, head) rows of one sequence and kv head and a
-// range of its pages; each of its four warps takes 16 keys of every page through a ring of its own.
+// bfloat16: each sequence's own pages, by warp-level products.  A block has 16 (token, head) rows of one sequence and kv head and a
+// range of its pages; each of its two warps takes 32 keys of every page, which the copy engine brings (128-byte swizzle) into a
+// ring of its own: a warp asks for its next keys itself, and nothing waits for the other warp before the end.
+// The rows' queries stay in registers as the products take them.  32 keys a turn and one rescaling for all of them: with 16, by four
+// warps, a turn's 450 instructions moved half as many bytes (64 sequences of 30 to 700 keys, 8 kv heads of 128: 35 us).
 // ---------------------------------------------------------------------------
-constexpr int OWN_THREADS = 128;
+constexpr int OWN_WARPS = 2, OWN_THREADS = 32 * OWN_WARPS, OWN_KEYS = PAGE / OWN_WARPS;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint64_t policy) {
-  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], const bf16* p) {
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(jb::smem_u32(p)));
+               : "r"(at));
 }
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const bf16* p) {
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(jb::smem_u32(p)));
+               : "r"(at));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -414,103 +540,102 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 
 template <int HDC, int STAGES>
 struct Own {
-  static constexpr int LD = HDC + 8;                           // padded rows: an odd number of 16-byte pieces
-  static constexpr int TILE = PAGE * LD, STAGE = 2 * TILE;
+  static constexpr int SLABS = HDC / 64, SLAB = OWN_KEYS * 128;            // bytes of 64 numbers of a warp's keys
+  static constexpr int TILE = SLABS * SLAB, STAGE = 2 * TILE;              // keys, values
+  static constexpr int RING = OWN_WARPS * STAGES * STAGE;
   static constexpr int RED_LD = HDC + 4;
-  static constexpr int RED = (4 * 16 * RED_LD + 4 * 16 * 2) * 4;
-  static constexpr int RING = STAGES * STAGE * 2;
-  static constexpr int SMEM = 16 * LD * 2 + (RING > RED ? RING : RED);
+  static constexpr int RED = (OWN_WARPS * 16 * RED_LD + OWN_WARPS * 16 * 2 + 16 * 2 + 16 * 64) * 4;
+  static constexpr int SMEM = (RING > RED ? RING : RED) + OWN_WARPS * STAGES * 8;
 };
 
 // What is left to do with a row's sums over the warps: join them with the prefix's partial results and write the output
 // (own_slots == 1), or leave them as one more partial result.
 template <int HDC, int STAGES>
-__global__ void __launch_bounds__(OWN_THREADS) own_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_cache,
+__global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                          const bf16* __restrict__ q, const bf16* __restrict__ k_cache,
                                                           const bf16* __restrict__ v_cache, bf16* __restrict__ out,
                                                           float* __restrict__ part_o, float2* __restrict__ part_ml, const Step s,
-                                                          int prefix_slots, int own_slots, int row_blocks) {
+                                                          const Slots parts, int own_slots, int row_blocks, int* __restrict__ status) {
   typedef Own<HDC, STAGES> C;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  __shared__ int not_finite[16];
-  bf16* q_s = reinterpret_cast<bf16*>(smem_raw);
-  bf16* kv_s = q_s + 16 * C::LD;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full = (uint64_t*)(smem + (C::RING > C::RED ? C::RING : C::RED));
   const int G = s.nh / s.nkv, seq = blockIdx.x, kvh = blockIdx.y / row_blocks, rb = blockIdx.y % row_blocks, split = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = s.hd;
-  if (prefix_slots == 0) jb::pdl_wait();
+  const uint32_t ring = jb::smem_u32(smem) + warp * STAGES * C::STAGE, bar = jb::smem_u32(full + warp * STAGES);
+  if (lane == 0) {
+    for (int i = 0; i < STAGES; ++i) jb::mbar_init(bar + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  if (parts.most == 0) jb::pdl_wait();
   jb::pdl_launch_dependents();
   const int start = s.q_start[seq], q_len = s.q_start[seq + 1] - start;
   const int row0 = rb * 16, n_rows = min(16, q_len * G - row0);
-  const int first_pos = s.kv_len[seq] - q_len;
+  const int first_pos = s.kv_len[seq] - q_len - s.prefix_len;   // among the own keys
   // own keys that the block's last row sees; pages are cut evenly among the splits
-  const int see = n_rows > 0 ? first_pos + (row0 + n_rows - 1) / G + 1 - s.prefix_len : 0;
+  const int see = n_rows > 0 ? first_pos + (row0 + n_rows - 1) / G + 1 : 0;
   const int pages = min(see > 0 ? (see + PAGE - 1) / PAGE : 0, s.width);
-  const int p_begin = (int)((long long)split * pages / own_slots), p_end = (int)((long long)(split + 1) * pages / own_slots);
+  const int p_begin = (int)((long long)split * pages / own_slots);
+  int p_end = (int)((long long)(split + 1) * pages / own_slots);
+  if (p_end > p_begin && (p_end - 1) * PAGE + warp * OWN_KEYS >= see) --p_end;   // this warp's part of the last page: nobody sees it
   const int* table = s.table + (size_t)seq * s.ld_table;
-  uint64_t policy;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-  const int chunks = hd / 8;
-  auto issue = [&](int p, int st) {
-    const size_t row = ((size_t)max(table[p], 0) * s.nkv + kvh) * PAGE + warp * 16;
-    const uint32_t k_d = jb::smem_u32(kv_s + (size_t)st * C::STAGE + warp * 16 * C::LD), v_d = k_d + C::TILE * 2;
-    for (int ch = lane; ch < 16 * chunks; ch += 32) {
-      const int r = ch / chunks, c = ch % chunks;
-      cp_async16(k_d + (r * C::LD + c * 8) * 2, k_cache + (row + r) * hd + c * 8, policy);
-      cp_async16(v_d + (r * C::LD + c * 8) * 2, v_cache + (row + r) * hd + c * 8, policy);
+  const uint64_t policy = jb::read_once_policy();
+  const int nslab = (hd + 63) / 64;
+  auto issue = [&](int p) {   // by one lane
+    const int st = (p - p_begin) % STAGES, row = (max(table[p], 0) * s.nkv + kvh) * PAGE + warp * OWN_KEYS;
+    const uint32_t at = ring + st * C::STAGE;
+    jb::mbar_expect_tx(bar + 8 * st, 2 * nslab * C::SLAB);
+    for (int h = 0; h < nslab; ++h) {
+      jb::tma_load_2d(at + h * C::SLAB, &map_k, bar + 8 * st, h * 64, row, policy);
+      jb::tma_load_2d(at + C::TILE + h * C::SLAB, &map_v, bar + 8 * st, h * 64, row, policy);
     }
   };
-  if (p_begin < p_end) {
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-      if (p_begin + i < p_end) issue(p_begin + i, i);
-      cp_async_commit();
-    }
-    if (hd < HDC) {   // columns behind the head's numbers
-      const int pad = HDC - hd;
-      for (int i = threadIdx.x; i < STAGES * 2 * PAGE * pad; i += OWN_THREADS)
-        kv_s[(size_t)(i / pad) * C::LD + hd + i % pad] = __float2bfloat16_rn(0.0f);
-    }
-    for (int i = threadIdx.x; i < 16 * (HDC / 8); i += OWN_THREADS) {
-      const int r = i / (HDC / 8), c = i % (HDC / 8), rr = row0 + r;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (r < n_rows && c * 8 < hd)
-        v = *reinterpret_cast<const uint4*>(q + ((size_t)(start + rr / G) * s.nh + kvh * G + rr % G) * hd + c * 8);
-      *reinterpret_cast<uint4*>(q_s + r * C::LD + c * 8) = v;
-    }
-  }
+  if (lane == 0)
+    for (int i = 0; i < STAGES; ++i)
+      if (p_begin + i < p_end) issue(p_begin + i);
+  // the rows' queries as the A operand of the products: lane (g, c) has rows g and g + 8, numbers 2 c, 2 c + 1 and 8 behind of every 16
+  uint32_t qa[HDC / 16][4];
   float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.0f, 0.0f}, o[HDC / 8][4];
-#pragma unroll
-  for (int j = 0; j < HDC / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
   int see_row[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const int row = (lane >> 2) + 8 * r;
-    see_row[r] = row < n_rows ? first_pos + (row0 + row) / G + 1 - s.prefix_len : 0;
-  }
-  __syncthreads();
-  for (int p = p_begin; p < p_end; ++p) {
-    const int st = (p - p_begin) % STAGES;
-    if (p + STAGES - 1 < p_end) issue(p + STAGES - 1, (p - p_begin + STAGES - 1) % STAGES);
-    cp_async_commit();
-    cp_async_wait<STAGES - 1>();
-    __syncwarp();
-    const bf16* k_t = kv_s + (size_t)st * C::STAGE + warp * 16 * C::LD;
-    const bf16* v_t = k_t + C::TILE;
-    float x[2][4];
+    const int row = (lane >> 2) + 8 * r, rr = row0 + row;
+    const bool valid = row < n_rows && p_begin < p_end;
+    see_row[r] = valid ? first_pos + rr / G + 1 : 0;
+    const bf16* src = q + ((size_t)(start + (valid ? rr / G : 0)) * s.nh + kvh * G + rr % G) * hd + 2 * (lane & 3);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.0f;
+    for (int ks = 0; ks < HDC / 16; ++ks)
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        qa[ks][r + 2 * half] = valid && ks * 16 + half * 8 < hd ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + half * 8) : 0u;
+  }
+#pragma unroll
+  for (int j = 0; j < HDC / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+  bool ok = true;
+  for (int p = p_begin; p < p_end; ++p) {
+    const int turn = p - p_begin, st = turn % STAGES;
+    ok = jb::mbar_wait(bar + 8 * st, (turn / STAGES) & 1, status, 53);
+    if (!ok) break;
+    const uint32_t k_t = ring + st * C::STAGE, v_t = k_t + C::TILE;
+    float x[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < HDC / 16; ++ks) {
       if (ks * 16 >= hd) break;
-      uint32_t a[4], b[4];
-      ldmatrix_x4(a, q_s + (lane & 15) * C::LD + ks * 16 + (lane >> 4) * 8);
-      ldmatrix_x4(b, k_t + ((lane & 7) + ((lane >> 4) << 3)) * C::LD + ks * 16 + ((lane >> 3) & 1) * 8);
-      mma_bf16(x[0], a, b[0], b[1]);
-      mma_bf16(x[1], a, b[2], b[3]);
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        uint32_t b[4];
+        const int key = j * 8 + (lane & 7) + ((lane >> 4) << 3), piece = (ks % 4) * 2 + ((lane >> 3) & 1);
+        ldmatrix_x4(b, k_t + (ks / 4) * C::SLAB + key * 128 + ((piece ^ (key & 7)) << 4));
+        mma_bf16(x[j], qa[ks], b[0], b[1]);
+        mma_bf16(x[j + 1], qa[ks], b[2], b[3]);
+      }
     }
     float mx[2] = {-CUDART_INF_F, -CUDART_INF_F}, corr[2], ref[2];
-    const int key0 = p * PAGE + warp * 16 + 2 * (lane & 3);
+    const int key0 = p * PAGE + warp * OWN_KEYS + 2 * (lane & 3);
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         x[j][e] = key0 + j * 8 + (e & 1) < see_row[e >> 1] ? x[j][e] * s.scale_log2 : -CUDART_INF_F;
@@ -522,34 +647,43 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const bf16* __restrict
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
       const float m_new = fmaxf(m[r], mx[r]);
       ref[r] = m_new == -CUDART_INF_F ? 0.0f : m_new;
-      corr[r] = exp2f(m[r] - ref[r]);
+      corr[r] = fast_exp2(m[r] - ref[r]);
       m[r] = m_new;
       l[r] *= corr[r];
     }
 #pragma unroll
     for (int j = 0; j < HDC / 8; ++j) o[j][0] *= corr[0], o[j][1] *= corr[0], o[j][2] *= corr[1], o[j][3] *= corr[1];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[j][e] = exp2f(x[j][e] - ref[e >> 1]);
+        x[j][e] = fast_exp2(x[j][e] - ref[e >> 1]);
         l[e >> 1] += x[j][e];
       }
-    uint32_t a[4] = {pack_bf16(x[0][0], x[0][1]), pack_bf16(x[0][2], x[0][3]), pack_bf16(x[1][0], x[1][1]), pack_bf16(x[1][2], x[1][3])};
 #pragma unroll
-    for (int j = 0; j < HDC / 8; j += 2) {
-      if (j * 8 >= hd) break;
-      uint32_t b[4];
-      ldmatrix_x4_trans(b, v_t + (lane & 15) * C::LD + j * 8 + (lane >> 4) * 8);
-      mma_bf16(o[j], a, b[0], b[1]);
-      mma_bf16(o[j + 1], a, b[2], b[3]);
+    for (int kk = 0; kk < 2; ++kk) {
+      const uint32_t a[4] = {pack_bf16(x[2 * kk][0], x[2 * kk][1]), pack_bf16(x[2 * kk][2], x[2 * kk][3]),
+                             pack_bf16(x[2 * kk + 1][0], x[2 * kk + 1][1]), pack_bf16(x[2 * kk + 1][2], x[2 * kk + 1][3])};
+#pragma unroll
+      for (int j = 0; j < HDC / 8; j += 2) {
+        if (j * 8 >= hd) break;
+        uint32_t b[4];
+        const int key = kk * 16 + (lane & 15), piece = j % 8 + (lane >> 4);
+        ldmatrix_x4_trans(b, v_t + (j / 8) * C::SLAB + key * 128 + ((piece ^ (key & 7)) << 4));
+        mma_bf16(o[j], a, b[0], b[1]);
+        mma_bf16(o[j + 1], a, b[2], b[3]);
+      }
     }
-    __syncwarp();
+    __syncwarp();   // the warp is done with the stage
+    if (lane == 0 && p + STAGES < p_end) issue(p + STAGES);
   }
   // ---- the warps' results meet in shared memory ----
-  __syncthreads();
-  float* red_o = reinterpret_cast<float*>(kv_s);
-  float* red_ml = red_o + 4 * 16 * C::RED_LD;
+  if (!__syncthreads_and(ok)) {   // (a wait ran out: the status word says so; nothing is in flight into the ring but what ran out)
+    jb::pdl_wait();
+    return;
+  }
+  float* red_o = reinterpret_cast<float*>(smem);
+  float* red_ml = red_o + OWN_WARPS * 16 * C::RED_LD;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -563,17 +697,19 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const bf16* __restrict
     for (int j = 0; j < HDC / 8; ++j)
       *reinterpret_cast<float2*>(red_o + row * C::RED_LD + j * 8 + 2 * (lane & 3)) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
   }
-  if (threadIdx.x < 16) not_finite[threadIdx.x] = 0;
   __syncthreads();
-  if (prefix_slots > 0) jb::pdl_wait();   // the prefix's partial results are there
-  finish_rows<bf16, 4, 16, OWN_THREADS>(q, k_cache, v_cache, out, part_o, part_ml, s, red_o, red_ml, C::RED_LD, not_finite, max(n_rows, 0),
-                                        row0, start, seq, kvh, prefix_slots, own_slots, split);
+  if (parts.most > 0) jb::pdl_wait();   // the prefix's partial results are there
+  finish_rows<bf16, OWN_WARPS, 16, OWN_THREADS>(q, k_cache, v_cache, out, part_o, part_ml, s, parts, red_o, red_ml, C::RED_LD,
+                                                red_ml + OWN_WARPS * 16 * 2 + 32, red_ml + OWN_WARPS * 16 * 2, max(n_rows, 0), row0, start, seq,
+                                                kvh, own_slots > 1 ? parts.most + split : -1);
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-bool make_maps(CUtensorMap* mq, CUtensorMap* mk, CUtensorMap* mv, const void* q, const void* k, const void* v, const Step& s, int n_pages) {
+// q's tiles (null: none are wanted), and the pages in boxes of `keys` rows
+bool make_maps(CUtensorMap* mq, CUtensorMap* mk, CUtensorMap* mv, const void* q, const void* k, const void* v, const Step& s, int n_pages,
+               int keys) {
   static jb::EncodeTiledFn fn = nullptr;
   if (!fn) {
     void* p = nullptr;
@@ -583,7 +719,7 @@ bool make_maps(CUtensorMap* mq, CUtensorMap* mk, CUtensorMap* mv, const void* q,
     fn = (jb::EncodeTiledFn)p;
   }
   const cuuint32_t el[4] = {1, 1, 1, 1};
-  {
+  if (mq) {
     const cuuint64_t G = s.nh / s.nkv, hd = s.hd;
     const cuuint64_t dims[4] = {hd, G, (cuuint64_t)s.nkv, (cuuint64_t)s.T}, strides[3] = {hd * 2, G * hd * 2, (cuuint64_t)s.nh * hd * 2};
     const cuuint32_t box[4] = {64, (cuuint32_t)G, 1, (cuuint32_t)(BM / G)};
@@ -593,7 +729,7 @@ bool make_maps(CUtensorMap* mq, CUtensorMap* mk, CUtensorMap* mv, const void* q,
   }
   for (int which = 0; which < 2; ++which) {
     const cuuint64_t dims[2] = {(cuuint64_t)s.hd, (cuuint64_t)n_pages * s.nkv * PAGE}, strides[1] = {(cuuint64_t)s.hd * 2};
-    const cuuint32_t box[2] = {64, PAGE};
+    const cuuint32_t box[2] = {64, (cuuint32_t)keys};
     if (fn(which ? mv : mk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(which ? v : k), dims, strides, box, el,
            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
@@ -603,8 +739,8 @@ bool make_maps(CUtensorMap* mq, CUtensorMap* mk, CUtensorMap* mv, const void* q,
 }
 
 template <int HDC, int NT, int KB, Form FORM>
-cudaError_t tc_go(dim3 grid, cudaStream_t stream, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const bf16* q,
-                  const bf16* k, const bf16* v, bf16* out, float* part_o, float2* part_ml, const Step& s, int splits, int* status) {
+cudaError_t tc_go(dim3 grid, cudaStream_t stream, const CUtensorMap* maps, const bf16* q, const bf16* k, const bf16* v, bf16* out,
+                  float* part_o, float2* part_ml, const Step& s, const Slots& parts, int* status) {
   typedef Tc<HDC, NT, KB> C;
   static bool configured = false;
   if (!configured) {
@@ -613,12 +749,24 @@ cudaError_t tc_go(dim3 grid, cudaStream_t stream, const CUtensorMap& mq, const C
     configured = true;
   }
   jb::Launch cfg(grid, dim3(C::THREADS), C::SMEM, stream);
-  return cudaLaunchKernelEx(&cfg.c, prefix_tc_kernel<HDC, NT, KB, FORM>, mq, mk, mv, q, k, v, out, part_o, part_ml, s, splits, status);
+  return cudaLaunchKernelEx(&cfg.c, prefix_tc_kernel<HDC, NT, KB, FORM>, maps[0], maps[1], maps[2], q, k, v, out, part_o, part_ml, s, parts,
+                            status);
+}
+template <Form FORM>
+cudaError_t tc_pick(int nt, dim3 grid, cudaStream_t stream, const CUtensorMap* maps, const bf16* q, const bf16* k, const bf16* v, bf16* out,
+                    float* part_o, float2* part_ml, const Step& s, const Slots& parts, int* status) {
+#define JB_GO(HDC, NT, KB) return tc_go<HDC, NT, KB, FORM>(grid, stream, maps, q, k, v, out, part_o, part_ml, s, parts, status)
+  if (s.hd > 128) JB_GO(256, 1, 64);
+  if (s.hd > 64 && nt == 2) JB_GO(128, 2, 128);
+  if (s.hd > 64) JB_GO(128, 1, 128);
+  if (nt == 2) JB_GO(64, 2, 128);
+  JB_GO(64, 1, 128);
+#undef JB_GO
 }
 
 template <int HDC, int STAGES>
-cudaError_t own_go(dim3 grid, cudaStream_t stream, const bf16* q, const bf16* k, const bf16* v, bf16* out, float* part_o, float2* part_ml,
-                   const Step& s, int prefix_slots, int own_slots, int row_blocks) {
+cudaError_t own_go(dim3 grid, cudaStream_t stream, const CUtensorMap* maps, const bf16* q, const bf16* k, const bf16* v, bf16* out,
+                   float* part_o, float2* part_ml, const Step& s, const Slots& parts, int own_slots, int row_blocks, int* status) {
   typedef Own<HDC, STAGES> C;
   static bool configured = false;
   if (!configured) {
@@ -627,19 +775,21 @@ cudaError_t own_go(dim3 grid, cudaStream_t stream, const bf16* q, const bf16* k,
     configured = true;
   }
   jb::Launch cfg(grid, dim3(OWN_THREADS), C::SMEM, stream);
-  return cudaLaunchKernelEx(&cfg.c, own_kernel<HDC, STAGES>, q, k, v, out, part_o, part_ml, s, prefix_slots, own_slots, row_blocks);
+  return cudaLaunchKernelEx(&cfg.c, own_kernel<HDC, STAGES>, maps[0], maps[1], q, k, v, out, part_o, part_ml, s, parts, own_slots, row_blocks,
+                            status);
 }
 
 }  // namespace
 
-// bfloat16.  splits = 0: tiles of one sequence each walk all their keys (WHOLE).  Else the prefix's keys in `splits` ranges for all
-// rows together and the own keys in `own_slots` ranges a sequence; part_o [splits (+ own_slots if > 1)][T][nh][hd] float32 and
-// part_ml [..][T][nh][2] are scratch.  tiles: row tiles a CTA, 1 or 2.
+// q, out [T, nh hd], caches [n_pages, nkv, 64, hd], all bfloat16.  tiles: row tiles of a block, 1 or 2 (one for heads of more than 128
+// numbers).  shared_ctas > 0: the prefix for all rows together by that many blocks, which cut a row's keys into at most `most`
+// ranges; the own keys by tiles (own_tiles), or in own_slots ranges a sequence; part_o [most (+ own_slots if > 1)][T][nh][hd] float32
+// and part_ml [..][T][nh][2] are scratch.  shared_ctas = 0: tiles of one sequence each walk all their keys.
 JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const void* v_cache, void* out, float* part_o, float* part_ml,
                                        const int* prefix_pages, int prefix_len, const int* block_table, int ld_table, int width,
                                        const int* q_start, const int* kv_len, const int* positions, int T, int n_pages, int n_seqs,
-                                       int nh, int nkv, int hd, int page_size, float scale, int max_q_len, int tiles, int splits,
-                                       int own_slots, int* status, cudaStream_t stream) {
+                                       int nh, int nkv, int hd, int page_size, float scale, int max_q_len, int tiles, int shared_ctas,
+                                       int most, int own_tiles, int own_slots, int* status, cudaStream_t stream) {
   if (T <= 0 || n_seqs <= 0 || max_q_len <= 0) return 0;
   JB_REFUSE(page_size != PAGE, "attention_prefix: page size %d (need %d)", page_size, PAGE);
   JB_REFUSE(nkv <= 0 || nh % nkv != 0, "attention_prefix: %d heads are not a multiple of %d kv heads", nh, nkv);
@@ -649,46 +799,46 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
   JB_REFUSE(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15, "attention_prefix: operands must be 16-byte aligned");
   JB_REFUSE((long long)n_pages * nkv * PAGE > 0x7fffffffll, "attention_prefix: %d pages of %d heads are more rows than a tensor map counts",
             n_pages, nkv);
-  JB_REFUSE(splits < 0 || own_slots < 1 || splits > (prefix_len + 127) / 128, "attention_prefix: %d ranges of a prefix of %d tokens", splits,
-            prefix_len);
+  JB_REFUSE(n_seqs > 65535 || prefix_len < 0 || shared_ctas < 0 || own_slots < 1 || most < 0 || most > 64 || (shared_ctas > 0) != (most > 0) ||
+                (shared_ctas > 0 && prefix_len == 0) || (own_tiles && own_slots > 1),
+            "attention_prefix: a prefix of %d tokens in %d ranges by %d blocks, %d ranges of own keys of %d sequences", prefix_len, most,
+            shared_ctas, own_slots, n_seqs);
   const Step s{prefix_pages, block_table, q_start, kv_len, positions, prefix_len, ld_table, width, T, n_seqs, nh, nkv, hd, scale * LOG2E};
   const bf16 *qb = (const bf16*)q, *kb = (const bf16*)k_cache, *vb = (const bf16*)v_cache;
   bf16* ob = (bf16*)out;
   float2* ml = (float2*)part_ml;
-  const bool whole = splits == 0 && prefix_len > 0;
+  const int nt = hd > 128 ? 1 : tiles, step = nt * (BM / G), keys = hd > 128 ? 64 : 128;
+  Slots parts{0, 0, 0, 1, 0, 1};
+  CUtensorMap maps[3];
+  if ((shared_ctas > 0 || own_tiles) && !make_maps(&maps[0], &maps[1], &maps[2], q, k_cache, v_cache, s, n_pages, PAGE)) return JB_ERR_TENSORMAP;
   cudaError_t e = cudaSuccess;
-  if (whole || splits > 0) {
-    CUtensorMap mq, mk, mv;
-    if (!make_maps(&mq, &mk, &mv, q, k_cache, v_cache, s, n_pages)) return JB_ERR_TENSORMAP;
-    const int tpt = BM / G, nt = hd > 128 ? 1 : tiles;
-    if (whole) {
-      const dim3 grid(nkv, (max_q_len + nt * tpt - 1) / (nt * tpt), n_seqs);
-      if (hd > 128) return (int)tc_go<256, 1, 64, WHOLE>(grid, stream, mq, mk, mv, qb, kb, vb, ob, nullptr, nullptr, s, 0, status);
-      if (hd > 64)
-        return (int)(nt == 2 ? tc_go<128, 2, 128, WHOLE>(grid, stream, mq, mk, mv, qb, kb, vb, ob, nullptr, nullptr, s, 0, status)
-                             : tc_go<128, 1, 128, WHOLE>(grid, stream, mq, mk, mv, qb, kb, vb, ob, nullptr, nullptr, s, 0, status));
-      return (int)(nt == 2 ? tc_go<64, 2, 128, WHOLE>(grid, stream, mq, mk, mv, qb, kb, vb, ob, nullptr, nullptr, s, 0, status)
-                           : tc_go<64, 1, 128, WHOLE>(grid, stream, mq, mk, mv, qb, kb, vb, ob, nullptr, nullptr, s, 0, status));
-    }
-    const dim3 grid(nkv, (T + nt * tpt - 1) / (nt * tpt), splits);
-    if (hd > 128) e = tc_go<256, 1, 64, SPLIT>(grid, stream, mq, mk, mv, qb, kb, vb, ob, part_o, ml, s, splits, status);
-    else if (hd > 64)
-      e = nt == 2 ? tc_go<128, 2, 128, SPLIT>(grid, stream, mq, mk, mv, qb, kb, vb, ob, part_o, ml, s, splits, status)
-                  : tc_go<128, 1, 128, SPLIT>(grid, stream, mq, mk, mv, qb, kb, vb, ob, part_o, ml, s, splits, status);
-    else
-      e = nt == 2 ? tc_go<64, 2, 128, SPLIT>(grid, stream, mq, mk, mv, qb, kb, vb, ob, part_o, ml, s, splits, status)
-                  : tc_go<64, 1, 128, SPLIT>(grid, stream, mq, mk, mv, qb, kb, vb, ob, part_o, ml, s, splits, status);
+  if (shared_ctas > 0) {
+    const int blocks = (prefix_len + keys - 1) / keys;
+    const long long total = (long long)((T + step - 1) / step) * nkv * blocks;
+    JB_REFUSE(shared_ctas > total || total > 0x7fffffffll, "attention_prefix: %d blocks for %lld key blocks", shared_ctas, total);
+    parts = Slots{-1, most, blocks, (int)(total / shared_ctas), (int)(total % shared_ctas), step};
+    // a tile's blocks begin anywhere in a range, unless ranges divide them
+    const bool even = parts.longer == 0 && blocks % parts.per == 0;
+    JB_REFUSE((even ? blocks / parts.per : (blocks + parts.per - 2) / parts.per + 1) > most, "attention_prefix: %d blocks cut %d key blocks into more than %d ranges",
+              shared_ctas, blocks, most);
+    e = tc_pick<SHARED>(nt, dim3(shared_ctas), stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status);
     if (e != cudaSuccess) return (int)e;
   }
+  if (own_tiles) {
+    const dim3 grid(nkv, (max_q_len + step - 1) / step, n_seqs);
+    return (int)(shared_ctas > 0 ? tc_pick<OWN>(nt, grid, stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status)
+                                 : tc_pick<WHOLE>(nt, grid, stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status));
+  }
+  JB_REFUSE(shared_ctas == 0 && prefix_len > 0, "attention_prefix: nothing walks the prefix");
   const int row_blocks = (max_q_len * G + 15) / 16;
   const dim3 grid(n_seqs, nkv * row_blocks, own_slots);
-  if (hd > 128) e = own_go<256, 2>(grid, stream, qb, kb, vb, ob, part_o, ml, s, splits, own_slots, row_blocks);
-  else if (hd > 64) e = own_go<128, 3>(grid, stream, qb, kb, vb, ob, part_o, ml, s, splits, own_slots, row_blocks);
-  else e = own_go<64, 3>(grid, stream, qb, kb, vb, ob, part_o, ml, s, splits, own_slots, row_blocks);
-  if (e != cudaSuccess) return (int)e;
-  if (own_slots > 1) {
+  if (!make_maps(nullptr, &maps[1], &maps[2], q, k_cache, v_cache, s, n_pages, OWN_KEYS)) return JB_ERR_TENSORMAP;
+  if (hd > 128) e = own_go<256, 2>(grid, stream, maps + 1, qb, kb, vb, ob, part_o, ml, s, parts, own_slots, row_blocks, status);
+  else if (hd > 64) e = own_go<128, 2>(grid, stream, maps + 1, qb, kb, vb, ob, part_o, ml, s, parts, own_slots, row_blocks, status);
+  else e = own_go<64, 3>(grid, stream, maps + 1, qb, kb, vb, ob, part_o, ml, s, parts, own_slots, row_blocks, status);
+  if (e == cudaSuccess && own_slots > 1) {
     jb::Launch cfg(dim3((unsigned)(((long long)T * nh + 3) / 4)), dim3(128), 0, stream);
-    e = cudaLaunchKernelEx(&cfg.c, join_kernel<bf16>, qb, kb, vb, ob, (const float*)part_o, (const float2*)ml, s, splits + own_slots);
+    e = cudaLaunchKernelEx(&cfg.c, join_kernel<bf16>, qb, kb, vb, ob, (const float*)part_o, (const float2*)ml, s, parts, own_slots);
   }
   return (int)e;
 }

@@ -34,7 +34,7 @@ struct Tile {
   // queries, keys, values, weights; the rows' results take the place of keys and values at the end
   static constexpr int FLOATS = ROWS * LD + PAGE * LD + PAGE * LD + ROWS * LD_P;
   static constexpr int SMEM = FLOATS * 4;
-  static_assert(SMEM <= 232448 && ROWS <= 2 * PAGE, "shared memory of one block");
+  static_assert(SMEM <= 232448 && ROWS <= PAGE, "shared memory of one block");
 };
 
 // OWN: the rows of one sequence over its own pages.  Else the rows of all sequences over a range of the prefix's pages.
@@ -42,13 +42,13 @@ template <int HDC, int RR, bool OWN>
 __global__ void __launch_bounds__(THREADS) tile_f32_kernel(const float* __restrict__ q, const float* __restrict__ k_cache,
                                                            const float* __restrict__ v_cache, float* __restrict__ out,
                                                            float* __restrict__ part_o, float2* __restrict__ part_ml, const Step s,
-                                                           int prefix_slots, int own_slots, int row_blocks) {
+                                                           const Slots parts, int own_slots, int row_blocks) {
   typedef Tile<HDC, RR> C;
   extern __shared__ __align__(16) float smem[];
-  __shared__ int not_finite[C::ROWS];
-  __shared__ float red_ml[2 * C::ROWS];
+  __shared__ float red_ml[2 * C::ROWS], row_sums[2 * C::ROWS];
   float *q_s = smem, *k_s = q_s + C::ROWS * C::LD, *v_s = k_s + PAGE * C::LD, *p_s = v_s + PAGE * C::LD;
   const int G = s.nh / s.nkv, hd = s.hd, tid = threadIdx.x, x = tid & 15, y = tid >> 4;
+  const int prefix_slots = parts.fixed;
   if (!OWN || prefix_slots == 0) jb::pdl_wait();
   jb::pdl_launch_dependents();
   int seq = 0, kvh, split = blockIdx.z, token0 = 0, row0, n_rows, first_pos = 0, p_begin, p_end;
@@ -188,20 +188,16 @@ __global__ void __launch_bounds__(THREADS) tile_f32_kernel(const float* __restri
       if (4 * x + 64 * i < hd) *reinterpret_cast<ulonglong2*>(red_o + row * C::LD + 4 * x + 64 * i) = v;
     }
   }
-  for (int i = tid; i < C::ROWS; i += THREADS) not_finite[i] = 0;
   __syncthreads();
   if (OWN && prefix_slots > 0) jb::pdl_wait();
-  if constexpr (OWN)
-    finish_rows<float, 1, C::ROWS, THREADS>(q, k_cache, v_cache, out, part_o, part_ml, s, red_o, red_ml, C::LD, not_finite, max(n_rows, 0), row0,
-                                            token0, seq, kvh, prefix_slots, own_slots, split);
-  else   // one more partial result, in this range's slot
-    finish_rows<float, 1, C::ROWS, THREADS>(q, k_cache, v_cache, out, part_o, part_ml, s, red_o, red_ml, C::LD, not_finite, n_rows, row0, 0, 0,
-                                            kvh, 0, 2, split);
+  // (the slots' weights take the place of the values)
+  finish_rows<float, 1, C::ROWS, THREADS>(q, k_cache, v_cache, out, part_o, part_ml, s, parts, red_o, red_ml, C::LD, v_s, row_sums,
+                                          max(n_rows, 0), row0, token0, seq, kvh, !OWN ? split : own_slots > 1 ? parts.most + split : -1);
 }
 
 template <int HDC, int RR, bool OWN>
 cudaError_t go(dim3 grid, cudaStream_t stream, const float* q, const float* k, const float* v, float* out, float* part_o, float2* part_ml,
-               const Step& s, int prefix_slots, int own_slots, int row_blocks) {
+               const Step& s, const Slots& parts, int own_slots, int row_blocks) {
   typedef Tile<HDC, RR> C;
   static bool configured = false;
   if (!configured) {
@@ -210,14 +206,14 @@ cudaError_t go(dim3 grid, cudaStream_t stream, const float* q, const float* k, c
     configured = true;
   }
   jb::Launch cfg(grid, dim3(THREADS), C::SMEM, stream);
-  return cudaLaunchKernelEx(&cfg.c, tile_f32_kernel<HDC, RR, OWN>, q, k, v, out, part_o, part_ml, s, prefix_slots, own_slots, row_blocks);
+  return cudaLaunchKernelEx(&cfg.c, tile_f32_kernel<HDC, RR, OWN>, q, k, v, out, part_o, part_ml, s, parts, own_slots, row_blocks);
 }
 template <bool OWN>
 cudaError_t pick(int hd, int rows, dim3 grid, cudaStream_t stream, const float* q, const float* k, const float* v, float* out,
-                 float* part_o, float2* part_ml, const Step& s, int prefix_slots, int own_slots, int row_blocks) {
+                 float* part_o, float2* part_ml, const Step& s, const Slots& parts, int own_slots, int row_blocks) {
 #define JB_GO(HDC)                                                                                                              \
-  return rows == 16 ? go<HDC, 1, OWN>(grid, stream, q, k, v, out, part_o, part_ml, s, prefix_slots, own_slots, row_blocks)       \
-                    : go<HDC, 4, OWN>(grid, stream, q, k, v, out, part_o, part_ml, s, prefix_slots, own_slots, row_blocks)
+  return rows == 16 ? go<HDC, 1, OWN>(grid, stream, q, k, v, out, part_o, part_ml, s, parts, own_slots, row_blocks)       \
+                    : go<HDC, 4, OWN>(grid, stream, q, k, v, out, part_o, part_ml, s, parts, own_slots, row_blocks)
   if (hd > 128) JB_GO(256);
   if (hd > 64) JB_GO(128);
   JB_GO(64);
@@ -246,20 +242,21 @@ JB_EXPORT int jb_attention_prefix_f32(const void* q, const void* k_cache, const 
     jb::Launch cfg(dim3((unsigned)(((long long)T * nh + 3) / 4)), dim3(128), 0, stream);
     return (int)cudaLaunchKernelEx(&cfg.c, rows_f32_kernel, qf, kf, vf, of, s);
   }
-  JB_REFUSE((rows != 16 && rows != 64) || (own_rows != 16 && own_rows != 64) || own_slots < 1 || splits < 0 || (splits > 0 && prefix_len <= 0) ||
+  JB_REFUSE((rows != 16 && rows != 64) || (own_rows != 16 && own_rows != 64) || own_slots < 1 || splits < 0 || splits > 64 || (splits > 0 && prefix_len <= 0) ||
                 (splits == 0 && prefix_len > 0),
             "attention_prefix: %d ranges of a prefix of %d tokens, blocks of %d and %d rows", splits, prefix_len, rows, own_rows);
   const int G = nh / nkv;
+  const Slots parts{splits, splits, 0, 1, 0, 1};
   cudaError_t e = cudaSuccess;
   if (splits > 0)
-    e = pick<false>(hd, rows, dim3(nkv, (unsigned)(((long long)T * G + rows - 1) / rows), splits), stream, qf, kf, vf, of, part_o, ml, s, splits,
+    e = pick<false>(hd, rows, dim3(nkv, (unsigned)(((long long)T * G + rows - 1) / rows), splits), stream, qf, kf, vf, of, part_o, ml, s, parts,
                     own_slots, 0);
   if (e != cudaSuccess) return (int)e;
   const int row_blocks = (max_q_len * G + own_rows - 1) / own_rows;
-  e = pick<true>(hd, own_rows, dim3(n_seqs, nkv * row_blocks, own_slots), stream, qf, kf, vf, of, part_o, ml, s, splits, own_slots, row_blocks);
+  e = pick<true>(hd, own_rows, dim3(n_seqs, nkv * row_blocks, own_slots), stream, qf, kf, vf, of, part_o, ml, s, parts, own_slots, row_blocks);
   if (e == cudaSuccess && own_slots > 1) {
     jb::Launch cfg(dim3((unsigned)(((long long)T * nh + 3) / 4)), dim3(128), 0, stream);
-    e = cudaLaunchKernelEx(&cfg.c, join_kernel<float>, qf, kf, vf, of, (const float*)part_o, (const float2*)ml, s, splits + own_slots);
+    e = cudaLaunchKernelEx(&cfg.c, join_kernel<float>, qf, kf, vf, of, (const float*)part_o, (const float2*)ml, s, parts, own_slots);
   }
   return (int)e;
 }

@@ -26,10 +26,19 @@ constexpr int THREADS = 512, WARPS = THREADS / 32, PIECE = CHUNK / WARPS;   // a
 constexpr int MAX_CLUSTER = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 
-// The weight of x against a maximum; heat_log2 = log2(e) / T.  -inf, and what is not a number, weighs nothing.
+// 2^x by the special-function unit (2 ulp); -inf gives 0
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// What is not a number counts as -inf.
+__device__ __forceinline__ float number(float x) { return fmaxf(x, -CUDART_INF_F); }
+// The weight of x (a number, or -inf) against a maximum; heat_log2 = log2(e) / T, finite.  A maximum of +inf or -inf: `weight`.
+__device__ __forceinline__ float finite_weight(float x, float top, float heat_log2) { return fast_exp2((x - top) * heat_log2); }
 __device__ __forceinline__ float weight(float x, float top, float heat_log2) {
   if (!(x > -CUDART_INF_F)) return 0.0f;
-  return x == top ? 1.0f : exp2f((x - top) * heat_log2);
+  return x == top ? 1.0f : finite_weight(x, top, heat_log2);
 }
 
 struct Chunk {
@@ -42,7 +51,8 @@ __device__ __forceinline__ void keep_first(float& top, int& arg, float t, int i)
   if (t > top || (t == top && i < arg)) top = t, arg = i;
 }
 
-template <bool VECTORS>
+// ARGMAX: only where T = 0 asks for it (a third of the instructions a logit).
+template <bool VECTORS, bool ARGMAX>
 __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(const float* __restrict__ logits, Chunk* __restrict__ stats, int V,
                                                               int chunks, float heat_log2) {
   __shared__ float s_top[STATS_THREADS / 32], s_sum[STATS_THREADS / 32];
@@ -53,8 +63,6 @@ __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(const float* __res
   const float* x = logits + (size_t)row * V + v0;
   const int n = min(CHUNK, V - v0);
   float v[STATS_PER];
-  float top = -CUDART_INF_F;
-  int arg = 0x7fffffff;
   if constexpr (VECTORS) {
 #pragma unroll
     for (int i = 0; i < STATS_PER / 4; ++i) {
@@ -70,23 +78,45 @@ __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(const float* __res
       v[i] = at < n ? __ldcs(x + at) : -CUDART_INF_F;
     }
   }
+  float top = -CUDART_INF_F;
+  int arg = 0x7fffffff;
 #pragma unroll
-  for (int i = 0; i < STATS_PER; ++i)   // a thread's indices rise
-    if (v[i] > top) top = v[i], arg = v0 + (VECTORS ? (tid + STATS_THREADS * (i / 4)) * 4 + i % 4 : tid + STATS_THREADS * i);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float t = __shfl_xor_sync(0xffffffffu, top, o);
-    const int i = __shfl_xor_sync(0xffffffffu, arg, o);
-    keep_first(top, arg, t, i);
+  for (int i = 0; i < STATS_PER; ++i) {
+    v[i] = number(v[i]);
+    if constexpr (ARGMAX) {   // a thread's indices rise
+      if (v[i] > top) top = v[i], arg = v0 + (VECTORS ? (tid + STATS_THREADS * (i / 4)) * 4 + i % 4 : tid + STATS_THREADS * i);
+    } else {
+      top = fmaxf(top, v[i]);
+    }
   }
-  if (lane == 0) s_top[warp] = top, s_arg[warp] = arg;
+  if constexpr (ARGMAX) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float t = __shfl_xor_sync(0xffffffffu, top, o);
+      const int i = __shfl_xor_sync(0xffffffffu, arg, o);
+      keep_first(top, arg, t, i);
+    }
+    if (lane == 0) s_arg[warp] = arg;
+  } else {
+    top = jb::warp_max(top);
+  }
+  if (lane == 0) s_top[warp] = top;
   __syncthreads();
-  top = s_top[0], arg = s_arg[0];
+  top = s_top[0];
+  if constexpr (ARGMAX) arg = s_arg[0];
 #pragma unroll
-  for (int w = 1; w < STATS_THREADS / 32; ++w) keep_first(top, arg, s_top[w], s_arg[w]);
+  for (int w = 1; w < STATS_THREADS / 32; ++w) {
+    if constexpr (ARGMAX) keep_first(top, arg, s_top[w], s_arg[w]);
+    else top = fmaxf(top, s_top[w]);
+  }
   float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (fabsf(top) < CUDART_INF_F) {
 #pragma unroll
-  for (int i = 0; i < STATS_PER; ++i) part[i & 3] += weight(v[i], top, heat_log2);
+    for (int i = 0; i < STATS_PER; ++i) part[i & 3] += finite_weight(v[i], top, heat_log2);
+  } else {
+#pragma unroll
+    for (int i = 0; i < STATS_PER; ++i) part[i & 3] += weight(v[i], top, heat_log2);
+  }
   const float sum = jb::warp_sum((part[0] + part[1]) + (part[2] + part[3]));
   if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
@@ -139,7 +169,7 @@ struct Draw {
   int d, V;
   Form form;
   __device__ __forceinline__ float mass(int v, float xv, float qv) const {
-    const float w = weight(xv, top, heat_log2);
+    const float w = weight(number(xv), top, heat_log2);
     if (form == KEPT) return w;
     return form == LOOKED_UP ? (v == d ? 0.0f : w) : fmaxf(fmaf(w, inv_sum, -qv), 0.0f);
   }
@@ -164,6 +194,32 @@ struct Draw {
   }
 };
 
+// The first of n masses (in order) whose running sum from `before` on passes `target`, or the last with any mass should rounding let
+// none pass; -1: none has any.  start: the running sum in front of it; all: the sum of all.  By a whole warp, the same in every lane.
+__device__ __forceinline__ int first_past(const float* mass, int n, float before, float target, float& start, float& all) {
+  const int lane = threadIdx.x & 31;
+  int pick = -1, last = -1;
+  float run = before, last_start = before;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    const float m = i0 + lane < n ? mass[i0 + lane] : 0.0f, up = run + warp_inclusive(m);
+    const unsigned some = __ballot_sync(0xffffffffu, m > 0.0f), past = __ballot_sync(0xffffffffu, m > 0.0f && target < up);
+    const float in_front = __shfl_up_sync(0xffffffffu, up, 1);
+    const float mine = lane == 0 ? run : in_front;
+    if (pick < 0 && past) {
+      pick = i0 + __ffs(past) - 1;
+      start = __shfl_sync(0xffffffffu, mine, __ffs(past) - 1);
+    }
+    if (some) {
+      last = i0 + 31 - __clz(some);
+      last_start = __shfl_sync(0xffffffffu, mine, 31 - __clz(some));
+    }
+    run = __shfl_sync(0xffffffffu, up, 31);
+  }
+  all = run;
+  if (pick < 0) pick = last, start = last_start;
+  return pick;
+}
+
 // A chunk's masses, 16 a thread (warp w has PIECE neighbouring tokens, in four runs of four a lane), and the warp's sum: the sums
 // of runs in order.  run_end[k]: the warp's sum up to and with run k.
 __device__ __forceinline__ float warp_masses(const Draw& draw, int chunk, bool vectors, float (&w)[16], float (&run_end)[4]) {
@@ -179,7 +235,7 @@ __device__ __forceinline__ float warp_masses(const Draw& draw, int chunk, bool v
   return run;
 }
 
-__global__ void __launch_bounds__(THREADS) decide_kernel(const float* __restrict__ logits, const Chunk* __restrict__ stats,
+__global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restrict__ logits, const Chunk* __restrict__ stats,
                                                          const int* __restrict__ tokens, const int* __restrict__ q_start,
                                                          const int* __restrict__ kv_len, const float* __restrict__ u_accept,
                                                          const float* __restrict__ u_draw, const float* __restrict__ probs,
@@ -192,6 +248,7 @@ __global__ void __launch_bounds__(THREADS) decide_kernel(const float* __restrict
   float* row_sum = row_top + width;                         // [width]
   int* row_arg = reinterpret_cast<int*>(row_sum + width);   // [width]
   int* row_yes = row_arg + width;                           // [width] the draft behind the row is accepted
+  float* row_x = reinterpret_cast<float*>(row_yes + width); // [width] its logit
   __shared__ float s_warp[WARPS];
   __shared__ int s_token;
   const int size = cluster_size(), rank = cluster_rank(), b = blockIdx.x / size;
@@ -225,18 +282,20 @@ __global__ void __launch_bounds__(THREADS) decide_kernel(const float* __restrict
     if (arg == 0x7fffffff) arg = 0;
     if (lane == 0) {
       bool yes = false;
+      float x = 0.0f;
       if (r + 1 < rows) {
         const int t = lo + r + 1, d = tokens[t];
         if (d >= 0 && d < V) {
+          x = logits[(size_t)(lo + r) * V + d];
           if (heat > 0.0f) {
             const float q = probs ? probs[(size_t)t * V + d] : 1.0f;
-            yes = u_accept[t] * q * sum < weight(logits[(size_t)(lo + r) * V + d], top, heat_log2);
+            yes = u_accept[t] * q * sum < weight(x, top, heat_log2);
           } else {
             yes = d == arg;
           }
         }
       }
-      row_top[r] = top, row_sum[r] = sum, row_arg[r] = arg, row_yes[r] = yes;
+      row_top[r] = top, row_sum[r] = sum, row_arg[r] = arg, row_yes[r] = yes, row_x[r] = x;
     }
   }
   if (tid == 0) s_token = -1;
@@ -258,22 +317,22 @@ __global__ void __launch_bounds__(THREADS) decide_kernel(const float* __restrict
       const float mine = warp_masses(draw, i, vectors, w, run_end);
       if (lane == 0) s_warp[warp] = mine;
       __syncthreads();
-      float all = 0.0f;
-#pragma unroll
-      for (int v = 0; v < WARPS; ++v) all += s_warp[v];
+      float start, all;
+      first_past(s_warp, WARPS, 0.0f, 0.0f, start, all);
       __syncthreads();
       return all;
     };
     // the chunks' masses, known to every block
     if (draw.form == REFUSED) {
-      cluster_sync();   // every block is there to be written to
+      if (size > 1) cluster_sync();   // every block is there to be written to
       for (int i = c_begin; i < c_end; ++i) {
         const float all = chunk_mass(i);
-        for (int r = tid; r < size; r += THREADS) store_remote(in_block(chunk_sum + i, r), all);
+        if (size == 1 && tid == 0) chunk_sum[i] = all;
+        if (size > 1 && tid < size) store_remote(in_block(chunk_sum + i, tid), all);
       }
-      cluster_sync();
+      if (size > 1) cluster_sync();
     }
-    float total = 0.0f;
+    float total = 0.0f, before = 0.0f;
     for (int form = 0; form < 2; ++form) {
       if (form == 1 || draw.form != REFUSED) {
         const float again = d_chunk >= 0 && draw.form == LOOKED_UP ? chunk_mass(d_chunk) : 0.0f;
@@ -281,24 +340,14 @@ __global__ void __launch_bounds__(THREADS) decide_kernel(const float* __restrict
           chunk_sum[i] = i == d_chunk && draw.form == LOOKED_UP ? again : c[i].sum * weight(c[i].top, draw.top, heat_log2);
       }
       __syncthreads();
-      total = 0.0f;
-      for (int i = 0; i < chunks; ++i) total += chunk_sum[i];
+      first_past(chunk_sum, chunks, 0.0f, 0.0f, before, total);
       if (total > 0.0f || draw.form == KEPT) break;
       draw.form = KEPT;   // nothing is left: from the row itself
       __syncthreads();
     }
-    // the chunk where the drawn number falls (the last one with any mass, should rounding let none pass)
+    // the chunk where the drawn number falls
     const float target = u_draw[b] * total;
-    float before = 0.0f, run = 0.0f;
-    int pick = -1;
-    for (int i = 0; i < chunks; ++i) {
-      const float m = chunk_sum[i];
-      if (m > 0.0f) {
-        pick = i, before = run;
-        if (target < run + m) break;
-      }
-      run += m;
-    }
+    const int pick = first_past(chunk_sum, chunks, 0.0f, target, before, total);
     if (pick >= 0) {
       writer = 0;
       while (!(pick < (int)((long long)(writer + 1) * chunks / size))) ++writer;
@@ -307,17 +356,8 @@ __global__ void __launch_bounds__(THREADS) decide_kernel(const float* __restrict
       const float mine = warp_masses(draw, pick, vectors, w, run_end);
       if (lane == 0) s_warp[warp] = mine;
       __syncthreads();
-      // the first warp whose running sum passes the target, or the last one with any mass
-      int owner = -1;
-      float start = before, at = before;
-      for (int v = 0; v < WARPS; ++v) {
-        const float m = s_warp[v];
-        if (m > 0.0f) {
-          owner = v, start = at;
-          if (target < at + m) break;
-        }
-        at += m;
-      }
+      float start, all;
+      const int owner = first_past(s_warp, WARPS, before, target, start, all);
       if (warp == owner) {
         int hit = 0x7fffffff, last = -1;
 #pragma unroll
@@ -348,7 +388,7 @@ __global__ void __launch_bounds__(THREADS) decide_kernel(const float* __restrict
       float p = 0.0f;
       if (k <= accepted) {
         v = k < accepted ? tokens[lo + k + 1] : token;
-        const float x = logits[(size_t)(lo + k) * V + v], gap = x == row_top[k] ? 0.0f : x - row_top[k];
+        const float x = k < accepted ? row_x[k] : logits[(size_t)(lo + k) * V + v], gap = x == row_top[k] ? 0.0f : x - row_top[k];
         p = row_sum[k] > 0.0f ? gap * (heat > 0.0f ? 1.0f / heat : 1.0f) - logf(row_sum[k]) : -CUDART_INF_F;
       }
       my[k] = v, lp[k] = p;
@@ -366,18 +406,23 @@ JB_EXPORT int jb_verify_drafts(const float* logits, const int* tokens, const int
   if (B <= 0) return 0;
   JB_REFUSE(V <= 0 || width <= 0 || T < 0, "verify_drafts: %d rows of %d logits, %d tokens a request", T, V, width);
   const int chunks = (V + CHUNK - 1) / CHUNK;
-  const size_t smem = ((size_t)chunks + 4 * (size_t)width) * sizeof(float);
+  const size_t smem = ((size_t)chunks + 5 * (size_t)width) * sizeof(float);
   JB_REFUSE(smem > 48 * 1024, "verify_drafts: %d tokens a request over a vocabulary of %d", width, V);
   JB_REFUSE((long long)T * chunks > 0x7fffffffll || (long long)B * MAX_CLUSTER > 0x7fffffffll, "verify_drafts: %d rows of %d logits", T, V);
-  const float heat_log2 = heat > 0.0f ? LOG2E / heat : LOG2E;
+  const float heat_log2 = heat > 0.0f ? fminf(LOG2E / heat, 1e30f) : LOG2E;   // (finite: 0 times it is 0)
   const bool vectors = V % 4 == 0 && (((uintptr_t)logits | (uintptr_t)probs) & 15) == 0;
   cudaError_t e = cudaSuccess;
   if (T > 0) {
     jb::Launch cfg(dim3(T * chunks), dim3(STATS_THREADS), 0, stream);
-    e = cudaLaunchKernelEx(&cfg.c, vectors ? stats_kernel<true> : stats_kernel<false>, logits, (Chunk*)stats, V, chunks, heat_log2);
+    e = cudaLaunchKernelEx(&cfg.c, heat > 0.0f ? (vectors ? stats_kernel<true, false> : stats_kernel<false, false>)
+                                              : (vectors ? stats_kernel<true, true> : stats_kernel<false, true>), logits, (Chunk*)stats, V, chunks, heat_log2);
     if (e != cudaSuccess) return (int)e;
   }
-  const int size = chunks < MAX_CLUSTER ? chunks : MAX_CLUSTER;
+  // Blocks a request: as many as run at once (two a multiprocessor).  A block more takes its share of a row's chunks, but makes all of the
+  // request's decisions too: 256 requests by eight blocks each took 94 us, where one wave of single blocks has no such repetition.
+  int size = 2 * 148 / B;
+  size = size < 1 ? 1 : size > MAX_CLUSTER ? MAX_CLUSTER : size;
+  if (size > chunks) size = chunks;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = size, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;

@@ -32,9 +32,13 @@ def dtype_code(dtype: torch.dtype) -> int:
 _scope_stream = [None]
 
 
+# (`torch.cuda.current_stream()` makes a stream object of what is one number: several microseconds a launch)
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
 def _stream() -> int:
     s = _scope_stream[0]
-    return s if s is not None else torch.cuda.current_stream().cuda_stream
+    return s if s is not None else _raw_stream(_current_device())
 
 
 @contextlib.contextmanager
@@ -88,7 +92,7 @@ _SIGNATURES = {
     "jb_latent_heads": "piiiiiipppiiiipfpppip", "jb_latent_queries": "piiiiiiippppiiipfppip", "jb_latent_values": "pppippiipiiiiiip",
     "jb_latent_down": "piipfpiippiiippppplip",
     "jb_step_tables": "ppppppppppppppppppiiiiiiiip", "jb_attention_prefix_f32": "pppppppipiipppiiiiiifiiiiip",
-    "jb_attention_prefix_bf16": "pppppppipiipppiiiiiiifiiiipp",
+    "jb_attention_prefix_bf16": "pppppppipiipppiiiiiiifiiiiiipp",
     "jb_verify_drafts": "ppppppppppppiiiifp",
     "jb_gather_rows": "ppiipppiiip", "jb_latent_attention": "ppppppppiiiiiiifiipp", "jb_attention_tc_matrix": "ppppppiiiiiiiifpipp",
 }
@@ -144,6 +148,15 @@ def _need(t: torch.Tensor, name: str, dtype=None, shape=None) -> None:
         raise KernelError(f"{name}: expected {dtype}, got {t.dtype}")
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise KernelError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _need_all(what: str, dtype, tensors, shapes, names) -> None:
+    """`_need` of many tensors of one dtype: what is right passes in a glance at each, what is not goes there for its message.
+    (A call with a dozen tensors would otherwise spend longer on its checks than on its launch.)"""
+    for t, shape in zip(tensors, shapes):
+        if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous():
+            for t, shape, name in zip(tensors, shapes, names):
+                _need(t, f"{what} {name}", dtype, shape)
 
 
 _launches = [0]
@@ -2424,22 +2437,23 @@ def step_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, rows: torch.Ten
     zero the cache rows of tokens without a page are -1, and the step must not run.  Outputs are tensors of their own, not inputs."""
     B, (B0, W0), (_, W) = lengths.shape[0], old_table.shape, table.shape
     T, N, P = positions.shape[0], old_free.shape[0], prefix_pages.shape[0]
-    for t, name, shape in ((lengths, "lengths", (B,)), (new_tokens, "new tokens", (B,)), (rows, "rows", (B,)), (old_table, "table", (B0, W0)),
-                           (old_held, "held pages", (B0,)), (prefix_pages, "prefix pages", (P,)), (old_free, "free pages", (N,)),
-                           (old_n_free, "number of free pages", (1,)), (q_start, "q_start", (B + 1,)), (kv_len, "kv_len", (B,)),
-                           (positions, "positions", (T,)), (token_seq, "token sequences", (T,)), (dest_rows, "cache rows", (T,)),
-                           (table, "new table", (B, W)), (held, "new held pages", (B,)), (free_pages, "new free pages", (N,)),
-                           (n_free, "new number of free pages", (1,)), (missing, "missing pages", (1,))):
-        _need(t, "step_tables " + name, torch.int32, shape)
+    one, b = (1,), (B,)
+    tensors = (lengths, new_tokens, rows, old_table, old_held, prefix_pages, old_free, old_n_free, q_start, kv_len, positions, token_seq,
+               dest_rows, table, held, free_pages, n_free, missing)
+    if _checks[0]:
+        _need_all("step_tables", torch.int32, tensors,
+                  (b, b, b, (B0, W0), (B0,), (P,), (N,), one, (B + 1,), b, (T,), (T,), (T,), (B, W), b, (N,), one, one), _STEP_TABLES_NAMES)
     if W < W0 or P > W:
         raise KernelError(f"step_tables: a table of {W} pages a row cannot take over rows of {W0} behind {P} shared pages")
-    if any(a.numel() and a.data_ptr() == b.data_ptr() for a, b in ((table, old_table), (free_pages, old_free), (held, old_held),
-                                                                   (n_free, old_n_free), (kv_len, lengths))):
-        raise KernelError("step_tables: the new table and lists cannot lie where the old ones do")
-    _check(_lib("step_tables").jb_step_tables(
-        _ptr(lengths), _ptr(new_tokens), _ptr(rows), _ptr(old_table), _ptr(old_held), _ptr(prefix_pages), _ptr(old_free),
-        _ptr(old_n_free), _ptr(q_start), _ptr(kv_len), _ptr(positions), _ptr(token_seq), _ptr(dest_rows), _ptr(table), _ptr(held),
-        _ptr(free_pages), _ptr(n_free), _ptr(missing), B, B0, T, W0, W, P, N, int(page_size), _stream()), "step_tables")
+    at = [t.data_ptr() for t in tensors]
+    if len(set(at)) < 18 and any(t.numel() and t.data_ptr() in at[:8] for t in tensors[8:]):
+        raise KernelError("step_tables: what is made cannot lie where the old tables and lists do")
+    _check(_lib("step_tables").jb_step_tables(*at, B, B0, T, W0, W, P, N, int(page_size), _stream()), "step_tables")
+
+
+_STEP_TABLES_NAMES = ("lengths", "new tokens", "rows", "table", "held pages", "prefix pages", "free pages", "number of free pages",
+                      "q_start", "kv_len", "positions", "token sequences", "cache rows", "new table", "new held pages", "new free pages",
+                      "new number of free pages", "missing pages")
 
 
 def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, prefix_pages: torch.Tensor,
@@ -2451,18 +2465,14 @@ def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     is handed over as table[:, shared:]).  q and out: [T, nh hd], float32 or bfloat16 as the cache; positions [T].  Rows behind
     q_start[n_seqs] are left as they are.  max_q_len, max_kv_len: at least the longest of the step."""
     T, n_seqs, prefix_len = q.shape[0], kv_len.shape[0], int(prefix_len)
-    _need(q, "attention q", None, (T, nh * hd))
-    _need(out, "attention out", q.dtype, (T, nh * hd))
-    _need(prefix_pages, "prefix pages", torch.int32)
-    _need(q_start, "q_start", torch.int32, (n_seqs + 1,))
-    _need(kv_len, "kv_len", torch.int32, (n_seqs,))
-    _need(positions, "positions", torch.int32, (T,))
+    if dtype_code(q.dtype) == BF16 and hd % 8:
+        raise KernelError(f"attention_prefix: bfloat16 heads of {hd} numbers (they must be multiples of 8)")
     if _checks[0]:
-        for t, name in ((k_cache, "k cache"), (v_cache, "v cache")):
-            _need(t, name, q.dtype)
-            if t.dim() != 4 or tuple(t.shape[1:]) != (nkv, page_size, hd) or t.shape[0] != k_cache.shape[0]:
-                raise KernelError(f"attention_prefix: cache shape {tuple(t.shape)} is not [pages, {nkv}, {page_size}, {hd}]")
-        if not block_table.is_cuda or block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n_seqs:
+        width, cache = (T, nh * hd), (k_cache.shape[0], nkv, page_size, hd)
+        _need_all("attention_prefix", q.dtype, (q, out, k_cache, v_cache), (width, width, cache, cache), ("q", "out", "k cache", "v cache"))
+        _need_all("attention_prefix", torch.int32, (prefix_pages, q_start, kv_len, positions),
+                  (prefix_pages.shape, (n_seqs + 1,), (n_seqs,), (T,)), ("prefix pages", "q_start", "kv_len", "positions"))
+        if block_table.dtype is not torch.int32 or not block_table.is_cuda or block_table.dim() != 2 or block_table.shape[0] != n_seqs:
             raise KernelError(f"attention_prefix: the block table must be int32 [{n_seqs}, pages] on the device")
         if block_table.shape[1] > 1 and block_table.stride(1) != 1:
             raise KernelError("attention_prefix: a row of the block table must lie in one piece")
@@ -2475,7 +2485,8 @@ def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if q.dtype == torch.float32:
         rows, own_rows, splits, own_slots = attention_prefix_plan_f32(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv)
     else:
-        tiles, splits, own_slots = attention_prefix_plan(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv, hd)
+        tiles, ctas, splits, own_tiles, own_slots = attention_prefix_plan(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh,
+                                                                          nkv, hd)
     slots = splits + own_slots if own_slots > 1 else splits
     part_o = part_ml = None
     if slots:
@@ -2487,27 +2498,46 @@ def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
             float(scale), int(max_q_len), rows, own_rows, splits, own_slots, _stream()), "attention_prefix",
             kernels=1 if hd % 4 else (splits > 0) + 1 + (own_slots > 1))
         return
-    kernels = 1 if splits == 0 and prefix_len else (splits > 0) + 1 + (own_slots > 1)
-    _check(_lib("prefix_attention").jb_attention_prefix_bf16(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(part_o), _ptr(part_ml), *step,
-                                        k_cache.shape[0], n_seqs, nh, nkv, hd, page_size, float(scale), int(max_q_len), tiles, splits,
-                                        own_slots, _ptr(kernel_status(q.device)), _stream()), "attention_prefix", kernels=kernels)
+    _check(_lib("prefix_attention").jb_attention_prefix_bf16(
+        _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(part_o), _ptr(part_ml), *step, k_cache.shape[0], n_seqs, nh, nkv, hd,
+        page_size, float(scale), int(max_q_len), tiles, ctas, splits, own_tiles, own_slots, _ptr(kernel_status(q.device)), _stream()),
+        "attention_prefix", kernels=(ctas > 0) + 1 + (own_slots > 1))
+
+
+_PREFIX_MOST_RANGES = 64       # partial results over the prefix that a row's join takes
 
 
 @functools.lru_cache(maxsize=4096)
 def attention_prefix_plan(T: int, n_seqs: int, max_q_len: int, prefix_len: int, max_own: int, nh: int, nkv: int, hd: int):
-    """(row tiles a CTA, ranges of the prefix, ranges of a sequence's own keys) of a bfloat16 `attention_prefix`; no ranges of the
-    prefix: tiles of one sequence each walk all their keys."""
+    """How a bfloat16 `attention_prefix` runs: (row tiles a block, blocks that walk the prefix for all rows together (0: nobody does), the
+    most ranges in which a row's prefix keys come, whether own keys go by tiles, ranges of a sequence's own keys)."""
     group, sms = nh // nkv, SM_COUNT_TARGET // 2
-    rows = 128 // group                                    # tokens of a tile
-    pages = max(1, (max_own + 63) // 64)
-    tiles = 2 if hd <= 128 and min(T, max_q_len if T * group >= 64 * n_seqs else T) > rows else 1
-    if prefix_len and T * group >= 64 * n_seqs:
-        return tiles, 0, 1
-    blocks = (prefix_len + 127) // 128
-    splits = min(blocks, max(1, sms // (nkv * ((T + tiles * rows - 1) // (tiles * rows))))) if prefix_len else 0
-    ctas = n_seqs * nkv * ((max_q_len * group + 15) // 16)
-    own_slots = min(32, max(1, pages // 2), max(1, 2 * sms // max(1, ctas)))
-    return tiles, splits, own_slots
+    rows, keys = 128 // group, 64 if hd > 128 else 128     # tokens of a tile, keys of a block
+    own_tiles = max_q_len * group > 64
+    tiles = 2 if hd <= 128 and T > rows else 1
+    step = rows * tiles
+    blocks = (prefix_len + keys - 1) // keys
+    if own_tiles and prefix_len:
+        # tiles of one sequence over everything, or all rows together over the prefix and a join: waves of blocks of keys, and the
+        # partial results' way out and back
+        block_us = 2.2 if tiles == 2 else 1.5
+        own_blocks = (max_own + keys - 1) // keys
+        waves = -(-nkv * (T // step + (n_seqs + 1) // 2) // sms)
+        whole = waves * (blocks + own_blocks) * block_us
+        apart = -(-(-(-T // step) * nkv * blocks) // sms) * block_us + waves * own_blocks * block_us + 8 + T * nh * hd * 8 / 4e6
+        if whole <= apart:
+            return tiles, 0, 0, 1, 1
+    ctas = ranges = 0
+    if prefix_len:
+        total = -(-T // step) * nkv * blocks
+        per = max(-(-total // sms), -(-blocks // (_PREFIX_MOST_RANGES - 2)))
+        ctas = -(-total // per)
+        share, longer = divmod(total, ctas)
+        ranges = blocks // share if longer == 0 and blocks % share == 0 else (blocks + share - 2) // share + 1
+    if own_tiles:
+        return tiles, ctas, ranges, 1, 1
+    own_ctas = n_seqs * nkv * ((max_q_len * group + 15) // 16)
+    return tiles, ctas, ranges, 0, min(32, max(1, (max_own + 127) // 128), max(1, 2 * sms // max(1, own_ctas)))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2517,7 +2547,7 @@ def attention_prefix_plan_f32(T: int, n_seqs: int, max_q_len: int, prefix_len: i
     group, sms = nh // nkv, SM_COUNT_TARGET // 2
     rows, own_rows = (16 if n * group <= 32 else 64 for n in (T, max_q_len))
     pages = (prefix_len + 63) // 64
-    splits = min(pages, max(1, sms // (nkv * ((T * group + rows - 1) // rows)))) if prefix_len else 0
+    splits = min(64, pages, max(1, sms // (nkv * ((T * group + rows - 1) // rows)))) if prefix_len else 0
     ctas = n_seqs * nkv * ((max_q_len * group + own_rows - 1) // own_rows)
     return rows, own_rows, splits, min(32, max(1, (max_own + 127) // 128), max(1, 2 * sms // max(1, ctas)))
 
@@ -2538,18 +2568,14 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Ten
     the refused drafts.  A sequence without rows gets -1 and keeps kv_len.  Drafts past `width` - 1 are refused."""
     T, V = logits.shape
     B, width = accepted.shape[0], out_tokens.shape[1]
-    _need(logits, "verify logits", torch.float32)
-    _need(tokens, "verify tokens", torch.int32, (T,))
-    _need(q_start, "q_start", torch.int32, (B + 1,))
-    _need(kv_len, "kv_len", torch.int32, (B,))
-    _need(accepted, "accepted drafts", torch.int32)
-    _need(out_tokens, "verified tokens", torch.int32, (B, width))
-    _need(logprobs, "log-probabilities", torch.float32, (B, width))
-    _need(kept, "kept tokens", torch.int32, (B,))
-    _need(u_accept, "numbers of the tests", torch.float32, (T,))
-    _need(u_draw, "numbers of the draws", torch.float32, (B,))
-    if draft_probs is not None:
-        _need(draft_probs, "draft probabilities", torch.float32, (T, V))
+    if _checks[0]:
+        b, t, wide = (B,), (T,), (B, width)
+        _need_all("verify_drafts", torch.int32, (tokens, q_start, kv_len, accepted, out_tokens, kept), (t, (B + 1,), b, b, wide, b),
+                  ("tokens", "q_start", "kv_len", "accepted drafts", "verified tokens", "kept tokens"))
+        _need_all("verify_drafts", torch.float32, (logits, logprobs, u_accept, u_draw), ((T, V), wide, t, b),
+                  ("logits", "log-probabilities", "numbers of the tests", "numbers of the draws"))
+        if draft_probs is not None:
+            _need(draft_probs, "verify_drafts draft probabilities", torch.float32, (T, V))
     if not 0.0 <= temperature < float("inf"):
         raise KernelError(f"verify_drafts: temperature {temperature}")
     stats = workspace.get("verify_stats", (T * ((V + 8191) // 8192) * 3,), torch.float32)
