@@ -5,8 +5,8 @@
 // A softmax over a union of key sets joins from the sets' (maximum m, sum l, weighted values O):
 //   m = max m_i,  l = sum 2^(m_i - m) l_i,  O = sum 2^(m_i - m) O_i   (scores in units of log2).
 // So the prefix is attended once for all: the rows of ALL sequences' tokens make tiles of 128 for the tensor cores, which walk
-// the prefix's keys in ranges (`prefix_tc_kernel<SHARED>`), and each sequence's own pages are walked (`own_kernel`, or tiles again
-// where a sequence brings many tokens, `<OWN>`) and joined with the float32 partial results.  Steps whose sequences bring many tokens fill tiles by themselves: there a tile walks the prefix and then its own
+// the prefix's keys in ranges (`prefix_tc_kernel<SHARED>`), and each sequence's own pages are walked
+// (`own_kernel`; tiles again where a sequence brings many tokens, `<OWN>`); what they leave is float32 and is joined.  Steps whose sequences bring many tokens fill tiles by themselves: there a tile walks the prefix and then its own
 // pages and nothing is joined (`prefix_tc_kernel<WHOLE>`).
 #include <cuda.h>
 
@@ -28,6 +28,22 @@ namespace {
 // ---------------------------------------------------------------------------
 constexpr int BM = 128;
 constexpr float RESCALE_LOG2 = 8.0f;
+
+// Bounded wait: false (and *status = code) if the phase did not complete in 4e9 cycles, about two seconds.  The clock is read
+// once in 64 tries, and it is the multiprocessor's own: the time in nanoseconds takes as long to read as a block's products.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* status, int code) {
+  if (jb::mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (jb::mbar_try(bar, parity)) return true;
+    if (clock64() - t0 > 4000000000ll) {
+      atomicCAS(status, 0, code);
+      return false;
+    }
+  }
+}
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
   asm volatile(
@@ -91,22 +107,26 @@ __device__ __forceinline__ float row_max(const uint32_t* sr) {
   }
   return max3(m[0], m[1], fmaxf(m[2], m[3]));
 }
+__device__ __forceinline__ jb::Pair add2(jb::Pair a, jb::Pair b) {
+  jb::Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 // p[c] = 2^(s[c] scale + neg_ref) for N scores in sr; bfloat16 pairs over the first N / 2 words; returns their float32 sum.
+// (Three of eight by a polynomial instead of the special-function unit changed nothing for one tile a block, and spilled with two.)
 template <int N>
 __device__ __forceinline__ float exp_pack_sum(uint32_t* sr, float scale_log2, float neg_ref) {
-  const jb::Pair s2 = jb::pair(scale_log2, scale_log2), n2 = jb::pair(neg_ref, neg_ref), one = jb::pair(1.0f, 1.0f);
+  const jb::Pair s2 = jb::pair(scale_log2, scale_log2), n2 = jb::pair(neg_ref, neg_ref);
   jb::Pair acc[4] = {0ull, 0ull, 0ull, 0ull};   // the bit pattern of (0.0f, 0.0f)
 #pragma unroll
   for (int c = 0; c < N / 2; ++c) {
     const jb::Pair x = jb::fma2(jb::pair(__uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1])), s2, n2);
     const float p0 = fast_exp2(jb::lo(x)), p1 = fast_exp2(jb::hi(x));
-    acc[c & 3] = jb::fma2(jb::pair(p0, p1), one, acc[c & 3]);
+    acc[c & 3] = add2(acc[c & 3], jb::pair(p0, p1));
     sr[c] = pack_bf16(p0, p1);
   }
-  float sum = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) sum += jb::lo(acc[e]) + jb::hi(acc[e]);
-  return sum;
+  const jb::Pair all = add2(add2(acc[0], acc[1]), add2(acc[2], acc[3]));
+  return jb::lo(all) + jb::hi(all);
 }
 
 template <int HDC, int NT, int KB>
@@ -117,9 +137,23 @@ struct Tc {
   static constexpr int SWAP = NT * 2 * BM;                     // floats: what the two halves of a row tell each other
   static constexpr int SMEM = NT * Q_BYTES + 4 * KV_BYTES + SWAP * 4 + NT * 4 * 4 + BARS * 8 + 16;
   static constexpr int THREADS = 64 + NT * 256;
+  // (one tile of up to 128 numbers a row: 96 registers a thread, as 576 threads have, so that a block of own_kernel finds registers
+  // beside this one; rows of up to 64 leave enough anyway)
+  static constexpr int BOUND = HDC == 128 ? 576 : THREADS;
   static constexpr int COLS = 2 * KB + NT * HDC <= 256 ? 256 : 512;
   static_assert(2 * KB + NT * HDC <= 512 && SMEM <= 232448, "tensor and shared memory of one CTA");
 };
+// One lane of a warp whose lanes are all here.  (Work given to lane 0 by its number is not known to the compiler to be one thread's:
+// every operand of a product then went through a vector register, and issuing products took twice as long as computing them.)
+__device__ __forceinline__ bool elected() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0u;
+}
 // A barrier of two warps that tells both whether any of their threads says `yes`.
 __device__ __forceinline__ bool pair_any(int barrier, bool yes) {
   uint32_t any;
@@ -152,7 +186,7 @@ __device__ __forceinline__ void load8(const float* p, float* r) {
 }
 
 template <int HDC, int NT, int KB, Form FORM>
-__global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
+__global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
     const bf16* __restrict__ q, const bf16* __restrict__ k_cache, const bf16* __restrict__ v_cache, bf16* __restrict__ out,
     float* __restrict__ part_o, float2* __restrict__ part_ml, const Step s, const Slots parts, int* __restrict__ status) {
@@ -171,7 +205,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
   auto o_full = [&](int w) { return bar0 + 104 + 24 * w; };   // a block's product has landed in O
   auto o_done = [&](int w) { return bar0 + 112 + 24 * w; };   // ... the last block's of a segment
   auto o_free = [&](int w) { return bar0 + 120 + 24 * w; };   // O has been read and may be begun anew
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     jb::mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
@@ -180,12 +214,12 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
       jb::mbar_init(v_full + 8 * i, 1);
       jb::mbar_init(v_empty + 8 * i, 1);
       jb::mbar_init(s_full(i), 1);
-      jb::mbar_init(p_full(i), 256);
+      jb::mbar_init(p_full(i), 8);      // an arrival a warp: one a thread would be 256 operations on one word
     }
     for (int w = 0; w < NT; ++w) {
       jb::mbar_init(o_full(w), 1);
       jb::mbar_init(o_done(w), 1);
-      jb::mbar_init(o_free(w), 256);
+      jb::mbar_init(o_free(w), 8);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -194,7 +228,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
   jb::tc_fence_before();
   __syncthreads();
   jb::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   if (FORM != OWN || parts.most == 0) jb::pdl_wait();
   // (after the wait: a kernel that starts early may read what the launch before this one wrote)
   jb::pdl_launch_dependents();
@@ -207,7 +241,8 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
     int slot;
   };
   int seq = 0, seq_start = 0, seq_pos = 0;        // SHARED: not used
-  const int flat_begin = FORM == SHARED ? range_start(parts, blockIdx.x) : 0, flat_end = FORM == SHARED ? range_start(parts, blockIdx.x + 1) : 1;
+  const int flat_begin = FORM == SHARED ? blockIdx.x * parts.per : 0;
+  const int flat_end = FORM == SHARED ? min(flat_begin + parts.per, (s.T + parts.tile_tokens - 1) / parts.tile_tokens * s.nkv * parts.blocks) : 1;
   if constexpr (FORM != SHARED) seq = blockIdx.z, seq_start = s.q_start[seq], seq_pos = s.kv_len[seq] - (s.q_start[seq + 1] - seq_start);
   // the segment that begins at place `at` of the list; steps `at` on to the next
   auto segment = [&](int& at) {
@@ -218,7 +253,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
       g.nb = g.n_shared = min(parts.blocks - g.block0, flat_end - at);
       g.kvh = item % s.nkv, g.tok0 = item / s.nkv * NT * tpt;
       g.n_tok = min(NT * tpt, total_tokens - g.tok0);
-      g.slot = blockIdx.x - (g.block0 == 0 ? blockIdx.x : range_of(parts, item * parts.blocks));
+      g.slot = blockIdx.x - item * parts.blocks / parts.per;
       at += g.nb;
     } else {
       const int q_len = s.q_start[seq + 1] - seq_start, first = (gridDim.y - 1 - blockIdx.y) * NT * tpt;
@@ -233,7 +268,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
   const int nslab = (s.hd + 63) / 64;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elected()) {
       const int last_shared = max((s.prefix_len - 1) / PAGE, 0);
       bool ok = true;
       int it = 0;                                             // blocks since the kernel's begin
@@ -241,7 +276,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
         const Segment g = segment(at);
         if (g.nb == 0) break;
         // every product with the queries before these is done when the last block's keys are free
-        if (it > 0) ok = jb::mbar_wait(k_empty + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, status, 41);
+        if (it > 0) ok = mbar_wait(k_empty + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, status, 41);
         if (!ok) break;
         jb::mbar_expect_tx(q_full, NT * nslab * tpt * G * 128);   // a box holds tpt tokens x G heads
         for (int w = 0; w < NT; ++w)
@@ -258,13 +293,13 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
             else page = s.table[(size_t)seq * s.ld_table + min((j - g.n_shared) * (KB / PAGE) + half, last_own)];
             row0[half] = (max(page, 0) * s.nkv + g.kvh) * PAGE;
           }
-          if (it >= 2 && !(ok = jb::mbar_wait(k_empty + 8 * st, ((it >> 1) - 1) & 1, status, 41))) break;
+          if (it >= 2 && !(ok = mbar_wait(k_empty + 8 * st, ((it >> 1) - 1) & 1, status, 41))) break;
           jb::mbar_expect_tx(k_full + 8 * st, nslab * KB * 128);
 #pragma unroll
           for (int half = 0; half < KB / PAGE; ++half)
             for (int h = 0; h < nslab; ++h)
               jb::tma_load_2d(k_s + st * C::KV_BYTES + h * KB * 128 + half * PAGE * 128, &map_k, k_full + 8 * st, h * 64, row0[half]);
-          if (it >= 2 && !(ok = jb::mbar_wait(v_empty + 8 * st, ((it >> 1) - 1) & 1, status, 41))) break;
+          if (it >= 2 && !(ok = mbar_wait(v_empty + 8 * st, ((it >> 1) - 1) & 1, status, 41))) break;
           jb::mbar_expect_tx(v_full + 8 * st, nslab * KB * 128);
 #pragma unroll
           for (int half = 0; half < KB / PAGE; ++half)
@@ -274,12 +309,12 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elected()) {
       const uint32_t idesc_s = jb::instr_desc_bf16(KB);
       const uint32_t idesc_o = jb::instr_desc_bf16((s.hd + 15) & ~15) | (1u << 16);   // values: MN-major
       auto issue_s = [&](int w, int it) -> bool {
         const int st = it & 1, b = NT == 2 ? w : it & 1;
-        if (!jb::mbar_wait(k_full + 8 * st, (it >> 1) & 1, status, 42)) return false;
+        if (!mbar_wait(k_full + 8 * st, (it >> 1) & 1, status, 42)) return false;
         jb::tc_fence_after();
 #pragma unroll
         for (int h = 0; h < C::SLABS; ++h) {
@@ -296,7 +331,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
       int at = flat_begin;
       Segment g = segment(at);
       int n = 0, j = 0, turn = 0;                              // blocks of the segment, the next one of them, segments so far
-      bool ok = g.nb > 0 && jb::mbar_wait(q_full, 0, status, 42);
+      bool ok = g.nb > 0 && mbar_wait(q_full, 0, status, 42);
       n = g.nb;
       for (int w = 0; w < NT && ok; ++w) ok = issue_s(w, 0);
       for (int it = 0; ok; ++it) {
@@ -304,14 +339,14 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
         const bool last = j == n - 1, more = !last || at < flat_end;
         bool fresh_q = last && more;                           // the next block is the first of another segment
         if (NT == 1 && more) {
-          if (fresh_q) ok = jb::mbar_wait(q_full, (turn + 1) & 1, status, 42);
+          if (fresh_q) ok = mbar_wait(q_full, (turn + 1) & 1, status, 42);
           ok = ok && issue_s(0, it + 1);
         }
         for (int w = 0; w < NT && ok; ++w) {
           const int b = NT == 2 ? w : it & 1;
-          ok = jb::mbar_wait(p_full(b), (NT == 2 ? it : it >> 1) & 1, status, 42);
-          if (ok && w == 0) ok = jb::mbar_wait(v_full + 8 * st, (it >> 1) & 1, status, 42);
-          if (ok && j == 0 && turn > 0) ok = jb::mbar_wait(o_free(w), (turn - 1) & 1, status, 42);
+          ok = mbar_wait(p_full(b), (NT == 2 ? it : it >> 1) & 1, status, 42);
+          if (ok && w == 0) ok = mbar_wait(v_full + 8 * st, (it >> 1) & 1, status, 42);
+          if (ok && j == 0 && turn > 0) ok = mbar_wait(o_free(w), (turn - 1) & 1, status, 42);
           if (!ok) break;
           jb::tc_fence_after();
 #pragma unroll
@@ -322,7 +357,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
           if (last) jb::umma_commit(o_done(w));
           if (w == NT - 1) jb::umma_commit(v_empty + 8 * st);
           if (NT == 2 && more) {
-            if (fresh_q) ok = jb::mbar_wait(q_full, (turn + 1) & 1, status, 42), fresh_q = false;
+            if (fresh_q) ok = mbar_wait(q_full, (turn + 1) & 1, status, 42), fresh_q = false;
             ok = ok && issue_s(w, it + 1);
           }
         }
@@ -368,7 +403,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
       for (int j = 0; j < g.nb; ++j, ++it) {
         const int b = NT == 2 ? w : it & 1;
         const uint32_t s_at = lane_addr + b * KB;
-        ok = __all_sync(0xffffffffu, ok && jb::mbar_wait(s_full(b), (NT == 2 ? it : it >> 1) & 1, status, 43));
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(s_full(b), (NT == 2 ? it : it >> 1) & 1, status, 43));
         jb::tc_fence_after();
         uint32_t sr[KH];
 #pragma unroll
@@ -392,7 +427,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
           if (!both) break;
           const float m_new = fmaxf(m_ref, mx);
           if (j > 0) {
-            ok = __all_sync(0xffffffffu, jb::mbar_wait(o_full(w), (it - 1) & 1, status, 43));
+            ok = __all_sync(0xffffffffu, mbar_wait(o_full(w), (it - 1) & 1, status, 43));
             if (!ok) continue;
             jb::tc_fence_after();
             const float corr = m_new == -CUDART_INF_F ? 1.0f : exp2f(m_ref - m_new);
@@ -416,10 +451,11 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
         for (int c0 = 0; c0 < KH / 2; c0 += 16) tmem_st16(s_at + half * (KH / 2) + c0, sr + c0);
         tmem_st_wait();
         jb::tc_fence_before();
-        jb::mbar_arrive(p_full(b));
+        __syncwarp();
+        if (lane == 0) jb::mbar_arrive(p_full(b));
       }
       if (!both) break;
-      if (ok && g.nb > 0) ok = __all_sync(0xffffffffu, jb::mbar_wait(o_done(w), turn & 1, status, 43));
+      if (ok && g.nb > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(w), turn & 1, status, 43));
       const float theirs = meet(l);   // the row's sum over both halves
       if (!both) break;
       l = half == 0 ? l + theirs : theirs + l;
@@ -440,7 +476,8 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
           if (valid && c0 + 8 < s.hd) store8(part_o + item * s.hd + c0 + 8, r + 8);
         }
         jb::tc_fence_before();
-        jb::mbar_arrive(o_free(w));
+        __syncwarp();
+        if (lane == 0) jb::mbar_arrive(o_free(w));
       } else {
         // the parts over the prefix weigh in (OWN); few, or the steps of many tokens that come here would not cut the prefix
         const int slots = FORM == OWN && valid ? slots_of(parts, s, token, g.kvh) : 0;
@@ -453,7 +490,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
           const float2 ml = part_ml[i * all + place];
           l = fmaf(exp2f(ml.x - ref), ml.y, l);
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = top == -CUDART_INF_F ? 0.0f : 1.0f / l;   // (a row that sees nothing)
         bool finite = true;
 #pragma unroll
         for (int c1 = 0; c1 < DH; c1 += 16) {
@@ -512,13 +549,14 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::THREADS, 1) prefix_tc_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// bfloat16: each sequence's own pages, by warp-level products.  A block has 16 (token, head) rows of one sequence and kv head and a
-// range of its pages; each of its two warps takes 32 keys of every page, which the copy engine brings (128-byte swizzle) into a
-// ring of its own: a warp asks for its next keys itself, and nothing waits for the other warp before the end.
-// The rows' queries stay in registers as the products take them.  32 keys a turn and one rescaling for all of them: with 16, by four
-// warps, a turn's 450 instructions moved half as many bytes (64 sequences of 30 to 700 keys, 8 kv heads of 128: 35 us).
+// bfloat16: each sequence's own pages, by warp-level products.  The work is a flat list: sequence after sequence, its (kv head, 16 rows)
+// pairs, their tiles of 32 keys.  Every warp has an even, consecutive share of it and works by itself: the copy engine brings its
+// tiles (128-byte swizzle) into a ring of its own, ahead across the ends of rows, the rows' queries stay in registers as the
+// products take them, and where a row's keys end (or the share does) the sums go out as a partial result.  How many a row has is
+// written beside (own_count).  A block of its own for every row waited for the longest row, and for what it had to fetch before
+// its first key: 256 sequences of 3 to 2,500 keys moved 2.8 TB/s.
 // ---------------------------------------------------------------------------
-constexpr int OWN_WARPS = 2, OWN_THREADS = 32 * OWN_WARPS, OWN_KEYS = PAGE / OWN_WARPS;
+constexpr int OWN_WARPS = 4, OWN_THREADS = 32 * OWN_WARPS, OWN_KEYS = 32, OWN_HALVES = PAGE / OWN_KEYS;
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -543,79 +581,137 @@ struct Own {
   static constexpr int SLABS = HDC / 64, SLAB = OWN_KEYS * 128;            // bytes of 64 numbers of a warp's keys
   static constexpr int TILE = SLABS * SLAB, STAGE = 2 * TILE;              // keys, values
   static constexpr int RING = OWN_WARPS * STAGES * STAGE;
-  static constexpr int RED_LD = HDC + 4;
-  static constexpr int RED = (OWN_WARPS * 16 * RED_LD + OWN_WARPS * 16 * 2 + 16 * 2 + 16 * 64) * 4;
-  static constexpr int SMEM = (RING > RED ? RING : RED) + OWN_WARPS * STAGES * 8;
+  static constexpr int SMEM = RING + OWN_WARPS * STAGES * 16;
 };
 
-// What is left to do with a row's sums over the warps: join them with the prefix's partial results and write the output
-// (own_slots == 1), or leave them as one more partial result.
+// A place of the list: the tile, and what its rows are.
+struct Cursor {
+  int seq, kvh, rb, tile;           // sequence; kv head, block of 16 rows; tile of the row's keys
+  int tiles, row_blocks, start, q_len;
+};
+// What sequence `seq` adds to the list: every row has a tile, also one that sees no key of its own.
+__device__ __forceinline__ void look_up(const Step& s, int seq, Cursor& c) {
+  c.seq = seq, c.start = s.q_start[seq], c.q_len = s.q_start[seq + 1] - c.start;
+  c.row_blocks = c.q_len > 0 ? (c.q_len * (s.nh / s.nkv) + 15) / 16 : 0;
+  c.tiles = min(max((s.kv_len[seq] - s.prefix_len + OWN_KEYS - 1) / OWN_KEYS, 1), max(s.width * OWN_HALVES, 1));
+}
+__device__ __forceinline__ int places(const Step& s, const Cursor& c) { return s.nkv * c.row_blocks * c.tiles; }
+__device__ __forceinline__ void step_on(const Step& s, Cursor& c) {
+  if (++c.tile < c.tiles) return;
+  c.tile = 0;
+  if (++c.rb < c.row_blocks) return;
+  c.rb = 0;
+  if (++c.kvh < s.nkv) return;
+  c.kvh = 0;
+  do {
+    if (c.seq + 1 >= s.n_seqs) return;   // (behind the list's end: nobody goes there)
+    look_up(s, c.seq + 1, c);
+  } while (c.row_blocks == 0);
+}
+
 template <int HDC, int STAGES>
 __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                          const bf16* __restrict__ q, const bf16* __restrict__ k_cache,
-                                                          const bf16* __restrict__ v_cache, bf16* __restrict__ out,
-                                                          float* __restrict__ part_o, float2* __restrict__ part_ml, const Step s,
-                                                          const Slots parts, int own_slots, int row_blocks, int* __restrict__ status) {
+                                                          const bf16* __restrict__ q, float* __restrict__ part_o, float2* __restrict__ part_ml,
+                                                          int* __restrict__ own_count, const Step s, int first_slot, int after_prefix,
+                                                          int fewest, int* __restrict__ status) {
   typedef Own<HDC, STAGES> C;
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint64_t* full = (uint64_t*)(smem + (C::RING > C::RED ? C::RING : C::RED));
-  const int G = s.nh / s.nkv, seq = blockIdx.x, kvh = blockIdx.y / row_blocks, rb = blockIdx.y % row_blocks, split = blockIdx.z;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = s.hd;
-  const uint32_t ring = jb::smem_u32(smem) + warp * STAGES * C::STAGE, bar = jb::smem_u32(full + warp * STAGES);
+  uint64_t* full = (uint64_t*)(smem + C::RING);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, hd = s.hd, G = s.nh / s.nkv;
+  const uint32_t ring = jb::smem_u32(smem) + warp * STAGES * C::STAGE, bar = jb::smem_u32(full + warp * STAGES * 2);
   if (lane == 0) {
-    for (int i = 0; i < STAGES; ++i) jb::mbar_init(bar + 8 * i, 1);
+    for (int i = 0; i < STAGES * 2; ++i) jb::mbar_init(bar + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
-  if (parts.most == 0) jb::pdl_wait();
+  if (!after_prefix) jb::pdl_wait();
   jb::pdl_launch_dependents();
-  const int start = s.q_start[seq], q_len = s.q_start[seq + 1] - start;
-  const int row0 = rb * 16, n_rows = min(16, q_len * G - row0);
-  const int first_pos = s.kv_len[seq] - q_len - s.prefix_len;   // among the own keys
-  // own keys that the block's last row sees; pages are cut evenly among the splits
-  const int see = n_rows > 0 ? first_pos + (row0 + n_rows - 1) / G + 1 : 0;
-  const int pages = min(see > 0 ? (see + PAGE - 1) / PAGE : 0, s.width);
-  const int p_begin = (int)((long long)split * pages / own_slots);
-  int p_end = (int)((long long)(split + 1) * pages / own_slots);
-  if (p_end > p_begin && (p_end - 1) * PAGE + warp * OWN_KEYS >= see) --p_end;   // this warp's part of the last page: nobody sees it
-  const int* table = s.table + (size_t)seq * s.ld_table;
+  // ---- the list's length, and this warp's share ----
+  Cursor c{};
+  const int chunk = (s.n_seqs + 31) / 32, seq0 = min(lane * chunk, s.n_seqs), seq1 = min(seq0 + chunk, s.n_seqs);
+  int mine = 0;
+#pragma unroll 4
+  for (int i = seq0; i < seq1; ++i) {
+    Cursor x;
+    look_up(s, i, x);
+    mine += places(s, x);
+  }
+  int up = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += t;
+  }
+  const int total = __shfl_sync(0xffffffffu, up, 31), worker = blockIdx.x * OWN_WARPS + warp;
+  const int per = max(fewest, (total + (int)gridDim.x * OWN_WARPS - 1) / ((int)gridDim.x * OWN_WARPS));
+  const int begin = min(worker * per, total), end = min(begin + per, total);
+  if (begin < end) {
+    const int owner = __ffs(__ballot_sync(0xffffffffu, begin < up)) - 1;
+    int before = __shfl_sync(0xffffffffu, up - mine, owner);
+    for (int i = owner * chunk;; ++i) {
+      look_up(s, i, c);
+      const int n = places(s, c);
+      if (begin < before + n) break;
+      before += n;
+    }
+    const int y = (begin - before) / c.tiles;
+    c.tile = (begin - before) - y * c.tiles, c.kvh = y / c.row_blocks, c.rb = y - c.kvh * c.row_blocks;
+  }
   const uint64_t policy = jb::read_once_policy();
   const int nslab = (hd + 63) / 64;
-  auto issue = [&](int p) {   // by one lane
-    const int st = (p - p_begin) % STAGES, row = (max(table[p], 0) * s.nkv + kvh) * PAGE + warp * OWN_KEYS;
-    const uint32_t at = ring + st * C::STAGE;
-    jb::mbar_expect_tx(bar + 8 * st, 2 * nslab * C::SLAB);
-    for (int h = 0; h < nslab; ++h) {
-      jb::tma_load_2d(at + h * C::SLAB, &map_k, bar + 8 * st, h * 64, row, policy);
-      jb::tma_load_2d(at + C::TILE + h * C::SLAB, &map_v, bar + 8 * st, h * 64, row, policy);
+  Cursor ahead = c;
+  int asked = begin;
+  // (a tile's page is looked up a turn before it is asked for, or every turn would wait for memory)
+  auto page_of = [&](const Cursor& x) { return s.width > 0 ? s.table[(size_t)x.seq * s.ld_table + x.tile / OWN_HALVES] : 0; };
+  int page = begin < end ? page_of(ahead) : 0;
+  // Keys and values of a tile have a barrier each: with one stage the next keys are on their way while this tile's softmax and the
+  // values' product run, the next values during the scores.
+  auto issue = [&](int what) {   // 0: the keys of the next tile that has not been asked for; 1: its values, and on to the one behind
+    const int st = (asked - begin) % STAGES;
+    if (elected()) {
+      const int row = (max(page, 0) * s.nkv + ahead.kvh) * PAGE + ahead.tile % OWN_HALVES * OWN_KEYS;
+      const uint32_t at = ring + st * C::STAGE + what * C::TILE, full_at = bar + 16 * st + 8 * what;
+      jb::mbar_expect_tx(full_at, nslab * C::SLAB);
+      for (int h = 0; h < nslab; ++h) jb::tma_load_2d(at + h * C::SLAB, what ? &map_v : &map_k, full_at, h * 64, row, policy);
+    }
+    __syncwarp();
+    if (what == 0) return;
+    ++asked;
+    if (asked < end) {
+      step_on(s, ahead);
+      page = page_of(ahead);
     }
   };
-  if (lane == 0)
-    for (int i = 0; i < STAGES; ++i)
-      if (p_begin + i < p_end) issue(p_begin + i);
+  for (int i = 0; i < STAGES; ++i)
+    if (asked < end) issue(0), issue(1);
   // the rows' queries as the A operand of the products: lane (g, c) has rows g and g + 8, numbers 2 c, 2 c + 1 and 8 behind of every 16
   uint32_t qa[HDC / 16][4];
-  float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.0f, 0.0f}, o[HDC / 8][4];
+  float m[2], l[2], o[HDC / 8][4];
   int see_row[2];
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int row = (lane >> 2) + 8 * r, rr = row0 + row;
-    const bool valid = row < n_rows && p_begin < p_end;
-    see_row[r] = valid ? first_pos + rr / G + 1 : 0;
-    const bf16* src = q + ((size_t)(start + (valid ? rr / G : 0)) * s.nh + kvh * G + rr % G) * hd + 2 * (lane & 3);
-#pragma unroll
-    for (int ks = 0; ks < HDC / 16; ++ks)
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-        qa[ks][r + 2 * half] = valid && ks * 16 + half * 8 < hd ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + half * 8) : 0u;
-  }
-#pragma unroll
-  for (int j = 0; j < HDC / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
   bool ok = true;
-  for (int p = p_begin; p < p_end; ++p) {
-    const int turn = p - p_begin, st = turn % STAGES;
-    ok = jb::mbar_wait(bar + 8 * st, (turn / STAGES) & 1, status, 53);
-    if (!ok) break;
+  for (int i = begin; i < end; ++i) {
+    if (i == begin || c.tile == 0) {
+      const int kvh = c.kvh, row0 = c.rb * 16, n_rows = min(16, c.q_len * G - row0);
+      const int first_pos = s.kv_len[c.seq] - c.q_len - s.prefix_len;   // among the own keys
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = (lane >> 2) + 8 * r, token = (row0 + row) / G, head = kvh * G + (row0 + row) % G;
+        const bool valid = row < n_rows;
+        see_row[r] = valid ? min(first_pos + token + 1, s.width * PAGE) : 0;
+        m[r] = -CUDART_INF_F, l[r] = 0.0f;
+        const bf16* src = q + ((size_t)(c.start + (valid ? token : 0)) * s.nh + head) * hd + 2 * (lane & 3);
+#pragma unroll
+        for (int ks = 0; ks < HDC / 16; ++ks)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            qa[ks][r + 2 * half] = valid && ks * 16 + half * 8 < hd ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + half * 8) : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < HDC / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+    }
+    const int turn = i - begin, st = turn % STAGES;
+    ok = mbar_wait(bar + 16 * st, (turn / STAGES) & 1, status, 53);
+    if (__any_sync(0xffffffffu, !ok)) break;
     const uint32_t k_t = ring + st * C::STAGE, v_t = k_t + C::TILE;
     float x[4][4];
 #pragma unroll
@@ -632,8 +728,10 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
         mma_bf16(x[j + 1], qa[ks], b[2], b[3]);
       }
     }
+    __syncwarp();   // the warp is done with the keys
+    if (asked < end) issue(0);
     float mx[2] = {-CUDART_INF_F, -CUDART_INF_F}, corr[2], ref[2];
-    const int key0 = p * PAGE + warp * OWN_KEYS + 2 * (lane & 3);
+    const int key0 = c.tile * OWN_KEYS + 2 * (lane & 3);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -660,6 +758,8 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
         x[j][e] = fast_exp2(x[j][e] - ref[e >> 1]);
         l[e >> 1] += x[j][e];
       }
+    ok = mbar_wait(bar + 16 * st + 8, (turn / STAGES) & 1, status, 53);
+    if (__any_sync(0xffffffffu, !ok)) break;
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       const uint32_t a[4] = {pack_bf16(x[2 * kk][0], x[2 * kk][1]), pack_bf16(x[2 * kk][2], x[2 * kk][3]),
@@ -674,34 +774,30 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
         mma_bf16(o[j + 1], a, b[2], b[3]);
       }
     }
-    __syncwarp();   // the warp is done with the stage
-    if (lane == 0 && p + STAGES < p_end) issue(p + STAGES);
-  }
-  // ---- the warps' results meet in shared memory ----
-  if (!__syncthreads_and(ok)) {   // (a wait ran out: the status word says so; nothing is in flight into the ring but what ran out)
-    jb::pdl_wait();
-    return;
-  }
-  float* red_o = reinterpret_cast<float*>(smem);
-  float* red_ml = red_o + OWN_WARPS * 16 * C::RED_LD;
+    __syncwarp();   // ... and with the values
+    if (asked < end) issue(1);
+    if (i + 1 == end || c.tile + 1 == c.tiles) {   // the row's keys end here, or the share does
+      const int place = i - c.tile, first = place / per, slot = worker - first;
+      const int kvh = c.kvh, row0 = c.rb * 16, n_rows = min(16, c.q_len * G - row0);
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    const int row = warp * 16 + (lane >> 2) + 8 * r;
-    if ((lane & 3) == 0) {
-      red_ml[2 * row] = m[r];
-      red_ml[2 * row + 1] = l[r];
+      for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        const int row = (lane >> 2) + 8 * r, token = c.start + (row0 + row) / G, head = kvh * G + (row0 + row) % G;
+        if (row >= n_rows) continue;
+        const size_t item = ((size_t)(first_slot + slot) * s.T + token) * s.nh + head;
+        if ((lane & 3) == 0) {
+          part_ml[item] = make_float2(m[r], l[r]);
+          if (slot == 0) own_count[token * s.nkv + kvh] = (place + c.tiles - 1) / per - first + 1;
+        }
+#pragma unroll
+        for (int j = 0; j < HDC / 8; ++j)
+          if (j * 8 < hd) *reinterpret_cast<float2*>(part_o + item * hd + j * 8 + 2 * (lane & 3)) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
+      }
     }
-#pragma unroll
-    for (int j = 0; j < HDC / 8; ++j)
-      *reinterpret_cast<float2*>(red_o + row * C::RED_LD + j * 8 + 2 * (lane & 3)) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
+    if (i + 1 < end) step_on(s, c);
   }
-  __syncthreads();
-  if (parts.most > 0) jb::pdl_wait();   // the prefix's partial results are there
-  finish_rows<bf16, OWN_WARPS, 16, OWN_THREADS>(q, k_cache, v_cache, out, part_o, part_ml, s, parts, red_o, red_ml, C::RED_LD,
-                                                red_ml + OWN_WARPS * 16 * 2 + 32, red_ml + OWN_WARPS * 16 * 2, max(n_rows, 0), row0, start, seq,
-                                                kvh, own_slots > 1 ? parts.most + split : -1);
+  if (after_prefix) jb::pdl_wait();   // (so that who waits for this launch has waited for the one before it)
 }
 
 // ---------------------------------------------------------------------------
@@ -744,7 +840,7 @@ cudaError_t tc_go(dim3 grid, cudaStream_t stream, const CUtensorMap* maps, const
   typedef Tc<HDC, NT, KB> C;
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(prefix_tc_kernel<HDC, NT, KB, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    cudaError_t e = set_up(prefix_tc_kernel<HDC, NT, KB, FORM>, C::SMEM);
     if (e != cudaSuccess) return e;
     configured = true;
   }
@@ -765,31 +861,33 @@ cudaError_t tc_pick(int nt, dim3 grid, cudaStream_t stream, const CUtensorMap* m
 }
 
 template <int HDC, int STAGES>
-cudaError_t own_go(dim3 grid, cudaStream_t stream, const CUtensorMap* maps, const bf16* q, const bf16* k, const bf16* v, bf16* out,
-                   float* part_o, float2* part_ml, const Step& s, const Slots& parts, int own_slots, int row_blocks, int* status) {
+cudaError_t own_go(int blocks, cudaStream_t stream, const CUtensorMap* maps, const bf16* q, float* part_o, float2* part_ml, int* own_count,
+                   const Step& s, int first_slot, int after_prefix, int fewest, int* status) {
   typedef Own<HDC, STAGES> C;
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(own_kernel<HDC, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    cudaError_t e = set_up(own_kernel<HDC, STAGES>, C::SMEM);
     if (e != cudaSuccess) return e;
     configured = true;
   }
-  jb::Launch cfg(grid, dim3(OWN_THREADS), C::SMEM, stream);
-  return cudaLaunchKernelEx(&cfg.c, own_kernel<HDC, STAGES>, maps[0], maps[1], q, k, v, out, part_o, part_ml, s, parts, own_slots, row_blocks,
-                            status);
+  jb::Launch cfg(dim3(blocks), dim3(OWN_THREADS), C::SMEM, stream);
+  return cudaLaunchKernelEx(&cfg.c, own_kernel<HDC, STAGES>, maps[0], maps[1], q, part_o, part_ml, own_count, s, first_slot, after_prefix,
+                            fewest, status);
 }
 
 }  // namespace
 
 // q, out [T, nh hd], caches [n_pages, nkv, 64, hd], all bfloat16.  tiles: row tiles of a block, 1 or 2 (one for heads of more than 128
 // numbers).  shared_ctas > 0: the prefix for all rows together by that many blocks, which cut a row's keys into at most `most`
-// ranges; the own keys by tiles (own_tiles), or in own_slots ranges a sequence; part_o [most (+ own_slots if > 1)][T][nh][hd] float32
-// and part_ml [..][T][nh][2] are scratch.  shared_ctas = 0: tiles of one sequence each walk all their keys.
+// ranges.  own_tiles: own keys by tiles of a sequence each (all keys, where nobody walks the prefix apart); else by the warps of
+// own_ctas blocks, which get no less than `fewest` tiles of 32 keys each, so that a row has at most own_most partial results.
+// Scratch: part_o [most (+ own_most without own_tiles)][T][nh][hd] float32, part_ml [..][T][nh][2], own_count int [T][nkv].
 JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const void* v_cache, void* out, float* part_o, float* part_ml,
-                                       const int* prefix_pages, int prefix_len, const int* block_table, int ld_table, int width,
-                                       const int* q_start, const int* kv_len, const int* positions, int T, int n_pages, int n_seqs,
-                                       int nh, int nkv, int hd, int page_size, float scale, int max_q_len, int tiles, int shared_ctas,
-                                       int most, int own_tiles, int own_slots, int* status, cudaStream_t stream) {
+                                       int* own_count, const int* prefix_pages, int prefix_len, const int* block_table, int ld_table,
+                                       int width, const int* q_start, const int* kv_len, const int* positions, int T, int n_pages,
+                                       int n_seqs, int nh, int nkv, int hd, int page_size, float scale, int max_q_len, int max_kv_len,
+                                       int tiles, int shared_ctas, int most, int own_tiles, int own_ctas, int fewest, int own_most,
+                                       int* status, cudaStream_t stream) {
   if (T <= 0 || n_seqs <= 0 || max_q_len <= 0) return 0;
   JB_REFUSE(page_size != PAGE, "attention_prefix: page size %d (need %d)", page_size, PAGE);
   JB_REFUSE(nkv <= 0 || nh % nkv != 0, "attention_prefix: %d heads are not a multiple of %d kv heads", nh, nkv);
@@ -799,16 +897,15 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
   JB_REFUSE(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15, "attention_prefix: operands must be 16-byte aligned");
   JB_REFUSE((long long)n_pages * nkv * PAGE > 0x7fffffffll, "attention_prefix: %d pages of %d heads are more rows than a tensor map counts",
             n_pages, nkv);
-  JB_REFUSE(n_seqs > 65535 || prefix_len < 0 || shared_ctas < 0 || own_slots < 1 || most < 0 || most > 64 || (shared_ctas > 0) != (most > 0) ||
-                (shared_ctas > 0 && prefix_len == 0) || (own_tiles && own_slots > 1),
-            "attention_prefix: a prefix of %d tokens in %d ranges by %d blocks, %d ranges of own keys of %d sequences", prefix_len, most,
-            shared_ctas, own_slots, n_seqs);
+  JB_REFUSE(n_seqs > 65535 || prefix_len < 0 || shared_ctas < 0 || most < 0 || most > 64 || (shared_ctas > 0) != (most > 0) ||
+                (shared_ctas > 0 && prefix_len == 0),
+            "attention_prefix: a prefix of %d tokens in %d ranges by %d blocks for %d sequences", prefix_len, most, shared_ctas, n_seqs);
   const Step s{prefix_pages, block_table, q_start, kv_len, positions, prefix_len, ld_table, width, T, n_seqs, nh, nkv, hd, scale * LOG2E};
   const bf16 *qb = (const bf16*)q, *kb = (const bf16*)k_cache, *vb = (const bf16*)v_cache;
   bf16* ob = (bf16*)out;
   float2* ml = (float2*)part_ml;
   const int nt = hd > 128 ? 1 : tiles, step = nt * (BM / G), keys = hd > 128 ? 64 : 128;
-  Slots parts{0, 0, 0, 1, 0, 1};
+  Slots parts{0, 0, 0, 1, 1};
   CUtensorMap maps[3];
   if ((shared_ctas > 0 || own_tiles) && !make_maps(&maps[0], &maps[1], &maps[2], q, k_cache, v_cache, s, n_pages, PAGE)) return JB_ERR_TENSORMAP;
   cudaError_t e = cudaSuccess;
@@ -816,11 +913,11 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
     const int blocks = (prefix_len + keys - 1) / keys;
     const long long total = (long long)((T + step - 1) / step) * nkv * blocks;
     JB_REFUSE(shared_ctas > total || total > 0x7fffffffll, "attention_prefix: %d blocks for %lld key blocks", shared_ctas, total);
-    parts = Slots{-1, most, blocks, (int)(total / shared_ctas), (int)(total % shared_ctas), step};
+    parts = Slots{-1, most, blocks, (int)((total + shared_ctas - 1) / shared_ctas), step};
     // a tile's blocks begin anywhere in a range, unless ranges divide them
-    const bool even = parts.longer == 0 && blocks % parts.per == 0;
-    JB_REFUSE((even ? blocks / parts.per : (blocks + parts.per - 2) / parts.per + 1) > most, "attention_prefix: %d blocks cut %d key blocks into more than %d ranges",
-              shared_ctas, blocks, most);
+    JB_REFUSE((total + parts.per - 1) / parts.per != shared_ctas ||
+                  (blocks % parts.per == 0 ? blocks / parts.per : (blocks + parts.per - 2) / parts.per + 1) > most,
+              "attention_prefix: %d blocks cut %d key blocks into more than %d ranges", shared_ctas, blocks, most);
     e = tc_pick<SHARED>(nt, dim3(shared_ctas), stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status);
     if (e != cudaSuccess) return (int)e;
   }
@@ -830,15 +927,15 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
                                  : tc_pick<WHOLE>(nt, grid, stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status));
   }
   JB_REFUSE(shared_ctas == 0 && prefix_len > 0, "attention_prefix: nothing walks the prefix");
-  const int row_blocks = (max_q_len * G + 15) / 16;
-  const dim3 grid(n_seqs, nkv * row_blocks, own_slots);
+  const int row_blocks = (max_q_len * G + 15) / 16, tiles_most = (max_kv_len - prefix_len + OWN_KEYS - 1) / OWN_KEYS;
+  JB_REFUSE(own_ctas < 1 || fewest < 1 || own_most > 64 || (tiles_most + fewest - 2) / fewest + 1 > own_most ||
+                (long long)n_seqs * nkv * row_blocks * (tiles_most < 1 ? 1 : tiles_most) > 0x3fffffffll,
+            "attention_prefix: %d blocks for %d tiles of own keys of %d sequences", own_ctas, tiles_most, n_seqs);
   if (!make_maps(nullptr, &maps[1], &maps[2], q, k_cache, v_cache, s, n_pages, OWN_KEYS)) return JB_ERR_TENSORMAP;
-  if (hd > 128) e = own_go<256, 2>(grid, stream, maps + 1, qb, kb, vb, ob, part_o, ml, s, parts, own_slots, row_blocks, status);
-  else if (hd > 64) e = own_go<128, 2>(grid, stream, maps + 1, qb, kb, vb, ob, part_o, ml, s, parts, own_slots, row_blocks, status);
-  else e = own_go<64, 3>(grid, stream, maps + 1, qb, kb, vb, ob, part_o, ml, s, parts, own_slots, row_blocks, status);
-  if (e == cudaSuccess && own_slots > 1) {
-    jb::Launch cfg(dim3((unsigned)(((long long)T * nh + 3) / 4)), dim3(128), 0, stream);
-    e = cudaLaunchKernelEx(&cfg.c, join_kernel<bf16>, qb, kb, vb, ob, (const float*)part_o, (const float2*)ml, s, parts, own_slots);
-  }
-  return (int)e;
+  const int behind = shared_ctas > 0;
+  if (hd > 128) e = own_go<256, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, fewest, status);
+  else if (hd > 64) e = own_go<128, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, fewest, status);
+  else e = own_go<64, 2>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, fewest, status);
+  if (e != cudaSuccess) return (int)e;
+  return (int)join_go<bf16>(stream, qb, kb, vb, ob, part_o, ml, own_count, s, parts, 0);
 }

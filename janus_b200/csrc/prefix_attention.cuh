@@ -85,48 +85,52 @@ __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<f
 
 // Where the partial results over the prefix lie: slot i of a row is part_o [i][token][head][hd], part_ml [i][token][head].  How many
 // slots a row has: `fixed`, or, where blocks cut the flat list of (tile of tile_tokens tokens, kv head) x `blocks` key blocks into
-// ranges (the first `longer` of per + 1 places, the others of `per`), the ranges that its tile is in.  Results over own keys, where
-// there are several, begin at slot `most`.
+// ranges of `per` places, the ranges that its tile is in.  Results over own keys begin at slot `most`.
 struct Slots {
-  int fixed, most, blocks, per, longer, tile_tokens;
+  int fixed, most, blocks, per, tile_tokens;
 };
-__device__ __forceinline__ int range_start(const Slots& p, int range) { return range * p.per + min(range, p.longer); }
-__device__ __forceinline__ int range_of(const Slots& p, int place) {
-  const int in_longer = p.longer * (p.per + 1);
-  return place < in_longer ? place / (p.per + 1) : p.longer + (place - in_longer) / p.per;
-}
 __device__ __forceinline__ int slots_of(const Slots& p, const Step& s, int token, int kvh) {
   if (p.fixed >= 0) return p.fixed;
   const int place = (token / p.tile_tokens * s.nkv + kvh) * p.blocks;
-  return range_of(p, place + p.blocks - 1) - range_of(p, place) + 1;
+  return (place + p.blocks - 1) / p.per - place / p.per + 1;
 }
 
-// One warp a (token, query head): all partial results joined in the order of their slots.
+// One warp a (token, query head): all partial results joined in the order of their slots, the prefix's first, then those over own
+// keys: own_count[token][kv head] of them, or own_slots where that is null.  All of a row's slots are asked for at once; joined by the
+// blocks that walk the own keys, one row after another, the wait for them took longer than the keys (48 sequences of up to 24 rows:
+// 24 of 34 us).
 template <typename E>
 __global__ void __launch_bounds__(128) join_kernel(const E* __restrict__ q, const E* __restrict__ k_cache,
                                                    const E* __restrict__ v_cache, E* __restrict__ out,
-                                                   const float* __restrict__ part_o, const float2* __restrict__ part_ml, const Step s,
-                                                   const Slots parts, int own_slots) {
-  jb::pdl_launch_dependents();
-  jb::pdl_wait();
+                                                   const float* __restrict__ part_o, const float2* __restrict__ part_ml,
+                                                   const int* __restrict__ own_count, const Step s, const Slots parts, int own_slots) {
   const int item = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int t = item / s.nh, h = item % s.nh;
-  if (t >= min(s.T, s.q_start[s.n_seqs])) return;
+  const int t = item / s.nh, h = item - t * s.nh, kvh = h / (s.nh / s.nkv);
   const size_t all = (size_t)s.T * s.nh;
-  const int shared = slots_of(parts, s, t, h / (s.nh / s.nkv)), slots = shared + own_slots;
+  const int shared = t < s.T ? slots_of(parts, s, t, kvh) : 0;
+  jb::pdl_wait();
+  jb::pdl_launch_dependents();
+  if (t >= s.T) return;
+  const int total = s.q_start[s.n_seqs], own = own_count ? own_count[t * s.nkv + kvh] : own_slots;
   auto place = [&](int i) { return (i < shared ? i : parts.most + i - shared) * all + item; };
-  float top = -CUDART_INF_F, sum = 0.0f;
-  for (int i = lane; i < slots; i += 32) top = fmaxf(top, part_ml[place(i)].x);
+  // (at most 64 prefix slots and 64 others; asked for before it is known how many there are)
+  float2 first = make_float2(-CUDART_INF_F, 0.0f);
+  if (lane < shared) first = part_ml[place(lane)];
+  if (t >= total) return;
+  const int slots = shared + own;
+  if (lane >= shared && lane < slots) first = part_ml[place(lane)];
+  float top = first.x, sum = 0.0f;
+  for (int i = lane + 32; i < slots; i += 32) top = fmaxf(top, part_ml[place(i)].x);
   top = jb::warp_max(top);
   const float ref = top == -CUDART_INF_F ? 0.0f : top;
   float4 acc[2];
   acc[0] = acc[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int i0 = 0; i0 < slots; i0 += 32) {
-    const float2 ml = i0 + lane < slots ? part_ml[place(i0 + lane)] : make_float2(-CUDART_INF_F, 0.0f);
+    const float2 ml = i0 == 0 ? first : i0 + lane < slots ? part_ml[place(i0 + lane)] : make_float2(-CUDART_INF_F, 0.0f);
     const float mine = exp2f(ml.x - ref);
     sum = fmaf(mine, ml.y, sum);
     const int n = min(32, slots - i0);
-#pragma unroll 4
+#pragma unroll 8
     for (int j = 0; j < n; ++j) {
       const float f = __shfl_sync(0xffffffffu, mine, j);
       const float* row = part_o + place(i0 + j) * s.hd;
@@ -154,86 +158,26 @@ __global__ void __launch_bounds__(128) join_kernel(const E* __restrict__ q, cons
   if (__any_sync(0xffffffffu, !finite)) one_row(q, k_cache, v_cache, out, s, sequence_of(s, t), t, h);
 }
 
-// The last step of a block that holds WARPS partial results of each of `n_rows` rows in shared memory (red_o [WARPS][ROWS][ld],
-// red_ml [WARPS][ROWS][2]): one more partial result in slot `put` of device memory (put >= 0), or joined with the prefix's and
-// written, and a row that is not finite is made once more by itself.  Row r of the block is (token0 + (row0 + r) / G, query head
-// kvh G + (row0 + r) % G).  `weights`: ROWS * parts.most floats of shared memory, `row_sums`: 2 ROWS floats.  All of a row's slots are
-// asked for at once: one after another their latencies took longer than the sequence's own keys (18 slots, 64 sequences: 35 us).
-template <typename E, int WARPS, int ROWS, int THREADS>
-__device__ __forceinline__ void finish_rows(const E* q, const E* k_cache, const E* v_cache, E* out, float* part_o, float2* part_ml,
-                                            const Step& s, const Slots& parts, const float* red_o, const float* red_ml, int ld,
-                                            float* weights, float* row_sums, int n_rows, int row0, int token0, int seq, int kvh, int put) {
-  const int G = s.nh / s.nkv, quads = s.hd / 4, lane = threadIdx.x & 31, most = put >= 0 ? 0 : parts.most;
-  const size_t all = (size_t)s.T * s.nh;
-  auto place_of = [&](int row) { return (size_t)(token0 + (row0 + row) / G) * s.nh + kvh * G + (row0 + row) % G; };
-  // a warp a row: its maximum, its sum, and what each slot weighs
-  for (int row = threadIdx.x >> 5; row < n_rows; row += THREADS / 32) {
-    const size_t place = place_of(row);
-    const int slots = most ? slots_of(parts, s, token0 + (row0 + row) / G, kvh) : 0;
-    float top = -CUDART_INF_F, sum = 0.0f;
-    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, red_ml[2 * (w * ROWS + row)]);
-    float2 ml[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {       // (at most 64 slots)
-      ml[e] = lane + 32 * e < slots ? part_ml[(lane + 32 * e) * all + place] : make_float2(-CUDART_INF_F, 0.0f);
-      top = fmaxf(top, ml[e].x);
-    }
-    top = jb::warp_max(top);
-    const float ref = top == -CUDART_INF_F ? 0.0f : top;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float f = exp2f(ml[e].x - ref);
-      if (lane + 32 * e < most) weights[row * most + lane + 32 * e] = lane + 32 * e < slots ? f : -1.0f;
-      sum = fmaf(f, ml[e].y, sum);
-    }
-    sum = jb::warp_sum(sum);
-    for (int w = 0; w < WARPS; ++w) sum = fmaf(exp2f(red_ml[2 * (w * ROWS + row)] - ref), red_ml[2 * (w * ROWS + row) + 1], sum);
-    if (lane == 0) row_sums[2 * row] = top, row_sums[2 * row + 1] = sum;
+// What a kernel needs set once: its shared memory's limit, and all of a multiprocessor's memory that can be shared as shared: kernels
+// of unlike splits between cache and shared memory do not run on one multiprocessor together, and these are launched to overlap.
+template <typename Kernel>
+cudaError_t set_up(Kernel* kernel, int smem) {
+  cudaError_t e = smem > 0 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) : cudaSuccess;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  return e;
+}
+
+template <typename E>
+cudaError_t join_go(cudaStream_t stream, const E* q, const E* k, const E* v, E* out, const float* part_o, const float2* part_ml,
+                    const int* own_count, const Step& s, const Slots& parts, int own_slots) {
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = set_up(join_kernel<E>, 0);
+    if (e != cudaSuccess) return e;
+    configured = true;
   }
-  __syncthreads();
-  unsigned wrong = 0u;   // rows this thread found not finite, a bit for every row of its own
-  int turn = 0;
-  for (int idx = threadIdx.x; idx < n_rows * quads; idx += THREADS, ++turn) {
-    const int row = idx / quads, d = idx % quads * 4;
-    const size_t place = place_of(row);
-    const float top = row_sums[2 * row], ref = top == -CUDART_INF_F ? 0.0f : top;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    auto add = [&](float f, const float4 v) {
-      acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
-    };
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const int at = w * ROWS + row;
-      add(exp2f(red_ml[2 * at] - ref), *reinterpret_cast<const float4*>(red_o + (size_t)at * ld + d));
-    }
-    if (put >= 0) {
-      const size_t item = put * all + place;
-      *reinterpret_cast<float4*>(part_o + item * s.hd + d) = acc;
-      if (d == 0) part_ml[item] = make_float2(top, row_sums[2 * row + 1]);
-      continue;
-    }
-    const float* from = part_o + place * s.hd + d;
-#pragma unroll 8
-    for (int i = 0; i < most; ++i) {
-      const float f = weights[row * most + i];
-      if (f >= 0.0f) add(f, *reinterpret_cast<const float4*>(from + i * all * s.hd));
-    }
-    const float sum = row_sums[2 * row + 1], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    acc.x *= inv, acc.y *= inv, acc.z *= inv, acc.w *= inv;
-    store4(out + place * s.hd + d, acc);
-    if (!(isfinite(acc.x) && isfinite(acc.y) && isfinite(acc.z) && isfinite(acc.w))) wrong |= 1u << min(turn, 31);
-  }
-  if (put >= 0) return;
-  // (rare: nothing more is done where every number is finite)
-  if (!__syncthreads_or(wrong != 0u)) return;
-  for (int row = threadIdx.x; row < n_rows; row += THREADS) row_sums[2 * row] = 0.0f;
-  __syncthreads();
-  turn = 0;
-  for (int idx = threadIdx.x; idx < n_rows * quads; idx += THREADS, ++turn)
-    if (wrong >> min(turn, 31) & 1u) row_sums[2 * (idx / quads)] = 1.0f;
-  __syncthreads();
-  for (int row = threadIdx.x >> 5; row < n_rows; row += THREADS / 32)
-    if (row_sums[2 * row] != 0.0f) one_row(q, k_cache, v_cache, out, s, seq, token0 + (row0 + row) / G, kvh * G + (row0 + row) % G);
+  jb::Launch cfg(dim3((unsigned)(((long long)s.T * s.nh + 3) / 4)), dim3(128), 0, stream);
+  return cudaLaunchKernelEx(&cfg.c, join_kernel<E>, q, k, v, out, part_o, part_ml, own_count, s, parts, own_slots);
 }
 
 }  // namespace

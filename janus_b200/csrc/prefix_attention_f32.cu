@@ -40,15 +40,17 @@ struct Tile {
 // OWN: the rows of one sequence over its own pages.  Else the rows of all sequences over a range of the prefix's pages.
 template <int HDC, int RR, bool OWN>
 __global__ void __launch_bounds__(THREADS) tile_f32_kernel(const float* __restrict__ q, const float* __restrict__ k_cache,
-                                                           const float* __restrict__ v_cache, float* __restrict__ out,
-                                                           float* __restrict__ part_o, float2* __restrict__ part_ml, const Step s,
+                                                           const float* __restrict__ v_cache, float* __restrict__ part_o,
+                                                           float2* __restrict__ part_ml, const Step s,
                                                            const Slots parts, int own_slots, int row_blocks) {
   typedef Tile<HDC, RR> C;
   extern __shared__ __align__(16) float smem[];
-  __shared__ float red_ml[2 * C::ROWS], row_sums[2 * C::ROWS];
+  __shared__ float red_ml[2 * C::ROWS];
   float *q_s = smem, *k_s = q_s + C::ROWS * C::LD, *v_s = k_s + PAGE * C::LD, *p_s = v_s + PAGE * C::LD;
   const int G = s.nh / s.nkv, hd = s.hd, tid = threadIdx.x, x = tid & 15, y = tid >> 4;
   const int prefix_slots = parts.fixed;
+  // (a launch over own keys right behind the one over the prefix finds everything in its place but that one's results, which it
+  // does not read)
   if (!OWN || prefix_slots == 0) jb::pdl_wait();
   jb::pdl_launch_dependents();
   int seq = 0, kvh, split = blockIdx.z, token0 = 0, row0, n_rows, first_pos = 0, p_begin, p_end;
@@ -189,31 +191,35 @@ __global__ void __launch_bounds__(THREADS) tile_f32_kernel(const float* __restri
     }
   }
   __syncthreads();
-  if (OWN && prefix_slots > 0) jb::pdl_wait();
-  // (the slots' weights take the place of the values)
-  finish_rows<float, 1, C::ROWS, THREADS>(q, k_cache, v_cache, out, part_o, part_ml, s, parts, red_o, red_ml, C::LD, v_s, row_sums,
-                                          max(n_rows, 0), row0, token0, seq, kvh, !OWN ? split : own_slots > 1 ? parts.most + split : -1);
+  const int slot = OWN ? parts.most + split : split;
+  for (int i = tid; i < n_rows * quads; i += THREADS) {
+    const int r = i / quads, d = i % quads * 4, rr = row0 + r;
+    const size_t item = (size_t)slot * s.T * s.nh + (size_t)(token0 + rr / G) * s.nh + kvh * G + rr % G;
+    *reinterpret_cast<float4*>(part_o + item * hd + d) = *reinterpret_cast<const float4*>(red_o + r * C::LD + d);
+    if (d == 0) part_ml[item] = make_float2(red_ml[2 * r], red_ml[2 * r + 1]);
+  }
+  if (OWN && prefix_slots > 0) jb::pdl_wait();   // (so that who waits for this launch has waited for the one before it)
 }
 
 template <int HDC, int RR, bool OWN>
-cudaError_t go(dim3 grid, cudaStream_t stream, const float* q, const float* k, const float* v, float* out, float* part_o, float2* part_ml,
+cudaError_t go(dim3 grid, cudaStream_t stream, const float* q, const float* k, const float* v, float* part_o, float2* part_ml,
                const Step& s, const Slots& parts, int own_slots, int row_blocks) {
   typedef Tile<HDC, RR> C;
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(tile_f32_kernel<HDC, RR, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    cudaError_t e = set_up(tile_f32_kernel<HDC, RR, OWN>, C::SMEM);
     if (e != cudaSuccess) return e;
     configured = true;
   }
   jb::Launch cfg(grid, dim3(THREADS), C::SMEM, stream);
-  return cudaLaunchKernelEx(&cfg.c, tile_f32_kernel<HDC, RR, OWN>, q, k, v, out, part_o, part_ml, s, parts, own_slots, row_blocks);
+  return cudaLaunchKernelEx(&cfg.c, tile_f32_kernel<HDC, RR, OWN>, q, k, v, part_o, part_ml, s, parts, own_slots, row_blocks);
 }
 template <bool OWN>
-cudaError_t pick(int hd, int rows, dim3 grid, cudaStream_t stream, const float* q, const float* k, const float* v, float* out,
-                 float* part_o, float2* part_ml, const Step& s, const Slots& parts, int own_slots, int row_blocks) {
+cudaError_t pick(int hd, int rows, dim3 grid, cudaStream_t stream, const float* q, const float* k, const float* v, float* part_o,
+                 float2* part_ml, const Step& s, const Slots& parts, int own_slots, int row_blocks) {
 #define JB_GO(HDC)                                                                                                              \
-  return rows == 16 ? go<HDC, 1, OWN>(grid, stream, q, k, v, out, part_o, part_ml, s, parts, own_slots, row_blocks)       \
-                    : go<HDC, 4, OWN>(grid, stream, q, k, v, out, part_o, part_ml, s, parts, own_slots, row_blocks)
+  return rows == 16 ? go<HDC, 1, OWN>(grid, stream, q, k, v, part_o, part_ml, s, parts, own_slots, row_blocks)       \
+                    : go<HDC, 4, OWN>(grid, stream, q, k, v, part_o, part_ml, s, parts, own_slots, row_blocks)
   if (hd > 128) JB_GO(256);
   if (hd > 64) JB_GO(128);
   JB_GO(64);
@@ -223,8 +229,8 @@ cudaError_t pick(int hd, int rows, dim3 grid, cudaStream_t stream, const float* 
 }  // namespace
 
 // q, out [T, nh hd], caches [n_pages, nkv, 64, hd], all float32.  splits: ranges of the prefix (0: there is none), own_slots: ranges
-// of a sequence's own keys; rows, own_rows: rows of a block over the prefix and over own keys, 16 or 64; part_o [splits (+ own_slots
-// if > 1)][T][nh][hd] and part_ml [..][T][nh][2] are scratch.  Head sizes that are no multiple of 4 use none of these.
+// of a sequence's own keys; rows, own_rows: rows of a block over the prefix and over own keys, 16 or 64; part_o [splits + own_slots]
+// [T][nh][hd] and part_ml [..][T][nh][2] are scratch.  Head sizes that are no multiple of 4 use none of these.
 JB_EXPORT int jb_attention_prefix_f32(const void* q, const void* k_cache, const void* v_cache, void* out, float* part_o, float* part_ml,
                                       const int* prefix_pages, int prefix_len, const int* block_table, int ld_table, int width,
                                       const int* q_start, const int* kv_len, const int* positions, int T, int n_seqs, int nh, int nkv,
@@ -242,21 +248,18 @@ JB_EXPORT int jb_attention_prefix_f32(const void* q, const void* k_cache, const 
     jb::Launch cfg(dim3((unsigned)(((long long)T * nh + 3) / 4)), dim3(128), 0, stream);
     return (int)cudaLaunchKernelEx(&cfg.c, rows_f32_kernel, qf, kf, vf, of, s);
   }
-  JB_REFUSE((rows != 16 && rows != 64) || (own_rows != 16 && own_rows != 64) || own_slots < 1 || splits < 0 || splits > 64 || (splits > 0 && prefix_len <= 0) ||
+  JB_REFUSE((rows != 16 && rows != 64) || (own_rows != 16 && own_rows != 64) || own_slots < 1 || own_slots > 64 || splits < 0 || splits > 64 || (splits > 0 && prefix_len <= 0) ||
                 (splits == 0 && prefix_len > 0),
             "attention_prefix: %d ranges of a prefix of %d tokens, blocks of %d and %d rows", splits, prefix_len, rows, own_rows);
   const int G = nh / nkv;
-  const Slots parts{splits, splits, 0, 1, 0, 1};
+  const Slots parts{splits, splits, 0, 1, 1};
   cudaError_t e = cudaSuccess;
   if (splits > 0)
-    e = pick<false>(hd, rows, dim3(nkv, (unsigned)(((long long)T * G + rows - 1) / rows), splits), stream, qf, kf, vf, of, part_o, ml, s, parts,
+    e = pick<false>(hd, rows, dim3(nkv, (unsigned)(((long long)T * G + rows - 1) / rows), splits), stream, qf, kf, vf, part_o, ml, s, parts,
                     own_slots, 0);
   if (e != cudaSuccess) return (int)e;
   const int row_blocks = (max_q_len * G + own_rows - 1) / own_rows;
-  e = pick<true>(hd, own_rows, dim3(n_seqs, nkv * row_blocks, own_slots), stream, qf, kf, vf, of, part_o, ml, s, parts, own_slots, row_blocks);
-  if (e == cudaSuccess && own_slots > 1) {
-    jb::Launch cfg(dim3((unsigned)(((long long)T * nh + 3) / 4)), dim3(128), 0, stream);
-    e = cudaLaunchKernelEx(&cfg.c, join_kernel<float>, qf, kf, vf, of, (const float*)part_o, (const float2*)ml, s, parts, own_slots);
-  }
+  e = pick<true>(hd, own_rows, dim3(n_seqs, nkv * row_blocks, own_slots), stream, qf, kf, vf, part_o, ml, s, parts, own_slots, row_blocks);
+  if (e == cudaSuccess) e = join_go<float>(stream, qf, kf, vf, of, part_o, ml, nullptr, s, parts, own_slots);
   return (int)e;
 }

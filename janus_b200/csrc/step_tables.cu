@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const Args a) {
   exclusive_sums([&](int r) { return (goes_on[r >> 5] >> (r & 31)) & 1u ? 0 : max(0, held_of(r) - a.P); }, a.B0, gives, warp_sum);
   __syncthreads();
   const int n_free = min(max(*a.n_free, 0), a.N);
-  const int have = min(n_free + gives[a.B0], a.N), took = min(takes[a.B], have), left = have - took;
+  const int have = n_free + gives[a.B0], took = min(takes[a.B], have), left = have - took;
   auto pool = [&](int i) {
     if (i < n_free) return a.free_pages[i];
     const int r = owner(gives, a.B0, i - n_free);
@@ -165,8 +165,8 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const Args a) {
     __syncthreads();
     if (threadIdx.x == 0) {
       for (int w = 1; w < WARPS; ++w) over += warp_sum[w];
-      *a.missing = takes[a.B] - took + over;
-      *a.n_free_out = left;
+      *a.missing = takes[a.B] - took + over + max(0, left - a.N);   // (what the new list has no place for is lost)
+      *a.n_free_out = min(left, a.N);
     }
   }
 }

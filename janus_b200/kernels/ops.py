@@ -92,7 +92,7 @@ _SIGNATURES = {
     "jb_latent_heads": "piiiiiipppiiiipfpppip", "jb_latent_queries": "piiiiiiippppiiipfppip", "jb_latent_values": "pppippiipiiiiiip",
     "jb_latent_down": "piipfpiippiiippppplip",
     "jb_step_tables": "ppppppppppppppppppiiiiiiiip", "jb_attention_prefix_f32": "pppppppipiipppiiiiiifiiiiip",
-    "jb_attention_prefix_bf16": "pppppppipiipppiiiiiiifiiiiiipp",
+    "jb_attention_prefix_bf16": "ppppppppipiipppiiiiiiifiiiiiiiiipp",
     "jb_verify_drafts": "ppppppppppppiiiifp",
     "jb_gather_rows": "ppiipppiiip", "jb_latent_attention": "ppppppppiiiiiiifiipp", "jb_attention_tc_matrix": "ppppppiiiiiiiifpipp",
 }
@@ -2429,12 +2429,12 @@ def step_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, rows: torch.Ten
     last step's `old_table` lists (its first old_held[row] entries), or begins (rows[b] = -1) with the shared `prefix_pages`, which
     stand in front of every row and are never given back.  Two requests do not go on with the same row.  A row nobody goes on
     with gives its own pages back: they follow the free pages old_free[:old_n_free], row after row.  Requests take the pages they
-    lack from the front of that list, in order; free_pages[:n_free] is what is left of it.
+    lack from the front of that list, in order; free_pages[:n_free] is what is left of it (a tensor with a place for every page).
 
     Made besides: q_start [B + 1] and kv_len [B]; table [B, width] (-1 where a row holds nothing), held [B]; for every place of
     the token arrays (as many as a step is laid out for) its position, request and cache row page * page_size + row, -1 in the
-    places behind the last token.  `missing`: pages that neither the free list nor the table's width could give; where it is not
-    zero the cache rows of tokens without a page are -1, and the step must not run.  Outputs are tensors of their own, not inputs."""
+    places behind the last token.  `missing`: pages that neither the free list nor the table's width could give, and free ones that
+    the new list has no place for; where it is not zero the cache rows of tokens without a page are -1, and the step must not run.  Outputs are tensors of their own, not inputs."""
     B, (B0, W0), (_, W) = lengths.shape[0], old_table.shape, table.shape
     T, N, P = positions.shape[0], old_free.shape[0], prefix_pages.shape[0]
     one, b = (1,), (B,)
@@ -2480,64 +2480,75 @@ def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise KernelError(f"attention_prefix: {prefix_pages.shape[0]} pages do not hold a prefix of {prefix_len} tokens")
     if max_q_len < 0 or block_table.shape[1] * page_size < max_kv_len - prefix_len:
         raise KernelError(f"attention_prefix: {block_table.shape[1]} pages a sequence do not hold {max_kv_len} tokens behind {prefix_len}")
-    step = (_ptr(prefix_pages), prefix_len, _ptr(block_table), block_table.stride(0), block_table.shape[1],
-            _ptr(q_start), _ptr(kv_len), _ptr(positions), T)
+    wide = block_table.shape[1]
+    step = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr())
+    rest = (prefix_pages.data_ptr(), prefix_len, block_table.data_ptr(), block_table.stride(0), wide, q_start.data_ptr(), kv_len.data_ptr(),
+            positions.data_ptr(), T)
     if q.dtype == torch.float32:
         rows, own_rows, splits, own_slots = attention_prefix_plan_f32(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv)
+        slots = splits + own_slots
     else:
-        tiles, ctas, splits, own_tiles, own_slots = attention_prefix_plan(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh,
-                                                                          nkv, hd)
-    slots = splits + own_slots if own_slots > 1 else splits
-    part_o = part_ml = None
+        tiles, ctas, splits, own_tiles, own_ctas, fewest, own_slots = attention_prefix_plan(
+            T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv, hd)
+        slots = splits + own_slots
+    part_o = part_ml = own_count = None
     if slots:
         part_o = workspace.get("prefix_part_o", (slots * T * nh * hd,), torch.float32)
         part_ml = workspace.get("prefix_part_ml", (slots * T * nh * 2,), torch.float32)
     if q.dtype == torch.float32:
         _check(_lib("prefix_attention_f32").jb_attention_prefix_f32(
-            _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(part_o), _ptr(part_ml), *step, n_seqs, nh, nkv, hd, page_size,
-            float(scale), int(max_q_len), rows, own_rows, splits, own_slots, _stream()), "attention_prefix",
-            kernels=1 if hd % 4 else (splits > 0) + 1 + (own_slots > 1))
+            *step, _ptr(part_o), _ptr(part_ml), *rest, n_seqs, nh, nkv, hd, page_size, float(scale), int(max_q_len), rows, own_rows,
+            splits, own_slots, _stream()), "attention_prefix", kernels=1 if hd % 4 else (splits > 0) + 2)
         return
+    if own_slots:
+        own_count = workspace.get("prefix_own_count", (T * nkv,), torch.int32).data_ptr()
     _check(_lib("prefix_attention").jb_attention_prefix_bf16(
-        _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(part_o), _ptr(part_ml), *step, k_cache.shape[0], n_seqs, nh, nkv, hd,
-        page_size, float(scale), int(max_q_len), tiles, ctas, splits, own_tiles, own_slots, _ptr(kernel_status(q.device)), _stream()),
-        "attention_prefix", kernels=(ctas > 0) + 1 + (own_slots > 1))
+        *step, _ptr(part_o), _ptr(part_ml), own_count, *rest, k_cache.shape[0], n_seqs, nh, nkv, hd, page_size, float(scale),
+        int(max_q_len), int(max_kv_len), tiles, ctas, splits, own_tiles, own_ctas, fewest, own_slots, _ptr(kernel_status(q.device)),
+        _stream()), "attention_prefix", kernels=(ctas > 0) + (1 if own_tiles else 2))
 
 
 _PREFIX_MOST_RANGES = 64       # partial results over the prefix that a row's join takes
 
 
+def _even_ranges(total: int, blocks: int, most_ctas: int):
+    """(blocks with equal ranges of `total` places, the last one with what is left; the most of their ranges that `blocks` consecutive
+    places from a multiple of it on are in)."""
+    per = max(-(-total // most_ctas), -(-blocks // (_PREFIX_MOST_RANGES - 2)))
+    return -(-total // per), blocks // per if blocks % per == 0 else (blocks + per - 2) // per + 1
+
+
 @functools.lru_cache(maxsize=4096)
 def attention_prefix_plan(T: int, n_seqs: int, max_q_len: int, prefix_len: int, max_own: int, nh: int, nkv: int, hd: int):
     """How a bfloat16 `attention_prefix` runs: (row tiles a block, blocks that walk the prefix for all rows together (0: nobody does), the
-    most ranges in which a row's prefix keys come, whether own keys go by tiles, ranges of a sequence's own keys)."""
+    most ranges in which a row's prefix keys come, whether own keys go by tiles, blocks that walk own keys otherwise, the fewest
+    tiles of 32 keys of a warp of theirs, the most partial results that makes a row)."""
     group, sms = nh // nkv, SM_COUNT_TARGET // 2
     rows, keys = 128 // group, 64 if hd > 128 else 128     # tokens of a tile, keys of a block
-    own_tiles = max_q_len * group > 64
-    tiles = 2 if hd <= 128 and T > rows else 1
-    step = rows * tiles
     blocks = (prefix_len + keys - 1) // keys
-    if own_tiles and prefix_len:
+    if max_q_len * group > 64:
+        tiles = 2 if hd <= 128 and max_q_len > rows else 1
+        step = rows * tiles
+        if not prefix_len:
+            return tiles, 0, 0, 1, 0, 0, 0
         # tiles of one sequence over everything, or all rows together over the prefix and a join: waves of blocks of keys, and the
         # partial results' way out and back
-        block_us = 2.2 if tiles == 2 else 1.5
+        block_us = 1.8 if tiles == 2 else 0.95
         own_blocks = (max_own + keys - 1) // keys
         waves = -(-nkv * (T // step + (n_seqs + 1) // 2) // sms)
         whole = waves * (blocks + own_blocks) * block_us
         apart = -(-(-(-T // step) * nkv * blocks) // sms) * block_us + waves * own_blocks * block_us + 8 + T * nh * hd * 8 / 4e6
         if whole <= apart:
-            return tiles, 0, 0, 1, 1
-    ctas = ranges = 0
-    if prefix_len:
-        total = -(-T // step) * nkv * blocks
-        per = max(-(-total // sms), -(-blocks // (_PREFIX_MOST_RANGES - 2)))
-        ctas = -(-total // per)
-        share, longer = divmod(total, ctas)
-        ranges = blocks // share if longer == 0 and blocks % share == 0 else (blocks + share - 2) // share + 1
-    if own_tiles:
-        return tiles, ctas, ranges, 1, 1
-    own_ctas = n_seqs * nkv * ((max_q_len * group + 15) // 16)
-    return tiles, ctas, ranges, 0, min(32, max(1, (max_own + 127) // 128), max(1, 2 * sms // max(1, own_ctas)))
+            return tiles, 0, 0, 1, 0, 0, 0
+        return tiles, *_even_ranges(-(-T // step) * nkv * blocks, blocks, sms), 1, 0, 0, 0
+    # one tile a block over the prefix: with two a block, its keys are fetched once for both, but the own keys' blocks then find no
+    # room beside it (64 single tokens behind 8,192: 31 us and 40)
+    ctas, ranges = _even_ranges(-(-T // rows) * nkv * blocks, blocks, sms) if prefix_len else (0, 0)
+    own_blocks = max(1, (max_own + 31) // 32)
+    places = n_seqs * nkv * ((max_q_len * group + 15) // 16) * own_blocks
+    fewest = max(1, min(4, places // (8 * sms)), -(-own_blocks // 30))
+    own_ctas = max(1, min((3 if hd <= 128 else 1) * sms, -(-places // (4 * fewest))))
+    return 1, ctas, ranges, 0, own_ctas, fewest, (own_blocks + fewest - 2) // fewest + 1
 
 
 @functools.lru_cache(maxsize=4096)
