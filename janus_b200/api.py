@@ -16,6 +16,7 @@ from . import log
 from .cache import PAGE_SIZE
 from .config import read_config_json, resolve_architecture
 from .engine.generate import plan_prompt_steps, run_generation
+from .engine.shared_prefix import LookupDrafter, SharedPrefixRunner
 from .engine.step import Engine, EngineOptions, StepEntry
 from .sampling import DeviceSampler, SamplerConfig
 from .weights import FolderCheckpoint, RandomCheckpoint, parse_dtype
@@ -157,13 +158,7 @@ class Model:
                 self._samplers.clear()
             sampler = DeviceSampler(sc, self.engine.model.vocab_size, cache.n_slots, seed, self.device)
             self._samplers[skey] = sampler
-        if ignore_eos:
-            stop = []
-        elif hasattr(self.config, "stop_token_ids"):
-            stop = list(self.config.stop_token_ids())
-        else:
-            stop = list(getattr(self.config, "eos_token_id", ()) or ())
-        stop += list(stop_token_ids or ())
+        stop = self._stop_tokens(ignore_eos, stop_token_ids)
         # room that is free now: a caller of alloc_slot/step may hold pages of its own
         free_tokens = min((g.pool.n_free for g in cache.groups), default=cache.n_pages) * PAGE_SIZE
         captures_before = self.engine.graph_captures
@@ -178,6 +173,35 @@ class Model:
                         f"tokens at {stats.prefill_tokens_per_s:.0f} tok/s; decode {stats.decode_tokens} tokens in "
                         f"{stats.decode_steps} steps at {stats.decode_tokens_per_s:.0f} tok/s; "
                         f"{stats.graph_captures} decode graphs recorded")
+        if return_reasons:
+            return outputs, reasons, stats
+        return outputs, stats
+
+
+    def _stop_tokens(self, ignore_eos: bool, more: Optional[Sequence[int]]) -> List[int]:
+        if ignore_eos:
+            stop = []
+        elif hasattr(self.config, "stop_token_ids"):
+            stop = list(self.config.stop_token_ids())
+        else:
+            stop = list(getattr(self.config, "eos_token_id", ()) or ())
+        return stop + list(more or ())
+
+    def generate_shared(self, prefix: Sequence[int], prompts: Sequence[Sequence[int]], max_tokens: int = 128, drafts: int = 4,
+                        temperature: float = 0.0, seed: int = 0, stop_token_ids: Optional[Sequence[int]] = None,
+                        ignore_eos: bool = False, batch_size: Optional[int] = None,
+                        callback: Optional[Callable[[int, int], bool]] = None, return_reasons: bool = False, drafter=LookupDrafter):
+        """As `generate` for the prompts prefix + prompt, with the prefix computed, cached and read once for all of them, and up to
+        `drafts` drafted tokens a request verified in each step (0: one token a step).  Drafts are looked up in a request's own
+        text, or come from `drafter(tokens)`, an object with `draft(most)` and `extend(tokens)`.  What is generated follows the
+        model's distribution at `temperature` (0: its argmax) whatever is drafted.  Returns (tokens, stats), stats with the drafted
+        and the accepted tokens; or (tokens, reasons, stats) with `return_reasons`.  Models whose mixers are all grouped-query
+        attention without a window."""
+        outputs, reasons, stats = SharedPrefixRunner(self.engine).generate(
+            prefix, prompts, max_tokens, self._stop_tokens(ignore_eos, stop_token_ids), drafts, temperature, seed, batch_size, callback,
+            drafter)
+        log.log("info", f"generate_shared: {stats.requests} requests behind {len(prefix)} shared tokens; {stats.decode_tokens} tokens in "
+                        f"{stats.decode_steps} steps, {stats.accepted} of {stats.drafted} drafts accepted")
         if return_reasons:
             return outputs, reasons, stats
         return outputs, stats

@@ -61,6 +61,10 @@ def main(argv=None) -> int:
     ap.add_argument("--random-weights", action="store_true",
                     help="the folder holds only config.json: run it with random weights")
     ap.add_argument("--seed-weights", type=int, default=0, help="seed of --random-weights")
+    ap.add_argument("--shared-prefix", default=None, metavar="IDS",
+                    help="token ids that stand in front of every prompt: computed and cached once for all of them")
+    ap.add_argument("--drafts", type=int, default=4,
+                    help="with --shared-prefix: tokens drafted from a request's own text and verified per step (default: 4)")
     ap.add_argument("--json", action="store_true", help="print one JSON object instead of text")
     ap.add_argument("--profile", metavar="FILE", default=None,
                     help="after generating, time the kernels of the first batch's prompt step and of one decode "
@@ -73,27 +77,37 @@ def main(argv=None) -> int:
             prompts += [parse_prompt(line) for line in f if line.strip()]
     if not prompts:
         ap.error("give at least one prompt")
+    prefix = parse_prompt(args.shared_prefix) if args.shared_prefix is not None else []
+    if prefix and (args.top_k or args.top_p < 1.0 or args.repetition_penalty != 1.0 or args.profile):
+        ap.error("--shared-prefix goes with --temperature only, not with --top-k, --top-p, --repetition-penalty or --profile")
 
     import janus_b200
     from janus_b200.engine.generate import tokens_held
 
     batch = max(1, min(args.batch_size, len(prompts)))
-    room = sorted((tokens_held(len(p), args.max_tokens, 64) for p in prompts), reverse=True)
+    more = len(prefix) + args.drafts + 1 if prefix else 0
+    room = sorted((tokens_held(len(p) + more, args.max_tokens, 64) for p in prompts), reverse=True)
+    slots = batch + (1 if prefix else 0)
     dtype = {"bf16": "bfloat16", "fp32": "float32"}.get(args.dtype, args.dtype)
     if args.random_weights:
         with open(os.path.join(args.model_dir, "config.json")) as f:
             config = json.load(f)
-        model = janus_b200.load_random(config, seed=args.seed_weights, dtype=dtype, max_tokens=sum(room[:batch]),
-                                       max_seq_len=args.context_size, max_slots=batch,
+        model = janus_b200.load_random(config, seed=args.seed_weights, dtype=dtype, max_tokens=sum(room[:batch]) + len(prefix),
+                                       max_seq_len=args.context_size, max_slots=slots,
                                        max_step_tokens=args.max_step_tokens or None)
     else:
-        model = janus_b200.load(args.model_dir, dtype=dtype, max_tokens=sum(room[:batch]),
-                                max_seq_len=args.context_size, max_slots=batch,
+        model = janus_b200.load(args.model_dir, dtype=dtype, max_tokens=sum(room[:batch]) + len(prefix),
+                                max_seq_len=args.context_size, max_slots=slots,
                                 max_step_tokens=args.max_step_tokens or None)
-    out, reasons, stats = model.generate(
-        prompts, max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
-        repetition_penalty=args.repetition_penalty, seed=args.seed, stop_token_ids=args.stop_id,
-        ignore_eos=args.ignore_eos, batch_size=batch, return_reasons=True)
+    if prefix:
+        out, reasons, stats = model.generate_shared(
+            prefix, prompts, max_tokens=args.max_tokens, drafts=args.drafts, temperature=args.temperature, seed=args.seed,
+            stop_token_ids=args.stop_id, ignore_eos=args.ignore_eos, batch_size=batch, return_reasons=True)
+    else:
+        out, reasons, stats = model.generate(
+            prompts, max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
+            repetition_penalty=args.repetition_penalty, seed=args.seed, stop_token_ids=args.stop_id,
+            ignore_eos=args.ignore_eos, batch_size=batch, return_reasons=True)
     if args.profile:
         with open(args.profile, "w") as f:
             json.dump(model.profile(prompts[:batch]), f, indent=1)

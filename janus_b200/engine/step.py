@@ -73,6 +73,9 @@ class StepContext:
         self.kv_total = 0
         self.feedback: torch.Tensor = None    # decode only: per slot the token sampled last (for ids < 0)
         self.groups: List[GroupStepView] = []
+        # sequences that begin with the same tokens: the pages (int32, on the device) that stand in front of every row of the
+        # block table and are read once for all of them; None: nothing is shared
+        self.prefix_pages: Optional[torch.Tensor] = None
         self.workspace: Workspace = None
         self.cache: SequenceCache = None
         self.dtype: torch.dtype = None

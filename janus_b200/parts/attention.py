@@ -160,6 +160,9 @@ class GQAttention(Mixer):
         ops.rope_cache_write(qkv, q, table, ctx.positions, group.dest_rows if writes_cache else None,
                              cache_view.k if writes_cache else None, cache_view.v if writes_cache else None,
                              self.nh, self.nkv, self.hd, group.page_size, write_kv=writes_cache)
+        if getattr(ctx, "prefix_pages", None) is not None:
+            self._attend_prompt(q, residual, ctx, cache_view)
+            return
         if self.dtype == torch.float32:
             ops.attention_f32(q, cache_view.k, cache_view.v, attn, group.block_table, ctx.token_seq,
                               ctx.positions, self.nh, self.nkv, self.hd, group.page_size, self.window,
@@ -174,9 +177,18 @@ class GQAttention(Mixer):
         self.o.forward_add(attn, residual)
 
     def _attend_prompt(self, q: torch.Tensor, residual: torch.Tensor, ctx, cache_view) -> None:
-        """bfloat16 attention of several new tokens per sequence over the cache, then the output projection."""
+        """bfloat16 attention of several new tokens per sequence over the cache (either dtype, where the sequences share a prefix),
+        then the output projection."""
         group = cache_view.group
         attn = ctx.workspace.get("attn_out", (q.shape[0], self.q_width), self.dtype)
+        shared = getattr(ctx, "prefix_pages", None)
+        if shared is not None:
+            n = shared.shape[0]
+            ops.attention_prefix(q, cache_view.k, cache_view.v, attn, shared, n * group.page_size, group.block_table[:, n:], ctx.q_start,
+                                 ctx.kv_len, ctx.positions, self.nh, self.nkv, self.hd, group.page_size, self.scale, ctx.workspace,
+                                 ctx.max_q_len, ctx.max_kv_len_bound)
+            self.o.forward_add(attn, residual)
+            return
         if ops.attention_tc_supported(self.nh, self.nkv, self.hd):
             # head sizes up to 128: flash attention on the tcgen05 tensor cores
             ops.attention_tc_prefill(q, cache_view.k, cache_view.v, attn, group.block_table, ctx.q_start,

@@ -540,3 +540,119 @@ def test_plans_cover_what_they_cut():
         owner = np.arange(items * blocks) // per
         for i in range(items):
             assert owner[(i + 1) * blocks - 1] - owner[i * blocks] + 1 <= ranges
+
+
+# -- the three together: generation behind a shared prefix -----------------------------------------------------------
+def test_lookup_drafts():
+    from janus_b200.engine.shared_prefix import LookupDrafter
+    d = LookupDrafter([1, 2, 3, 4, 1, 2])
+    assert d.draft(3) == [3, 4, 1] and d.draft(0) == []
+    d.extend([3])
+    assert d.draft(2) == [4, 1]
+    d.extend([9])
+    assert d.draft(2) == [] and LookupDrafter([5]).draft(4) == [] and LookupDrafter([]).draft(4) == []
+    assert LookupDrafter([7, 7, 7]).draft(4) == [7]
+
+
+class EveryToken:
+    """Drafts that are mostly wrong."""
+
+    def __init__(self, tokens):
+        self.n = len(tokens)
+
+    def extend(self, tokens):
+        self.n += len(tokens)
+
+    def draft(self, most):
+        return [(self.n * 7 + j) % 200 for j in range(most)]
+
+
+@gpu
+@pytest.mark.parametrize("which", ["A", "B"])
+@pytest.mark.parametrize("prefix_len", [0, 3, 64, 70])
+def test_generate_shared_equals_generate_in_float32(tmp_path, which, prefix_len):
+    """Greedy tokens behind a shared prefix are those of whole prompts, with drafts that are right, wrong or none, in batches."""
+    import janus_b200
+    from helpers import TINY, make_model_dir, random_tokens
+    cfg = TINY[which]
+    model = janus_b200.load(make_model_dir(cfg, str(tmp_path), seed=2, dtype="float32"), dtype="float32", max_tokens=2048)
+    prefix = random_tokens(prefix_len, cfg["vocab_size"], 5)
+    prompts = [random_tokens(n, cfg["vocab_size"], n) for n in (1, 9, 2, 17)]
+    prompts.append(prompts[1][:4] * 3)
+    n = 24
+    want, _ = model.generate([prefix + p for p in prompts], max_tokens=n, ignore_eos=True)
+    for drafts, batch, drafter in ((0, None, None), (4, None, None), (3, 2, None), (5, None, EveryToken)):
+        more = {} if drafter is None else dict(drafter=drafter)
+        got, reasons, stats = model.generate_shared(prefix, prompts, max_tokens=n, drafts=drafts, batch_size=batch, ignore_eos=True,
+                                                    return_reasons=True, **more)
+        assert got == want and reasons == ["length"] * len(prompts)
+        assert stats.drafted >= stats.accepted and (drafts == 0) == (stats.drafted == 0)
+        model.engine.cache.check()
+        assert model.engine.cache.groups[0].pool.n_held == 0
+    stop = want[1][5]
+    got, reasons, _ = model.generate_shared(prefix, prompts, max_tokens=n, stop_token_ids=[stop], return_reasons=True, ignore_eos=True)
+    for g, w, r in zip(got, want, reasons):
+        assert g == (w[: w.index(stop)] if stop in w else w) and r == ("stop" if stop in w else "length")
+
+
+@gpu
+def test_generate_shared_in_bfloat16_stays_with_the_plain_model(tmp_path):
+    import janus_b200
+    import plain_llama as P
+    from helpers import BF16_TOL, TINY_A, make_model_dir, random_tokens
+    d = make_model_dir(TINY_A, str(tmp_path), seed=1, dtype="bfloat16")
+    cfg, w = P.read_model_dir(d)
+    model = janus_b200.load(d, dtype="bfloat16", max_tokens=2048)
+    prefix = random_tokens(70, cfg["vocab_size"], 1)
+    prompts = [random_tokens(n, cfg["vocab_size"], 10 + n) for n in (1, 4, 8)]
+    out, stats = model.generate_shared(prefix, prompts, max_tokens=16, drafts=3, ignore_eos=True, drafter=EveryToken)
+    assert stats.drafted > 0
+    for p, o in zip(prompts, out):
+        logits = P.forward(cfg, w, prefix + p + o)
+        for j, t in enumerate(o):
+            row = logits[len(prefix) + len(p) - 1 + j]
+            assert float(row.max() - row[t]) <= BF16_TOL * float(row.abs().max())
+
+
+@gpu
+def test_generate_shared_draws_like_the_model(tmp_path):
+    """At a temperature the first tokens of many requests follow the model's distribution, drafts or not, and a seed repeats them."""
+    import janus_b200
+    import plain_llama as P
+    from helpers import TINY_A, make_model_dir, random_tokens
+    d = make_model_dir(TINY_A, str(tmp_path), seed=4, dtype="float32")
+    cfg, w = P.read_model_dir(d)
+    model = janus_b200.load(d, dtype="float32", max_tokens=65536, max_slots=1024)
+    prefix, n = random_tokens(64, cfg["vocab_size"], 3), 900
+    p = torch.softmax(P.forward(cfg, w, prefix + [5])[-1].double() / 0.05, 0).numpy()
+    one, _ = model.generate_shared(prefix, [[5]] * n, max_tokens=3, drafts=2, temperature=0.05, seed=7, ignore_eos=True, drafter=EveryToken)
+    two, _ = model.generate_shared(prefix, [[5]] * n, max_tokens=3, drafts=2, temperature=0.05, seed=7, ignore_eos=True, drafter=EveryToken)
+    assert one == two
+    count = np.bincount([o[0] for o in one], minlength=len(p))
+    # n draws: a token's count has standard deviation sqrt(n p (1 - p)); five of them, and a little for the rarest
+    assert (np.abs(count - n * p) <= 5.0 * np.sqrt(n * p * (1.0 - p)) + 2.0).all()
+
+
+@gpu
+def test_generate_shared_refusals(tmp_path):
+    import janus_b200
+    from helpers import TINY_A, make_model_dir
+    from janus_b200.cache import CacheFull
+    from janus_b200.engine.step import StepError
+    folder = make_model_dir(TINY_A, str(tmp_path), seed=0, dtype="float32")
+    model = janus_b200.load(folder, dtype="float32", max_tokens=192)
+    for error, args in ((ValueError, dict(prefix=[], prompts=[[]])), (StepError, dict(prefix=[1] * 100, prompts=[[1] * 40])),
+                        (StepError, dict(prefix=[1], prompts=[[999]])), (ValueError, dict(prefix=[1], prompts=[[1]], drafts=-1)),
+                        (ValueError, dict(prefix=[1], prompts=[[1]], temperature=-0.5))):
+        with pytest.raises(error):
+            model.generate_shared(**{**dict(max_tokens=4), **args})
+    small = janus_b200.load(folder, dtype="float32", max_tokens=64, max_slots=2)     # one page: the prefix takes it
+    with pytest.raises(CacheFull):
+        small.generate_shared([1] * 64, [[1, 2]], max_tokens=4)
+    for m in (model, small):
+        m.engine.cache.check()
+        assert m.engine.cache.groups[0].pool.n_held == 0
+    with pytest.raises(ValueError, match="grouped-query attention"):
+        from janus_b200.engine.shared_prefix import SharedPrefixRunner
+        model.engine.cache.states[0] = torch.zeros(1)
+        SharedPrefixRunner(model.engine)
