@@ -135,7 +135,7 @@ struct Tc {
   static constexpr int Q_BYTES = SLABS * BM * 128, KV_BYTES = SLABS * KB * 128;
   static constexpr int BARS = 1 + 8 + 2 * 2 + 3 * NT;          // q_full; k, v full and empty x 2; s_full, p_full x 2; o_full, o_done, o_free
   static constexpr int SWAP = NT * 2 * BM;                     // floats: what the two halves of a row tell each other
-  static constexpr int SMEM = NT * Q_BYTES + 4 * KV_BYTES + SWAP * 4 + NT * 4 * 4 + BARS * 8 + 16;
+  static constexpr int SMEM = NT * Q_BYTES + 4 * KV_BYTES + SWAP * 4 + NT * 4 * 4 + 8 + BARS * 8 + 16;
   static constexpr int THREADS = 64 + NT * 256;
   // (one tile of up to 128 numbers a row: 96 registers a thread, as 576 threads have, so that a block of own_kernel finds registers
   // beside this one; rows of up to 64 leave enough anyway)
@@ -170,7 +170,7 @@ __device__ __forceinline__ bool pair_any(int barrier, bool yes) {
 __device__ __forceinline__ void pair_sync(int barrier) { asm volatile("bar.sync %0, 64;" ::"r"(barrier) : "memory"); }
 
 // SHARED: the step's tokens over the prefix, results left as parts.  WHOLE: one sequence's tokens over all that they see.  OWN: one
-// sequence's tokens over its own keys, joined with the parts over the prefix.
+// sequence's tokens over its own keys, joined with the part over the prefix, or left as one more where there are several.
 enum Form { SHARED, WHOLE, OWN };
 
 __device__ __forceinline__ void store8(float* p, const uint32_t* r) {   // a whole 32-byte sector of a row
@@ -195,7 +195,8 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
   const uint32_t q_s = jb::smem_u32(smem), k_s = q_s + NT * C::Q_BYTES, v_s = k_s + 2 * C::KV_BYTES;
   float* swap = (float*)(smem + NT * C::Q_BYTES + 4 * C::KV_BYTES);   // [tile][half][row]
   int* gave_up = (int*)(swap + C::SWAP);                       // [tile][quarter]: one of the two warps has
-  uint64_t* bars = (uint64_t*)(gave_up + NT * 4);
+  int* found = gave_up + NT * 4;                               // WHOLE, OWN: the block's sequence and tile of it
+  uint64_t* bars = (uint64_t*)(found + 2);
   uint32_t* tmem_slot = (uint32_t*)(bars + C::BARS);
   const uint32_t bar0 = jb::smem_u32(bars);
   const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 24, v_full = bar0 + 40, v_empty = bar0 + 56;
@@ -230,6 +231,35 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
   jb::tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   if (FORM != OWN || parts.most == 0) jb::pdl_wait();
+  // WHOLE, OWN: which tile of which sequence this block has, by a list of the sequences' tiles (a grid of the longest one's would be
+  // mostly blocks without work, and each has the multiprocessor to itself)
+  if constexpr (FORM != SHARED) {
+    if (warp == 2) {
+      const int chunk = (s.n_seqs + 31) / 32, seq0 = min(lane * chunk, s.n_seqs), seq1 = min(seq0 + chunk, s.n_seqs), rows = NT * (BM / (s.nh / s.nkv));
+      int mine = 0;
+#pragma unroll 4
+      for (int i = seq0; i < seq1; ++i) mine += (max(s.q_start[i + 1] - s.q_start[i], 0) + rows - 1) / rows;
+      int up = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += t;
+      }
+      const int tile = blockIdx.y;
+      if (lane == 0) found[0] = -1, found[1] = 0;
+      __syncwarp();
+      if (tile < up && tile >= up - mine) {
+        int at = up - mine, i = seq0;
+        for (;; ++i) {
+          const int n = (max(s.q_start[i + 1] - s.q_start[i], 0) + rows - 1) / rows;
+          if (tile < at + n) break;
+          at += n;
+        }
+        found[0] = i, found[1] = (at + (max(s.q_start[i + 1] - s.q_start[i], 0) + rows - 1) / rows - 1) - tile;   // the longest first
+      }
+    }
+    __syncthreads();
+  }
   // (after the wait: a kernel that starts early may read what the launch before this one wrote)
   jb::pdl_launch_dependents();
 
@@ -243,7 +273,10 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
   int seq = 0, seq_start = 0, seq_pos = 0;        // SHARED: not used
   const int flat_begin = FORM == SHARED ? blockIdx.x * parts.per : 0;
   const int flat_end = FORM == SHARED ? min(flat_begin + parts.per, (s.T + parts.tile_tokens - 1) / parts.tile_tokens * s.nkv * parts.blocks) : 1;
-  if constexpr (FORM != SHARED) seq = blockIdx.z, seq_start = s.q_start[seq], seq_pos = s.kv_len[seq] - (s.q_start[seq + 1] - seq_start);
+  if constexpr (FORM != SHARED) {
+    seq = found[0];
+    if (seq >= 0) seq_start = s.q_start[seq], seq_pos = s.kv_len[seq] - (s.q_start[seq + 1] - seq_start);
+  }
   // the segment that begins at place `at` of the list; steps `at` on to the next
   auto segment = [&](int& at) {
     Segment g;
@@ -256,7 +289,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
       g.slot = blockIdx.x - item * parts.blocks / parts.per;
       at += g.nb;
     } else {
-      const int q_len = s.q_start[seq + 1] - seq_start, first = (gridDim.y - 1 - blockIdx.y) * NT * tpt;
+      const int q_len = seq < 0 ? 0 : s.q_start[seq + 1] - seq_start, first = found[1] * NT * tpt;
       g.kvh = blockIdx.x, g.tok0 = seq_start + first, g.n_tok = min(NT * tpt, q_len - first), g.block0 = 0, g.slot = 0;
       const int see = seq_pos + first + g.n_tok;             // keys that the last token sees
       g.n_shared = FORM == WHOLE ? (max(min(see, s.prefix_len), 0) + KB - 1) / KB : 0;
@@ -462,8 +495,8 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
       pair_sync(pair);                // (the place is read before it is written again)
       jb::tc_fence_after();
       const size_t place = (size_t)token * s.nh + head, all = (size_t)s.T * s.nh;
-      if constexpr (FORM == SHARED) {
-        const size_t item = g.slot * all + place;
+      if (FORM == SHARED || (FORM == OWN && parts.most > 1)) {
+        const size_t item = (FORM == SHARED ? g.slot : parts.most) * all + place;
         if (valid && half == 0) part_ml[item] = make_float2(m_ref, l);
 #pragma unroll
         for (int c1 = 0; c1 < DH; c1 += 16) {
@@ -472,6 +505,10 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
           uint32_t r[16];
           tmem_ld16(lane_addr + o_col + c0, r);   // warp-wide: rows without a token load too and store nothing
           jb::tmem_ld_wait();
+          if (FORM == OWN && g.nb == 0) {         // (no product has written there)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = 0u;
+          }
           if (valid) store8(part_o + item * s.hd + c0, r);
           if (valid && c0 + 8 < s.hd) store8(part_o + item * s.hd + c0 + 8, r + 8);
         }
@@ -479,8 +516,8 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
         __syncwarp();
         if (lane == 0) jb::mbar_arrive(o_free(w));
       } else {
-        // the parts over the prefix weigh in (OWN); few, or the steps of many tokens that come here would not cut the prefix
-        const int slots = FORM == OWN && valid ? slots_of(parts, s, token, g.kvh) : 0;
+        // the one part over the prefix weighs in (OWN)
+        const int slots = FORM == OWN && valid ? parts.most : 0;
         if (FORM == OWN && parts.most > 0) jb::pdl_wait();
         float top = m_ref;
         for (int i = 0; i < slots; ++i) top = fmaxf(top, part_ml[i * all + place].x);
@@ -878,15 +915,16 @@ cudaError_t own_go(int blocks, cudaStream_t stream, const CUtensorMap* maps, con
 }  // namespace
 
 // q, out [T, nh hd], caches [n_pages, nkv, 64, hd], all bfloat16.  tiles: row tiles of a block, 1 or 2 (one for heads of more than 128
-// numbers).  shared_ctas > 0: the prefix for all rows together by that many blocks, which cut a row's keys into at most `most`
-// ranges.  own_tiles: own keys by tiles of a sequence each (all keys, where nobody walks the prefix apart); else by the warps of
+// numbers).  shared_per > 0: the prefix for all rows together by blocks of that many key blocks each, which cut a row's keys into at
+// most `most` ranges.  own_tiles: own keys by tiles of a sequence each (all keys, where nobody walks the prefix apart); else by the warps of
 // own_ctas blocks, which get no less than `fewest` tiles of 32 keys each, so that a row has at most own_most partial results.
-// Scratch: part_o [most (+ own_most without own_tiles)][T][nh][hd] float32, part_ml [..][T][nh][2], own_count int [T][nkv].
+// Scratch: part_o [most + own_most][T][nh][hd] float32 (own_most 1 with
+// own_tiles and several ranges), part_ml [..][T][nh][2], own_count int [T][nkv].
 JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const void* v_cache, void* out, float* part_o, float* part_ml,
                                        int* own_count, const int* prefix_pages, int prefix_len, const int* block_table, int ld_table,
                                        int width, const int* q_start, const int* kv_len, const int* positions, int T, int n_pages,
                                        int n_seqs, int nh, int nkv, int hd, int page_size, float scale, int max_q_len, int max_kv_len,
-                                       int tiles, int shared_ctas, int most, int own_tiles, int own_ctas, int fewest, int own_most,
+                                       int tiles, int shared_per, int most, int own_tiles, int own_ctas, int fewest, int own_most,
                                        int* status, cudaStream_t stream) {
   if (T <= 0 || n_seqs <= 0 || max_q_len <= 0) return 0;
   JB_REFUSE(page_size != PAGE, "attention_prefix: page size %d (need %d)", page_size, PAGE);
@@ -897,9 +935,9 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
   JB_REFUSE(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15, "attention_prefix: operands must be 16-byte aligned");
   JB_REFUSE((long long)n_pages * nkv * PAGE > 0x7fffffffll, "attention_prefix: %d pages of %d heads are more rows than a tensor map counts",
             n_pages, nkv);
-  JB_REFUSE(n_seqs > 65535 || prefix_len < 0 || shared_ctas < 0 || most < 0 || most > 64 || (shared_ctas > 0) != (most > 0) ||
-                (shared_ctas > 0 && prefix_len == 0),
-            "attention_prefix: a prefix of %d tokens in %d ranges by %d blocks for %d sequences", prefix_len, most, shared_ctas, n_seqs);
+  JB_REFUSE(n_seqs > 65535 || prefix_len < 0 || shared_per < 0 || most < 0 || most > 64 || (shared_per > 0) != (most > 0) ||
+                (shared_per > 0 && prefix_len == 0),
+            "attention_prefix: a prefix of %d tokens in %d ranges of %d key blocks for %d sequences", prefix_len, most, shared_per, n_seqs);
   const Step s{prefix_pages, block_table, q_start, kv_len, positions, prefix_len, ld_table, width, T, n_seqs, nh, nkv, hd, scale * LOG2E};
   const bf16 *qb = (const bf16*)q, *kb = (const bf16*)k_cache, *vb = (const bf16*)v_cache;
   bf16* ob = (bf16*)out;
@@ -907,32 +945,34 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
   const int nt = hd > 128 ? 1 : tiles, step = nt * (BM / G), keys = hd > 128 ? 64 : 128;
   Slots parts{0, 0, 0, 1, 1};
   CUtensorMap maps[3];
-  if ((shared_ctas > 0 || own_tiles) && !make_maps(&maps[0], &maps[1], &maps[2], q, k_cache, v_cache, s, n_pages, PAGE)) return JB_ERR_TENSORMAP;
+  if ((shared_per > 0 || own_tiles) && !make_maps(&maps[0], &maps[1], &maps[2], q, k_cache, v_cache, s, n_pages, PAGE)) return JB_ERR_TENSORMAP;
   cudaError_t e = cudaSuccess;
-  if (shared_ctas > 0) {
+  if (shared_per > 0) {
     const int blocks = (prefix_len + keys - 1) / keys;
-    const long long total = (long long)((T + step - 1) / step) * nkv * blocks;
-    JB_REFUSE(shared_ctas > total || total > 0x7fffffffll, "attention_prefix: %d blocks for %lld key blocks", shared_ctas, total);
-    parts = Slots{-1, most, blocks, (int)((total + shared_ctas - 1) / shared_ctas), step};
-    // a tile's blocks begin anywhere in a range, unless ranges divide them
-    JB_REFUSE((total + parts.per - 1) / parts.per != shared_ctas ||
-                  (blocks % parts.per == 0 ? blocks / parts.per : (blocks + parts.per - 2) / parts.per + 1) > most,
-              "attention_prefix: %d blocks cut %d key blocks into more than %d ranges", shared_ctas, blocks, most);
-    e = tc_pick<SHARED>(nt, dim3(shared_ctas), stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status);
+    const long long total = (long long)((T + step - 1) / step) * nkv * blocks, ctas = (total + shared_per - 1) / shared_per;
+    // a tile's blocks begin anywhere in a range, unless ranges divide them, or are whole tiles
+    JB_REFUSE(total > 0x3fffffffll, "attention_prefix: %lld key blocks", total);
+    JB_REFUSE((shared_per % blocks == 0 ? 1 : blocks % shared_per == 0 ? blocks / shared_per : (blocks + shared_per - 2) / shared_per + 1) > most,
+              "attention_prefix: ranges of %d cut %d key blocks into more than %d", shared_per, blocks, most);
+    parts = Slots{-1, most, blocks, shared_per, step};
+    e = tc_pick<SHARED>(nt, dim3((unsigned)ctas), stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status);
     if (e != cudaSuccess) return (int)e;
   }
   if (own_tiles) {
-    const dim3 grid(nkv, (max_q_len + step - 1) / step, n_seqs);
-    return (int)(shared_ctas > 0 ? tc_pick<OWN>(nt, grid, stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status)
-                                 : tc_pick<WHOLE>(nt, grid, stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status));
+    const dim3 grid(nkv, T / step + (n_seqs < T ? n_seqs : T));   // no more tiles than that, however the tokens are shared out
+    JB_REFUSE(grid.y > 65535, "attention_prefix: %d tokens of %d sequences", T, n_seqs);
+    e = shared_per > 0 ? tc_pick<OWN>(nt, grid, stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status)
+                       : tc_pick<WHOLE>(nt, grid, stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status);
+    if (e != cudaSuccess || most <= 1) return (int)e;
+    return (int)join_go<bf16>(stream, qb, kb, vb, ob, part_o, ml, nullptr, s, parts, 1);
   }
-  JB_REFUSE(shared_ctas == 0 && prefix_len > 0, "attention_prefix: nothing walks the prefix");
+  JB_REFUSE(shared_per == 0 && prefix_len > 0, "attention_prefix: nothing walks the prefix");
   const int row_blocks = (max_q_len * G + 15) / 16, tiles_most = (max_kv_len - prefix_len + OWN_KEYS - 1) / OWN_KEYS;
   JB_REFUSE(own_ctas < 1 || fewest < 1 || own_most > 64 || (tiles_most + fewest - 2) / fewest + 1 > own_most ||
                 (long long)n_seqs * nkv * row_blocks * (tiles_most < 1 ? 1 : tiles_most) > 0x3fffffffll,
             "attention_prefix: %d blocks for %d tiles of own keys of %d sequences", own_ctas, tiles_most, n_seqs);
   if (!make_maps(nullptr, &maps[1], &maps[2], q, k_cache, v_cache, s, n_pages, OWN_KEYS)) return JB_ERR_TENSORMAP;
-  const int behind = shared_ctas > 0;
+  const int behind = shared_per > 0;
   if (hd > 128) e = own_go<256, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, fewest, status);
   else if (hd > 64) e = own_go<128, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, fewest, status);
   else e = own_go<64, 2>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, fewest, status);

@@ -2488,7 +2488,7 @@ def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         rows, own_rows, splits, own_slots = attention_prefix_plan_f32(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv)
         slots = splits + own_slots
     else:
-        tiles, ctas, splits, own_tiles, own_ctas, fewest, own_slots = attention_prefix_plan(
+        tiles, per, splits, own_tiles, own_ctas, fewest, own_slots = attention_prefix_plan(
             T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv, hd)
         slots = splits + own_slots
     part_o = part_ml = own_count = None
@@ -2500,28 +2500,28 @@ def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
             *step, _ptr(part_o), _ptr(part_ml), *rest, n_seqs, nh, nkv, hd, page_size, float(scale), int(max_q_len), rows, own_rows,
             splits, own_slots, _stream()), "attention_prefix", kernels=1 if hd % 4 else (splits > 0) + 2)
         return
-    if own_slots:
+    if own_ctas:
         own_count = workspace.get("prefix_own_count", (T * nkv,), torch.int32).data_ptr()
     _check(_lib("prefix_attention").jb_attention_prefix_bf16(
         *step, _ptr(part_o), _ptr(part_ml), own_count, *rest, k_cache.shape[0], n_seqs, nh, nkv, hd, page_size, float(scale),
-        int(max_q_len), int(max_kv_len), tiles, ctas, splits, own_tiles, own_ctas, fewest, own_slots, _ptr(kernel_status(q.device)),
-        _stream()), "attention_prefix", kernels=(ctas > 0) + (1 if own_tiles else 2))
+        int(max_q_len), int(max_kv_len), tiles, per, splits, own_tiles, own_ctas, fewest, own_slots, _ptr(kernel_status(q.device)),
+        _stream()), "attention_prefix", kernels=(per > 0) + 1 + (own_slots > 0))
 
 
 _PREFIX_MOST_RANGES = 64       # partial results over the prefix that a row's join takes
 
 
-def _even_ranges(total: int, blocks: int, most_ctas: int):
-    """(blocks with equal ranges of `total` places, the last one with what is left; the most of their ranges that `blocks` consecutive
-    places from a multiple of it on are in)."""
+def _prefix_ranges(total: int, blocks: int, most_ctas: int):
+    """(length of equal ranges for at most `most_ctas` blocks of `total` places, the most of them that `blocks` consecutive places from a
+    multiple of it on are in)."""
     per = max(-(-total // most_ctas), -(-blocks // (_PREFIX_MOST_RANGES - 2)))
-    return -(-total // per), blocks // per if blocks % per == 0 else (blocks + per - 2) // per + 1
+    return per, 1 if per % blocks == 0 else blocks // per if blocks % per == 0 else (blocks + per - 2) // per + 1
 
 
 @functools.lru_cache(maxsize=4096)
 def attention_prefix_plan(T: int, n_seqs: int, max_q_len: int, prefix_len: int, max_own: int, nh: int, nkv: int, hd: int):
-    """How a bfloat16 `attention_prefix` runs: (row tiles a block, blocks that walk the prefix for all rows together (0: nobody does), the
-    most ranges in which a row's prefix keys come, whether own keys go by tiles, blocks that walk own keys otherwise, the fewest
+    """How a bfloat16 `attention_prefix` runs: (row tiles a block, key blocks of each block that walks the prefix for all rows together
+    (0: nobody does), the most ranges in which a row's prefix keys come, whether own keys go by tiles, blocks that walk own keys otherwise, the fewest
     tiles of 32 keys of a warp of theirs, the most partial results that makes a row)."""
     group, sms = nh // nkv, SM_COUNT_TARGET // 2
     rows, keys = 128 // group, 64 if hd > 128 else 128     # tokens of a tile, keys of a block
@@ -2537,18 +2537,22 @@ def attention_prefix_plan(T: int, n_seqs: int, max_q_len: int, prefix_len: int, 
         own_blocks = (max_own + keys - 1) // keys
         waves = -(-nkv * (T // step + (n_seqs + 1) // 2) // sms)
         whole = waves * (blocks + own_blocks) * block_us
-        apart = -(-(-(-T // step) * nkv * blocks) // sms) * block_us + waves * own_blocks * block_us + 8 + T * nh * hd * 8 / 4e6
+        items = -(-T // step) * nkv
+        even = -(-items * blocks // sms)                   # key blocks of a block, cut evenly
+        uncut = -(-items // sms) * blocks                  # ... in whole tiles: one partial result a row
+        apart = min(even * 1.1, uncut) * block_us + waves * own_blocks * block_us + 12 + T * nh * hd * 8 / 4e6
         if whole <= apart:
             return tiles, 0, 0, 1, 0, 0, 0
-        return tiles, *_even_ranges(-(-T // step) * nkv * blocks, blocks, sms), 1, 0, 0, 0
+        per, ranges = (uncut, 1) if uncut <= 1.1 * even else _prefix_ranges(items * blocks, blocks, sms)
+        return tiles, per, ranges, 1, 0, 0, 1 if ranges > 1 else 0
     # one tile a block over the prefix: with two a block, its keys are fetched once for both, but the own keys' blocks then find no
     # room beside it (64 single tokens behind 8,192: 31 us and 40)
-    ctas, ranges = _even_ranges(-(-T // rows) * nkv * blocks, blocks, sms) if prefix_len else (0, 0)
+    per, ranges = _prefix_ranges(-(-T // rows) * nkv * blocks, blocks, sms) if prefix_len else (0, 0)
     own_blocks = max(1, (max_own + 31) // 32)
     places = n_seqs * nkv * ((max_q_len * group + 15) // 16) * own_blocks
     fewest = max(1, min(4, places // (8 * sms)), -(-own_blocks // 30))
     own_ctas = max(1, min((3 if hd <= 128 else 1) * sms, -(-places // (4 * fewest))))
-    return 1, ctas, ranges, 0, own_ctas, fewest, (own_blocks + fewest - 2) // fewest + 1
+    return 1, per, ranges, 0, own_ctas, fewest, (own_blocks + fewest - 2) // fewest + 1
 
 
 @functools.lru_cache(maxsize=4096)

@@ -527,16 +527,14 @@ def test_plans_cover_what_they_cut():
         n = int(rng.integers(1, 300))
         q = int(rng.choice([1, 1, 2, 7, 100]))
         T, prefix, own = n * q, int(rng.integers(1, 30000)), int(rng.integers(1, 4000))
-        tiles, ctas, ranges, own_tiles, own_ctas, fewest, own_most = ops.attention_prefix_plan(T, n, q, prefix, own, group * nkv, nkv, hd)
+        tiles, per, ranges, own_tiles, own_ctas, fewest, own_most = ops.attention_prefix_plan(T, n, q, prefix, own, group * nkv, nkv, hd)
         assert 0 <= ranges <= 64 and own_most <= 64 and (own_tiles or own_ctas >= 1)
-        if not ctas:
+        if not per:
             assert own_tiles
             continue
         keys = 64 if hd > 128 else 128
         blocks, step = -(-prefix // keys), 128 // group * tiles
         items = -(-T // step) * nkv
-        per = -(-items * blocks // ctas)
-        assert -(-items * blocks // per) == ctas
         owner = np.arange(items * blocks) // per
         for i in range(items):
             assert owner[(i + 1) * blocks - 1] - owner[i * blocks] + 1 <= ranges
