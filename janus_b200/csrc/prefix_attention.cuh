@@ -95,25 +95,28 @@ __device__ __forceinline__ int slots_of(const Slots& p, const Step& s, int token
   return (place + p.blocks - 1) / p.per - place / p.per + 1;
 }
 
-// One warp a (token, query head): all partial results joined in the order of their slots, the prefix's first, then those over own
-// keys: own_count[token][kv head] of them, or own_slots where that is null.  All of a row's slots are asked for at once; joined by the
-// blocks that walk the own keys, one row after another, the wait for them took longer than the keys (48 sequences of up to 24 rows:
-// 24 of 34 us).
-template <typename E>
+// All partial results of a (token, query head) joined in the order of their slots, the prefix's first, then those over own keys:
+// own_count[token][kv head] of them, or own_slots where that is null.  WARPS warps a row, each with every WARPS-th slot: four where
+// there are few rows, which otherwise wait for one slot after another (464 rows of 35 slots: 19 us by one warp each), one where there
+// are many.  Joined by the blocks that walk the own keys, one row after another, the wait took longer than the keys (48 sequences of up
+// to 24 rows: 24 of 34 us).
+template <typename E, int WARPS>
 __global__ void __launch_bounds__(128) join_kernel(const E* __restrict__ q, const E* __restrict__ k_cache,
                                                    const E* __restrict__ v_cache, E* __restrict__ out,
                                                    const float* __restrict__ part_o, const float2* __restrict__ part_ml,
                                                    const int* __restrict__ own_count, const Step s, const Slots parts, int own_slots) {
-  const int item = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  __shared__ float4 red[WARPS > 1 ? WARPS * 64 : 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = WARPS > 1 ? warp : 0;
+  const int item = WARPS > 1 ? blockIdx.x : blockIdx.x * 4 + warp;
   const int t = item / s.nh, h = item - t * s.nh, kvh = h / (s.nh / s.nkv);
   const size_t all = (size_t)s.T * s.nh;
   const int shared = t < s.T ? slots_of(parts, s, t, kvh) : 0;
   jb::pdl_wait();
   jb::pdl_launch_dependents();
   if (t >= s.T) return;
-  const int total = s.q_start[s.n_seqs], own = own_count ? own_count[t * s.nkv + kvh] : own_slots;
   auto place = [&](int i) { return (i < shared ? i : parts.most + i - shared) * all + item; };
-  // (at most 64 prefix slots and 64 others; asked for before it is known how many there are)
+  const int total = s.q_start[s.n_seqs], own = own_count ? own_count[t * s.nkv + kvh] : own_slots;
+  // (asked for before it is known whether the row is anybody's)
   float2 first = make_float2(-CUDART_INF_F, 0.0f);
   if (lane < shared) first = part_ml[place(lane)];
   if (t >= total) return;
@@ -131,7 +134,7 @@ __global__ void __launch_bounds__(128) join_kernel(const E* __restrict__ q, cons
     sum = fmaf(mine, ml.y, sum);
     const int n = min(32, slots - i0);
 #pragma unroll 8
-    for (int j = 0; j < n; ++j) {
+    for (int j = part; j < n; j += WARPS) {
       const float f = __shfl_sync(0xffffffffu, mine, j);
       const float* row = part_o + place(i0 + j) * s.hd;
 #pragma unroll
@@ -145,6 +148,18 @@ __global__ void __launch_bounds__(128) join_kernel(const E* __restrict__ q, cons
     }
   }
   sum = jb::warp_sum(sum);
+  if constexpr (WARPS > 1) {
+    red[warp * 64 + lane] = acc[0], red[warp * 64 + 32 + lane] = acc[1];
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float4 v = red[w * 64 + 32 * e + lane];
+        acc[e].x += v.x, acc[e].y += v.y, acc[e].z += v.z, acc[e].w += v.w;
+      }
+  }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   bool finite = true;
 #pragma unroll
@@ -167,17 +182,25 @@ cudaError_t set_up(Kernel* kernel, int smem) {
   return e;
 }
 
-template <typename E>
-cudaError_t join_go(cudaStream_t stream, const E* q, const E* k, const E* v, E* out, const float* part_o, const float2* part_ml,
+template <typename E, int WARPS>
+cudaError_t join_as(cudaStream_t stream, const E* q, const E* k, const E* v, E* out, const float* part_o, const float2* part_ml,
                     const int* own_count, const Step& s, const Slots& parts, int own_slots) {
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = set_up(join_kernel<E>, 0);
+    cudaError_t e = set_up(join_kernel<E, WARPS>, 0);
     if (e != cudaSuccess) return e;
     configured = true;
   }
-  jb::Launch cfg(dim3((unsigned)(((long long)s.T * s.nh + 3) / 4)), dim3(128), 0, stream);
-  return cudaLaunchKernelEx(&cfg.c, join_kernel<E>, q, k, v, out, part_o, part_ml, own_count, s, parts, own_slots);
+  const long long rows = (long long)s.T * s.nh;
+  jb::Launch cfg(dim3((unsigned)(WARPS > 1 ? rows : (rows + 3) / 4)), dim3(128), 0, stream);
+  return cudaLaunchKernelEx(&cfg.c, join_kernel<E, WARPS>, q, k, v, out, part_o, part_ml, own_count, s, parts, own_slots);
+}
+// (four warps a row up to what fits the multiprocessors at once, sixteen blocks each)
+template <typename E>
+cudaError_t join_go(cudaStream_t stream, const E* q, const E* k, const E* v, E* out, const float* part_o, const float2* part_ml,
+                    const int* own_count, const Step& s, const Slots& parts, int own_slots) {
+  return (long long)s.T * s.nh <= 148 * 16 ? join_as<E, 4>(stream, q, k, v, out, part_o, part_ml, own_count, s, parts, own_slots)
+                                           : join_as<E, 1>(stream, q, k, v, out, part_o, part_ml, own_count, s, parts, own_slots);
 }
 
 }  // namespace

@@ -3,8 +3,7 @@
 // The same split: the prefix's keys in ranges for the rows of all sequences together, each sequence's own pages, partial results
 // joined.  A block has 16 RR rows (token, query head of one kv head) and walks pages of 64 keys.  Thread (y, x) of 16 x 16 has RR
 // rows and keys x, x + 16, .. of the scores, then the same rows and numbers 4 x .. 4 x + 3, 64 further, .. of the weighted values:
-// products of RR x 4 out of shared memory, two multiply-adds an instruction.  The next page's keys are on their way during the
-// softmax and the values' product, its values during the scores' product.  Head sizes that are no multiple of 4 go row by row.
+// products of RR x 4 out of shared memory, two multiply-adds an instruction.  A page's values are on their way during its scores.  Head sizes that are no multiple of 4 go row by row.
 #include "prefix_attention.cuh"
 
 namespace {
@@ -31,22 +30,24 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 template <int HDC, int RR>
 struct Tile {
   static constexpr int ROWS = 16 * RR, LD = HDC + 4, LD_P = PAGE + 4;
-  // queries, keys, values, weights; the rows' results take the place of keys and values at the end
-  static constexpr int FLOATS = ROWS * LD + PAGE * LD + PAGE * LD + ROWS * LD_P;
-  static constexpr int SMEM = FLOATS * 4;
+  // queries, keys, values.  The weights take the keys' place once the scores are made, the rows' results the place of keys and values
+  // at the end.  Two blocks share a multiprocessor (heads of up to 128 numbers), and one's products hide the other's loads.
+  static constexpr int FLOATS = ROWS * LD + PAGE * LD + PAGE * LD;
+  static constexpr int SMEM = FLOATS * 4, BLOCKS = HDC <= 128 ? 2 : 1;
+  static_assert(ROWS * LD_P <= PAGE * LD, "the weights' place");
   static_assert(SMEM <= 232448 && ROWS <= PAGE, "shared memory of one block");
 };
 
 // OWN: the rows of one sequence over its own pages.  Else the rows of all sequences over a range of the prefix's pages.
 template <int HDC, int RR, bool OWN>
-__global__ void __launch_bounds__(THREADS) tile_f32_kernel(const float* __restrict__ q, const float* __restrict__ k_cache,
+__global__ void __launch_bounds__(THREADS, (Tile<HDC, RR>::BLOCKS)) tile_f32_kernel(const float* __restrict__ q, const float* __restrict__ k_cache,
                                                            const float* __restrict__ v_cache, float* __restrict__ part_o,
                                                            float2* __restrict__ part_ml, const Step s,
                                                            const Slots parts, int own_slots, int row_blocks) {
   typedef Tile<HDC, RR> C;
   extern __shared__ __align__(16) float smem[];
   __shared__ float red_ml[2 * C::ROWS];
-  float *q_s = smem, *k_s = q_s + C::ROWS * C::LD, *v_s = k_s + PAGE * C::LD, *p_s = v_s + PAGE * C::LD;
+  float *q_s = smem, *k_s = q_s + C::ROWS * C::LD, *v_s = k_s + PAGE * C::LD, *p_s = k_s;
   const int G = s.nh / s.nkv, hd = s.hd, tid = threadIdx.x, x = tid & 15, y = tid >> 4;
   const int prefix_slots = parts.fixed;
   // (a launch over own keys right behind the one over the prefix finds everything in its place but that one's results, which it
@@ -121,9 +122,7 @@ __global__ void __launch_bounds__(THREADS) tile_f32_kernel(const float* __restri
         for (int k = 0; k < 4; ++k) acc[r][k] = jb::fma2(qv.y, kv[k].y, jb::fma2(qv.x, kv[k].x, acc[r][k]));
       }
     }
-    __syncthreads();
-    if (p + 1 < p_end) load(k_s, k_cache, p + 1);
-    else cp_async_commit();
+    __syncthreads();             // the keys have been read
     float corr[RR];
 #pragma unroll
     for (int r = 0; r < RR; ++r) {
@@ -148,7 +147,7 @@ __global__ void __launch_bounds__(THREADS) tile_f32_kernel(const float* __restri
 #pragma unroll
       for (int i = 0; i < HDC / 32; ++i) o[r][i] = jb::mul2(o[r][i], jb::pair(corr[r], corr[r]));
     }
-    cp_async_wait<1>();          // the page's values
+    cp_async_wait<0>();          // the page's values
     __syncthreads();
 #pragma unroll 2
     for (int k = 0; k < PAGE; k += 4) {
@@ -172,8 +171,10 @@ __global__ void __launch_bounds__(THREADS) tile_f32_kernel(const float* __restri
       }
     }
     __syncthreads();
-    if (p + 1 < p_end) load(v_s, v_cache, p + 1);
-    else cp_async_commit();
+    if (p + 1 < p_end) {
+      load(k_s, k_cache, p + 1);
+      load(v_s, v_cache, p + 1);
+    }
   }
   __syncthreads();
   float* red_o = k_s;

@@ -2562,7 +2562,7 @@ def attention_prefix_plan_f32(T: int, n_seqs: int, max_q_len: int, prefix_len: i
     group, sms = nh // nkv, SM_COUNT_TARGET // 2
     rows, own_rows = (16 if n * group <= 32 else 64 for n in (T, max_q_len))
     pages = (prefix_len + 63) // 64
-    splits = min(64, pages, max(1, sms // (nkv * ((T * group + rows - 1) // rows)))) if prefix_len else 0
+    splits = min(64, pages, max(1, 2 * sms // (nkv * ((T * group + rows - 1) // rows)))) if prefix_len else 0    # two blocks an SM
     ctas = n_seqs * nkv * ((max_q_len * group + own_rows - 1) // own_rows)
     return rows, own_rows, splits, min(32, max(1, (max_own + 127) // 128), max(1, 2 * sms // max(1, ctas)))
 
