@@ -625,12 +625,14 @@ struct Own {
 struct Cursor {
   int seq, kvh, rb, tile;           // sequence; kv head, block of 16 rows; tile of the row's keys
   int tiles, row_blocks, start, q_len;
+  int shared;                       // tiles of the prefix in front, where the list holds them
 };
 // What sequence `seq` adds to the list: every row has a tile, also one that sees no key of its own.
-__device__ __forceinline__ void look_up(const Step& s, int seq, Cursor& c) {
+__device__ __forceinline__ void look_up(const Step& s, int seq, int shared, Cursor& c) {
   c.seq = seq, c.start = s.q_start[seq], c.q_len = s.q_start[seq + 1] - c.start;
   c.row_blocks = c.q_len > 0 ? (c.q_len * (s.nh / s.nkv) + 15) / 16 : 0;
-  c.tiles = min(max((s.kv_len[seq] - s.prefix_len + OWN_KEYS - 1) / OWN_KEYS, 1), max(s.width * OWN_HALVES, 1));
+  c.shared = shared;
+  c.tiles = shared + min(max((s.kv_len[seq] - s.prefix_len + OWN_KEYS - 1) / OWN_KEYS, 1), max(s.width * OWN_HALVES, 1));
 }
 __device__ __forceinline__ int places(const Step& s, const Cursor& c) { return s.nkv * c.row_blocks * c.tiles; }
 __device__ __forceinline__ void step_on(const Step& s, Cursor& c) {
@@ -642,7 +644,7 @@ __device__ __forceinline__ void step_on(const Step& s, Cursor& c) {
   c.kvh = 0;
   do {
     if (c.seq + 1 >= s.n_seqs) return;   // (behind the list's end: nobody goes there)
-    look_up(s, c.seq + 1, c);
+    look_up(s, c.seq + 1, c.shared, c);
   } while (c.row_blocks == 0);
 }
 
@@ -650,7 +652,7 @@ template <int HDC, int STAGES>
 __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                           const bf16* __restrict__ q, float* __restrict__ part_o, float2* __restrict__ part_ml,
                                                           int* __restrict__ own_count, const Step s, int first_slot, int after_prefix,
-                                                          int fewest, int* __restrict__ status) {
+                                                          int shared, int fewest, int* __restrict__ status) {
   typedef Own<HDC, STAGES> C;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = (uint64_t*)(smem + C::RING);
@@ -670,7 +672,7 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
 #pragma unroll 4
   for (int i = seq0; i < seq1; ++i) {
     Cursor x;
-    look_up(s, i, x);
+    look_up(s, i, shared, x);
     mine += places(s, x);
   }
   int up = mine;
@@ -686,7 +688,7 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
     const int owner = __ffs(__ballot_sync(0xffffffffu, begin < up)) - 1;
     int before = __shfl_sync(0xffffffffu, up - mine, owner);
     for (int i = owner * chunk;; ++i) {
-      look_up(s, i, c);
+      look_up(s, i, shared, c);
       const int n = places(s, c);
       if (begin < before + n) break;
       before += n;
@@ -699,14 +701,18 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
   Cursor ahead = c;
   int asked = begin;
   // (a tile's page is looked up a turn before it is asked for, or every turn would wait for memory)
-  auto page_of = [&](const Cursor& x) { return s.width > 0 ? s.table[(size_t)x.seq * s.ld_table + x.tile / OWN_HALVES] : 0; };
+  auto page_of = [&](const Cursor& x) {
+    if (x.tile < x.shared) return s.prefix_pages[x.tile / OWN_HALVES];
+    return s.width > 0 ? s.table[(size_t)x.seq * s.ld_table + (x.tile - x.shared) / OWN_HALVES] : 0;
+  };
   int page = begin < end ? page_of(ahead) : 0;
   // Keys and values of a tile have a barrier each: with one stage the next keys are on their way while this tile's softmax and the
   // values' product run, the next values during the scores.
   auto issue = [&](int what) {   // 0: the keys of the next tile that has not been asked for; 1: its values, and on to the one behind
     const int st = (asked - begin) % STAGES;
     if (elected()) {
-      const int row = (max(page, 0) * s.nkv + ahead.kvh) * PAGE + ahead.tile % OWN_HALVES * OWN_KEYS;
+      const int half = (ahead.tile < ahead.shared ? ahead.tile : ahead.tile - ahead.shared) % OWN_HALVES;
+      const int row = (max(page, 0) * s.nkv + ahead.kvh) * PAGE + half * OWN_KEYS;
       const uint32_t at = ring + st * C::STAGE + what * C::TILE, full_at = bar + 16 * st + 8 * what;
       jb::mbar_expect_tx(full_at, nslab * C::SLAB);
       for (int h = 0; h < nslab; ++h) jb::tma_load_2d(at + h * C::SLAB, what ? &map_v : &map_k, full_at, h * 64, row, policy);
@@ -729,12 +735,12 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
   for (int i = begin; i < end; ++i) {
     if (i == begin || c.tile == 0) {
       const int kvh = c.kvh, row0 = c.rb * 16, n_rows = min(16, c.q_len * G - row0);
-      const int first_pos = s.kv_len[c.seq] - c.q_len - s.prefix_len;   // among the own keys
+      const int first_pos = s.kv_len[c.seq] - c.q_len;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int row = (lane >> 2) + 8 * r, token = (row0 + row) / G, head = kvh * G + (row0 + row) % G;
         const bool valid = row < n_rows;
-        see_row[r] = valid ? min(first_pos + token + 1, s.width * PAGE) : 0;
+        see_row[r] = valid ? first_pos + token + 1 : 0;   // keys that the row sees, the prefix's first
         m[r] = -CUDART_INF_F, l[r] = 0.0f;
         const bf16* src = q + ((size_t)(c.start + (valid ? token : 0)) * s.nh + head) * hd + 2 * (lane & 3);
 #pragma unroll
@@ -768,12 +774,16 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
     __syncwarp();   // the warp is done with the keys
     if (asked < end) issue(0);
     float mx[2] = {-CUDART_INF_F, -CUDART_INF_F}, corr[2], ref[2];
-    const int key0 = c.tile * OWN_KEYS + 2 * (lane & 3);
+    const bool of_prefix = c.tile < c.shared;
+    const int key0 = (of_prefix ? c.tile : c.tile - c.shared) * OWN_KEYS + 2 * (lane & 3);
+    int limit[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) limit[r] = of_prefix ? min(see_row[r], s.prefix_len) : min(see_row[r] - s.prefix_len, s.width * PAGE);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[j][e] = key0 + j * 8 + (e & 1) < see_row[e >> 1] ? x[j][e] * s.scale_log2 : -CUDART_INF_F;
+        x[j][e] = key0 + j * 8 + (e & 1) < limit[e >> 1] ? x[j][e] * s.scale_log2 : -CUDART_INF_F;
         mx[e >> 1] = fmaxf(mx[e >> 1], x[j][e]);
       }
 #pragma unroll
@@ -899,7 +909,7 @@ cudaError_t tc_pick(int nt, dim3 grid, cudaStream_t stream, const CUtensorMap* m
 
 template <int HDC, int STAGES>
 cudaError_t own_go(int blocks, cudaStream_t stream, const CUtensorMap* maps, const bf16* q, float* part_o, float2* part_ml, int* own_count,
-                   const Step& s, int first_slot, int after_prefix, int fewest, int* status) {
+                   const Step& s, int first_slot, int after_prefix, int shared, int fewest, int* status) {
   typedef Own<HDC, STAGES> C;
   static bool configured = false;
   if (!configured) {
@@ -909,23 +919,26 @@ cudaError_t own_go(int blocks, cudaStream_t stream, const CUtensorMap* maps, con
   }
   jb::Launch cfg(dim3(blocks), dim3(OWN_THREADS), C::SMEM, stream);
   return cudaLaunchKernelEx(&cfg.c, own_kernel<HDC, STAGES>, maps[0], maps[1], q, part_o, part_ml, own_count, s, first_slot, after_prefix,
-                            fewest, status);
+                            shared, fewest, status);
 }
 
 }  // namespace
 
 // q, out [T, nh hd], caches [n_pages, nkv, 64, hd], all bfloat16.  tiles: row tiles of a block, 1 or 2 (one for heads of more than 128
 // numbers).  shared_per > 0: the prefix for all rows together by blocks of that many key blocks each, which cut a row's keys into at
-// most `most` ranges.  own_tiles: own keys by tiles of a sequence each (all keys, where nobody walks the prefix apart); else by the warps of
-// own_ctas blocks, which get no less than `fewest` tiles of 32 keys each, so that a row has at most own_most partial results.
-// Scratch: part_o [most + own_most][T][nh][hd] float32 (own_most 1 with
-// own_tiles and several ranges), part_ml [..][T][nh][2], own_count int [T][nkv].
-JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const void* v_cache, void* out, float* part_o, float* part_ml,
-                                       int* own_count, const int* prefix_pages, int prefix_len, const int* block_table, int ld_table,
-                                       int width, const int* q_start, const int* kv_len, const int* positions, int T, int n_pages,
-                                       int n_seqs, int nh, int nkv, int hd, int page_size, float scale, int max_q_len, int max_kv_len,
-                                       int tiles, int shared_per, int most, int own_tiles, int own_ctas, int fewest, int own_most,
-                                       int* status, cudaStream_t stream) {
+// most `most` ranges.  own_tiles: own keys by tiles of a sequence each, else by the warps of
+// own_ctas blocks, which get no less than `fewest` tiles of 32 keys each, so that a row has at most own_most partial results; with the prefix's keys, where
+// nobody walks those apart.
+// scratch: floats [most + own_most][T][nh][hd], then
+// [..][T][nh][2], then T nkv whole numbers (own_most 1 with own_tiles and several ranges).
+// sizes: host memory, see Sizes.
+JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const void* v_cache, void* out, float* scratch,
+                                       const int* prefix_pages, const int* block_table, const int* q_start, const int* kv_len,
+                                       const int* positions, const void* sizes, int* status, cudaStream_t stream) {
+  const Sizes& z = *(const Sizes*)sizes;
+  const int prefix_len = z.prefix_len, T = z.T, n_pages = z.n_pages, n_seqs = z.n_seqs, nh = z.nh, nkv = z.nkv, hd = z.hd;
+  const int page_size = z.page_size, max_q_len = z.max_q_len, max_kv_len = z.max_kv_len, tiles = z.tiles, shared_per = z.shared_per;
+  const int most = z.most, own_tiles = z.own_tiles, own_ctas = z.own_ctas, fewest = z.fewest, own_most = z.own_most;
   if (T <= 0 || n_seqs <= 0 || max_q_len <= 0) return 0;
   JB_REFUSE(page_size != PAGE, "attention_prefix: page size %d (need %d)", page_size, PAGE);
   JB_REFUSE(nkv <= 0 || nh % nkv != 0, "attention_prefix: %d heads are not a multiple of %d kv heads", nh, nkv);
@@ -938,10 +951,13 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
   JB_REFUSE(n_seqs > 65535 || prefix_len < 0 || shared_per < 0 || most < 0 || most > 64 || (shared_per > 0) != (most > 0) ||
                 (shared_per > 0 && prefix_len == 0),
             "attention_prefix: a prefix of %d tokens in %d ranges of %d key blocks for %d sequences", prefix_len, most, shared_per, n_seqs);
-  const Step s{prefix_pages, block_table, q_start, kv_len, positions, prefix_len, ld_table, width, T, n_seqs, nh, nkv, hd, scale * LOG2E};
+  const Step s{prefix_pages, block_table, q_start, kv_len, positions, prefix_len, z.ld_table, z.width, T, n_seqs, nh, nkv, hd, z.scale * LOG2E};
   const bf16 *qb = (const bf16*)q, *kb = (const bf16*)k_cache, *vb = (const bf16*)v_cache;
   bf16* ob = (bf16*)out;
-  float2* ml = (float2*)part_ml;
+  const size_t rows_of_parts = (size_t)(most + own_most) * T * nh;
+  float* part_o = scratch;
+  float2* ml = (float2*)(scratch + rows_of_parts * hd);
+  int* own_count = (int*)(ml + rows_of_parts);
   const int nt = hd > 128 ? 1 : tiles, step = nt * (BM / G), keys = hd > 128 ? 64 : 128;
   Slots parts{0, 0, 0, 1, 1};
   CUtensorMap maps[3];
@@ -966,16 +982,18 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
     if (e != cudaSuccess || most <= 1) return (int)e;
     return (int)join_go<bf16>(stream, qb, kb, vb, ob, part_o, ml, nullptr, s, parts, 1);
   }
-  JB_REFUSE(shared_per == 0 && prefix_len > 0, "attention_prefix: nothing walks the prefix");
-  const int row_blocks = (max_q_len * G + 15) / 16, tiles_most = (max_kv_len - prefix_len + OWN_KEYS - 1) / OWN_KEYS;
+  // where nobody walks the prefix for all, every sequence's rows walk it with their own keys
+  const int shared = shared_per > 0 ? 0 : (prefix_len + OWN_KEYS - 1) / OWN_KEYS;
+  const int row_blocks = (max_q_len * G + 15) / 16;
+  const int own_tiles_most = (max_kv_len - prefix_len + OWN_KEYS - 1) / OWN_KEYS, tiles_most = shared + (own_tiles_most < 1 ? 1 : own_tiles_most);
   JB_REFUSE(own_ctas < 1 || fewest < 1 || own_most > 64 || (tiles_most + fewest - 2) / fewest + 1 > own_most ||
                 (long long)n_seqs * nkv * row_blocks * (tiles_most < 1 ? 1 : tiles_most) > 0x3fffffffll,
             "attention_prefix: %d blocks for %d tiles of own keys of %d sequences", own_ctas, tiles_most, n_seqs);
   if (!make_maps(nullptr, &maps[1], &maps[2], q, k_cache, v_cache, s, n_pages, OWN_KEYS)) return JB_ERR_TENSORMAP;
   const int behind = shared_per > 0;
-  if (hd > 128) e = own_go<256, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, fewest, status);
-  else if (hd > 64) e = own_go<128, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, fewest, status);
-  else e = own_go<64, 2>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, fewest, status);
+  if (hd > 128) e = own_go<256, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, shared, fewest, status);
+  else if (hd > 64) e = own_go<128, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, shared, fewest, status);
+  else e = own_go<64, 2>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, shared, fewest, status);
   if (e != cudaSuccess) return (int)e;
   return (int)join_go<bf16>(stream, qb, kb, vb, ob, part_o, ml, own_count, s, parts, 0);
 }

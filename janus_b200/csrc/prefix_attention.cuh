@@ -13,6 +13,14 @@ typedef __nv_bfloat16 bf16;
 constexpr int PAGE = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 
+// The sizes of a call and how it runs, as the caller hands them over (in one piece: passing them one by one cost the host more than a
+// launch).  bfloat16: see jb_attention_prefix_bf16.  float32: `tiles` and `shared_per` are the rows of a block over the prefix and over
+// own keys, `most` and `own_most` the ranges of both.
+struct Sizes {
+  int prefix_len, ld_table, width, T, n_pages, n_seqs, nh, nkv, hd, page_size, max_q_len, max_kv_len;
+  int tiles, shared_per, most, own_tiles, own_ctas, fewest, own_most;
+  float scale;
+};
 // What every kernel of a call knows.
 struct Step {
   const int* prefix_pages;

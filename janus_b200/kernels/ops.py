@@ -91,8 +91,7 @@ _SIGNATURES = {
     "jb_activate": "ppilip", "jb_tanh_norm": "ppppffippfpipiiplplp",
     "jb_latent_heads": "piiiiiipppiiiipfpppip", "jb_latent_queries": "piiiiiiippppiiipfppip", "jb_latent_values": "pppippiipiiiiiip",
     "jb_latent_down": "piipfpiippiiippppplip",
-    "jb_step_tables": "ppppppppppppppppppiiiiiiiip", "jb_attention_prefix_f32": "pppppppipiipppiiiiiifiiiiip",
-    "jb_attention_prefix_bf16": "ppppppppipiipppiiiiiiifiiiiiiiiipp",
+    "jb_step_tables": "ppppppppppppppppppiiiiiiiip", "jb_attention_prefix_f32": "pppppppppppp", "jb_attention_prefix_bf16": "ppppppppppppp",
     "jb_verify_drafts": "ppppppppppppiiiifp",
     "jb_gather_rows": "ppiipppiiip", "jb_latent_attention": "ppppppppiiiiiiifiipp", "jb_attention_tc_matrix": "ppppppiiiiiiiifpipp",
 }
@@ -2480,35 +2479,47 @@ def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise KernelError(f"attention_prefix: {prefix_pages.shape[0]} pages do not hold a prefix of {prefix_len} tokens")
     if max_q_len < 0 or block_table.shape[1] * page_size < max_kv_len - prefix_len:
         raise KernelError(f"attention_prefix: {block_table.shape[1]} pages a sequence do not hold {max_kv_len} tokens behind {prefix_len}")
-    wide = block_table.shape[1]
-    step = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr())
-    rest = (prefix_pages.data_ptr(), prefix_len, block_table.data_ptr(), block_table.stride(0), wide, q_start.data_ptr(), kv_len.data_ptr(),
-            positions.data_ptr(), T)
-    if q.dtype == torch.float32:
-        rows, own_rows, splits, own_slots = attention_prefix_plan_f32(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv)
-        slots = splits + own_slots
+    sizes, floats, kernels = _attention_prefix_sizes(
+        prefix_len, block_table.stride(0), block_table.shape[1], T, k_cache.shape[0], n_seqs, nh, nkv, hd, page_size, int(max_q_len),
+        int(max_kv_len), float(scale), q.dtype is torch.float32)
+    args = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+            workspace.get("prefix_parts", (floats,), torch.float32).data_ptr(), prefix_pages.data_ptr(), block_table.data_ptr(),
+            q_start.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), ctypes.addressof(sizes))
+    if q.dtype is torch.float32:
+        _check(_lib("prefix_attention_f32").jb_attention_prefix_f32(*args, _stream()), "attention_prefix", kernels=kernels)
     else:
-        tiles, per, splits, own_tiles, own_ctas, fewest, own_slots = attention_prefix_plan(
-            T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv, hd)
-        slots = splits + own_slots
-    part_o = part_ml = own_count = None
-    if slots:
-        part_o = workspace.get("prefix_part_o", (slots * T * nh * hd,), torch.float32)
-        part_ml = workspace.get("prefix_part_ml", (slots * T * nh * 2,), torch.float32)
-    if q.dtype == torch.float32:
-        _check(_lib("prefix_attention_f32").jb_attention_prefix_f32(
-            *step, _ptr(part_o), _ptr(part_ml), *rest, n_seqs, nh, nkv, hd, page_size, float(scale), int(max_q_len), rows, own_rows,
-            splits, own_slots, _stream()), "attention_prefix", kernels=1 if hd % 4 else (splits > 0) + 2)
-        return
-    if own_ctas:
-        own_count = workspace.get("prefix_own_count", (T * nkv,), torch.int32).data_ptr()
-    _check(_lib("prefix_attention").jb_attention_prefix_bf16(
-        *step, _ptr(part_o), _ptr(part_ml), own_count, *rest, k_cache.shape[0], n_seqs, nh, nkv, hd, page_size, float(scale),
-        int(max_q_len), int(max_kv_len), tiles, per, splits, own_tiles, own_ctas, fewest, own_slots, _ptr(kernel_status(q.device)),
-        _stream()), "attention_prefix", kernels=(per > 0) + 1 + (own_slots > 0))
+        _check(_lib("prefix_attention").jb_attention_prefix_bf16(*args, kernel_status(q.device).data_ptr(), _stream()), "attention_prefix",
+               kernels=kernels)
+
+
+class _PrefixSizes(ctypes.Structure):
+    """`Sizes` of csrc/prefix_attention.cuh."""
+    _fields_ = [(n, ctypes.c_int) for n in (
+        "prefix_len", "ld_table", "width", "T", "n_pages", "n_seqs", "nh", "nkv", "hd", "page_size", "max_q_len", "max_kv_len",
+        "tiles", "shared_per", "most", "own_tiles", "own_ctas", "fewest", "own_most")] + [("scale", ctypes.c_float)]
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_prefix_sizes(prefix_len: int, ld_table: int, width: int, T: int, n_pages: int, n_seqs: int, nh: int, nkv: int, hd: int,
+                            page_size: int, max_q_len: int, max_kv_len: int, scale: float, f32: bool):
+    """(the call's sizes and plan as the C function takes them, its scratch in floats, its launches)."""
+    if f32:
+        rows, own_rows, most, own_most = attention_prefix_plan_f32(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv)
+        plan = (rows, own_rows, most, 0, 0, 0, own_most)
+        kernels = 1 if hd % 4 else (most > 0) + 2
+    else:
+        plan = attention_prefix_plan(T, n_seqs, max_q_len, prefix_len, max_kv_len - prefix_len, nh, nkv, hd)
+        kernels = (plan[1] > 0) + 1 + (plan[6] > 0)
+    slots = plan[2] + plan[6]
+    return (_PrefixSizes(prefix_len, ld_table, width, T, n_pages, n_seqs, nh, nkv, hd, page_size, max_q_len, max_kv_len, *plan, scale),
+            slots * T * nh * (hd + 2) + T * nkv, kernels)
 
 
 _PREFIX_MOST_RANGES = 64       # partial results over the prefix that a row's join takes
+# Tiles of 32 keys of all rows together, from which the prefix has a launch of its own.  A warp takes 2 us a tile, one after another, a
+# launch costs the host 2.5: 384 tiles (4 sequences behind 173 tokens) 6.8 us together and 8.6 apart, 1,184 (behind 1,000) 10.9 and
+# 9.5, 1,920 13.3 and 11.5.
+_PREFIX_APART_FROM = 1200
 
 
 def _prefix_ranges(total: int, blocks: int, most_ctas: int):
@@ -2545,11 +2556,16 @@ def attention_prefix_plan(T: int, n_seqs: int, max_q_len: int, prefix_len: int, 
             return tiles, 0, 0, 1, 0, 0, 0
         per, ranges = (uncut, 1) if uncut <= 1.1 * even else _prefix_ranges(items * blocks, blocks, sms)
         return tiles, per, ranges, 1, 0, 0, 1 if ranges > 1 else 0
+    row_blocks = n_seqs * nkv * ((max_q_len * group + 15) // 16)
+    own_blocks = max(1, (max_own + 31) // 32)
+    # few rows behind a short prefix: they walk it themselves, a launch less
+    tiles = (prefix_len + 31) // 32 + own_blocks
+    if row_blocks * tiles <= _PREFIX_APART_FROM and tiles <= 60:
+        return 1, 0, 0, 0, max(1, min((3 if hd <= 128 else 1) * sms, -(-row_blocks * tiles // 4))), 1, tiles
     # one tile a block over the prefix: with two a block, its keys are fetched once for both, but the own keys' blocks then find no
     # room beside it (64 single tokens behind 8,192: 31 us and 40)
     per, ranges = _prefix_ranges(-(-T // rows) * nkv * blocks, blocks, sms) if prefix_len else (0, 0)
-    own_blocks = max(1, (max_own + 31) // 32)
-    places = n_seqs * nkv * ((max_q_len * group + 15) // 16) * own_blocks
+    places = row_blocks * own_blocks
     fewest = max(1, min(4, places // (8 * sms)), -(-own_blocks // 30))
     own_ctas = max(1, min((3 if hd <= 128 else 1) * sms, -(-places // (4 * fewest))))
     return 1, per, ranges, 0, own_ctas, fewest, (own_blocks + fewest - 2) // fewest + 1

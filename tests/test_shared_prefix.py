@@ -530,7 +530,6 @@ def test_plans_cover_what_they_cut():
         tiles, per, ranges, own_tiles, own_ctas, fewest, own_most = ops.attention_prefix_plan(T, n, q, prefix, own, group * nkv, nkv, hd)
         assert 0 <= ranges <= 64 and own_most <= 64 and (own_tiles or own_ctas >= 1)
         if not per:
-            assert own_tiles
             continue
         keys = 64 if hd > 128 else 128
         blocks, step = -(-prefix // keys), 128 // group * tiles
