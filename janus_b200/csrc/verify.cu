@@ -244,7 +244,8 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
                                                          int T, float heat, float heat_log2, int vectors) {
   extern __shared__ float dyn[];
   float* chunk_sum = dyn;                                   // [chunks] masses of the drawn row's chunks
-  float* row_top = chunk_sum + chunks;                      // [width] of the request's rows
+  float* warp_sums = chunk_sum + chunks;                    // [chunks][WARPS] ... of their warps' parts
+  float* row_top = warp_sums + chunks * WARPS;              // [width] of the request's rows
   float* row_sum = row_top + width;                         // [width]
   int* row_arg = reinterpret_cast<int*>(row_sum + width);   // [width]
   int* row_yes = row_arg + width;                           // [width] the draft behind the row is accepted
@@ -255,13 +256,14 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   jb::pdl_wait();
   jb::pdl_launch_dependents();
-  const int lo = min(max(q_start[b], 0), T), hi = min(max(q_start[b + 1], lo), T), rows = min(hi - lo, width);
+  const int lo = min(max(q_start[b], 0), T), hi = min(max(q_start[b + 1], lo), T), rows = min(hi - lo, width), cached = kv_len[b];
+  const float u_token = u_draw[b];
   int* my = out + (size_t)b * width;
   float* lp = logprobs + (size_t)b * width;
   if (rows == 0) {   // (the whole cluster)
     if (rank == 0) {
       for (int k = tid; k < width; k += THREADS) my[k] = -1, lp[k] = 0.0f;
-      if (tid == 0) accepted_out[b] = 0, kept[b] = kv_len[b];
+      if (tid == 0) accepted_out[b] = 0, kept[b] = cached;
     }
     return;
   }
@@ -270,6 +272,11 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
     const Chunk* c = stats + (size_t)(lo + r) * chunks;
     float top = -CUDART_INF_F, sum = 0.0f;
     int arg = 0x7fffffff;
+    // (the draft and what is known of it, on its way beside the chunks')
+    const int t = lo + r + 1, d = r + 1 < rows ? tokens[t] : -1;
+    const bool there = d >= 0 && d < V;
+    const float x = there ? logits[(size_t)(lo + r) * V + d] : 0.0f;
+    const float q = there && probs && heat > 0.0f ? probs[(size_t)t * V + d] : 1.0f, u = there ? u_accept[t] : 1.0f;
     for (int i = lane; i < chunks; i += 32) keep_first(top, arg, c[i].top, c[i].arg);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -281,20 +288,7 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
     sum = jb::warp_sum(sum);
     if (arg == 0x7fffffff) arg = 0;
     if (lane == 0) {
-      bool yes = false;
-      float x = 0.0f;
-      if (r + 1 < rows) {
-        const int t = lo + r + 1, d = tokens[t];
-        if (d >= 0 && d < V) {
-          x = logits[(size_t)(lo + r) * V + d];
-          if (heat > 0.0f) {
-            const float q = probs ? probs[(size_t)t * V + d] : 1.0f;
-            yes = u_accept[t] * q * sum < weight(x, top, heat_log2);
-          } else {
-            yes = d == arg;
-          }
-        }
-      }
+      const bool yes = there && (heat > 0.0f ? u * q * sum < weight(x, top, heat_log2) : d == arg);
       row_top[r] = top, row_sum[r] = sum, row_arg[r] = arg, row_yes[r] = yes, row_x[r] = x;
     }
   }
@@ -325,10 +319,17 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
     // the chunks' masses, known to every block
     if (draw.form == REFUSED) {
       if (size > 1) cluster_sync();   // every block is there to be written to
+      // (the warps do not wait for one another before the last chunk)
       for (int i = c_begin; i < c_end; ++i) {
-        const float all = chunk_mass(i);
-        if (size == 1 && tid == 0) chunk_sum[i] = all;
-        if (size > 1 && tid < size) store_remote(in_block(chunk_sum + i, tid), all);
+        const float mine = warp_masses(draw, i, vectors, w, run_end);
+        if (lane == 0) warp_sums[i * WARPS + warp] = mine;
+      }
+      __syncthreads();
+      for (int i = c_begin + warp; i < c_end; i += WARPS) {
+        float start, all;
+        first_past(warp_sums + i * WARPS, WARPS, 0.0f, 0.0f, start, all);
+        if (size == 1 && lane == 0) chunk_sum[i] = all;
+        if (size > 1 && lane < size) store_remote(in_block(chunk_sum + i, lane), all);
       }
       if (size > 1) cluster_sync();
     }
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
       __syncthreads();
     }
     // the chunk where the drawn number falls
-    const float target = u_draw[b] * total;
+    const float target = u_token * total;
     const int pick = first_past(chunk_sum, chunks, 0.0f, target, before, total);
     if (pick >= 0) {
       writer = 0;
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
       }
       my[k] = v, lp[k] = p;
     }
-    if (tid == 0) accepted_out[b] = accepted, kept[b] = kv_len[b] - (hi - lo - 1) + accepted;
+    if (tid == 0) accepted_out[b] = accepted, kept[b] = cached - (hi - lo - 1) + accepted;
   }
 }
 
@@ -406,7 +407,7 @@ JB_EXPORT int jb_verify_drafts(const float* logits, const int* tokens, const int
   if (B <= 0) return 0;
   JB_REFUSE(V <= 0 || width <= 0 || T < 0, "verify_drafts: %d rows of %d logits, %d tokens a request", T, V, width);
   const int chunks = (V + CHUNK - 1) / CHUNK;
-  const size_t smem = ((size_t)chunks + 5 * (size_t)width) * sizeof(float);
+  const size_t smem = ((size_t)chunks * (1 + WARPS) + 5 * (size_t)width) * sizeof(float);
   JB_REFUSE(smem > 48 * 1024, "verify_drafts: %d tokens a request over a vocabulary of %d", width, V);
   JB_REFUSE((long long)T * chunks > 0x7fffffffll || (long long)B * MAX_CLUSTER > 0x7fffffffll, "verify_drafts: %d rows of %d logits", T, V);
   const float heat_log2 = heat > 0.0f ? fminf(LOG2E / heat, 1e30f) : LOG2E;   // (finite: 0 times it is 0)
@@ -418,9 +419,9 @@ JB_EXPORT int jb_verify_drafts(const float* logits, const int* tokens, const int
                                               : (vectors ? stats_kernel<true, true> : stats_kernel<false, true>), logits, (Chunk*)stats, V, chunks, heat_log2);
     if (e != cudaSuccess) return (int)e;
   }
-  // Blocks a request: as many as run at once (two a multiprocessor).  A block more takes its share of a row's chunks, but makes all of the
-  // request's decisions too: 256 requests by eight blocks each took 94 us, where one wave of single blocks has no such repetition.
-  int size = 2 * 148 / B;
+  // Blocks a request: as many as run at once (two a multiprocessor), twice.  A block more takes its share of a row's chunks, but makes all
+  // of the request's decisions too: 256 requests took 94 us by eight blocks each, 66 by one, whose sixteen chunks follow one another.
+  int size = 4 * 148 / B;
   size = size < 1 ? 1 : size > MAX_CLUSTER ? MAX_CLUSTER : size;
   if (size > chunks) size = chunks;
   cudaLaunchAttribute attr[2];
