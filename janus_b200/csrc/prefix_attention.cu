@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
       } else {
         // the one part over the prefix weighs in (OWN)
         const int slots = FORM == OWN && valid ? parts.most : 0;
-        if (FORM == OWN && parts.most > 0) jb::pdl_wait();
+        if (FORM == OWN) jb::pdl_wait();
         float top = m_ref;
         for (int i = 0; i < slots; ++i) top = fmaxf(top, part_ml[i * all + place].x);
         const float ref = top == -CUDART_INF_F ? 0.0f : top, own_weight = exp2f(m_ref - ref);
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
     }
     jb::tc_fence_before();
   }
-  if (FORM == OWN && parts.most > 0) jb::pdl_wait();   // (every thread, before the kernel ends)
+  if (FORM == OWN && (parts.most == 1 || blockIdx.x + blockIdx.y == 0)) jb::pdl_wait();   // (see own_kernel's end)
   __syncthreads();
   if (warp == 1) {
     jb::tc_fence_after();
@@ -844,7 +844,9 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
     }
     if (i + 1 < end) step_on(s, c);
   }
-  if (after_prefix) jb::pdl_wait();   // (so that who waits for this launch has waited for the one before it)
+  // Who waits for this launch has to have waited for the one before it: one block sees to that.  (All of them waiting held their places
+  // on the multiprocessors until the prefix was done, and the blocks behind them had none: 256 long sequences 144 us.)
+  if (after_prefix && blockIdx.x == 0) jb::pdl_wait();
 }
 
 // ---------------------------------------------------------------------------

@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(THREADS, (Tile<HDC, RR>::BLOCKS)) tile_f32_ker
     *reinterpret_cast<float4*>(part_o + item * hd + d) = *reinterpret_cast<const float4*>(red_o + r * C::LD + d);
     if (d == 0) part_ml[item] = make_float2(red_ml[2 * r], red_ml[2 * r + 1]);
   }
-  if (OWN && prefix_slots > 0) jb::pdl_wait();   // (so that who waits for this launch has waited for the one before it)
+  // (who waits for this launch has to have waited for the one before it: one block sees to that)
+  if (OWN && prefix_slots > 0 && blockIdx.x + blockIdx.y + blockIdx.z == 0) jb::pdl_wait();
 }
 
 template <int HDC, int RR, bool OWN>
