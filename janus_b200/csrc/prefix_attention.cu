@@ -283,11 +283,11 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
     if constexpr (FORM == SHARED) {
       const int item = at / parts.blocks;
       g.block0 = at - item * parts.blocks;
-      g.nb = g.n_shared = min(parts.blocks - g.block0, flat_end - at);
+      g.nb = g.n_shared = min((s.prefix_len + KB - 1) / KB - g.block0, flat_end - at);
       g.kvh = item % s.nkv, g.tok0 = item / s.nkv * NT * tpt;
       g.n_tok = min(NT * tpt, total_tokens - g.tok0);
       g.slot = blockIdx.x - item * parts.blocks / parts.per;
-      at += g.nb;
+      at += min(parts.blocks - g.block0, flat_end - at);
     } else {
       const int q_len = seq < 0 ? 0 : s.q_start[seq + 1] - seq_start, first = found[1] * NT * tpt;
       g.kvh = blockIdx.x, g.tok0 = seq_start + first, g.n_tok = min(NT * tpt, q_len - first), g.block0 = 0, g.slot = 0;
@@ -966,8 +966,13 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
   if ((shared_per > 0 || own_tiles) && !make_maps(&maps[0], &maps[1], &maps[2], q, k_cache, v_cache, s, n_pages, PAGE)) return JB_ERR_TENSORMAP;
   cudaError_t e = cudaSuccess;
   if (shared_per > 0) {
-    const int blocks = (prefix_len + keys - 1) / keys;
-    const long long total = (long long)((T + step - 1) / step) * nkv * blocks, ctas = (total + shared_per - 1) / shared_per;
+    int blocks = (prefix_len + keys - 1) / keys;
+    const long long items = (long long)((T + step - 1) / step) * nkv;
+    // A tile's last range may be shorter than the others, where all of them still run at once: a block that goes from one tile to the
+    // next in its range pays queries, result and the start of its products twice.
+    const int even = (blocks + shared_per - 1) / shared_per;
+    if (shared_per < blocks && items * even <= SMS) blocks = even * shared_per;
+    const long long total = items * blocks, ctas = (total + shared_per - 1) / shared_per;
     // a tile's blocks begin anywhere in a range, unless ranges divide them, or are whole tiles
     JB_REFUSE(total > 0x3fffffffll, "attention_prefix: %lld key blocks", total);
     JB_REFUSE((shared_per % blocks == 0 ? 1 : blocks % shared_per == 0 ? blocks / shared_per : (blocks + shared_per - 2) / shared_per + 1) > most,

@@ -11,6 +11,7 @@ namespace {
 typedef __nv_bfloat16 bf16;
 
 constexpr int PAGE = 64;
+constexpr int SMS = 148;                 // multiprocessors
 constexpr float LOG2E = 1.4426950408889634f;
 
 // The sizes of a call and how it runs, as the caller hands them over (in one piece: passing them one by one cost the host more than a
@@ -207,7 +208,7 @@ cudaError_t join_as(cudaStream_t stream, const E* q, const E* k, const E* v, E* 
 template <typename E>
 cudaError_t join_go(cudaStream_t stream, const E* q, const E* k, const E* v, E* out, const float* part_o, const float2* part_ml,
                     const int* own_count, const Step& s, const Slots& parts, int own_slots) {
-  return (long long)s.T * s.nh <= 148 * 16 ? join_as<E, 4>(stream, q, k, v, out, part_o, part_ml, own_count, s, parts, own_slots)
+  return (long long)s.T * s.nh <= SMS * 16 ? join_as<E, 4>(stream, q, k, v, out, part_o, part_ml, own_count, s, parts, own_slots)
                                            : join_as<E, 1>(stream, q, k, v, out, part_o, part_ml, own_count, s, parts, own_slots);
 }
 

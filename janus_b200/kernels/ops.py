@@ -2522,10 +2522,17 @@ _PREFIX_MOST_RANGES = 64       # partial results over the prefix that a row's jo
 _PREFIX_APART_FROM = 1200
 
 
-def _prefix_ranges(total: int, blocks: int, most_ctas: int):
-    """(length of equal ranges for at most `most_ctas` blocks of `total` places, the most of them that `blocks` consecutive places from a
-    multiple of it on are in)."""
-    per = max(-(-total // most_ctas), -(-blocks // (_PREFIX_MOST_RANGES - 2)))
+def _prefix_ranges(items: int, blocks: int, most_ctas: int, hd: int):
+    """(key blocks of a range for at most `most_ctas` blocks over `items` tiles of `blocks` key blocks, the most ranges that a tile can be
+    in).  Every tile is cut by itself where that makes ranges no more than four key blocks longer (two, with heads of 64 numbers, whose
+    results are half as large): a block that goes from one tile to the next has queries, result and the start of its products twice (64
+    sequences behind 8,192: 36 us by ranges of 7, 30 of 8, which cut tiles evenly; 132 tokens behind 6,001, heads of 64: 29 by 13, 31 by
+    16; heads of 128: 36 and 34)."""
+    per = -(-items * blocks // most_ctas)
+    if items <= most_ctas:
+        alone = -(-blocks // (most_ctas // items))
+        per = alone if alone <= per + (4 if hd > 64 else 2) else per
+    per = max(per, -(-blocks // (_PREFIX_MOST_RANGES - 2)))
     return per, 1 if per % blocks == 0 else blocks // per if blocks % per == 0 else (blocks + per - 2) // per + 1
 
 
@@ -2554,7 +2561,7 @@ def attention_prefix_plan(T: int, n_seqs: int, max_q_len: int, prefix_len: int, 
         apart = min(even * 1.1, uncut) * block_us + waves * own_blocks * block_us + 12 + T * nh * hd * 8 / 4e6
         if whole <= apart:
             return tiles, 0, 0, 1, 0, 0, 0
-        per, ranges = (uncut, 1) if uncut <= 1.1 * even else _prefix_ranges(items * blocks, blocks, sms)
+        per, ranges = (uncut, 1) if uncut <= 1.1 * even else _prefix_ranges(items, blocks, sms, hd)
         return tiles, per, ranges, 1, 0, 0, 1 if ranges > 1 else 0
     row_blocks = n_seqs * nkv * ((max_q_len * group + 15) // 16)
     own_blocks = max(1, (max_own + 31) // 32)
@@ -2562,13 +2569,19 @@ def attention_prefix_plan(T: int, n_seqs: int, max_q_len: int, prefix_len: int, 
     tiles = (prefix_len + 31) // 32 + own_blocks
     if row_blocks * tiles <= _PREFIX_APART_FROM and tiles <= 60:
         return 1, 0, 0, 0, max(1, min((3 if hd <= 128 else 1) * sms, -(-row_blocks * tiles // 4))), 1, tiles
-    # one tile a block over the prefix: with two a block, its keys are fetched once for both, but the own keys' blocks then find no
-    # room beside it (64 single tokens behind 8,192: 31 us and 40)
-    per, ranges = _prefix_ranges(-(-T // rows) * nkv * blocks, blocks, sms) if prefix_len else (0, 0)
+    # Own keys' mean length is not known: a third of the longest.  Where they take 4 us or more, the prefix leaves 20 multiprocessors to
+    # them (72 sequences behind 2,036: 29 and 24 us).  One tile a block over the prefix: with two its keys are fetched once for both, but
+    # the own keys' blocks find no room beside it (64 single tokens behind 8,192: 30 us and 36).  Two, on two thirds of the
+    # multiprocessors, where both are long: products bound the one, memory the other (256 sequences behind 16,384: 132 and 121 us).
+    own_us, items, pairs = n_seqs * nkv * hd * max_own * 4 / 3 / 5.2e6, -(-T // rows) * nkv, -(-T // (2 * rows)) * nkv
+    tiles = 2 if hd <= 128 and own_us > pairs * blocks * 1.8 / sms > 35 else 1
+    per, ranges = 0, 0
+    if prefix_len:
+        per, ranges = _prefix_ranges(*((pairs, blocks, 100) if tiles == 2 else (items, blocks, 128 if own_us > 4 else sms)), hd)
     places = row_blocks * own_blocks
     fewest = max(1, min(4, places // (8 * sms)), -(-own_blocks // 30))
     own_ctas = max(1, min((3 if hd <= 128 else 1) * sms, -(-places // (4 * fewest))))
-    return 1, per, ranges, 0, own_ctas, fewest, (own_blocks + fewest - 2) // fewest + 1
+    return tiles, per, ranges, 0, own_ctas, fewest, (own_blocks + fewest - 2) // fewest + 1
 
 
 @functools.lru_cache(maxsize=4096)
