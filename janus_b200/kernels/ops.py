@@ -2590,10 +2590,14 @@ def attention_prefix_plan_f32(T: int, n_seqs: int, max_q_len: int, prefix_len: i
     `attention_prefix`."""
     group, sms = nh // nkv, SM_COUNT_TARGET // 2
     rows, own_rows = (16 if n * group <= 32 else 64 for n in (T, max_q_len))
-    pages = (prefix_len + 63) // 64
-    splits = min(64, pages, max(1, 2 * sms // (nkv * ((T * group + rows - 1) // rows)))) if prefix_len else 0    # two blocks an SM
-    ctas = n_seqs * nkv * ((max_q_len * group + own_rows - 1) // own_rows)
-    return rows, own_rows, splits, min(32, max(1, (max_own + 127) // 128), max(1, 2 * sms // max(1, ctas)))
+    pages, own_pages, splits = (prefix_len + 63) // 64, (max_own + 63) // 64, 0
+    if prefix_len:                                                           # two blocks an SM, of as many pages each
+        splits = min(64, pages, max(1, 2 * sms // (nkv * ((T * group + rows - 1) // rows))))
+        splits = -(-pages // -(-pages // splits))
+    # A block loads a page, then works on it: short ranges of own pages, several of which share an SM (29 tokens of 16 sequences
+    # with up to 254 own tokens behind 2,050: 47 us by two ranges, 41 by four; 40 single tokens with 556 behind 3,000: 164 by one, 131
+    # by five; by nine of one page 139).
+    return rows, own_rows, splits, min(32, max(1, min(own_pages, 4), (own_pages + 1) // 2))
 
 
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, accepted: torch.Tensor,
