@@ -84,6 +84,16 @@ __device__ __forceinline__ float fast_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The same by multiply-adds: 2^f for |f| <= 1/2 by the cubic with value 1 at 0 and the least greatest relative error (1.0e-4, a
+// twentieth of the rounding to bfloat16 that follows), the whole part added to the exponent's bits.  Anything to -127 gives 0 (a masked
+// key's -inf must: a stale value may lie behind it), NaN a result that rounds to infinity, for which the row is made anew.
+__device__ __forceinline__ float poly_exp2(float x) {
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(-127.0f));
+  const float t = x + 12582912.0f;   // 1.5 x 2^23: the whole part in the low bits
+  const float f = x - (t - 12582912.0f);
+  const float p = fmaf(fmaf(fmaf(0.05500893f, f, 0.24221096f), f, 0.69328293f), f, 1.0f);
+  return __int_as_float(__float_as_int(p) + (__float_as_int(t) << 23));
+}
 // MN-major operand (values: a 128-byte row holds 64 consecutive numbers of one key, 8 keys a 1,024-byte atom): the leading
 // offset is the distance of the next 64 numbers, the stride offset that of the next 8 keys.
 __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t lead, uint32_t stride) {
@@ -113,15 +123,18 @@ __device__ __forceinline__ jb::Pair add2(jb::Pair a, jb::Pair b) {
   return d;
 }
 // p[c] = 2^(s[c] scale + neg_ref) for N scores in sr; bfloat16 pairs over the first N / 2 words; returns their float32 sum.
-// (Three of eight by a polynomial instead of the special-function unit changed nothing for one tile a block, and spilled with two.)
-template <int N>
+// POLY: one of eight by multiply-adds, while the special-function unit makes the others: with two tiles a block, each's weights are what
+// the other's products wait for (8 prompts of up to 510 tokens behind 4,100: 104 and 100 us; one of four 103, and with more
+// registers spill).  With one tile a block it changes nothing.
+template <int N, bool POLY>
 __device__ __forceinline__ float exp_pack_sum(uint32_t* sr, float scale_log2, float neg_ref) {
   const jb::Pair s2 = jb::pair(scale_log2, scale_log2), n2 = jb::pair(neg_ref, neg_ref);
   jb::Pair acc[4] = {0ull, 0ull, 0ull, 0ull};   // the bit pattern of (0.0f, 0.0f)
 #pragma unroll
   for (int c = 0; c < N / 2; ++c) {
     const jb::Pair x = jb::fma2(jb::pair(__uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1])), s2, n2);
-    const float p0 = fast_exp2(jb::lo(x)), p1 = fast_exp2(jb::hi(x));
+    const bool poly = POLY && c % 8 == 7;
+    const float p0 = poly ? poly_exp2(jb::lo(x)) : fast_exp2(jb::lo(x)), p1 = poly ? poly_exp2(jb::hi(x)) : fast_exp2(jb::hi(x));
     acc[c & 3] = add2(acc[c & 3], jb::pair(p0, p1));
     sr[c] = pack_bf16(p0, p1);
   }
@@ -133,10 +146,11 @@ template <int HDC, int NT, int KB>
 struct Tc {
   static constexpr int SLABS = HDC / 64;                       // 64-number slabs of a row
   static constexpr int Q_BYTES = SLABS * BM * 128, KV_BYTES = SLABS * KB * 128;
-  static constexpr int BARS = 1 + 8 + 2 * 2 + 3 * NT;          // q_full; k, v full and empty x 2; s_full, p_full x 2; o_full, o_done, o_free
+  static constexpr int BARS = 1 + 8 + 3 * 2 + 3 * NT;          // q_full; k, v full and empty x 2; s_full, p_half, p_full x 2; o_full, o_done, o_free
   static constexpr int SWAP = NT * 2 * BM;                     // floats: what the two halves of a row tell each other
   static constexpr int SMEM = NT * Q_BYTES + 4 * KV_BYTES + SWAP * 4 + NT * 4 * 4 + 8 + BARS * 8 + 16;
   static constexpr int THREADS = 64 + NT * 256;
+  static constexpr int CHUNKS = KB / 64;                       // in which a block's weights are handed on
   // (one tile of up to 128 numbers a row: 96 registers a thread, as 576 threads have, so that a block of own_kernel finds registers
   // beside this one; rows of up to 64 leave enough anyway)
   static constexpr int BOUND = HDC == 128 ? 576 : THREADS;
@@ -201,11 +215,12 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
   const uint32_t bar0 = jb::smem_u32(bars);
   const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 24, v_full = bar0 + 40, v_empty = bar0 + 56;
   // an S buffer belongs to a tile (NT = 2), or to the even or odd blocks of the one tile
-  auto s_full = [&](int b) { return bar0 + 72 + 16 * b; };
-  auto p_full = [&](int b) { return bar0 + 80 + 16 * b; };
-  auto o_full = [&](int w) { return bar0 + 104 + 24 * w; };   // a block's product has landed in O
-  auto o_done = [&](int w) { return bar0 + 112 + 24 * w; };   // ... the last block's of a segment
-  auto o_free = [&](int w) { return bar0 + 120 + 24 * w; };   // O has been read and may be begun anew
+  auto s_full = [&](int b) { return bar0 + 72 + 24 * b; };
+  auto p_half = [&](int b) { return bar0 + 80 + 24 * b; };
+  auto p_full = [&](int b) { return bar0 + 88 + 24 * b; };
+  auto o_full = [&](int w) { return bar0 + 120 + 24 * w; };   // a block's product has landed in O
+  auto o_done = [&](int w) { return bar0 + 128 + 24 * w; };   // ... the last block's of a segment
+  auto o_free = [&](int w) { return bar0 + 136 + 24 * w; };   // O has been read and may be begun anew
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     jb::mbar_init(q_full, 1);
@@ -215,6 +230,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
       jb::mbar_init(v_full + 8 * i, 1);
       jb::mbar_init(v_empty + 8 * i, 1);
       jb::mbar_init(s_full(i), 1);
+      jb::mbar_init(p_half(i), 8);
       jb::mbar_init(p_full(i), 8);      // an arrival a warp: one a thread would be 256 operations on one word
     }
     for (int w = 0; w < NT; ++w) {
@@ -377,15 +393,21 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
         }
         for (int w = 0; w < NT && ok; ++w) {
           const int b = NT == 2 ? w : it & 1;
-          ok = mbar_wait(p_full(b), (NT == 2 ? it : it >> 1) & 1, status, 42);
-          if (ok && w == 0) ok = mbar_wait(v_full + 8 * st, (it >> 1) & 1, status, 42);
+          if (w == 0) ok = mbar_wait(v_full + 8 * st, (it >> 1) & 1, status, 42);
           if (ok && j == 0 && turn > 0) ok = mbar_wait(o_free(w), (turn - 1) & 1, status, 42);
-          if (!ok) break;
-          jb::tc_fence_after();
 #pragma unroll
-          for (int ks = 0; ks < KB / 16; ++ks)
-            umma_ts(tmem + 2 * KB + w * HDC, tmem + b * KB + ks * 8, desc_mn_sw128(v_s + st * C::KV_BYTES + ks * 2048, KB * 128, 1024),
-                    idesc_o, (j | ks) ? 1u : 0u);
+          for (int c = 0; c < C::CHUNKS && ok; ++c) {
+            ok = mbar_wait(c < C::CHUNKS - 1 ? p_half(b) : p_full(b), (NT == 2 ? it : it >> 1) & 1, status, 42);
+            if (!ok) break;
+            jb::tc_fence_after();
+#pragma unroll
+            for (int k2 = 0; k2 < 4; ++k2) {                    // 32 keys of each of a block's halves (with 64 keys a block: all)
+              const int ks = (k2 >> 1) * (KB / 32) + c * 2 + (k2 & 1);
+              umma_ts(tmem + 2 * KB + w * HDC, tmem + b * KB + ks * 8, desc_mn_sw128(v_s + st * C::KV_BYTES + ks * 2048, KB * 128, 1024),
+                      idesc_o, (j | ks) ? 1u : 0u);
+            }
+          }
+          if (!ok) break;
           jb::umma_commit(o_full(w));
           if (last) jb::umma_commit(o_done(w));
           if (w == NT - 1) jb::umma_commit(v_empty + 8 * st);
@@ -479,13 +501,16 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
           }
           m_ref = m_new;
         }
-        l += exp_pack_sum<KH>(sr, s.scale_log2, m_ref == -CUDART_INF_F ? 0.0f : -m_ref);
+        // 32 keys of each half at a time: the product with the first ones' values runs while the others' weights are made
 #pragma unroll
-        for (int c0 = 0; c0 < KH / 2; c0 += 16) tmem_st16(s_at + half * (KH / 2) + c0, sr + c0);
-        tmem_st_wait();
-        jb::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) jb::mbar_arrive(p_full(b));
+        for (int c = 0; c < C::CHUNKS; ++c) {
+          l += exp_pack_sum<32, NT == 2>(sr + 32 * c, s.scale_log2, m_ref == -CUDART_INF_F ? 0.0f : -m_ref);
+          tmem_st16(s_at + half * (KH / 2) + 16 * c, sr + 32 * c);
+          tmem_st_wait();
+          jb::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) jb::mbar_arrive(c < C::CHUNKS - 1 ? p_half(b) : p_full(b));
+        }
       }
       if (!both) break;
       if (ok && g.nb > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(w), turn & 1, status, 43));
