@@ -265,6 +265,40 @@ def test_attention_masked_values_that_are_not_numbers(dtype, new):
 
 @gpu
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("new", [[1, 1, 1], [4, 1, 3], [130, 90, 70]])
+def test_attention_stale_numbers_and_keys_that_are_not_numbers(dtype, new):
+    """Finite numbers of any size behind a sequence's end weigh nothing at all; a key of the prefix that is not a number, wherever
+    it lies in a block of keys, shows in every row."""
+    owned = [n + b * 40 for b, n in enumerate(new)]
+    c = attention_case(8, dtype, 8, 2, 128, 1400, new, owned)
+    want = attention_oracle(c)
+    for b, o in enumerate(owned):
+        if o % PAGE:
+            page = int(c["table"][b, o // PAGE])
+            c["k"][page, :, o % PAGE:], c["v"][page, :, o % PAGE:] = 0.0, 3e38
+    last = int(c["prefix_pages"][-1])
+    c["k"][last, :, 1400 % PAGE:], c["v"][last, :, 1400 % PAGE:] = 0.0, -3e38
+    close(attention(c), want, dtype)
+    for at in (0, 15, 30, 63, 1399):
+        page, row = int(c["prefix_pages"][at // PAGE]), at % PAGE
+        kept = c["k"][page, 0, row].clone()
+        c["k"][page, 0, row] = float("nan")
+        got = attention(c)
+        assert torch.isnan(got[:, :4 * 128]).all()                       # the query heads of kv head 0
+        close(torch.cat([torch.zeros_like(got[:, :4 * 128]), got[:, 4 * 128:]], 1), torch.cat([0 * want[:, :4 * 128], want[:, 4 * 128:]], 1), dtype)
+        c["k"][page, 0, row] = kept
+
+
+@gpu
+@pytest.mark.parametrize("n,prefix,longest,new", [(400, 16000, 1000, 1), (64, 3000, 900, 1), (40, 2500, 130, 4), (12, 6000, 60, 100), (9, 1900, 60, 130)])
+def test_attention_of_many_sequences(n, prefix, longest, new):
+    """Steps whose prefix is cut in ranges, by one and by two tiles a block, beside long own keys."""
+    c = attention_case(11, BF, 16, 4, 128, prefix, [new] * n, [new + i * 37 % longest for i in range(n)])
+    close(attention(c), attention_oracle(c), BF)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_attention_loud_keys_and_rows_that_see_nothing(dtype):
     c = attention_case(9, dtype, 8, 2, 128, 300, [2, 1, 3], [2, 90, 40], sharp=40.0)      # weights of nearly one key each
     largest = float(c["q"].float().view(-1, 128).norm(dim=1).max() * c["k"].float().norm(dim=-1).max()) * c["scale"]
