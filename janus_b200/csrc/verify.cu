@@ -173,24 +173,20 @@ struct Draw {
     if (form == KEPT) return w;
     return form == LOOKED_UP ? (v == d ? 0.0f : w) : fmaxf(fmaf(w, inv_sum, -qv), 0.0f);
   }
-  // the masses of four neighbouring tokens
-  __device__ __forceinline__ void four(int v0, bool vectors, float* out) const {
-    float xv[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F}, qv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  // four neighbouring tokens' logits, and their probabilities (REFUSED)
+  __device__ __forceinline__ void load(int v0, bool vectors, float* xv, float* qv) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xv[i] = -CUDART_INF_F, qv[i] = 0.0f;
     if (vectors) {
-      if (v0 < V) {
-        *reinterpret_cast<float4*>(xv) = *reinterpret_cast<const float4*>(x + v0);
-        if (form == REFUSED) *reinterpret_cast<float4*>(qv) = __ldcs(reinterpret_cast<const float4*>(q + v0));
-      }
+      if (v0 < V) *reinterpret_cast<float4*>(xv) = *reinterpret_cast<const float4*>(x + v0);
+      if (v0 < V && form == REFUSED) *reinterpret_cast<float4*>(qv) = __ldcs(reinterpret_cast<const float4*>(q + v0));
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (v0 + i < V) {
-          xv[i] = x[v0 + i];
-          if (form == REFUSED) qv[i] = q[v0 + i];
-        }
+      for (int i = 0; i < 4; ++i) {
+        if (v0 + i < V) xv[i] = x[v0 + i];
+        if (v0 + i < V && form == REFUSED) qv[i] = q[v0 + i];
+      }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = mass(v0 + i, xv[i], qv[i]);
   }
 };
 
@@ -224,8 +220,12 @@ __device__ __forceinline__ int first_past(const float* mass, int n, float before
 // of runs in order.  run_end[k]: the warp's sum up to and with run k.
 __device__ __forceinline__ float warp_masses(const Draw& draw, int chunk, bool vectors, float (&w)[16], float (&run_end)[4]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int v0 = chunk * CHUNK + warp * PIECE + lane * 4;
+  float q[16];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) draw.four(chunk * CHUNK + warp * PIECE + k * 128 + lane * 4, vectors, w + 4 * k);
+  for (int k = 0; k < 4; ++k) draw.load(v0 + k * 128, vectors, w + 4 * k, q + 4 * k);   // all on their way before the first is looked at
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = draw.mass(v0 + i / 4 * 128 + i % 4, w[i], q[i]);
   float run = 0.0f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -254,12 +254,25 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
   __shared__ int s_token;
   const int size = cluster_size(), rank = cluster_rank(), b = blockIdx.x / size;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  jb::pdl_wait();
-  jb::pdl_launch_dependents();
+  // What this launch reads was there before stats_kernel began (which has waited for it, where it ran), but for the chunks' results:
+  // a row's draft and what is known of it are on their way while those are made.
+  if (T == 0) jb::pdl_wait();
   const int lo = min(max(q_start[b], 0), T), hi = min(max(q_start[b + 1], lo), T), rows = min(hi - lo, width), cached = kv_len[b];
   const float u_token = u_draw[b];
   int* my = out + (size_t)b * width;
   float* lp = logprobs + (size_t)b * width;
+  struct Draft {
+    int d;
+    float x, q, u;
+  };
+  auto draft_behind = [&](int r) {
+    const int t = lo + r + 1, d = r + 1 < rows ? tokens[t] : -1;
+    if (d < 0 || d >= V) return Draft{-1, 0.0f, 1.0f, 1.0f};
+    return Draft{d, logits[(size_t)(lo + r) * V + d], probs && heat > 0.0f ? probs[(size_t)t * V + d] : 1.0f, u_accept[t]};
+  };
+  Draft draft = warp < rows ? draft_behind(warp) : Draft{};
+  if (T > 0) jb::pdl_wait();
+  jb::pdl_launch_dependents();
   if (rows == 0) {   // (the whole cluster)
     if (rank == 0) {
       for (int k = tid; k < width; k += THREADS) my[k] = -1, lp[k] = 0.0f;
@@ -272,11 +285,7 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
     const Chunk* c = stats + (size_t)(lo + r) * chunks;
     float top = -CUDART_INF_F, sum = 0.0f;
     int arg = 0x7fffffff;
-    // (the draft and what is known of it, on its way beside the chunks')
-    const int t = lo + r + 1, d = r + 1 < rows ? tokens[t] : -1;
-    const bool there = d >= 0 && d < V;
-    const float x = there ? logits[(size_t)(lo + r) * V + d] : 0.0f;
-    const float q = there && probs && heat > 0.0f ? probs[(size_t)t * V + d] : 1.0f, u = there ? u_accept[t] : 1.0f;
+    if (r != warp) draft = draft_behind(r);
     for (int i = lane; i < chunks; i += 32) keep_first(top, arg, c[i].top, c[i].arg);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -288,8 +297,8 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
     sum = jb::warp_sum(sum);
     if (arg == 0x7fffffff) arg = 0;
     if (lane == 0) {
-      const bool yes = there && (heat > 0.0f ? u * q * sum < weight(x, top, heat_log2) : d == arg);
-      row_top[r] = top, row_sum[r] = sum, row_arg[r] = arg, row_yes[r] = yes, row_x[r] = x;
+      const bool yes = draft.d >= 0 && (heat > 0.0f ? draft.u * draft.q * sum < weight(draft.x, top, heat_log2) : draft.d == arg);
+      row_top[r] = top, row_sum[r] = sum, row_arg[r] = arg, row_yes[r] = yes, row_x[r] = draft.x;
     }
   }
   if (tid == 0) s_token = -1;
@@ -420,8 +429,8 @@ JB_EXPORT int jb_verify_drafts(const float* logits, const int* tokens, const int
     if (e != cudaSuccess) return (int)e;
   }
   // Blocks a request: as many as run at once (two a multiprocessor), twice.  A block more takes its share of a row's chunks, but makes all
-  // of the request's decisions too: 256 requests took 94 us by eight blocks each, 66 by one, whose sixteen chunks follow one another.
-  int size = 4 * 148 / B;
+  // of the request's decisions too.  One where no row is passed over, drafts having been looked up (221 requests: 49 us, 58 by two each).
+  int size = probs && heat > 0.0f ? 4 * 148 / B : 1;
   size = size < 1 ? 1 : size > MAX_CLUSTER ? MAX_CLUSTER : size;
   if (size > chunks) size = chunks;
   cudaLaunchAttribute attr[2];
