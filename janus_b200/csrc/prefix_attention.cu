@@ -1027,5 +1027,5 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
   else if (hd > 64) e = own_go<128, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, shared, fewest, status);
   else e = own_go<64, 2>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, shared, fewest, status);
   if (e != cudaSuccess) return (int)e;
-  return (int)join_go<bf16>(stream, qb, kb, vb, ob, part_o, ml, own_count, s, parts, 0);
+  return (int)join_go<bf16>(stream, qb, kb, vb, ob, part_o, ml, own_count, s, parts, own_most);
 }

@@ -105,7 +105,7 @@ __device__ __forceinline__ int slots_of(const Slots& p, const Step& s, int token
 }
 
 // All partial results of a (token, query head) joined in the order of their slots, the prefix's first, then those over own keys:
-// own_count[token][kv head] of them, or own_slots where that is null.  WARPS warps a row, each with every WARPS-th slot: four where
+// own_count[token][kv head] of them (own_slots at most), or own_slots where that is null.  WARPS warps a row, each with every WARPS-th slot: four where
 // there are few rows, which otherwise wait for one slot after another (464 rows of 35 slots: 19 us by one warp each), one where there
 // are many.  Joined by the blocks that walk the own keys, one row after another, the wait took longer than the keys (48 sequences of up
 // to 24 rows: 24 of 34 us).
@@ -120,17 +120,27 @@ __global__ void __launch_bounds__(128) join_kernel(const E* __restrict__ q, cons
   const int t = item / s.nh, h = item - t * s.nh, kvh = h / (s.nh / s.nkv);
   const size_t all = (size_t)s.T * s.nh;
   const int shared = t < s.T ? slots_of(parts, s, t, kvh) : 0;
+  const int total = s.q_start[s.n_seqs];   // (there since before the first of a call's launches, as all but partial results)
   jb::pdl_wait();
   jb::pdl_launch_dependents();
-  if (t >= s.T) return;
+  if (t >= total || t >= s.T) return;
   auto place = [&](int i) { return (i < shared ? i : parts.most + i - shared) * all + item; };
-  const int total = s.q_start[s.n_seqs], own = own_count ? own_count[t * s.nkv + kvh] : own_slots;
-  // (asked for before it is known whether the row is anybody's)
+  // How many results there are over own keys comes with the first results: what lies in places of none is not used.
+  const int own = own_count ? own_count[t * s.nkv + kvh] : own_slots;
   float2 first = make_float2(-CUDART_INF_F, 0.0f);
-  if (lane < shared) first = part_ml[place(lane)];
-  if (t >= total) return;
+  if (lane < shared + own_slots) first = part_ml[place(lane)];
+  constexpr int EARLY = WARPS > 1 ? 2 : 0;   // (many rows hide one another's waits)
+  float4 early[EARLY + 1][2];
+#pragma unroll
+  for (int i = 0; i < EARLY; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      early[i][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (part + i * WARPS < shared && lane * 4 + 128 * e < s.hd)
+        early[i][e] = *reinterpret_cast<const float4*>(part_o + place(part + i * WARPS) * s.hd + lane * 4 + 128 * e);
+    }
   const int slots = shared + own;
-  if (lane >= shared && lane < slots) first = part_ml[place(lane)];
+  if (lane >= slots) first = make_float2(-CUDART_INF_F, 0.0f);
   float top = first.x, sum = 0.0f;
   for (int i = lane + 32; i < slots; i += 32) top = fmaxf(top, part_ml[place(i)].x);
   top = jb::warp_max(top);
@@ -142,8 +152,22 @@ __global__ void __launch_bounds__(128) join_kernel(const E* __restrict__ q, cons
     const float mine = exp2f(ml.x - ref);
     sum = fmaf(mine, ml.y, sum);
     const int n = min(32, slots - i0);
+    int j = part;
+    if (i0 == 0) {
+#pragma unroll
+      for (int i = 0; i < EARLY; ++i)
+        if (j < shared && j < n) {
+          const float f = __shfl_sync(0xffffffffu, mine, j);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float4 v = early[i][e];
+            acc[e].x = fmaf(f, v.x, acc[e].x), acc[e].y = fmaf(f, v.y, acc[e].y), acc[e].z = fmaf(f, v.z, acc[e].z), acc[e].w = fmaf(f, v.w, acc[e].w);
+          }
+          j += WARPS;
+        }
+    }
 #pragma unroll 8
-    for (int j = part; j < n; j += WARPS) {
+    for (; j < n; j += WARPS) {
       const float f = __shfl_sync(0xffffffffu, mine, j);
       const float* row = part_o + place(i0 + j) * s.hd;
 #pragma unroll
