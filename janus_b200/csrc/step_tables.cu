@@ -8,9 +8,10 @@
 // request b takes pool[E_b, E_b + need_b) with E the exclusive sum of need, and what is left over is the next free list.
 // The same lists give the same tables whatever the launch looks like: there are no atomics but on a bitmap.
 //
-// One launch.  Every block makes the three sums (new tokens, pages needed, pages given back) by itself in shared memory, which
-// costs less than a second launch or a wait between blocks: 1,024 requests are one to four elements a thread.  Then the blocks
-// share the outputs out among themselves.
+// One launch, bound by how often it waits for memory: 3.9 us for 4 requests, 4.8 for 256, 9.7 for 1,024 of up to 512 pages each.  Every
+// block makes the three sums (new tokens, pages needed, pages given back) by itself in shared memory, in one pass, which costs less
+// than a second launch or a wait between blocks.  Then table rows, tokens and free pages each have blocks of their own: made one list
+// after another by the same threads their waits added up (256 requests: 8.3 us, with three passes for the sums).
 #include <stdio.h>
 
 #include "common.cuh"
@@ -19,6 +20,7 @@ namespace {
 
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
+constexpr int SMS = 148;
 
 struct Args {
   const int* lengths;
@@ -40,38 +42,10 @@ struct Args {
   int* n_free_out;
   int* missing;
   int B, B0, T, W0, W, P, N, page_size;
+  int blocks[3];          // that make table rows, tokens, free pages
 };
 
 __device__ __forceinline__ int pages_of(int tokens, int page_size) { return tokens / page_size + (tokens % page_size != 0); }
-
-// Exclusive sums of n values, value(i) for i < n, into out[0 .. n] (out[n]: the sum of all).  `warp_sum`: WARPS ints.
-template <typename F>
-__device__ __forceinline__ void exclusive_sums(F&& value, int n, int* out, int* warp_sum) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int carry = 0;
-  for (int i0 = 0; i0 < n; i0 += THREADS) {
-    const int i = i0 + threadIdx.x;
-    const int v = i < n ? value(i) : 0;
-    int s = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += t;
-    }
-    if (lane == 31) warp_sum[warp] = s;
-    __syncthreads();
-    int before = carry, all = carry;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w == warp) before = all;
-      all += warp_sum[w];
-    }
-    if (i < n) out[i] = before + s - v;
-    carry = all;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) out[n] = carry;
-}
 
 // The largest i with sums[i] <= x, of sums[0 .. n] rising, sums[0] <= x < sums[n].
 __device__ __forceinline__ int owner(const int* sums, int n, int x) {
@@ -86,7 +60,7 @@ __device__ __forceinline__ int owner(const int* sums, int n, int x) {
 
 __global__ void __launch_bounds__(THREADS) step_tables_kernel(const Args a) {
   extern __shared__ int smem[];
-  __shared__ int warp_sum[WARPS];
+  __shared__ int warp_sum[3][WARPS];
   int* starts = smem;                     // [B + 1] first token of each request
   int* takes = starts + a.B + 1;          // [B + 1] first place of the pool that each request takes
   int* gives = takes + a.B + 1;           // [B0 + 1] first given-back place of each old row
@@ -104,21 +78,62 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const Args a) {
   auto held_before = [&](int r) { return r < 0 ? min(a.P, a.W) : held_of(r); };
   auto length_of = [&](int b) { return max(a.lengths[b], 0); };
   auto fresh_of = [&](int b) { return max(a.fresh[b], 0); };
-  for (int b = threadIdx.x; b < a.B; b += THREADS) {
-    const int r = row_of(b);
+  // ---- the sums: what a thread needs of the first THREADS requests and rows is asked for at once ----
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  struct Item {
+    int length, fresh, row, held;   // of request i; the pages that old row i holds
+  };
+  auto load = [&](int i) {
+    Item x{0, 0, -1, 0};
+    if (i < a.B) x.length = length_of(i), x.fresh = fresh_of(i), x.row = row_of(i);
+    if (i < a.B0) x.held = held_of(i);
+    return x;
+  };
+  Item x = load(threadIdx.x);
+  const int listed = min(max(*a.n_free, 0), a.N);
+  for (int i = threadIdx.x; i < a.B; i += THREADS) {
+    const int r = i == threadIdx.x ? x.row : row_of(i);
     if (r >= 0) atomicOr(&goes_on[r >> 5], 1u << (r & 31));
   }
+  int before = threadIdx.x < a.B ? held_before(x.row) : 0;
   __syncthreads();
-  exclusive_sums([&](int b) { return fresh_of(b); }, a.B, starts, warp_sum);
-  exclusive_sums(
-      [&](int b) {
-        const int want = min(pages_of(length_of(b) + fresh_of(b), a.page_size), a.W);
-        return max(0, want - held_before(row_of(b)));
-      },
-      a.B, takes, warp_sum);
-  exclusive_sums([&](int r) { return (goes_on[r >> 5] >> (r & 31)) & 1u ? 0 : max(0, held_of(r) - a.P); }, a.B0, gives, warp_sum);
+  int carry[3] = {0, 0, 0};
+  for (int i0 = 0; i0 < max(a.B, a.B0); i0 += THREADS) {
+    const int i = i0 + threadIdx.x;
+    if (i0 > 0) {
+      x = load(i);
+      before = i < a.B ? held_before(x.row) : 0;
+    }
+    int v[3] = {0, 0, 0}, up[3];
+    if (i < a.B) v[0] = x.fresh, v[1] = max(0, min(pages_of(x.length + x.fresh, a.page_size), a.W) - before);
+    if (i < a.B0 && !((goes_on[i >> 5] >> (i & 31)) & 1u)) v[2] = max(0, x.held - a.P);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      up[k] = v[k];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, up[k], o);
+        if (lane >= o) up[k] += t;
+      }
+      if (lane == 31) warp_sum[k][warp] = up[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      int in_front = carry[k];
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        if (w == warp) in_front = carry[k];
+        carry[k] += warp_sum[k][w];
+      }
+      int* out = k == 0 ? starts : k == 1 ? takes : gives;
+      if (i < (k < 2 ? a.B : a.B0)) out[i] = in_front + up[k] - v[k];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) starts[a.B] = carry[0], takes[a.B] = carry[1], gives[a.B0] = carry[2];
   __syncthreads();
-  const int n_free = min(max(*a.n_free, 0), a.N);
+  const int n_free = listed;
   const int have = n_free + gives[a.B0], took = min(takes[a.B], have), left = have - took;
   auto pool = [&](int i) {
     if (i < n_free) return a.free_pages[i];
@@ -130,41 +145,48 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const Args a) {
     const int i = takes[b] + c - held0;
     return i < takes[b + 1] && i < have ? pool(i) : -1;
   };
-  const int lane = threadIdx.x & 31;
-  const int warp = blockIdx.x * WARPS + (threadIdx.x >> 5), warps = gridDim.x * WARPS;
-  const int thread = blockIdx.x * THREADS + threadIdx.x, threads = gridDim.x * THREADS;
-  for (int b = warp; b < a.B; b += warps) {
-    const int r = row_of(b), held0 = held_before(r);
-    int* row = a.table + (size_t)b * a.W;
-    for (int c = lane; c < a.W; c += 32) row[c] = page_at(b, r, held0, c);
-    if (lane == 0) {
-      a.kv_len[b] = length_of(b) + fresh_of(b);
-      a.held[b] = held0 + max(0, min(takes[b + 1], have) - min(takes[b], have));
+  // ---- the outputs: table rows, tokens, free pages, each by blocks of their own, as a thread's would follow one another ----
+  const int kind = blockIdx.x < a.blocks[0] ? 0 : blockIdx.x < a.blocks[0] + a.blocks[1] ? 1 : 2;
+  const int first = kind == 0 ? 0 : kind == 1 ? a.blocks[0] : a.blocks[0] + a.blocks[1];
+  const int thread = (blockIdx.x - first) * THREADS + threadIdx.x, threads = a.blocks[kind] * THREADS;
+  if (kind == 0) {
+    for (int b = thread >> 5; b < a.B; b += threads >> 5) {
+      const int r = row_of(b), held0 = held_before(r);
+      int* row = a.table + (size_t)b * a.W;
+      for (int c = lane; c < a.W; c += 32) row[c] = page_at(b, r, held0, c);
+      if (lane == 0) {
+        a.kv_len[b] = length_of(b) + fresh_of(b);
+        a.held[b] = held0 + max(0, min(takes[b + 1], have) - min(takes[b], have));
+      }
     }
+    return;
   }
-  for (int t = thread; t < a.T; t += threads) {
-    int position = -1, b = -1, dest = -1;
-    if (t < starts[a.B]) {
-      b = owner(starts, a.B, t);
-      position = length_of(b) + t - starts[b];
-      const int c = position / a.page_size, r = row_of(b);
-      const int page = c < a.W ? page_at(b, r, held_before(r), c) : -1;
-      if (page >= 0) dest = page * a.page_size + position % a.page_size;
+  if (kind == 1) {
+    for (int t = thread; t < a.T; t += threads) {
+      int position = -1, b = -1, dest = -1;
+      if (t < starts[a.B]) {
+        b = owner(starts, a.B, t);
+        position = length_of(b) + t - starts[b];
+        const int c = position / a.page_size, r = row_of(b);
+        const int page = c < a.W ? page_at(b, r, held_before(r), c) : -1;
+        if (page >= 0) dest = page * a.page_size + position % a.page_size;
+      }
+      a.positions[t] = position;
+      a.token_seq[t] = b;
+      a.dest[t] = dest;
     }
-    a.positions[t] = position;
-    a.token_seq[t] = b;
-    a.dest[t] = dest;
+    return;
   }
   for (int i = thread; i < a.N; i += threads) a.free_out[i] = i < left ? pool(took + i) : -1;
   for (int b = thread; b <= a.B; b += threads) a.q_start[b] = starts[b];
-  if (blockIdx.x == 0) {
+  if (blockIdx.x == first) {
     int over = 0;
     for (int b = threadIdx.x; b < a.B; b += THREADS) over += max(0, pages_of(length_of(b) + fresh_of(b), a.page_size) - a.W);
     over = __reduce_add_sync(0xffffffffu, over);
-    if (lane == 0) warp_sum[threadIdx.x >> 5] = over;
+    if (lane == 0) warp_sum[0][warp] = over;
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int w = 1; w < WARPS; ++w) over += warp_sum[w];
+      for (int w = 1; w < WARPS; ++w) over += warp_sum[0][w];
       *a.missing = takes[a.B] - took + over + max(0, left - a.N);   // (what the new list has no place for is lost)
       *a.n_free_out = min(left, a.N);
     }
@@ -193,10 +215,19 @@ JB_EXPORT int jb_step_tables(const int* lengths, const int* fresh, const int* ro
       allowed = smem;
     }
   }
-  const Args a{lengths, fresh, rows, old_table, old_held, prefix, free_pages, n_free, q_start, kv_len, positions, token_seq, dest,
-               table, held, free_out, n_free_out, missing, B, B0, T, W0, W, P, N, page_size};
-  const long long work = (long long)B * W + 3ll * T + N;
-  const int blocks = (int)(work / 4096 < 1 ? 1 : work / 4096 > 148 ? 148 : work / 4096);
+  Args a{lengths, fresh, rows, old_table, old_held, prefix, free_pages, n_free, q_start, kv_len, positions, token_seq, dest,
+         table, held, free_out, n_free_out, missing, B, B0, T, W0, W, P, N, page_size, {}};
+  // A block for THREADS places of a list, but about one a multiprocessor in all, shared by the lists' work: more blocks make the sums more
+  // often (1,024 requests of up to 512 pages: 9.7 us, 12.4 by 148 blocks a list).  A token, whose request is searched for, is as much
+  // work as four places of the table.
+  const long long items[3] = {(long long)B * W, T, N}, all = items[0] + 4 * items[1] + items[2];
+  int blocks = 0;
+  for (int k = 0; k < 3; ++k) {
+    const long long wanted = (items[k] + THREADS - 1) / THREADS, share = all > 0 ? items[k] * (k == 1 ? 4 : 1) * SMS / all : 0;
+    const long long n = wanted < share || wanted <= SMS / 3 ? wanted : share;
+    a.blocks[k] = n < 1 ? 1 : (int)n;
+    blocks += a.blocks[k];
+  }
   jb::Launch cfg(dim3(blocks), dim3(THREADS), smem, stream);
   return (int)cudaLaunchKernelEx(&cfg.c, step_tables_kernel, a);
 }
