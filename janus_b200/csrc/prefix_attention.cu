@@ -5,9 +5,19 @@
 // A softmax over a union of key sets joins from the sets' (maximum m, sum l, weighted values O):
 //   m = max m_i,  l = sum 2^(m_i - m) l_i,  O = sum 2^(m_i - m) O_i   (scores in units of log2).
 // So the prefix is attended once for all: the rows of ALL sequences' tokens make tiles of 128 for the tensor cores, which walk
-// the prefix's keys in ranges (`prefix_tc_kernel<SHARED>`), and each sequence's own pages are walked
-// (`own_kernel`; tiles again where a sequence brings many tokens, `<OWN>`); what they leave is float32 and is joined.  Steps whose sequences bring many tokens fill tiles by themselves: there a tile walks the prefix and then its own
-// pages and nothing is joined (`prefix_tc_kernel<WHOLE>`).
+// the prefix's keys in ranges (`prefix_tc_kernel<SHARED>`), and each sequence's own pages are walked (`own_kernel`; tiles again
+// where a sequence brings many tokens, `<OWN>`); what they leave is float32 and is joined.  Where sequences bring many tokens behind a
+// prefix that is not much longer, a tile walks the prefix and then its own pages and nothing is joined (`<WHOLE>`).  Few rows behind a
+// short prefix walk it with their own keys (`own_kernel` alone): a launch less.
+//
+// The launches overlap (each begins before the one in front of it has ended, and asks for its results last).  What bounds them, of
+// the measured 6,537 GB/s and 1,637 TFLOP/s, with 32 heads over 8 of 128 numbers:
+//   64 single tokens behind 8,192, 30 to 700 own: 29 us; the prefix 18 us of them by 128 blocks, each waiting on its own row tile's
+//     chain (scores, weights, values), the own keys' 40 MB beside it, 5 us for the join's launch and one round of loads
+//   256 behind 16,384, 3 to 2,500 own: 122 us; prefix products at 1,100 TFLOP/s (of all multiprocessors) while they run, own keys at
+//     5.2 TB/s while they do, each on a part of the multiprocessors
+//   8 prompts of up to 510 tokens behind 4,100: 99 us; the prefix 80 us at 57 % of the tensor pipe's cycles (a block of keys for two tiles
+//     takes 3,400 cycles: 2,048 of products, 2,048 of the special-function unit, which hide each other in part), own keys the rest
 #include <cuda.h>
 
 #include "prefix_attention.cuh"
@@ -22,9 +32,11 @@ namespace {
 //   warps 2..  two threads a row, each with half of a block's keys: softmax in float32 against a reference maximum that is raised
 //              (and O rescaled) only when a row's maximum has grown by 2^8; P, in bfloat16 as the tensor core takes it, over the
 //              first half of S.  (With one thread a row the softmax took twice as long as the products it has to hide behind.)
-// Two tiles a CTA take turns on the tensor core (NT = 2); a single tile has two S buffers and works a block ahead.
-// SHARED walks an even share of a list of (tile, kv head, key block): a tile's blocks end in one block and go on in the next,
-// which leaves a partial result of its own, and no multiprocessor waits for another's last wave.
+// Two tiles a CTA take turns on the tensor core (NT = 2); a single tile has two S buffers and works a block ahead.  P is handed over in
+// two parts, 32 keys of each half first: their product with the values runs while the others' weights are made (8 prompts: 107 us
+// with one, 103 with two).
+// SHARED walks an even share of a list of (tile, kv head, key block), each share a partial result of every tile that it has a part of.
+// A tile's places of the list may be more than its blocks, so that shares end where tiles do.
 // ---------------------------------------------------------------------------
 constexpr int BM = 128;
 constexpr float RESCALE_LOG2 = 8.0f;
@@ -616,7 +628,8 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
 // tiles (128-byte swizzle) into a ring of its own, ahead across the ends of rows, the rows' queries stay in registers as the
 // products take them, and where a row's keys end (or the share does) the sums go out as a partial result.  How many a row has is
 // written beside (own_count).  A block of its own for every row waited for the longest row, and for what it had to fetch before
-// its first key: 256 sequences of 3 to 2,500 keys moved 2.8 TB/s.
+// its first key: 256 sequences of 3 to 2,500 keys moved 2.8 TB/s; by shares 5.2 (359 MB in 69 us, the machine to itself).  Warp-level
+// products, as the 16 rows that a sequence has are an eighth of a tensor-core tile.
 // ---------------------------------------------------------------------------
 constexpr int OWN_WARPS = 4, OWN_THREADS = 32 * OWN_WARPS, OWN_KEYS = 32, OWN_HALVES = PAGE / OWN_KEYS;
 
@@ -953,11 +966,10 @@ cudaError_t own_go(int blocks, cudaStream_t stream, const CUtensorMap* maps, con
 
 // q, out [T, nh hd], caches [n_pages, nkv, 64, hd], all bfloat16.  tiles: row tiles of a block, 1 or 2 (one for heads of more than 128
 // numbers).  shared_per > 0: the prefix for all rows together by blocks of that many key blocks each, which cut a row's keys into at
-// most `most` ranges.  own_tiles: own keys by tiles of a sequence each, else by the warps of
-// own_ctas blocks, which get no less than `fewest` tiles of 32 keys each, so that a row has at most own_most partial results; with the prefix's keys, where
-// nobody walks those apart.
-// scratch: floats [most + own_most][T][nh][hd], then
-// [..][T][nh][2], then T nkv whole numbers (own_most 1 with own_tiles and several ranges).
+// most `most` ranges.  own_tiles: own keys by tiles of a sequence each, else by the warps of own_ctas blocks, which get no less than
+// `fewest` tiles of 32 keys each, so that a row has at most own_most partial results; with the prefix's keys, where nobody walks those
+// apart.  scratch: floats [most + own_most][T][nh][hd], then [..][T][nh][2], then T nkv whole numbers (own_most 1 with own_tiles and
+// several ranges).
 // sizes: host memory, see Sizes.
 JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const void* v_cache, void* out, float* scratch,
                                        const int* prefix_pages, const int* block_table, const int* q_start, const int* kv_len,

@@ -105,9 +105,9 @@ __device__ __forceinline__ int slots_of(const Slots& p, const Step& s, int token
 }
 
 // All partial results of a (token, query head) joined in the order of their slots, the prefix's first, then those over own keys:
-// own_count[token][kv head] of them (own_slots at most), or own_slots where that is null.  WARPS warps a row, each with every WARPS-th slot: four where
-// there are few rows, which otherwise wait for one slot after another (464 rows of 35 slots: 19 us by one warp each), one where there
-// are many.  Joined by the blocks that walk the own keys, one row after another, the wait took longer than the keys (48 sequences of up
+// own_count[token][kv head] of them (own_slots at most), or own_slots where that is null.  WARPS warps a row, each with every WARPS-th
+// slot: four where there are few rows, which otherwise wait for one slot after another (464 rows of 35 slots: 19 us by one warp each),
+// one where there are many.  Joined by the blocks that walk the own keys, one row after another, the wait took longer than the keys (48 sequences of up
 // to 24 rows: 24 of 34 us).
 template <typename E, int WARPS>
 __global__ void __launch_bounds__(128) join_kernel(const E* __restrict__ q, const E* __restrict__ k_cache,

@@ -13,6 +13,11 @@
 // where drafts of a drafting model were refused the blocks share out the pass over the row's weights and the draft's
 // probabilities and tell one another the chunks' sums through distributed shared memory.  The chunk in which the drawn number falls
 // is then read once more by the block that has it.  All sums are float32 in a fixed order.
+//
+// 256 requests of 1 to 5 drafts with probabilities, 128,256 logits: 100 us, the least 90 (587 MB at the measured 6,537 GB/s);
+// stats_kernel 67 us of them at 6.8 TB/s, decide_kernel the rest: its passes over refused rows at 4 to 5 TB/s, behind 4.7 us of
+// decisions.  64 requests over 32,000: 17.6 us for 32 MB, and one request 10.4: the second launch is a chain of waits (rows' results,
+// the draw's chunk sums, the chunk, the token), which no bandwidth shortens.
 #include <math_constants.h>
 #include <stdio.h>
 
