@@ -970,11 +970,13 @@ cudaError_t own_go(int blocks, cudaStream_t stream, const CUtensorMap* maps, con
 // `fewest` tiles of 32 keys each, so that a row has at most own_most partial results; with the prefix's keys, where nobody walks those
 // apart.  scratch: floats [most + own_most][T][nh][hd], then [..][T][nh][2], then T nkv whole numbers (own_most 1 with own_tiles and
 // several ranges).
-// sizes: host memory, see Sizes.
-JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const void* v_cache, void* out, float* scratch,
-                                       const int* prefix_pages, const int* block_table, const int* q_start, const int* kv_len,
-                                       const int* positions, const void* sizes, int* status, cudaStream_t stream) {
+// tensors, sizes: host memory, see Tensors and Sizes.
+JB_EXPORT int jb_attention_prefix_bf16(const void* tensors, const void* sizes, int* status, cudaStream_t stream) {
+  const Tensors& t = *(const Tensors*)tensors;
   const Sizes& z = *(const Sizes*)sizes;
+  const void *q = t.q, *k_cache = t.k_cache, *v_cache = t.v_cache;
+  void* out = t.out;
+  float* scratch = t.scratch;
   const int prefix_len = z.prefix_len, T = z.T, n_pages = z.n_pages, n_seqs = z.n_seqs, nh = z.nh, nkv = z.nkv, hd = z.hd;
   const int page_size = z.page_size, max_q_len = z.max_q_len, max_kv_len = z.max_kv_len, tiles = z.tiles, shared_per = z.shared_per;
   const int most = z.most, own_tiles = z.own_tiles, own_ctas = z.own_ctas, fewest = z.fewest, own_most = z.own_most;
@@ -990,7 +992,7 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* q, const void* k_cache, const
   JB_REFUSE(n_seqs > 65535 || prefix_len < 0 || shared_per < 0 || most < 0 || most > 64 || (shared_per > 0) != (most > 0) ||
                 (shared_per > 0 && prefix_len == 0),
             "attention_prefix: a prefix of %d tokens in %d ranges of %d key blocks for %d sequences", prefix_len, most, shared_per, n_seqs);
-  const Step s{prefix_pages, block_table, q_start, kv_len, positions, prefix_len, z.ld_table, z.width, T, n_seqs, nh, nkv, hd, z.scale * LOG2E};
+  const Step s{t.prefix_pages, t.block_table, t.q_start, t.kv_len, t.positions, prefix_len, z.ld_table, z.width, T, n_seqs, nh, nkv, hd, z.scale * LOG2E};
   const bf16 *qb = (const bf16*)q, *kb = (const bf16*)k_cache, *vb = (const bf16*)v_cache;
   bf16* ob = (bf16*)out;
   const size_t rows_of_parts = (size_t)(most + own_most) * T * nh;

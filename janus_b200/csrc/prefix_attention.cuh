@@ -22,6 +22,13 @@ struct Sizes {
   int tiles, shared_per, most, own_tiles, own_ctas, fewest, own_most;
   float scale;
 };
+// ... and its tensors' places, in one piece as well.  scratch: see the entry points.
+struct Tensors {
+  const void *q, *k_cache, *v_cache;
+  void* out;
+  float* scratch;
+  const int *prefix_pages, *block_table, *q_start, *kv_len, *positions;
+};
 // What every kernel of a call knows.
 struct Step {
   const int* prefix_pages;

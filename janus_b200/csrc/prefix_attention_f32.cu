@@ -238,18 +238,20 @@ cudaError_t pick(int hd, int rows, dim3 grid, cudaStream_t stream, const float* 
 // q, out [T, nh hd], caches [n_pages, nkv, 64, hd], all float32.  splits: ranges of the prefix (0: there is none), own_slots: ranges
 // of a sequence's own keys; rows, own_rows: rows of a block over the prefix and over own keys, 16 or 64; scratch: floats
 // [splits + own_slots][T][nh][hd], then [..][T][nh][2].  Head sizes that are no multiple of 4 use none of these.
-// sizes: host memory, see Sizes.
-JB_EXPORT int jb_attention_prefix_f32(const void* q, const void* k_cache, const void* v_cache, void* out, float* scratch,
-                                      const int* prefix_pages, const int* block_table, const int* q_start, const int* kv_len,
-                                      const int* positions, const void* sizes, cudaStream_t stream) {
+// tensors, sizes: host memory, see Tensors and Sizes.
+JB_EXPORT int jb_attention_prefix_f32(const void* tensors, const void* sizes, cudaStream_t stream) {
+  const Tensors& t = *(const Tensors*)tensors;
   const Sizes& z = *(const Sizes*)sizes;
+  const void *q = t.q, *k_cache = t.k_cache, *v_cache = t.v_cache;
+  void* out = t.out;
+  float* scratch = t.scratch;
   const int prefix_len = z.prefix_len, T = z.T, n_seqs = z.n_seqs, nh = z.nh, nkv = z.nkv, hd = z.hd, page_size = z.page_size;
   const int max_q_len = z.max_q_len, rows = z.tiles, own_rows = z.shared_per, splits = z.most, own_slots = z.own_most;
   if (T <= 0 || n_seqs <= 0 || max_q_len <= 0) return 0;
   JB_REFUSE(page_size != PAGE, "attention_prefix: page size %d (need %d)", page_size, PAGE);
   JB_REFUSE(nkv <= 0 || nh % nkv != 0, "attention_prefix: %d heads are not a multiple of %d kv heads", nh, nkv);
   JB_REFUSE(hd <= 0 || hd > 256, "attention_prefix: head size %d", hd);
-  const Step s{prefix_pages, block_table, q_start, kv_len, positions, prefix_len, z.ld_table, z.width, T, n_seqs, nh, nkv, hd, z.scale * LOG2E};
+  const Step s{t.prefix_pages, t.block_table, t.q_start, t.kv_len, t.positions, prefix_len, z.ld_table, z.width, T, n_seqs, nh, nkv, hd, z.scale * LOG2E};
   const float *qf = (const float*)q, *kf = (const float*)k_cache, *vf = (const float*)v_cache;
   float* of = (float*)out;
   float* part_o = scratch;

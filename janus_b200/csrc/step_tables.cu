@@ -12,7 +12,9 @@
 // block makes the three sums (new tokens, pages needed, pages given back) by itself in shared memory, in one pass, which costs less
 // than a second launch or a wait between blocks.  Then table rows, tokens and free pages each have blocks of their own: made one list
 // after another by the same threads their waits added up (256 requests: 8.3 us, with three passes for the sums).
+#include <stddef.h>
 #include <stdio.h>
+#include <string.h>
 
 #include "common.cuh"
 
@@ -197,11 +199,13 @@ size_t smem_for(int B, int B0) { return (size_t)(2 * (B + 1) + B0 + 1 + (B0 + 31
 
 }  // namespace
 
-// Every pointer is device memory of int32, see Args; outputs overlap no input.  n_free_out, missing: one int each.
-JB_EXPORT int jb_step_tables(const int* lengths, const int* fresh, const int* rows, const int* old_table, const int* old_held,
-                             const int* prefix, const int* free_pages, const int* n_free, int* q_start, int* kv_len,
-                             int* positions, int* token_seq, int* dest, int* table, int* held, int* free_out, int* n_free_out,
-                             int* missing, int B, int B0, int T, int W0, int W, int P, int N, int page_size, cudaStream_t stream) {
+// given: an Args without its last member, in host memory (18 pointers one by one cost the host as much as a launch).  Every pointer
+// is device memory of int32; outputs overlap no input.  n_free_out, missing: one int each.
+JB_EXPORT int jb_step_tables(const void* given, cudaStream_t stream) {
+  static_assert(offsetof(Args, blocks) == 18 * 8 + 8 * 4, "as the caller packs it");
+  Args a{};
+  memcpy(&a, given, offsetof(Args, blocks));
+  const int B = a.B, B0 = a.B0, T = a.T, W0 = a.W0, W = a.W, P = a.P, N = a.N, page_size = a.page_size;
   JB_REFUSE(B < 0 || B0 < 0 || T < 0 || W <= 0 || W0 < 0 || P < 0 || N < 0 || page_size <= 0, "step_tables: sizes %d %d %d %d %d %d %d %d", B, B0,
             T, W, W0, P, N, page_size);
   JB_REFUSE(W < W0 || P > W, "step_tables: a table of %d pages a row cannot take over rows of %d behind %d shared pages", W, W0, P);
@@ -215,8 +219,6 @@ JB_EXPORT int jb_step_tables(const int* lengths, const int* fresh, const int* ro
       allowed = smem;
     }
   }
-  Args a{lengths, fresh, rows, old_table, old_held, prefix, free_pages, n_free, q_start, kv_len, positions, token_seq, dest,
-         table, held, free_out, n_free_out, missing, B, B0, T, W0, W, P, N, page_size, {}};
   // A block for THREADS places of a list, but about one a multiprocessor in all, shared by the lists' work: more blocks make the sums more
   // often (1,024 requests of up to 512 pages: 9.7 us, 12.4 by 148 blocks a list).  A token, whose request is searched for, is as much
   // work as four places of the table.

@@ -19,6 +19,7 @@
 // decisions.  64 requests over 32,000: 17.6 us for 32 MB, and one request 10.4: the second launch is a chain of waits (rows' results,
 // the draw's chunk sums, the chunk, the token), which no bandwidth shortens.
 #include <math_constants.h>
+#include <stddef.h>
 #include <stdio.h>
 
 #include "common.cuh"
@@ -412,12 +413,28 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
   }
 }
 
+struct Verify {
+  const float* logits;
+  const int *tokens, *q_start, *kv_len;
+  const float *u_accept, *u_draw, *probs;   // probs: null where drafts were looked up
+  int* accepted;
+  int* out;
+  float* logprobs;
+  int* kept;
+  void* stats;            // scratch of 3 floats a row and chunk of 8,192 logits
+  int T, B, V, width;
+  float heat;
+};
 }  // namespace
 
-// stats: scratch of 3 floats a row and chunk of 8,192 logits.  The launch of decide_kernel is by clusters.
-JB_EXPORT int jb_verify_drafts(const float* logits, const int* tokens, const int* q_start, const int* kv_len, const float* u_accept,
-                               const float* u_draw, const float* probs, int* accepted, int* out, float* logprobs, int* kept, void* stats,
-                               int T, int B, int V, int width, float heat, cudaStream_t stream) {
+// given: a Verify in host memory.  The launch of decide_kernel is by clusters.
+JB_EXPORT int jb_verify_drafts(const void* given, cudaStream_t stream) {
+  static_assert(offsetof(Verify, heat) == 12 * 8 + 4 * 4, "as the caller packs it");
+  const Verify& g = *(const Verify*)given;
+  const float *logits = g.logits, *u_accept = g.u_accept, *u_draw = g.u_draw, *probs = g.probs;
+  const int T = g.T, B = g.B, V = g.V, width = g.width;
+  const float heat = g.heat;
+  void* stats = g.stats;
   if (B <= 0) return 0;
   JB_REFUSE(V <= 0 || width <= 0 || T < 0, "verify_drafts: %d rows of %d logits, %d tokens a request", T, V, width);
   const int chunks = (V + CHUNK - 1) / CHUNK;
@@ -446,6 +463,6 @@ JB_EXPORT int jb_verify_drafts(const float* logits, const int* tokens, const int
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(B * size), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
   cfg.attrs = attr, cfg.numAttrs = jb::pdl_enabled() ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, decide_kernel, logits, (const Chunk*)stats, tokens, q_start, kv_len, u_accept, u_draw, probs, accepted,
-                                 out, logprobs, kept, V, chunks, width, T, heat, heat_log2, (int)vectors);
+  return (int)cudaLaunchKernelEx(&cfg, decide_kernel, logits, (const Chunk*)stats, g.tokens, g.q_start, g.kv_len, u_accept, u_draw, probs,
+                                 g.accepted, g.out, g.logprobs, g.kept, V, chunks, width, T, heat, heat_log2, (int)vectors);
 }

@@ -8,6 +8,7 @@ import contextlib
 import ctypes
 import functools
 import os
+import struct
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -91,8 +92,8 @@ _SIGNATURES = {
     "jb_activate": "ppilip", "jb_tanh_norm": "ppppffippfpipiiplplp",
     "jb_latent_heads": "piiiiiipppiiiipfpppip", "jb_latent_queries": "piiiiiiippppiiipfppip", "jb_latent_values": "pppippiipiiiiiip",
     "jb_latent_down": "piipfpiippiiippppplip",
-    "jb_step_tables": "ppppppppppppppppppiiiiiiiip", "jb_attention_prefix_f32": "pppppppppppp", "jb_attention_prefix_bf16": "ppppppppppppp",
-    "jb_verify_drafts": "ppppppppppppiiiifp",
+    "jb_step_tables": "pp", "jb_attention_prefix_f32": "ppp", "jb_attention_prefix_bf16": "pppp",
+    "jb_verify_drafts": "pp",
     "jb_gather_rows": "ppiipppiiip", "jb_latent_attention": "ppppppppiiiiiiifiipp", "jb_attention_tc_matrix": "ppppppiiiiiiiifpipp",
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "u": ctypes.c_ulonglong,
@@ -2447,7 +2448,10 @@ def step_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, rows: torch.Ten
     at = [t.data_ptr() for t in tensors]
     if len(set(at)) < 18 and any(t.numel() and t.data_ptr() in at[:8] for t in tensors[8:]):
         raise KernelError("step_tables: what is made cannot lie where the old tables and lists do")
-    _check(_lib("step_tables").jb_step_tables(*at, B, B0, T, W0, W, P, N, int(page_size), _stream()), "step_tables")
+    _check(_lib("step_tables").jb_step_tables(_STEP_TABLES(*at, B, B0, T, W0, W, P, N, int(page_size)), _stream()), "step_tables")
+
+
+_STEP_TABLES = struct.Struct("18P8i").pack     # `Args` of csrc/step_tables.cu, but for its last member
 
 
 _STEP_TABLES_NAMES = ("lengths", "new tokens", "rows", "table", "held pages", "prefix pages", "free pages", "number of free pages",
@@ -2482,14 +2486,17 @@ def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     sizes, floats, kernels = _attention_prefix_sizes(
         prefix_len, block_table.stride(0), block_table.shape[1], T, k_cache.shape[0], n_seqs, nh, nkv, hd, page_size, int(max_q_len),
         int(max_kv_len), float(scale), q.dtype is torch.float32)
-    args = (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
-            workspace.get("prefix_parts", (floats,), torch.float32).data_ptr(), prefix_pages.data_ptr(), block_table.data_ptr(),
-            q_start.data_ptr(), kv_len.data_ptr(), positions.data_ptr(), ctypes.addressof(sizes))
+    args = (_PREFIX_TENSORS(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+                            workspace.get("prefix_parts", (floats,), torch.float32).data_ptr(), prefix_pages.data_ptr(),
+                            block_table.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), positions.data_ptr()), ctypes.addressof(sizes))
     if q.dtype is torch.float32:
         _check(_lib("prefix_attention_f32").jb_attention_prefix_f32(*args, _stream()), "attention_prefix", kernels=kernels)
     else:
         _check(_lib("prefix_attention").jb_attention_prefix_bf16(*args, kernel_status(q.device).data_ptr(), _stream()), "attention_prefix",
                kernels=kernels)
+
+
+_PREFIX_TENSORS = struct.Struct("10P").pack     # `Tensors` of csrc/prefix_attention.cuh
 
 
 class _PrefixSizes(ctypes.Structure):
@@ -2627,6 +2634,11 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Ten
     if not 0.0 <= temperature < float("inf"):
         raise KernelError(f"verify_drafts: temperature {temperature}")
     stats = workspace.get("verify_stats", (T * ((V + 8191) // 8192) * 3,), torch.float32)
-    _check(_lib("verify").jb_verify_drafts(
-        _ptr(logits), _ptr(tokens), _ptr(q_start), _ptr(kv_len), _ptr(u_accept), _ptr(u_draw), _ptr(draft_probs), _ptr(accepted),
-        _ptr(out_tokens), _ptr(logprobs), _ptr(kept), _ptr(stats), T, B, V, width, float(temperature), _stream()), "verify_drafts", kernels=2)
+    given = _VERIFY(
+        logits.data_ptr(), tokens.data_ptr(), q_start.data_ptr(), kv_len.data_ptr(), u_accept.data_ptr(), u_draw.data_ptr(),
+        0 if draft_probs is None else draft_probs.data_ptr(), accepted.data_ptr(), out_tokens.data_ptr(), logprobs.data_ptr(),
+        kept.data_ptr(), stats.data_ptr(), T, B, V, width, min(temperature, 3e38))
+    _check(_lib("verify").jb_verify_drafts(given, _stream()), "verify_drafts", kernels=2)
+
+
+_VERIFY = struct.Struct("12P4if").pack     # `Verify` of csrc/verify.cu
