@@ -32,7 +32,8 @@ namespace {
 //   warps 2..  two threads a row, each with half of a block's keys: softmax in float32 against a reference maximum that is raised
 //              (and O rescaled) only when a row's maximum has grown by 2^8; P, in bfloat16 as the tensor core takes it, over the
 //              first half of S.  (With one thread a row the softmax took twice as long as the products it has to hide behind.)
-// Two tiles a CTA take turns on the tensor core (NT = 2); a single tile has two S buffers and works a block ahead.  P is handed over in
+// Two tiles a CTA take turns on the tensor core (NT = 2); a single tile has two S buffers and works a block ahead, or (SPLIT) is worked on
+// by two groups, which work two blocks ahead and join their sums at the end.  P is handed over in
 // two parts, 32 keys of each half first: their product with the values runs while the others' weights are made (8 prompts: 107 us
 // with one, 103 with two).
 // SHARED walks an even share of a list of (tile, kv head, key block), each share a partial result of every tile that it has a part of.
@@ -158,16 +159,22 @@ template <int HDC, int NT, int KB>
 struct Tc {
   static constexpr int SLABS = HDC / 64;                       // 64-number slabs of a row
   static constexpr int Q_BYTES = SLABS * BM * 128, KV_BYTES = SLABS * KB * 128;
-  static constexpr int BARS = 1 + 8 + 3 * 2 + 3 * NT;          // q_full; k, v full and empty x 2; s_full, p_half, p_full x 2; o_full, o_done, o_free
+  // Heads of up to 64 numbers, one tile: two groups of warps, each with every second block of 64 keys, sums and an O of its own, so that
+  // one's weights are made while the other waits for scores (132 tokens behind 6,001: 28.9 -> 27.5 us, 100 behind 5,000 24.0 -> 22.3).
+  // With 128 numbers it is between 9 % faster and 7 % slower: there the keys' way from L2 is what one tile's block waits for (64 KB for
+  // 1.25 us of work, 6.7 TB/s of 128 blocks).
+  static constexpr bool SPLIT = NT == 1 && HDC == 64;
+  static constexpr int ST = SPLIT ? 4 : 2, SB = SPLIT ? 4 : 2, OB = SPLIT ? 2 : NT;   // stages of keys and of values; S and O buffers
+  static constexpr int BARS = 1 + 4 * ST + 3 * SB + 3 * OB;    // q_full; k, v full and empty; s_full, p_half, p_full; o_full, o_done, o_free
   static constexpr int SWAP = NT * 2 * BM;                     // floats: what the two halves of a row tell each other
-  static constexpr int SMEM = NT * Q_BYTES + 4 * KV_BYTES + SWAP * 4 + NT * 4 * 4 + 8 + BARS * 8 + 16;
+  static constexpr int SMEM = NT * Q_BYTES + 2 * ST * KV_BYTES + SWAP * 4 + NT * 4 * 4 + 8 + BARS * 8 + 16;
   static constexpr int THREADS = 64 + NT * 256;
   static constexpr int CHUNKS = KB / 64;                       // in which a block's weights are handed on
   // (one tile of up to 128 numbers a row: 96 registers a thread, as 576 threads have, so that a block of own_kernel finds registers
   // beside this one; rows of up to 64 leave enough anyway)
   static constexpr int BOUND = HDC == 128 ? 576 : THREADS;
-  static constexpr int COLS = 2 * KB + NT * HDC <= 256 ? 256 : 512;
-  static_assert(2 * KB + NT * HDC <= 512 && SMEM <= 232448, "tensor and shared memory of one CTA");
+  static constexpr int COLS = SB * KB + OB * HDC <= 256 ? 256 : 512;
+  static_assert(SB * KB + OB * HDC <= 512 && SMEM <= 232448, "tensor and shared memory of one CTA");
 };
 // One lane of a warp whose lanes are all here.  (Work given to lane 0 by its number is not known to the compiler to be one thread's:
 // every operand of a product then went through a vector register, and issuing products took twice as long as computing them.)
@@ -218,34 +225,37 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
     float* __restrict__ part_o, float2* __restrict__ part_ml, const Step s, const Slots parts, int* __restrict__ status) {
   typedef Tc<HDC, NT, KB> C;
   extern __shared__ __align__(1024) uint8_t smem[];            // (no static shared memory: it begins where it is declared to)
-  const uint32_t q_s = jb::smem_u32(smem), k_s = q_s + NT * C::Q_BYTES, v_s = k_s + 2 * C::KV_BYTES;
-  float* swap = (float*)(smem + NT * C::Q_BYTES + 4 * C::KV_BYTES);   // [tile][half][row]
+  const uint32_t q_s = jb::smem_u32(smem), k_s = q_s + NT * C::Q_BYTES, v_s = k_s + C::ST * C::KV_BYTES;
+  float* swap = (float*)(smem + NT * C::Q_BYTES + 2 * C::ST * C::KV_BYTES);   // [tile][half][row]
   int* gave_up = (int*)(swap + C::SWAP);                       // [tile][quarter]: one of the two warps has
   int* found = gave_up + NT * 4;                               // WHOLE, OWN: the block's sequence and tile of it
   uint64_t* bars = (uint64_t*)(found + 2);
   uint32_t* tmem_slot = (uint32_t*)(bars + C::BARS);
   const uint32_t bar0 = jb::smem_u32(bars);
-  const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 24, v_full = bar0 + 40, v_empty = bar0 + 56;
-  // an S buffer belongs to a tile (NT = 2), or to the even or odd blocks of the one tile
-  auto s_full = [&](int b) { return bar0 + 72 + 24 * b; };
-  auto p_half = [&](int b) { return bar0 + 80 + 24 * b; };
-  auto p_full = [&](int b) { return bar0 + 88 + 24 * b; };
-  auto o_full = [&](int w) { return bar0 + 120 + 24 * w; };   // a block's product has landed in O
-  auto o_done = [&](int w) { return bar0 + 128 + 24 * w; };   // ... the last block's of a segment
-  auto o_free = [&](int w) { return bar0 + 136 + 24 * w; };   // O has been read and may be begun anew
+  const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = k_full + 8 * C::ST, v_full = k_empty + 8 * C::ST, v_empty = v_full + 8 * C::ST;
+  const uint32_t s_bars = v_empty + 8 * C::ST, o_bars = s_bars + 24 * C::SB;
+  // an S buffer belongs to a tile (NT = 2), to the even or odd blocks of the one tile, or (SPLIT) of one group's
+  auto s_full = [&](int b) { return s_bars + 24 * b; };
+  auto p_half = [&](int b) { return s_bars + 24 * b + 8; };
+  auto p_full = [&](int b) { return s_bars + 24 * b + 16; };
+  auto o_full = [&](int w) { return o_bars + 24 * w; };        // a block's product has landed in O
+  auto o_done = [&](int w) { return o_bars + 24 * w + 8; };    // ... the last block's of a segment
+  auto o_free = [&](int w) { return o_bars + 24 * w + 16; };   // O has been read and may be begun anew
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     jb::mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < C::ST; ++i) {
       jb::mbar_init(k_full + 8 * i, 1);
       jb::mbar_init(k_empty + 8 * i, 1);
       jb::mbar_init(v_full + 8 * i, 1);
       jb::mbar_init(v_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < C::SB; ++i) {
       jb::mbar_init(s_full(i), 1);
       jb::mbar_init(p_half(i), 8);
-      jb::mbar_init(p_full(i), 8);      // an arrival a warp: one a thread would be 256 operations on one word
+      jb::mbar_init(p_full(i), C::SPLIT ? 4 : 8);   // an arrival a warp: one a thread would be 256 operations on one word
     }
-    for (int w = 0; w < NT; ++w) {
+    for (int w = 0; w < C::OB; ++w) {
       jb::mbar_init(o_full(w), 1);
       jb::mbar_init(o_done(w), 1);
       jb::mbar_init(o_free(w), 8);
@@ -337,7 +347,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
         const Segment g = segment(at);
         if (g.nb == 0) break;
         // every product with the queries before these is done when the last block's keys are free
-        if (it > 0) ok = mbar_wait(k_empty + 8 * ((it - 1) & 1), ((it - 1) >> 1) & 1, status, 41);
+        if (it > 0) ok = mbar_wait(k_empty + 8 * ((it - 1) % C::ST), (it - 1) / C::ST & 1, status, 41);
         if (!ok) break;
         jb::mbar_expect_tx(q_full, NT * nslab * tpt * G * 128);   // a box holds tpt tokens x G heads
         for (int w = 0; w < NT; ++w)
@@ -345,7 +355,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
             tma_load_4d(q_s + w * C::Q_BYTES + h * BM * 128, &map_q, q_full, h * 64, 0, g.kvh, g.tok0 + w * tpt);
         const int last_own = FORM != SHARED ? max(min((seq_pos + g.tok0 - seq_start + g.n_tok - s.prefix_len - 1) / PAGE, s.width - 1), 0) : 0;
         for (int j = 0; j < g.nb; ++j, ++it) {
-          const int st = it & 1;
+          const int st = it % C::ST;
           int row0[KB / PAGE];
 #pragma unroll
           for (int half = 0; half < KB / PAGE; ++half) {   // a block's second page may lie behind the last: those keys are masked
@@ -354,19 +364,61 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
             else page = s.table[(size_t)seq * s.ld_table + min((j - g.n_shared) * (KB / PAGE) + half, last_own)];
             row0[half] = (max(page, 0) * s.nkv + g.kvh) * PAGE;
           }
-          if (it >= 2 && !(ok = mbar_wait(k_empty + 8 * st, ((it >> 1) - 1) & 1, status, 41))) break;
+          if (it >= C::ST && !(ok = mbar_wait(k_empty + 8 * st, (it / C::ST - 1) & 1, status, 41))) break;
           jb::mbar_expect_tx(k_full + 8 * st, nslab * KB * 128);
 #pragma unroll
           for (int half = 0; half < KB / PAGE; ++half)
             for (int h = 0; h < nslab; ++h)
               jb::tma_load_2d(k_s + st * C::KV_BYTES + h * KB * 128 + half * PAGE * 128, &map_k, k_full + 8 * st, h * 64, row0[half]);
-          if (it >= 2 && !(ok = mbar_wait(v_empty + 8 * st, ((it >> 1) - 1) & 1, status, 41))) break;
+          if (it >= C::ST && !(ok = mbar_wait(v_empty + 8 * st, (it / C::ST - 1) & 1, status, 41))) break;
           jb::mbar_expect_tx(v_full + 8 * st, nslab * KB * 128);
 #pragma unroll
           for (int half = 0; half < KB / PAGE; ++half)
             for (int h = 0; h < nslab; ++h)
               jb::tma_load_2d(v_s + st * C::KV_BYTES + h * KB * 128 + half * PAGE * 128, &map_v, v_full + 8 * st, h * 64, row0[half]);
         }
+      }
+    }
+  } else if (warp == 1 && C::SPLIT) {
+    if (elected()) {
+      const uint32_t idesc_s = jb::instr_desc_bf16(KB), idesc_o = jb::instr_desc_bf16((s.hd + 15) & ~15) | (1u << 16);   // values: MN-major
+      bool ok = true;
+      int begun = 0, scored[2] = {0, 0}, weighed[2] = {0, 0};   // blocks of the segments before; each group's scored, weighed
+      for (int at = flat_begin, turn = 0; at < flat_end && ok; ++turn) {
+        const Segment g = segment(at);
+        if (g.nb == 0 || !(ok = mbar_wait(q_full, turn & 1, status, 42))) break;
+        auto scores = [&](int j) -> bool {
+          const int st = (begun + j) % C::ST, w = j & 1, b = 2 * w + (w ? scored[1]++ : scored[0]++) % 2;
+          if (!mbar_wait(k_full + 8 * st, (begun + j) / C::ST & 1, status, 42)) return false;
+          jb::tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < C::SLABS; ++h) {
+            const uint64_t a = jb::smem_desc_sw128(q_s + h * BM * 128), k = jb::smem_desc_sw128(k_s + st * C::KV_BYTES + h * KB * 128);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              if (h * 64 + ks * 16 < s.hd) jb::umma_bf16(tmem + b * KB, a + 2 * ks, k + 2 * ks, idesc_s, (h | ks) ? 1u : 0u);
+          }
+          jb::umma_commit(s_full(b));
+          jb::umma_commit(k_empty + 8 * st);
+          return true;
+        };
+        ok = scores(0) && (g.nb == 1 || scores(1));
+        for (int j = 0; j < g.nb && ok; ++j) {
+          const int st = (begun + j) % C::ST, w = j & 1, i = w ? weighed[1]++ : weighed[0]++, b = 2 * w + i % 2;
+          if (j + 2 < g.nb) ok = scores(j + 2);                // (where this group's weights of two blocks ago have been used)
+          ok = ok && mbar_wait(v_full + 8 * st, (begun + j) / C::ST & 1, status, 42);
+          if (ok && j == 0 && turn > 0) ok = mbar_wait(o_free(0), (turn - 1) & 1, status, 42);
+          if (!ok || !(ok = mbar_wait(p_full(b), i / 2 & 1, status, 42))) break;
+          jb::tc_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < KB / 16; ++ks)
+            umma_ts(tmem + C::SB * KB + w * HDC, tmem + b * KB + ks * 8, desc_mn_sw128(v_s + st * C::KV_BYTES + ks * 2048, KB * 128, 1024),
+                    idesc_o, j > 1 || ks > 0 ? 1u : 0u);
+          jb::umma_commit(o_full(w));
+          jb::umma_commit(v_empty + 8 * st);
+          if (j == g.nb - 1) jb::umma_commit(o_done(0));
+        }
+        begun += g.nb;
       }
     }
   } else if (warp == 1) {
@@ -437,10 +489,10 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
       }
     }
   } else {
-    // two warps have the same 32 rows, each half of a block's keys (and of O's columns)
+    // two warps have the same 32 rows, each half of a block's keys (SPLIT: every second block of keys, of 64), and half of O's columns
     const int w = (warp - 2) >> 3, quarter = warp & 3, half = (warp - 2) >> 2 & 1, row = quarter * 32 + lane, pair = 1 + w * 4 + quarter;
-    constexpr int KH = KB / 2, DH = HDC / 2;
-    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16), o_col = 2 * KB + w * HDC;
+    constexpr int KH = C::SPLIT ? KB : KB / 2, DH = HDC / 2;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16), o_col = C::SB * KB + w * HDC;
     float* mine = swap + (w * 2 + half) * BM + row;
     const float* other = swap + (w * 2 + (half ^ 1)) * BM + row;
     // The two say to each other that a row's maximum has grown, or that a wait has run out: then both leave, behind a barrier that
@@ -463,11 +515,90 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
       int see_shared = 0, see_own = 0;                         // keys that the row sees, counted from its half's first
       if (valid) {
         const int see = (FORM == SHARED ? s.positions[token] : seq_pos + token - seq_start) + 1;
-        see_shared = min(see, s.prefix_len) - g.block0 * KB - half * KH;
-        see_own = see - s.prefix_len - half * KH;
+        see_shared = min(see, s.prefix_len) - g.block0 * KB - (C::SPLIT ? 0 : half * KH);
+        see_own = see - s.prefix_len - (C::SPLIT ? 0 : half * KH);
       }
       float m_ref = -CUDART_INF_F, l = 0.0f;
-      for (int j = 0; j < g.nb; ++j, ++it) {
+      float weight[2] = {1.0f, 0.0f};                          // SPLIT: of the groups' O, once they are joined
+      if constexpr (C::SPLIT) {
+        const uint32_t my_o = lane_addr + o_col + half * HDC;
+        for (int j = half; j < g.nb; j += 2, ++it) {
+          const int b = 2 * half + (it & 1);
+          const uint32_t s_at = lane_addr + b * KB;
+          ok = __all_sync(0xffffffffu, mbar_wait(s_full(b), (it >> 1) & 1, status, 43));
+          if (!ok) break;
+          jb::tc_fence_after();
+          uint32_t sr[KH];
+#pragma unroll
+          for (int c0 = 0; c0 < KH; c0 += 16) tmem_ld16(s_at + c0, sr + c0);
+          jb::tmem_ld_wait();
+          const int see = j < g.n_shared ? see_shared - j * KB : see_own - (j - g.n_shared) * KB;
+          if (see < KH) {
+#pragma unroll
+            for (int c = 0; c < KH; ++c)
+              if (c >= see) sr[c] = 0xff800000u;   // -inf
+          }
+          const float mx = row_max<KH>(sr) * s.scale_log2;
+          if (__any_sync(0xffffffffu, mx > m_ref + RESCALE_LOG2 || (m_ref == -CUDART_INF_F && mx > -CUDART_INF_F))) {
+            const float m_new = fmaxf(m_ref, mx);
+            if (j > 1) {
+              ok = __all_sync(0xffffffffu, mbar_wait(o_full(half), (it - 1) & 1, status, 43));
+              if (!ok) break;
+              jb::tc_fence_after();
+              const float corr = m_new == -CUDART_INF_F ? 1.0f : exp2f(m_ref - m_new);
+#pragma unroll
+              for (int c0 = 0; c0 < HDC; c0 += 16) {
+                if (c0 >= s.hd) break;
+                uint32_t r[16];
+                tmem_ld16(my_o + c0, r);
+                jb::tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * corr);
+                tmem_st16(my_o + c0, r);
+              }
+              l *= corr;
+            }
+            m_ref = m_new;
+          }
+          l += exp_pack_sum<KH, false>(sr, s.scale_log2, m_ref == -CUDART_INF_F ? 0.0f : -m_ref);
+#pragma unroll
+          for (int c0 = 0; c0 < KH / 2; c0 += 16) tmem_st16(s_at + c0, sr + c0);
+          tmem_st_wait();
+          jb::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) jb::mbar_arrive(p_full(b));
+        }
+        if (ok && g.nb > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(0), turn & 1, status, 43));
+        // both groups' sums, joined as those of any two sets of keys
+        const float their_m = meet(m_ref);
+        if (!both) break;
+        pair_sync(pair);                // (the place is read before it is written again)
+        const float their_l = meet(l);
+        if (!both) break;
+        pair_sync(pair);
+        const float top = fmaxf(m_ref, their_m), ref = top == -CUDART_INF_F ? 0.0f : top;
+        weight[half] = exp2f(m_ref - ref), weight[half ^ 1] = exp2f(their_m - ref);
+        l = half == 0 ? fmaf(l, weight[0], their_l * weight[1]) : fmaf(their_l, weight[0], l * weight[1]);
+        m_ref = top;
+        jb::tc_fence_after();
+      }
+      // 16 columns of O
+      auto load_o = [&](int c0, uint32_t* r) {
+        tmem_ld16(lane_addr + o_col + c0, r);   // warp-wide: rows without a token load too
+        if constexpr (C::SPLIT) {
+          if (g.nb > 1) {
+            uint32_t second[16];
+            tmem_ld16(lane_addr + o_col + HDC + c0, second);
+            jb::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              r[i] = __float_as_uint(fmaf(__uint_as_float(r[i]), weight[0], __uint_as_float(second[i]) * weight[1]));
+            return;
+          }
+        }
+        jb::tmem_ld_wait();
+      };
+      for (int j = 0; j < g.nb && !C::SPLIT; ++j, ++it) {
         const int b = NT == 2 ? w : it & 1;
         const uint32_t s_at = lane_addr + b * KB;
         ok = __all_sync(0xffffffffu, ok && mbar_wait(s_full(b), (NT == 2 ? it : it >> 1) & 1, status, 43));
@@ -524,13 +655,15 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
           if (lane == 0) jb::mbar_arrive(c < C::CHUNKS - 1 ? p_half(b) : p_full(b));
         }
       }
-      if (!both) break;
-      if (ok && g.nb > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(w), turn & 1, status, 43));
-      const float theirs = meet(l);   // the row's sum over both halves
-      if (!both) break;
-      l = half == 0 ? l + theirs : theirs + l;
-      pair_sync(pair);                // (the place is read before it is written again)
-      jb::tc_fence_after();
+      if constexpr (!C::SPLIT) {
+        if (!both) break;
+        if (ok && g.nb > 0) ok = __all_sync(0xffffffffu, mbar_wait(o_done(w), turn & 1, status, 43));
+        const float theirs = meet(l);   // the row's sum over both halves
+        if (!both) break;
+        l = half == 0 ? l + theirs : theirs + l;
+        pair_sync(pair);                // (the place is read before it is written again)
+        jb::tc_fence_after();
+      }
       const size_t place = (size_t)token * s.nh + head, all = (size_t)s.T * s.nh;
       if (FORM == SHARED || (FORM == OWN && parts.most > 1)) {
         const size_t item = (FORM == SHARED ? g.slot : parts.most) * all + place;
@@ -540,8 +673,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
           const int c0 = half * DH + c1;
           if (c0 >= s.hd) break;
           uint32_t r[16];
-          tmem_ld16(lane_addr + o_col + c0, r);   // warp-wide: rows without a token load too and store nothing
-          jb::tmem_ld_wait();
+          load_o(c0, r);
           if (FORM == OWN && g.nb == 0) {         // (no product has written there)
 #pragma unroll
             for (int i = 0; i < 16; ++i) r[i] = 0u;
@@ -571,10 +703,7 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
           const int c0 = half * DH + c1;
           if (c0 >= s.hd) break;
           uint32_t r[16];
-          if (g.nb > 0) {
-            tmem_ld16(lane_addr + o_col + c0, r);
-            jb::tmem_ld_wait();
-          }
+          if (g.nb > 0) load_o(c0, r);
           float v[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) v[i] = g.nb > 0 ? __uint_as_float(r[i]) * own_weight : 0.0f;
@@ -943,7 +1072,7 @@ cudaError_t tc_pick(int nt, dim3 grid, cudaStream_t stream, const CUtensorMap* m
   if (s.hd > 64 && nt == 2) JB_GO(128, 2, 128);
   if (s.hd > 64) JB_GO(128, 1, 128);
   if (nt == 2) JB_GO(64, 2, 128);
-  JB_GO(64, 1, 128);
+  JB_GO(64, 1, 64);
 #undef JB_GO
 }
 
@@ -1016,7 +1145,8 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* tensors, const void* sizes, i
     JB_REFUSE(total > 0x3fffffffll, "attention_prefix: %lld key blocks", total);
     JB_REFUSE((shared_per % blocks == 0 ? 1 : blocks % shared_per == 0 ? blocks / shared_per : (blocks + shared_per - 2) / shared_per + 1) > most,
               "attention_prefix: ranges of %d cut %d key blocks into more than %d", shared_per, blocks, most);
-    parts = Slots{-1, most, blocks, shared_per, step};
+    const int finer = hd <= 64 && nt == 1 ? 2 : 1;             // such a tile's blocks have 64 keys
+    parts = Slots{-1, most, blocks * finer, shared_per * finer, step};
     e = tc_pick<SHARED>(nt, dim3((unsigned)ctas), stream, maps, qb, kb, vb, ob, part_o, ml, s, parts, status);
     if (e != cudaSuccess) return (int)e;
   }

@@ -298,6 +298,19 @@ def test_attention_of_many_sequences(n, prefix, longest, new):
 
 
 @gpu
+@pytest.mark.parametrize("n,prefix,new,heads,kv_heads,dim", [
+    (66, 6001, 2, 32, 8, 64),       # ranges of 13 key blocks that go from one row tile to the next
+    (300, 60, 1, 16, 8, 64),        # one block of 64 keys, for the first of two groups only
+    (300, 190, 1, 16, 8, 40),       # three
+    (700, 900, 1, 8, 8, 48),        # a last tile with few rows
+    (90, 2500, 3, 8, 1, 32),
+])
+def test_attention_of_narrow_heads_behind_a_prefix(n, prefix, new, heads, kv_heads, dim):
+    c = attention_case(12, BF, heads, kv_heads, dim, prefix, [new] * n, [new + i * 37 % 90 for i in range(n)], sharp=3.0)
+    close(attention(c), attention_oracle(c), BF)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_attention_loud_keys_and_rows_that_see_nothing(dtype):
     c = attention_case(9, dtype, 8, 2, 128, 300, [2, 1, 3], [2, 90, 40], sharp=40.0)      # weights of nearly one key each
