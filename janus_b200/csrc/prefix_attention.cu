@@ -758,7 +758,8 @@ __global__ void __launch_bounds__(Tc<HDC, NT, KB>::BOUND, 1) prefix_tc_kernel(
 // products take them, and where a row's keys end (or the share does) the sums go out as a partial result.  How many a row has is
 // written beside (own_count).  A block of its own for every row waited for the longest row, and for what it had to fetch before
 // its first key: 256 sequences of 3 to 2,500 keys moved 2.8 TB/s; by shares 5.2 (359 MB in 69 us, the machine to itself).  Warp-level
-// products, as the 16 rows that a sequence has are an eighth of a tensor-core tile.
+// products, as the 16 rows that a sequence has are an eighth of a tensor-core tile.  The count is one of each (token, query head): 16
+// rows end inside a token where the heads of a group do not divide them, and its other heads are then cut at other places.
 // ---------------------------------------------------------------------------
 constexpr int OWN_WARPS = 4, OWN_THREADS = 32 * OWN_WARPS, OWN_KEYS = 32, OWN_HALVES = PAGE / OWN_KEYS;
 
@@ -1002,7 +1003,7 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
         const size_t item = ((size_t)(first_slot + slot) * s.T + token) * s.nh + head;
         if ((lane & 3) == 0) {
           part_ml[item] = make_float2(m[r], l[r]);
-          if (slot == 0) own_count[token * s.nkv + kvh] = (place + c.tiles - 1) / per - first + 1;
+          if (slot == 0) own_count[token * s.nh + head] = (place + c.tiles - 1) / per - first + 1;
         }
 #pragma unroll
         for (int j = 0; j < HDC / 8; ++j)
@@ -1097,7 +1098,7 @@ cudaError_t own_go(int blocks, cudaStream_t stream, const CUtensorMap* maps, con
 // numbers).  shared_per > 0: the prefix for all rows together by blocks of that many key blocks each, which cut a row's keys into at
 // most `most` ranges.  own_tiles: own keys by tiles of a sequence each, else by the warps of own_ctas blocks, which get no less than
 // `fewest` tiles of 32 keys each, so that a row has at most own_most partial results; with the prefix's keys, where nobody walks those
-// apart.  scratch: floats [most + own_most][T][nh][hd], then [..][T][nh][2], then T nkv whole numbers (own_most 1 with own_tiles and
+// apart.  scratch: floats [most + own_most][T][nh][hd], then [..][T][nh][2], then T nh whole numbers (own_most 1 with own_tiles and
 // several ranges).
 // tensors, sizes: host memory, see Tensors and Sizes.
 JB_EXPORT int jb_attention_prefix_bf16(const void* tensors, const void* sizes, int* status, cudaStream_t stream) {

@@ -112,7 +112,7 @@ __device__ __forceinline__ int slots_of(const Slots& p, const Step& s, int token
 }
 
 // All partial results of a (token, query head) joined in the order of their slots, the prefix's first, then those over own keys:
-// own_count[token][kv head] of them (own_slots at most), or own_slots where that is null.  WARPS warps a row, each with every WARPS-th
+// own_count[token][query head] of them (own_slots at most), or own_slots where that is null.  WARPS warps a row, each with every WARPS-th
 // slot: four where there are few rows, which otherwise wait for one slot after another (464 rows of 35 slots: 19 us by one warp each),
 // one where there are many.  Joined by the blocks that walk the own keys, one row after another, the wait took longer than the keys (48 sequences of up
 // to 24 rows: 24 of 34 us).
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(128) join_kernel(const E* __restrict__ q, cons
   if (t >= total || t >= s.T) return;
   auto place = [&](int i) { return (i < shared ? i : parts.most + i - shared) * all + item; };
   // How many results there are over own keys comes with the first results: what lies in places of none is not used.
-  const int own = own_count ? own_count[t * s.nkv + kvh] : own_slots;
+  const int own = own_count ? own_count[item] : own_slots;
   float2 first = make_float2(-CUDART_INF_F, 0.0f);
   if (lane < shared + own_slots) first = part_ml[place(lane)];
   constexpr int EARLY = WARPS > 1 ? 2 : 0;   // (many rows hide one another's waits)

@@ -2519,7 +2519,7 @@ def _attention_prefix_sizes(prefix_len: int, ld_table: int, width: int, T: int, 
         kernels = (plan[1] > 0) + 1 + (plan[6] > 0)
     slots = plan[2] + plan[6]
     return (_PrefixSizes(prefix_len, ld_table, width, T, n_pages, n_seqs, nh, nkv, hd, page_size, max_q_len, max_kv_len, *plan, scale),
-            slots * T * nh * (hd + 2) + T * nkv, kernels)
+            slots * T * nh * (hd + 2) + T * nh, kernels)
 
 
 _PREFIX_MOST_RANGES = 64       # partial results over the prefix that a row's join takes
