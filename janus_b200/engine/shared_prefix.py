@@ -157,7 +157,7 @@ class SharedPrefixRunner:
                 for q in live:
                     room = q.limit - q.length - len(q.own)
                     wanted = max_tokens - len(outputs[q.index]) - 1
-                    q.drafts = [] if first else [int(t) for t in q.drafter.draft(max(0, min(drafts, room, wanted)))]
+                    q.drafts = [] if first else self._drafts(q.drafter, max(0, min(drafts, room, wanted)))
                 state, tokens = self._step(live, state, prefix_pages, shared, width, temperature, first)
                 for b, q in enumerate(live):
                     q.length += len(q.own)
@@ -185,6 +185,16 @@ class SharedPrefixRunner:
             for p in mine:
                 group.pool.give_back(p)
         return pending[len(chosen):]
+
+    def _drafts(self, drafter, most: int) -> List[int]:
+        """What a drafter says, up to the first id outside the vocabulary: verification would refuse that one and with it all behind,
+        but the step looks embeddings up before it verifies."""
+        tokens = []
+        for t in drafter.draft(most):
+            if not 0 <= int(t) < self.model.vocab_size:
+                break
+            tokens.append(int(t))
+        return tokens
 
     @staticmethod
     def _accept(q, got, outputs, reasons, max_tokens, stop, callback, longest) -> bool:

@@ -1,0 +1,128 @@
+"""Generation behind a shared prefix without a device: the real runner over stand-ins for the engine and the three faces, which answer
+on the host (the index tables and the verification by their definitions) and note every step's tokens.  The model's next token
+goes by the last one alone, so what has to come out is known.
+"""
+import types
+
+import numpy as np
+import pytest
+import torch
+
+from janus_b200.cache import PAGE_SIZE
+from janus_b200.cache.pages import PagePool
+from janus_b200.engine import shared_prefix
+from janus_b200.engine.shared_prefix import SharedPrefixRunner
+from janus_b200.kernels import ops
+from test_shared_prefix import tables_oracle, verify_oracle
+
+V = 50
+
+
+def next_token(t):
+    return (3 * t + 1) % V
+
+
+def continuation(last, n):
+    out = []
+    for _ in range(n):
+        last = next_token(last)
+        out.append(last)
+    return out
+
+
+class Host:
+    """A runner whose steps are noted in `steps` (token ids, positions, cache rows, rows of the table)."""
+
+    def __init__(self, monkeypatch, pages=64, longest=4096, max_step_tokens=None):
+        self.steps, self.prefix_steps = [], []
+        pool, held = PagePool(pages), []
+
+        def step(entries):
+            (e,) = entries
+            self.prefix_steps.append(len(e.tokens))
+            need = -(-sum(self.prefix_steps) // PAGE_SIZE)
+            while len(held) < need:
+                held.append(pool.take())
+
+        def free_slot(slot):
+            while held:
+                pool.give_back(held.pop())
+
+        def forward(ctx, want, logits):
+            ids, rows = ctx.token_ids.tolist(), ctx.groups[0].dest_rows.tolist()
+            assert all(0 <= t < V for t in ids), ids
+            assert min(rows) >= 0 and len(set(rows)) == len(rows), rows
+            assert max(ctx.positions.tolist()) < longest
+            self.steps.append(types.SimpleNamespace(ids=ids, positions=ctx.positions.tolist(), rows=rows, most=ctx.max_q_len,
+                                                    lengths=ctx.kv_len.tolist(), bound=ctx.max_kv_len_bound))
+            logits[:] = -1.0
+            for i, w in enumerate(want.tolist()):
+                logits[i, next_token(ids[w])] = 30.0
+
+        group = types.SimpleNamespace(pool=pool, pages=[held])
+        engine = types.SimpleNamespace(max_seq_len=longest, options=types.SimpleNamespace(max_step_tokens=max_step_tokens), workspace=None,
+                                       cache=None, dtype=torch.float32, alloc_slot=lambda: 0, free_slot=free_slot, step=step)
+        runner = SharedPrefixRunner.__new__(SharedPrefixRunner)
+        runner.engine, runner.group, runner.device = engine, group, torch.device("cpu")
+        runner.model = types.SimpleNamespace(vocab_size=V, forward=forward)
+        self.runner, self.pool = runner, pool
+        monkeypatch.setattr(torch.cuda, "synchronize", lambda *a: None)
+        monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t: t)
+        monkeypatch.setattr(ops, "check_kernel_status", lambda device: None)
+        monkeypatch.setattr(ops, "step_tables", self._tables)
+        monkeypatch.setattr(ops, "verify_drafts", self._verify)
+
+    @staticmethod
+    def _tables(lengths, new, rows, old_table, old_held, prefix, old_free, old_n_free, *, page_size, **out):
+        got = tables_oracle(lengths.tolist(), new.tolist(), rows.tolist(), old_table.tolist(), old_held.tolist(), prefix.tolist(),
+                            old_free.tolist(), int(old_n_free), out["table"].shape[1], out["positions"].shape[0], page_size)
+        for k, v in out.items():
+            v.copy_(torch.tensor(got[k], dtype=torch.int32).reshape(v.shape))
+
+    @staticmethod
+    def _verify(logits, tokens, q_start, kv_len, accepted, out, logprobs, kept, heat, u_accept, u_draw, probs, workspace):
+        got = verify_oracle(dict(logits=logits, tokens=tokens, q_start=q_start, kv_len=kv_len, heat=heat, width=out.shape[1], probs=probs,
+                                 u_accept=u_accept, u_draw=u_draw))
+        for mine, theirs in zip((accepted, out, logprobs, kept), got):
+            mine.copy_(torch.as_tensor(theirs).reshape(mine.shape))
+
+    def generate(self, prefix, prompts, n, **more):
+        out, reasons, stats = self.runner.generate(prefix, prompts, n, **more)
+        self.pool.check()
+        assert self.pool.n_held == 0
+        return out, reasons, stats
+
+
+def drafting(answer):
+    """A drafter whose answer is answer(tokens so far, how many were asked for)."""
+    class Drafter:
+        def __init__(self, tokens):
+            self.tokens = list(tokens)
+
+        def extend(self, tokens):
+            self.tokens += tokens
+
+        def draft(self, most):
+            return answer(self.tokens, most)
+    return Drafter
+
+
+@pytest.mark.parametrize("prefix", [0, 5, 64, 150])
+def test_generation_on_the_host_gives_what_the_model_says(monkeypatch, prefix):
+    prompts = [[7, 8], [9], [1, 2, 3] * 30]
+    for drafter in (drafting(lambda t, most: continuation(t[-1], most)), drafting(lambda t, most: [3] * most), drafting(lambda t, most: [])):
+        host = Host(monkeypatch)
+        out, reasons, stats = host.generate([4] * prefix, prompts, 20, drafts=3, drafter=drafter)
+        assert out == [continuation(p[-1], 20) for p in prompts] and reasons == ["length"] * 3
+        assert stats.prefill_tokens == prefix // PAGE_SIZE * PAGE_SIZE + sum(prefix % PAGE_SIZE + len(p) for p in prompts)
+
+
+@pytest.mark.parametrize("bad", [-1, V, 2 ** 31 - 1, -2 ** 31, 2 ** 40])
+def test_a_draft_outside_the_vocabulary_ends_the_drafts(monkeypatch, bad):
+    """Verification refuses such a draft; the step, which reads its embedding first, must not see it."""
+    host = Host(monkeypatch)
+    drafter = drafting(lambda t, most: (continuation(t[-1], 2) + [bad] + [0] * most)[:most])
+    out, _, stats = host.generate([4] * 70, [[7], [9, 2]], 12, drafts=4, drafter=drafter)
+    assert out == [continuation(7, 12), continuation(2, 12)]
+    assert stats.accepted == stats.drafted > 0
+    assert max(s.most for s in host.steps[1:]) == 3
