@@ -187,11 +187,12 @@ class SharedPrefixRunner:
         return pending[len(chosen):]
 
     def _drafts(self, drafter, most: int) -> List[int]:
-        """What a drafter says, up to the first id outside the vocabulary: verification would refuse that one and with it all behind,
-        but the step looks embeddings up before it verifies."""
-        tokens = []
+        """What a drafter says, no more than it was asked for (the request's pages have no room for more), up to the first id outside
+        the vocabulary: verification would refuse that one and with it all behind, but the step looks embeddings up before it
+        verifies."""
+        tokens: List[int] = []
         for t in drafter.draft(most):
-            if not 0 <= int(t) < self.model.vocab_size:
+            if len(tokens) == most or not 0 <= int(t) < self.model.vocab_size:
                 break
             tokens.append(int(t))
         return tokens

@@ -126,3 +126,20 @@ def test_a_draft_outside_the_vocabulary_ends_the_drafts(monkeypatch, bad):
     assert out == [continuation(7, 12), continuation(2, 12)]
     assert stats.accepted == stats.drafted > 0
     assert max(s.most for s in host.steps[1:]) == 3
+
+
+@pytest.mark.parametrize("right", [True, False])
+def test_more_drafts_than_were_asked_for_are_left_out(monkeypatch, right):
+    """They would pass the request's pages and the longest length."""
+    asked = []
+
+    def answer(tokens, most):
+        asked.append(most)
+        return continuation(tokens[-1], 200) if right else [3] * 200
+    host = Host(monkeypatch, pages=1 + 2 * 2, longest=64 + 70)
+    out, reasons, stats = host.generate([4] * 64, [[7, 8, 9], [5]], 60, drafts=3, drafter=drafting(answer))
+    assert out == [continuation(9, 60), continuation(5, 60)] and reasons == ["length"] * 2
+    assert max(s.most for s in host.steps[1:]) == 4 and stats.drafted <= sum(asked)
+    host = Host(monkeypatch, longest=64 + 70)                       # up to the longest length
+    out, reasons, _ = host.generate([4] * 64, [[7, 8, 9]], 999, drafts=5, drafter=drafting(answer))
+    assert out == [continuation(9, 70 - 3 + 1)]
