@@ -58,6 +58,7 @@ class _Request:
     drafter: object
     random: np.random.Generator
     limit: int                  # tokens that its pages have room for
+    held: int                   # pages of its row, the shared ones among them
 
 
 class SharedPrefixRunner:
@@ -143,7 +144,8 @@ class SharedPrefixRunner:
         for r in chosen:
             own = rest + prompts[r]
             held = min(longest, len(prefix) + len(prompts[r]) + max_tokens - 1 + drafts)
-            live.append(_Request(r, own, shared * PAGE_SIZE, -1, drafter(prefix + prompts[r]), np.random.default_rng((seed, r)), held))
+            live.append(_Request(r, own, shared * PAGE_SIZE, -1, drafter(prefix + prompts[r]), np.random.default_rng((seed, r)), held,
+                                 shared))
         mine = [group.pool.take() for _ in range(own_pages)]
         stats.batches += 1
         try:
@@ -220,6 +222,13 @@ class SharedPrefixRunner:
         brought = [q.own + q.drafts for q in live]
         lens = [len(t) for t in brought]
         T = sum(lens)
+        # a step whose tokens have no page must not run: its tables would send them to a row in front of the cache
+        held = [max(q.held, -(-(q.length + n) // PAGE_SIZE)) for q, n in zip(live, lens)]
+        lacking = sum(held) - B * shared - state["free_pages"].shape[0]
+        if lacking > 0 or max(held) > width:
+            raise CacheFull(f"a step of {T} tokens needs {max(lacking, max(held) - width)} pages more than its requests have room for")
+        for q, n in zip(live, held):
+            q.held = n
         ends = np.cumsum(lens)
         # logits are wanted behind a prompt's last token, or behind every token of a step that verifies drafts
         wanted = (ends - 1) if prompts else np.arange(T)

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from janus_b200.cache import PAGE_SIZE
+from janus_b200.cache import PAGE_SIZE, CacheFull
 from janus_b200.cache.pages import PagePool
 from janus_b200.engine import shared_prefix
 from janus_b200.engine.shared_prefix import SharedPrefixRunner
@@ -143,3 +143,13 @@ def test_more_drafts_than_were_asked_for_are_left_out(monkeypatch, right):
     host = Host(monkeypatch, longest=64 + 70)                       # up to the longest length
     out, reasons, _ = host.generate([4] * 64, [[7, 8, 9]], 999, drafts=5, drafter=drafting(answer))
     assert out == [continuation(9, 70 - 3 + 1)]
+
+
+@pytest.mark.parametrize("prompts,pages", [([[7, 8, 9]], 2), ([[7], [8], [9, 9]], 4)])
+def test_a_step_without_pages_for_its_tokens_is_not_launched(monkeypatch, prompts, pages):
+    """Should anything count wrong: the request's row is too narrow, or the others' pages would go."""
+    host = Host(monkeypatch, pages=pages)
+    host.runner._drafts = lambda drafter, most: [3] * (200 if len(prompts) == 1 else 64)
+    with pytest.raises(CacheFull, match="pages more"):
+        host.generate([4] * 64, prompts, 30, drafts=3)
+    assert len(host.steps) == 1 and host.pool.n_held == 0
