@@ -10,8 +10,9 @@ The reference runs one token per row and step and each row's whole prompt
 """
 from __future__ import annotations
 
+import itertools
 import time
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -20,7 +21,7 @@ import torch
 from ..cache import PAGE_SIZE, CacheFull, GroupStepView
 from ..kernels import ops
 from ..parts.attention import GQAttention
-from .generate import GenerationStats
+from .generate import GenerationStats, plan_prompt_steps
 from .step import Engine, StepContext, StepEntry, StepError
 
 
@@ -52,13 +53,14 @@ class LookupDrafter:
 @dataclass
 class _Request:
     index: int
-    own: List[int]              # tokens of its own that the next step brings first: the prompt, then the token it ended with
+    own: List[int]              # its tokens that are not in the cache yet: the prompt, then the token it ended with
     length: int                 # tokens in the cache
     row: int                    # row of the last step's table, -1 before the first
     drafter: object
     random: np.random.Generator
     limit: int                  # tokens that its pages have room for
     held: int                   # pages of its row, the shared ones among them
+    drafts: List[int] = field(default_factory=list)    # of the step that is running
 
 
 class SharedPrefixRunner:
@@ -156,20 +158,29 @@ class SharedPrefixRunner:
             first = True
             while live:
                 t0 = time.perf_counter()
-                for q in live:
-                    room = q.limit - q.length - len(q.own)
-                    wanted = max_tokens - len(outputs[q.index]) - 1
-                    q.drafts = [] if first else self._drafts(q.drafter, max(0, min(drafts, room, wanted)))
-                state, tokens = self._step(live, state, prefix_pages, shared, width, temperature, first)
-                for b, q in enumerate(live):
-                    q.length += len(q.own)
-                    q.row = b
+                if first:
+                    # prompts in as many steps as the limit asks for; every request is in every one of them (the pages of a row
+                    # that nobody goes on with are given back), with no tokens where its turn is over or still to come
+                    tokens: List[List[int]] = [[] for _ in live]
+                    for pieces in plan_prompt_steps([len(q.own) for q in live], self.engine.options.max_step_tokens):
+                        brought, judged = [[] for _ in live], [0] * len(live)
+                        for i, begin, end in pieces:
+                            brought[i], judged[i] = live[i].own[begin:end], int(end == len(live[i].own))
+                        state, got = self._step(live, brought, judged, state, prefix_pages, shared, width, temperature)
+                        tokens = [t + more for t, more in zip(tokens, got)]
+                else:
+                    for q in live:
+                        room = q.limit - q.length - len(q.own)
+                        wanted = max_tokens - len(outputs[q.index]) - 1
+                        q.drafts = self._drafts(q.drafter, max(0, min(drafts, room, wanted)))
+                    brought = [q.own + q.drafts for q in live]
+                    state, tokens = self._step(live, brought, [len(t) for t in brought], state, prefix_pages, shared, width, temperature)
                 still = []
                 for q, got in zip(live, tokens):
                     n = len(got) - 1
                     stats.drafted += len(q.drafts)
                     stats.accepted += n
-                    q.length += n
+                    q.length -= len(q.drafts) - n       # refused drafts
                     q.own = [got[-1]]
                     if self._accept(q, got, outputs, reasons, max_tokens, stop, callback, longest):
                         still.append(q)
@@ -216,10 +227,12 @@ class SharedPrefixRunner:
         q.drafter.extend(got)
         return q.length + 1 <= longest
 
-    def _step(self, live: List[_Request], state, prefix_pages, shared: int, width: int, temperature: float, prompts: bool):
-        """One step of every live request; returns the next state and each request's new tokens."""
+    def _step(self, live: List[_Request], brought: List[List[int]], judged: List[int], state, prefix_pages, shared: int, width: int,
+              temperature: float):
+        """One step: request i brings the tokens brought[i], and the logits behind its last judged[i] tokens verify the drafts among them
+        and give one more (none behind a prompt's part that is not its last).  Returns the next state and each request's new tokens;
+        the requests' lengths, rows and pages are those after the step, refused drafts still counted."""
         B = len(live)
-        brought = [q.own + q.drafts for q in live]
         lens = [len(t) for t in brought]
         T = sum(lens)
         # a step whose tokens have no page must not run: its tables would send them to a row in front of the cache
@@ -229,18 +242,16 @@ class SharedPrefixRunner:
             raise CacheFull(f"a step of {T} tokens needs {max(lacking, max(held) - width)} pages more than its requests have room for")
         for q, n in zip(live, held):
             q.held = n
-        ends = np.cumsum(lens)
-        # logits are wanted behind a prompt's last token, or behind every token of a step that verifies drafts
-        wanted = (ends - 1) if prompts else np.arange(T)
+        all_tokens, at = np.fromiter(itertools.chain.from_iterable(brought), np.int64, T), np.arange(T)
+        wanted = at[at >= np.repeat(np.cumsum(lens) - judged, lens)]
         W = len(wanted)
-        verified = np.concatenate([t[-1:] for t in brought]) if prompts else np.concatenate(brought)
-        starts = np.arange(B + 1) if prompts else np.concatenate([[0], ends])
-        u = np.concatenate([q.random.random(1 + (1 if prompts else n)) for q, n in zip(live, lens)]).astype(np.float32)
+        starts = np.concatenate([[0], np.cumsum(judged)])
+        u = np.concatenate([q.random.random(1 + n) if n else np.zeros(1) for q, n in zip(live, judged)]).astype(np.float32)
         u = np.minimum(u, np.float32(1.0 - 2.0 ** -24))            # (rounding may have made it one)
         first_u = starts[:-1] + np.arange(B)                       # a request's numbers: one for its draw, one for each row's test
         tests = np.delete(u, first_u)
-        parts = [[q.length for q in live], lens, [q.row for q in live], np.concatenate(brought), wanted, verified, starts,
-                 u[first_u].view(np.int32), tests.view(np.int32)]
+        parts = [[q.length for q in live], lens, [q.row for q in live], all_tokens, wanted, all_tokens[wanted], starts, u[first_u].view(np.int32),
+                 tests.view(np.int32)]
         sizes = [len(p) for p in parts]
         offsets = np.concatenate([[0], np.cumsum([(n + 3) // 4 * 4 for n in sizes])])
         host = np.zeros(offsets[-1], dtype=np.int32)
@@ -266,15 +277,20 @@ class SharedPrefixRunner:
         logits = torch.empty((W, self.model.vocab_size), dtype=torch.float32, device=self.device)
         self.model.forward(ctx, want, logits)
 
-        most = 1 if prompts else max(lens)
-        result = new(B, 1 + most)
-        accepted, tokens, kept = new(B), new(B, most), new(B)
-        logprobs = torch.empty((B, most), dtype=torch.float32, device=self.device)
-        ops.verify_drafts(logits, verified, starts, made["kv_len"], accepted, tokens, logprobs, kept, temperature, u_accept.view(torch.float32),
-                          u_draw.view(torch.float32), None, engine.workspace)
-        result[:, 0].copy_(accepted)
-        result[:, 1:].copy_(tokens)
-        back, missing = result.cpu().tolist(), int(made["missing"])
+        for b, (q, n) in enumerate(zip(live, lens)):
+            q.length, q.row = q.length + n, b
+        tokens_of = [[] for _ in live]
+        if W:
+            most = max(judged)
+            result = new(B, 1 + most)
+            accepted, tokens, kept = new(B), new(B, most), new(B)
+            logprobs = torch.empty((B, most), dtype=torch.float32, device=self.device)
+            ops.verify_drafts(logits, verified, starts, made["kv_len"], accepted, tokens, logprobs, kept, temperature,
+                              u_accept.view(torch.float32), u_draw.view(torch.float32), None, engine.workspace)
+            result[:, 0].copy_(accepted)
+            result[:, 1:].copy_(tokens)
+            tokens_of = [row[1: 2 + row[0]] if n else [] for row, n in zip(result.cpu().tolist(), judged)]
+        missing = int(made["missing"])
         if missing:
             raise CacheFull(f"{missing} pages are missing for a step of {T} tokens")
-        return made, [row[1: 2 + row[0]] for row in back]
+        return made, tokens_of

@@ -4,7 +4,6 @@ goes by the last one alone, so what has to come out is known.
 """
 import types
 
-import numpy as np
 import pytest
 import torch
 
@@ -153,3 +152,58 @@ def test_a_step_without_pages_for_its_tokens_is_not_launched(monkeypatch, prompt
     with pytest.raises(CacheFull, match="pages more"):
         host.generate([4] * 64, prompts, 30, drafts=3)
     assert len(host.steps) == 1 and host.pool.n_held == 0
+
+
+@pytest.mark.parametrize("most", [1, 7, 64, 100, 1000, None, 0])
+@pytest.mark.parametrize("prefix", [0, 70, 128])
+def test_prompts_run_in_steps_of_at_most_the_limit(monkeypatch, most, prefix):
+    host = Host(monkeypatch, max_step_tokens=most)
+    prompts = [[7] * 40 + [8], [9], [1, 2, 3] * 30, [5] * 64, [11]]
+    out, reasons, stats = host.generate([4] * prefix, prompts, 9, drafts=3, drafter=drafting(lambda t, n: continuation(t[-1], n)))
+    assert out == [continuation(p[-1], 9) for p in prompts] and reasons == ["length"] * 5
+    brought = sum(prefix % PAGE_SIZE + len(p) for p in prompts)
+    limit = most or brought
+    steps = host.steps[:-(-brought // limit)]
+    assert all(len(s.ids) <= limit for s in steps) and sum(len(s.ids) for s in steps) == brought
+    assert stats.prefill_tokens == prefix // PAGE_SIZE * PAGE_SIZE + brought
+    assert max(host.prefix_steps, default=0) <= (most or prefix)
+    for s in host.steps:
+        assert s.bound >= max(s.lengths)
+
+
+def test_draws_do_not_go_by_how_prompts_were_cut(monkeypatch):
+    prompts = [[7] * 40 + [8], [9], [1, 2, 3] * 30]
+    more = dict(drafts=2, temperature=9.0, seed=5, drafter=drafting(lambda t, n: [3] * n))
+    want = Host(monkeypatch).generate([4] * 70, prompts, 9, **more)[0]
+    assert Host(monkeypatch, max_step_tokens=13).generate([4] * 70, prompts, 9, **more)[0] == want
+    assert any(w != continuation(p[-1], 9) for w, p in zip(want, prompts))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_prompts_cut_in_steps_give_the_same_tokens(tmp_path, dtype):
+    import janus_b200
+    from helpers import BF16_TOL, TINY_A, make_model_dir, random_tokens
+    folder = make_model_dir(TINY_A, str(tmp_path), seed=2, dtype=dtype)
+    prefix = random_tokens(70, 256, 5)
+    prompts = [random_tokens(n, 256, n) for n in (1, 29, 2, 17, 40)]
+    out = []
+    for most in (11, 64, 32768):
+        model = janus_b200.load(folder, dtype=dtype, max_tokens=2048, max_step_tokens=most)
+        tokens, counts, forward = [], [], model.engine.model.forward
+        model.engine.model.forward = lambda ctx, want, logits: (counts.append(ctx.n_tokens), forward(ctx, want, logits))[1]
+        tokens, _ = model.generate_shared(prefix, prompts, max_tokens=10, drafts=3, ignore_eos=True)
+        assert max(counts) <= max(most, 5 * 4) and counts[0] <= most
+        out.append(tokens)
+        want, _ = model.generate([prefix + p for p in prompts], max_tokens=10, ignore_eos=True)
+        if dtype == "float32":
+            assert tokens == want
+    if dtype == "bfloat16":              # sums in another order: a token may differ where two logits nearly tie
+        import plain_llama as P
+        cfg, w = P.read_model_dir(folder)
+        for tokens in out:
+            for p, o in zip(prompts, tokens):
+                logits = P.forward(cfg, w, prefix + p + o)
+                for j, t in enumerate(o):
+                    row = logits[len(prefix) + len(p) - 1 + j]
+                    assert float(row.max() - row[t]) <= BF16_TOL * float(row.abs().max())
