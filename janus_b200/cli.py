@@ -83,20 +83,22 @@ def main(argv=None) -> int:
 
     import janus_b200
     from janus_b200.engine.generate import tokens_held
+    from janus_b200.engine.shared_prefix import room_for_batch
 
     batch = max(1, min(args.batch_size, len(prompts)))
-    more = len(prefix) + args.drafts + 1 if prefix else 0
-    room = sorted((tokens_held(len(p) + more, args.max_tokens, 64) for p in prompts), reverse=True)
-    slots = batch + (1 if prefix else 0)
+    if prefix:                       # the prefix lies in the cache once, in a slot of its own; its requests take none
+        room, slots = room_for_batch(len(prefix), [len(p) for p in prompts], args.max_tokens, max(0, args.drafts), batch), 1
+    else:
+        room, slots = sum(sorted((tokens_held(len(p), args.max_tokens, 64) for p in prompts), reverse=True)[:batch]), batch
     dtype = {"bf16": "bfloat16", "fp32": "float32"}.get(args.dtype, args.dtype)
     if args.random_weights:
         with open(os.path.join(args.model_dir, "config.json")) as f:
             config = json.load(f)
-        model = janus_b200.load_random(config, seed=args.seed_weights, dtype=dtype, max_tokens=sum(room[:batch]) + len(prefix),
+        model = janus_b200.load_random(config, seed=args.seed_weights, dtype=dtype, max_tokens=room,
                                        max_seq_len=args.context_size, max_slots=slots,
                                        max_step_tokens=args.max_step_tokens or None)
     else:
-        model = janus_b200.load(args.model_dir, dtype=dtype, max_tokens=sum(room[:batch]) + len(prefix),
+        model = janus_b200.load(args.model_dir, dtype=dtype, max_tokens=room,
                                 max_seq_len=args.context_size, max_slots=slots,
                                 max_step_tokens=args.max_step_tokens or None)
     if prefix:

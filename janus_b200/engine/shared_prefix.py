@@ -50,6 +50,21 @@ class LookupDrafter:
         return self.tokens[at: at + most] if at is not None else []
 
 
+def pages_behind_prefix(prefix_len: int, prompt_len: int, max_tokens: int, drafts: int, shared: int, longest: Optional[int] = None) -> int:
+    """Pages of its own that a request takes at most, behind `shared` whole pages of the prefix.  (The last token is never fed back;
+    drafts behind it are.)"""
+    held = prefix_len + prompt_len + max(0, max_tokens - 1) + drafts
+    return -(-(held if longest is None else min(longest, held)) // PAGE_SIZE) - shared
+
+
+def room_for_batch(prefix_len: int, prompt_lens: Sequence[int], max_tokens: int, drafts: int, batch_size: int) -> int:
+    """Cache tokens, in whole pages, with room for the prefix once and beside it any `batch_size` of the requests (none of whose prompts is
+    empty)."""
+    shared = prefix_len // PAGE_SIZE
+    own = sorted((pages_behind_prefix(prefix_len, n, max_tokens, drafts, shared) for n in prompt_lens), reverse=True)
+    return (shared + sum(own[:batch_size])) * PAGE_SIZE
+
+
 @dataclass
 class _Request:
     index: int
@@ -132,9 +147,7 @@ class SharedPrefixRunner:
         rest = prefix[shared * PAGE_SIZE:]
         chosen, own_pages, width = [], 0, 0
         for r in pending:
-            # (the last token is never fed back; drafts behind it are)
-            held = min(longest, len(prefix) + len(prompts[r]) + max_tokens - 1 + drafts)
-            pages = (held + PAGE_SIZE - 1) // PAGE_SIZE - shared
+            pages = pages_behind_prefix(len(prefix), len(prompts[r]), max_tokens, drafts, shared, longest)
             if len(chosen) == batch_size or own_pages + pages > group.pool.n_free:
                 break
             chosen.append(r)

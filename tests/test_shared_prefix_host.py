@@ -207,3 +207,70 @@ def test_prompts_cut_in_steps_give_the_same_tokens(tmp_path, dtype):
                 for j, t in enumerate(o):
                     row = logits[len(prefix) + len(p) - 1 + j]
                     assert float(row.max() - row[t]) <= BF16_TOL * float(row.abs().max())
+
+
+def run_command(monkeypatch, tmp_path, args):
+    """The command line over a model that notes how it was asked for and what it was called with."""
+    import json
+    import janus_b200
+    from janus_b200 import cli
+    asked = {}
+
+    class Model:
+        def generate_shared(self, prefix, prompts, **more):
+            asked.update(prefix=prefix, prompts=prompts, **{f"call_{k}": v for k, v in more.items()})
+            return [[1]] * len(prompts), ["length"] * len(prompts), shared_prefix.SharedPrefixStats()
+
+        def generate(self, prompts, **more):
+            return self.generate_shared(None, prompts, **more)
+
+    def load_random(config, **more):
+        asked.update(more)
+        return Model()
+    monkeypatch.setattr(janus_b200, "load_random", load_random)
+    (tmp_path / "config.json").write_text(json.dumps({}))
+    assert cli.main([str(tmp_path)] + args + ["--random-weights", "--json"]) == 0
+    return asked
+
+
+@pytest.mark.parametrize("prefix,lens,batch,n,drafts", [(8192, [100] * 64, 64, 50, 4), (5, [3], 1, 1, 0), (64, [1, 200, 7], 2, 65, 9),
+                                                         (191, [64] * 5, 3, 1, 0), (1, [1, 1], 9, 0, 4)])
+def test_command_line_makes_room_for_the_prefix_once(monkeypatch, tmp_path, prefix, lens, batch, n, drafts):
+    """What it makes room for is what the requests of a batch hold: they run together, and a page less would not do."""
+    prompts = [[7 + i % 9] * m for i, m in enumerate(lens)]
+    text = [" ".join(map(str, p)) for p in prompts]
+    asked = run_command(monkeypatch, tmp_path, text + ["--shared-prefix", " ".join(["4"] * prefix), "--drafts", str(drafts), "--max-tokens", str(n),
+                                                       "--batch-size", str(batch), "--max-step-tokens", "777"])
+    assert asked["prefix"] == [4] * prefix and asked["prompts"] == prompts and asked["call_drafts"] == drafts
+    assert asked["max_step_tokens"] == 777 and asked["call_batch_size"] == min(batch, len(lens))
+    pages = asked["max_tokens"] // PAGE_SIZE
+    assert asked["max_tokens"] % PAGE_SIZE == 0
+    own = sorted((-(-(prefix + m + max(0, n - 1) + drafts) // PAGE_SIZE) - prefix // PAGE_SIZE for m in lens), reverse=True)
+    assert pages == prefix // PAGE_SIZE + sum(own[:batch])
+    if n == 0:
+        return
+    drafter = drafting(lambda t, most: [3] * most)
+    host = Host(monkeypatch, pages=pages, longest=1 << 20)
+    out, _, stats = host.generate([4] * prefix, prompts, n, drafts=drafts, drafter=drafter, batch_size=asked["call_batch_size"])
+    assert out == [continuation(p[-1], n) for p in prompts] and stats.batches == -(-len(lens) // batch)
+
+
+def test_command_line_without_a_prefix_is_as_it_was(monkeypatch, tmp_path):
+    asked = run_command(monkeypatch, tmp_path, ["1 2 3", "4", "5 6", "--max-tokens", "63", "--batch-size", "2"])
+    assert asked["max_tokens"] == 128 + 64 and asked["max_slots"] == 2 and asked["prefix"] is None
+
+
+@pytest.mark.gpu
+def test_command_line_behind_a_prefix(tmp_path, capsys):
+    import json
+    import janus_b200
+    from helpers import TINY_A, make_model_dir, random_tokens
+    from janus_b200 import cli
+    folder = make_model_dir(TINY_A, str(tmp_path), seed=2, dtype="float32")
+    prefix, prompts = random_tokens(70, 256, 5), [random_tokens(n, 256, n) for n in (3, 20, 1)]
+    text = [" ".join(map(str, p)) for p in prompts]
+    assert cli.main([folder] + text + ["--shared-prefix", " ".join(map(str, prefix)), "--drafts", "3", "--max-tokens", "12", "--dtype", "fp32",
+                                       "--ignore-eos", "--json"]) == 0
+    got = json.loads(capsys.readouterr().out.strip().splitlines()[-1])["tokens"]
+    want, _ = janus_b200.load(folder, dtype="float32", max_tokens=1024).generate([prefix + p for p in prompts], max_tokens=12, ignore_eos=True)
+    assert got == want
