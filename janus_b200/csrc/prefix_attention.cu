@@ -794,13 +794,15 @@ struct Cursor {
   int seq, kvh, rb, tile;           // sequence; kv head, block of 16 rows; tile of the row's keys
   int tiles, row_blocks, start, q_len;
   int shared;                       // tiles of the prefix in front, where the list holds them
+  int most;                         // tiles of own keys at most
 };
-// What sequence `seq` adds to the list: every row has a tile, also one that sees no key of its own.
-__device__ __forceinline__ void look_up(const Step& s, int seq, int shared, Cursor& c) {
+// What sequence `seq` adds to the list: every row has a tile, also one that sees no key of its own.  No more than `most` behind the
+// prefix, by the caller's bound of the lengths: the places for partial results are counted by it, whatever kv_len says.
+__device__ __forceinline__ void look_up(const Step& s, int seq, int shared, int most, Cursor& c) {
   c.seq = seq, c.start = s.q_start[seq], c.q_len = s.q_start[seq + 1] - c.start;
   c.row_blocks = c.q_len > 0 ? (c.q_len * (s.nh / s.nkv) + 15) / 16 : 0;
-  c.shared = shared;
-  c.tiles = shared + min(max((s.kv_len[seq] - s.prefix_len + OWN_KEYS - 1) / OWN_KEYS, 1), max(s.width * OWN_HALVES, 1));
+  c.shared = shared, c.most = most;
+  c.tiles = shared + min(max((s.kv_len[seq] - s.prefix_len + OWN_KEYS - 1) / OWN_KEYS, 1), most);
 }
 __device__ __forceinline__ int places(const Step& s, const Cursor& c) { return s.nkv * c.row_blocks * c.tiles; }
 __device__ __forceinline__ void step_on(const Step& s, Cursor& c) {
@@ -812,7 +814,7 @@ __device__ __forceinline__ void step_on(const Step& s, Cursor& c) {
   c.kvh = 0;
   do {
     if (c.seq + 1 >= s.n_seqs) return;   // (behind the list's end: nobody goes there)
-    look_up(s, c.seq + 1, c.shared, c);
+    look_up(s, c.seq + 1, c.shared, c.most, c);
   } while (c.row_blocks == 0);
 }
 
@@ -820,7 +822,7 @@ template <int HDC, int STAGES>
 __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                           const bf16* __restrict__ q, float* __restrict__ part_o, float2* __restrict__ part_ml,
                                                           int* __restrict__ own_count, const Step s, int first_slot, int after_prefix,
-                                                          int shared, int fewest, int* __restrict__ status) {
+                                                          int shared, int most, int fewest, int* __restrict__ status) {
   typedef Own<HDC, STAGES> C;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = (uint64_t*)(smem + C::RING);
@@ -840,7 +842,7 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
 #pragma unroll 4
   for (int i = seq0; i < seq1; ++i) {
     Cursor x;
-    look_up(s, i, shared, x);
+    look_up(s, i, shared, most, x);
     mine += places(s, x);
   }
   int up = mine;
@@ -856,7 +858,7 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const __grid_constant_
     const int owner = __ffs(__ballot_sync(0xffffffffu, begin < up)) - 1;
     int before = __shfl_sync(0xffffffffu, up - mine, owner);
     for (int i = owner * chunk;; ++i) {
-      look_up(s, i, shared, c);
+      look_up(s, i, shared, most, c);
       const int n = places(s, c);
       if (begin < before + n) break;
       before += n;
@@ -1079,7 +1081,7 @@ cudaError_t tc_pick(int nt, dim3 grid, cudaStream_t stream, const CUtensorMap* m
 
 template <int HDC, int STAGES>
 cudaError_t own_go(int blocks, cudaStream_t stream, const CUtensorMap* maps, const bf16* q, float* part_o, float2* part_ml, int* own_count,
-                   const Step& s, int first_slot, int after_prefix, int shared, int fewest, int* status) {
+                   const Step& s, int first_slot, int after_prefix, int shared, int most, int fewest, int* status) {
   typedef Own<HDC, STAGES> C;
   static bool configured = false;
   if (!configured) {
@@ -1089,7 +1091,7 @@ cudaError_t own_go(int blocks, cudaStream_t stream, const CUtensorMap* maps, con
   }
   jb::Launch cfg(dim3(blocks), dim3(OWN_THREADS), C::SMEM, stream);
   return cudaLaunchKernelEx(&cfg.c, own_kernel<HDC, STAGES>, maps[0], maps[1], q, part_o, part_ml, own_count, s, first_slot, after_prefix,
-                            shared, fewest, status);
+                            shared, most, fewest, status);
 }
 
 }  // namespace
@@ -1163,14 +1165,15 @@ JB_EXPORT int jb_attention_prefix_bf16(const void* tensors, const void* sizes, i
   const int shared = shared_per > 0 ? 0 : (prefix_len + OWN_KEYS - 1) / OWN_KEYS;
   const int row_blocks = (max_q_len * G + 15) / 16;
   const int own_tiles_most = (max_kv_len - prefix_len + OWN_KEYS - 1) / OWN_KEYS, tiles_most = shared + (own_tiles_most < 1 ? 1 : own_tiles_most);
+  const int in_table = s.width > 0 ? s.width * OWN_HALVES : 1, own_bound = tiles_most - shared < in_table ? tiles_most - shared : in_table;
   JB_REFUSE(own_ctas < 1 || fewest < 1 || own_most > 64 || (tiles_most + fewest - 2) / fewest + 1 > own_most ||
                 (long long)n_seqs * nkv * row_blocks * (tiles_most < 1 ? 1 : tiles_most) > 0x3fffffffll,
             "attention_prefix: %d blocks for %d tiles of own keys of %d sequences", own_ctas, tiles_most, n_seqs);
   if (!make_maps(nullptr, &maps[1], &maps[2], q, k_cache, v_cache, s, n_pages, OWN_KEYS)) return JB_ERR_TENSORMAP;
   const int behind = shared_per > 0;
-  if (hd > 128) e = own_go<256, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, shared, fewest, status);
-  else if (hd > 64) e = own_go<128, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, shared, fewest, status);
-  else e = own_go<64, 2>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, shared, fewest, status);
+  if (hd > 128) e = own_go<256, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, shared, own_bound, fewest, status);
+  else if (hd > 64) e = own_go<128, 1>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, shared, own_bound, fewest, status);
+  else e = own_go<64, 2>(own_ctas, stream, maps + 1, qb, part_o, ml, own_count, s, most, behind, shared, own_bound, fewest, status);
   if (e != cudaSuccess) return (int)e;
   return (int)join_go<bf16>(stream, qb, kb, vb, ob, part_o, ml, own_count, s, parts, own_most);
 }

@@ -88,6 +88,33 @@ def test_ranges_of_the_prefix_as_they_are_launched():
                 assert max(c * per, i * blocks) - i * blocks < real
 
 
+def test_lengths_beyond_the_bound_take_no_places_beyond_the_scratch():
+    """A caller's bound that is too low: shares counted by the device's lengths have more results than places, by the bound they fit."""
+    beyond = 0
+    for new, owned, prefix, nkv, group, hd in cases(200):
+        bound = max(1, max(owned) // 5)
+        plan = ops.attention_prefix_plan(sum(new), len(new), max(new), prefix, bound, nkv * group, nkv, hd)
+        args = (plan, new, owned, prefix, nkv, group, plan[1] > 0)
+        beyond += max(b[4] for b in own_shares(*args)) > plan[6]
+        assert max(b[4] for b in own_shares(*args, bound=max(1, -(-bound // 32)))) <= plan[6]
+    assert beyond > 10
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("prefix,n,new", [(0, 5, 1), (100, 5, 1), (3000, 40, 2), (3000, 6, 90)])
+def test_bounds_that_are_too_low_write_nothing_beyond_the_scratch(dtype, prefix, n, new):
+    from janus_b200.engine.workspace import Workspace
+    c = attention_case(14, dtype, 8, 2, 64, prefix, [new] * n, [new + 400 + 97 * i for i in range(n)])
+    c["workspace"], c["most"] = Workspace(torch.device("cuda")), prefix + 40
+    _, floats, _ = ops._attention_prefix_sizes(prefix, c["table"].stride(0), c["table"].shape[1], n * new, c["k"].shape[0], n, 8, 2, 64, 64, new,
+                                               c["most"], float(c["scale"]), dtype is torch.float32)
+    scratch = c["workspace"].get("prefix_parts", (40 * floats,), torch.float32).fill_(3.0)
+    attention(c)
+    assert (scratch[floats:] == 3.0).all()
+    ops.check_kernel_status(torch.device("cuda"))
+
+
 @gpu
 @pytest.mark.parametrize("heads,kv_heads,dim,n,new,before,prefix", [
     (24, 8, 128, 48, 6, 200, 4096),      # heads of a group that do not divide 16 rows
