@@ -1,0 +1,71 @@
+"""Refusals of the faces of a step behind a shared prefix that go by sizes and places alone: on the host, with nothing launched."""
+import types
+
+import pytest
+import torch
+
+from janus_b200.kernels import ops
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The entry points' calls, which do nothing."""
+    calls = []
+
+    def entry(name):
+        return lambda *args: (calls.append(name), 0)[1]
+    names = ("jb_step_tables", "jb_attention_prefix_f32", "jb_attention_prefix_bf16", "jb_verify_drafts")
+    monkeypatch.setattr(ops, "_lib", lambda *args: types.SimpleNamespace(**{n: entry(n) for n in names}))
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "kernel_status", lambda device: torch.zeros(1, dtype=torch.int32))
+    with ops.unchecked():           # (the checks of tensors want a device)
+        yield calls
+
+
+INPUTS = ("lengths", "new_tokens", "rows", "old_table", "old_held", "prefix_pages", "old_free", "old_n_free")
+
+
+def tables_tensors(B=5, B0=4, W0=6, W=8, P=2, N=30, T=40):
+    z = lambda *shape: torch.zeros(shape, dtype=torch.int32)      # noqa: E731
+    return dict(lengths=z(B), new_tokens=z(B), rows=z(B), old_table=z(B0, W0), old_held=z(B0), prefix_pages=z(P), old_free=z(N), old_n_free=z(1),
+                q_start=z(B + 1), kv_len=z(B), positions=z(T), token_seq=z(T), dest_rows=z(T), table=z(B, W), held=z(B), free_pages=z(N),
+                n_free=z(1), missing=z(1))
+
+
+def run_tables(t):
+    ops.step_tables(*(t[n] for n in INPUTS), **{n: v for n, v in t.items() if n not in INPUTS}, page_size=64)
+
+
+def laid_over(t, first, second, shift):
+    """`first` and `second` as views of one tensor, the second `shift` numbers behind the first's begin."""
+    n, m = t[first].numel(), t[second].numel()
+    low = min(0, shift)
+    both = torch.zeros(max(n, shift + m) - low, dtype=torch.int32)
+    return {**t, first: both[-low:n - low].view(t[first].shape), second: both[shift - low:shift - low + m].view(t[second].shape)}
+
+
+@pytest.mark.parametrize("made", ["q_start", "table", "free_pages", "n_free"])
+@pytest.mark.parametrize("given", ["lengths", "old_table", "old_free", "old_n_free"])
+def test_tables_are_not_made_over_what_they_are_made_from(launches, given, made):
+    t = tables_tensors()
+    n, m = t[given].numel(), t[made].numel()
+    for shift in {0, n - 1, 1 - m, n // 2, -(m // 2)}:
+        with pytest.raises(ops.KernelError, match="cannot lie"):
+            run_tables(laid_over(t, given, made, shift))
+    assert not launches
+    for shift in (n, -m):                                          # side by side
+        run_tables(laid_over(t, given, made, shift))
+    assert launches == ["jb_step_tables"] * 2
+
+
+def test_tables_are_not_made_over_each_other_and_inputs_may_share(launches):
+    t = tables_tensors()
+    with pytest.raises(ops.KernelError, match="each other"):
+        run_tables(laid_over(t, "positions", "dest_rows", 39))
+    assert not launches
+    run_tables(laid_over(t, "lengths", "old_table", 1))
+    run_tables({**t, "new_tokens": t["lengths"]})
+    run_tables(tables_tensors(B0=0, P=0, T=0))
+    everything = torch.zeros(sum(v.numel() for v in t.values()), dtype=torch.int32)
+    run_tables({k: piece.view(v.shape) for (k, v), piece in zip(t.items(), everything.split([v.numel() for v in t.values()]))})
+    assert len(launches) == 4
