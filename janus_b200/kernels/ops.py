@@ -2482,6 +2482,9 @@ def attention_prefix(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     T, n_seqs, prefix_len = q.shape[0], kv_len.shape[0], int(prefix_len)
     if dtype_code(q.dtype) == BF16 and hd % 8:
         raise KernelError(f"attention_prefix: bfloat16 heads of {hd} numbers (they must be multiples of 8)")
+    if nkv < 1 or nh < 1 or nh % nkv or not 1 <= hd <= 256 or (q.dtype is torch.bfloat16 and nh // nkv > 128):
+        raise KernelError(f"attention_prefix: {nh} heads over {nkv} kv heads of {hd} numbers (a multiple of the kv heads, groups of up to 128 "
+                          f"in bfloat16, up to 256 numbers)")
     if _checks[0]:
         width, cache = (T, nh * hd), (k_cache.shape[0], nkv, page_size, hd)
         _need_all("attention_prefix", q.dtype, (q, out, k_cache, v_cache), (width, width, cache, cache), ("q", "out", "k cache", "v cache"))

@@ -69,3 +69,26 @@ def test_tables_are_not_made_over_each_other_and_inputs_may_share(launches):
     everything = torch.zeros(sum(v.numel() for v in t.values()), dtype=torch.int32)
     run_tables({k: piece.view(v.shape) for (k, v), piece in zip(t.items(), everything.split([v.numel() for v in t.values()]))})
     assert len(launches) == 4
+
+
+def run_attention(dtype=torch.bfloat16, nh=8, nkv=2, hd=64, T=3, n=2):
+    z = lambda *shape, dtype=torch.int32: torch.zeros(shape, dtype=dtype)      # noqa: E731
+    from janus_b200.engine.workspace import Workspace
+    ops.attention_prefix(z(T, nh * hd, dtype=dtype), z(4, max(nkv, 0), 64, hd, dtype=dtype), z(4, max(nkv, 0), 64, hd, dtype=dtype),
+                         z(T, nh * hd, dtype=dtype), z(1), 64, z(n, 1), z(n + 1), z(n), z(T), nh, nkv, hd, 64, 0.125,
+                         Workspace(torch.device("cpu")), 2, 128)
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", [
+    (torch.bfloat16, 129, 1, 64), (torch.bfloat16, 516, 4, 64), (torch.bfloat16, 2, 4, 64), (torch.bfloat16, 6, 4, 64), (torch.bfloat16, 8, 0, 64),
+    (torch.float32, 2, 4, 64), (torch.float32, 7, 2, 64), (torch.float32, 8, 0, 64), (torch.float32, 4, 2, 257), (torch.bfloat16, 4, 2, 264)])
+def test_attention_refuses_heads_that_it_does_not_take(launches, dtype, nh, nkv, hd):
+    with pytest.raises(ops.KernelError, match="attention_prefix"):
+        run_attention(dtype, nh, nkv, hd)
+    assert not launches
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,hd", [(torch.bfloat16, 128, 1, 64), (torch.bfloat16, 7, 7, 256), (torch.float32, 129, 1, 37), (torch.float32, 8, 4, 256)])
+def test_attention_takes_the_heads_at_its_limits(launches, dtype, nh, nkv, hd):
+    run_attention(dtype, nh, nkv, hd)
+    assert len(launches) == 1
