@@ -33,13 +33,21 @@ def dtype_code(dtype: torch.dtype) -> int:
 _scope_stream = [None]
 
 
-# (`torch.cuda.current_stream()` makes a stream object of what is one number: several microseconds a launch)
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+def _stream_reader():
+    """What says which stream is the current one.  `torch.cuda.current_stream()` makes a stream object of what is one number, several
+    microseconds a launch; the number itself has names that are torch's own, which a torch without CUDA, or another one, may lack."""
+    raw, device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
+    if raw is None or device is None:
+        return lambda: torch.cuda.current_stream().cuda_stream
+    return lambda: raw(device())
+
+
+_current_stream = _stream_reader()
 
 
 def _stream() -> int:
     s = _scope_stream[0]
-    return s if s is not None else _raw_stream(_current_device())
+    return s if s is not None else _current_stream()
 
 
 @contextlib.contextmanager

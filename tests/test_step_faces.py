@@ -92,3 +92,16 @@ def test_attention_refuses_heads_that_it_does_not_take(launches, dtype, nh, nkv,
 def test_attention_takes_the_heads_at_its_limits(launches, dtype, nh, nkv, hd):
     run_attention(dtype, nh, nkv, hd)
     assert len(launches) == 1
+
+
+@pytest.mark.parametrize("name", ["_cuda_getCurrentRawStream", "_cuda_getDevice"])
+def test_the_current_stream_is_found_without_names_of_torchs_own(name):
+    """A torch that lacks them (one without CUDA, a later one) still imports the library, and the public way answers."""
+    import os
+    import subprocess
+    import sys
+    code = (f"import types, torch\ndel torch._C.{name}\nimport janus_b200.kernels.ops as ops\n"
+            "torch.cuda.current_stream = lambda: types.SimpleNamespace(cuda_stream=1234)\nassert ops._stream() == 1234")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(ops.__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(root), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
