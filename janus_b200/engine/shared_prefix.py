@@ -65,6 +65,11 @@ def room_for_batch(prefix_len: int, prompt_lens: Sequence[int], max_tokens: int,
     return (shared + sum(own[:batch_size])) * PAGE_SIZE
 
 
+def _random(seed: int, request: int) -> np.random.Generator:
+    """A request's random numbers.  A negative seed stands for its 64 bits, as the plain generation's sampler takes it."""
+    return np.random.default_rng((int(seed) if seed >= 0 else int(seed) % (1 << 64), request))
+
+
 @dataclass
 class _Request:
     index: int
@@ -159,7 +164,7 @@ class SharedPrefixRunner:
         for r in chosen:
             own = rest + prompts[r]
             held = min(longest, len(prefix) + len(prompts[r]) + max_tokens - 1 + drafts)
-            live.append(_Request(r, own, shared * PAGE_SIZE, -1, drafter(prefix + prompts[r]), np.random.default_rng((seed, r)), held,
+            live.append(_Request(r, own, shared * PAGE_SIZE, -1, drafter(prefix + prompts[r]), _random(seed, r), held,
                                  shared))
         mine = [group.pool.take() for _ in range(own_pages)]
         stats.batches += 1

@@ -274,3 +274,10 @@ def test_command_line_behind_a_prefix(tmp_path, capsys):
     got = json.loads(capsys.readouterr().out.strip().splitlines()[-1])["tokens"]
     want, _ = janus_b200.load(folder, dtype="float32", max_tokens=1024).generate([prefix + p for p in prompts], max_tokens=12, ignore_eos=True)
     assert got == want
+
+
+def test_any_whole_number_is_a_seed(monkeypatch):
+    """As for the plain generation; a seed repeats its numbers, another one has others."""
+    more = dict(drafts=2, temperature=9.0, drafter=drafting(lambda t, n: [3] * n))
+    seen = [Host(monkeypatch).generate([4] * 70, [[7], [8]], 20, seed=seed, **more)[0] for seed in (-1, -1, -2, 0, 1, 2 ** 40)]
+    assert seen[0] == seen[1] and all(a != b for i, a in enumerate(seen[1:]) for b in seen[2 + i:])
