@@ -405,7 +405,9 @@ __global__ void __launch_bounds__(THREADS, 2) decide_kernel(const float* __restr
       if (k <= accepted) {
         v = k < accepted ? tokens[lo + k + 1] : token;
         const float x = k < accepted ? row_x[k] : logits[(size_t)(lo + k) * V + v], gap = x == row_top[k] ? 0.0f : x - row_top[k];
-        p = row_sum[k] > 0.0f ? gap * (heat > 0.0f ? 1.0f / heat : 1.0f) - logf(row_sum[k]) : -CUDART_INF_F;
+        // (one over a temperature below 2.9e-39 is infinite, and 0 times it would not be a number)
+        const float scaled = gap == 0.0f ? 0.0f : gap * (heat > 0.0f ? 1.0f / heat : 1.0f);
+        p = row_sum[k] > 0.0f ? scaled - logf(row_sum[k]) : -CUDART_INF_F;
       }
       my[k] = v, lp[k] = p;
     }
