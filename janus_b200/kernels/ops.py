@@ -2627,7 +2627,12 @@ def attention_prefix_plan_f32(T: int, n_seqs: int, max_q_len: int, prefix_len: i
     # A block loads a page, then works on it: short ranges of own pages, several of which share an SM (29 tokens of 16 sequences
     # with up to 254 own tokens behind 2,050: 47 us by two ranges, 41 by four; 40 single tokens with 556 behind 3,000: 164 by one, 131
     # by five; by nine of one page 139).
-    return rows, own_rows, splits, min(32, max(1, min(own_pages, 4), (own_pages + 1) // 2))
+    own = max(1, min(own_pages, 4), (own_pages + 1) // 2)
+    # ... but no more than make eight times the blocks that run at once: every range is a partial result for every row, and rows alone may
+    # fill the machine.  32 heads over 8 of 128: 8 prompts of 2,000 tokens 13.7 ms by one range, 16.2 by sixteen, 8 of 4,000 1.1 GB of
+    # partial results and 17; one of 1,500 0.83 ms by four, 0.92 by one, 0.94 by twelve; 64 single tokens with 700 0.15 by five or six.
+    row_blocks = nkv * min(n_seqs * -(-max_q_len * group // own_rows), T * group // own_rows + n_seqs)
+    return rows, own_rows, splits, min(32, own, max(1, -(-8 * 2 * sms // max(1, row_blocks))))
 
 
 def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, accepted: torch.Tensor,

@@ -100,6 +100,27 @@ def test_lengths_beyond_the_bound_take_no_places_beyond_the_scratch():
     assert beyond > 10
 
 
+def test_scratch_of_float32_goes_by_the_rows():
+    """Two results a row where rows alone fill the machine; where they do not, no more than 64 rows each of ranges that fill it eight
+    times (and of the prefix twice), whatever the lengths."""
+    rng = np.random.default_rng(4)
+    for _ in range(2000):
+        group, nkv, hd = int(rng.integers(1, 17)), int(rng.integers(1, 33)), int(rng.choice([64, 128, 256]))
+        n, new = int(rng.integers(1, 65)), int(2 ** rng.uniform(0, 12))
+        T, prefix, own = max(new, int(n * new * rng.uniform(0.3, 1.0))), int(2 ** rng.uniform(0, 14)), new + int(2 ** rng.uniform(0, 14))
+        _, floats, _ = ops._attention_prefix_sizes(prefix, 99, 99, T, 999, n, nkv * group, nkv, hd, 64, new, prefix + own, 1.0, True)
+        rows = T * nkv * group
+        assert floats <= (2 * rows + 64 * (8 * 296 + 2 * 296 + nkv * n * 2)) * (hd + 2) + rows, (group, nkv, hd, n, new, T)
+    _, floats, _ = ops._attention_prefix_sizes(1000, 99, 99, 32000, 999, 8, 32, 8, 128, 64, 4000, 5000, 1.0, True)
+    assert floats * 4 < 1.1e9
+
+
+@gpu
+def test_attention_of_float32_prompts_beside_single_tokens():
+    c = attention_case(15, torch.float32, 8, 2, 64, 200, [700, 1, 300, 0, 1], [900, 2000, 300, 50, 1])
+    close(attention(c), attention_oracle(c), torch.float32)
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("prefix,n,new", [(0, 5, 1), (100, 5, 1), (3000, 40, 2), (3000, 6, 90)])
