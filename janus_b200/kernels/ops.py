@@ -2546,10 +2546,15 @@ def _attention_prefix_sizes(prefix_len: int, ld_table: int, width: int, T: int, 
 
 
 _PREFIX_MOST_RANGES = 64       # partial results over the prefix that a row's join takes
-# Tiles of 32 keys of all rows together, from which the prefix has a launch of its own.  A warp takes 2 us a tile, one after another, a
-# launch costs the host 2.5: 384 tiles (4 sequences behind 173 tokens) 6.8 us together and 8.6 apart, 1,184 (behind 1,000) 10.9 and
-# 9.5, 1,920 13.3 and 11.5.
-_PREFIX_APART_FROM = 1200
+# Few rows behind a short prefix walk it with their own keys: a launch less, which is 2.1 us of the host's 14.3 a call.  That pays while
+# the device hides behind the 12.2 that are left, and two things take it beyond: partial results on their way out and back (numbers of
+# them: a row has one for every tile of 32 keys), and warps that have more than a tile (tiles of all rows x numbers of a head).  By
+# calls one after another, together and apart: 4 sequences behind 1,000, 32 heads over 8 of 128 (0.6 million numbers, 139,000) 12.4 and 14.3
+# us, 4 tokens of each (2.2 million) 15.2 and 14.3; 8 behind 600 (0.7, 172,000) 12.4 and 14.3, behind 1,800 (1.9, 483,000) 15.4 and
+# 14.5; 64 of two tokens behind 1,146, 2 heads of 80 (0.8, 389,000) 15.4 and 14.2.  263 shapes: 0.1 us a call above the better form on
+# average.  (Where launches cost the host nothing, in a graph, the line would lie at 15 to 20 tiles a row: 4 sequences behind 400
+# 7.6 and 7.9 us on the device, behind 600 8.7 and 8.0, behind 1,000 10.4 and 8.1.)
+_PREFIX_TOGETHER_PARTS, _PREFIX_TOGETHER_KEYS = 1_000_000, 240_000
 
 
 def _prefix_ranges(items: int, blocks: int, most_ctas: int, hd: int):
@@ -2597,7 +2602,7 @@ def attention_prefix_plan(T: int, n_seqs: int, max_q_len: int, prefix_len: int, 
     own_blocks = max(1, (max_own + 31) // 32)
     # few rows behind a short prefix: they walk it themselves, a launch less
     tiles = (prefix_len + 31) // 32 + own_blocks
-    if row_blocks * tiles <= _PREFIX_APART_FROM and tiles <= 60:
+    if T * nh * tiles * hd <= _PREFIX_TOGETHER_PARTS and row_blocks * tiles * hd <= _PREFIX_TOGETHER_KEYS and tiles <= 60:
         return 1, 0, 0, 0, max(1, min((3 if hd <= 128 else 1) * sms, -(-row_blocks * tiles // 4))), 1, tiles
     # Own keys' mean length is not known: a third of the longest.  Where they take 4 us or more, the prefix leaves 20 multiprocessors to
     # them (72 sequences behind 2,036: 29 and 24 us).  One tile a block over the prefix: with two its keys are fetched once for both, but

@@ -100,6 +100,16 @@ def test_lengths_beyond_the_bound_take_no_places_beyond_the_scratch():
     assert beyond > 10
 
 
+@pytest.mark.parametrize("n,new,prefix,heads,kv_heads,dim,together", [
+    (4, 1, 1000, 32, 8, 128, True), (16, 1, 400, 32, 8, 64, True), (8, 1, 600, 32, 8, 128, True), (8, 1, 1400, 32, 8, 64, True),
+    (4, 4, 1000, 32, 8, 128, False), (4, 4, 1600, 32, 8, 128, False), (8, 1, 1800, 32, 8, 128, False), (64, 2, 1146, 2, 2, 80, False),
+    (4, 1, 903, 32, 16, 256, False), (32, 1, 400, 32, 8, 128, False)])
+def test_who_walks_the_prefix_is_the_faster_form_by_calls(n, new, prefix, heads, kv_heads, dim, together):
+    """Shapes on both sides of the line whose forms were timed 0.9 to 5 us apart."""
+    plan = ops.attention_prefix_plan(n * new, n, new, prefix, 60, heads, kv_heads, dim)
+    assert (plan[1] == 0) == together
+
+
 def test_scratch_of_float32_goes_by_the_rows():
     """Two results a row where rows alone fill the machine; where they do not, no more than 64 rows each of ranges that fill it eight
     times (and of the prefix twice), whatever the lengths."""
