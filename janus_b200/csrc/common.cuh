@@ -16,6 +16,7 @@
 #define JB_ERR_BAD_SIZE 10001     // a size the kernel cannot take (message printed to stderr)
 #define JB_ERR_BAD_DTYPE 10002
 #define JB_ERR_TENSORMAP 10003
+#define JB_ERR_OVERLAP 10004      // an output lies over an input or another output
 
 #define JB_EXPORT extern "C" __attribute__((visibility("default")))
 

@@ -195,6 +195,19 @@ __global__ void __launch_bounds__(THREADS) step_tables_kernel(const Args a) {
   }
 }
 
+// Whether one of the ten outputs lies over one of the eight inputs or over another output, wherever each begins (inputs may share places).
+bool made_over_others(const Args& a) {
+  const char* at[18];
+  static_assert(offsetof(Args, B) == sizeof(at), "18 tensors, the inputs first");
+  memcpy(at, &a, sizeof(at));
+  const size_t n[18] = {(size_t)a.B, (size_t)a.B, (size_t)a.B, (size_t)a.B0 * a.W0, (size_t)a.B0, (size_t)a.P, (size_t)a.N, 1, (size_t)a.B + 1, (size_t)a.B,
+                        (size_t)a.T, (size_t)a.T, (size_t)a.T, (size_t)a.B * a.W, (size_t)a.B, (size_t)a.N, 1, 1};
+  for (int i = 8; i < 18; ++i)
+    for (int j = 0; j < i; ++j)
+      if (n[i] > 0 && n[j] > 0 && at[i] < at[j] + 4 * n[j] && at[j] < at[i] + 4 * n[i]) return true;
+  return false;
+}
+
 size_t smem_for(int B, int B0) { return (size_t)(2 * (B + 1) + B0 + 1 + (B0 + 31) / 32) * sizeof(int); }
 
 }  // namespace
@@ -209,6 +222,7 @@ JB_EXPORT int jb_step_tables(const void* given, cudaStream_t stream) {
   JB_REFUSE(B < 0 || B0 < 0 || T < 0 || W <= 0 || W0 < 0 || P < 0 || N < 0 || page_size <= 0, "step_tables: sizes %d %d %d %d %d %d %d %d", B, B0,
             T, W, W0, P, N, page_size);
   JB_REFUSE(W < W0 || P > W, "step_tables: a table of %d pages a row cannot take over rows of %d behind %d shared pages", W, W0, P);
+  if (made_over_others(a)) return JB_ERR_OVERLAP;
   const size_t smem = smem_for(B, B0);
   JB_REFUSE(smem > 200 * 1024, "step_tables: %d requests after %d are more than a block's memory holds sums of", B, B0);
   if (smem > 48 * 1024) {

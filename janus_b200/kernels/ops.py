@@ -205,7 +205,8 @@ def _check(code: int, what: str, kernels: int = 1) -> None:
         return
     if code >= 10000:
         names = {10001: "size not supported (see stderr)", 10002: "dtype not supported",
-                 10003: "tensor map could not be encoded"}
+                 10003: "tensor map could not be encoded",
+                 10004: "what is made cannot lie where the old tables and lists do, or in each other's place"}
         raise KernelError(f"{what}: {names.get(code, 'error')} (code {code})")
     raise KernelError(f"{what}: CUDA error {code}")
 
@@ -2454,24 +2455,10 @@ def step_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, rows: torch.Ten
     if W < W0 or P > W:
         raise KernelError(f"step_tables: a table of {W} pages a row cannot take over rows of {W0} behind {P} shared pages")
     at = [t.data_ptr() for t in tensors]
-    # what is made lies by itself: in the order of their places, none begins before one in front of it ends (inputs may share theirs)
-    ends = made_ends = 0
-    for start, n, made in sorted(zip(at, (B, B, B, B0 * W0, B0, P, N, 1, B + 1, B, T, T, T, B * W, B, N, 1, 1), _STEP_TABLES_MADE)):
-        if n:
-            if start < made_ends or (made and start < ends):
-                raise KernelError("step_tables: what is made cannot lie where the old tables and lists do, or in each other's place")
-            end = start + 4 * n
-            if end > ends:
-                ends = end
-            if made:
-                made_ends = end
     _check(_lib("step_tables").jb_step_tables(_STEP_TABLES(*at, B, B0, T, W0, W, P, N, int(page_size)), _stream()), "step_tables")
 
 
 _STEP_TABLES = struct.Struct("18P8i").pack     # `Args` of csrc/step_tables.cu, but for its last member
-
-
-_STEP_TABLES_MADE = (0,) * 8 + (1,) * 10
 
 
 _STEP_TABLES_NAMES = ("lengths", "new tokens", "rows", "table", "held pages", "prefix pages", "free pages", "number of free pages",
