@@ -14,8 +14,9 @@
 // the measured 6,537 GB/s and 1,637 TFLOP/s, with 32 heads over 8 of 128 numbers:
 //   64 single tokens behind 8,192, 30 to 700 own: 29 us; the prefix 18 us of them by 128 blocks, each waiting on its own row tile's
 //     chain (scores, weights, values), the own keys' 40 MB beside it, 5 us for the join's launch and one round of loads
-//   256 behind 16,384, 3 to 2,500 own: 122 us; prefix products at 1,100 TFLOP/s (of all multiprocessors) while they run, own keys at
-//     5.2 TB/s while they do, each on a part of the multiprocessors
+//   256 behind 16,384, 3 to 2,500 own: 122 us in the first 0.1 s of such calls, 140 once the power limit has lowered the clock; prefix
+//     products at 1,100 TFLOP/s (of all multiprocessors) while they run, own keys at 5.2 TB/s while they do, each on a part of the
+//     multiprocessors
 //   8 prompts of up to 510 tokens behind 4,100: 99 us; the prefix 80 us at 57 % of the tensor pipe's cycles (a block of keys for two tiles
 //     takes 3,400 cycles: 2,048 of products, 2,048 of the special-function unit, which hide each other in part), own keys the rest
 #include <cuda.h>
