@@ -34,9 +34,12 @@ class SharedPrefixStats(GenerationStats):
 class LookupDrafter:
     """Drafts for one request from its own text: the tokens that followed the last time its last two tokens stood there."""
 
-    def __init__(self, tokens: Sequence[int]):
-        self.tokens: List[int] = []
+    def __init__(self, tokens: Sequence[int], before: Optional["LookupDrafter"] = None):
+        """`before`: a drafter of the text in front of `tokens`, whose places are looked up where its own have no answer (requests behind
+        one prefix share the prefix's)."""
+        self.tokens: List[int] = list(before.tokens) if before is not None else []
         self.seen: Dict[Tuple[int, int], int] = {}       # a pair -> the place behind its latest occurrence but the last
+        self.seen_before = before.seen if before is not None else {}
         self.extend(tokens)
 
     def extend(self, tokens: Sequence[int]) -> None:
@@ -46,7 +49,10 @@ class LookupDrafter:
             self.tokens.append(int(t))
 
     def draft(self, most: int) -> List[int]:
-        at = self.seen.get(tuple(self.tokens[-2:])) if len(self.tokens) >= 2 else None
+        if len(self.tokens) < 2:
+            return []
+        pair = (self.tokens[-2], self.tokens[-1])
+        at = self.seen.get(pair, self.seen_before.get(pair))
         return self.tokens[at: at + most] if at is not None else []
 
 
@@ -123,13 +129,18 @@ class SharedPrefixRunner:
         shared = len(prefix) // PAGE_SIZE
         while shared and shared * PAGE_SIZE == len(prefix) and any(not p for p in prompts):
             shared -= 1
+        if drafter is LookupDrafter:
+            before = LookupDrafter(prefix)
+            begin = lambda prompt: LookupDrafter(prompt, before)      # noqa: E731
+        else:
+            begin = lambda prompt: drafter(prefix + prompt)           # noqa: E731
         slot = self.engine.alloc_slot()
         try:
             self._run_prefix(slot, prefix[: shared * PAGE_SIZE], stats)
             pending = list(range(len(prompts)))
             while pending:
                 pending = self._run_batch(slot, shared, prefix, prompts, pending, outputs, reasons, max_tokens, set(int(t) for t in stop),
-                                          drafts, temperature, seed, batch_size or len(prompts), callback, drafter, stats)
+                                          drafts, temperature, seed, batch_size or len(prompts), callback, begin, stats)
         finally:
             torch.cuda.synchronize(self.device)
             self.engine.free_slot(slot)
@@ -164,7 +175,7 @@ class SharedPrefixRunner:
         for r in chosen:
             own = rest + prompts[r]
             held = min(longest, len(prefix) + len(prompts[r]) + max_tokens - 1 + drafts)
-            live.append(_Request(r, own, shared * PAGE_SIZE, -1, drafter(prefix + prompts[r]), _random(seed, r), held,
+            live.append(_Request(r, own, shared * PAGE_SIZE, -1, drafter(prompts[r]), _random(seed, r), held,
                                  shared))
         mine = [group.pool.take() for _ in range(own_pages)]
         stats.batches += 1

@@ -281,3 +281,31 @@ def test_any_whole_number_is_a_seed(monkeypatch):
     more = dict(drafts=2, temperature=9.0, drafter=drafting(lambda t, n: [3] * n))
     seen = [Host(monkeypatch).generate([4] * 70, [[7], [8]], 20, seed=seed, **more)[0] for seed in (-1, -1, -2, 0, 1, 2 ** 40)]
     assert seen[0] == seen[1] and all(a != b for i, a in enumerate(seen[1:]) for b in seen[2 + i:])
+
+
+def test_the_prefix_is_looked_through_once_for_all_requests(monkeypatch):
+    """Its pairs of tokens lie in one table: a table of each request's own made 256 requests behind 16,384 tokens wait for 1.5 s and took
+    half a gigabyte of the host."""
+    looked_at = []
+    extend = shared_prefix.LookupDrafter.extend
+    monkeypatch.setattr(shared_prefix.LookupDrafter, "extend", lambda self, tokens: (looked_at.append(len(tokens)), extend(self, tokens))[1])
+    prompts = [[7 + i, 8] for i in range(30)]
+    out, _, stats = Host(monkeypatch, pages=200).generate([4] * 1000, prompts, 30)
+    assert out == [continuation(8, 30)] * 30 and stats.accepted > 0
+    assert sum(looked_at) <= 1000 + 30 * (2 + 30)
+
+
+def test_drafts_behind_a_shared_text_are_those_of_the_whole_text():
+    import random
+    rng = random.Random(5)
+    for _ in range(400):
+        text = lambda n: [rng.randrange(4) for _ in range(n)]      # noqa: E731
+        prefix, prompt = text(rng.randrange(30)), text(rng.randrange(6))
+        before = shared_prefix.LookupDrafter(prefix)
+        whole, behind = shared_prefix.LookupDrafter(prefix + prompt), shared_prefix.LookupDrafter(prompt, before)
+        other = shared_prefix.LookupDrafter(text(9), before)       # (another request does not change it)
+        for _ in range(12):
+            assert behind.draft(3) == whole.draft(3)
+            more = text(rng.randrange(1, 4))
+            whole.extend(more), behind.extend(more), other.extend(text(2))
+        assert before.tokens == prefix
