@@ -1,0 +1,411 @@
+// The continuations that a step of beam search goes on with and the ones that end.
+//
+// Beam b of a request has score s_b and logits x_b over the vocabulary; a continuation (b, v) is worth
+//   s_b + x_bv - log sum_u exp x_bu.
+// The K best that are no stop token go on; a stop token among the K best of all ends its beam's text.  A beam's best continuation
+// stays in the beam's row, so that cache rows and states move only where a beam is lost; the others take the rows left, in order.
+//
+// Two launches.  The first reads every logit once, in registers: a thread's own running maximum and sum of exponentials, and the K
+// largest logits of a range of a row, which needs a look at single numbers only where one passes the K-th found so far.  The second,
+// a block a request, joins ranges and beams.  Within a beam the order is that of the logits (equal ones: the lowest token first),
+// which no rounding touches; between beams it is that of the totals, whose sum of exponentials is taken to 64 bits where
+// threads meet: 32 bits would turn two beams round now and then.
+#include <math_constants.h>
+#include <stdio.h>
+
+#include "common.cuh"
+
+namespace {
+
+typedef unsigned long long Key;      // a logit that sorts as a whole number, above the complement of its token: no two are equal; 0: none
+
+constexpr int THREADS = 256;
+constexpr int WARPS = THREADS / 32;
+constexpr int VECTORS = 4;                                // of 16 bytes that a thread has of a piece of a row
+constexpr int PER = 4 * VECTORS;
+constexpr int PIECE = THREADS * PER;
+constexpr int MOST_BEAMS = 32, MOST_STOPS = 32, MOST_RANGES = 32;
+constexpr int FEW = 64;                                   // threads with something new whose numbers are looked at without a bound
+constexpr int ROOM = FEW * PER + MOST_BEAMS;              // (the other way: at most MOST_BEAMS threads' numbers)
+
+__device__ __forceinline__ unsigned sortable(float x) {   // of numbers, -0 taken as 0
+  const unsigned u = __float_as_uint(x + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float number(unsigned u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+__device__ __forceinline__ Key key_of(float x, int token) { return ((Key)sortable(x) << 32) | (unsigned)~token; }
+__device__ __forceinline__ float logit_of(Key k) { return number((unsigned)(k >> 32)); }
+__device__ __forceinline__ int token_of(Key k) { return (int)~(unsigned)k; }
+
+// The keys of a warp, the largest in lane 0.
+__device__ __forceinline__ Key warp_sorted(Key k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) {
+      const Key other = __shfl_xor_sync(0xffffffffu, k, o);
+      const bool wants_more = ((lane & size) == 0) == ((lane & o) == 0);
+      if ((other > k) == wants_more) k = other;
+    }
+  }
+  return k;
+}
+
+struct Stat {
+  double sum;        // of exp(x - most); of entries at +inf, if that is the largest
+  float most;
+  int unused;
+};
+
+struct Args {
+  const float* logits;
+  const float* scores;
+  const int* stops;
+  int* parents;
+  int* tokens;
+  float* next_scores;
+  int* ended_parents;
+  int* ended_tokens;
+  float* ended_scores;
+  Key* keys;          // [rows][ranges][K]
+  Stat* stats;        // [rows][ranges]
+  int R, K, V, S, ranges;
+};
+
+__device__ __forceinline__ bool dead(float score) { return !(score > -CUDART_INF_F); }
+
+// exp(d) for d <= 0; the product with log2(e) in two parts, as its rounding would be the largest error of the sum
+__device__ __forceinline__ float exp_below(float d) {
+  constexpr float L = 1.44269504088896341f, L_LOW = 1.92596299112661746887e-8f, LN2 = 0.693147180559945309f;
+  d = fmaxf(d, -200.0f);             // (also what is not a number, and -inf less -inf)
+  const float hi = d * L;
+  const float lo = fmaf(d, L_LOW, fmaf(d, L, -hi));
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
+  return fmaf(e, lo * LN2, e);
+}
+
+__global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
+  __shared__ Key found[ROOM];          // the best so far, then what a piece adds
+  __shared__ Key heads[WARPS * MOST_BEAMS];
+  __shared__ Key edge;
+  __shared__ int n_found;
+  __shared__ int stops[MOST_STOPS];
+  __shared__ float most_of[WARPS];
+  __shared__ double sum_of[WARPS];
+  jb::pdl_launch_dependents();
+  const int row = blockIdx.x / a.ranges, range = blockIdx.x % a.ranges;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.K;
+  jb::pdl_wait();
+  if (dead(a.scores[row])) return;                        // (the second launch asks for nothing of it)
+  if (tid < a.S) stops[tid] = a.stops[tid];
+  if (tid < K) found[tid] = 0;
+  const float* x_row = a.logits + (size_t)row * a.V;
+  const int lead = (int)(((uintptr_t)x_row >> 2) & 3);    // numbers in front of the row in its first 16 bytes
+  const int pieces = (a.V + lead + PIECE - 1) / PIECE;
+  const int first = (int)((long long)range * pieces / a.ranges), last = (int)((long long)(range + 1) * pieces / a.ranges);
+  float x[PER], next[PER];
+  auto load = [&](float (&to)[PER], int piece) {
+#pragma unroll
+    for (int i = 0; i < VECTORS; ++i) {
+      const int at = piece * PIECE + i * THREADS * 4 + tid * 4 - lead;
+      if (at >= 0 && at + 4 <= a.V) {
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(x_row + at));
+        to[4 * i] = v.x, to[4 * i + 1] = v.y, to[4 * i + 2] = v.z, to[4 * i + 3] = v.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[4 * i + j] = at + j >= 0 && at + j < a.V ? __ldcs(x_row + at + j) : -CUDART_INF_F;
+      }
+    }
+  };
+  float most = -CUDART_INF_F;
+  double sum = 0.0;
+  Key bound = 0;                       // the K-th best so far, 0 while there are fewer
+  if (first < last) load(x, first);
+  __syncthreads();
+  for (int piece = first; piece < last; ++piece) {
+    if (piece + 1 < last) load(next, piece + 1);
+    // ---- maximum and sum of the thread's numbers ----
+    float top = -CUDART_INF_F;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) top = fmaxf(top, x[e]);
+    if (top > most) {
+      if (top == CUDART_INF_F) sum = 0.0;
+      else sum *= exp((double)most - (double)top);          // (0 of nothing: exp(-inf))
+      most = top;
+    }
+    if (most == CUDART_INF_F) {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) sum += x[e] == CUDART_INF_F ? 1.0 : 0.0;
+    } else {
+      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int e = 0; e < PER; ++e) s[e & 3] += exp_below(x[e] - most);
+      sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
+    }
+    // ---- stop tokens are no candidates here ----
+    for (int s = 0; s < a.S; ++s) {
+      const int at = stops[s] + lead - piece * PIECE;
+      if (at >= 0 && at < PIECE && stops[s] >= 0 && stops[s] < a.V && ((at >> 2) & (THREADS - 1)) == tid) {
+        const int mine = (at / (THREADS * 4)) * 4 + (at & 3);
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+          if (e == mine) x[e] = -CUDART_INF_F;
+      }
+    }
+    // ---- the thread's best ----
+    float best = -CUDART_INF_F;
+    int best_at = 0;
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (x[e] > best) best = x[e], best_at = e;
+    const int origin = piece * PIECE + tid * 4 - lead;
+    auto token = [&](int e) { return origin + (e >> 2) * THREADS * 4 + (e & 3); };
+    const Key mine = best > -CUDART_INF_F ? key_of(best, token(best_at)) : 0;
+    const int new_threads = __syncthreads_count(mine > bound);
+    if (new_threads > 0) {
+      Key least = bound;               // what is looked at lies above
+      if (tid == 0) n_found = K, edge = 0;
+      if (new_threads > FEW) {
+        // the K-th largest of the threads' best: no more than K threads have anything at or above it
+        const Key sorted = warp_sorted(mine);
+        if (lane < K) heads[warp * K + lane] = sorted;
+        __syncthreads();
+        if (tid < WARPS * K) {
+          const Key h = heads[tid];
+          int above = 0;
+          for (int i = 0; i < WARPS * K; ++i) above += heads[i] > h;
+          if (above == K - 1 && h > 0) edge = h;
+        }
+        __syncthreads();
+        if (edge > 0 && edge - 1 > least) least = edge - 1;
+      } else {
+        __syncthreads();
+      }
+      if (mine > least) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          if (x[e] > -CUDART_INF_F) {
+            const Key k = key_of(x[e], token(e));
+            if (k > least) found[atomicAdd(&n_found, 1)] = k;
+          }
+        }
+      }
+      __syncthreads();
+      // the K best of what was there and what came, in order: a key's place is the number of larger ones
+      const int n = n_found;
+      Key k[(ROOM + THREADS - 1) / THREADS];
+      int place[(ROOM + THREADS - 1) / THREADS];
+#pragma unroll
+      for (int u = 0; u < (ROOM + THREADS - 1) / THREADS; ++u) {
+        const int i = tid + u * THREADS;
+        place[u] = K;
+        if (i < n) {
+          k[u] = found[i];
+          int above = 0;
+          for (int j = 0; j < n; ++j) above += found[j] > k[u];
+          if (k[u] > 0) place[u] = above;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < (ROOM + THREADS - 1) / THREADS; ++u)
+        if (place[u] < K) found[place[u]] = k[u];
+      __syncthreads();
+      bound = found[K - 1];
+    }
+#pragma unroll
+    for (int e = 0; e < PER; ++e) x[e] = next[e];
+  }
+  // ---- the range's maximum and sum ----
+  const float warp_most = jb::warp_max(most);
+  if (lane == 0) most_of[warp] = warp_most;
+  __syncthreads();
+  float all = most_of[0];
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) all = fmaxf(all, most_of[w]);
+  if (all == CUDART_INF_F) sum = most == all ? sum : 0.0;
+  else if (most < all) sum *= exp((double)most - (double)all);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sum_of[warp] = sum;
+  __syncthreads();
+  const size_t list = (size_t)row * a.ranges + range;
+  if (tid == 0) {
+    double s = 0.0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) s += sum_of[w];
+    a.stats[list] = Stat{s, all, 0};
+  }
+  if (tid < K) a.keys[list * K + tid] = found[tid];
+}
+
+// Whether continuation (x, i) comes in front of (y, j): by total, then by beam and token.
+__device__ __forceinline__ bool in_front(double x, long long i, double y, long long j) { return x > y || (x == y && i < j); }
+
+// One block a request.  Dynamic memory: WARPS * K * K keys, then for K * K continuations (total, place), their shortened list, and
+// for K * S stop tokens the same.
+__global__ void __launch_bounds__(THREADS) beam_join_kernel(const Args a) {
+  extern __shared__ __align__(16) uint8_t memory[];
+  __shared__ double base[MOST_BEAMS];      // score - log sum exp, of a live beam
+  __shared__ float most_of[MOST_BEAMS];
+  __shared__ double kth[MOST_BEAMS], head[MOST_BEAMS];
+  __shared__ double on[MOST_BEAMS];
+  __shared__ long long on_at[MOST_BEAMS];
+  __shared__ int n_list, n_stop;
+  const int r = blockIdx.x, K = a.K, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, KK = K * K;
+  Key* lists = reinterpret_cast<Key*>(memory);                           // [WARPS][K * K]
+  double* totals = reinterpret_cast<double*>(lists + WARPS * KK);        // [K][K]
+  double* short_total = totals + KK;
+  double* stop_total = short_total + KK;                                 // [K * S]
+  int* token = reinterpret_cast<int*>(stop_total + K * a.S);             // [K][K]
+  int* short_at = token + KK;                                            // beam * K + place
+  int* stop_at = short_at + KK;                                          // beam * S + stop
+  jb::pdl_launch_dependents();
+  jb::pdl_wait();
+  if (tid == 0) n_list = n_stop = 0;
+  if (tid < K) {
+    a.ended_parents[r * K + tid] = a.ended_tokens[r * K + tid] = -1;
+    a.ended_scores[r * K + tid] = -CUDART_INF_F;
+    on[tid] = -CUDART_INF;
+    on_at[tid] = 0;
+  }
+  // ---- every beam's K best, a warp a beam ----
+  Key* mine = lists + warp * KK;
+  for (int b = warp; b < K; b += WARPS) {
+    const int row = r * K + b;
+    const float score = a.scores[row];
+    for (int j = lane; j < K; j += 32) totals[b * K + j] = -CUDART_INF, token[b * K + j] = 0;
+    if (lane == 0) base[b] = -CUDART_INF, most_of[b] = -CUDART_INF_F;
+    if (!dead(score)) {
+      const Key* keys = a.keys + (size_t)row * a.ranges * K;
+      Key edge = lane < a.ranges ? keys[lane * K] : 0;
+      Stat s{0.0, -CUDART_INF_F, 0};
+      if (lane < a.ranges) s = a.stats[(size_t)row * a.ranges + lane];
+      const float most = jb::warp_max(s.most);
+      double sum = most == CUDART_INF_F ? (s.most == most ? s.sum : 0.0) : s.most > -CUDART_INF_F ? s.sum * exp((double)s.most - (double)most) : 0.0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const double less = log(sum);                       // (a number wherever the row has one above -inf)
+      if (lane == 0) base[b] = (double)score - less, most_of[b] = most;
+      edge = __shfl_sync(0xffffffffu, warp_sorted(edge), K - 1);          // no more than K ranges have anything at or above it
+      int n = 0;
+      for (int i0 = 0; i0 < a.ranges * K; i0 += 32) {
+        const Key k = i0 + lane < a.ranges * K ? keys[i0 + lane] : 0;
+        const bool takes = k > 0 && k >= edge;
+        const unsigned who = __ballot_sync(0xffffffffu, takes);
+        if (takes) mine[n + __popc(who & ((1u << lane) - 1u))] = k;
+        n += __popc(who);
+      }
+      __syncwarp();
+      for (int i = lane; i < n; i += 32) {
+        const Key k = mine[i];
+        int above = 0;
+        for (int j = 0; j < n; ++j) above += mine[j] > k;
+        if (above < K) {
+          const float x = logit_of(k);
+          const double z = most == CUDART_INF_F ? (x == most ? 0.0 : -CUDART_INF) : (double)x - (double)most;
+          totals[b * K + above] = (double)score - less + z;
+          token[b * K + above] = token_of(k);
+        }
+      }
+      __syncwarp();
+    }
+    if (lane == 0) head[b] = totals[b * K], kth[b] = totals[b * K + K - 1];
+  }
+  __syncthreads();
+  // ---- the K best of all beams: at least K lie at or above the largest K-th of a beam, and above the least of the beams' best ----
+  double edge = -CUDART_INF, least = CUDART_INF;
+  for (int b = 0; b < K; ++b) edge = fmax(edge, kth[b]), least = fmin(least, head[b]);
+  edge = fmax(edge, least);
+  for (int i = tid; i < KK; i += THREADS) {
+    if (totals[i] > -CUDART_INF && totals[i] >= edge) {
+      const int at = atomicAdd(&n_list, 1);
+      short_total[at] = totals[i];
+      short_at[at] = i;
+    }
+  }
+  __syncthreads();
+  const long long V = a.V;
+  for (int i = tid; i < n_list; i += THREADS) {
+    const double t = short_total[i];
+    const long long at = short_at[i] / K * V + token[short_at[i]];
+    int before = 0;
+    for (int j = 0; j < n_list; ++j) before += in_front(short_total[j], short_at[j] / K * V + token[short_at[j]], t, at);
+    if (before < K) on[before] = t, on_at[before] = at;
+  }
+  __syncthreads();
+  // ---- stop tokens that stand among the K best ----
+  for (int i = tid; i < K * a.S; i += THREADS) {
+    const int b = i / a.S, stop = a.stops[i % a.S];
+    bool again = false;
+    for (int s = 0; s < i % a.S; ++s) again |= a.stops[s] == stop;
+    if (stop < 0 || stop >= a.V || again || !(base[b] > -CUDART_INF)) continue;
+    const float x = a.logits[((size_t)r * K + b) * a.V + stop], most = most_of[b];
+    if (!(x > -CUDART_INF_F)) continue;
+    const double t = base[b] + (most == CUDART_INF_F ? (x == most ? 0.0 : -CUDART_INF) : (double)x - (double)most);
+    if (!(t > -CUDART_INF) || !in_front(t, b * V + stop, on[K - 1], on[K - 1] > -CUDART_INF ? on_at[K - 1] : K * V)) continue;
+    const int at = atomicAdd(&n_stop, 1);
+    stop_total[at] = t;
+    stop_at[at] = i;
+  }
+  __syncthreads();
+  for (int i = tid; i < n_stop; i += THREADS) {
+    const double t = stop_total[i];
+    const int b = stop_at[i] / a.S, stop = a.stops[stop_at[i] % a.S];
+    int place = 0, before = 0;
+    for (int j = 0; j < n_stop; ++j) place += in_front(stop_total[j], stop_at[j] / a.S * V + a.stops[stop_at[j] % a.S], t, b * V + stop);
+    for (int j = 0; j < K; ++j) before += on[j] > -CUDART_INF && in_front(on[j], on_at[j], t, b * V + stop);
+    if (place + before < K) {
+      a.ended_parents[r * K + place] = b;
+      a.ended_tokens[r * K + place] = stop;
+      a.ended_scores[r * K + place] = (float)t;
+    }
+  }
+  // ---- rows: a beam's best continuation stays in the beam's row ----
+  if (warp == 0) {
+    const bool live = lane < K && on[lane] > -CUDART_INF;
+    const int parent = live ? (int)(on_at[lane] / V) : -1 - lane;
+    const unsigned same = __match_any_sync(0xffffffffu, parent);
+    const bool stays = live && (same & ((1u << lane) - 1u)) == 0;
+    const unsigned kept = __reduce_or_sync(0xffffffffu, stays ? 1u << parent : 0u);
+    const unsigned moves = __ballot_sync(0xffffffffu, lane < K && !stays);
+    if (lane < K) {
+      int row = parent;
+      if (!stays) {
+        unsigned left = ~kept;
+        for (int n = __popc(moves & ((1u << lane) - 1u)); n > 0; --n) left &= left - 1;
+        row = __ffs(left) - 1;
+      }
+      a.parents[r * K + row] = live ? parent : -1;
+      a.tokens[r * K + row] = live ? (int)(on_at[lane] % V) : 0;
+      a.next_scores[r * K + row] = (float)on[lane];
+    }
+  }
+}
+
+size_t join_memory(int K, int S) { return (size_t)WARPS * K * K * 8 + (size_t)K * K * (8 + 8 + 4 + 4) + (size_t)K * S * (8 + 4); }
+
+}  // namespace
+
+// Scratch: keys R * K * ranges * K of 8 bytes, stats R * K * ranges of 16.
+JB_EXPORT int jb_beam_select(const float* logits, const float* scores, const int* stops, int* parents, int* tokens, float* next_scores,
+                             int* ended_parents, int* ended_tokens, float* ended_scores, void* keys, void* stats, int R, int K, int V,
+                             int S, int ranges, cudaStream_t stream) {
+  JB_REFUSE(R < 1 || K < 1 || K > MOST_BEAMS || V < 1 || S < 0 || S > MOST_STOPS || ranges < 1 || ranges > MOST_RANGES ||
+                (long long)R * K * ranges > 0x7fffffffLL || V > 0x7fffffff - PIECE,
+            "beam_select: %d requests of %d beams, vocabulary %d, %d stop tokens, %d ranges", R, K, V, S, ranges);
+  const Args a{logits, scores, stops, parents, tokens, next_scores, ended_parents, ended_tokens, ended_scores, (Key*)keys, (Stat*)stats,
+               R, K, V, S, ranges};
+  jb::Launch rows(dim3(R * K * ranges), dim3(THREADS), 0, stream);
+  cudaError_t e = cudaLaunchKernelEx(&rows.c, beam_rows_kernel, a);
+  if (e != cudaSuccess) return (int)e;
+  const size_t memory = join_memory(K, S);
+  if (memory > 48 * 1024) {
+    e = cudaFuncSetAttribute(beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)join_memory(MOST_BEAMS, MOST_STOPS));
+    if (e != cudaSuccess) return (int)e;
+  }
+  jb::Launch join(dim3(R), dim3(THREADS), memory, stream);
+  return (int)cudaLaunchKernelEx(&join.c, beam_join_kernel, a);
+}

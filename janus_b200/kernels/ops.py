@@ -102,6 +102,8 @@ _SIGNATURES = {
     "jb_latent_down": "piipfpiippiiippppplip",
     "jb_step_tables": "pp", "jb_attention_prefix_f32": "ppp", "jb_attention_prefix_bf16": "pppp",
     "jb_verify_drafts": "pp",
+    "jb_beam_select": "pppppppppppiiiiip", "jb_fork_pages": "pp", "jb_copy_pages": "pppipppiiip", "jb_reorder_rows": "ppippiiip",
+    "jb_attention_beams": "ppppppppiiiiiiifp",
     "jb_gather_rows": "ppiipppiiip", "jb_latent_attention": "ppppppppiiiiiiifiipp", "jb_attention_tc_matrix": "ppppppiiiiiiiifpipp",
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "u": ctypes.c_ulonglong,
@@ -2662,3 +2664,194 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, q_start: torch.Ten
 
 
 _VERIFY = struct.Struct("12P4if").pack     # `Verify` of csrc/verify.cu
+
+
+# -- beam search over a paged cache ------------------------------------------------------------------------------------
+MOST_BEAMS = 32          # beams of a request
+MOST_BEAM_STOPS = 32     # stop tokens
+
+
+def _on_current_device(what: str, tensors) -> None:
+    """All tensors on one CUDA device, the current one, whose stream the launch goes to."""
+    if not _checks[0]:
+        return
+    device = tensors[0].get_device()
+    if device < 0 or any(t.get_device() != device for t in tensors) or device != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensors must be on the current CUDA device (there is no CPU path)")
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, stop_tokens: torch.Tensor, *, parents: torch.Tensor, tokens: torch.Tensor,
+                next_scores: torch.Tensor, ended_parents: torch.Tensor, ended_tokens: torch.Tensor, ended_scores: torch.Tensor,
+                workspace) -> None:
+    """The continuations a step of beam search goes on with.  R requests have K beams each (up to MOST_BEAMS); beam b of request r has the
+    score scores[r, b] (float32; -inf, or not a number: no beam) and the logits of row r K + b (float32 [R K, V]).  A continuation by
+    token v is worth the score plus the log-probability log softmax(logits)[v]; continuations are ordered by that, taken to 64 bits, equal ones by
+    beam and token (within a beam by logit and token).  Logits that are -inf or not numbers have no weight and are never chosen.
+
+    Out, [R, K]: the K best continuations whose token is none of `stop_tokens` (int32, up to MOST_BEAM_STOPS; ids outside the vocabulary
+    mean nothing) as parents (the beam that is continued), tokens and next_scores.  A beam's best continuation stands in the beam's own place, the
+    others in the places left, in order; where there are fewer than K, the places left have parent -1, token 0 and score -inf.
+    The continuations by stop tokens that are among the K best of all, in order, as ended_parents, ended_tokens and ended_scores; -1,
+    -1 and -inf behind them.  next_scores may be `scores` itself."""
+    R, K = scores.shape
+    rows, V = logits.shape
+    if not 1 <= K <= MOST_BEAMS or R < 1 or V < 1 or stop_tokens.shape[0] > MOST_BEAM_STOPS:
+        raise KernelError(f"beam_select: {R} requests of {K} beams over {V} tokens with {stop_tokens.shape[0]} stop tokens (1 to {MOST_BEAMS} "
+                          f"beams, up to {MOST_BEAM_STOPS} stop tokens)")
+    if _checks[0]:
+        b = (R, K)
+        _need_all("beam_select", torch.float32, (logits, scores, next_scores, ended_scores), ((R * K, V), b, b, b),
+                  ("logits", "scores", "next scores", "scores of ended texts"))
+        _need_all("beam_select", torch.int32, (stop_tokens, parents, tokens, ended_parents, ended_tokens), (stop_tokens.shape[:1], b, b, b, b),
+                  ("stop tokens", "parents", "tokens", "parents of ended texts", "tokens of ended texts"))
+        _on_current_device("beam_select", (logits, scores, stop_tokens, parents, tokens, next_scores, ended_parents, ended_tokens, ended_scores))
+    ranges = beam_ranges(rows, V)
+    keys = workspace.get("beam_keys", (rows * ranges * K,), torch.int64)
+    stats = workspace.get("beam_stats", (rows * ranges * 2,), torch.float64)
+    _check(_lib("beam_select").jb_beam_select(
+        logits.data_ptr(), scores.data_ptr(), stop_tokens.data_ptr(), parents.data_ptr(), tokens.data_ptr(), next_scores.data_ptr(),
+        ended_parents.data_ptr(), ended_tokens.data_ptr(), ended_scores.data_ptr(), keys.data_ptr(), stats.data_ptr(), R, K, V,
+        stop_tokens.shape[0], ranges, _stream()), "beam_select", kernels=2)
+
+
+def beam_ranges(rows: int, vocab: int) -> int:
+    """Ranges that a row of logits is cut into: enough blocks for six a multiprocessor, none with less than a piece of 4,096 logits."""
+    return max(1, min(32, -(-vocab // 4096), -(-6 * SM_COUNT_TARGET // 2 // rows)))
+
+
+def fork_pages(parents: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, free_pages: torch.Tensor,
+               n_free: torch.Tensor, *, kv_len: torch.Tensor, positions: torch.Tensor, dest_rows: torch.Tensor, new_table: torch.Tensor,
+               new_refs: torch.Tensor, new_free: torch.Tensor, new_n_free: torch.Tensor, copy_src: torch.Tensor, copy_dst: torch.Tensor,
+               copy_rows: torch.Tensor, shared: torch.Tensor, missing: torch.Tensor, spare: int, page_size: int) -> None:
+    """The block tables of the next step's rows, which go on with rows of this one; all int32, in one launch.
+
+    Rows come in R groups of K (up to MOST_BEAMS).  Row r K + k goes on with what row r K + parents[r, k] holds: lengths[r, parents[r, k]]
+    tokens in the pages that `table` [R K, W] lists for it; a parent outside 0 .. K - 1 means that the row does not go on.  refs [P] counts who
+    holds a page: rows of the table, and anybody else (a page that is to stay has a holder outside).  free_pages[:n_free] are pages
+    that nobody holds.  Each row that goes on is made ready for one more token.  Whole pages are held by all rows that go on with
+    them.  The page that the token goes to stays with the lowest row of the group that holds it, if nobody else does; any other row
+    takes a page of its own from the back of the free list, with a copy to be made where the page is partly filled (a partly filled page is
+    held by the rows of one group only, or by holders outside).  Pages that nobody holds any longer come back first, behind the free
+    ones, in order of number.
+
+    Made: new_table, new_refs, new_free (-1 behind new_n_free); kv_len, positions and dest_rows [R, K], the length with the token, its
+    position and its cache row; copy_src, copy_dst and copy_rows [R, K], what `copy_pages` has to copy (-1, -1, 0: nothing);
+    shared [R], the leading whole pages that all rows of a group that go on have in common; missing [1], rows
+    without a page because list or table had no place, and pages that the new list has no place for: where it is not zero the step must not run.  Rows that do not
+    go on get a table row of page `spare`, which is counted for nobody, kv_len 1 and position 0, so that a step may run them for nothing; rows
+    without a page get its first cache row too.
+
+    kv_len, new_table, new_refs, new_free and new_n_free may be lengths, table, refs, free_pages and n_free themselves, which are
+    then changed in place; other outputs are tensors of their own."""
+    (R, K), (N, W), P, F = parents.shape, table.shape, refs.shape[0], free_pages.shape[0]
+    if not 1 <= K <= MOST_BEAMS or R < 1 or W < 1 or not 0 <= spare < P or page_size < 1:
+        raise KernelError(f"fork_pages: {R} groups of {K} rows (1 to {MOST_BEAMS}) of {W} pages, spare page {spare} of {P}, pages of {page_size}")
+    tensors = (parents, lengths, table, refs, free_pages, n_free, kv_len, positions, dest_rows, new_table, new_refs, new_free, new_n_free,
+               copy_src, copy_dst, copy_rows, shared, missing)
+    if _checks[0]:
+        b, one = (R, K), (1,)
+        _need_all("fork_pages", torch.int32, tensors,
+                  (b, b, (R * K, W), (P,), (F,), one, b, b, b, (R * K, W), (P,), (F,), one, b, b, b, (R,), one), _FORK_PAGES_NAMES)
+        _on_current_device("fork_pages", tensors)
+    _check(_lib("beam_cache").jb_fork_pages(_FORK_PAGES(*(t.data_ptr() for t in tensors), R, K, W, P, F, int(spare), int(page_size)), _stream()),
+           "fork_pages")
+
+
+_FORK_PAGES = struct.Struct("18P7i4x").pack     # `Fork` of csrc/beam_cache.cu
+_FORK_PAGES_NAMES = ("parents", "lengths", "table", "page counts", "free pages", "number of free pages", "kv_len", "positions", "cache rows",
+                     "new table", "new page counts", "new free pages", "new number of free pages", "pages to copy from", "pages to copy to",
+                     "tokens to copy", "shared pages", "missing pages")
+
+
+COPY_PAGES = 128        # tensors that one launch of `copy_pages` takes
+
+
+def copy_pages(tensors: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor, rows: torch.Tensor) -> None:
+    """For every i with src[i] and dst[i] among the pages: the first rows[i] tokens of each head of page src[i] are copied to page dst[i], in
+    every tensor ([pages, heads, page size, numbers], 2 or 4 bytes a number; heads and numbers may differ).  src, dst, rows: int32
+    [n].  Pages that are copied to differ from one another and from those that are copied from.  Up to COPY_PAGES tensors go in
+    one launch."""
+    n = src.shape[0]
+    if not tensors or n == 0:
+        return
+    pages, size = tensors[0].shape[0], tensors[0].shape[2] if tensors[0].dim() == 4 else 0
+    if _checks[0]:
+        _need_all("copy_pages", torch.int32, (src, dst, rows), ((n,), (n,), (n,)), ("pages to copy from", "pages to copy to", "tokens to copy"))
+        for t in tensors:
+            _need(t, "copy_pages tensor")
+            if t.dim() != 4 or t.shape[0] != pages or t.shape[2] != size or t.numel() == 0 or t.element_size() not in (2, 4):
+                raise KernelError(f"copy_pages: tensors are [{pages}, heads, {size}, numbers] of 2 or 4 bytes, got {t.dtype} {tuple(t.shape)}")
+        _on_current_device("copy_pages", (src, dst, rows, *tensors))
+    lib = _lib("beam_cache")
+    for first in range(0, len(tensors), COPY_PAGES):
+        some = tensors[first: first + COPY_PAGES]
+        m = len(some)
+        _check(lib.jb_copy_pages(struct.pack(f"{m}P", *(t.data_ptr() for t in some)), struct.pack(f"{m}i", *(t.shape[1] for t in some)),
+                                 struct.pack(f"{m}i", *(t.shape[3] * t.element_size() for t in some)), m, src.data_ptr(), dst.data_ptr(),
+                                 rows.data_ptr(), n, pages, size, _stream()), "copy_pages")
+
+
+REORDER_ROWS = 64       # matrices that one launch of `reorder_rows` takes
+
+
+def reorder_rows(matrices: Sequence[torch.Tensor], slots: torch.Tensor, parents: torch.Tensor) -> None:
+    """In every float32 tensor (its first axis: slots), in place: row slots[r K + k] becomes what row slots[r K + parents[r, k]] was.
+    parents [R, K] (up to MOST_BEAMS), slots [R K], int32, no slot twice; a parent outside 0 .. K - 1, or a slot outside the tensor, leaves
+    the row as it was.  Up to REORDER_ROWS tensors go in one launch."""
+    R, K = parents.shape
+    if not 1 <= K <= MOST_BEAMS:
+        raise KernelError(f"reorder_rows: groups of {K} rows (1 to {MOST_BEAMS})")
+    if not matrices or R == 0:
+        return
+    n = matrices[0].shape[0]
+    if _checks[0]:
+        _need_all("reorder_rows", torch.int32, (slots, parents), ((R * K,), (R, K)), ("slots", "parents"))
+        for m in matrices:
+            _need(m, "reorder_rows matrix", torch.float32)
+            if m.shape[0] != n or m.numel() == 0:
+                raise KernelError(f"reorder_rows: matrices have {n} slots, got {tuple(m.shape)}")
+        _on_current_device("reorder_rows", (slots, parents, *matrices))
+    lib = _lib("beam_cache")
+    for first in range(0, len(matrices), REORDER_ROWS):
+        some = matrices[first: first + REORDER_ROWS]
+        m = len(some)
+        _check(lib.jb_reorder_rows(struct.pack(f"{m}P", *(t.data_ptr() for t in some)), struct.pack(f"{m}q", *(t.numel() // n for t in some)), m,
+                                   slots.data_ptr(), parents.data_ptr(), R, K, n, _stream()), "reorder_rows")
+
+
+def attention_beams(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
+                    kv_len: torch.Tensor, shared: torch.Tensor, beams: int, nh: int, nkv: int, hd: int, page_size: int, scale: float,
+                    workspace, max_kv_len: int) -> None:
+    """Attention of one query token a row over the row's first kv_len[row] keys.  Rows come in groups of `beams` (up to MOST_BEAMS); the
+    first shared[r] pages of the rows of group r are the same and are read once for all of them (a row of fewer tokens reads its
+    own).  bfloat16: q and out [rows, nh hd], caches [pages, nkv, page_size, hd]; int32: block_table [rows, W], kv_len [rows] (up to W
+    pages), shared [rows / beams].  Heads of up to 256 numbers, multiples of 8; pages of 64 tokens.  A row without keys is 0.  max_kv_len: at least the
+    longest row's keys."""
+    N, W = block_table.shape
+    if not 1 <= beams <= MOST_BEAMS or N < 1 or N % beams or page_size != 64 or W < 1:
+        raise KernelError(f"attention_beams: {N} rows of {W} pages in groups of {beams} (1 to {MOST_BEAMS}), pages of {page_size} (64)")
+    if nkv < 1 or nh < nkv or nh % nkv or not 8 <= hd <= ATTENTION_MAX_HEAD_DIM or hd % 8:
+        raise KernelError(f"attention_beams: {nh} heads over {nkv} of {hd} numbers (multiples of 8 up to {ATTENTION_MAX_HEAD_DIM})")
+    if _checks[0]:
+        width, cache = (N, nh * hd), (k_cache.shape[0], nkv, page_size, hd)
+        _need_all("attention_beams", torch.bfloat16, (q, out, k_cache, v_cache), (width, width, cache, cache), ("q", "out", "k cache", "v cache"))
+        _need_all("attention_beams", torch.int32, (block_table, kv_len, shared), ((N, W), (N,), (N // beams,)),
+                  ("block table", "kv_len", "shared pages"))
+        _on_current_device("attention_beams", (q, k_cache, v_cache, out, block_table, kv_len, shared))
+    splits = beam_splits(N // beams, beams, nh, nkv, hd, min(int(max_kv_len), W * page_size))
+    part = workspace.get("beam_parts", (N * nh * splits * (hd + 2) if splits > 1 else 1,), torch.float32)
+    _check(_lib("beam_attention", hd, _head_dim_defines).jb_attention_beams(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), part.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(),
+        shared.data_ptr(), N // beams, beams, nh, nkv, W, k_cache.shape[0], splits, float(scale), _stream()), "attention_beams",
+        kernels=2 if splits > 1 else 1)
+
+
+def _head_dim_defines(hd: int) -> dict:
+    return {"JB_HEAD_DIM": hd}
+
+
+def beam_splits(groups: int, beams: int, nh: int, nkv: int, hd: int, max_kv_len: int) -> int:
+    """Ranges that a group's pages are cut into."""
+    rows = 16 if hd > 128 else 32
+    blocks = groups * nkv * -(-beams * (nh // nkv) // rows)
+    return max(1, min(-(-max_kv_len // 64), -(-4 * SM_COUNT_TARGET // blocks)))
