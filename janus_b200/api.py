@@ -15,6 +15,7 @@ import torch
 from . import log
 from .cache import PAGE_SIZE
 from .config import read_config_json, resolve_architecture
+from .engine.beams import BeamRunner
 from .engine.generate import plan_prompt_steps, run_generation
 from .engine.shared_prefix import LookupDrafter, SharedPrefixRunner
 from .engine.step import Engine, EngineOptions, StepEntry
@@ -99,6 +100,7 @@ class Model:
         self.device = engine.device
         self.dtype = engine.dtype
         self._samplers = {}
+        self._beams: Optional[BeamRunner] = None
 
     # -- the step function, for callers that schedule themselves ---------------
     def alloc_slot(self) -> int:
@@ -205,6 +207,23 @@ class Model:
         if return_reasons:
             return outputs, reasons, stats
         return outputs, stats
+
+    def generate_beams(self, prompts: Sequence[Sequence[int]], beams: int = 4, max_tokens: int = 128, length_penalty: float = 1.0,
+                       early_stopping: bool = False, stop_token_ids: Optional[Sequence[int]] = None, ignore_eos: bool = False,
+                       batch_size: Optional[int] = None, return_all: bool = False):
+        """Beam search: the texts of up to `max_tokens` new tokens that `beams` continuations kept at a time find most probable.  A text's
+        score is the sum of its tokens' log-probabilities; texts are compared by score / length ** length_penalty (a stop token
+        counts to both and is not part of the text).  A request ends when it has as many ended texts as beams and none that is
+        still open can become better, or, with `early_stopping`, as soon as it has that many.  Returns (tokens of each request's best
+        text, stats); with `return_all` (up to `beams` texts a request with tokens, score, value and reason, the best first;
+        stats).  A beam takes a slot of the cache, and pages of its own behind the whole pages of its prompt."""
+        if self._beams is None:
+            self._beams = BeamRunner(self.engine)
+        texts, stats = self._beams.generate(prompts, beams, max_tokens, self._stop_tokens(ignore_eos, stop_token_ids), length_penalty,
+                                            early_stopping, batch_size)
+        log.log("info", f"generate_beams: {stats.requests} requests of {beams} beams in {stats.batches} batches; {stats.decode_steps} steps, "
+                        f"{stats.graph_captures} graphs recorded")
+        return (texts if return_all else [t[0].tokens if t else [] for t in texts]), stats
 
 
 _WHOLE = object()        # max_step_tokens left at the engine's default

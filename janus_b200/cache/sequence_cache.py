@@ -85,6 +85,7 @@ class GroupStepView:
     dest_rows: torch.Tensor        # int32 [T]
     block_table: torch.Tensor      # int32 [n_seqs, max_pages]
     page_size: int
+    shared: Optional[torch.Tensor] = None   # beam search: int32, leading pages that all beams of a request have in common
 
 
 @dataclass

@@ -65,6 +65,10 @@ def main(argv=None) -> int:
                     help="token ids that stand in front of every prompt: computed and cached once for all of them")
     ap.add_argument("--drafts", type=int, default=4,
                     help="with --shared-prefix: tokens drafted from a request's own text and verified per step (default: 4)")
+    ap.add_argument("--beams", type=int, default=0,
+                    help="beam search with this many beams a prompt (default: 0, sampling)")
+    ap.add_argument("--length-penalty", type=float, default=1.0,
+                    help="with --beams: texts are compared by score / length ** this (default: 1)")
     ap.add_argument("--json", action="store_true", help="print one JSON object instead of text")
     ap.add_argument("--profile", metavar="FILE", default=None,
                     help="after generating, time the kernels of the first batch's prompt step and of one decode "
@@ -81,13 +85,19 @@ def main(argv=None) -> int:
     if prefix and (args.top_k or args.top_p < 1.0 or args.repetition_penalty != 1.0 or args.profile):
         ap.error("--shared-prefix goes with --temperature only, not with --top-k, --top-p, --repetition-penalty or --profile")
 
+    if args.beams and (prefix or args.temperature > 0 or args.top_k or args.top_p < 1.0 or args.repetition_penalty != 1.0 or args.profile):
+        ap.error("--beams goes without --shared-prefix, --temperature, --top-k, --top-p, --repetition-penalty and --profile")
+
     import janus_b200
+    from janus_b200.engine.beams import room_for_beams
     from janus_b200.engine.generate import tokens_held
     from janus_b200.engine.shared_prefix import room_for_batch
 
     batch = max(1, min(args.batch_size, len(prompts)))
     if prefix:                       # the prefix lies in the cache once, in a slot of its own; its requests take none
         room, slots = room_for_batch(len(prefix), [len(p) for p in prompts], args.max_tokens, max(0, args.drafts), batch), 1
+    elif args.beams:                 # a beam takes a slot, and pages of its own behind its prompt's
+        room, slots = room_for_beams([len(p) for p in prompts], args.max_tokens, max(1, args.beams), batch), batch * max(1, args.beams)
     else:
         room, slots = sum(sorted((tokens_held(len(p), args.max_tokens, 64) for p in prompts), reverse=True)[:batch]), batch
     dtype = {"bf16": "bfloat16", "fp32": "float32"}.get(args.dtype, args.dtype)
@@ -105,6 +115,10 @@ def main(argv=None) -> int:
         out, reasons, stats = model.generate_shared(
             prefix, prompts, max_tokens=args.max_tokens, drafts=args.drafts, temperature=args.temperature, seed=args.seed,
             stop_token_ids=args.stop_id, ignore_eos=args.ignore_eos, batch_size=batch, return_reasons=True)
+    elif args.beams:
+        texts, stats = model.generate_beams(prompts, beams=args.beams, max_tokens=args.max_tokens, length_penalty=args.length_penalty,
+                                            stop_token_ids=args.stop_id, ignore_eos=args.ignore_eos, batch_size=batch, return_all=True)
+        out, reasons = [t[0].tokens if t else [] for t in texts], [t[0].reason if t else "stop" for t in texts]
     else:
         out, reasons, stats = model.generate(
             prompts, max_tokens=args.max_tokens, temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,

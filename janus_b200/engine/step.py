@@ -76,6 +76,8 @@ class StepContext:
         # sequences that begin with the same tokens: the pages (int32, on the device) that stand in front of every row of the
         # block table and are read once for all of them; None: nothing is shared
         self.prefix_pages: Optional[torch.Tensor] = None
+        # beam search: rows of a decode step that follow one another as the beams of a request; 0: none do
+        self.beams = 0
         self.workspace: Workspace = None
         self.cache: SequenceCache = None
         self.dtype: torch.dtype = None

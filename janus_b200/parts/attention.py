@@ -147,7 +147,8 @@ class GQAttention(Mixer):
                 self.position.apply(qkv[:, self.q_width: self.q_width + self.kv_width], self.nkv, self.hd,
                                     ctx.positions)
         attn = ws.get("attn_out", (T, self.q_width), self.dtype)
-        if ctx.is_decode and self.dtype == torch.bfloat16 and _FUSED_DECODE and not custom_positions:
+        beams = self._beams_share_pages(ctx, group)
+        if ctx.is_decode and self.dtype == torch.bfloat16 and _FUSED_DECODE and not custom_positions and not beams:
             # one token per sequence: rotation and cache append happen inside the attention kernel
             # (one launch and one round trip of q less)
             ops.attention_bf16_decode(None, cache_view.k, cache_view.v, attn, group.block_table, ctx.kv_len,
@@ -163,6 +164,11 @@ class GQAttention(Mixer):
         if getattr(ctx, "prefix_pages", None) is not None:
             self._attend_prompt(q, residual, ctx, cache_view)
             return
+        if beams:
+            ops.attention_beams(q, cache_view.k, cache_view.v, attn, group.block_table, ctx.kv_len, group.shared, ctx.beams, self.nh, self.nkv,
+                                self.hd, group.page_size, self.scale, ws, ctx.max_kv_len_bound)
+            self.o.forward_add(attn, residual)
+            return
         if self.dtype == torch.float32:
             ops.attention_f32(q, cache_view.k, cache_view.v, attn, group.block_table, ctx.token_seq,
                               ctx.positions, self.nh, self.nkv, self.hd, group.page_size, self.window,
@@ -175,6 +181,11 @@ class GQAttention(Mixer):
             self._attend_prompt(q, residual, ctx, cache_view)
             return
         self.o.forward_add(attn, residual)
+
+    def _beams_share_pages(self, ctx, group) -> bool:
+        """Whether a step of beam search reads pages that beams share once for all of them."""
+        return (getattr(ctx, "beams", 0) > 1 and getattr(group, "shared", None) is not None and self.dtype == torch.bfloat16
+                and self.window == 0 and self.hd % 8 == 0)
 
     def _attend_prompt(self, q: torch.Tensor, residual: torch.Tensor, ctx, cache_view) -> None:
         """bfloat16 attention of several new tokens per sequence over the cache (either dtype, where the sequences share a prefix),

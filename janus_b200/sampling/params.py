@@ -15,7 +15,7 @@ class SamplerConfig:
     top_k: int = 0                    # 0 = off; applied to the logits before the temperature (sampler.rs:623-626)
     top_p: float = 1.0                # 1 = off; nucleus over the probabilities (sampler.rs:637-642)
     repetition_penalty: float = 1.0   # over the tokens generated so far (sampler.rs:599-613)
-    beam_width: int = 1               # the reference has no beam loop either (sampler.rs:804-847); only 1 is taken
+    beam_width: int = 1               # sampling has one beam (the reference has no beam loop, sampler.rs:804-847); see Model.generate_beams
     max_tokens: int = 128             # new tokens per sequence at most (sampler.rs:31-38)
 
     def validate(self) -> None:
@@ -28,6 +28,6 @@ class SamplerConfig:
         if not self.repetition_penalty > 0.0:
             raise ValueError(f"repetition_penalty must be positive, got {self.repetition_penalty}")
         if self.beam_width != 1:
-            raise ValueError("beam search is not built (beam_width must be 1)")
+            raise ValueError("sampling keeps one text at a time (beam_width must be 1); beam search is Model.generate_beams")
         if self.max_tokens < 0:
             raise ValueError(f"max_tokens must not be negative, got {self.max_tokens}")
