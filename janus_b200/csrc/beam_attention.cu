@@ -1,5 +1,4 @@
-// Attention of beams over a paged cache, one query token a beam, compiled for one head size (-DJB_HEAD_DIM=..., a multiple of 8 up to
-// 256; in shared memory rows are zero-padded to the next multiple of 16, the k extent of one MMA).
+// Attention of beams over a paged cache, one query token a beam.
 //
 //   out_i = softmax(q_i K_i' scale) V_i over the first kv_len[i] keys of beam i; scores, maximum and sum in float32, weights
 //   rounded to bfloat16 for the product with V, whose accumulators are float32.
@@ -7,62 +6,62 @@
 // Beams of a request hold the same pages up to where they parted.  The rows of a tile are the (beam, query head) pairs of one key
 // head, so that a shared page is read once for all beams; behind it every beam's own pages follow, one beam after another, for
 // the rows of that beam alone.  A softmax over a union of keys joins from (maximum, sum, weighted values), whoever made the parts.
+//
+// Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their units of 32 keys.  Every
+// team of warps has an even, consecutive share of it: the copy engine brings its units (128-byte swizzle) into a ring of the team's
+// own, ahead across the ends of requests.  A warp has 16 rows; a team is as many warps as the rows need, up to eight, all on the same
+// units.  Warp-level products (mma.sync): a request's rows are an eighth to a half of a tensor-core tile.  Where a share ends inside a block of
+// rows, the sums go out as a partial result; a second launch joins those.
 #include <math_constants.h>
 #include <stdio.h>
 
-#include "common.cuh"
-
-#ifndef JB_HEAD_DIM
-#define JB_HEAD_DIM 128
-#endif
+#include "tc_common.cuh"
 
 namespace {
 
 typedef __nv_bfloat16 bf16;
 
-constexpr int HD = JB_HEAD_DIM;
-static_assert(HD % 8 == 0 && HD >= 8 && HD <= 256, "head size must be a multiple of 8 in [8, 256]");
-constexpr int HDP = (HD + 15) / 16 * 16;
-constexpr int PAGE = 64;
-constexpr int LD = HDP + 8;                        // padded row: an odd number of 16-byte chunks, conflict-free ldmatrix
-constexpr int CHUNKS = HD / 8;
-constexpr int THREADS = 128;
-constexpr int TILE = PAGE * LD, STAGE = 2 * TILE;  // elements
-constexpr int STAGES = HD > 128 ? 2 : 3;
-constexpr int MT = HD > 128 ? 1 : 2;               // row tiles of 16 a block: what the registers hold of float32 results
-constexpr int ROWS = 16 * MT;
-constexpr int RED_LD = HD + 8;
+constexpr int PAGE = 64, KEYS = 32;                // keys of a page, of a unit
 constexpr int MOST_BEAMS = 32;
+constexpr float RESCALE_LOG2 = 8.0f;               // weights may grow to 2^8 before what was summed up is scaled down
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Args {
   const bf16* q;
-  const bf16* k_cache;
-  const bf16* v_cache;
   bf16* out;
-  float* part_o;       // [rows of beams][heads][splits][HD], not divided by their sums
-  float* part_ml;      // ... [2]: maximum (in units of log2), sum
+  float* part_o;       // [teams][2][rows of a team][hd], not divided by their sums; of a share's first rows (0) and last rows (1)
+  float2* part_ml;     // ... maximum (in units of log2), sum
+  int2* parts;         // [beams][heads]: first team with a part of the row, number of teams
   const int* table;
   const int* kv_len;
   const int* shared;
-  int R, K, nh, nkv, W, n_pages, splits;
+  int R, K, nh, nkv, hd, W, n_pages;
+  int team, row_blocks, fewest;                    // warps of a team; blocks of rows of a request; units of a share at least
   float scale_log2;
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], const void* p) {
+constexpr int ROWS = 16;                           // of a warp
+
+template <int HDC>
+struct Shape {
+  static constexpr int SLABS = HDC / 64, SLAB = KEYS * 128;                // 64 numbers of the keys of a unit
+  static constexpr int TILE = SLABS * SLAB, STAGE = 2 * TILE;              // keys, values
+  static constexpr int STAGES = HDC > 128 ? 6 : 12, RING = STAGES * STAGE;
+  // queries lie in registers, as the products take them, where results leave room for them
+  static constexpr bool Q_REGS = HDC <= 128;
+  static constexpr int Q_SLAB = ROWS * 128, Q = Q_REGS ? 0 : SLABS * Q_SLAB;
+  static constexpr int Q_WARPS = 4;                                        // (at most, where queries lie in shared memory)
+  static constexpr int SMEM = RING + Q_WARPS * Q + STAGES * 24;            // ... and two barriers and a unit's description a stage
+  static_assert(SMEM <= 227 * 1024, "shared memory of a block");
+};
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)));
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const void* p) {
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)));
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -72,323 +71,422 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-
-// What a block reads next: a page, how many of its keys count, and for whose rows (-1: all that share it).
-struct Unit {
-  int page, keys, beam;
-};
-
-__global__ void __launch_bounds__(THREADS) beam_attention_kernel(const Args a) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  bf16* q_s = reinterpret_cast<bf16*>(smem_raw);       // [ROWS][LD]
-  bf16* kv_s = q_s + ROWS * LD;                        // [STAGES][K [64][LD], V [64][LD]]; the warps' exchange at the end
-  __shared__ int length_s[MOST_BEAMS], first_s[MOST_BEAMS];   // keys of a beam; its first page of its own
-  __shared__ int upto_s[MOST_BEAMS];                   // own pages of the beams up to this one
-  __shared__ int shared_s, head_s;
-  jb::pdl_launch_dependents();
-  const int K = a.K, G = a.nh / a.nkv, blocks = (K * G + ROWS - 1) / ROWS;
-  const int split = blockIdx.x, kvh = blockIdx.y / blocks, rho0 = blockIdx.y % blocks * ROWS, r = blockIdx.z;
-  const int n_rows = min(ROWS, K * G - rho0);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  jb::pdl_wait();
-  // ---- which pages: shared ones first, then each beam's own (of the beams whose rows the block has) ----
-  const int beam0 = rho0 / G, beam1 = (rho0 + n_rows - 1) / G;
-  if (warp == 0) {
-    const int len = lane < K ? min(max(a.kv_len[r * K + lane], 0), a.W * PAGE) : 0, pages = (len + PAGE - 1) / PAGE;
-    const int most = __reduce_max_sync(0xffffffffu, len);
-    const int head = __ffs(__ballot_sync(0xffffffffu, lane < K && len == most)) - 1;
-    const int common = min(max(a.shared[r], 0), most / PAGE);
-    const int first = len < common * PAGE ? 0 : common;      // shorter beams read all they have by themselves
-    int n = lane >= beam0 && lane <= beam1 ? pages - first : 0;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, n, o);
-      if (lane >= o) n += t;
-    }
-    length_s[lane] = len;
-    first_s[lane] = first;
-    upto_s[lane] = n;
-    if (lane == 0) shared_s = common, head_s = head;
-  }
-  __syncthreads();
-  const int common = shared_s, units = common + upto_s[beam1];
-  const int* head_pages = a.table + ((size_t)r * K + head_s) * a.W;
-  const int u_start = (int)((long long)split * units / a.splits), u_end = (int)((long long)(split + 1) * units / a.splits);
-  auto unit_of = [&](int u) {
-    Unit x;
-    if (u < common) {
-      x.page = head_pages[u];
-      x.keys = PAGE;
-      x.beam = -1;
-    } else {
-      const int i = u - common;
-      int b = beam0;
-      while (upto_s[b] <= i) ++b;
-      const int column = first_s[b] + i - (b > 0 ? upto_s[b - 1] : 0);
-      x.page = a.table[((size_t)r * K + b) * a.W + column];
-      x.keys = min(PAGE, length_s[b] - column * PAGE);
-      x.beam = b;
-    }
-    if (x.page < 0 || x.page >= a.n_pages) x.page = 0, x.keys = 0;     // no page: no keys
-    return x;
-  };
-  // Every warp loads, waits for and computes its own 16 keys of each page: no barrier of the block in the loop.
-  auto issue = [&](const Unit& x, int stage) {
-    const size_t row0 = ((size_t)x.page * a.nkv + kvh) * PAGE + warp * 16;
-    bf16* k_rows = kv_s + (size_t)stage * STAGE + warp * 16 * LD;
-    bf16* v_rows = k_rows + TILE;
-    for (int ch = lane; ch < 16 * CHUNKS; ch += 32) {
-      const int row = ch / CHUNKS, col = ch % CHUNKS;
-      cp_async16(k_rows + row * LD + col * 8, a.k_cache + (row0 + row) * HD + col * 8);
-      cp_async16(v_rows + row * LD + col * 8, a.v_cache + (row0 + row) * HD + col * 8);
-    }
-  };
-  if constexpr (HDP != HD) {         // columns behind the head's numbers are never loaded
-    constexpr int PAD = HDP > HD ? HDP - HD : 1;
-    for (int i = threadIdx.x; i < STAGES * 2 * PAGE * PAD; i += THREADS) kv_s[(i / PAD) * LD + HD + i % PAD] = __float2bfloat16_rn(0.0f);
-  }
-  Unit ring[STAGES];
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) {
-    if (u_start + s < u_end) {
-      ring[s] = unit_of(u_start + s);
-      issue(ring[s], s);
-    }
-    cp_async_commit();
-  }
-  for (int ch = threadIdx.x; ch < ROWS * (HDP / 8); ch += THREADS) {
-    const int row = ch / (HDP / 8), col = ch % (HDP / 8), rho = rho0 + row;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (row < n_rows && col < CHUNKS)
-      v = *reinterpret_cast<const uint4*>(a.q + (((size_t)r * K + rho / G) * a.nh + kvh * G + rho % G) * HD + col * 8);
-    *reinterpret_cast<uint4*>(q_s + row * LD + col * 8) = v;
-  }
-  __syncthreads();
-  int beam_of[MT][2];                // of this thread's rows; -1: no row
-  bool joins[MT][2];                 // whether the row reads the shared pages
-  float m[MT][2], l[MT][2], o[MT][HDP / 8][4];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = t * 16 + (lane >> 2) + 8 * h;
-      beam_of[t][h] = row < n_rows ? (rho0 + row) / G : -1;
-      joins[t][h] = row < n_rows && length_s[beam_of[t][h]] >= common * PAGE;
-      m[t][h] = -CUDART_INF_F;
-      l[t][h] = 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < HDP / 8; ++j) o[t][j][0] = o[t][j][1] = o[t][j][2] = o[t][j][3] = 0.0f;
-  }
-  const int c = lane & 3;
-  for (int u0 = u_start; u0 < u_end; u0 += STAGES) {
-#pragma unroll
-    for (int stage = 0; stage < STAGES; ++stage) {
-      const int u = u0 + stage;
-      if (u >= u_end) break;
-      constexpr int AHEAD = STAGES - 1;
-      if (u + AHEAD < u_end) {
-        ring[(stage + AHEAD) % STAGES] = unit_of(u + AHEAD);
-        issue(ring[(stage + AHEAD) % STAGES], (stage + AHEAD) % STAGES);
-      }
-      cp_async_commit();
-      cp_async_wait<AHEAD>();
-      __syncwarp();
-      const Unit x = ring[stage];
-      bf16* k_tile = kv_s + (size_t)stage * STAGE + warp * 16 * LD;
-      bf16* v_tile = k_tile + TILE;
-      const int keys = x.keys - warp * 16;            // of this warp's 16
-      if (keys > 0) {
-        if (keys < 16) {                              // values behind the last key: a weight of 0 does not silence what is no number
-          for (int i = lane; i < (16 - keys) * (HDP / 8); i += 32)
-            *reinterpret_cast<uint4*>(v_tile + (keys + i / (HDP / 8)) * LD + i % (HDP / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
-          __syncwarp();
-        }
-        bool skip[MT];
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-          skip[t] = x.beam >= 0 && ((x.beam + 1) * G <= rho0 + t * 16 || x.beam * G >= rho0 + t * 16 + 16);
-        float s[MT][2][4];
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) s[t][j][0] = s[t][j][1] = s[t][j][2] = s[t][j][3] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < HDP / 16; ++ks) {
-          uint32_t b[4];
-          ldmatrix_x4(b, k_tile + ((lane & 7) + ((lane >> 4) << 3)) * LD + ks * 16 + ((lane >> 3) & 1) * 8);
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            if (!skip[t]) {
-              uint32_t qa[4];
-              ldmatrix_x4(qa, q_s + (t * 16 + (lane & 15)) * LD + ks * 16 + (lane >> 4) * 8);
-              mma_bf16(s[t][0], qa, b[0], b[1]);
-              mma_bf16(s[t][1], qa, b[2], b[3]);
-            }
-          }
-        }
-        uint32_t pa[MT][4];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          if (skip[t]) continue;
-          float mx[2] = {-CUDART_INF_F, -CUDART_INF_F}, corr[2], use[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int h = e >> 1, key = j * 8 + 2 * c + (e & 1);
-              const bool ok = key < keys && (x.beam < 0 ? joins[t][h] : beam_of[t][h] == x.beam);
-              s[t][j][e] = ok ? s[t][j][e] * a.scale_log2 : -CUDART_INF_F;
-              mx[h] = fmaxf(mx[h], s[t][j][e]);
-            }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            const float next = fmaxf(m[t][h], mx[h]);
-            use[h] = next == -CUDART_INF_F ? 0.0f : next;
-            corr[h] = exp2f(m[t][h] - use[h]);
-            m[t][h] = next;
-            l[t][h] *= corr[h];
-          }
-#pragma unroll
-          for (int j = 0; j < HDP / 8; ++j) {
-            o[t][j][0] *= corr[0];
-            o[t][j][1] *= corr[0];
-            o[t][j][2] *= corr[1];
-            o[t][j][3] *= corr[1];
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              s[t][j][e] = exp2f(s[t][j][e] - use[e >> 1]);
-              l[t][e >> 1] += s[t][j][e];
-            }
-          pa[t][0] = pack_bf16(s[t][0][0], s[t][0][1]);
-          pa[t][1] = pack_bf16(s[t][0][2], s[t][0][3]);
-          pa[t][2] = pack_bf16(s[t][1][0], s[t][1][1]);
-          pa[t][3] = pack_bf16(s[t][1][2], s[t][1][3]);
-        }
-#pragma unroll
-        for (int j = 0; j < HDP / 8; j += 2) {
-          uint32_t b[4];
-          ldmatrix_x4_trans(b, v_tile + (lane & 15) * LD + j * 8 + (lane >> 4) * 8);
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            if (!skip[t]) {
-              mma_bf16(o[t][j], pa[t], b[0], b[1]);
-              mma_bf16(o[t][j + 1], pa[t], b[2], b[3]);
-            }
-          }
-        }
-      }
-      __syncwarp();   // the warp is done with its rows of this stage before its next loads overwrite them
-    }
-  }
-  cp_async_wait<0>();
-  __syncthreads();    // every warp has left the ring: its memory becomes the exchange
-  float* red_o = reinterpret_cast<float*>(kv_s);             // [4][ROWS][RED_LD]
-  float* red_ml = red_o + 4 * ROWS * RED_LD;                 // [4][ROWS][2]
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float sum = l[t][h];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const int row = t * 16 + (lane >> 2) + 8 * h;
-      if (c == 0) red_ml[(warp * ROWS + row) * 2] = m[t][h], red_ml[(warp * ROWS + row) * 2 + 1] = sum;
-#pragma unroll
-      for (int j = 0; j < HDP / 8; ++j)
-        if (j * 8 < HD)
-          *reinterpret_cast<float2*>(red_o + (size_t)(warp * ROWS + row) * RED_LD + j * 8 + 2 * c) = make_float2(o[t][j][2 * h], o[t][j][2 * h + 1]);
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n_rows * HD; i += THREADS) {
-    const int row = i / HD, d = i % HD, rho = rho0 + row;
-    float most = -CUDART_INF_F;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) most = fmaxf(most, red_ml[(w * ROWS + row) * 2]);
-    const float use = most == -CUDART_INF_F ? 0.0f : most;
-    float value = 0.0f, sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = exp2f(red_ml[(w * ROWS + row) * 2] - use);
-      value += red_o[(size_t)(w * ROWS + row) * RED_LD + d] * f;
-      sum += red_ml[(w * ROWS + row) * 2 + 1] * f;
-    }
-    const size_t item = ((size_t)r * K + rho / G) * a.nh + kvh * G + rho % G;
-    if (a.splits == 1) {
-      a.out[item * HD + d] = __float2bfloat16_rn(sum > 0.0f ? value / sum : 0.0f);
-    } else {
-      const size_t part = item * a.splits + split;
-      if (most > -CUDART_INF_F) a.part_o[part * HD + d] = value;       // (a part without keys weighs nothing and is not read)
-      if (d == 0) a.part_ml[part * 2] = most, a.part_ml[part * 2 + 1] = sum;
-    }
-  }
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// A warp a (beam, head): the parts of its keys joined.
-__global__ void __launch_bounds__(128) beam_attention_join_kernel(const Args a) {
+// A block of rows of a request, as a warp knows it; lane b knows beam b.
+struct Rows {
+  int request, rho0, n_rows;        // rows rho0 .. of the request's beams * group
+  int common, head;                 // pages that its beams share; the beam whose table lists them
+  int units;
+  int len, first, own, upto;        // of the lane's beam: keys, first page of its own, units of its own, of the beams up to it
+};
+
+__device__ __forceinline__ Rows look_up(const Args& a, int block) {
+  const int lane = threadIdx.x & 31, G = a.nh / a.nkv, all = ROWS * a.team;
+  Rows x;
+  x.request = block / a.row_blocks;
+  x.rho0 = block % a.row_blocks * all;
+  x.n_rows = min(all, a.K * G - x.rho0);
+  x.len = lane < a.K ? min(max(a.kv_len[x.request * a.K + lane], 0), a.W * PAGE) : 0;
+  const int most = __reduce_max_sync(0xffffffffu, x.len);
+  x.head = __ffs(__ballot_sync(0xffffffffu, lane < a.K && x.len == most)) - 1;
+  x.common = min(max(a.shared[x.request], 0), most / PAGE);
+  x.first = x.len < x.common * PAGE ? 0 : x.common;        // shorter beams read all they have by themselves
+  x.own = lane >= x.rho0 / G && lane <= (x.rho0 + x.n_rows - 1) / G ? (x.len - x.first * PAGE + KEYS - 1) / KEYS : 0;
+  x.upto = x.own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, x.upto, o);
+    if (lane >= o) x.upto += t;
+  }
+  x.units = max(1, x.common * (PAGE / KEYS) + __shfl_sync(0xffffffffu, x.upto, 31));     // (rows without keys have a unit as well)
+  return x;
+}
+// The units of a block, by one thread.
+__device__ __forceinline__ int count_units(const Args& a, int block) {
+  const int G = a.nh / a.nkv, all = ROWS * a.team, r = block / a.row_blocks, rho0 = block % a.row_blocks * all;
+  const int beam0 = rho0 / G, beam1 = (min(rho0 + all, a.K * G) - 1) / G;
+  int most = 0;
+#pragma unroll 4
+  for (int k = 0; k < a.K; ++k) most = max(most, min(max(a.kv_len[r * a.K + k], 0), a.W * PAGE));
+  const int common = min(max(a.shared[r], 0), most / PAGE);
+  int n = common * (PAGE / KEYS);
+#pragma unroll 4
+  for (int k = beam0; k <= beam1; ++k) {
+    const int len = min(max(a.kv_len[r * a.K + k], 0), a.W * PAGE);
+    n += (len - (len < common * PAGE ? 0 : common * PAGE) + KEYS - 1) / KEYS;
+  }
+  return max(1, n);
+}
+
+// A unit: where its keys lie (row of the tensor map / KEYS, of the first key head), how many count, for whose rows (-1: all that share them).
+struct Unit {
+  int page, half, keys, beam;
+};
+__device__ __forceinline__ Unit unit_of(const Args& a, const Rows& x, int i) {
+  Unit u{0, 0, 0, -1};
+  const int shared_units = x.common * (PAGE / KEYS), j = i - shared_units;
+  if (j < 0) {
+    u.page = a.table[((size_t)x.request * a.K + x.head) * a.W + i / (PAGE / KEYS)];
+    u.half = i % (PAGE / KEYS);
+    u.keys = KEYS;
+  } else {
+    const unsigned behind = __ballot_sync(0xffffffffu, x.upto > j);
+    if (behind != 0u) {
+      u.beam = __ffs(behind) - 1;
+      const int before = __shfl_sync(0xffffffffu, x.upto - x.own, u.beam), first = __shfl_sync(0xffffffffu, x.first, u.beam);
+      const int at = first * PAGE + (j - before) * KEYS;
+      u.page = a.table[((size_t)x.request * a.K + u.beam) * a.W + at / PAGE];
+      u.half = at / KEYS % (PAGE / KEYS);
+      u.keys = min(KEYS, __shfl_sync(0xffffffffu, x.len, u.beam) - at);
+    }
+  }
+  return u;
+}
+
+template <int HDC>
+__global__ void __launch_bounds__(256) beam_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                             const Args a, int* __restrict__ status) {
+  typedef Shape<HDC> C;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, hd = a.hd, G = a.nh / a.nkv;
+  const int T = a.team, here = blockDim.x / 32 / T, team = warp / T, member = warp % T, stages = C::STAGES / here;
+  const uint32_t base = jb::smem_u32(smem), ring = base + team * stages * C::STAGE;
+  const uint32_t bars = base + C::RING + C::Q_WARPS * C::Q + team * stages * 16;   // of a stage: full, empty
+  int2* about = reinterpret_cast<int2*>(smem + C::RING + C::Q_WARPS * C::Q + C::STAGES * 16) + team * stages;   // keys, beam
+  if (member == 0 && lane == 0) {
+    for (int i = 0; i < stages; ++i) jb::mbar_init(bars + 16 * i, 1), jb::mbar_init(bars + 16 * i + 8, T);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  jb::pdl_launch_dependents();
+  jb::pdl_wait();
+  // ---- the list's length, and this team's share ----
+  const int blocks = a.R * a.row_blocks, chunk = (blocks + 31) / 32, block0 = min(lane * chunk, blocks), block1 = min(block0 + chunk, blocks);
+  int mine = 0;
+  for (int i = block0; i < block1; ++i) mine += count_units(a, i);
+  mine *= a.nkv;
+  int up = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += t;
+  }
+  const int total = __shfl_sync(0xffffffffu, up, 31), teams = gridDim.x * here, worker = blockIdx.x * here + team;
+  const int per = max(a.fewest, (total + teams - 1) / teams);
+  const int begin = min(worker * per, total), end = min(begin + per, total);
+  if (begin >= end) return;                                // (a whole team)
+  Rows x;
+  int block, kvh, unit;                                    // the place of the list
+  {
+    const int owner = __ffs(__ballot_sync(0xffffffffu, begin < up)) - 1;
+    int before = __shfl_sync(0xffffffffu, up - mine, owner);
+    for (block = owner * chunk;; ++block) {
+      x = look_up(a, block);
+      if (begin < before + x.units * a.nkv) break;
+      before += x.units * a.nkv;
+    }
+    kvh = (begin - before) / x.units;
+    unit = begin - before - kvh * x.units;
+  }
+  // ---- the team's first warp asks for units, ahead across the ends of rows ----
+  Rows ahead_x = x;
+  int ahead_block = block, ahead_kvh = kvh, ahead_unit = unit, asked = begin, asked_stage = 0;
+  Unit next{0, 0, 0, -1};
+  if (member == 0) next = unit_of(a, ahead_x, ahead_unit);
+  auto issue = [&]() {                                     // by all lanes of the first warp
+    const bool there = next.page >= 0 && next.page < a.n_pages;     // (no page: no keys)
+    const int row = ((there ? next.page : 0) * a.nkv + ahead_kvh) * PAGE + next.half * KEYS;
+    if (lane == 0) {
+      about[asked_stage] = make_int2(there ? next.keys : 0, next.beam);
+      const uint32_t full = bars + 16 * asked_stage, to = ring + asked_stage * C::STAGE;
+      jb::mbar_expect_tx(full, C::STAGE);                  // (behind the head's numbers the copy engine writes zeroes)
+#pragma unroll
+      for (int h = 0; h < C::SLABS; ++h) jb::tma_load_2d(to + h * C::SLAB, &map_k, full, h * 64, row);
+#pragma unroll
+      for (int h = 0; h < C::SLABS; ++h) jb::tma_load_2d(to + C::TILE + h * C::SLAB, &map_v, full, h * 64, row);
+    }
+    __syncwarp();
+    if (++asked_stage == stages) asked_stage = 0;
+    if (++asked < end) {                                   // (a unit's page is looked up a turn before it is asked for)
+      if (++ahead_unit == ahead_x.units) {
+        ahead_unit = 0;
+        if (++ahead_kvh == a.nkv) {
+          ahead_kvh = 0;
+          ahead_x = look_up(a, ++ahead_block);
+        }
+      }
+      next = unit_of(a, ahead_x, ahead_unit);
+    }
+  };
+  if (member == 0)
+    for (int i = 0; i < stages && asked < end; ++i) issue();
+  // Places of the operands in swizzled rows: 16 bytes `piece` of row r lie at piece ^ (r % 8), so that a step of 32 bytes is an
+  // exclusive or.
+  const int c = lane & 3, r8 = lane & 7;
+  const uint32_t k_lane = (r8 + ((lane >> 4) << 3)) * 128 + ((((lane >> 3) & 1) ^ r8) << 4);
+  const uint32_t v_lane = (lane & 15) * 128 + (((lane >> 4) ^ r8) << 4);
+  const uint32_t q_at = base + C::RING + warp * C::Q;
+  int beam_of[2] = {-1, -1};         // of this thread's rows; -1: no row
+  bool joins[2] = {false, false};    // whether the row reads the shared pages
+  bool all_join = false;
+  int beam_first = 0, beam_last = -1;     // of the warp's rows
+  float m[2], l[2], o[HDC / 8][4];
+  uint32_t q[C::Q_REGS ? HDC / 16 : 1][4];
+  bool ok = true;
+  int st = 0, st_before = 0;
+  uint32_t phase = 0, phase_before = 0;
+  for (int i = begin; i < end; ++i) {
+    if (i > begin && member == 0 && asked < end) {         // the stage of the turn before, when all warps are done with it
+      ok = jb::mbar_wait(bars + 16 * st_before + 8, phase_before, status, 54);
+      if (__any_sync(0xffffffffu, !ok)) break;
+      issue();
+    }
+    if (i == begin || unit == 0) {
+      const int row0 = member * ROWS, rho0 = x.rho0 + row0, n_rows = min(ROWS, x.n_rows - row0);
+      beam_first = rho0 / G, beam_last = n_rows > 0 ? (rho0 + n_rows - 1) / G : -1;
+      bool every = true;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = (lane >> 2) + 8 * h;
+        const bool valid = row < n_rows;
+        beam_of[h] = valid ? (rho0 + row) / G : -1;
+        const int len = __shfl_sync(0xffffffffu, x.len, max(beam_of[h], 0));
+        joins[h] = valid && len >= x.common * PAGE;
+        every = every && (joins[h] || !valid);
+        m[h] = -CUDART_INF_F;
+        l[h] = 0.0f;
+        if constexpr (C::Q_REGS) {
+          const bf16* src = a.q + (((size_t)x.request * a.K + max(beam_of[h], 0)) * a.nh + kvh * G + (valid ? (rho0 + row) % G : 0)) * hd + 2 * c;
+#pragma unroll
+          for (int ks = 0; ks < HDC / 16; ++ks)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+              q[ks][h + 2 * half] = valid && ks * 16 + half * 8 < hd ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + half * 8) : 0u;
+        }
+      }
+      if constexpr (!C::Q_REGS) {
+        for (int ch = lane; ch < ROWS * C::SLABS * 8; ch += 32) {
+          const int row = ch / (C::SLABS * 8), piece = ch % (C::SLABS * 8), rho = rho0 + row;
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (row < n_rows && piece * 8 < hd)
+            v = *reinterpret_cast<const uint4*>(a.q + (((size_t)x.request * a.K + rho / G) * a.nh + kvh * G + rho % G) * hd + piece * 8);
+          *reinterpret_cast<uint4*>(smem + C::RING + warp * C::Q + (piece / 8) * C::Q_SLAB + row * 128 + (((piece % 8) ^ (row & 7)) << 4)) = v;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < HDC / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+      all_join = __all_sync(0xffffffffu, every);           // (rows behind the last may do as they like)
+      __syncwarp();
+    }
+    ok = jb::mbar_wait(bars + 16 * st, phase, status, 53);
+    if (__any_sync(0xffffffffu, !ok)) break;
+    const int2 info = about[st];
+    const int keys = info.x, beam = info.y;
+    const uint32_t k_t = ring + st * C::STAGE, v_t = k_t + C::TILE;
+    // (units of another warp's beams are nothing to this one)
+    if (keys > 0 && (beam < 0 ? beam_last >= 0 : beam >= beam_first && beam <= beam_last)) {
+      if (keys < KEYS) {                                   // values behind the last key: a weight of 0 does not silence what is no number
+        for (int p = lane; p < (KEYS - keys) * C::SLABS * 8; p += 32) {
+          const int row = keys + p / (C::SLABS * 8), piece = p % (C::SLABS * 8);
+          *reinterpret_cast<uint4*>(smem + (v_t - base) + (piece / 8) * C::SLAB + row * 128 + ((piece % 8) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+      }
+      float s[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < HDC / 16; ++ks) {
+        uint32_t qa[4], b[2][4];
+        const uint32_t at = k_t + (k_lane ^ ((ks % 4) << 5)) + (ks / 4) * C::SLAB;
+        ldmatrix_x4(b[0], at);
+        ldmatrix_x4(b[1], at + 16 * 128);
+        if constexpr (C::Q_REGS) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qa[e] = q[ks][e];
+        } else {
+          ldmatrix_x4(qa, q_at + (v_lane ^ ((ks % 4) << 5)) + (ks / 4) * C::Q_SLAB);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          mma_bf16(s[2 * j], qa, b[j][0], b[j][1]);
+          mma_bf16(s[2 * j + 1], qa, b[j][2], b[j][3]);
+        }
+      }
+      if (beam >= 0 || keys < KEYS || !all_join) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int h = e >> 1, key = j * 8 + 2 * c + (e & 1);
+            if (!(key < keys && (beam < 0 ? joins[h] : beam_of[h] == beam))) s[j][e] = -CUDART_INF_F;
+          }
+      }
+      float mx[2], use[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mx[h] = fmaxf(fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1])),
+                      fmaxf(fmaxf(s[2][2 * h], s[2][2 * h + 1]), fmaxf(s[3][2 * h], s[3][2 * h + 1])));
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * a.scale_log2;
+      }
+      // (also the first number of all)
+      if (__any_sync(0xffffffffu, mx[0] > m[0] + RESCALE_LOG2 || mx[1] > m[1] + RESCALE_LOG2)) {
+        float corr[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float top = fmaxf(m[h], mx[h]);
+          corr[h] = top == -CUDART_INF_F ? 1.0f : fast_exp2(m[h] - top);
+          m[h] = top;
+          l[h] *= corr[h];
+        }
+#pragma unroll
+        for (int j = 0; j < HDC / 8; ++j) o[j][0] *= corr[0], o[j][1] *= corr[0], o[j][2] *= corr[1], o[j][3] *= corr[1];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) use[h] = m[h] == -CUDART_INF_F ? 0.0f : m[h];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][e] = fast_exp2(fmaf(s[j][e], a.scale_log2, -use[e >> 1]));
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        l[h] += ((s[0][2 * h] + s[0][2 * h + 1]) + (s[1][2 * h] + s[1][2 * h + 1])) + ((s[2][2 * h] + s[2][2 * h + 1]) + (s[3][2 * h] + s[3][2 * h + 1]));
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const uint32_t pa[4] = {pack_bf16(s[2 * kk][0], s[2 * kk][1]), pack_bf16(s[2 * kk][2], s[2 * kk][3]),
+                                pack_bf16(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack_bf16(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+        for (int j = 0; j < HDC / 8; j += 2) {
+          uint32_t b[4];
+          ldmatrix_x4_trans(b, v_t + (v_lane ^ ((j % 8) << 4)) + (j / 8) * C::SLAB + kk * 16 * 128);
+          mma_bf16(o[j], pa, b[0], b[1]);
+          mma_bf16(o[j + 1], pa, b[2], b[3]);
+        }
+      }
+      if (keys < KEYS) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // zeroes, before the copy engine writes there again
+    }
+    __syncwarp();
+    if (lane == 0) jb::mbar_arrive(bars + 16 * st + 8);
+    st_before = st, phase_before = phase;
+    if (++st == stages) st = 0, phase ^= 1;
+    if (unit + 1 == x.units || i + 1 == end) {             // the rows' keys end here, or the share does
+      const int start = i - unit, first = start / per, last = (start + x.units - 1) / per;
+      const bool complete = first == last;
+      const size_t record = ((size_t)worker * 2 + (worker == first ? 1 : 0)) * (ROWS * T) + member * ROWS;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float sum = l[h];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const int row = (lane >> 2) + 8 * h, rho = x.rho0 + member * ROWS + row;
+        if (beam_of[h] < 0) continue;
+        const size_t item = ((size_t)x.request * a.K + beam_of[h]) * a.nh + kvh * G + rho % G;
+        if (c == 0) {
+          if (worker == first) a.parts[item] = make_int2(first, last - first + 1);
+          if (!complete) a.part_ml[record + row] = make_float2(m[h], sum);
+        }
+        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+        for (int j = 0; j < HDC / 8; ++j) {
+          if (j * 8 < hd) {
+            if (complete) *reinterpret_cast<uint32_t*>(a.out + item * hd + j * 8 + 2 * c) = pack_bf16(o[j][2 * h] * inv, o[j][2 * h + 1] * inv);
+            else *reinterpret_cast<float2*>(a.part_o + (record + row) * hd + j * 8 + 2 * c) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+          }
+        }
+      }
+    }
+    if (++unit == x.units) {
+      unit = 0;
+      if (++kvh == a.nkv) {
+        kvh = 0;
+        if (i + 1 < end) x = look_up(a, ++block);
+      }
+    }
+  }
+  if (!ok && member == 0)                                  // gave up: what is still on its way arrives first (or its wait gives up as well)
+    for (int turn = max(0, asked - begin - stages); turn < asked - begin; ++turn)
+      jb::mbar_wait(bars + 16 * (turn % stages), (turn / stages) & 1, status, 53);
+}
+
+// A warp a (beam, head): the parts of its keys joined, where there are several.
+__global__ void __launch_bounds__(128) beam_attention_join_kernel(const Args a, int rows) {
   jb::pdl_launch_dependents();
   jb::pdl_wait();
   const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, G = a.nh / a.nkv;
   if (item >= (long long)a.R * a.K * a.nh) return;
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + item * a.splits;
+  const int2 parts = a.parts[item];
+  if (parts.y <= 1) return;
+  const int head = (int)(item % a.nh), beam = (int)(item / a.nh % a.K), row = (beam * G + head % G) % rows;
+  auto record = [&](int p) { return ((size_t)(parts.x + p) * 2 + (p == 0 ? 1 : 0)) * rows + row; };
   float most = -CUDART_INF_F;
-  for (int s = lane; s < a.splits; s += 32) most = fmaxf(most, ml[s].x);
+  for (int p = lane; p < parts.y; p += 32) most = fmaxf(most, a.part_ml[record(p)].x);
   most = jb::warp_max(most);
   const float use = most == -CUDART_INF_F ? 0.0f : most;
-  constexpr int N = (HD + 31) / 32;
-  float o[N], sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) o[i] = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 x = ml[s];
-    if (x.x == -CUDART_INF_F) continue;
-    const float f = exp2f(x.x - use);
-    sum += x.y * f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i * 32 + lane < HD) o[i] += a.part_o[(item * a.splits + s) * HD + i * 32 + lane] * f;
+  for (int d = lane * 4; d < a.hd; d += 128) {
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int p = 0; p < parts.y; ++p) {
+      const float2 ml = a.part_ml[record(p)];
+      const float4 v = *reinterpret_cast<const float4*>(a.part_o + record(p) * a.hd + d);
+      const float f = fast_exp2(ml.x - use);
+      sum = fmaf(f, ml.y, sum);
+      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    *reinterpret_cast<uint2*>(a.out + item * a.hd + d) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (i * 32 + lane < HD) a.out[item * HD + i * 32 + lane] = __float2bfloat16_rn(sum > 0.0f ? o[i] / sum : 0.0f);
 }
 
-constexpr int RING_BYTES = STAGES * STAGE * 2, RED_BYTES = 4 * ROWS * (RED_LD + 2) * 4;
-constexpr int SMEM = ROWS * LD * 2 + (RING_BYTES > RED_BYTES ? RING_BYTES : RED_BYTES);
-static_assert(SMEM <= 227 * 1024, "shared memory of a block");
-
-}  // namespace
-
-// part: float32 scratch of R K nh splits (HD + 2) numbers where splits > 1.
-JB_EXPORT int jb_attention_beams(const void* q, const void* k_cache, const void* v_cache, void* out, void* part, const int* table,
-                                 const int* kv_len, const int* shared, int R, int K, int nh, int nkv, int W, int n_pages, int splits,
-                                 float scale, cudaStream_t stream) {
-  const int blocks = nkv > 0 && nh > 0 ? nkv * ((K * (nh / nkv) + ROWS - 1) / ROWS) : 0;
-  JB_REFUSE(R < 1 || R > 65535 || K < 1 || K > MOST_BEAMS || nkv < 1 || nh < nkv || nh % nkv || W < 1 || W > 0x7fffffff / PAGE || n_pages < 1 ||
-                splits < 1 || blocks > 65535,
-            "attention_beams: %d groups of %d beams, %d heads over %d, %d pages a row, %d splits", R, K, nh, nkv, W, splits);
+template <int HDC>
+cudaError_t go(const CUtensorMap* maps, Args a, int blocks, int warps, int* status, cudaStream_t stream) {
+  typedef Shape<HDC> C;
   static bool ready[64] = {};
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
-  if (e != cudaSuccess) return (int)e;
+  if (e != cudaSuccess) return e;
   if (device >= 64 || !ready[device]) {
-    e = cudaFuncSetAttribute(beam_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-    if (e != cudaSuccess) return (int)e;
+    e = cudaFuncSetAttribute(beam_attention_kernel<HDC>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
     if (device < 64) ready[device] = true;
   }
-  float* part_o = (float*)part;
-  Args a{(const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, (bf16*)out, part_o,
-         part_o + (splits > 1 ? (size_t)R * K * nh * splits * HD : 0), table, kv_len, shared, R, K, nh, nkv, W, n_pages, splits, scale * LOG2E};
-  jb::Launch cfg(dim3(splits, blocks, R), dim3(THREADS), SMEM, stream);
-  e = cudaLaunchKernelEx(&cfg.c, beam_attention_kernel, a);
-  if (e != cudaSuccess || splits == 1) return (int)e;
-  jb::Launch join(dim3((unsigned)(((long long)R * K * nh + 3) / 4)), dim3(128), 0, stream);
-  return (int)cudaLaunchKernelEx(&join.c, beam_attention_join_kernel, a);
+  jb::Launch cfg(dim3(blocks), dim3(32 * warps), C::SMEM, stream);
+  e = cudaLaunchKernelEx(&cfg.c, beam_attention_kernel<HDC>, maps[0], maps[1], a, status);
+  if (e != cudaSuccess) return e;
+  jb::Launch join(dim3((unsigned)(((long long)a.R * a.K * a.nh + 3) / 4)), dim3(128), 0, stream);
+  return cudaLaunchKernelEx(&join.c, beam_attention_join_kernel, a, ROWS * a.team);
+}
+
+}  // namespace
+
+// part: float32 scratch of blocks * warps * 16 * 2 (hd + 2) + 2 R K nh numbers.  blocks, warps of a block, team (warps that work on the same
+// units, a divisor of them): see `ops.beam_attention_plan`.
+JB_EXPORT int jb_attention_beams(const void* q, const void* k_cache, const void* v_cache, void* out, void* part, const int* table,
+                                 const int* kv_len, const int* shared, int R, int K, int nh, int nkv, int hd, int W, int n_pages, int blocks,
+                                 int warps, int team, int fewest, float scale, int* status, cudaStream_t stream) {
+  JB_REFUSE(R < 1 || K < 1 || K > MOST_BEAMS || nkv < 1 || nh < nkv || nh % nkv || hd < 8 || hd > 256 || hd % 8 || W < 1 || W > 0x7fffffff / PAGE ||
+                n_pages < 1 || (long long)n_pages * nkv * PAGE > 0x7fffffffLL || blocks < 1 || fewest < 1 || team < 1 || warps < team ||
+                warps % team || warps > (hd > 128 ? 4 : 8) || warps / team > (hd > 128 ? 3 : 6) || !(scale > 0.0f),
+            "attention_beams: %d groups of %d beams, %d heads over %d of %d numbers, %d pages a row of %d, plan %d %d %d %d, scale %g", R, K, nh,
+            nkv, hd, W, n_pages, blocks, warps, team, fewest, scale);
+  CUtensorMap maps[2];
+  if (!jb::make_map_64(&maps[0], k_cache, (uint64_t)n_pages * nkv * PAGE, hd, KEYS, true) ||
+      !jb::make_map_64(&maps[1], v_cache, (uint64_t)n_pages * nkv * PAGE, hd, KEYS, true))
+    return JB_ERR_TENSORMAP;
+  Args a{};
+  a.q = (const bf16*)q, a.out = (bf16*)out, a.table = table, a.kv_len = kv_len, a.shared = shared;
+  const size_t records = (size_t)blocks * warps * ROWS * 2;
+  a.part_o = (float*)part, a.part_ml = (float2*)(a.part_o + records * hd), a.parts = (int2*)(a.part_ml + records);
+  a.R = R, a.K = K, a.nh = nh, a.nkv = nkv, a.hd = hd, a.W = W, a.n_pages = n_pages;
+  a.team = team, a.fewest = fewest, a.scale_log2 = scale * LOG2E;
+  a.row_blocks = (K * (nh / nkv) + ROWS * team - 1) / (ROWS * team);
+  return (int)(hd > 128 ? go<256>(maps, a, blocks, warps, status, stream) : hd > 64 ? go<128>(maps, a, blocks, warps, status, stream)
+                                                                               : go<64>(maps, a, blocks, warps, status, stream));
 }
