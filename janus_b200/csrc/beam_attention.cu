@@ -10,8 +10,8 @@
 // Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their units of 32 keys.  Every
 // team of warps has an even, consecutive share of it: the copy engine brings its units (128-byte swizzle) into a ring of the team's
 // own, ahead across the ends of requests.  A warp has 16 rows; a team is as many warps as the rows need, up to eight, all on the same
-// units.  Warp-level products (mma.sync): a request's rows are an eighth to a half of a tensor-core tile.  Where a share ends inside a block of
-// rows, the sums go out as a partial result; a second launch joins those.
+// units, the first of which asks for them.  Warp-level products (mma.sync): a request's rows are an eighth to a half of a
+// tensor-core tile.  Where a share ends inside a block of rows, the sums go out as a partial result; a second launch joins those.
 #include <math_constants.h>
 #include <stdio.h>
 
@@ -50,6 +50,7 @@ struct Shape {
   // queries lie in registers, as the products take them, where results leave room for them
   static constexpr bool Q_REGS = HDC <= 128;
   static constexpr int Q_SLAB = ROWS * 128, Q = Q_REGS ? 0 : SLABS * Q_SLAB;
+  static constexpr int WARPS = HDC > 128 ? 4 : 8, THREADS = 32 * WARPS;   // at most
   static constexpr int Q_WARPS = 4;                                        // (at most, where queries lie in shared memory)
   static constexpr int SMEM = RING + Q_WARPS * Q + STAGES * 24;            // ... and two barriers and a unit's description a stage
   static_assert(SMEM <= 227 * 1024, "shared memory of a block");
@@ -75,6 +76,21 @@ __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Bounded wait: false (and *status = code) if the phase did not complete in 4e9 cycles, about two seconds.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* status, int code) {
+  if (jb::mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (jb::mbar_try(bar, parity)) return true;
+    if (clock64() - t0 > 4000000000ll) {
+      atomicCAS(status, 0, code);
+      return false;
+    }
+  }
 }
 
 // A block of rows of a request, as a warp knows it; lane b knows beam b.
@@ -123,33 +139,66 @@ __device__ __forceinline__ int count_units(const Args& a, int block) {
   return max(1, n);
 }
 
-// A unit: where its keys lie (row of the tensor map / KEYS, of the first key head), how many count, for whose rows (-1: all that share them).
-struct Unit {
-  int page, half, keys, beam;
-};
-__device__ __forceinline__ Unit unit_of(const Args& a, const Rows& x, int i) {
-  Unit u{0, 0, 0, -1};
-  const int shared_units = x.common * (PAGE / KEYS), j = i - shared_units;
-  if (j < 0) {
-    u.page = a.table[((size_t)x.request * a.K + x.head) * a.W + i / (PAGE / KEYS)];
-    u.half = i % (PAGE / KEYS);
-    u.keys = KEYS;
-  } else {
-    const unsigned behind = __ballot_sync(0xffffffffu, x.upto > j);
-    if (behind != 0u) {
-      u.beam = __ffs(behind) - 1;
-      const int before = __shfl_sync(0xffffffffu, x.upto - x.own, u.beam), first = __shfl_sync(0xffffffffu, x.first, u.beam);
-      const int at = first * PAGE + (j - before) * KEYS;
-      u.page = a.table[((size_t)x.request * a.K + u.beam) * a.W + at / PAGE];
-      u.half = at / KEYS % (PAGE / KEYS);
-      u.keys = min(KEYS, __shfl_sync(0xffffffffu, x.len, u.beam) - at);
+// A place of the list as one thread walks it: the unit's beam (-1: all that share it), its first key, and where its page stands.
+struct Cursor {
+  int block, kvh, unit, units, shared_units;
+  int request, head, common, beam0, beam1;
+  int beam, at, keys;
+  const int* entry;                 // of the table; null: a unit without keys
+
+  __device__ __forceinline__ int length(const Args& a, int b) const { return min(max(a.kv_len[request * a.K + b], 0), a.W * PAGE); }
+  __device__ __forceinline__ int own_from(int len) const { return len < common * PAGE ? 0 : common * PAGE; }
+  __device__ __forceinline__ void enter(const Args& a, int to) {
+    const int G = a.nh / a.nkv, all = ROWS * a.team, rho0 = to % a.row_blocks * all;
+    block = to, request = to / a.row_blocks, beam0 = rho0 / G, beam1 = (min(rho0 + all, a.K * G) - 1) / G;
+    int most = -1;
+    head = 0;
+    for (int k = 0; k < a.K; ++k) {
+      const int len = length(a, k);
+      if (len > most) most = len, head = k;
     }
+    common = min(max(a.shared[request], 0), most / PAGE);
+    units = shared_units = common * (PAGE / KEYS);
+    for (int k = beam0; k <= beam1; ++k) {
+      const int len = length(a, k);
+      units += (len - own_from(len) + KEYS - 1) / KEYS;
+    }
+    units = max(1, units);
   }
-  return u;
-}
+  __device__ __forceinline__ void find(const Args& a) {      // the unit's keys
+    if (unit < shared_units) {
+      beam = -1, at = unit * KEYS, keys = KEYS;
+      entry = a.table + ((size_t)request * a.K + head) * a.W + at / PAGE;
+      return;
+    }
+    int left = unit - shared_units;
+    for (beam = beam0; beam <= beam1; ++beam) {
+      const int len = length(a, beam), from = own_from(len), own = (len - from + KEYS - 1) / KEYS;
+      if (left < own) {
+        at = from + left * KEYS, keys = min(KEYS, len - at);
+        entry = a.table + ((size_t)request * a.K + beam) * a.W + at / PAGE;
+        return;
+      }
+      left -= own;
+    }
+    beam = -1, at = keys = 0, entry = nullptr;
+  }
+  __device__ __forceinline__ void step(const Args& a) {
+    if (++unit == units) {
+      unit = 0;
+      if (++kvh == a.nkv) kvh = 0, enter(a, block + 1);
+    } else if (beam >= 0 && at + KEYS < length(a, beam)) {  // the next keys of the same beam
+      entry += (at % PAGE + KEYS) / PAGE;
+      at += KEYS;
+      keys = min(KEYS, length(a, beam) - at);
+      return;
+    }
+    find(a);
+  }
+};
 
 template <int HDC>
-__global__ void __launch_bounds__(256) beam_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(Shape<HDC>::THREADS, HDC <= 64 ? 2 : 1) beam_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                              const Args a, int* __restrict__ status) {
   typedef Shape<HDC> C;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -194,17 +243,21 @@ __global__ void __launch_bounds__(256) beam_attention_kernel(const __grid_consta
     unit = begin - before - kvh * x.units;
   }
   // ---- the team's first warp asks for units, ahead across the ends of rows ----
-  Rows ahead_x = x;
-  int ahead_block = block, ahead_kvh = kvh, ahead_unit = unit, asked = begin, asked_stage = 0;
-  Unit next{0, 0, 0, -1};
-  if (member == 0) next = unit_of(a, ahead_x, ahead_unit);
-  auto issue = [&]() {                                     // by all lanes of the first warp
-    const bool there = next.page >= 0 && next.page < a.n_pages;     // (no page: no keys)
-    const int row = ((there ? next.page : 0) * a.nkv + ahead_kvh) * PAGE + next.half * KEYS;
+  Cursor u{};
+  int page = -1, asked = begin, asked_stage = 0;
+  if (member == 0) {
+    u.enter(a, block);
+    u.kvh = kvh, u.unit = unit;
+    u.find(a);
+    page = u.entry != nullptr ? *u.entry : -1;
+  }
+  auto issue = [&]() {
     if (lane == 0) {
-      about[asked_stage] = make_int2(there ? next.keys : 0, next.beam);
+      const bool there = page >= 0 && page < a.n_pages;     // (no page: no keys)
+      const int row = ((there ? page : 0) * a.nkv + u.kvh) * PAGE + u.at % PAGE;
+      about[asked_stage] = make_int2(there ? u.keys : 0, u.beam);
       const uint32_t full = bars + 16 * asked_stage, to = ring + asked_stage * C::STAGE;
-      jb::mbar_expect_tx(full, C::STAGE);                  // (behind the head's numbers the copy engine writes zeroes)
+      jb::mbar_expect_tx(full, C::STAGE);                   // (behind the head's numbers the copy engine writes zeroes)
 #pragma unroll
       for (int h = 0; h < C::SLABS; ++h) jb::tma_load_2d(to + h * C::SLAB, &map_k, full, h * 64, row);
 #pragma unroll
@@ -212,15 +265,9 @@ __global__ void __launch_bounds__(256) beam_attention_kernel(const __grid_consta
     }
     __syncwarp();
     if (++asked_stage == stages) asked_stage = 0;
-    if (++asked < end) {                                   // (a unit's page is looked up a turn before it is asked for)
-      if (++ahead_unit == ahead_x.units) {
-        ahead_unit = 0;
-        if (++ahead_kvh == a.nkv) {
-          ahead_kvh = 0;
-          ahead_x = look_up(a, ++ahead_block);
-        }
-      }
-      next = unit_of(a, ahead_x, ahead_unit);
+    if (++asked < end) {                                    // (a unit's page is looked up a turn before it is asked for)
+      u.step(a);
+      page = u.entry != nullptr ? *u.entry : -1;
     }
   };
   if (member == 0)
@@ -242,8 +289,8 @@ __global__ void __launch_bounds__(256) beam_attention_kernel(const __grid_consta
   uint32_t phase = 0, phase_before = 0;
   for (int i = begin; i < end; ++i) {
     if (i > begin && member == 0 && asked < end) {         // the stage of the turn before, when all warps are done with it
-      ok = jb::mbar_wait(bars + 16 * st_before + 8, phase_before, status, 54);
-      if (__any_sync(0xffffffffu, !ok)) break;
+      ok = __all_sync(0xffffffffu, mbar_wait(bars + 16 * st_before + 8, phase_before, status, 54));
+      if (!ok) break;
       issue();
     }
     if (i == begin || unit == 0) {
@@ -283,8 +330,8 @@ __global__ void __launch_bounds__(256) beam_attention_kernel(const __grid_consta
       all_join = __all_sync(0xffffffffu, every);           // (rows behind the last may do as they like)
       __syncwarp();
     }
-    ok = jb::mbar_wait(bars + 16 * st, phase, status, 53);
-    if (__any_sync(0xffffffffu, !ok)) break;
+    ok = __all_sync(0xffffffffu, mbar_wait(bars + 16 * st, phase, status, 53));
+    if (!ok) break;
     const int2 info = about[st];
     const int keys = info.x, beam = info.y;
     const uint32_t k_t = ring + st * C::STAGE, v_t = k_t + C::TILE;
@@ -297,9 +344,11 @@ __global__ void __launch_bounds__(256) beam_attention_kernel(const __grid_consta
         }
         __syncwarp();
       }
-      float s[4][4];
+      float s[4][4], s_odd[4][4];                          // (two chains of products, a half as long each)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][e] = s_odd[j][e] = 0.0f;
 #pragma unroll
       for (int ks = 0; ks < HDC / 16; ++ks) {
         uint32_t qa[4], b[2][4];
@@ -314,10 +363,14 @@ __global__ void __launch_bounds__(256) beam_attention_kernel(const __grid_consta
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          mma_bf16(s[2 * j], qa, b[j][0], b[j][1]);
-          mma_bf16(s[2 * j + 1], qa, b[j][2], b[j][3]);
+          mma_bf16(ks & 1 ? s_odd[2 * j] : s[2 * j], qa, b[j][0], b[j][1]);
+          mma_bf16(ks & 1 ? s_odd[2 * j + 1] : s[2 * j + 1], qa, b[j][2], b[j][3]);
         }
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][e] += s_odd[j][e];
       if (beam >= 0 || keys < KEYS || !all_join) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -329,17 +382,16 @@ __global__ void __launch_bounds__(256) beam_attention_kernel(const __grid_consta
       }
       float mx[2], use[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h)
         mx[h] = fmaxf(fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1])),
-                      fmaxf(fmaxf(s[2][2 * h], s[2][2 * h + 1]), fmaxf(s[3][2 * h], s[3][2 * h + 1])));
-        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * a.scale_log2;
-      }
-      // (also the first number of all)
+                      fmaxf(fmaxf(s[2][2 * h], s[2][2 * h + 1]), fmaxf(s[3][2 * h], s[3][2 * h + 1]))) * a.scale_log2;
+      // what weights are relative to is raised only when a score passes it by RESCALE_LOG2 (also the first number of all)
       if (__any_sync(0xffffffffu, mx[0] > m[0] + RESCALE_LOG2 || mx[1] > m[1] + RESCALE_LOG2)) {
         float corr[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
           const float top = fmaxf(m[h], mx[h]);
           corr[h] = top == -CUDART_INF_F ? 1.0f : fast_exp2(m[h] - top);
           m[h] = top;
@@ -409,9 +461,9 @@ __global__ void __launch_bounds__(256) beam_attention_kernel(const __grid_consta
       }
     }
   }
-  if (!ok && member == 0)                                  // gave up: what is still on its way arrives first (or its wait gives up as well)
-    for (int turn = max(0, asked - begin - stages); turn < asked - begin; ++turn)
-      jb::mbar_wait(bars + 16 * (turn % stages), (turn / stages) & 1, status, 53);
+  // gave up: what is still on its way arrives before the block ends (or its wait gives up as well)
+  if (!ok && member == 0)
+    for (int turn = max(0, asked - begin - stages); turn < asked - begin; ++turn) mbar_wait(bars + 16 * (turn % stages), (turn / stages) & 1, status, 53);
 }
 
 // A warp a (beam, head): the parts of its keys joined, where there are several.
@@ -473,7 +525,7 @@ JB_EXPORT int jb_attention_beams(const void* q, const void* k_cache, const void*
                                  int warps, int team, int fewest, float scale, int* status, cudaStream_t stream) {
   JB_REFUSE(R < 1 || K < 1 || K > MOST_BEAMS || nkv < 1 || nh < nkv || nh % nkv || hd < 8 || hd > 256 || hd % 8 || W < 1 || W > 0x7fffffff / PAGE ||
                 n_pages < 1 || (long long)n_pages * nkv * PAGE > 0x7fffffffLL || blocks < 1 || fewest < 1 || team < 1 || warps < team ||
-                warps % team || warps > (hd > 128 ? 4 : 8) || warps / team > (hd > 128 ? 3 : 6) || !(scale > 0.0f),
+                warps % team || warps > (hd > 128 ? Shape<256>::WARPS : Shape<128>::WARPS) || warps / team > (hd > 128 ? 3 : 6) || !(scale > 0.0f),
             "attention_beams: %d groups of %d beams, %d heads over %d of %d numbers, %d pages a row of %d, plan %d %d %d %d, scale %g", R, K, nh,
             nkv, hd, W, n_pages, blocks, warps, team, fewest, scale);
   CUtensorMap maps[2];
