@@ -5,11 +5,12 @@
 // The K best that are no stop token go on; a stop token among the K best of all ends its beam's text.  A beam's best continuation
 // stays in the beam's row, so that cache rows and states move only where a beam is lost; the others take the rows left, in order.
 //
-// Two launches.  The first reads every logit once, in registers: a thread's own running maximum and sum of exponentials, and the K
-// largest logits of a range of a row, which needs a look at single numbers only where one passes the K-th found so far.  The second,
-// a block a request, joins ranges and beams.  Within a beam the order is that of the logits (equal ones: the lowest token first),
-// which no rounding touches; between beams it is that of the totals, whose sum of exponentials is taken to 64 bits where
-// threads meet: 32 bits would turn two beams round now and then.
+// Two launches.  The first reads every logit once and keeps, in registers, each thread's largest one and its sum of exponentials: nothing
+// is compared with a list on the way.  Then the K-th largest of the threads' maxima bounds the K-th largest logit of the range from below, and
+// only the K threads' numbers at or above it are looked at again (from L2).  The second, a block a request, joins ranges and beams.
+// Within a beam the order is that of the logits (equal ones: the lowest token first), which no rounding touches; between beams it is
+// that of the totals, whose sum of exponentials is taken to 64 bits where threads meet: 32 bits would turn two beams round now and
+// then.
 #include <math_constants.h>
 #include <stdio.h>
 
@@ -21,12 +22,12 @@ typedef unsigned long long Key;      // a logit that sorts as a whole number, ab
 
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
-constexpr int VECTORS = 4;                                // of 16 bytes that a thread has of a piece of a row
+constexpr int VECTORS = 4;                                // of 16 bytes that a thread has on its way at a time
 constexpr int PER = 4 * VECTORS;
 constexpr int PIECE = THREADS * PER;
 constexpr int MOST_BEAMS = 32, MOST_STOPS = 32, MOST_RANGES = 32;
-constexpr int FEW = 64;                                   // threads with something new whose numbers are looked at without a bound
-constexpr int ROOM = FEW * PER + MOST_BEAMS;              // (the other way: at most MOST_BEAMS threads' numbers)
+constexpr int ROOM = THREADS * 4 + MOST_BEAMS;            // candidates at a time
+constexpr float FAR = 30.0f;                              // how far a number may lie above what a thread's sum is relative to
 
 __device__ __forceinline__ unsigned sortable(float x) {   // of numbers, -0 taken as 0
   const unsigned u = __float_as_uint(x + 0.0f);
@@ -37,14 +38,15 @@ __device__ __forceinline__ Key key_of(float x, int token) { return ((Key)sortabl
 __device__ __forceinline__ float logit_of(Key k) { return number((unsigned)(k >> 32)); }
 __device__ __forceinline__ int token_of(Key k) { return (int)~(unsigned)k; }
 
-// The keys of a warp, the largest in lane 0.
-__device__ __forceinline__ Key warp_sorted(Key k) {
+// The numbers of a warp, the largest in lane 0.
+template <typename T>
+__device__ __forceinline__ T warp_sorted(T k) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1) {
 #pragma unroll
     for (int o = size >> 1; o > 0; o >>= 1) {
-      const Key other = __shfl_xor_sync(0xffffffffu, k, o);
+      const T other = __shfl_xor_sync(0xffffffffu, k, o);
       const bool wants_more = ((lane & size) == 0) == ((lane & o) == 0);
       if ((other > k) == wants_more) k = other;
     }
@@ -53,8 +55,8 @@ __device__ __forceinline__ Key warp_sorted(Key k) {
 }
 
 struct Stat {
-  double sum;        // of exp(x - most); of entries at +inf, if that is the largest
-  float most;
+  double sum;        // of exp(x - ref); of entries at +inf, if that is the largest
+  float most;        // ref: near the largest number, +inf if that is it, -inf if there is none
   int unused;
 };
 
@@ -75,8 +77,8 @@ struct Args {
 
 __device__ __forceinline__ bool dead(float score) { return !(score > -CUDART_INF_F); }
 
-// exp(d) for d <= 0; the product with log2(e) in two parts, as its rounding would be the largest error of the sum
-__device__ __forceinline__ float exp_below(float d) {
+// exp(d) for d up to FAR; the product with log2(e) in two parts, as its rounding would be the largest error of the sum
+__device__ __forceinline__ float exp_near(float d) {
   constexpr float L = 1.44269504088896341f, L_LOW = 1.92596299112661746887e-8f, LN2 = 0.693147180559945309f;
   d = fmaxf(d, -200.0f);             // (also what is not a number, and -inf less -inf)
   const float hi = d * L;
@@ -87,10 +89,11 @@ __device__ __forceinline__ float exp_below(float d) {
 }
 
 __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
-  __shared__ Key found[ROOM];          // the best so far, then what a piece adds
-  __shared__ Key heads[WARPS * MOST_BEAMS];
-  __shared__ Key edge;
-  __shared__ int n_found;
+  __shared__ Key found[ROOM];          // the best so far, then what came
+  __shared__ float maxima[THREADS];
+  __shared__ int chosen[THREADS];      // threads whose numbers are looked at again
+  __shared__ float edge;
+  __shared__ int n_found, n_chosen;
   __shared__ int stops[MOST_STOPS];
   __shared__ float most_of[WARPS];
   __shared__ double sum_of[WARPS];
@@ -101,135 +104,124 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
   if (dead(a.scores[row])) return;                        // (the second launch asks for nothing of it)
   if (tid < a.S) stops[tid] = a.stops[tid];
   if (tid < K) found[tid] = 0;
+  if (tid == 0) edge = -CUDART_INF_F, n_found = K, n_chosen = 0;
   const float* x_row = a.logits + (size_t)row * a.V;
   const int lead = (int)(((uintptr_t)x_row >> 2) & 3);    // numbers in front of the row in its first 16 bytes
-  const int pieces = (a.V + lead + PIECE - 1) / PIECE;
-  const int first = (int)((long long)range * pieces / a.ranges), last = (int)((long long)(range + 1) * pieces / a.ranges);
-  float x[PER], next[PER];
-  auto load = [&](float (&to)[PER], int piece) {
-#pragma unroll
-    for (int i = 0; i < VECTORS; ++i) {
-      const int at = piece * PIECE + i * THREADS * 4 + tid * 4 - lead;
-      if (at >= 0 && at + 4 <= a.V) {
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(x_row + at));
-        to[4 * i] = v.x, to[4 * i + 1] = v.y, to[4 * i + 2] = v.z, to[4 * i + 3] = v.w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) to[4 * i + j] = at + j >= 0 && at + j < a.V ? __ldcs(x_row + at + j) : -CUDART_INF_F;
-      }
-    }
+  const int vectors = (a.V + lead + 3) / 4;               // of the row; vector i holds numbers 4 i - lead ..
+  const int first = (int)((long long)range * vectors / a.ranges), last = (int)((long long)(range + 1) * vectors / a.ranges);
+  auto load = [&](int i) {
+    const int at = 4 * i - lead;
+    if (at >= 0 && at + 4 <= a.V) return *reinterpret_cast<const float4*>(x_row + at);
+    float4 v = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+    if (at >= 0 && at < a.V) v.x = x_row[at];
+    if (at + 1 >= 0 && at + 1 < a.V) v.y = x_row[at + 1];
+    if (at + 2 >= 0 && at + 2 < a.V) v.z = x_row[at + 2];
+    if (at + 3 >= 0 && at + 3 < a.V) v.w = x_row[at + 3];
+    return v;
   };
-  float most = -CUDART_INF_F;
+  // ---- maximum and sum of the thread's numbers: vectors first + tid, + THREADS, ... ----
+  // The sum is relative to a number near the first ones' maximum, which is left where it is until one lies FAR above: what changes with
+  // every new maximum would cost a warp as much as the numbers themselves.
+  float top = -CUDART_INF_F, ref = -CUDART_INF_F;
   double sum = 0.0;
-  Key bound = 0;                       // the K-th best so far, 0 while there are fewer
-  if (first < last) load(x, first);
-  __syncthreads();
-  for (int piece = first; piece < last; ++piece) {
-    if (piece + 1 < last) load(next, piece + 1);
-    // ---- maximum and sum of the thread's numbers ----
-    float top = -CUDART_INF_F;
+  const float4 none = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+  for (int i0 = first + tid; i0 < last; i0 += THREADS * VECTORS) {
+    float x[PER];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) top = fmaxf(top, x[e]);
-    if (top > most) {
-      if (top == CUDART_INF_F) sum = 0.0;
-      else sum *= exp((double)most - (double)top);          // (0 of nothing: exp(-inf))
-      most = top;
+    for (int u = 0; u < VECTORS; ++u) {
+      const float4 v = i0 + u * THREADS < last ? load(i0 + u * THREADS) : none;
+      x[4 * u] = v.x, x[4 * u + 1] = v.y, x[4 * u + 2] = v.z, x[4 * u + 3] = v.w;
     }
-    if (most == CUDART_INF_F) {
+    float high = -CUDART_INF_F;                           // (a number that is none is never the larger)
+#pragma unroll
+    for (int e = 0; e < PER; ++e) high = fmaxf(high, x[e]);
+    top = fmaxf(top, high);
+    if (high > ref + FAR) {
+      sum = high == CUDART_INF_F ? 0.0 : sum * exp((double)ref - (double)high);
+      ref = high;
+    }
+    if (ref == CUDART_INF_F) {
 #pragma unroll
       for (int e = 0; e < PER; ++e) sum += x[e] == CUDART_INF_F ? 1.0 : 0.0;
     } else {
       float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int e = 0; e < PER; ++e) s[e & 3] += exp_below(x[e] - most);
+      for (int e = 0; e < PER; ++e) s[e & 3] += exp_near(x[e] - ref);
       sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
     }
-    // ---- stop tokens are no candidates here ----
-    for (int s = 0; s < a.S; ++s) {
-      const int at = stops[s] + lead - piece * PIECE;
-      if (at >= 0 && at < PIECE && stops[s] >= 0 && stops[s] < a.V && ((at >> 2) & (THREADS - 1)) == tid) {
-        const int mine = (at / (THREADS * 4)) * 4 + (at & 3);
-#pragma unroll
-        for (int e = 0; e < PER; ++e)
-          if (e == mine) x[e] = -CUDART_INF_F;
-      }
-    }
-    // ---- the thread's best ----
-    float best = -CUDART_INF_F;
-    int best_at = 0;
-#pragma unroll
-    for (int e = 0; e < PER; ++e)
-      if (x[e] > best) best = x[e], best_at = e;
-    const int origin = piece * PIECE + tid * 4 - lead;
-    auto token = [&](int e) { return origin + (e >> 2) * THREADS * 4 + (e & 3); };
-    const Key mine = best > -CUDART_INF_F ? key_of(best, token(best_at)) : 0;
-    const int new_threads = __syncthreads_count(mine > bound);
-    if (new_threads > 0) {
-      Key least = bound;               // what is looked at lies above
-      if (tid == 0) n_found = K, edge = 0;
-      if (new_threads > FEW) {
-        // the K-th largest of the threads' best: no more than K threads have anything at or above it
-        const Key sorted = warp_sorted(mine);
-        if (lane < K) heads[warp * K + lane] = sorted;
-        __syncthreads();
-        if (tid < WARPS * K) {
-          const Key h = heads[tid];
-          int above = 0;
-          for (int i = 0; i < WARPS * K; ++i) above += heads[i] > h;
-          if (above == K - 1 && h > 0) edge = h;
-        }
-        __syncthreads();
-        if (edge > 0 && edge - 1 > least) least = edge - 1;
-      } else {
-        __syncthreads();
-      }
-      if (mine > least) {
-#pragma unroll
-        for (int e = 0; e < PER; ++e) {
-          if (x[e] > -CUDART_INF_F) {
-            const Key k = key_of(x[e], token(e));
-            if (k > least) found[atomicAdd(&n_found, 1)] = k;
-          }
-        }
-      }
-      __syncthreads();
-      // the K best of what was there and what came, in order: a key's place is the number of larger ones
-      const int n = n_found;
-      Key k[(ROOM + THREADS - 1) / THREADS];
-      int place[(ROOM + THREADS - 1) / THREADS];
-#pragma unroll
-      for (int u = 0; u < (ROOM + THREADS - 1) / THREADS; ++u) {
-        const int i = tid + u * THREADS;
-        place[u] = K;
-        if (i < n) {
-          k[u] = found[i];
-          int above = 0;
-          for (int j = 0; j < n; ++j) above += found[j] > k[u];
-          if (k[u] > 0) place[u] = above;
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int u = 0; u < (ROOM + THREADS - 1) / THREADS; ++u)
-        if (place[u] < K) found[place[u]] = k[u];
-      __syncthreads();
-      bound = found[K - 1];
-    }
-#pragma unroll
-    for (int e = 0; e < PER; ++e) x[e] = next[e];
   }
-  // ---- the range's maximum and sum ----
-  const float warp_most = jb::warp_max(most);
+  // ---- the range's sum, relative to the largest reference ----
+  const float warp_most = jb::warp_max(ref);
   if (lane == 0) most_of[warp] = warp_most;
   __syncthreads();
   float all = most_of[0];
 #pragma unroll
   for (int w = 1; w < WARPS; ++w) all = fmaxf(all, most_of[w]);
-  if (all == CUDART_INF_F) sum = most == all ? sum : 0.0;
-  else if (most < all) sum *= exp((double)most - (double)all);
+  if (all == CUDART_INF_F) sum = ref == all ? sum : 0.0;
+  else if (ref < all) sum *= exp((double)ref - (double)all);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) sum_of[warp] = sum;
+  // ---- the threads whose numbers may be among the K largest that are no stop token: a stop token is at most one thread's maximum ----
+  const int wanted = K + a.S, heads = min(wanted, 32);
+  const float sorted = warp_sorted(top);
+  if (lane < heads) maxima[warp * heads + lane] = sorted;
+  __syncthreads();
+  if (tid < WARPS * heads && maxima[tid] > -CUDART_INF_F) {
+    const float mine = maxima[tid];
+    int above = 0, level = 0;                             // larger ones, equal ones
+#pragma unroll 4
+    for (int i = 0; i < WARPS * heads; ++i) above += maxima[i] > mine, level += maxima[i] == mine;
+    if (above < wanted && above + level >= wanted) edge = mine;   // (all who are level write the same)
+  }
+  __syncthreads();
+  const float least = edge;                               // -inf: fewer threads than that have a number
+  if (top > -CUDART_INF_F && top >= least) chosen[atomicAdd(&n_chosen, 1)] = tid;
+  __syncthreads();
+  // ---- their numbers at or above it, in rounds of a vector a thread (one or two rounds, unless many maxima are equal) ----
+  const int each = (last - first + THREADS - 1) / THREADS, n = n_chosen * each;
+  Key bound = 0;                       // the K-th best so far, 0 while there are fewer
+  for (int j0 = 0; j0 < n; j0 += THREADS) {
+    const int j = j0 + tid, i = j < n ? first + chosen[j / each] + j % each * THREADS : last;
+    if (i < last) {
+      const float4 v = load(i);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (x[e] >= least && x[e] > -CUDART_INF_F) {
+          const int token = 4 * i - lead + e;
+          const Key k = key_of(x[e], token);
+          bool stop = false;
+          for (int s = 0; s < a.S; ++s) stop |= stops[s] == token;
+          if (k > bound && !stop) found[atomicAdd(&n_found, 1)] = k;
+        }
+      }
+    }
+    // (rounds whose numbers still have room beside the next one's are put in order later)
+    const bool full = __syncthreads_or(n_found > ROOM - 4 * THREADS) != 0;
+    if (!full && j0 + THREADS < n) continue;
+    // the K best of what was there and what came, in order: a key's place is the number of larger ones
+    const int m = n_found;
+    Key k[(ROOM + THREADS - 1) / THREADS];
+    int place[(ROOM + THREADS - 1) / THREADS];
+#pragma unroll
+    for (int u = 0; u < (ROOM + THREADS - 1) / THREADS; ++u) {
+      place[u] = K;
+      if (tid + u * THREADS < m) {
+        k[u] = found[tid + u * THREADS];
+        int above = 0;
+        for (int q = 0; q < m; ++q) above += found[q] > k[u];
+        if (k[u] > 0) place[u] = above;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < (ROOM + THREADS - 1) / THREADS; ++u)
+      if (place[u] < K) found[place[u]] = k[u];
+    if (tid == 0) n_found = K;
+    __syncthreads();
+    bound = found[K - 1];
+  }
   __syncthreads();
   const size_t list = (size_t)row * a.ranges + range;
   if (tid == 0) {
