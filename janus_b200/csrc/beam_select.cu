@@ -27,7 +27,8 @@ constexpr int PER = 4 * VECTORS;
 constexpr int PIECE = THREADS * PER;
 constexpr int MOST_BEAMS = 32, MOST_STOPS = 32, MOST_RANGES = 32;
 constexpr int ROOM = THREADS * 4 + MOST_BEAMS;            // candidates at a time
-constexpr float FAR = 30.0f;                              // how far a number may lie above what a thread's sum is relative to
+constexpr float FAR = 40.0f;                              // how far a power may lie above what a thread's sum is relative to
+constexpr float WIDE = 1e8f;                              // powers beyond are made by 64-bit arithmetic
 
 __device__ __forceinline__ unsigned sortable(float x) {   // of numbers, -0 taken as 0
   const unsigned u = __float_as_uint(x + 0.0f);
@@ -55,9 +56,9 @@ __device__ __forceinline__ T warp_sorted(T k) {
 }
 
 struct Stat {
-  double sum;        // of exp(x - ref); of entries at +inf, if that is the largest
-  float most;        // ref: near the largest number, +inf if that is it, -inf if there is none
-  int unused;
+  double sum;        // of exp(x) / 2^scale; of entries at +inf, if there are any
+  double scale;
+  double top;        // the largest number; -inf if there is none
 };
 
 struct Args {
@@ -77,15 +78,32 @@ struct Args {
 
 __device__ __forceinline__ bool dead(float score) { return !(score > -CUDART_INF_F); }
 
-// exp(d) for d up to FAR; the product with log2(e) in two parts, as its rounding would be the largest error of the sum
-__device__ __forceinline__ float exp_near(float d) {
-  constexpr float L = 1.44269504088896341f, L_LOW = 1.92596299112661746887e-8f, LN2 = 0.693147180559945309f;
-  d = fmaxf(d, -200.0f);             // (also what is not a number, and -inf less -inf)
-  const float hi = d * L;
-  const float lo = fmaf(d, L_LOW, fmaf(d, L, -hi));
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
-  return fmaf(e, lo * LN2, e);
+// exp(x) / 2^scale = 2^(x log2(e) - scale), two numbers at a time; log2(e) in two parts, the small one last, where the difference is small.
+__device__ __forceinline__ jb::Pair powers(jb::Pair x, jb::Pair minus_scale) {
+  constexpr float L = 1.44269504088896341f, L_LOW = 1.92596299112661746887e-8f;
+  const jb::Pair p = jb::fma2(x, jb::pair(L_LOW, L_LOW), jb::fma2(x, jb::pair(L, L), minus_scale));
+  float lo, hi;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(lo) : "f"(jb::lo(p)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(hi) : "f"(jb::hi(p)));
+  return jb::pair(lo, hi);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+constexpr double LOG2E = 1.4426950408889634074;
+// exp(x) as a power of two, rounded, so that the same numbers' powers are equal (a fused multiply-add would find their rounding)
+__device__ __forceinline__ double power_of(double x) { return __dmul_rn(x, LOG2E); }
+// A part's sum relative to exp(top), the largest number of all.
+__device__ __forceinline__ double relative(const Stat& s, double top) {
+  if (top == CUDART_INF) return s.top == top ? s.sum : 0.0;
+  return s.top > -CUDART_INF ? s.sum * exp2(s.scale - power_of(top)) : 0.0;
+}
+__device__ __forceinline__ double warp_max(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
 
 __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
@@ -95,8 +113,7 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
   __shared__ float edge;
   __shared__ int n_found, n_chosen;
   __shared__ int stops[MOST_STOPS];
-  __shared__ float most_of[WARPS];
-  __shared__ double sum_of[WARPS];
+  __shared__ double top_of[WARPS], sum_of[WARPS];
   jb::pdl_launch_dependents();
   const int row = blockIdx.x / a.ranges, range = blockIdx.x % a.ranges;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.K;
@@ -120,45 +137,67 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
     return v;
   };
   // ---- maximum and sum of the thread's numbers: vectors first + tid, + THREADS, ... ----
-  // The sum is relative to a number near the first ones' maximum, which is left where it is until one lies FAR above: what changes with
-  // every new maximum would cost a warp as much as the numbers themselves.
-  float top = -CUDART_INF_F, ref = -CUDART_INF_F;
+  // The sum is relative to a power of two near the first numbers' maximum, which is left where it is until one lies FAR above: what changes
+  // with every new maximum would cost a warp as much as the numbers themselves.  Powers beyond WIDE below that are 0; where they are
+  // all there is, where one lies beyond WIDE above, and where something is no number, the thread goes over its numbers once more.
+  float top = -CUDART_INF_F, scale = -CUDART_INF_F;
+  bool wide = false;
   double sum = 0.0;
   const float4 none = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
-  for (int i0 = first + tid; i0 < last; i0 += THREADS * VECTORS) {
-    float x[PER];
+  auto take = [&](const float4 (&v)[VECTORS]) {
+    float high = -CUDART_INF_F;                           // (what is no number is never the larger)
+#pragma unroll
+    for (int u = 0; u < VECTORS; ++u) high = max3(max3(high, v[u].x, v[u].y), v[u].z, v[u].w);
+    top = fmaxf(top, high);
+    const float power = high * (float)LOG2E;
+    if (!(power >= -WIDE)) return;
+    if (power > scale + FAR) {
+      wide |= !(power <= WIDE);
+      const float next = rintf(fminf(power, WIDE));
+      sum *= exp2((double)scale - (double)next);          // (0 of nothing)
+      scale = next;
+    }
+    jb::Pair s = jb::pair(0.0f, 0.0f), t = s;
+    const jb::Pair minus = jb::pair(-scale, -scale), one = jb::pair(1.0f, 1.0f);
 #pragma unroll
     for (int u = 0; u < VECTORS; ++u) {
-      const float4 v = i0 + u * THREADS < last ? load(i0 + u * THREADS) : none;
-      x[4 * u] = v.x, x[4 * u + 1] = v.y, x[4 * u + 2] = v.z, x[4 * u + 3] = v.w;
+      s = jb::fma2(powers(jb::pair(v[u].x, v[u].y), minus), one, s);
+      t = jb::fma2(powers(jb::pair(v[u].z, v[u].w), minus), one, t);
     }
-    float high = -CUDART_INF_F;                           // (a number that is none is never the larger)
+    sum += (double)((jb::lo(s) + jb::hi(s)) + (jb::lo(t) + jb::hi(t)));
+  };
+  const int whole0 = lead > 0 ? 1 : 0, whole1 = (a.V + lead) / 4;      // vectors that lie inside the row
+  for (int i0 = first + tid; i0 < last; i0 += THREADS * VECTORS) {
+    float4 v[VECTORS];
+    if (i0 >= whole0 && i0 + (VECTORS - 1) * THREADS < min(last, whole1)) {
+      const float4* at = reinterpret_cast<const float4*>(x_row - lead) + i0;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) high = fmaxf(high, x[e]);
-    top = fmaxf(top, high);
-    if (high > ref + FAR) {
-      sum = high == CUDART_INF_F ? 0.0 : sum * exp((double)ref - (double)high);
-      ref = high;
-    }
-    if (ref == CUDART_INF_F) {
-#pragma unroll
-      for (int e = 0; e < PER; ++e) sum += x[e] == CUDART_INF_F ? 1.0 : 0.0;
+      for (int u = 0; u < VECTORS; ++u) v[u] = at[u * THREADS];
     } else {
-      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int e = 0; e < PER; ++e) s[e & 3] += exp_near(x[e] - ref);
-      sum += (double)((s[0] + s[1]) + (s[2] + s[3]));
+      for (int u = 0; u < VECTORS; ++u) v[u] = i0 + u * THREADS < last ? load(i0 + u * THREADS) : none;
+    }
+    take(v);
+  }
+  Stat mine{sum, (double)scale, (double)top};
+  if (wide || sum != sum || (scale == -CUDART_INF_F && top > -CUDART_INF_F)) {
+    mine.sum = 0.0, mine.scale = power_of(mine.top);
+    for (int i = first + tid; i < last; i += THREADS) {
+      const float4 v = load(i);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (x[e] > -CUDART_INF_F) mine.sum += top == CUDART_INF_F ? (x[e] == top ? 1.0 : 0.0) : exp((double)x[e] - mine.top);
     }
   }
-  // ---- the range's sum, relative to the largest reference ----
-  const float warp_most = jb::warp_max(ref);
-  if (lane == 0) most_of[warp] = warp_most;
+  // ---- the range's sum, relative to its largest number ----
+  const double warp_top = warp_max(mine.top);
+  if (lane == 0) top_of[warp] = warp_top;
   __syncthreads();
-  float all = most_of[0];
+  double all = top_of[0];
 #pragma unroll
-  for (int w = 1; w < WARPS; ++w) all = fmaxf(all, most_of[w]);
-  if (all == CUDART_INF_F) sum = ref == all ? sum : 0.0;
-  else if (ref < all) sum *= exp((double)ref - (double)all);
+  for (int w = 1; w < WARPS; ++w) all = fmax(all, top_of[w]);
+  sum = relative(mine, all);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) sum_of[warp] = sum;
@@ -228,7 +267,7 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
     double s = 0.0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) s += sum_of[w];
-    a.stats[list] = Stat{s, all, 0};
+    a.stats[list] = Stat{s, power_of(all), all};
   }
   if (tid < K) a.keys[list * K + tid] = found[tid];
 }
@@ -236,12 +275,17 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
 // Whether continuation (x, i) comes in front of (y, j): by total, then by beam and token.
 __device__ __forceinline__ bool in_front(double x, long long i, double y, long long j) { return x > y || (x == y && i < j); }
 
+// A logit's distance from its row's largest; beside entries at +inf, 0 for those and -inf for others.
+__device__ __forceinline__ double worth(float x, double top) {
+  return top == CUDART_INF ? (x == CUDART_INF_F ? 0.0 : -CUDART_INF) : (double)x - top;
+}
+
 // One block a request.  Dynamic memory: WARPS * K * K keys, then for K * K continuations (total, place), their shortened list, and
 // for K * S stop tokens the same.
 __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t memory[];
-  __shared__ double base[MOST_BEAMS];      // score - log sum exp, of a live beam
-  __shared__ float most_of[MOST_BEAMS];
+  __shared__ double base[MOST_BEAMS];      // score - log sum exp(x - top), of a live beam
+  __shared__ double top_of[MOST_BEAMS];    // its largest logit
   __shared__ double kth[MOST_BEAMS], head[MOST_BEAMS];
   __shared__ double on[MOST_BEAMS];
   __shared__ long long on_at[MOST_BEAMS];
@@ -269,18 +313,18 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Args a) {
     const int row = r * K + b;
     const float score = a.scores[row];
     for (int j = lane; j < K; j += 32) totals[b * K + j] = -CUDART_INF, token[b * K + j] = 0;
-    if (lane == 0) base[b] = -CUDART_INF, most_of[b] = -CUDART_INF_F;
+    if (lane == 0) base[b] = top_of[b] = -CUDART_INF;
     if (!dead(score)) {
       const Key* keys = a.keys + (size_t)row * a.ranges * K;
       Key edge = lane < a.ranges ? keys[lane * K] : 0;
-      Stat s{0.0, -CUDART_INF_F, 0};
+      Stat s{0.0, -CUDART_INF, -CUDART_INF};
       if (lane < a.ranges) s = a.stats[(size_t)row * a.ranges + lane];
-      const float most = jb::warp_max(s.most);
-      double sum = most == CUDART_INF_F ? (s.most == most ? s.sum : 0.0) : s.most > -CUDART_INF_F ? s.sum * exp((double)s.most - (double)most) : 0.0;
+      const double top = warp_max(s.top);
+      double sum = relative(s, top);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const double less = log(sum);                       // (a number wherever the row has one above -inf)
-      if (lane == 0) base[b] = (double)score - less, most_of[b] = most;
+      const double start = (double)score - log(sum);      // (a number wherever the row has one above -inf)
+      if (lane == 0) base[b] = start, top_of[b] = top;
       edge = __shfl_sync(0xffffffffu, warp_sorted(edge), K - 1);          // no more than K ranges have anything at or above it
       int n = 0;
       for (int i0 = 0; i0 < a.ranges * K; i0 += 32) {
@@ -296,9 +340,7 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Args a) {
         int above = 0;
         for (int j = 0; j < n; ++j) above += mine[j] > k;
         if (above < K) {
-          const float x = logit_of(k);
-          const double z = most == CUDART_INF_F ? (x == most ? 0.0 : -CUDART_INF) : (double)x - (double)most;
-          totals[b * K + above] = (double)score - less + z;
+          totals[b * K + above] = start + worth(logit_of(k), top);
           token[b * K + above] = token_of(k);
         }
       }
@@ -334,9 +376,9 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Args a) {
     bool again = false;
     for (int s = 0; s < i % a.S; ++s) again |= a.stops[s] == stop;
     if (stop < 0 || stop >= a.V || again || !(base[b] > -CUDART_INF)) continue;
-    const float x = a.logits[((size_t)r * K + b) * a.V + stop], most = most_of[b];
+    const float x = a.logits[((size_t)r * K + b) * a.V + stop];
     if (!(x > -CUDART_INF_F)) continue;
-    const double t = base[b] + (most == CUDART_INF_F ? (x == most ? 0.0 : -CUDART_INF) : (double)x - (double)most);
+    const double t = base[b] + worth(x, top_of[b]);
     if (!(t > -CUDART_INF) || !in_front(t, b * V + stop, on[K - 1], on[K - 1] > -CUDART_INF ? on_at[K - 1] : K * V)) continue;
     const int at = atomicAdd(&n_stop, 1);
     stop_total[at] = t;
@@ -381,7 +423,7 @@ size_t join_memory(int K, int S) { return (size_t)WARPS * K * K * 8 + (size_t)K 
 
 }  // namespace
 
-// Scratch: keys R * K * ranges * K of 8 bytes, stats R * K * ranges of 16.
+// Scratch: keys R * K * ranges * K of 8 bytes, stats R * K * ranges of 24.
 JB_EXPORT int jb_beam_select(const float* logits, const float* scores, const int* stops, int* parents, int* tokens, float* next_scores,
                              int* ended_parents, int* ended_tokens, float* ended_scores, void* keys, void* stats, int R, int K, int V,
                              int S, int ranges, cudaStream_t stream) {

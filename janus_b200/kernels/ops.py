@@ -2707,7 +2707,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, stop_tokens: torch.T
         _on_current_device("beam_select", (logits, scores, stop_tokens, parents, tokens, next_scores, ended_parents, ended_tokens, ended_scores))
     ranges = beam_ranges(rows, V)
     keys = workspace.get("beam_keys", (rows * ranges * K,), torch.int64)
-    stats = workspace.get("beam_stats", (rows * ranges * 2,), torch.float64)
+    stats = workspace.get("beam_stats", (rows * ranges * 3,), torch.float64)
     _check(_lib("beam_select").jb_beam_select(
         logits.data_ptr(), scores.data_ptr(), stop_tokens.data_ptr(), parents.data_ptr(), tokens.data_ptr(), next_scores.data_ptr(),
         ended_parents.data_ptr(), ended_tokens.data_ptr(), ended_scores.data_ptr(), keys.data_ptr(), stats.data_ptr(), R, K, V,
