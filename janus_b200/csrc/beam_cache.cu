@@ -24,9 +24,7 @@ constexpr int MOST_BEAMS = 32;
 // atomics meet in any order: only a count's last change can be to 0), then who holds a partly filled page alone, and which
 // places of the free list they take otherwise.  Pages that come back are marked in a bitmap of the cluster's first block and numbered
 // from it, so that lists are the same whatever the launch looks like.
-constexpr int FORK_THREADS = 512;
 constexpr int FORK_BLOCKS = 8;
-constexpr int FORK_WARPS = FORK_THREADS / 32;
 
 struct Fork {
   const int* parents;
@@ -50,7 +48,8 @@ struct Fork {
   int R, K, W, P, F, spare, page_size;
 };
 
-// The sum over the block's threads up to this one, and over all of them in `all`.  scratch: FORK_WARPS ints.
+// The sum over the block's threads up to this one, and over all of them in `all`.  scratch: an int a warp.
+template <int WARPS>
 __device__ __forceinline__ int block_scan(int v, int& all, int* scratch) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -61,18 +60,14 @@ __device__ __forceinline__ int block_scan(int v, int& all, int* scratch) {
   __syncthreads();
   if (lane == 31) scratch[warp] = v;
   __syncthreads();
-  int before = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < FORK_WARPS; ++w) {
-    if (w < warp) before += scratch[w];
-    all += scratch[w];
-  }
-  return before + v;
+  int sums = lane < WARPS ? scratch[lane] : 0;            // (every warp adds them up for itself)
+  all = __reduce_add_sync(0xffffffffu, sums);
+  return __reduce_add_sync(0xffffffffu, lane < warp ? sums : 0) + v;
 }
 
-template <int KM>
+template <int KM, int FORK_THREADS>
 __global__ void __cluster_dims__(FORK_BLOCKS, 1, 1) __launch_bounds__(FORK_THREADS) fork_pages_kernel(const Fork a) {
+  constexpr int FORK_WARPS = FORK_THREADS / 32;
   extern __shared__ unsigned smem[];
   __shared__ int scratch[FORK_WARPS];
   __shared__ int held_of[FORK_THREADS];
@@ -81,92 +76,99 @@ __global__ void __cluster_dims__(FORK_BLOCKS, 1, 1) __launch_bounds__(FORK_THREA
   unsigned* bits = smem;                                 // pages that come back (of the first block)
   int* ranks = reinterpret_cast<int*>(smem + words);     // ... in front of each word
   unsigned* bits0 = cluster.map_shared_rank(bits, 0);
-  const int tid = threadIdx.x, K = a.K, W = a.W, p = a.page_size;
+  const int tid = threadIdx.x, lane = tid & 31, K = a.K, W = a.W, p = a.page_size;
   const int thread = cluster.block_rank() * FORK_THREADS + tid;
   constexpr int ALL = FORK_BLOCKS * FORK_THREADS;
+  for (int i = tid; i < words; i += FORK_THREADS) bits[i] = 0u;
   jb::pdl_launch_dependents();
   jb::pdl_wait();
   auto pages_of = [&](int tokens) { return tokens > 0 ? (tokens - 1) / p + 1 : 0; };
   auto counted = [&](int page) { return page >= 0 && page < a.P && page != a.spare; };
+  // ---- what later parts count from ----
+  const int n0 = min(max(*a.n_free, 0), a.F);
+  if (a.new_refs != a.refs)
+    for (int i = thread; i < a.P; i += ALL) a.new_refs[i] = a.refs[i];
+  if (a.new_free != a.free_pages)
+    for (int i = thread; i < a.F; i += ALL) a.new_free[i] = i < n0 ? a.free_pages[i] : -1;
+  for (int r = thread; r < a.R; r += ALL) a.shared[r] = W;
+  // ---- rows of the new table, but for the page that takes the next token, and the pages' counts ----
+  // A warp has 32 columns of a group; lane k knows row k: which it goes on with, and how many pages the two hold.
+  const int tiles = (W + 31) / 32;
+  bool counts_ready = false;
+  for (long long tile = thread >> 5;; tile += ALL / 32) {
+    const bool there = tile < (long long)a.R * tiles;
+    const int r = there ? (int)(tile / tiles) : 0, c = there ? (int)(tile % tiles) * 32 + lane : W, row0 = r * K;
+    const int parent = lane < K ? a.parents[row0 + lane] : -1, length = lane < K ? max(a.lengths[row0 + lane], 0) : 0;
+    const int src = parent >= 0 && parent < K ? parent : -1;
+    const int length_now = __shfl_sync(0xffffffffu, length, max(src, 0));
+    const int pages_now = src >= 0 ? pages_of(length_now) : 0, pages_was = pages_of(length);
+    int was[KM], now[KM];
+#pragma unroll
+    for (int k = 0; k < KM; ++k) was[k] = k < K && c < W ? a.table[(size_t)(row0 + k) * W + c] : -1;
+#pragma unroll
+    for (int k = 0; k < KM; ++k) {
+      const int from = __shfl_sync(0xffffffffu, src, k), pages = __shfl_sync(0xffffffffu, pages_now, k);
+      now[k] = from < 0 && c == 0 && k < K ? a.spare : -1;
+      if (from >= 0 && c < pages && c < W) now[k] = a.table[(size_t)(row0 + from) * W + c];   // (the lines are on their way already)
+    }
+    const unsigned goes_on = __ballot_sync(0xffffffffu, src >= 0);
+    // the first column in which the rows that go on differ, and no more than the whole pages of the shortest
+    bool differs = false;
+    int head = 0;
+    bool seen = false;
+#pragma unroll
+    for (int k = 0; k < KM; ++k) {
+      if ((goes_on >> k) & 1u) {
+        if (!seen) head = now[k], seen = true;
+        else differs = differs || now[k] != head;
+      }
+    }
+    const unsigned where = __ballot_sync(0xffffffffu, differs && c < W);
+    const int lead = __reduce_min_sync(0xffffffffu, src >= 0 ? length_now / p : W);
+    if (!counts_ready) {
+      cluster.sync();                                    // (the first tile's numbers are on their way meanwhile)
+      counts_ready = true;
+    }
+    if (!there) break;
+    if (lane == 0) {
+      const int first = min(where ? c + __ffs(where) - 1 : W, goes_on ? lead : 0);
+      if (first < W) atomicMin(&a.shared[r], first);
+    }
+    bool changes = false;
+#pragma unroll
+    for (int k = 0; k < KM; ++k) {
+      const int held = c < __shfl_sync(0xffffffffu, pages_was, k) ? was[k] : -1;
+      changes = changes || now[k] != held;
+    }
+    if (__any_sync(0xffffffffu, changes)) {
+#pragma unroll
+      for (int k = 0; k < KM; ++k) {
+        const int held = c < __shfl_sync(0xffffffffu, pages_was, k) ? was[k] : -1;
+        if (now[k] != held && counted(now[k])) atomicAdd(&a.new_refs[now[k]], 1);
+      }
+#pragma unroll
+      for (int k = 0; k < KM; ++k) {
+        const int held = c < __shfl_sync(0xffffffffu, pages_was, k) ? was[k] : -1;
+        if (now[k] != held && counted(held) && atomicSub(&a.new_refs[held], 1) == 1) atomicOr(&bits0[held >> 5], 1u << (held & 31));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < KM; ++k)
+      if (k < K && c < W && (a.new_table != a.table || now[k] != was[k])) a.new_table[(size_t)(row0 + k) * W + c] = now[k];
+  }
+  cluster.sync();
+  if (cluster.block_rank() != 0) return;
   auto source = [&](int row) {                           // the row that a row goes on with, or -1
     const int b = a.parents[row];
     return b >= 0 && b < K ? row / K * K + b : -1;
   };
   auto length_of = [&](int row) { return max(a.lengths[row], 0); };
-  // ---- what later parts count from ----
-  const int n0 = min(max(*a.n_free, 0), a.F);
-  for (int i = tid; i < words; i += FORK_THREADS) bits[i] = 0u;
-  if (a.new_refs != a.refs)
-    for (int i = thread; i < a.P; i += ALL) a.new_refs[i] = a.refs[i];
-  if (a.new_free != a.free_pages)
-    for (int i = thread; i < a.F; i += ALL) a.new_free[i] = i < n0 ? a.free_pages[i] : -1;
-  for (int r = thread; r < a.R; r += ALL) {
-    int lead = W;
-    bool any = false;
-    for (int k = 0; k < K; ++k) {
-      const int s = source(r * K + k);
-      if (s >= 0) lead = min(lead, length_of(s) / p), any = true;
-    }
-    a.shared[r] = any ? lead : 0;
-  }
-  cluster.sync();
-  // ---- rows of the new table, but for the page that takes the next token, and the pages' counts ----
-  for (long long item = thread; item < (long long)a.R * W; item += ALL) {
-    const int r = (int)(item / W), c = (int)(item % W), row0 = r * K;
-    int was[KM], held[KM], now[KM];
-    int head = -1, differs = 0;
-    bool changes = false;
-#pragma unroll
-    for (int k = 0; k < KM; ++k) {
-      was[k] = held[k] = now[k] = -1;
-      if (k < K) {
-        const int s = source(row0 + k);
-        was[k] = a.table[(size_t)(row0 + k) * W + c];
-        held[k] = c < pages_of(length_of(row0 + k)) ? was[k] : -1;
-        if (s >= 0) {
-          if (c < pages_of(length_of(s))) now[k] = a.table[(size_t)s * W + c];
-          if (head < 0) head = k;
-          else differs |= now[k] ^ now[0] ? 1 : 0;
-        } else if (c == 0) {
-          now[k] = a.spare;
-        }
-        changes |= now[k] != held[k];
-      }
-    }
-    if (head > 0) {                                      // (the first row does not go on: compare with the first that does)
-      differs = 0;
-      int first = -1;
-      bool seen = false;
-#pragma unroll
-      for (int k = 0; k < KM; ++k) {
-        if (k < K && source(row0 + k) >= 0) {
-          if (!seen) first = now[k], seen = true;
-          else differs |= now[k] != first;
-        }
-      }
-    }
-    if (differs) atomicMin(&a.shared[r], c);
-    if (changes) {
-#pragma unroll
-      for (int k = 0; k < KM; ++k)
-        if (k < K && now[k] != held[k] && counted(now[k])) atomicAdd(&a.new_refs[now[k]], 1);
-#pragma unroll
-      for (int k = 0; k < KM; ++k)
-        if (k < K && now[k] != held[k] && counted(held[k]) && atomicSub(&a.new_refs[held[k]], 1) == 1)
-          atomicOr(&bits0[held[k] >> 5], 1u << (held[k] & 31));
-    }
-#pragma unroll
-    for (int k = 0; k < KM; ++k)
-      if (k < K && (a.new_table != a.table || now[k] != was[k])) a.new_table[(size_t)(row0 + k) * W + c] = now[k];
-  }
-  cluster.sync();
-  if (cluster.block_rank() != 0) return;
   // ---- pages that came back, numbered ----
   int freed = 0;
   for (int i0 = 0; i0 < words; i0 += FORK_THREADS) {
     const int i = i0 + tid, n = i < words ? __popc(bits[i]) : 0;
     int all;
-    const int upto = block_scan(n, all, scratch);
+    const int upto = block_scan<FORK_WARPS>(n, all, scratch);
     if (i < words) ranks[i] = freed + upto - n;
     freed += all;
   }
@@ -210,7 +212,7 @@ __global__ void __cluster_dims__(FORK_BLOCKS, 1, 1) __launch_bounds__(FORK_THREA
     }
     const bool needs = s >= 0 && fits && !keeps;
     int all;
-    const int upto = block_scan(needs, all, scratch);    // (every count above is read before one changes below)
+    const int upto = block_scan<FORK_WARPS>(needs, all, scratch);    // (every count above is read before one changes below)
     const int i = total - taken - upto;
     taken += all;
     if (mine) {
@@ -236,7 +238,7 @@ __global__ void __cluster_dims__(FORK_BLOCKS, 1, 1) __launch_bounds__(FORK_THREA
   const int left = max(0, total - taken), listed = min(left, a.F);
   for (int i = min(n0, listed) + tid; i < max(n0, listed); i += FORK_THREADS) a.new_free[i] = i < listed ? back(i - n0) : -1;
   int all;
-  block_scan(lacking, all, scratch);
+  block_scan<FORK_WARPS>(lacking, all, scratch);
   if (tid == 0) {
     *a.new_n_free = listed;
     *a.missing = all + max(0, left - a.F);               // (what the list has no place for is lost)
@@ -256,15 +258,15 @@ bool fork_overlaps(const Fork& a) {
   return false;
 }
 
-template <int KM>
+template <int KM, int THREADS>
 cudaError_t fork_launch(const Fork& a, cudaStream_t stream) {
   const size_t memory = (size_t)((a.P + 31) / 32) * 8;
-  if (memory > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(fork_pages_kernel<KM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)memory);
+  if (memory > 40 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(fork_pages_kernel<KM, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)memory);
     if (e != cudaSuccess) return e;
   }
-  jb::Launch cfg(dim3(FORK_BLOCKS), dim3(FORK_THREADS), memory, stream);
-  return cudaLaunchKernelEx(&cfg.c, fork_pages_kernel<KM>, a);
+  jb::Launch cfg(dim3(FORK_BLOCKS), dim3(THREADS), memory, stream);
+  return cudaLaunchKernelEx(&cfg.c, fork_pages_kernel<KM, THREADS>, a);
 }
 
 // ------------------------------------------------------------ copies ------------------------------------------------------------
@@ -403,8 +405,8 @@ JB_EXPORT int jb_fork_pages(const void* given, cudaStream_t stream) {
             "fork_pages: %d groups of %d rows of %d pages, %d pages of %d tokens, %d free places, spare page %d", a.R, a.K, a.W, a.P, a.page_size,
             a.F, a.spare);
   if (fork_overlaps(a)) return JB_ERR_OVERLAP;
-  return (int)(a.K <= 4 ? fork_launch<4>(a, stream) : a.K <= 8 ? fork_launch<8>(a, stream) : a.K <= 16 ? fork_launch<16>(a, stream)
-                                                                                                     : fork_launch<32>(a, stream));
+  return (int)(a.K <= 4 ? fork_launch<4, 1024>(a, stream) : a.K <= 8 ? fork_launch<8, 1024>(a, stream)
+               : a.K <= 16 ? fork_launch<16, 512>(a, stream) : fork_launch<32, 512>(a, stream));
 }
 
 // pages, heads, row_bytes: host arrays of n_tensors; src, dst, rows: device arrays of n.

@@ -13,6 +13,7 @@
 // then.
 #include <math_constants.h>
 #include <stdio.h>
+#include <string.h>
 
 #include "common.cuh"
 
@@ -423,15 +424,14 @@ size_t join_memory(int K, int S) { return (size_t)WARPS * K * K * 8 + (size_t)K 
 
 }  // namespace
 
-// Scratch: keys R * K * ranges * K of 8 bytes, stats R * K * ranges of 24.
-JB_EXPORT int jb_beam_select(const float* logits, const float* scores, const int* stops, int* parents, int* tokens, float* next_scores,
-                             int* ended_parents, int* ended_tokens, float* ended_scores, void* keys, void* stats, int R, int K, int V,
-                             int S, int ranges, cudaStream_t stream) {
+// given: an Args in host memory.  Scratch: keys R * K * ranges * K of 8 bytes, stats R * K * ranges of 24.
+JB_EXPORT int jb_beam_select(const void* given, cudaStream_t stream) {
+  Args a;
+  memcpy(&a, given, sizeof(a));
+  const int R = a.R, K = a.K, V = a.V, S = a.S, ranges = a.ranges;
   JB_REFUSE(R < 1 || K < 1 || K > MOST_BEAMS || V < 1 || S < 0 || S > MOST_STOPS || ranges < 1 || ranges > MOST_RANGES ||
                 (long long)R * K * ranges > 0x7fffffffLL || V > 0x7fffffff - PIECE,
             "beam_select: %d requests of %d beams, vocabulary %d, %d stop tokens, %d ranges", R, K, V, S, ranges);
-  const Args a{logits, scores, stops, parents, tokens, next_scores, ended_parents, ended_tokens, ended_scores, (Key*)keys, (Stat*)stats,
-               R, K, V, S, ranges};
   jb::Launch rows(dim3(R * K * ranges), dim3(THREADS), 0, stream);
   cudaError_t e = cudaLaunchKernelEx(&rows.c, beam_rows_kernel, a);
   if (e != cudaSuccess) return (int)e;

@@ -102,7 +102,7 @@ _SIGNATURES = {
     "jb_latent_down": "piipfpiippiiippppplip",
     "jb_step_tables": "pp", "jb_attention_prefix_f32": "ppp", "jb_attention_prefix_bf16": "pppp",
     "jb_verify_drafts": "pp",
-    "jb_beam_select": "pppppppppppiiiiip", "jb_fork_pages": "pp", "jb_copy_pages": "pppipppiiip", "jb_reorder_rows": "ppippiiip",
+    "jb_beam_select": "pp", "jb_fork_pages": "pp", "jb_copy_pages": "pppipppiiip", "jb_reorder_rows": "ppippiiip",
     "jb_attention_beams": "ppppppppiiiiiiiiiiifpp",
     "jb_gather_rows": "ppiipppiiip", "jb_latent_attention": "ppppppppiiiiiiifiipp", "jb_attention_tc_matrix": "ppppppiiiiiiiifpipp",
 }
@@ -2671,13 +2671,17 @@ MOST_BEAMS = 32          # beams of a request
 MOST_BEAM_STOPS = 32     # stop tokens
 
 
-def _on_current_device(what: str, tensors) -> None:
-    """All tensors on one CUDA device, the current one, whose stream the launch goes to."""
-    if not _checks[0]:
-        return
-    device = tensors[0].get_device()
-    if device < 0 or any(t.get_device() != device for t in tensors) or device != torch.cuda.current_device():
-        raise KernelError(f"{what}: tensors must be on the current CUDA device (there is no CPU path)")
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _all_here(what: str, dtype, tensors, shapes, names) -> None:
+    """`_need_all`, and all tensors on the current device, whose stream the launch goes to."""
+    device = _current_device() if tensors[0].is_cuda else -2
+    for t, shape in zip(tensors, shapes):
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+            for t, shape, name in zip(tensors, shapes, names):
+                _need(t, f"{what} {name}", dtype, shape)
+            raise KernelError(f"{what}: tensors must be on the current CUDA device")
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, stop_tokens: torch.Tensor, *, parents: torch.Tensor, tokens: torch.Tensor,
@@ -2700,20 +2704,23 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, stop_tokens: torch.T
                           f"beams, up to {MOST_BEAM_STOPS} stop tokens)")
     if _checks[0]:
         b = (R, K)
-        _need_all("beam_select", torch.float32, (logits, scores, next_scores, ended_scores), ((R * K, V), b, b, b),
+        _all_here("beam_select", torch.float32, (logits, scores, next_scores, ended_scores), ((R * K, V), b, b, b),
                   ("logits", "scores", "next scores", "scores of ended texts"))
-        _need_all("beam_select", torch.int32, (stop_tokens, parents, tokens, ended_parents, ended_tokens), (stop_tokens.shape[:1], b, b, b, b),
+        _all_here("beam_select", torch.int32, (stop_tokens, parents, tokens, ended_parents, ended_tokens), (stop_tokens.shape[:1], b, b, b, b),
                   ("stop tokens", "parents", "tokens", "parents of ended texts", "tokens of ended texts"))
-        _on_current_device("beam_select", (logits, scores, stop_tokens, parents, tokens, next_scores, ended_parents, ended_tokens, ended_scores))
     ranges = beam_ranges(rows, V)
     keys = workspace.get("beam_keys", (rows * ranges * K,), torch.int64)
     stats = workspace.get("beam_stats", (rows * ranges * 3,), torch.float64)
-    _check(_lib("beam_select").jb_beam_select(
+    _check(_lib("beam_select").jb_beam_select(_BEAM_SELECT(
         logits.data_ptr(), scores.data_ptr(), stop_tokens.data_ptr(), parents.data_ptr(), tokens.data_ptr(), next_scores.data_ptr(),
         ended_parents.data_ptr(), ended_tokens.data_ptr(), ended_scores.data_ptr(), keys.data_ptr(), stats.data_ptr(), R, K, V,
-        stop_tokens.shape[0], ranges, _stream()), "beam_select", kernels=2)
+        stop_tokens.shape[0], ranges), _stream()), "beam_select", kernels=2)
 
 
+_BEAM_SELECT = struct.Struct("11P5i4x").pack     # `Args` of csrc/beam_select.cu
+
+
+@functools.lru_cache(maxsize=4096)
 def beam_ranges(rows: int, vocab: int) -> int:
     """Ranges that a row of logits is cut into: enough blocks for six a multiprocessor, none with less than a piece of 4,096 logits."""
     return max(1, min(32, -(-vocab // 4096), -(-6 * SM_COUNT_TARGET // 2 // rows)))
@@ -2750,11 +2757,10 @@ def fork_pages(parents: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
                copy_src, copy_dst, copy_rows, shared, missing)
     if _checks[0]:
         b, one = (R, K), (1,)
-        _need_all("fork_pages", torch.int32, tensors,
+        _all_here("fork_pages", torch.int32, tensors,
                   (b, b, (R * K, W), (P,), (F,), one, b, b, b, (R * K, W), (P,), (F,), one, b, b, b, (R,), one), _FORK_PAGES_NAMES)
-        _on_current_device("fork_pages", tensors)
-    _check(_lib("beam_cache").jb_fork_pages(_FORK_PAGES(*(t.data_ptr() for t in tensors), R, K, W, P, F, int(spare), int(page_size)), _stream()),
-           "fork_pages")
+    _check(_lib("beam_cache").jb_fork_pages(_FORK_PAGES(*map(torch.Tensor.data_ptr, tensors), R, K, W, P, F, int(spare), int(page_size)),
+                                            _stream()), "fork_pages")
 
 
 _FORK_PAGES = struct.Struct("18P7i4x").pack     # `Fork` of csrc/beam_cache.cu
@@ -2774,21 +2780,30 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Te
     n = src.shape[0]
     if not tensors or n == 0:
         return
-    pages, size = tensors[0].shape[0], tensors[0].shape[2] if tensors[0].dim() == 4 else 0
+    first = tensors[0]
+    pages, size = first.shape[0], first.shape[2] if first.dim() == 4 else 0
+    device = _current_device() if src.is_cuda else -2
     if _checks[0]:
-        _need_all("copy_pages", torch.int32, (src, dst, rows), ((n,), (n,), (n,)), ("pages to copy from", "pages to copy to", "tokens to copy"))
-        for t in tensors:
-            _need(t, "copy_pages tensor")
-            if t.dim() != 4 or t.shape[0] != pages or t.shape[2] != size or t.numel() == 0 or t.element_size() not in (2, 4):
+        _all_here("copy_pages", torch.int32, (src, dst, rows), ((n,), (n,), (n,)), ("pages to copy from", "pages to copy to", "tokens to copy"))
+    at, heads, row_bytes, kind = [], [], [], None
+    for t in tensors:
+        if kind is None or t.shape != kind[0] or t.dtype is not kind[1]:
+            kind = t.shape, t.dtype
+            if len(kind[0]) != 4 or kind[0][0] != pages or kind[0][2] != size or t.numel() == 0 or t.element_size() not in (2, 4):
                 raise KernelError(f"copy_pages: tensors are [{pages}, heads, {size}, numbers] of 2 or 4 bytes, got {t.dtype} {tuple(t.shape)}")
-        _on_current_device("copy_pages", (src, dst, rows, *tensors))
-    lib = _lib("beam_cache")
-    for first in range(0, len(tensors), COPY_PAGES):
-        some = tensors[first: first + COPY_PAGES]
-        m = len(some)
-        _check(lib.jb_copy_pages(struct.pack(f"{m}P", *(t.data_ptr() for t in some)), struct.pack(f"{m}i", *(t.shape[1] for t in some)),
-                                 struct.pack(f"{m}i", *(t.shape[3] * t.element_size() for t in some)), m, src.data_ptr(), dst.data_ptr(),
-                                 rows.data_ptr(), n, pages, size, _stream()), "copy_pages")
+            h, b = kind[0][1], kind[0][3] * t.element_size()
+        if t.get_device() != device or not t.is_contiguous():
+            _need(t, "copy_pages tensor")
+            raise KernelError("copy_pages: tensors must be on the current CUDA device")
+        at.append(t.data_ptr())
+        heads.append(h)
+        row_bytes.append(b)
+    lib, stream = _lib("beam_cache"), _stream()
+    for first in range(0, len(at), COPY_PAGES):
+        some = slice(first, first + COPY_PAGES)
+        m = len(at[some])
+        _check(lib.jb_copy_pages(struct.pack(f"{m}P", *at[some]), struct.pack(f"{m}i", *heads[some]), struct.pack(f"{m}i", *row_bytes[some]), m,
+                                 src.data_ptr(), dst.data_ptr(), rows.data_ptr(), n, pages, size, stream), "copy_pages")
 
 
 REORDER_ROWS = 64       # matrices that one launch of `reorder_rows` takes
@@ -2803,20 +2818,22 @@ def reorder_rows(matrices: Sequence[torch.Tensor], slots: torch.Tensor, parents:
         raise KernelError(f"reorder_rows: groups of {K} rows (1 to {MOST_BEAMS})")
     if not matrices or R == 0:
         return
-    n = matrices[0].shape[0]
+    n, device = matrices[0].shape[0], _current_device() if slots.is_cuda else -2
     if _checks[0]:
-        _need_all("reorder_rows", torch.int32, (slots, parents), ((R * K,), (R, K)), ("slots", "parents"))
-        for m in matrices:
+        _all_here("reorder_rows", torch.int32, (slots, parents), ((R * K,), (R, K)), ("slots", "parents"))
+    at, numbers = [], []
+    for m in matrices:
+        if m.dtype is not torch.float32 or m.get_device() != device or not m.is_contiguous() or m.shape[0] != n or m.numel() == 0:
             _need(m, "reorder_rows matrix", torch.float32)
-            if m.shape[0] != n or m.numel() == 0:
-                raise KernelError(f"reorder_rows: matrices have {n} slots, got {tuple(m.shape)}")
-        _on_current_device("reorder_rows", (slots, parents, *matrices))
-    lib = _lib("beam_cache")
-    for first in range(0, len(matrices), REORDER_ROWS):
-        some = matrices[first: first + REORDER_ROWS]
-        m = len(some)
-        _check(lib.jb_reorder_rows(struct.pack(f"{m}P", *(t.data_ptr() for t in some)), struct.pack(f"{m}q", *(t.numel() // n for t in some)), m,
-                                   slots.data_ptr(), parents.data_ptr(), R, K, n, _stream()), "reorder_rows")
+            raise KernelError(f"reorder_rows: matrices of {n} slots on the current CUDA device are taken, got {tuple(m.shape)}")
+        at.append(m.data_ptr())
+        numbers.append(m.numel() // n)
+    lib, stream = _lib("beam_cache"), _stream()
+    for first in range(0, len(at), REORDER_ROWS):
+        some = slice(first, first + REORDER_ROWS)
+        m = len(at[some])
+        _check(lib.jb_reorder_rows(struct.pack(f"{m}P", *at[some]), struct.pack(f"{m}q", *numbers[some]), m, slots.data_ptr(), parents.data_ptr(),
+                                   R, K, n, stream), "reorder_rows")
 
 
 def attention_beams(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, block_table: torch.Tensor,
@@ -2834,10 +2851,9 @@ def attention_beams(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise KernelError(f"attention_beams: {nh} heads over {nkv} of {hd} numbers (multiples of 8 up to {ATTENTION_MAX_HEAD_DIM})")
     if _checks[0]:
         width, cache = (N, nh * hd), (k_cache.shape[0], nkv, page_size, hd)
-        _need_all("attention_beams", torch.bfloat16, (q, out, k_cache, v_cache), (width, width, cache, cache), ("q", "out", "k cache", "v cache"))
-        _need_all("attention_beams", torch.int32, (block_table, kv_len, shared), ((N, W), (N,), (N // beams,)),
+        _all_here("attention_beams", torch.bfloat16, (q, out, k_cache, v_cache), (width, width, cache, cache), ("q", "out", "k cache", "v cache"))
+        _all_here("attention_beams", torch.int32, (block_table, kv_len, shared), ((N, W), (N,), (N // beams,)),
                   ("block table", "kv_len", "shared pages"))
-        _on_current_device("attention_beams", (q, k_cache, v_cache, out, block_table, kv_len, shared))
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attention_beams: scale {scale}")
     blocks, warps, team, fewest = beam_attention_plan(N // beams, beams, nh, nkv, hd, min(int(max_kv_len), W * page_size))
