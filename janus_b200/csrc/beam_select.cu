@@ -5,9 +5,11 @@
 // The K best that are no stop token go on; a stop token among the K best of all ends its beam's text.  A beam's best continuation
 // stays in the beam's row, so that cache rows and states move only where a beam is lost; the others take the rows left, in order.
 //
-// Two launches.  The first reads every logit once and keeps, in registers, each thread's largest one and its sum of exponentials: nothing
-// is compared with a list on the way.  Then the K-th largest of the threads' maxima bounds the K-th largest logit of the range from below, and
-// only the K threads' numbers at or above it are looked at again (from L2).  The second, a block a request, joins ranges and beams.
+// Three launches.  The first reads every logit once and does nothing but keep, in registers, each thread's largest one and its sum of
+// exponentials.  In the second a block a beam finds the beam's K best: the K-th largest of the threads' maxima bounds the K-th largest
+// logit of the row from below, and only the few threads' numbers at or above it are looked at again (from L2).  The third, a block a
+// request, joins its beams.  64 requests of 8 beams over 128,256 tokens: 59 us, the first 45.  (With the second step done by each block
+// of the first launch 63 us: memory stood still meanwhile; with a warp a beam in the third 76.)
 // Within a beam the order is that of the logits (equal ones: the lowest token first), which no rounding touches; between beams it is
 // that of the totals, whose sum of exponentials is taken to 64 bits where threads meet: 32 bits would turn two beams round now and
 // then.
@@ -24,10 +26,8 @@ typedef unsigned long long Key;      // a logit that sorts as a whole number, ab
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
 constexpr int VECTORS = 4;                                // of 16 bytes that a thread has on its way at a time
-constexpr int PER = 4 * VECTORS;
-constexpr int PIECE = THREADS * PER;
-constexpr int MOST_BEAMS = 32, MOST_STOPS = 32, MOST_RANGES = 32;
-constexpr int ROOM = THREADS * 4 + MOST_BEAMS;            // candidates at a time
+constexpr int MOST_BEAMS = 32, MOST_STOPS = 32, MOST_RANGES = 8;
+constexpr int ROOM = THREADS * 4 + MOST_BEAMS;            // candidates of a beam at a time
 constexpr float FAR = 40.0f;                              // how far a power may lie above what a thread's sum is relative to
 constexpr float WIDE = 1e8f;                              // powers beyond are made by 64-bit arithmetic
 
@@ -40,26 +40,14 @@ __device__ __forceinline__ Key key_of(float x, int token) { return ((Key)sortabl
 __device__ __forceinline__ float logit_of(Key k) { return number((unsigned)(k >> 32)); }
 __device__ __forceinline__ int token_of(Key k) { return (int)~(unsigned)k; }
 
-// The numbers of a warp, the largest in lane 0.
-template <typename T>
-__device__ __forceinline__ T warp_sorted(T k) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int size = 2; size <= 32; size <<= 1) {
-#pragma unroll
-    for (int o = size >> 1; o > 0; o >>= 1) {
-      const T other = __shfl_xor_sync(0xffffffffu, k, o);
-      const bool wants_more = ((lane & size) == 0) == ((lane & o) == 0);
-      if ((other > k) == wants_more) k = other;
-    }
-  }
-  return k;
-}
-
 struct Stat {
   double sum;        // of exp(x) / 2^scale; of entries at +inf, if there are any
   double scale;
   double top;        // the largest number; -inf if there is none
+};
+
+struct Best {          // of a beam: score - log sum exp(x - top), and top, its largest logit; -inf, -inf: there is nothing
+  double base, top;
 };
 
 struct Args {
@@ -72,8 +60,10 @@ struct Args {
   int* ended_parents;
   int* ended_tokens;
   float* ended_scores;
-  Key* keys;          // [rows][ranges][K]
+  float* maxima;      // [rows][ranges][THREADS]
   Stat* stats;        // [rows][ranges]
+  Best* best;         // [rows]
+  Key* keys;          // [rows][K]
   int R, K, V, S, ranges;
 };
 
@@ -107,36 +97,37 @@ __device__ __forceinline__ double warp_max(double v) {
   return v;
 }
 
+// A row of logits in vectors of 16 bytes; vector i holds numbers 4 i - lead .., of which the first and the last may lie outside the row.
+// Range r of the row has vectors begin(r) .. begin(r + 1), its thread t those at begin(r) + t, + THREADS, ...
+struct Row {
+  const float* x;
+  int lead, vectors, V, ranges;
+  __device__ __forceinline__ Row(const Args& a, int row) : x(a.logits + (size_t)row * a.V), V(a.V), ranges(a.ranges) {
+    lead = (int)(((uintptr_t)x >> 2) & 3);
+    vectors = (V + lead + 3) / 4;
+  }
+  __device__ __forceinline__ int begin(int range) const { return (int)((long long)range * vectors / ranges); }
+  __device__ __forceinline__ float4 load(int i) const {
+    const int at = 4 * i - lead;
+    if (at >= 0 && at + 4 <= V) return *reinterpret_cast<const float4*>(x + at);
+    float4 v = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+    if (at >= 0 && at < V) v.x = x[at];
+    if (at + 1 >= 0 && at + 1 < V) v.y = x[at + 1];
+    if (at + 2 >= 0 && at + 2 < V) v.z = x[at + 2];
+    if (at + 3 >= 0 && at + 3 < V) v.w = x[at + 3];
+    return v;
+  }
+};
+
 __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
-  __shared__ Key found[ROOM];          // the best so far, then what came
-  __shared__ float maxima[THREADS];
-  __shared__ int chosen[THREADS];      // threads whose numbers are looked at again
-  __shared__ float edge;
-  __shared__ int n_found, n_chosen;
-  __shared__ int stops[MOST_STOPS];
   __shared__ double top_of[WARPS], sum_of[WARPS];
   jb::pdl_launch_dependents();
   const int row = blockIdx.x / a.ranges, range = blockIdx.x % a.ranges;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.K;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Row x(a, row);
+  const int first = x.begin(range), last = x.begin(range + 1);
   jb::pdl_wait();
   if (dead(a.scores[row])) return;                        // (the second launch asks for nothing of it)
-  if (tid < a.S) stops[tid] = a.stops[tid];
-  if (tid < K) found[tid] = 0;
-  if (tid == 0) edge = -CUDART_INF_F, n_found = K, n_chosen = 0;
-  const float* x_row = a.logits + (size_t)row * a.V;
-  const int lead = (int)(((uintptr_t)x_row >> 2) & 3);    // numbers in front of the row in its first 16 bytes
-  const int vectors = (a.V + lead + 3) / 4;               // of the row; vector i holds numbers 4 i - lead ..
-  const int first = (int)((long long)range * vectors / a.ranges), last = (int)((long long)(range + 1) * vectors / a.ranges);
-  auto load = [&](int i) {
-    const int at = 4 * i - lead;
-    if (at >= 0 && at + 4 <= a.V) return *reinterpret_cast<const float4*>(x_row + at);
-    float4 v = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
-    if (at >= 0 && at < a.V) v.x = x_row[at];
-    if (at + 1 >= 0 && at + 1 < a.V) v.y = x_row[at + 1];
-    if (at + 2 >= 0 && at + 2 < a.V) v.z = x_row[at + 2];
-    if (at + 3 >= 0 && at + 3 < a.V) v.w = x_row[at + 3];
-    return v;
-  };
   // ---- maximum and sum of the thread's numbers: vectors first + tid, + THREADS, ... ----
   // The sum is relative to a power of two near the first numbers' maximum, which is left where it is until one lies FAR above: what changes
   // with every new maximum would cost a warp as much as the numbers themselves.  Powers beyond WIDE below that are 0; where they are
@@ -167,16 +158,16 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
     }
     sum += (double)((jb::lo(s) + jb::hi(s)) + (jb::lo(t) + jb::hi(t)));
   };
-  const int whole0 = lead > 0 ? 1 : 0, whole1 = (a.V + lead) / 4;      // vectors that lie inside the row
+  const int whole0 = x.lead > 0 ? 1 : 0, whole1 = min(last, (x.V + x.lead) / 4);     // vectors that lie inside the row
   for (int i0 = first + tid; i0 < last; i0 += THREADS * VECTORS) {
     float4 v[VECTORS];
-    if (i0 >= whole0 && i0 + (VECTORS - 1) * THREADS < min(last, whole1)) {
-      const float4* at = reinterpret_cast<const float4*>(x_row - lead) + i0;
+    if (i0 >= whole0 && i0 + (VECTORS - 1) * THREADS < whole1) {
+      const float4* at = reinterpret_cast<const float4*>(x.x - x.lead) + i0;
 #pragma unroll
       for (int u = 0; u < VECTORS; ++u) v[u] = at[u * THREADS];
     } else {
 #pragma unroll
-      for (int u = 0; u < VECTORS; ++u) v[u] = i0 + u * THREADS < last ? load(i0 + u * THREADS) : none;
+      for (int u = 0; u < VECTORS; ++u) v[u] = i0 + u * THREADS < last ? x.load(i0 + u * THREADS) : none;
     }
     take(v);
   }
@@ -184,11 +175,11 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
   if (wide || sum != sum || (scale == -CUDART_INF_F && top > -CUDART_INF_F)) {
     mine.sum = 0.0, mine.scale = power_of(mine.top);
     for (int i = first + tid; i < last; i += THREADS) {
-      const float4 v = load(i);
-      const float x[4] = {v.x, v.y, v.z, v.w};
+      const float4 v = x.load(i);
+      const float y[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (x[e] > -CUDART_INF_F) mine.sum += top == CUDART_INF_F ? (x[e] == top ? 1.0 : 0.0) : exp((double)x[e] - mine.top);
+        if (y[e] > -CUDART_INF_F) mine.sum += top == CUDART_INF_F ? (y[e] == top ? 1.0 : 0.0) : exp((double)y[e] - mine.top);
     }
   }
   // ---- the range's sum, relative to its largest number ----
@@ -202,44 +193,118 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) sum_of[warp] = sum;
-  // ---- the threads whose numbers may be among the K largest that are no stop token: a stop token is at most one thread's maximum ----
-  const int wanted = K + a.S, heads = min(wanted, 32);
-  const float sorted = warp_sorted(top);
-  if (lane < heads) maxima[warp * heads + lane] = sorted;
   __syncthreads();
-  if (tid < WARPS * heads && maxima[tid] > -CUDART_INF_F) {
-    const float mine = maxima[tid];
+  const size_t list = (size_t)row * a.ranges + range;
+  if (tid == 0) {
+    double s = 0.0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) s += sum_of[w];
+    a.stats[list] = Stat{s, power_of(all), all};
+  }
+  a.maxima[list * THREADS + tid] = top;
+}
+
+// Whether continuation (x, i) comes in front of (y, j): by total, then by beam and token.
+__device__ __forceinline__ bool in_front(double x, long long i, double y, long long j) { return x > y || (x == y && i < j); }
+
+// A logit's distance from its row's largest; beside entries at +inf, 0 for those and -inf for others.
+__device__ __forceinline__ double worth(float x, double top) {
+  return top == CUDART_INF ? (x == CUDART_INF_F ? 0.0 : -CUDART_INF) : (double)x - top;
+}
+
+// The numbers of a warp, the largest in lane 0.
+__device__ __forceinline__ float warp_sorted(float k) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, k, o);
+      const bool wants_more = ((lane & size) == 0) == ((lane & o) == 0);
+      if ((other > k) == wants_more) k = other;
+    }
+  }
+  return k;
+}
+
+__global__ void __launch_bounds__(THREADS) beam_best_kernel(const Args a) {
+  __shared__ Key found[ROOM];          // the best so far, then what came
+  __shared__ float heads[THREADS];
+  __shared__ unsigned short chosen[MOST_RANGES * THREADS];    // threads of the first launch whose numbers are looked at again
+  __shared__ float edge;
+  __shared__ int n_found, n_chosen;
+  __shared__ int stops[MOST_STOPS];
+  jb::pdl_launch_dependents();
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.K;
+  const Row x(a, row);
+  if (tid < K) found[tid] = 0;
+  if (tid == 0) edge = -CUDART_INF_F, n_found = K, n_chosen = 0;
+  jb::pdl_wait();
+  const float score = a.scores[row];
+  if (dead(score)) {
+    if (tid < K) a.keys[(size_t)row * K + tid] = 0;
+    if (tid == 0) a.best[row] = Best{-CUDART_INF, -CUDART_INF};
+    return;
+  }
+  if (tid < a.S) stops[tid] = a.stops[tid];
+  float maxima[MOST_RANGES], top = -CUDART_INF_F;
+#pragma unroll
+  for (int r = 0; r < MOST_RANGES; ++r) {
+    maxima[r] = r < a.ranges ? a.maxima[((size_t)row * a.ranges + r) * THREADS + tid] : -CUDART_INF_F;
+    top = fmaxf(top, maxima[r]);
+  }
+  // ---- the bound: a stop token is at most one thread's maximum ----
+  const int wanted = K + a.S, per_warp = min(wanted, 32);
+  const float sorted = warp_sorted(top);
+  if (lane < per_warp) heads[warp * per_warp + lane] = sorted;
+  __syncthreads();
+  if (tid < WARPS * per_warp && heads[tid] > -CUDART_INF_F) {
+    const float mine = heads[tid];
     int above = 0, level = 0;                             // larger ones, equal ones
-#pragma unroll 4
-    for (int i = 0; i < WARPS * heads; ++i) above += maxima[i] > mine, level += maxima[i] == mine;
+#pragma unroll 8
+    for (int i = 0; i < WARPS * per_warp; ++i) above += heads[i] > mine, level += heads[i] == mine;
     if (above < wanted && above + level >= wanted) edge = mine;   // (all who are level write the same)
+  }
+  if (warp == WARPS - 1) {                                // ... and, by a warp with nothing to do, the row's sum
+    Stat s{0.0, -CUDART_INF, -CUDART_INF};
+    if (lane < a.ranges) s = a.stats[(size_t)row * a.ranges + lane];
+    const double most = warp_max(s.top);
+    double sum = relative(s, most);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) a.best[row] = most > -CUDART_INF ? Best{(double)score - log(sum), most} : Best{-CUDART_INF, -CUDART_INF};
   }
   __syncthreads();
   const float least = edge;                               // -inf: fewer threads than that have a number
-  if (top > -CUDART_INF_F && top >= least) chosen[atomicAdd(&n_chosen, 1)] = tid;
+#pragma unroll
+  for (int r = 0; r < MOST_RANGES; ++r)
+    if (maxima[r] >= least && maxima[r] > -CUDART_INF_F) chosen[atomicAdd(&n_chosen, 1)] = (unsigned short)(r * THREADS + tid);
   __syncthreads();
-  // ---- their numbers at or above it, in rounds of a vector a thread (one or two rounds, unless many maxima are equal) ----
-  const int each = (last - first + THREADS - 1) / THREADS, n = n_chosen * each;
+  // ---- their numbers at or above it, in rounds of a vector a thread (two or three, unless many maxima are equal) ----
+  const int each = (x.vectors + a.ranges - 1) / a.ranges / THREADS + 1, n = n_chosen * each;       // vectors of a thread, at most
   Key bound = 0;                       // the K-th best so far, 0 while there are fewer
   for (int j0 = 0; j0 < n; j0 += THREADS) {
-    const int j = j0 + tid, i = j < n ? first + chosen[j / each] + j % each * THREADS : last;
-    if (i < last) {
-      const float4 v = load(i);
-      const float x[4] = {v.x, v.y, v.z, v.w};
+    const int j = j0 + tid;
+    if (j < n) {
+      const int slot = chosen[j / each], range = slot / THREADS, i = x.begin(range) + slot % THREADS + j % each * THREADS;
+      if (i < x.begin(range + 1)) {
+        const float4 v = x.load(i);
+        const float y[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (x[e] >= least && x[e] > -CUDART_INF_F) {
-          const int token = 4 * i - lead + e;
-          const Key k = key_of(x[e], token);
-          bool stop = false;
-          for (int s = 0; s < a.S; ++s) stop |= stops[s] == token;
-          if (k > bound && !stop) found[atomicAdd(&n_found, 1)] = k;
+        for (int e = 0; e < 4; ++e) {
+          if (y[e] >= least && y[e] > -CUDART_INF_F) {
+            const int token = 4 * i - x.lead + e;
+            const Key k = key_of(y[e], token);
+            bool stop = false;
+            for (int s = 0; s < a.S; ++s) stop |= stops[s] == token;
+            if (k > bound && !stop) found[atomicAdd(&n_found, 1)] = k;
+          }
         }
       }
     }
-    // (rounds whose numbers still have room beside the next one's are put in order later)
-    const bool full = __syncthreads_or(n_found > ROOM - 4 * THREADS) != 0;
-    if (!full && j0 + THREADS < n) continue;
+    // (rounds whose numbers leave room for the next one's are put in order later)
+    const bool last = j0 + THREADS >= n, full = __syncthreads_or(n_found > ROOM - 4 * THREADS) != 0;
+    if (!full && !last) continue;
     // the K best of what was there and what came, in order: a key's place is the number of larger ones
     const int m = n_found;
     Key k[(ROOM + THREADS - 1) / THREADS];
@@ -262,38 +327,21 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
     __syncthreads();
     bound = found[K - 1];
   }
-  __syncthreads();
-  const size_t list = (size_t)row * a.ranges + range;
-  if (tid == 0) {
-    double s = 0.0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) s += sum_of[w];
-    a.stats[list] = Stat{s, power_of(all), all};
-  }
-  if (tid < K) a.keys[list * K + tid] = found[tid];
+  if (tid < K) a.keys[(size_t)row * K + tid] = found[tid];     // (0 where the row has fewer)
 }
 
-// Whether continuation (x, i) comes in front of (y, j): by total, then by beam and token.
-__device__ __forceinline__ bool in_front(double x, long long i, double y, long long j) { return x > y || (x == y && i < j); }
+constexpr int JOIN_THREADS = 256;
 
-// A logit's distance from its row's largest; beside entries at +inf, 0 for those and -inf for others.
-__device__ __forceinline__ double worth(float x, double top) {
-  return top == CUDART_INF ? (x == CUDART_INF_F ? 0.0 : -CUDART_INF) : (double)x - top;
-}
-
-// One block a request.  Dynamic memory: WARPS * K * K keys, then for K * K continuations (total, place), their shortened list, and
-// for K * S stop tokens the same.
-__global__ void __launch_bounds__(THREADS) beam_join_kernel(const Args a) {
+// One block a request.  Dynamic memory: K * K continuations (total, place), their shortened list, and for K * S stop tokens the same.
+__global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t memory[];
-  __shared__ double base[MOST_BEAMS];      // score - log sum exp(x - top), of a live beam
-  __shared__ double top_of[MOST_BEAMS];    // its largest logit
+  __shared__ double base[MOST_BEAMS], top_of[MOST_BEAMS];  // see Best
   __shared__ double kth[MOST_BEAMS], head[MOST_BEAMS];
   __shared__ double on[MOST_BEAMS];
   __shared__ long long on_at[MOST_BEAMS];
   __shared__ int n_list, n_stop;
   const int r = blockIdx.x, K = a.K, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, KK = K * K;
-  Key* lists = reinterpret_cast<Key*>(memory);                           // [WARPS][K * K]
-  double* totals = reinterpret_cast<double*>(lists + WARPS * KK);        // [K][K]
+  double* totals = reinterpret_cast<double*>(memory);                    // [K][K]
   double* short_total = totals + KK;
   double* stop_total = short_total + KK;                                 // [K * S]
   int* token = reinterpret_cast<int*>(stop_total + K * a.S);             // [K][K]
@@ -307,54 +355,27 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Args a) {
     a.ended_scores[r * K + tid] = -CUDART_INF_F;
     on[tid] = -CUDART_INF;
     on_at[tid] = 0;
+    const Best best = a.best[r * K + tid];
+    base[tid] = best.base, top_of[tid] = best.top;
   }
-  // ---- every beam's K best, a warp a beam ----
-  Key* mine = lists + warp * KK;
-  for (int b = warp; b < K; b += WARPS) {
-    const int row = r * K + b;
-    const float score = a.scores[row];
-    for (int j = lane; j < K; j += 32) totals[b * K + j] = -CUDART_INF, token[b * K + j] = 0;
-    if (lane == 0) base[b] = top_of[b] = -CUDART_INF;
-    if (!dead(score)) {
-      const Key* keys = a.keys + (size_t)row * a.ranges * K;
-      Key edge = lane < a.ranges ? keys[lane * K] : 0;
-      Stat s{0.0, -CUDART_INF, -CUDART_INF};
-      if (lane < a.ranges) s = a.stats[(size_t)row * a.ranges + lane];
-      const double top = warp_max(s.top);
-      double sum = relative(s, top);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      const double start = (double)score - log(sum);      // (a number wherever the row has one above -inf)
-      if (lane == 0) base[b] = start, top_of[b] = top;
-      edge = __shfl_sync(0xffffffffu, warp_sorted(edge), K - 1);          // no more than K ranges have anything at or above it
-      int n = 0;
-      for (int i0 = 0; i0 < a.ranges * K; i0 += 32) {
-        const Key k = i0 + lane < a.ranges * K ? keys[i0 + lane] : 0;
-        const bool takes = k > 0 && k >= edge;
-        const unsigned who = __ballot_sync(0xffffffffu, takes);
-        if (takes) mine[n + __popc(who & ((1u << lane) - 1u))] = k;
-        n += __popc(who);
-      }
-      __syncwarp();
-      for (int i = lane; i < n; i += 32) {
-        const Key k = mine[i];
-        int above = 0;
-        for (int j = 0; j < n; ++j) above += mine[j] > k;
-        if (above < K) {
-          totals[b * K + above] = start + worth(logit_of(k), top);
-          token[b * K + above] = token_of(k);
-        }
-      }
-      __syncwarp();
-    }
-    if (lane == 0) head[b] = totals[b * K], kth[b] = totals[b * K + K - 1];
+  for (int i = tid; i < KK; i += JOIN_THREADS) {
+    const Best best = a.best[r * K + i / K];
+    const Key k = a.keys[(size_t)r * KK + i];
+    const double total = k > 0 ? best.base + worth(logit_of(k), best.top) : -CUDART_INF;
+    totals[i] = total;
+    token[i] = k > 0 ? token_of(k) : 0;
+    if (i % K == 0) head[i / K] = total;
+    if (i % K == K - 1) kth[i / K] = total;
   }
+  // (a stop token's logit is on its way meanwhile)
+  const int b0 = a.S > 0 ? tid / a.S : K, stop0 = b0 < K ? a.stops[tid % a.S] : -1;
+  const float x0 = b0 < K && stop0 >= 0 && stop0 < a.V ? a.logits[((size_t)r * K + b0) * a.V + stop0] : -CUDART_INF_F;
   __syncthreads();
   // ---- the K best of all beams: at least K lie at or above the largest K-th of a beam, and above the least of the beams' best ----
   double edge = -CUDART_INF, least = CUDART_INF;
   for (int b = 0; b < K; ++b) edge = fmax(edge, kth[b]), least = fmin(least, head[b]);
   edge = fmax(edge, least);
-  for (int i = tid; i < KK; i += THREADS) {
+  for (int i = tid; i < KK; i += JOIN_THREADS) {
     if (totals[i] > -CUDART_INF && totals[i] >= edge) {
       const int at = atomicAdd(&n_list, 1);
       short_total[at] = totals[i];
@@ -363,7 +384,7 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Args a) {
   }
   __syncthreads();
   const long long V = a.V;
-  for (int i = tid; i < n_list; i += THREADS) {
+  for (int i = tid; i < n_list; i += JOIN_THREADS) {
     const double t = short_total[i];
     const long long at = short_at[i] / K * V + token[short_at[i]];
     int before = 0;
@@ -372,12 +393,12 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Args a) {
   }
   __syncthreads();
   // ---- stop tokens that stand among the K best ----
-  for (int i = tid; i < K * a.S; i += THREADS) {
+  for (int i = tid; i < K * a.S; i += JOIN_THREADS) {
     const int b = i / a.S, stop = a.stops[i % a.S];
     bool again = false;
     for (int s = 0; s < i % a.S; ++s) again |= a.stops[s] == stop;
     if (stop < 0 || stop >= a.V || again || !(base[b] > -CUDART_INF)) continue;
-    const float x = a.logits[((size_t)r * K + b) * a.V + stop];
+    const float x = i == tid ? x0 : a.logits[((size_t)r * K + b) * a.V + stop];
     if (!(x > -CUDART_INF_F)) continue;
     const double t = base[b] + worth(x, top_of[b]);
     if (!(t > -CUDART_INF) || !in_front(t, b * V + stop, on[K - 1], on[K - 1] > -CUDART_INF ? on_at[K - 1] : K * V)) continue;
@@ -386,7 +407,7 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Args a) {
     stop_at[at] = i;
   }
   __syncthreads();
-  for (int i = tid; i < n_stop; i += THREADS) {
+  for (int i = tid; i < n_stop; i += JOIN_THREADS) {
     const double t = stop_total[i];
     const int b = stop_at[i] / a.S, stop = a.stops[stop_at[i] % a.S];
     int place = 0, before = 0;
@@ -420,26 +441,27 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const Args a) {
   }
 }
 
-size_t join_memory(int K, int S) { return (size_t)WARPS * K * K * 8 + (size_t)K * K * (8 + 8 + 4 + 4) + (size_t)K * S * (8 + 4); }
+size_t join_memory(int K, int S) { return (size_t)K * K * (8 + 8 + 4 + 4) + (size_t)K * S * (8 + 4); }
+static_assert(MOST_BEAMS * (MOST_BEAMS * 24 + MOST_STOPS * 12) <= 40 * 1024, "the third launch's memory");
 
 }  // namespace
 
-// given: an Args in host memory.  Scratch: keys R * K * ranges * K of 8 bytes, stats R * K * ranges of 24.
+// given: an Args in host memory.  Scratch: maxima R * K * ranges * 256 float32, stats R * K * ranges of 24 bytes,
+// best R * K of 16, keys R * K * K of 8.
 JB_EXPORT int jb_beam_select(const void* given, cudaStream_t stream) {
   Args a;
   memcpy(&a, given, sizeof(a));
   const int R = a.R, K = a.K, V = a.V, S = a.S, ranges = a.ranges;
   JB_REFUSE(R < 1 || K < 1 || K > MOST_BEAMS || V < 1 || S < 0 || S > MOST_STOPS || ranges < 1 || ranges > MOST_RANGES ||
-                (long long)R * K * ranges > 0x7fffffffLL || V > 0x7fffffff - PIECE,
+                (long long)R * K * ranges > 0x7fffffffLL || V > 0x7fffffff - 65536,
             "beam_select: %d requests of %d beams, vocabulary %d, %d stop tokens, %d ranges", R, K, V, S, ranges);
   jb::Launch rows(dim3(R * K * ranges), dim3(THREADS), 0, stream);
   cudaError_t e = cudaLaunchKernelEx(&rows.c, beam_rows_kernel, a);
   if (e != cudaSuccess) return (int)e;
+  jb::Launch best(dim3(R * K), dim3(THREADS), 0, stream);
+  e = cudaLaunchKernelEx(&best.c, beam_best_kernel, a);
+  if (e != cudaSuccess) return (int)e;
   const size_t memory = join_memory(K, S);
-  if (memory > 48 * 1024) {
-    e = cudaFuncSetAttribute(beam_join_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)join_memory(MOST_BEAMS, MOST_STOPS));
-    if (e != cudaSuccess) return (int)e;
-  }
-  jb::Launch join(dim3(R), dim3(THREADS), memory, stream);
+  jb::Launch join(dim3(R), dim3(JOIN_THREADS), memory, stream);
   return (int)cudaLaunchKernelEx(&join.c, beam_join_kernel, a);
 }

@@ -2709,21 +2709,22 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, stop_tokens: torch.T
         _all_here("beam_select", torch.int32, (stop_tokens, parents, tokens, ended_parents, ended_tokens), (stop_tokens.shape[:1], b, b, b, b),
                   ("stop tokens", "parents", "tokens", "parents of ended texts", "tokens of ended texts"))
     ranges = beam_ranges(rows, V)
-    keys = workspace.get("beam_keys", (rows * ranges * K,), torch.int64)
-    stats = workspace.get("beam_stats", (rows * ranges * 3,), torch.float64)
+    maxima = workspace.get("beam_maxima", (rows * ranges * 256,), torch.float32)
+    stats = workspace.get("beam_stats", (rows * (3 * ranges + 2 + K),), torch.float64)      # 24 bytes a range, then 16 + 8 K a row
+    best = stats.data_ptr() + 24 * rows * ranges
     _check(_lib("beam_select").jb_beam_select(_BEAM_SELECT(
         logits.data_ptr(), scores.data_ptr(), stop_tokens.data_ptr(), parents.data_ptr(), tokens.data_ptr(), next_scores.data_ptr(),
-        ended_parents.data_ptr(), ended_tokens.data_ptr(), ended_scores.data_ptr(), keys.data_ptr(), stats.data_ptr(), R, K, V,
-        stop_tokens.shape[0], ranges), _stream()), "beam_select", kernels=2)
+        ended_parents.data_ptr(), ended_tokens.data_ptr(), ended_scores.data_ptr(), maxima.data_ptr(), stats.data_ptr(), best, best + 16 * rows, R, K, V,
+        stop_tokens.shape[0], ranges), _stream()), "beam_select", kernels=3)
 
 
-_BEAM_SELECT = struct.Struct("11P5i4x").pack     # `Args` of csrc/beam_select.cu
+_BEAM_SELECT = struct.Struct("13P5i4x").pack     # `Args` of csrc/beam_select.cu
 
 
 @functools.lru_cache(maxsize=4096)
 def beam_ranges(rows: int, vocab: int) -> int:
-    """Ranges that a row of logits is cut into: enough blocks for six a multiprocessor, none with less than a piece of 4,096 logits."""
-    return max(1, min(32, -(-vocab // 4096), -(-6 * SM_COUNT_TARGET // 2 // rows)))
+    """Ranges that a row of logits is cut into: enough blocks for ten a multiprocessor, none with less than a round of 4,096 logits."""
+    return max(1, min(8, -(-vocab // 4096), -(-10 * SM_COUNT_TARGET // 2 // rows)))
 
 
 def fork_pages(parents: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, free_pages: torch.Tensor,
