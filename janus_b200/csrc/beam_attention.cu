@@ -37,6 +37,7 @@ struct Args {
   const int* shared;
   int R, K, nh, nkv, hd, W, n_pages;
   int team, row_blocks, fewest;                    // warps of a team; blocks of rows of a request; units of a share at least
+  int block_rows;                                  // rows of a block
   float scale_log2;
 };
 
@@ -102,7 +103,7 @@ struct Rows {
 };
 
 __device__ __forceinline__ Rows look_up(const Args& a, int block) {
-  const int lane = threadIdx.x & 31, G = a.nh / a.nkv, all = ROWS * a.team;
+  const int lane = threadIdx.x & 31, G = a.nh / a.nkv, all = a.block_rows;
   Rows x;
   x.request = block / a.row_blocks;
   x.rho0 = block % a.row_blocks * all;
@@ -124,14 +125,14 @@ __device__ __forceinline__ Rows look_up(const Args& a, int block) {
 }
 // The units of a block, by one thread.
 __device__ __forceinline__ int count_units(const Args& a, int block) {
-  const int G = a.nh / a.nkv, all = ROWS * a.team, r = block / a.row_blocks, rho0 = block % a.row_blocks * all;
+  const int G = a.nh / a.nkv, all = a.block_rows, r = block / a.row_blocks, rho0 = block % a.row_blocks * all;
   const int beam0 = rho0 / G, beam1 = (min(rho0 + all, a.K * G) - 1) / G;
   int most = 0;
-#pragma unroll 4
+#pragma unroll 8
   for (int k = 0; k < a.K; ++k) most = max(most, min(max(a.kv_len[r * a.K + k], 0), a.W * PAGE));
   const int common = min(max(a.shared[r], 0), most / PAGE);
   int n = common * (PAGE / KEYS);
-#pragma unroll 4
+#pragma unroll 8
   for (int k = beam0; k <= beam1; ++k) {
     const int len = min(max(a.kv_len[r * a.K + k], 0), a.W * PAGE);
     n += (len - (len < common * PAGE ? 0 : common * PAGE) + KEYS - 1) / KEYS;
@@ -142,14 +143,15 @@ __device__ __forceinline__ int count_units(const Args& a, int block) {
 // A place of the list as one thread walks it: the unit's beam (-1: all that share it), its first key, and where its page stands.
 struct Cursor {
   int block, kvh, unit, units, shared_units;
-  int request, head, common, beam0, beam1;
+  int request, head, common, beam0, beam1, rho0, n_rows;
   int beam, at, keys;
   const int* entry;                 // of the table; null: a unit without keys
 
   __device__ __forceinline__ int length(const Args& a, int b) const { return min(max(a.kv_len[request * a.K + b], 0), a.W * PAGE); }
   __device__ __forceinline__ int own_from(int len) const { return len < common * PAGE ? 0 : common * PAGE; }
   __device__ __forceinline__ void enter(const Args& a, int to) {
-    const int G = a.nh / a.nkv, all = ROWS * a.team, rho0 = to % a.row_blocks * all;
+    const int G = a.nh / a.nkv, all = a.block_rows;
+    rho0 = to % a.row_blocks * all, n_rows = min(all, a.K * G - rho0);
     block = to, request = to / a.row_blocks, beam0 = rho0 / G, beam1 = (min(rho0 + all, a.K * G) - 1) / G;
     int most = -1;
     head = 0;
@@ -183,17 +185,19 @@ struct Cursor {
     }
     beam = -1, at = keys = 0, entry = nullptr;
   }
-  __device__ __forceinline__ void step(const Args& a) {
+  __device__ __forceinline__ bool step(const Args& a) {      // whether another block of rows has begun
+    bool entered = false;
     if (++unit == units) {
       unit = 0;
-      if (++kvh == a.nkv) kvh = 0, enter(a, block + 1);
+      if (++kvh == a.nkv) kvh = 0, enter(a, block + 1), entered = true;
     } else if (beam >= 0 && at + KEYS < length(a, beam)) {  // the next keys of the same beam
       entry += (at % PAGE + KEYS) / PAGE;
       at += KEYS;
       keys = min(KEYS, length(a, beam) - at);
-      return;
+      return false;
     }
     find(a);
+    return entered;
   }
 };
 
@@ -466,6 +470,527 @@ __global__ void __launch_bounds__(Shape<HDC>::THREADS, HDC <= 64 ? 2 : 1) beam_a
     for (int turn = max(0, asked - begin - stages); turn < asked - begin; ++turn) mbar_wait(bars + 16 * (turn % stages), (turn / stages) & 1, status, 53);
 }
 
+// ---------------------------------------------------------------------------
+// Heads of up to 128 numbers: the tensor cores of tcgen05, keys on the tile's 128 rows, the beams' queries on its N columns, so that a
+// request's few rows are no padding:  S' = K Q' and O' = V' P', both accumulated in tensor memory.
+//   warp 0       walks the block's share of the list and brings its units, four (128 keys) a stage, by the copy engine
+//   warp 1       one lane issues the products; the next stage's scores before this one's values, where its keys are there
+//   warps 4-11   two groups of four, each with half the columns: a thread has one key.  Weights relative to a number a row that is raised
+//                only when a score passes it by RESCALE_LOG2 (then the sums and O' are scaled down); P to shared memory, a row a key
+// A stage's units may be different beams' own; a mask of rows goes with each.
+// ---------------------------------------------------------------------------
+constexpr int SUB = 4, BLOCK_KEYS = SUB * KEYS;              // units of a stage
+constexpr int TC_THREADS = 384;
+constexpr float NOTHING = -1e30f;                            // what weights are relative to before a row has seen a key
+
+struct Info {                                                // of a stage
+  int first, last, final_, whole;                            // of its block of rows' keys in this share; of the share; no mask
+  int request, rho0, n_rows, kvh;
+  int piece0, piece1;                                        // shares that the block of rows has parts in
+  int keys[SUB];
+  unsigned long long rows[SUB][2];                           // that see the unit's keys
+};
+
+template <int HDC, int N>
+struct Tc {
+  static constexpr int SLABS = HDC / 64, SLAB = BLOCK_KEYS * 128, STAGE = 2 * SLABS * SLAB;      // values, then keys
+  static constexpr int Q = SLABS * N * 128, P = (N > 64 ? 2 : 1) * BLOCK_KEYS * 128;
+  static constexpr int MISC = 4 * N + 16 * N + 1200;         // ref, exchange, barriers and descriptions
+  static constexpr int FIT = (232448 - Q - P - MISC) / STAGE, STAGES = FIT > 6 ? 6 : FIT;
+  static constexpr int AT_Q = STAGES * STAGE, AT_P = AT_Q + Q, AT_REF = AT_P + P, AT_SWAP = AT_REF + 4 * N, AT_INFO = AT_SWAP + 16 * N,
+                       AT_BARS = AT_INFO + STAGES * (int)sizeof(Info), SMEM = AT_BARS + (3 * STAGES + 6) * 8 + 16;
+  static constexpr int COLS = 3 * N <= 64 ? 64 : 3 * N <= 128 ? 128 : 3 * N <= 256 ? 256 : 512;  // two S', one O'
+  static constexpr int HALF = N / 2;                         // columns of a group of warps
+  static_assert(STAGES >= 2 && SMEM <= 232448, "shared memory of a block");
+};
+
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0u;
+}
+__device__ __forceinline__ bool elected() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0u;
+}
+// A barrier of a group of four warps that tells all whether any of its threads says `yes`.
+__device__ __forceinline__ bool group_any(int barrier, bool yes) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(barrier), "r"((uint32_t)yes)
+      : "memory");
+  return any != 0u;
+}
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, uint32_t lead, uint32_t stride) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)((lead >> 4) & 0x3FFF) << 16 | (uint64_t)((stride >> 4) & 0x3FFF) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "f"(r[0]), "f"(r[1]), "f"(r[2]),
+               "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Rows [from, to) of a block, as bits.
+__device__ __forceinline__ void add_rows(unsigned long long (&bits)[2], int from, int to) {
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const int a = min(max(from - 64 * w, 0), 64), b = min(max(to - 64 * w, 0), 64);
+    if (b > a) bits[w] |= (b - a == 64 ? ~0ull : ((1ull << (b - a)) - 1ull)) << a;
+  }
+}
+
+// out[c] = the sum of v[c] over the warp's lanes, for C columns (a power of two from 8 to 64).
+template <int C>
+__device__ __forceinline__ void columns_summed(const float (&v)[C], float* out) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (C == 64) {
+    float lo[32], hi[32];
+#pragma unroll
+    for (int c = 0; c < 32; ++c) lo[c] = v[c], hi[c] = v[32 + c];
+    columns_summed<32>(lo, out);
+    columns_summed<32>(hi, out + 32);
+  } else {
+    float t[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) t[c] = v[c];
+    int o = 16, left = C;
+#pragma unroll
+    for (int step = 0; step < 5; ++step, o >>= 1) {
+      if (left > 1) {
+        left >>= 1;
+        const bool up = (lane & o) != 0;
+#pragma unroll
+        for (int c = 0; c < C / 2; ++c) {
+          if (c < left) {
+            const float mine = up ? t[left + c] : t[c], other = up ? t[c] : t[left + c];
+            t[c] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+          }
+        }
+      } else {
+        t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
+      }
+    }
+    // lane bits from the top name the column, as far as they were needed
+    constexpr int BITS = C == 8 ? 3 : C == 16 ? 4 : 5;
+    if ((lane & ((1 << (5 - BITS)) - 1)) == 0) out[lane >> (5 - BITS)] = t[0];
+  }
+}
+
+template <int HDC, int N>
+__global__ void __launch_bounds__(TC_THREADS, 1) beam_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                        const __grid_constant__ CUtensorMap map_v, const Args a,
+                                                                        int* __restrict__ status) {
+  typedef Tc<HDC, N> C;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, G = a.nh / a.nkv, hd = a.hd;
+  const uint32_t base = jb::smem_u32(smem), q_at = base + C::AT_Q, p_at = base + C::AT_P;
+  float* ref = reinterpret_cast<float*>(smem + C::AT_REF);             // [N] in units of log2
+  float* swap = reinterpret_cast<float*>(smem + C::AT_SWAP);           // [4][N]
+  Info* info = reinterpret_cast<Info*>(smem + C::AT_INFO);             // [STAGES]
+  const uint32_t bars = base + C::AT_BARS, kv_full = bars, kv_empty = bars + 8 * C::STAGES, s_full = bars + 16 * C::STAGES, p_full = s_full + 16,
+                 pv_done = p_full + 8, q_full = pv_done + 8, o_full = q_full + 8, told = o_full + 8;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::AT_BARS + (3 * C::STAGES + 6) * 8);
+  if (tid == 0) {
+    for (int i = 0; i < C::STAGES; ++i) jb::mbar_init(kv_full + 8 * i, 1), jb::mbar_init(kv_empty + 8 * i, 1), jb::mbar_init(told + 8 * i, 1);
+    jb::mbar_init(s_full, 1), jb::mbar_init(s_full + 8, 1), jb::mbar_init(p_full, 8), jb::mbar_init(pv_done, 1), jb::mbar_init(q_full, 8);
+    jb::mbar_init(o_full, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) jb::tmem_alloc<C::COLS>(jb::smem_u32((const void*)tmem_slot));
+  jb::pdl_launch_dependents();
+  jb::pdl_wait();
+  // ---- the list's length: a thread's blocks of rows, then all threads' ----
+  int* sums = reinterpret_cast<int*>(smem + C::AT_P);                  // (P is not there yet)
+  const int blocks = a.R * a.row_blocks, chunk = (blocks + TC_THREADS - 1) / TC_THREADS;
+  {
+    int mine = 0;
+    for (int i = tid * chunk; i < min((tid + 1) * chunk, blocks); ++i) mine += count_units(a, i);
+    sums[tid] = mine * a.nkv;
+  }
+  jb::tc_fence_before();
+  __syncthreads();
+  jb::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (warp == 0) {
+    constexpr int EACH = TC_THREADS / 32;
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) mine += sums[lane * EACH + i];
+    int up = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += t;
+    }
+    const int total = __shfl_sync(0xffffffffu, up, 31);
+    // shares are whole stages, so that where one ends inside a block of rows no stage is cut
+    const int per = max(a.fewest, (total + (int)gridDim.x - 1) / (int)gridDim.x + SUB - 1) / SUB * SUB;
+    const int begin = min((int)blockIdx.x * per, total), end = min(begin + per, total);
+    const int owner = begin < end ? __ffs(__ballot_sync(0xffffffffu, begin < up)) - 1 : 0, before_owner = __shfl_sync(0xffffffffu, up - mine, owner);
+    int block = 0, kvh = 0, unit = 0, at = begin, st = 0, round = 0;
+    bool ok = true;
+    Rows x{};
+    if (begin >= end) {                                                // nothing: one stage that says so
+      if (lane == 0) {
+        info[0].final_ = 2;
+        jb::mbar_arrive(told);
+        jb::mbar_arrive(kv_full);
+      }
+    } else {
+      int before = before_owner, t = owner * EACH;
+      while (begin >= before + sums[t]) before += sums[t++];
+      for (block = t * chunk;; ++block) {
+        x = look_up(a, block);
+        if (begin < before + x.units * a.nkv) break;
+        before += x.units * a.nkv;
+      }
+      kvh = (begin - before) / x.units;
+      unit = begin - before - kvh * x.units;
+    }
+    // Lanes 0 to 3 have a unit of a stage each.  A stage's pages are looked up while the one before is asked for.
+    unsigned long long joining[2] = {0ull, 0ull}, all[2] = {0ull, 0ull};
+    auto entered = [&]() {                                             // rows that read the shared pages; all rows
+      joining[0] = joining[1] = all[0] = all[1] = 0ull;
+      unsigned who = __ballot_sync(0xffffffffu, lane < a.K && x.len >= x.common * PAGE);
+      while (who) {
+        const int b = __ffs(who) - 1;
+        who &= who - 1;
+        add_rows(joining, max(b * G - x.rho0, 0), min((b + 1) * G - x.rho0, x.n_rows));
+      }
+      add_rows(all, 0, x.n_rows);
+    };
+    int n = 0, keys = 0, from = 0, beam = -1;                          // units of the stage; the lane's: keys, place in its page, beam
+    const int* entry = nullptr;
+    auto find = [&]() {
+      n = min(min(SUB, x.units - unit), end - at);
+      const int shared_units = x.common * (PAGE / KEYS), mine = unit + lane;
+      beam = -1, keys = 0, entry = nullptr;
+      if (lane < n && mine < shared_units) {
+        keys = KEYS, from = mine * KEYS % PAGE;
+        entry = a.table + ((size_t)x.request * a.K + x.head) * a.W + mine / (PAGE / KEYS);
+      }
+      for (int i = max(shared_units - unit, 0); i < n; ++i) {          // beams' own
+        const int j = unit + i - shared_units;
+        const unsigned behind = __ballot_sync(0xffffffffu, x.upto > j);
+        if (behind == 0u) break;                                       // (rows without keys)
+        const int b = __ffs(behind) - 1;
+        const int first = __shfl_sync(0xffffffffu, x.first, b), before = __shfl_sync(0xffffffffu, x.upto - x.own, b), len = __shfl_sync(0xffffffffu, x.len, b);
+        if (lane == i) {
+          const int key = first * PAGE + (j - before) * KEYS;
+          beam = b, keys = min(KEYS, len - key), from = key % PAGE;
+          entry = a.table + ((size_t)x.request * a.K + b) * a.W + key / PAGE;
+        }
+      }
+    };
+    int page = -1;
+    if (at < end) {
+      entered();
+      find();
+      page = entry != nullptr ? *entry : -1;
+    }
+    while (at < end) {
+      if (round > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(kv_empty + 8 * st, (round - 1) & 1, status, 54));
+        if (!ok) break;
+      }
+      const bool there = keys > 0 && page >= 0 && page < a.n_pages;    // (no page: no keys)
+      const bool first = at == begin || unit == 0, last = unit + n == x.units || at + n == end;
+      unsigned long long rows[2] = {joining[0], joining[1]};
+      if (beam >= 0) {
+        rows[0] = rows[1] = 0ull;
+        add_rows(rows, max(beam * G - x.rho0, 0), min((beam + 1) * G - x.rho0, x.n_rows));
+      }
+      const unsigned loads = __ballot_sync(0xffffffffu, there);
+      const bool whole = __all_sync(0xffffffffu, lane >= SUB || (there && keys == KEYS && rows[0] == all[0] && rows[1] == all[1]));
+      Info& to = info[st];
+      if (lane < SUB) to.keys[lane] = there ? keys : 0, to.rows[lane][0] = rows[0], to.rows[lane][1] = rows[1];
+      const uint32_t full = kv_full + 8 * st, stage = base + st * C::STAGE;
+      if (lane == 0) {
+        const int start = at - unit;                                   // the block of rows' first place of the list
+        to.first = first, to.last = last, to.final_ = at + n == end, to.whole = whole;
+        to.request = x.request, to.rho0 = x.rho0, to.n_rows = x.n_rows, to.kvh = kvh;
+        to.piece0 = start / per, to.piece1 = (start + x.units - 1) / per;
+      }
+      __syncwarp();
+      if (lane == 0) {
+        jb::mbar_arrive(told + 8 * st);
+        if (loads) jb::mbar_expect_tx(full, __popc(loads) * 2 * C::SLABS * KEYS * 128);
+        else jb::mbar_arrive(full);
+      }
+      __syncwarp();
+      if (there) {
+        const int row = (page * a.nkv + kvh) * PAGE + from;
+#pragma unroll
+        for (int h = 0; h < C::SLABS; ++h) {
+          jb::tma_load_2d(stage + (C::SLABS + h) * C::SLAB + lane * KEYS * 128, &map_k, full, h * 64, row);
+          jb::tma_load_2d(stage + h * C::SLAB + lane * KEYS * 128, &map_v, full, h * 64, row);
+        }
+      }
+      if (++st == C::STAGES) st = 0, ++round;
+      at += n, unit += n;
+      if (at < end) {
+        if (unit == x.units) {
+          unit = 0;
+          if (++kvh == a.nkv) {
+            kvh = 0;
+            x = look_up(a, ++block);
+            entered();
+          }
+        }
+        find();
+        page = entry != nullptr ? *entry : -1;
+      }
+    }
+    // gave up: what is still on its way arrives before the block ends (or its wait gives up as well)
+    if (!ok && lane == 0)
+      for (int i = 0; i < C::STAGES; ++i) mbar_wait(kv_full + 8 * i, (i < st ? round : round - 1) & 1, status, 53);
+  } else if (warp == 1) {
+    if (elected()) {
+      const uint32_t idesc_s = jb::instr_desc_bf16(N), idesc_o = jb::instr_desc_bf16(N) | (1u << 15) | (1u << 16);   // values and weights: MN-major
+      const uint32_t o_col = tmem + 2 * N;
+      int st = 0, it = 0, turn = 0;
+      uint32_t phase = 0;
+      bool ok = true, ahead = false;                                   // the stage's scores are under way already
+      auto scores = [&](int stage, int buffer) {
+        const uint32_t k_s = base + stage * C::STAGE + C::SLABS * C::SLAB;
+        jb::tc_fence_after();
+#pragma unroll
+        for (int h = 0; h < C::SLABS; ++h) {
+          const uint64_t k = jb::smem_desc_sw128(k_s + h * C::SLAB), q = jb::smem_desc_sw128(q_at + h * N * 128);
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) jb::umma_bf16(tmem + buffer * N, k + 2 * ks, q + 2 * ks, idesc_s, (h | ks) ? 1u : 0u);
+        }
+        jb::umma_commit(s_full + 8 * buffer);
+      };
+      for (;; ++it) {
+        if (!ahead) {
+          ok = mbar_wait(kv_full + 8 * st, phase, status, 53);
+          if (!ok || info[st].final_ == 2) break;
+          if (info[st].first) ok = mbar_wait(q_full, turn++ & 1, status, 55);
+          if (!ok) break;
+          scores(st, it & 1);
+        }
+        const bool first = info[st].first, last = info[st].last, final_ = info[st].final_;
+        const int st1 = st + 1 == C::STAGES ? 0 : st + 1;
+        const uint32_t phase1 = st1 == 0 ? phase ^ 1 : phase;
+        ahead = false;
+        if (!last && mbar_test(kv_full + 8 * st1, phase1)) {
+          scores(st1, (it + 1) & 1);
+          ahead = true;
+        }
+        ok = mbar_wait(p_full, it & 1, status, 56);
+        if (!ok) break;
+        jb::tc_fence_after();
+        const uint32_t v_s = base + st * C::STAGE;
+#pragma unroll
+        for (int ks = 0; ks < BLOCK_KEYS / 16; ++ks)
+          jb::umma_bf16(o_col, desc_mn_sw128(v_s + ks * 2048, C::SLAB, 1024), desc_mn_sw128(p_at + ks * 2048, BLOCK_KEYS * 128, 1024), idesc_o,
+                        first && ks == 0 ? 0u : 1u);
+        jb::umma_commit(kv_empty + 8 * st);
+        jb::umma_commit(pv_done);
+        if (last) jb::umma_commit(o_full);
+        if (final_) break;
+        st = st1, phase = phase1;
+      }
+    }
+  } else if (warp >= 4) {
+    const int group = (warp - 4) >> 2, quarter = warp & 3, key = quarter * 32 + lane, c0 = group * C::HALF;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    float* my_ref = ref + c0;
+    float l[C::HALF];
+    int st = 0, turn = 0, request = 0, rho0 = 0, n_rows = 0, kvh = 0;
+    uint32_t phase = 0;
+    bool ok = true, first = true;
+    for (int it = 0;; ++it) {
+      // a block of rows begins: its queries, by all eight warps, while its first keys are on their way
+      const Info* x = info + st;
+      if (first) {
+        ok = ok && mbar_wait(told + 8 * st, phase, status, 53);
+        if (group_any(1 + group, !ok)) break;                          // (a wait ran out, of one of the group's warps: all leave)
+        request = x->request, rho0 = x->rho0, n_rows = x->n_rows, kvh = x->kvh;
+        if (x->final_ == 2) break;                                     // (the block has no share)
+        for (int ch = tid - 128; ch < N * C::SLABS * 8; ch += 256) {
+          const int row = ch / (C::SLABS * 8), piece = ch % (C::SLABS * 8), rho = rho0 + row;
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (row < n_rows && piece * 8 < hd)
+            v = *reinterpret_cast<const uint4*>(a.q + (((size_t)request * a.K + rho / G) * a.nh + kvh * G + rho % G) * hd + piece * 8);
+          *reinterpret_cast<uint4*>(smem + C::AT_Q + (piece / 8) * N * 128 + row * 128 + (((piece % 8) ^ (row & 7)) << 4)) = v;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) jb::mbar_arrive(q_full);
+        if (key < C::HALF) my_ref[key] = NOTHING;
+#pragma unroll
+        for (int c = 0; c < C::HALF; ++c) l[c] = 0.0f;
+      }
+      ok = ok && mbar_wait(kv_full + 8 * st, phase, status, 53);
+      if (group_any(1 + group, !ok)) break;
+      const bool last = x->last;
+      const int final_ = x->final_, keys = x->keys[quarter];
+      const bool masked = !x->whole;
+      unsigned long long rows = 0ull;
+      if (masked) {
+        rows = N > 64 ? x->rows[quarter][group] : x->rows[quarter][0] >> c0;
+        if (lane >= keys) rows = 0ull;
+      }
+      ok = ok && mbar_wait(s_full + 8 * (it & 1), (it >> 1) & 1, status, 57);
+      if (it > 0) ok = ok && mbar_wait(pv_done, (it - 1) & 1, status, 58);     // P is free, and O' at rest
+      jb::tc_fence_after();
+      float s[C::HALF];
+#pragma unroll
+      for (int c = 0; c < C::HALF; c += 8) {
+        float v[8];
+        jb::tmem_ld8(lanes + (it & 1) * N + c0 + c, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[c + e] = v[e];
+      }
+      jb::tmem_ld_wait();
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < C::HALF; ++c)
+          if (!((rows >> c) & 1ull)) s[c] = -CUDART_INF_F;
+      }
+      // weights relative to the rows' numbers
+      float high = -CUDART_INF_F;
+#pragma unroll
+      for (int c = 0; c < C::HALF; c += 4) {
+        const float4 r = *reinterpret_cast<const float4*>(my_ref + c);
+        high = fmaxf(high, fmaf(s[c], a.scale_log2, -r.x)), high = fmaxf(high, fmaf(s[c + 1], a.scale_log2, -r.y));
+        high = fmaxf(high, fmaf(s[c + 2], a.scale_log2, -r.z)), high = fmaxf(high, fmaf(s[c + 3], a.scale_log2, -r.w));
+      }
+      if (group_any(1 + group, high > RESCALE_LOG2)) {
+        // the rows' largest scores over the block's keys
+#pragma unroll
+        for (int c = 0; c < C::HALF; ++c) {
+          const float top = jb::warp_max(s[c]);
+          if (lane == 0) swap[quarter * N + c0 + c] = top;
+        }
+        group_any(1 + group, false);
+        float old = 0.0f, now = 0.0f;
+        if (key < C::HALF) {
+          const float* t = swap + c0 + key;
+          old = my_ref[key];
+          now = fmaxf(old, fmaxf(fmaxf(t[0], t[N]), fmaxf(t[2 * N], t[3 * N])) * a.scale_log2);
+        }
+        group_any(1 + group, false);
+        if (key < C::HALF) my_ref[key] = now, swap[c0 + key] = fast_exp2(old - now);
+        group_any(1 + group, false);
+#pragma unroll
+        for (int c = 0; c < C::HALF; c += 8) {
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = swap[c0 + c + e], l[c + e] *= f[e];
+          if (!first) {
+            float v[8];
+            jb::tmem_ld8(lanes + 2 * N + c0 + c, v);
+            jb::tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= f[e];
+            tmem_st8(lanes + 2 * N + c0 + c, v);
+          }
+        }
+        tmem_st_wait();
+      }
+      // values behind the last key: a weight of 0 does not silence what is no number
+      if (masked && lane >= keys && group == 0) {
+#pragma unroll
+        for (int p = 0; p < C::SLABS * 8; ++p)
+          *reinterpret_cast<uint4*>(smem + st * C::STAGE + (p / 8) * C::SLAB + key * 128 + (((p ^ key) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      uint8_t* p_row = smem + C::AT_P + (N > 64 ? group * BLOCK_KEYS * 128 : 0) + key * 128;
+#pragma unroll
+      for (int c = 0; c < C::HALF; c += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 r = *reinterpret_cast<const float2*>(my_ref + c + 2 * e);
+          const float p0 = fast_exp2(fmaf(s[c + 2 * e], a.scale_log2, -r.x)), p1 = fast_exp2(fmaf(s[c + 2 * e + 1], a.scale_log2, -r.y));
+          l[c + 2 * e] += p0, l[c + 2 * e + 1] += p1;
+          w[e] = pack_bf16(p0, p1);
+        }
+        const int piece = (N > 64 ? 0 : c0 / 8) + c / 8;
+        *reinterpret_cast<uint4*>(p_row + ((piece ^ (key & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      const int piece0 = x->piece0, piece1 = x->piece1;                // (read before the stage is given back)
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      jb::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) jb::mbar_arrive(p_full);
+      if (last) {
+        group_any(1 + group, false);                                   // (nobody reads there any longer)
+        // the sums over the keys: half the columns go to the other half of the lanes, and so on, until a lane has one
+        columns_summed<C::HALF>(l, swap + quarter * N + c0);
+        ok = ok && mbar_wait(o_full, turn++ & 1, status, 59);
+        jb::tc_fence_after();
+        group_any(1 + group, false);
+        const int piece = (int)blockIdx.x;
+        const bool complete = piece0 == piece1;
+        const size_t record = ((size_t)piece * 2 + (piece == piece0 ? 1 : 0)) * N;
+        // a thread a row: where its numbers go (times the heads' numbers), and what they are divided by
+        if (key < C::HALF) {
+          const int row = c0 + key, rho = rho0 + row;
+          float* t = swap + c0 + key;
+          const float sum = (t[0] + t[N]) + (t[2 * N] + t[3 * N]);
+          t[0] = complete ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
+          if (row < n_rows) {
+            const int item = (request * a.K + rho / G) * a.nh + kvh * G + rho % G;
+            t[N] = __int_as_float(complete ? item : (int)record + row);
+            if (piece == piece0) a.parts[item] = make_int2(piece0, piece1 - piece0 + 1);
+            if (!complete) a.part_ml[record + row] = make_float2(my_ref[key] > 0.5f * NOTHING ? my_ref[key] : -CUDART_INF_F, sum);
+          }
+        }
+        group_any(1 + group, false);
+#pragma unroll
+        for (int c = 0; c < C::HALF; c += 8) {
+          float v[8];
+          jb::tmem_ld8(lanes + 2 * N + c0 + c, v);
+          jb::tmem_ld_wait();
+          if (key < hd) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int row = c0 + c + e;
+              if (row < n_rows) {
+                const size_t to = (size_t)__float_as_int(swap[N + row]) * hd + key;
+                if (complete) a.out[to] = __float2bfloat16_rn(v[e] * swap[row]);
+                else a.part_o[to] = v[e];
+              }
+            }
+          }
+        }
+        jb::tc_fence_before();
+        group_any(1 + group, false);                                   // (what was exchanged has been read)
+      }
+      first = last;
+      if (final_) break;
+      if (++st == C::STAGES) st = 0, phase ^= 1;
+    }
+  }
+  jb::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    jb::tc_fence_after();
+    jb::tmem_dealloc<C::COLS>(tmem);
+  }
+}
+
 // A warp a (beam, head): the parts of its keys joined, where there are several.
 __global__ void __launch_bounds__(128) beam_attention_join_kernel(const Args a, int rows) {
   jb::pdl_launch_dependents();
@@ -516,29 +1041,57 @@ cudaError_t go(const CUtensorMap* maps, Args a, int blocks, int warps, int* stat
   return cudaLaunchKernelEx(&join.c, beam_attention_join_kernel, a, ROWS * a.team);
 }
 
+template <int HDC, int N>
+cudaError_t tc_go(const CUtensorMap* maps, Args a, int blocks, int* status, cudaStream_t stream) {
+  typedef Tc<HDC, N> C;
+  static bool ready[64] = {};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device >= 64 || !ready[device]) {
+    e = cudaFuncSetAttribute(beam_attention_tc_kernel<HDC, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    if (device < 64) ready[device] = true;
+  }
+  jb::Launch cfg(dim3(blocks), dim3(TC_THREADS), C::SMEM, stream);
+  e = cudaLaunchKernelEx(&cfg.c, beam_attention_tc_kernel<HDC, N>, maps[0], maps[1], a, status);
+  if (e != cudaSuccess) return e;
+  jb::Launch join(dim3((unsigned)(((long long)a.R * a.K * a.nh + 3) / 4)), dim3(128), 0, stream);
+  return cudaLaunchKernelEx(&join.c, beam_attention_join_kernel, a, N);
+}
+template <int HDC>
+cudaError_t tc_for(const CUtensorMap* maps, const Args& a, int blocks, int* status, cudaStream_t stream) {
+  return a.block_rows == 16 ? tc_go<HDC, 16>(maps, a, blocks, status, stream) : a.block_rows == 32 ? tc_go<HDC, 32>(maps, a, blocks, status, stream)
+         : a.block_rows == 64 ? tc_go<HDC, 64>(maps, a, blocks, status, stream) : tc_go<HDC, 128>(maps, a, blocks, status, stream);
+}
+
 }  // namespace
 
-// part: float32 scratch of blocks * warps * 16 * 2 (hd + 2) + 2 R K nh numbers.  blocks, warps of a block, team (warps that work on the same
-// units, a divisor of them): see `ops.beam_attention_plan`.
+// part: float32 scratch of `records` * (hd + 2) + 2 R K nh numbers.  rows: of a block.  Heads of up to 128 numbers: rows 16, 32, 64 or 128, warps
+// and team are not used, records blocks * 2 * rows; larger ones: rows 16 * team, team a divisor of warps, records blocks * warps * 2 * 16.
 JB_EXPORT int jb_attention_beams(const void* q, const void* k_cache, const void* v_cache, void* out, void* part, const int* table,
                                  const int* kv_len, const int* shared, int R, int K, int nh, int nkv, int hd, int W, int n_pages, int blocks,
-                                 int warps, int team, int fewest, float scale, int* status, cudaStream_t stream) {
+                                 int rows, int warps, int team, int fewest, float scale, int* status, cudaStream_t stream) {
   JB_REFUSE(R < 1 || K < 1 || K > MOST_BEAMS || nkv < 1 || nh < nkv || nh % nkv || hd < 8 || hd > 256 || hd % 8 || W < 1 || W > 0x7fffffff / PAGE ||
-                n_pages < 1 || (long long)n_pages * nkv * PAGE > 0x7fffffffLL || blocks < 1 || fewest < 1 || team < 1 || warps < team ||
-                warps % team || warps > (hd > 128 ? Shape<256>::WARPS : Shape<128>::WARPS) || warps / team > (hd > 128 ? 3 : 6) || !(scale > 0.0f),
-            "attention_beams: %d groups of %d beams, %d heads over %d of %d numbers, %d pages a row of %d, plan %d %d %d %d, scale %g", R, K, nh,
-            nkv, hd, W, n_pages, blocks, warps, team, fewest, scale);
+                n_pages < 1 || (long long)n_pages * nkv * PAGE > 0x7fffffffLL || blocks < 1 || fewest < 1 || !(scale > 0.0f),
+            "attention_beams: %d groups of %d beams, %d heads over %d of %d numbers, %d pages a row of %d, %d blocks, scale %g", R, K, nh, nkv, hd,
+            W, n_pages, blocks, scale);
+  if (hd <= 128)
+    JB_REFUSE(rows != 16 && rows != 32 && rows != 64 && rows != 128, "attention_beams: blocks of %d rows", rows);
+  else
+    JB_REFUSE(team < 1 || warps < team || warps % team || warps > Shape<256>::WARPS || warps / team > 3 || rows != ROWS * team,
+              "attention_beams: %d rows for teams of %d of %d warps", rows, team, warps);
   CUtensorMap maps[2];
   if (!jb::make_map_64(&maps[0], k_cache, (uint64_t)n_pages * nkv * PAGE, hd, KEYS, true) ||
       !jb::make_map_64(&maps[1], v_cache, (uint64_t)n_pages * nkv * PAGE, hd, KEYS, true))
     return JB_ERR_TENSORMAP;
   Args a{};
   a.q = (const bf16*)q, a.out = (bf16*)out, a.table = table, a.kv_len = kv_len, a.shared = shared;
-  const size_t records = (size_t)blocks * warps * ROWS * 2;
+  const size_t records = hd <= 128 ? (size_t)blocks * 2 * rows : (size_t)blocks * warps * ROWS * 2;
   a.part_o = (float*)part, a.part_ml = (float2*)(a.part_o + records * hd), a.parts = (int2*)(a.part_ml + records);
   a.R = R, a.K = K, a.nh = nh, a.nkv = nkv, a.hd = hd, a.W = W, a.n_pages = n_pages;
-  a.team = team, a.fewest = fewest, a.scale_log2 = scale * LOG2E;
-  a.row_blocks = (K * (nh / nkv) + ROWS * team - 1) / (ROWS * team);
-  return (int)(hd > 128 ? go<256>(maps, a, blocks, warps, status, stream) : hd > 64 ? go<128>(maps, a, blocks, warps, status, stream)
-                                                                               : go<64>(maps, a, blocks, warps, status, stream));
+  a.team = team, a.fewest = fewest, a.scale_log2 = scale * LOG2E, a.block_rows = rows;
+  a.row_blocks = (K * (nh / nkv) + rows - 1) / rows;
+  return (int)(hd > 128 ? go<256>(maps, a, blocks, warps, status, stream) : hd > 64 ? tc_for<128>(maps, a, blocks, status, stream)
+                                                                               : tc_for<64>(maps, a, blocks, status, stream));
 }

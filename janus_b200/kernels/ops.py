@@ -103,7 +103,7 @@ _SIGNATURES = {
     "jb_step_tables": "pp", "jb_attention_prefix_f32": "ppp", "jb_attention_prefix_bf16": "pppp",
     "jb_verify_drafts": "pp",
     "jb_beam_select": "pp", "jb_fork_pages": "pp", "jb_copy_pages": "pppipppiiip", "jb_reorder_rows": "ppippiiip",
-    "jb_attention_beams": "ppppppppiiiiiiiiiiifpp",
+    "jb_attention_beams": "ppppppppiiiiiiiiiiiifpp",
     "jb_gather_rows": "ppiipppiiip", "jb_latent_attention": "ppppppppiiiiiiifiipp", "jb_attention_tc_matrix": "ppppppiiiiiiiifpipp",
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "u": ctypes.c_ulonglong,
@@ -2857,23 +2857,25 @@ def attention_beams(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                   ("block table", "kv_len", "shared pages"))
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attention_beams: scale {scale}")
-    blocks, warps, team, fewest = beam_attention_plan(N // beams, beams, nh, nkv, hd, min(int(max_kv_len), W * page_size))
-    records = blocks * warps * 16 * 2
+    blocks, rows, warps, team, fewest = beam_attention_plan(N // beams, beams, nh, nkv, hd, min(int(max_kv_len), W * page_size))
+    records = blocks * 2 * (rows if hd <= 128 else 16 * warps)
     part = workspace.get("beam_parts", (records * (hd + 2) + 2 * N * nh,), torch.float32)
     _check(_lib("beam_attention").jb_attention_beams(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), part.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(),
-        shared.data_ptr(), N // beams, beams, nh, nkv, hd, W, k_cache.shape[0], blocks, warps, team, fewest, float(scale),
+        shared.data_ptr(), N // beams, beams, nh, nkv, hd, W, k_cache.shape[0], blocks, rows, warps, team, fewest, float(scale),
         kernel_status(q.device).data_ptr(), _stream()), "attention_beams", kernels=2)
 
 
 @functools.lru_cache(maxsize=4096)
 def beam_attention_plan(groups: int, beams: int, nh: int, nkv: int, hd: int, max_kv_len: int):
-    """How `attention_beams` runs: (blocks, warps of a block, warps of a team, units of 32 keys of a team's share at least)."""
+    """How `attention_beams` runs: (blocks, rows of a block's tile, warps of a block, warps of a team, units of 32 keys of a share at least)."""
     rows = beams * (nh // nkv)
-    team, most = 1, 4 if hd > 128 else 8
-    while team < most and rows > 16 * team:
-        team *= 2
-    teams = min(2 if hd > 128 else 4, most // team)
-    fewest = 2
-    units = groups * -(-rows // (16 * team)) * nkv * -(-max_kv_len // 32) * (beams + 1)      # (at most: nothing may be shared)
-    return max(1, min(SM_COUNT_TARGET // (1 if hd <= 64 else 2), -(-units // (fewest * teams)))), team * teams, team, fewest
+    if hd <= 128:
+        tile = next((n for n in (16, 32, 64) if rows <= n), 128)
+        warps, team, teams, fewest = 0, 1, 1, 4
+    else:
+        team, warps, fewest = 1 if rows <= 16 else 2 if rows <= 32 else 4, 4, 2
+        tile, teams = 16 * team, 2 if team < 4 else 1
+        warps = team * teams
+    units = groups * -(-rows // tile) * nkv * -(-max_kv_len // 32) * (beams + 1)      # (at most: nothing may be shared)
+    return max(1, min(SM_COUNT_TARGET // 2, -(-units // (fewest * teams)))), tile, warps, team, fewest
