@@ -8,10 +8,9 @@
 // the rows of that beam alone.  A softmax over a union of keys joins from (maximum, sum, weighted values), whoever made the parts.
 //
 // Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their units of 32 keys.  Every
-// team of warps has an even, consecutive share of it: the copy engine brings its units (128-byte swizzle) into a ring of the team's
-// own, ahead across the ends of requests.  A warp has 16 rows; a team is as many warps as the rows need, up to eight, all on the same
-// units, the first of which asks for them.  Warp-level products (mma.sync): a request's rows are an eighth to a half of a
-// tensor-core tile.  Where a share ends inside a block of rows, the sums go out as a partial result; a second launch joins those.
+// block of threads (or team of warps) has an even, consecutive share of it, and the copy engine brings its units (128-byte swizzle), ahead
+// across the ends of requests.  Where a share ends inside a block of rows, the sums go out as a partial result; a second launch joins
+// those.
 #include <math_constants.h>
 #include <stdio.h>
 
@@ -43,17 +42,13 @@ struct Args {
 
 constexpr int ROWS = 16;                           // of a warp
 
-template <int HDC>
-struct Shape {
-  static constexpr int SLABS = HDC / 64, SLAB = KEYS * 128;                // 64 numbers of the keys of a unit
+struct Wide {                                      // heads of more than 128 numbers
+  static constexpr int HDC = 256, SLABS = HDC / 64, SLAB = KEYS * 128;     // 64 numbers of the keys of a unit
   static constexpr int TILE = SLABS * SLAB, STAGE = 2 * TILE;              // keys, values
-  static constexpr int STAGES = HDC > 128 ? 6 : 12, RING = STAGES * STAGE;
-  // queries lie in registers, as the products take them, where results leave room for them
-  static constexpr bool Q_REGS = HDC <= 128;
-  static constexpr int Q_SLAB = ROWS * 128, Q = Q_REGS ? 0 : SLABS * Q_SLAB;
-  static constexpr int WARPS = HDC > 128 ? 4 : 8, THREADS = 32 * WARPS;   // at most
-  static constexpr int Q_WARPS = 4;                                        // (at most, where queries lie in shared memory)
-  static constexpr int SMEM = RING + Q_WARPS * Q + STAGES * 24;            // ... and two barriers and a unit's description a stage
+  static constexpr int STAGES = 6, RING = STAGES * STAGE;
+  static constexpr int WARPS = 4, THREADS = 32 * WARPS;                    // at most
+  static constexpr int Q_SLAB = ROWS * 128, Q = SLABS * Q_SLAB;            // a warp's queries
+  static constexpr int SMEM = RING + WARPS * Q + STAGES * 24;              // ... and two barriers and a unit's description a stage
   static_assert(SMEM <= 227 * 1024, "shared memory of a block");
 };
 
@@ -201,16 +196,21 @@ struct Cursor {
   }
 };
 
-template <int HDC>
-__global__ void __launch_bounds__(Shape<HDC>::THREADS, HDC <= 64 ? 2 : 1) beam_attention_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                             const Args a, int* __restrict__ status) {
-  typedef Shape<HDC> C;
+// ---------------------------------------------------------------------------
+// Heads of more than 128 numbers: a team of warps has a share of units of 32 keys, each warp 16 rows, by warp-level products (mma.sync); a stage
+// of 128 keys of tcgen05's tile would take half the shared memory.  The team's first warp asks for units, into a ring of the team's own.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k,
+                                                                               const __grid_constant__ CUtensorMap map_v, const Args a,
+                                                                               int* __restrict__ status) {
+  typedef Wide C;
+  constexpr int HDC = Wide::HDC;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, hd = a.hd, G = a.nh / a.nkv;
   const int T = a.team, here = blockDim.x / 32 / T, team = warp / T, member = warp % T, stages = C::STAGES / here;
   const uint32_t base = jb::smem_u32(smem), ring = base + team * stages * C::STAGE;
-  const uint32_t bars = base + C::RING + C::Q_WARPS * C::Q + team * stages * 16;   // of a stage: full, empty
-  int2* about = reinterpret_cast<int2*>(smem + C::RING + C::Q_WARPS * C::Q + C::STAGES * 16) + team * stages;   // keys, beam
+  const uint32_t bars = base + C::RING + C::WARPS * C::Q + team * stages * 16;   // of a stage: full, empty
+  int2* about = reinterpret_cast<int2*>(smem + C::RING + C::WARPS * C::Q + C::STAGES * 16) + team * stages;   // keys, beam
   if (member == 0 && lane == 0) {
     for (int i = 0; i < stages; ++i) jb::mbar_init(bars + 16 * i, 1), jb::mbar_init(bars + 16 * i + 8, T);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -287,7 +287,6 @@ __global__ void __launch_bounds__(Shape<HDC>::THREADS, HDC <= 64 ? 2 : 1) beam_a
   bool all_join = false;
   int beam_first = 0, beam_last = -1;     // of the warp's rows
   float m[2], l[2], o[HDC / 8][4];
-  uint32_t q[C::Q_REGS ? HDC / 16 : 1][4];
   bool ok = true;
   int st = 0, st_before = 0;
   uint32_t phase = 0, phase_before = 0;
@@ -311,23 +310,13 @@ __global__ void __launch_bounds__(Shape<HDC>::THREADS, HDC <= 64 ? 2 : 1) beam_a
         every = every && (joins[h] || !valid);
         m[h] = -CUDART_INF_F;
         l[h] = 0.0f;
-        if constexpr (C::Q_REGS) {
-          const bf16* src = a.q + (((size_t)x.request * a.K + max(beam_of[h], 0)) * a.nh + kvh * G + (valid ? (rho0 + row) % G : 0)) * hd + 2 * c;
-#pragma unroll
-          for (int ks = 0; ks < HDC / 16; ++ks)
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-              q[ks][h + 2 * half] = valid && ks * 16 + half * 8 < hd ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + half * 8) : 0u;
-        }
       }
-      if constexpr (!C::Q_REGS) {
-        for (int ch = lane; ch < ROWS * C::SLABS * 8; ch += 32) {
-          const int row = ch / (C::SLABS * 8), piece = ch % (C::SLABS * 8), rho = rho0 + row;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (row < n_rows && piece * 8 < hd)
-            v = *reinterpret_cast<const uint4*>(a.q + (((size_t)x.request * a.K + rho / G) * a.nh + kvh * G + rho % G) * hd + piece * 8);
-          *reinterpret_cast<uint4*>(smem + C::RING + warp * C::Q + (piece / 8) * C::Q_SLAB + row * 128 + (((piece % 8) ^ (row & 7)) << 4)) = v;
-        }
+      for (int ch = lane; ch < ROWS * C::SLABS * 8; ch += 32) {
+        const int row = ch / (C::SLABS * 8), piece = ch % (C::SLABS * 8), rho = rho0 + row;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < n_rows && piece * 8 < hd)
+          v = *reinterpret_cast<const uint4*>(a.q + (((size_t)x.request * a.K + rho / G) * a.nh + kvh * G + rho % G) * hd + piece * 8);
+        *reinterpret_cast<uint4*>(smem + C::RING + warp * C::Q + (piece / 8) * C::Q_SLAB + row * 128 + (((piece % 8) ^ (row & 7)) << 4)) = v;
       }
 #pragma unroll
       for (int j = 0; j < HDC / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
@@ -359,12 +348,7 @@ __global__ void __launch_bounds__(Shape<HDC>::THREADS, HDC <= 64 ? 2 : 1) beam_a
         const uint32_t at = k_t + (k_lane ^ ((ks % 4) << 5)) + (ks / 4) * C::SLAB;
         ldmatrix_x4(b[0], at);
         ldmatrix_x4(b[1], at + 16 * 128);
-        if constexpr (C::Q_REGS) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qa[e] = q[ks][e];
-        } else {
-          ldmatrix_x4(qa, q_at + (v_lane ^ ((ks % 4) << 5)) + (ks / 4) * C::Q_SLAB);
-        }
+        ldmatrix_x4(qa, q_at + (v_lane ^ ((ks % 4) << 5)) + (ks / 4) * C::Q_SLAB);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           mma_bf16(ks & 1 ? s_odd[2 * j] : s[2 * j], qa, b[j][0], b[j][1]);
@@ -991,73 +975,122 @@ __global__ void __launch_bounds__(TC_THREADS, 1) beam_attention_tc_kernel(const 
   }
 }
 
-// A warp a (beam, head): the parts of its keys joined, where there are several.
-__global__ void __launch_bounds__(128) beam_attention_join_kernel(const Args a, int rows) {
+// The parts of a (beam, head)'s keys joined, where there are several, by PER warps, each of which takes every PER-th, several on their way at
+// a time.
+constexpr int JOIN_WARPS = 4;
+template <int PER>
+__global__ void __launch_bounds__(32 * JOIN_WARPS) beam_attention_join_kernel(const Args a, int rows) {
+  __shared__ float4 sums[PER > 1 ? PER : 1][PER > 1 ? 64 : 1];
+  __shared__ float2 ml_of[PER];
   jb::pdl_launch_dependents();
   jb::pdl_wait();
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, G = a.nh / a.nkv;
-  if (item >= (long long)a.R * a.K * a.nh) return;
+  const int item = blockIdx.x * (JOIN_WARPS / PER) + (threadIdx.x >> 5) / PER, warp = (threadIdx.x >> 5) % PER, lane = threadIdx.x & 31;
+  const int G = a.nh / a.nkv;
+  if (item >= a.R * a.K * a.nh) return;
   const int2 parts = a.parts[item];
   if (parts.y <= 1) return;
-  const int head = (int)(item % a.nh), beam = (int)(item / a.nh % a.K), row = (beam * G + head % G) % rows;
+  const int head = item % a.nh, beam = item / a.nh % a.K, row = (beam * G + head % G) % rows;
   auto record = [&](int p) { return ((size_t)(parts.x + p) * 2 + (p == 0 ? 1 : 0)) * rows + row; };
-  float most = -CUDART_INF_F;
-  for (int p = lane; p < parts.y; p += 32) most = fmaxf(most, a.part_ml[record(p)].x);
-  most = jb::warp_max(most);
-  const float use = most == -CUDART_INF_F ? 0.0f : most;
-  for (int d = lane * 4; d < a.hd; d += 128) {
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float sum = 0.0f;
-#pragma unroll 4
-    for (int p = 0; p < parts.y; ++p) {
-      const float2 ml = a.part_ml[record(p)];
-      const float4 v = *reinterpret_cast<const float4*>(a.part_o + record(p) * a.hd + d);
-      const float f = fast_exp2(ml.x - use);
-      sum = fmaf(f, ml.y, sum);
-      o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+  constexpr int AHEAD = 4;
+  float4 o[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+  float most = -CUDART_INF_F, sum = 0.0f;
+  for (int p0 = warp; p0 < parts.y; p0 += PER * AHEAD) {
+    float2 ml[AHEAD];
+    float4 v[AHEAD][2];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int p = p0 + u * PER;
+      ml[u] = make_float2(-CUDART_INF_F, 0.0f);
+      v[u][0] = v[u][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (p < parts.y) {
+        const float* from = a.part_o + record(p) * a.hd;
+        ml[u] = a.part_ml[record(p)];
+        if (lane * 4 < a.hd) v[u][0] = *reinterpret_cast<const float4*>(from + lane * 4);
+        if (lane * 4 + 128 < a.hd) v[u][1] = *reinterpret_cast<const float4*>(from + lane * 4 + 128);
+      }
     }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const float top = fmaxf(most, ml[u].x);
+      if (top == -CUDART_INF_F) continue;
+      const float f = fast_exp2(most - top), g = fast_exp2(ml[u].x - top);
+      most = top;
+      sum = fmaf(sum, f, g * ml[u].y);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        o[h].x = fmaf(o[h].x, f, g * v[u][h].x), o[h].y = fmaf(o[h].y, f, g * v[u][h].y);
+        o[h].z = fmaf(o[h].z, f, g * v[u][h].z), o[h].w = fmaf(o[h].w, f, g * v[u][h].w);
+      }
+    }
+  }
+  if constexpr (PER == 1) {
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    *reinterpret_cast<uint2*>(a.out + item * a.hd + d) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (lane * 4 + 128 * h < a.hd)
+        *reinterpret_cast<uint2*>(a.out + (size_t)item * a.hd + lane * 4 + 128 * h) =
+            make_uint2(pack_bf16(o[h].x * inv, o[h].y * inv), pack_bf16(o[h].z * inv, o[h].w * inv));
+  } else {
+    static_assert(PER == JOIN_WARPS, "a block's barrier");
+    if (lane == 0) ml_of[warp] = make_float2(most, sum);
+    sums[warp][lane] = o[0], sums[warp][32 + lane] = o[1];
+    __syncthreads();
+    float top = -CUDART_INF_F, all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < PER; ++w) top = fmaxf(top, ml_of[w].x);
+    const float use = top == -CUDART_INF_F ? 0.0f : top;
+    float f[PER];
+#pragma unroll
+    for (int w = 0; w < PER; ++w) f[w] = fast_exp2(ml_of[w].x - use), all = fmaf(f[w], ml_of[w].y, all);
+    const float inv = all > 0.0f ? 1.0f / all : 0.0f;
+    for (int d = threadIdx.x; d < a.hd; d += 32 * JOIN_WARPS) {
+      float t = 0.0f;
+#pragma unroll
+      for (int w = 0; w < PER; ++w) t = fmaf(f[w], reinterpret_cast<const float*>(sums[w])[d], t);
+      a.out[(size_t)item * a.hd + d] = __float2bfloat16_rn(t * inv);
+    }
   }
 }
 
-template <int HDC>
-cudaError_t go(const CUtensorMap* maps, Args a, int blocks, int warps, int* status, cudaStream_t stream) {
-  typedef Shape<HDC> C;
-  static bool ready[64] = {};
+// The kernel's shared memory, asked for once a device.
+template <typename Kernel>
+cudaError_t allow(Kernel kernel, int bytes, bool (&ready)[64]) {
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
-  if (e != cudaSuccess) return e;
-  if (device >= 64 || !ready[device]) {
-    e = cudaFuncSetAttribute(beam_attention_kernel<HDC>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return e;
-    if (device < 64) ready[device] = true;
+  if (e != cudaSuccess || (device < 64 && ready[device])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && device < 64) ready[device] = true;
+  return e;
+}
+// `shares`: of the list, how many.  A block of rows that is cut into many parts has a block of warps a row (6 requests of 5 beams that parted
+// long ago, 12 to a block of rows: 20 us the call, 23 by a warp a row), others a warp (16 of 8 beams behind 6,000 to 24,000: 105 and 109).
+cudaError_t join(const Args& a, int rows, int shares, cudaStream_t stream) {
+  const int items = a.R * a.K * a.nh;
+  if (shares > 4 * a.R * a.row_blocks * a.nkv) {
+    jb::Launch cfg(dim3(items), dim3(32 * JOIN_WARPS), 0, stream);
+    return cudaLaunchKernelEx(&cfg.c, beam_attention_join_kernel<JOIN_WARPS>, a, rows);
   }
-  jb::Launch cfg(dim3(blocks), dim3(32 * warps), C::SMEM, stream);
-  e = cudaLaunchKernelEx(&cfg.c, beam_attention_kernel<HDC>, maps[0], maps[1], a, status);
+  jb::Launch cfg(dim3((items + JOIN_WARPS - 1) / JOIN_WARPS), dim3(32 * JOIN_WARPS), 0, stream);
+  return cudaLaunchKernelEx(&cfg.c, beam_attention_join_kernel<1>, a, rows);
+}
+cudaError_t wide_go(const CUtensorMap* maps, const Args& a, int blocks, int warps, int* status, cudaStream_t stream) {
+  static bool ready[64] = {};
+  cudaError_t e = allow(beam_attention_wide_kernel, Wide::SMEM, ready);
   if (e != cudaSuccess) return e;
-  jb::Launch join(dim3((unsigned)(((long long)a.R * a.K * a.nh + 3) / 4)), dim3(128), 0, stream);
-  return cudaLaunchKernelEx(&join.c, beam_attention_join_kernel, a, ROWS * a.team);
+  jb::Launch cfg(dim3(blocks), dim3(32 * warps), Wide::SMEM, stream);
+  e = cudaLaunchKernelEx(&cfg.c, beam_attention_wide_kernel, maps[0], maps[1], a, status);
+  return e != cudaSuccess ? e : join(a, a.block_rows, blocks * (warps / a.team), stream);
 }
 
 template <int HDC, int N>
 cudaError_t tc_go(const CUtensorMap* maps, Args a, int blocks, int* status, cudaStream_t stream) {
   typedef Tc<HDC, N> C;
   static bool ready[64] = {};
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
+  cudaError_t e = allow(beam_attention_tc_kernel<HDC, N>, C::SMEM, ready);
   if (e != cudaSuccess) return e;
-  if (device >= 64 || !ready[device]) {
-    e = cudaFuncSetAttribute(beam_attention_tc_kernel<HDC, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return e;
-    if (device < 64) ready[device] = true;
-  }
   jb::Launch cfg(dim3(blocks), dim3(TC_THREADS), C::SMEM, stream);
   e = cudaLaunchKernelEx(&cfg.c, beam_attention_tc_kernel<HDC, N>, maps[0], maps[1], a, status);
-  if (e != cudaSuccess) return e;
-  jb::Launch join(dim3((unsigned)(((long long)a.R * a.K * a.nh + 3) / 4)), dim3(128), 0, stream);
-  return cudaLaunchKernelEx(&join.c, beam_attention_join_kernel, a, N);
+  return e != cudaSuccess ? e : join(a, N, blocks, stream);
 }
 template <int HDC>
 cudaError_t tc_for(const CUtensorMap* maps, const Args& a, int blocks, int* status, cudaStream_t stream) {
@@ -1073,13 +1106,13 @@ JB_EXPORT int jb_attention_beams(const void* q, const void* k_cache, const void*
                                  const int* kv_len, const int* shared, int R, int K, int nh, int nkv, int hd, int W, int n_pages, int blocks,
                                  int rows, int warps, int team, int fewest, float scale, int* status, cudaStream_t stream) {
   JB_REFUSE(R < 1 || K < 1 || K > MOST_BEAMS || nkv < 1 || nh < nkv || nh % nkv || hd < 8 || hd > 256 || hd % 8 || W < 1 || W > 0x7fffffff / PAGE ||
-                n_pages < 1 || (long long)n_pages * nkv * PAGE > 0x7fffffffLL || blocks < 1 || fewest < 1 || !(scale > 0.0f),
+                n_pages < 1 || (long long)R * K * nh > 0x7fffffffLL || (long long)n_pages * nkv * PAGE > 0x7fffffffLL || blocks < 1 || fewest < 1 || !(scale > 0.0f),
             "attention_beams: %d groups of %d beams, %d heads over %d of %d numbers, %d pages a row of %d, %d blocks, scale %g", R, K, nh, nkv, hd,
             W, n_pages, blocks, scale);
   if (hd <= 128)
     JB_REFUSE(rows != 16 && rows != 32 && rows != 64 && rows != 128, "attention_beams: blocks of %d rows", rows);
   else
-    JB_REFUSE(team < 1 || warps < team || warps % team || warps > Shape<256>::WARPS || warps / team > 3 || rows != ROWS * team,
+    JB_REFUSE(team < 1 || warps < team || warps % team || warps > Wide::WARPS || warps / team > 3 || rows != ROWS * team,
               "attention_beams: %d rows for teams of %d of %d warps", rows, team, warps);
   CUtensorMap maps[2];
   if (!jb::make_map_64(&maps[0], k_cache, (uint64_t)n_pages * nkv * PAGE, hd, KEYS, true) ||
@@ -1092,6 +1125,6 @@ JB_EXPORT int jb_attention_beams(const void* q, const void* k_cache, const void*
   a.R = R, a.K = K, a.nh = nh, a.nkv = nkv, a.hd = hd, a.W = W, a.n_pages = n_pages;
   a.team = team, a.fewest = fewest, a.scale_log2 = scale * LOG2E, a.block_rows = rows;
   a.row_blocks = (K * (nh / nkv) + rows - 1) / rows;
-  return (int)(hd > 128 ? go<256>(maps, a, blocks, warps, status, stream) : hd > 64 ? tc_for<128>(maps, a, blocks, status, stream)
+  return (int)(hd > 128 ? wide_go(maps, a, blocks, warps, status, stream) : hd > 64 ? tc_for<128>(maps, a, blocks, status, stream)
                                                                                : tc_for<64>(maps, a, blocks, status, stream));
 }
