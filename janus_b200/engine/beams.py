@@ -324,8 +324,13 @@ class BeamRunner:
         cache, R, K = engine.cache, len(prompts), beams
         slots: List[int] = []
         mine: List[List[int]] = [[] for _ in cache.groups]
+        # rows without a beam use a page that is taken first and given back last, so that it is the same one batch after batch: a
+        # captured step knows it by number
+        spare: List[int] = []
         try:
             t0 = time.perf_counter()
+            for group in cache.groups:
+                spare.append(group.pool.take())
             for _ in range(R * K):
                 slots.append(engine.alloc_slot())
             step = self._step_for(R, K, max(-(-(len(p) + q.limit) // PAGE_SIZE) for p, q in zip(prompts, searches)), len(stop))
@@ -339,11 +344,11 @@ class BeamRunner:
                 step.logits[i * K].copy_(row)
             own = sum(beam_pages(len(p), q.limit) for p, q in zip(prompts, searches)) * K
             for g, group in enumerate(cache.groups):
-                for _ in range(own + 1):
+                for _ in range(own):
                     mine[g].append(group.pool.take())
             pages = [[g.pages[s] for s in heads] for g in cache.groups]
             if cache.groups:
-                step.begin(slots, [len(p) for p in prompts], pages, [m[1:] for m in mine], [m[0] for m in mine], stop)
+                step.begin(slots, [len(p) for p in prompts], pages, mine, spare, stop)
             else:                                            # pages of no storage: 0 spare, then the prompts', then the beams'
                 counts = [-(-len(p) // PAGE_SIZE) for p in prompts]
                 at = np.concatenate([[1], 1 + np.cumsum(counts)])
@@ -358,10 +363,12 @@ class BeamRunner:
         finally:
             torch.cuda.synchronize(engine.device)
             for group, pages in zip(cache.groups, mine):
-                for p in pages:
+                for p in reversed(pages):
                     group.pool.give_back(p)
             for s in slots:
                 engine.free_slot(s)
+            for group, p in zip(cache.groups, spare):
+                group.pool.give_back(p)
 
     def _search(self, step: _BeamStep, searches: List[_Search], K: int, length_penalty: float, early_stopping: bool, stats) -> None:
         """Steps until every request is done.  A step is launched before the host has read what the one before chose; a request that turns out

@@ -185,7 +185,8 @@ class GQAttention(Mixer):
     def _beams_share_pages(self, ctx, group) -> bool:
         """Whether a step of beam search reads pages that beams share once for all of them."""
         return (getattr(ctx, "beams", 0) > 1 and getattr(group, "shared", None) is not None and self.dtype == torch.bfloat16
-                and self.window == 0 and self.hd % 8 == 0)
+                and self.window == 0 and self.hd % 8 == 0
+                and ops.beams_pay(ctx.n_seqs, self.nkv, self.hd, ctx.max_kv_len_bound))
 
     def _attend_prompt(self, q: torch.Tensor, residual: torch.Tensor, ctx, cache_view) -> None:
         """bfloat16 attention of several new tokens per sequence over the cache (either dtype, where the sequences share a prefix),

@@ -218,10 +218,15 @@ def test_long_texts_cross_pages_and_batches_follow_one_another():
 
 
 @gpu
+@pytest.mark.parametrize("shared", [True, False])
 @pytest.mark.parametrize("name", ["llama A", "llama B", "zivitar A", "mugedra A"])
-def test_bfloat16_scores_are_the_texts_own(name):
-    """bfloat16: logits of a text by single tokens and by a prompt differ by the engine's tolerance (3e-2 of the largest), every token's
-    log-probability by twice that at most."""
+def test_bfloat16_scores_are_the_texts_own(name, shared, monkeypatch):
+    """bfloat16, with pages that beams share read once for all and by every row: logits of a text by single tokens and by a prompt differ by the
+    engine's tolerance (3e-2 of the largest), every token's log-probability by twice that at most."""
+    from janus_b200.kernels import ops
+    calls, attention = [], ops.attention_beams
+    monkeypatch.setattr(ops, "beams_pay", lambda *sizes: shared)
+    monkeypatch.setattr(ops, "attention_beams", lambda *a, **kw: (calls.append(1), attention(*a, **kw)))
     model = random_model(DESIGNS[name], "bfloat16")
     V = model.engine.model.vocab_size
     prompts = [random_tokens(n, V, n) for n in (200, 64, 9)]
@@ -233,6 +238,7 @@ def test_bfloat16_scores_are_the_texts_own(name):
             rows = torch.cat([by_prompts(model, prompt)([t.tokens[:i]]) for i in range(len(t.tokens))]).double()
             want = float(rows.log_softmax(1).gather(1, torch.tensor(t.tokens)[:, None]).sum())
             assert abs(want - t.score) <= 30 * 2 * 3e-2 * float(rows.abs().max())
+    assert bool(calls) == (shared and name.startswith("llama"))
 
 
 @gpu
@@ -259,6 +265,20 @@ def test_with_and_without_graphs():
         out.append([[(t.tokens, t.reason) for t in row] for row in texts])
         assert (stats.graph_captures > 0) == graphs
     assert out[0] == out[1]
+
+
+@gpu
+def test_a_captured_step_serves_later_calls():
+    """Batches of as many requests and beams, lengths up to as many pages (a power of two) and no more prompt tokens record one step."""
+    model = random_model(LLAMA_C, "float32")
+    first = [random_tokens(n, 256, n) for n in (90, 20)]
+    _, stats = model.generate_beams(first, beams=4, max_tokens=30, ignore_eos=True)
+    assert stats.graph_captures == 1
+    for lengths in ((30, 70), (3, 98)):
+        prompts = [random_tokens(n, 256, n) for n in lengths]
+        got, stats = model.generate_beams(prompts, beams=4, max_tokens=30, ignore_eos=True)
+        assert stats.graph_captures == 0
+        assert got == random_model(LLAMA_C, "float32").generate_beams(prompts, beams=4, max_tokens=30, ignore_eos=True)[0]
 
 
 @gpu
