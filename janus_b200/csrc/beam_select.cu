@@ -9,7 +9,9 @@
 // exponentials.  In the second a block a beam finds the beam's K best: the K-th largest of the threads' maxima bounds the K-th largest
 // logit of the row from below, and only the few threads' numbers at or above it are looked at again (from L2).  The third, a block a
 // request, joins its beams.  64 requests of 8 beams over 128,256 tokens: 59 us, the first 45.  (With the second step done by each block
-// of the first launch 63 us: memory stood still meanwhile; with a warp a beam in the third 76.)
+// of the first launch 63 us: memory stood still meanwhile; with a warp a beam in the third 76.  With fewer launches, the last block of a
+// row or of a request going on by a ticket: 61 by two, 65 by one, whose blocks that only read are fewer at a time; one request 12.8
+// and 13.6 us, by three 11.8.)
 // Within a beam the order is that of the logits (equal ones: the lowest token first), which no rounding touches; between beams it is
 // that of the totals, whose sum of exponentials is taken to 64 bits where threads meet: 32 bits would turn two beams round now and
 // then.
