@@ -95,7 +95,7 @@ __global__ void __cluster_dims__(FORK_BLOCKS, 1, 1) __launch_bounds__(FORK_THREA
   // A warp has 32 columns of a group; lane k knows row k: which it goes on with, and how many pages the two hold.
   const int tiles = (W + 31) / 32;
   bool counts_ready = false;
-  for (long long tile = thread >> 5;; tile += ALL / 32) {
+  for (long long tile = thread >> 5; !counts_ready || tile < (long long)a.R * tiles; tile += ALL / 32) {
     const bool there = tile < (long long)a.R * tiles;
     const int r = there ? (int)(tile / tiles) : 0, c = there ? (int)(tile % tiles) * 32 + lane : W, row0 = r * K;
     const int parent = lane < K ? a.parents[row0 + lane] : -1, length = lane < K ? max(a.lengths[row0 + lane], 0) : 0;
@@ -146,11 +146,15 @@ __global__ void __cluster_dims__(FORK_BLOCKS, 1, 1) __launch_bounds__(FORK_THREA
         const int held = c < __shfl_sync(0xffffffffu, pages_was, k) ? was[k] : -1;
         if (now[k] != held && counted(now[k])) atomicAdd(&a.new_refs[now[k]], 1);
       }
+      int before[KM];                                    // (all are under way before the first answer is looked at)
 #pragma unroll
       for (int k = 0; k < KM; ++k) {
         const int held = c < __shfl_sync(0xffffffffu, pages_was, k) ? was[k] : -1;
-        if (now[k] != held && counted(held) && atomicSub(&a.new_refs[held], 1) == 1) atomicOr(&bits0[held >> 5], 1u << (held & 31));
+        before[k] = now[k] != held && counted(held) ? atomicSub(&a.new_refs[held], 1) : 0;
       }
+#pragma unroll
+      for (int k = 0; k < KM; ++k)
+        if (before[k] == 1) atomicOr(&bits0[was[k] >> 5], 1u << (was[k] & 31));
     }
 #pragma unroll
     for (int k = 0; k < KM; ++k)
