@@ -459,12 +459,11 @@ __global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(c
 // request's few rows are no padding:  S' = K Q' and O' = V' P', both accumulated in tensor memory.
 //   warp 0       walks the block's share of the list and brings its units, four (128 keys) a stage, by the copy engine
 //   warp 1       one lane issues the products; the next stage's scores before this one's values, where its keys are there
-//   warps 4-11   two groups of four, each with half the columns: a thread has one key.  Weights relative to a number a row that is raised
+//   warps 4-     two or four groups of four, each with its columns: a thread has one key.  Weights relative to a number a row that is raised
 //                only when a score passes it by RESCALE_LOG2 (then the sums and O' are scaled down); P to shared memory, a row a key
 // A stage's units may be different beams' own; a mask of rows goes with each.
 // ---------------------------------------------------------------------------
 constexpr int SUB = 4, BLOCK_KEYS = SUB * KEYS;              // units of a stage
-constexpr int TC_THREADS = 384;
 constexpr float NOTHING = -1e30f;                            // what weights are relative to before a row has seen a key
 
 struct Info {                                                // of a stage
@@ -484,7 +483,8 @@ struct Tc {
   static constexpr int AT_Q = STAGES * STAGE, AT_P = AT_Q + Q, AT_REF = AT_P + P, AT_SWAP = AT_REF + 4 * N, AT_INFO = AT_SWAP + 16 * N,
                        AT_BARS = AT_INFO + STAGES * (int)sizeof(Info), SMEM = AT_BARS + (3 * STAGES + 6) * 8 + 16;
   static constexpr int COLS = 3 * N <= 64 ? 64 : 3 * N <= 128 ? 128 : 3 * N <= 256 ? 256 : 512;  // two S', one O'
-  static constexpr int HALF = N / 2;                         // columns of a group of warps
+  static constexpr int GROUPS = N > 32 ? 4 : 2, HALF = N / GROUPS;      // groups of four warps, columns of each
+  static constexpr int WARPS = 4 * GROUPS, THREADS = 128 + 32 * WARPS;
   static_assert(STAGES >= 2 && SMEM <= 232448, "shared memory of a block");
 };
 
@@ -579,7 +579,7 @@ __device__ __forceinline__ void columns_summed(const float (&v)[C], float* out) 
 }
 
 template <int HDC, int N>
-__global__ void __launch_bounds__(TC_THREADS, 1) beam_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                         const __grid_constant__ CUtensorMap map_v, const Args a,
                                                                         int* __restrict__ status) {
   typedef Tc<HDC, N> C;
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) beam_attention_tc_kernel(const 
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::AT_BARS + (3 * C::STAGES + 6) * 8);
   if (tid == 0) {
     for (int i = 0; i < C::STAGES; ++i) jb::mbar_init(kv_full + 8 * i, 1), jb::mbar_init(kv_empty + 8 * i, 1), jb::mbar_init(told + 8 * i, 1);
-    jb::mbar_init(s_full, 1), jb::mbar_init(s_full + 8, 1), jb::mbar_init(p_full, 8), jb::mbar_init(pv_done, 1), jb::mbar_init(q_full, 8);
+    jb::mbar_init(s_full, 1), jb::mbar_init(s_full + 8, 1), jb::mbar_init(p_full, C::WARPS), jb::mbar_init(pv_done, 1), jb::mbar_init(q_full, C::WARPS);
     jb::mbar_init(o_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) beam_attention_tc_kernel(const 
   jb::pdl_wait();
   // ---- the list's length: a thread's blocks of rows, then all threads' ----
   int* sums = reinterpret_cast<int*>(smem + C::AT_P);                  // (P is not there yet)
-  const int blocks = a.R * a.row_blocks, chunk = (blocks + TC_THREADS - 1) / TC_THREADS;
+  const int blocks = a.R * a.row_blocks, chunk = (blocks + C::THREADS - 1) / C::THREADS;
   {
     int mine = 0;
     for (int i = tid * chunk; i < min((tid + 1) * chunk, blocks); ++i) mine += count_units(a, i);
@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) beam_attention_tc_kernel(const 
   jb::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   if (warp == 0) {
-    constexpr int EACH = TC_THREADS / 32;
+    constexpr int EACH = C::THREADS / 32;
     int mine = 0;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) mine += sums[lane * EACH + i];
@@ -804,14 +804,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) beam_attention_tc_kernel(const 
     uint32_t phase = 0;
     bool ok = true, first = true;
     for (int it = 0;; ++it) {
-      // a block of rows begins: its queries, by all eight warps, while its first keys are on their way
+      // a block of rows begins: its queries, by all groups, while its first keys are on their way
       const Info* x = info + st;
       if (first) {
         ok = ok && mbar_wait(told + 8 * st, phase, status, 53);
         if (group_any(1 + group, !ok)) break;                          // (a wait ran out, of one of the group's warps: all leave)
         request = x->request, rho0 = x->rho0, n_rows = x->n_rows, kvh = x->kvh;
         if (x->final_ == 2) break;                                     // (the block has no share)
-        for (int ch = tid - 128; ch < N * C::SLABS * 8; ch += 256) {
+        for (int ch = tid - 128; ch < N * C::SLABS * 8; ch += 32 * C::WARPS) {
           const int row = ch / (C::SLABS * 8), piece = ch % (C::SLABS * 8), rho = rho0 + row;
           uint4 v = make_uint4(0u, 0u, 0u, 0u);
           if (row < n_rows && piece * 8 < hd)
@@ -832,36 +832,41 @@ __global__ void __launch_bounds__(TC_THREADS, 1) beam_attention_tc_kernel(const 
       const bool masked = !x->whole;
       unsigned long long rows = 0ull;
       if (masked) {
-        rows = N > 64 ? x->rows[quarter][group] : x->rows[quarter][0] >> c0;
+        rows = x->rows[quarter][c0 / 64] >> (c0 % 64);
         if (lane >= keys) rows = 0ull;
       }
       ok = ok && mbar_wait(s_full + 8 * (it & 1), (it >> 1) & 1, status, 57);
       if (it > 0) ok = ok && mbar_wait(pv_done, (it - 1) & 1, status, 58);     // P is free, and O' at rest
       jb::tc_fence_after();
       float s[C::HALF];
+      auto scores = [&]() {
 #pragma unroll
-      for (int c = 0; c < C::HALF; c += 8) {
-        float v[8];
-        jb::tmem_ld8(lanes + (it & 1) * N + c0 + c, v);
+        for (int c = 0; c < C::HALF; c += 8) {
+          float v[8];
+          jb::tmem_ld8(lanes + (it & 1) * N + c0 + c, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[c + e] = v[e];
-      }
-      jb::tmem_ld_wait();
-      if (masked) {
+          for (int e = 0; e < 8; ++e) s[c + e] = v[e];
+        }
+        jb::tmem_ld_wait();
+        if (masked) {
 #pragma unroll
-        for (int c = 0; c < C::HALF; ++c)
-          if (!((rows >> c) & 1ull)) s[c] = -CUDART_INF_F;
-      }
-      // weights relative to the rows' numbers
+          for (int c = 0; c < C::HALF; ++c)
+            if (!((rows >> c) & 1ull)) s[c] = -CUDART_INF_F;
+        }
+      };
+      scores();
+      // powers relative to the rows' numbers
       float high = -CUDART_INF_F;
 #pragma unroll
       for (int c = 0; c < C::HALF; c += 4) {
         const float4 r = *reinterpret_cast<const float4*>(my_ref + c);
-        high = fmaxf(high, fmaf(s[c], a.scale_log2, -r.x)), high = fmaxf(high, fmaf(s[c + 1], a.scale_log2, -r.y));
-        high = fmaxf(high, fmaf(s[c + 2], a.scale_log2, -r.z)), high = fmaxf(high, fmaf(s[c + 3], a.scale_log2, -r.w));
+        s[c] = fmaf(s[c], a.scale_log2, -r.x), s[c + 1] = fmaf(s[c + 1], a.scale_log2, -r.y);
+        s[c + 2] = fmaf(s[c + 2], a.scale_log2, -r.z), s[c + 3] = fmaf(s[c + 3], a.scale_log2, -r.w);
+        high = fmaxf(high, fmaxf(fmaxf(s[c], s[c + 1]), fmaxf(s[c + 2], s[c + 3])));
       }
       if (group_any(1 + group, high > RESCALE_LOG2)) {
-        // the rows' largest scores over the block's keys
+        // the rows' largest over the block's keys
+        scores();
 #pragma unroll
         for (int c = 0; c < C::HALF; ++c) {
           const float top = jb::warp_max(s[c]);
@@ -881,7 +886,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) beam_attention_tc_kernel(const 
         for (int c = 0; c < C::HALF; c += 8) {
           float f[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = swap[c0 + c + e], l[c + e] *= f[e];
+          for (int e = 0; e < 8; ++e) {
+            s[c + e] = fmaf(s[c + e], a.scale_log2, -my_ref[c + e]);
+            f[e] = swap[c0 + c + e], l[c + e] *= f[e];
+          }
           if (!first) {
             float v[8];
             jb::tmem_ld8(lanes + 2 * N + c0 + c, v);
@@ -899,18 +907,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) beam_attention_tc_kernel(const 
         for (int p = 0; p < C::SLABS * 8; ++p)
           *reinterpret_cast<uint4*>(smem + st * C::STAGE + (p / 8) * C::SLAB + key * 128 + (((p ^ key) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
       }
-      uint8_t* p_row = smem + C::AT_P + (N > 64 ? group * BLOCK_KEYS * 128 : 0) + key * 128;
+      uint8_t* p_row = smem + C::AT_P + (c0 / 64) * BLOCK_KEYS * 128 + key * 128;
 #pragma unroll
       for (int c = 0; c < C::HALF; c += 8) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 r = *reinterpret_cast<const float2*>(my_ref + c + 2 * e);
-          const float p0 = fast_exp2(fmaf(s[c + 2 * e], a.scale_log2, -r.x)), p1 = fast_exp2(fmaf(s[c + 2 * e + 1], a.scale_log2, -r.y));
+          const float p0 = fast_exp2(s[c + 2 * e]), p1 = fast_exp2(s[c + 2 * e + 1]);
           l[c + 2 * e] += p0, l[c + 2 * e + 1] += p1;
           w[e] = pack_bf16(p0, p1);
         }
-        const int piece = (N > 64 ? 0 : c0 / 8) + c / 8;
+        const int piece = (c0 % 64 + c) / 8;
         *reinterpret_cast<uint4*>(p_row + ((piece ^ (key & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
       const int piece0 = x->piece0, piece1 = x->piece1;                // (read before the stage is given back)
@@ -1088,7 +1095,7 @@ cudaError_t tc_go(const CUtensorMap* maps, Args a, int blocks, int* status, cuda
   static bool ready[64] = {};
   cudaError_t e = allow(beam_attention_tc_kernel<HDC, N>, C::SMEM, ready);
   if (e != cudaSuccess) return e;
-  jb::Launch cfg(dim3(blocks), dim3(TC_THREADS), C::SMEM, stream);
+  jb::Launch cfg(dim3(blocks), dim3(C::THREADS), C::SMEM, stream);
   e = cudaLaunchKernelEx(&cfg.c, beam_attention_tc_kernel<HDC, N>, maps[0], maps[1], a, status);
   return e != cudaSuccess ? e : join(a, N, blocks, stream);
 }
