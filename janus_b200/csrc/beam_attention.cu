@@ -20,7 +20,8 @@ namespace {
 
 typedef __nv_bfloat16 bf16;
 
-constexpr int PAGE = 64, KEYS = 32;                // keys of a page, of a unit
+constexpr int PAGE = 64;
+constexpr int KEYS = 32;                           // keys of a unit with heads of more than 128 numbers; below that a unit is a page
 constexpr int MOST_BEAMS = 32;
 constexpr float RESCALE_LOG2 = 8.0f;               // weights may grow to 2^8 before what was summed up is scaled down
 constexpr float LOG2E = 1.4426950408889634f;
@@ -97,6 +98,7 @@ struct Rows {
   int len, first, own, upto;        // of the lane's beam: keys, first page of its own, units of its own, of the beams up to it
 };
 
+template <int KEYS>
 __device__ __forceinline__ Rows look_up(const Args& a, int block) {
   const int lane = threadIdx.x & 31, G = a.nh / a.nkv, all = a.block_rows;
   Rows x;
@@ -119,6 +121,7 @@ __device__ __forceinline__ Rows look_up(const Args& a, int block) {
   return x;
 }
 // The units of a block, by one thread.
+template <int KEYS>
 __device__ __forceinline__ int count_units(const Args& a, int block) {
   const int G = a.nh / a.nkv, all = a.block_rows, r = block / a.row_blocks, rho0 = block % a.row_blocks * all;
   const int beam0 = rho0 / G, beam1 = (min(rho0 + all, a.K * G) - 1) / G;
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(c
   // ---- the list's length, and this team's share ----
   const int blocks = a.R * a.row_blocks, chunk = (blocks + 31) / 32, block0 = min(lane * chunk, blocks), block1 = min(block0 + chunk, blocks);
   int mine = 0;
-  for (int i = block0; i < block1; ++i) mine += count_units(a, i);
+  for (int i = block0; i < block1; ++i) mine += count_units<KEYS>(a, i);
   mine *= a.nkv;
   int up = mine;
 #pragma unroll
@@ -239,7 +242,7 @@ __global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(c
     const int owner = __ffs(__ballot_sync(0xffffffffu, begin < up)) - 1;
     int before = __shfl_sync(0xffffffffu, up - mine, owner);
     for (block = owner * chunk;; ++block) {
-      x = look_up(a, block);
+      x = look_up<KEYS>(a, block);
       if (begin < before + x.units * a.nkv) break;
       before += x.units * a.nkv;
     }
@@ -445,7 +448,7 @@ __global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(c
       unit = 0;
       if (++kvh == a.nkv) {
         kvh = 0;
-        if (i + 1 < end) x = look_up(a, ++block);
+        if (i + 1 < end) x = look_up<KEYS>(a, ++block);
       }
     }
   }
@@ -457,13 +460,13 @@ __global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(c
 // ---------------------------------------------------------------------------
 // Heads of up to 128 numbers: the tensor cores of tcgen05, keys on the tile's 128 rows, the beams' queries on its N columns, so that a
 // request's few rows are no padding:  S' = K Q' and O' = V' P', both accumulated in tensor memory.
-//   warp 0       walks the block's share of the list and brings its units, four (128 keys) a stage, by the copy engine
+//   warp 0       walks the block's share of the list and brings its pages, two (128 keys) a stage, by the copy engine
 //   warp 1       one lane issues the products; the next stage's scores before this one's values, where its keys are there
 //   warps 4-     two or four groups of four, each with its columns: a thread has one key.  Weights relative to a number a row that is raised
 //                only when a score passes it by RESCALE_LOG2 (then the sums and O' are scaled down); P to shared memory, a row a key
-// A stage's units may be different beams' own; a mask of rows goes with each.
+// A stage's pages may be different beams' own; a mask of rows goes with each.
 // ---------------------------------------------------------------------------
-constexpr int SUB = 4, BLOCK_KEYS = SUB * KEYS;              // units of a stage
+constexpr int SUB = 2, BLOCK_KEYS = SUB * PAGE;              // pages of a stage
 constexpr float NOTHING = -1e30f;                            // what weights are relative to before a row has seen a key
 
 struct Info {                                                // of a stage
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
   const int blocks = a.R * a.row_blocks, chunk = (blocks + C::THREADS - 1) / C::THREADS;
   {
     int mine = 0;
-    for (int i = tid * chunk; i < min((tid + 1) * chunk, blocks); ++i) mine += count_units(a, i);
+    for (int i = tid * chunk; i < min((tid + 1) * chunk, blocks); ++i) mine += count_units<PAGE>(a, i);
     sums[tid] = mine * a.nkv;
   }
   jb::tc_fence_before();
@@ -642,106 +645,118 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       int before = before_owner, t = owner * EACH;
       while (begin >= before + sums[t]) before += sums[t++];
       for (block = t * chunk;; ++block) {
-        x = look_up(a, block);
+        x = look_up<PAGE>(a, block);
         if (begin < before + x.units * a.nkv) break;
         before += x.units * a.nkv;
       }
       kvh = (begin - before) / x.units;
       unit = begin - before - kvh * x.units;
     }
-    // Lanes 0 to 3 have a unit of a stage each.  A stage's pages are looked up while the one before is asked for.
+    // Lanes 0 and 1 have a page of a stage each.  The next stage's pages are looked up while this one's are asked for.
     unsigned long long joining[2] = {0ull, 0ull}, all[2] = {0ull, 0ull};
+    int piece0 = 0, piece1 = 0;
     auto entered = [&]() {                                             // rows that read the shared pages; all rows
       joining[0] = joining[1] = all[0] = all[1] = 0ull;
+      add_rows(all, 0, x.n_rows);
+      const unsigned beams = a.K == 32 ? ~0u : (1u << a.K) - 1u;
       unsigned who = __ballot_sync(0xffffffffu, lane < a.K && x.len >= x.common * PAGE);
+      if (who == beams) {
+        joining[0] = all[0], joining[1] = all[1];
+        return;
+      }
       while (who) {
         const int b = __ffs(who) - 1;
         who &= who - 1;
         add_rows(joining, max(b * G - x.rho0, 0), min((b + 1) * G - x.rho0, x.n_rows));
       }
-      add_rows(all, 0, x.n_rows);
     };
-    int n = 0, keys = 0, from = 0, beam = -1;                          // units of the stage; the lane's: keys, place in its page, beam
-    const int* entry = nullptr;
+    auto begun = [&]() {                                               // the shares that this head's pages lie in
+      piece0 = (at - unit) / per, piece1 = (at - unit + x.units - 1) / per;
+    };
+    int n = 0, keys = 0, beam = -1, page = -1;                         // units of the next stage; the lane's: keys, beam, page
     auto find = [&]() {
       n = min(min(SUB, x.units - unit), end - at);
-      const int shared_units = x.common * (PAGE / KEYS), mine = unit + lane;
-      beam = -1, keys = 0, entry = nullptr;
-      if (lane < n && mine < shared_units) {
-        keys = KEYS, from = mine * KEYS % PAGE;
-        entry = a.table + ((size_t)x.request * a.K + x.head) * a.W + mine / (PAGE / KEYS);
+      beam = -1, keys = 0, page = -1;
+      const int* entry = nullptr;
+      if (lane < n && unit + lane < x.common) {
+        keys = PAGE;
+        entry = a.table + ((size_t)x.request * a.K + x.head) * a.W + unit + lane;
       }
-      for (int i = max(shared_units - unit, 0); i < n; ++i) {          // beams' own
-        const int j = unit + i - shared_units;
+      for (int i = max(x.common - unit, 0); i < n; ++i) {              // beams' own
+        const int j = unit + i - x.common;
         const unsigned behind = __ballot_sync(0xffffffffu, x.upto > j);
         if (behind == 0u) break;                                       // (rows without keys)
         const int b = __ffs(behind) - 1;
         const int first = __shfl_sync(0xffffffffu, x.first, b), before = __shfl_sync(0xffffffffu, x.upto - x.own, b), len = __shfl_sync(0xffffffffu, x.len, b);
         if (lane == i) {
-          const int key = first * PAGE + (j - before) * KEYS;
-          beam = b, keys = min(KEYS, len - key), from = key % PAGE;
-          entry = a.table + ((size_t)x.request * a.K + b) * a.W + key / PAGE;
+          const int column = first + j - before;
+          beam = b, keys = min(PAGE, len - column * PAGE);
+          entry = a.table + ((size_t)x.request * a.K + b) * a.W + column;
         }
       }
+      if (entry != nullptr) page = *entry;
     };
-    int page = -1;
     if (at < end) {
       entered();
+      begun();
       find();
-      page = entry != nullptr ? *entry : -1;
     }
     while (at < end) {
-      if (round > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(kv_empty + 8 * st, (round - 1) & 1, status, 54));
-        if (!ok) break;
-      }
-      const bool there = keys > 0 && page >= 0 && page < a.n_pages;    // (no page: no keys)
-      const bool first = at == begin || unit == 0, last = unit + n == x.units || at + n == end;
+      // ---- this stage, as it was found ----
+      const int n0 = n, keys0 = keys, page0 = page, kvh0 = kvh;
+      const bool first = at == begin || unit == 0, last = unit + n == x.units || at + n == end, final_ = at + n == end;
       unsigned long long rows[2] = {joining[0], joining[1]};
       if (beam >= 0) {
         rows[0] = rows[1] = 0ull;
         add_rows(rows, max(beam * G - x.rho0, 0), min((beam + 1) * G - x.rho0, x.n_rows));
       }
-      const unsigned loads = __ballot_sync(0xffffffffu, there);
-      const bool whole = __all_sync(0xffffffffu, lane >= SUB || (there && keys == KEYS && rows[0] == all[0] && rows[1] == all[1]));
-      Info& to = info[st];
-      if (lane < SUB) to.keys[lane] = there ? keys : 0, to.rows[lane][0] = rows[0], to.rows[lane][1] = rows[1];
-      const uint32_t full = kv_full + 8 * st, stage = base + st * C::STAGE;
-      if (lane == 0) {
-        const int start = at - unit;                                   // the block of rows' first place of the list
-        to.first = first, to.last = last, to.final_ = at + n == end, to.whole = whole;
-        to.request = x.request, to.rho0 = x.rho0, to.n_rows = x.n_rows, to.kvh = kvh;
-        to.piece0 = start / per, to.piece1 = (start + x.units - 1) / per;
-      }
-      __syncwarp();
-      if (lane == 0) {
-        jb::mbar_arrive(told + 8 * st);
-        if (loads) jb::mbar_expect_tx(full, __popc(loads) * 2 * C::SLABS * KEYS * 128);
-        else jb::mbar_arrive(full);
-      }
-      __syncwarp();
-      if (there) {
-        const int row = (page * a.nkv + kvh) * PAGE + from;
-#pragma unroll
-        for (int h = 0; h < C::SLABS; ++h) {
-          jb::tma_load_2d(stage + (C::SLABS + h) * C::SLAB + lane * KEYS * 128, &map_k, full, h * 64, row);
-          jb::tma_load_2d(stage + h * C::SLAB + lane * KEYS * 128, &map_v, full, h * 64, row);
-        }
-      }
-      if (++st == C::STAGES) st = 0, ++round;
+      const bool whole_rows = rows[0] == all[0] && rows[1] == all[1];
+      const int4 where = make_int4(x.request, x.rho0, x.n_rows, kvh), pieces = make_int4(piece0, piece1, 0, 0);
+      // ---- the next one's pages are on their way meanwhile ----
       at += n, unit += n;
       if (at < end) {
         if (unit == x.units) {
           unit = 0;
           if (++kvh == a.nkv) {
             kvh = 0;
-            x = look_up(a, ++block);
+            x = look_up<PAGE>(a, ++block);
             entered();
           }
+          begun();
         }
         find();
-        page = entry != nullptr ? *entry : -1;
       }
+      if (round > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(kv_empty + 8 * st, (round - 1) & 1, status, 54));
+        if (!ok) break;
+      }
+      const bool there = lane < n0 && keys0 > 0 && page0 >= 0 && page0 < a.n_pages;   // (no page: no keys)
+      const unsigned loads = __ballot_sync(0xffffffffu, there);
+      const bool whole = __all_sync(0xffffffffu, lane >= SUB || (there && keys0 == PAGE && whole_rows));
+      Info& to = info[st];
+      if (lane < SUB) to.keys[lane] = there ? keys0 : 0, to.rows[lane][0] = rows[0], to.rows[lane][1] = rows[1];
+      const uint32_t full = kv_full + 8 * st, stage = base + st * C::STAGE;
+      if (lane == 0) {
+        to.first = first, to.last = last, to.final_ = final_, to.whole = whole;
+        to.request = where.x, to.rho0 = where.y, to.n_rows = where.z, to.kvh = where.w;
+        to.piece0 = pieces.x, to.piece1 = pieces.y;
+      }
+      __syncwarp();
+      if (lane == 0) {
+        jb::mbar_arrive(told + 8 * st);
+        if (loads) jb::mbar_expect_tx(full, __popc(loads) * 2 * C::SLABS * PAGE * 128);
+        else jb::mbar_arrive(full);
+      }
+      __syncwarp();
+      if (there) {
+        const int row = (page0 * a.nkv + kvh0) * PAGE;
+#pragma unroll
+        for (int h = 0; h < C::SLABS; ++h) {
+          jb::tma_load_2d(stage + (C::SLABS + h) * C::SLAB + lane * PAGE * 128, &map_k, full, h * 64, row);
+          jb::tma_load_2d(stage + h * C::SLAB + lane * PAGE * 128, &map_v, full, h * 64, row);
+        }
+      }
+      if (++st == C::STAGES) st = 0, ++round;
     }
     // gave up: what is still on its way arrives before the block ends (or its wait gives up as well)
     if (!ok && lane == 0)
@@ -828,12 +843,12 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       ok = ok && mbar_wait(kv_full + 8 * st, phase, status, 53);
       if (group_any(1 + group, !ok)) break;
       const bool last = x->last;
-      const int final_ = x->final_, keys = x->keys[quarter];
+      const int final_ = x->final_, sub = quarter >> 1, in_page = (quarter & 1) * 32 + lane, keys = x->keys[sub];
       const bool masked = !x->whole;
       unsigned long long rows = 0ull;
       if (masked) {
-        rows = x->rows[quarter][c0 / 64] >> (c0 % 64);
-        if (lane >= keys) rows = 0ull;
+        rows = x->rows[sub][c0 / 64] >> (c0 % 64);
+        if (in_page >= keys) rows = 0ull;
       }
       ok = ok && mbar_wait(s_full + 8 * (it & 1), (it >> 1) & 1, status, 57);
       if (it > 0) ok = ok && mbar_wait(pv_done, (it - 1) & 1, status, 58);     // P is free, and O' at rest
@@ -902,7 +917,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
         tmem_st_wait();
       }
       // values behind the last key: a weight of 0 does not silence what is no number
-      if (masked && lane >= keys && group == 0) {
+      if (masked && in_page >= keys && group == 0) {
 #pragma unroll
         for (int p = 0; p < C::SLABS * 8; ++p)
           *reinterpret_cast<uint4*>(smem + st * C::STAGE + (p / 8) * C::SLAB + key * 128 + (((p ^ key) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
@@ -1122,8 +1137,9 @@ JB_EXPORT int jb_attention_beams(const void* q, const void* k_cache, const void*
     JB_REFUSE(team < 1 || warps < team || warps % team || warps > Wide::WARPS || warps / team > 3 || rows != ROWS * team,
               "attention_beams: %d rows for teams of %d of %d warps", rows, team, warps);
   CUtensorMap maps[2];
-  if (!jb::make_map_64(&maps[0], k_cache, (uint64_t)n_pages * nkv * PAGE, hd, KEYS, true) ||
-      !jb::make_map_64(&maps[1], v_cache, (uint64_t)n_pages * nkv * PAGE, hd, KEYS, true))
+  const int keys = hd > 128 ? KEYS : PAGE;
+  if (!jb::make_map_64(&maps[0], k_cache, (uint64_t)n_pages * nkv * PAGE, hd, keys, true) ||
+      !jb::make_map_64(&maps[1], v_cache, (uint64_t)n_pages * nkv * PAGE, hd, keys, true))
     return JB_ERR_TENSORMAP;
   Args a{};
   a.q = (const bf16*)q, a.out = (bf16*)out, a.table = table, a.kv_len = kv_len, a.shared = shared;

@@ -2878,14 +2878,14 @@ def beams_pay(rows: int, nkv: int, hd: int, max_kv_len: int) -> bool:
 
 @functools.lru_cache(maxsize=4096)
 def beam_attention_plan(groups: int, beams: int, nh: int, nkv: int, hd: int, max_kv_len: int):
-    """How `attention_beams` runs: (blocks, rows of a block's tile, warps of a block, warps of a team, units of 32 keys of a share at least)."""
+    """How `attention_beams` runs: (blocks, rows of a block's tile, warps of a block, warps of a team, units (pages; 32 keys) of a share at least)."""
     rows = beams * (nh // nkv)
     if hd <= 128:
-        tile = next((n for n in (16, 32, 64) if rows <= n), 128)
-        warps, team, teams, fewest = 0, 1, 1, 4
+        tile, unit = next((n for n in (16, 32, 64) if rows <= n), 128), 64
+        warps, team, teams, fewest = 0, 1, 1, 2
     else:
         team, warps, fewest = 1 if rows <= 16 else 2 if rows <= 32 else 4, 4, 2
-        tile, teams = 16 * team, 2 if team < 4 else 1
+        tile, teams, unit = 16 * team, 2 if team < 4 else 1, 32
         warps = team * teams
-    units = groups * -(-rows // tile) * nkv * -(-max_kv_len // 32) * (beams + 1)      # (at most: nothing may be shared)
+    units = groups * -(-rows // tile) * nkv * -(-max_kv_len // unit) * (beams + 1)      # (at most: nothing may be shared)
     return max(1, min(SM_COUNT_TARGET // 2, -(-units // (fewest * teams)))), tile, warps, team, fewest
