@@ -851,8 +851,12 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
         if (in_page >= keys) rows = 0ull;
       }
       ok = ok && mbar_wait(s_full + 8 * (it & 1), (it >> 1) & 1, status, 57);
-      if (it > 0) ok = ok && mbar_wait(pv_done, (it - 1) & 1, status, 58);     // P is free, and O' at rest
       jb::tc_fence_after();
+      bool rest = it == 0;                                             // P is free, and O' at rest
+      auto settle = [&]() {
+        if (!rest) ok = ok && mbar_wait(pv_done, (it - 1) & 1, status, 58), jb::tc_fence_after();
+        rest = true;
+      };
       float s[C::HALF];
       auto scores = [&]() {
 #pragma unroll
@@ -881,6 +885,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       }
       if (group_any(1 + group, high > RESCALE_LOG2)) {
         // the rows' largest over the block's keys
+        settle();
         scores();
 #pragma unroll
         for (int c = 0; c < C::HALF; ++c) {
@@ -922,18 +927,19 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
         for (int p = 0; p < C::SLABS * 8; ++p)
           *reinterpret_cast<uint4*>(smem + st * C::STAGE + (p / 8) * C::SLAB + key * 128 + (((p ^ key) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
       }
+      uint32_t w[C::HALF / 2];
+#pragma unroll
+      for (int c = 0; c < C::HALF; c += 2) {
+        const float p0 = fast_exp2(s[c]), p1 = fast_exp2(s[c + 1]);
+        l[c] += p0, l[c + 1] += p1;
+        w[c / 2] = pack_bf16(p0, p1);
+      }
+      settle();
       uint8_t* p_row = smem + C::AT_P + (c0 / 64) * BLOCK_KEYS * 128 + key * 128;
 #pragma unroll
       for (int c = 0; c < C::HALF; c += 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = fast_exp2(s[c + 2 * e]), p1 = fast_exp2(s[c + 2 * e + 1]);
-          l[c + 2 * e] += p0, l[c + 2 * e + 1] += p1;
-          w[e] = pack_bf16(p0, p1);
-        }
         const int piece = (c0 % 64 + c) / 8;
-        *reinterpret_cast<uint4*>(p_row + ((piece ^ (key & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(p_row + ((piece ^ (key & 7)) << 4)) = make_uint4(w[c / 2], w[c / 2 + 1], w[c / 2 + 2], w[c / 2 + 3]);
       }
       const int piece0 = x->piece0, piece1 = x->piece1;                // (read before the stage is given back)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
