@@ -138,6 +138,10 @@ __device__ __forceinline__ int count_units(const Args& a, int block) {
   return max(1, n);
 }
 
+// Whether one of two numbers is infinite or none (an exponent of ones carries into the sign's place).  A weight of 0 silences neither, so values
+// of pages that not all rows read are looked at: such a value is left out and the rows that read it become no numbers, their neighbours stay.
+__device__ __forceinline__ uint32_t not_finite(uint32_t two) { return ((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+
 // A place of the list as one thread walks it: the unit's beam (-1: all that share it), its first key, and where its page stands.
 struct Cursor {
   int block, kvh, unit, units, shared_units;
@@ -362,7 +366,9 @@ __global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(c
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[j][e] += s_odd[j][e];
-      if (beam >= 0 || keys < KEYS || !all_join) {
+      const bool masked = beam >= 0 || keys < KEYS || !all_join;
+      bool bad = false;                                    // some value is no finite number, and rows that do not see it are here
+      if (masked) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -408,9 +414,19 @@ __global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(c
         for (int j = 0; j < HDC / 8; j += 2) {
           uint32_t b[4];
           ldmatrix_x4_trans(b, v_t + (v_lane ^ ((j % 8) << 4)) + (j / 8) * C::SLAB + kk * 16 * 128);
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (not_finite(b[e])) b[e] = 0u, bad = true;
+          }
           mma_bf16(o[j], pa, b[0], b[1]);
           mma_bf16(o[j + 1], pa, b[2], b[3]);
         }
+      }
+      if (masked && __any_sync(0xffffffffu, bad)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (beam < 0 ? joins[h] : beam_of[h] == beam) l[h] = CUDART_NAN_F;
       }
       if (keys < KEYS) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // zeroes, before the copy engine writes there again
     }
@@ -432,9 +448,9 @@ __global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(c
         const size_t item = ((size_t)x.request * a.K + beam_of[h]) * a.nh + kvh * G + rho % G;
         if (c == 0) {
           if (worker == first) a.parts[item] = make_int2(first, last - first + 1);
-          if (!complete) a.part_ml[record + row] = make_float2(m[h], sum);
+          if (!complete) a.part_ml[record + row] = make_float2(sum == sum ? m[h] : 0.0f, sum);
         }
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
         for (int j = 0; j < HDC / 8; ++j) {
           if (j * 8 < hd) {
@@ -484,7 +500,7 @@ struct Tc {
   static constexpr int MISC = 4 * N + 16 * N + 1200;         // ref, exchange, barriers and descriptions
   static constexpr int FIT = (232448 - Q - P - MISC) / STAGE, STAGES = FIT > 6 ? 6 : FIT;
   static constexpr int AT_Q = STAGES * STAGE, AT_P = AT_Q + Q, AT_REF = AT_P + P, AT_SWAP = AT_REF + 4 * N, AT_INFO = AT_SWAP + 16 * N,
-                       AT_BARS = AT_INFO + STAGES * (int)sizeof(Info), SMEM = AT_BARS + (3 * STAGES + 6) * 8 + 16;
+                       AT_BARS = AT_INFO + STAGES * (int)sizeof(Info), AT_BAD = AT_BARS + (3 * STAGES + 6) * 8 + 16, SMEM = AT_BAD + 128;
   static constexpr int COLS = 3 * N <= 64 ? 64 : 3 * N <= 128 ? 128 : 3 * N <= 256 ? 256 : 512;  // two S', one O'
   static constexpr int GROUPS = N > 32 ? 4 : 2, HALF = N / GROUPS;      // groups of four warps, columns of each
   static constexpr int WARPS = 4 * GROUPS, THREADS = 128 + 32 * WARPS;
@@ -594,12 +610,14 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
   Info* info = reinterpret_cast<Info*>(smem + C::AT_INFO);             // [STAGES]
   const uint32_t bars = base + C::AT_BARS, kv_full = bars, kv_empty = bars + 8 * C::STAGES, s_full = bars + 16 * C::STAGES, p_full = s_full + 16,
                  pv_done = p_full + 8, q_full = pv_done + 8, o_full = q_full + 8, told = o_full + 8;
+  // [block of rows' parity][group][2]: rows that read a value that is no finite number, as the group has found
+  unsigned long long (*bad)[C::GROUPS][2] = reinterpret_cast<unsigned long long (*)[C::GROUPS][2]>(smem + C::AT_BAD);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::AT_BARS + (3 * C::STAGES + 6) * 8);
   if (tid == 0) {
     for (int i = 0; i < C::STAGES; ++i) jb::mbar_init(kv_full + 8 * i, 1), jb::mbar_init(kv_empty + 8 * i, 1), jb::mbar_init(told + 8 * i, 1);
     jb::mbar_init(s_full, 1), jb::mbar_init(s_full + 8, 1), jb::mbar_init(p_full, C::WARPS), jb::mbar_init(pv_done, 1), jb::mbar_init(q_full, C::WARPS);
-    jb::mbar_init(o_full, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    jb::mbar_init(o_full, 2);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) jb::tmem_alloc<C::COLS>(jb::smem_u32((const void*)tmem_slot));
   jb::pdl_launch_dependents();
@@ -805,7 +823,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
                         first && ks == 0 ? 0u : 1u);
         jb::umma_commit(kv_empty + 8 * st);
         jb::umma_commit(pv_done);
-        if (last) jb::umma_commit(o_full);
+        if (last) jb::umma_commit(o_full), jb::mbar_arrive(o_full);    // (by itself as well: what the groups wrote before is seen behind it)
         if (final_) break;
         st = st1, phase = phase1;
       }
@@ -837,6 +855,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
         __syncwarp();
         if (lane == 0) jb::mbar_arrive(q_full);
         if (key < C::HALF) my_ref[key] = NOTHING;
+        if (key < 2) bad[turn & 1][group][key] = 0ull;
 #pragma unroll
         for (int c = 0; c < C::HALF; ++c) l[c] = 0.0f;
       }
@@ -849,6 +868,21 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       if (masked) {
         rows = x->rows[sub][c0 / 64] >> (c0 % 64);
         if (in_page >= keys) rows = 0ull;
+        // values behind the last key, or that are no finite numbers: a weight of 0 does not silence them (a part of the head's numbers a
+        // group; while the scores are made)
+        uint8_t* values = smem + st * C::STAGE + key * 128;
+        uint32_t odd = 0u;
+#pragma unroll
+        for (int p = 0; p < C::SLABS * 8 / C::GROUPS; ++p) {
+          const int at = p * C::GROUPS + group;
+          const uint4 v = *reinterpret_cast<const uint4*>(values + (at / 8) * C::SLAB + (((at ^ key) & 7) << 4));
+          odd |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
+        }
+        if (odd != 0u || in_page >= keys) {
+          for (int at = group; at < C::SLABS * 8; at += C::GROUPS)
+            *reinterpret_cast<uint4*>(values + (at / 8) * C::SLAB + (((at ^ key) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+          if (in_page < keys) atomicOr(&bad[turn & 1][group][0], x->rows[sub][0]), atomicOr(&bad[turn & 1][group][1], x->rows[sub][1]);
+        }
       }
       ok = ok && mbar_wait(s_full + 8 * (it & 1), (it >> 1) & 1, status, 57);
       jb::tc_fence_after();
@@ -921,12 +955,6 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
         }
         tmem_st_wait();
       }
-      // values behind the last key: a weight of 0 does not silence what is no number
-      if (masked && in_page >= keys && group == 0) {
-#pragma unroll
-        for (int p = 0; p < C::SLABS * 8; ++p)
-          *reinterpret_cast<uint4*>(smem + st * C::STAGE + (p / 8) * C::SLAB + key * 128 + (((p ^ key) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
-      }
       uint32_t w[C::HALF / 2];
 #pragma unroll
       for (int c = 0; c < C::HALF; c += 2) {
@@ -950,6 +978,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
         group_any(1 + group, false);                                   // (nobody reads there any longer)
         // the sums over the keys: half the columns go to the other half of the lanes, and so on, until a lane has one
         columns_summed<C::HALF>(l, swap + quarter * N + c0);
+        const int spoil = turn & 1;
         ok = ok && mbar_wait(o_full, turn++ & 1, status, 59);
         jb::tc_fence_after();
         group_any(1 + group, false);
@@ -960,13 +989,17 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
         if (key < C::HALF) {
           const int row = c0 + key, rho = rho0 + row;
           float* t = swap + c0 + key;
-          const float sum = (t[0] + t[N]) + (t[2 * N] + t[3 * N]);
-          t[0] = complete ? (sum > 0.0f ? 1.0f / sum : 0.0f) : 1.0f;
+          float sum = (t[0] + t[N]) + (t[2 * N] + t[3 * N]);
+          unsigned long long spoilt = 0ull;
+#pragma unroll
+          for (int g = 0; g < C::GROUPS; ++g) spoilt |= bad[spoil][g][row / 64];
+          if ((spoilt >> (row % 64)) & 1ull) sum = CUDART_NAN_F;
+          t[0] = complete ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
           if (row < n_rows) {
             const int item = (request * a.K + rho / G) * a.nh + kvh * G + rho % G;
             t[N] = __int_as_float(complete ? item : (int)record + row);
             if (piece == piece0) a.parts[item] = make_int2(piece0, piece1 - piece0 + 1);
-            if (!complete) a.part_ml[record + row] = make_float2(my_ref[key] > 0.5f * NOTHING ? my_ref[key] : -CUDART_INF_F, sum);
+            if (!complete) a.part_ml[record + row] = make_float2(sum != sum ? 0.0f : my_ref[key] > 0.5f * NOTHING ? my_ref[key] : -CUDART_INF_F, sum);
           }
         }
         group_any(1 + group, false);
@@ -1052,7 +1085,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) beam_attention_join_kernel(co
     }
   }
   if constexpr (PER == 1) {
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       if (lane * 4 + 128 * h < a.hd)
@@ -1070,7 +1103,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) beam_attention_join_kernel(co
     float f[PER];
 #pragma unroll
     for (int w = 0; w < PER; ++w) f[w] = fast_exp2(ml_of[w].x - use), all = fmaf(f[w], ml_of[w].y, all);
-    const float inv = all > 0.0f ? 1.0f / all : 0.0f;
+    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
     for (int d = threadIdx.x; d < a.hd; d += 32 * JOIN_WARPS) {
       float t = 0.0f;
 #pragma unroll

@@ -411,6 +411,32 @@ def test_attention_many_rows(K, group):
 
 
 @gpu
+@pytest.mark.parametrize("hd", [40, 64, 128, 256])
+@pytest.mark.parametrize("K, group", [(4, 4), (5, 16), (11, 2)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_attention_numbers_that_are_not_finite_stay_with_their_readers(hd, K, group, what):
+    """In pages that only some beams read: the others' answers are as if they were not there."""
+    kv_len = [130] + [700] * (K - 2) + [650] + [700] * K
+    q, k, v, table, nh = attention_case(2, K, kv_len, [9, 9], 2, group, hd, 7)
+    v[table[1][5], 1, 17, hd - 3] = what                    # a page that all but the first beam share
+    k[table[2][10], 0, 3, 5] = what                         # own pages
+    v[table[K - 1][9], 0, 60, 0] = what
+    out = empty(2 * K, nh * hd, dtype=torch.bfloat16)
+    scale = 1.0 / math.sqrt(hd)
+    ops.attention_beams(q.cuda(), k.cuda(), v.cuda(), out, ints(table), ints(kv_len), ints([9, 9]), K, nh, 2, hd, PAGE, scale,
+                        Workspace(torch.device("cuda")), 700)
+    got = out.cpu().double().view(2 * K, 2, group, hd)
+    want, size = P.attention(q, k, v, table, kv_len, nh, 2, hd, scale)
+    want, size = want.view(2 * K, 2, group, hd), size.view(2 * K, 2, group, -1)
+    clean = torch.ones(2 * K, 2, dtype=torch.bool)
+    clean[1:K, 1] = clean[2, 0] = clean[K - 1, 0] = False
+    off = (got - want).abs() / (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -11) * size + 1e-30)
+    assert float(off[clean].max()) <= 1.0
+    bad = ~torch.isfinite(want)
+    assert bad[1, 1, :, hd - 3].all() and bad[K - 1, 0, :, 0].all() and not torch.isfinite(got[bad]).any()
+
+
+@gpu
 def test_attention_shared_pages_said_too_many():
     """More pages said to be shared than the rows have."""
     q, k, v, table, nh = attention_case(1, 2, [100, 100], [2], 1, 4, 64, 3)
