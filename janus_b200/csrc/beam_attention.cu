@@ -1175,6 +1175,10 @@ JB_EXPORT int jb_attention_beams(const void* q, const void* k_cache, const void*
   else
     JB_REFUSE(team < 1 || warps < team || warps % team || warps > Wide::WARPS || warps / team > 3 || rows != ROWS * team,
               "attention_beams: %d rows for teams of %d of %d warps", rows, team, warps);
+  JB_REFUSE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)part) % 16, "attention_beams: q, out or workspace not on a boundary of 16 bytes");
+  const size_t row_bytes = (size_t)R * K * nh * hd * 2, cache_bytes = (size_t)n_pages * nkv * PAGE * hd * 2;
+  auto over = [&](const void* other, size_t bytes) { return (uintptr_t)out < (uintptr_t)other + bytes && (uintptr_t)other < (uintptr_t)out + row_bytes; };
+  if (over(q, row_bytes) || over(k_cache, cache_bytes) || over(v_cache, cache_bytes)) return JB_ERR_OVERLAP;
   CUtensorMap maps[2];
   const int keys = hd > 128 ? KEYS : PAGE;
   if (!jb::make_map_64(&maps[0], k_cache, (uint64_t)n_pages * nkv * PAGE, hd, keys, true) ||

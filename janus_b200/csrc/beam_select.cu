@@ -17,6 +17,7 @@
 // then.
 #include <math_constants.h>
 #include <stdio.h>
+#include <stddef.h>
 #include <string.h>
 
 #include "common.cuh"
@@ -450,6 +451,18 @@ static_assert(MOST_BEAMS * (MOST_BEAMS * 24 + MOST_STOPS * 12) <= 40 * 1024, "th
 
 // given: an Args in host memory.  Scratch: maxima R * K * ranges * 256 float32, stats R * K * ranges of 24 bytes,
 // best R * K of 16, keys R * K * K of 8.
+// Whether an output lies over an input or another output (next_scores may be scores itself).
+static bool select_overlaps(const Args& a) {
+  const char* at[9];
+  static_assert(offsetof(Args, maxima) == sizeof(at), "nine tensors, the inputs first");
+  memcpy(at, &a, sizeof(at));
+  const size_t N = (size_t)a.R * a.K, n[9] = {N * a.V, N, (size_t)a.S, N, N, N, N, N, N};
+  for (int i = 3; i < 9; ++i)
+    for (int j = 0; j < i; ++j)
+      if (n[j] > 0 && at[i] < at[j] + 4 * n[j] && at[j] < at[i] + 4 * n[i] && !(i == 5 && j == 1 && at[i] == at[j])) return true;
+  return false;
+}
+
 JB_EXPORT int jb_beam_select(const void* given, cudaStream_t stream) {
   Args a;
   memcpy(&a, given, sizeof(a));
@@ -457,6 +470,7 @@ JB_EXPORT int jb_beam_select(const void* given, cudaStream_t stream) {
   JB_REFUSE(R < 1 || K < 1 || K > MOST_BEAMS || V < 1 || S < 0 || S > MOST_STOPS || ranges < 1 || ranges > MOST_RANGES ||
                 (long long)R * K * ranges > 0x7fffffffLL || V > 0x7fffffff - 65536,
             "beam_select: %d requests of %d beams, vocabulary %d, %d stop tokens, %d ranges", R, K, V, S, ranges);
+  if (select_overlaps(a)) return JB_ERR_OVERLAP;
   jb::Launch rows(dim3(R * K * ranges), dim3(THREADS), 0, stream);
   cudaError_t e = cudaLaunchKernelEx(&rows.c, beam_rows_kernel, a);
   if (e != cudaSuccess) return (int)e;

@@ -2829,6 +2829,8 @@ def reorder_rows(matrices: Sequence[torch.Tensor], slots: torch.Tensor, parents:
             raise KernelError(f"reorder_rows: matrices of {n} slots on the current CUDA device are taken, got {tuple(m.shape)}")
         at.append(m.data_ptr())
         numbers.append(m.numel() // n)
+    if len(set(at)) < len(at):
+        raise KernelError("reorder_rows: a matrix is given twice")
     lib, stream = _lib("beam_cache"), _stream()
     for first in range(0, len(at), REORDER_ROWS):
         some = slice(first, first + REORDER_ROWS)

@@ -447,6 +447,101 @@ def test_attention_shared_pages_said_too_many():
     assert torch.equal(out[0], out[1])
 
 
+# -- together ----------------------------------------------------------------------------------------------------------------
+class Step:
+    """A step's operators as a search has them: beams chosen, pages forked and copied, states moved, attention over the new tables."""
+
+    def __init__(self, R, K, V, seed, hd=64, prompt=200):
+        g = torch.Generator().manual_seed(seed)
+        W, own = 8, 3 * K * R
+        held = -(-prompt // PAGE)
+        pages = 1 + R * held + own
+        table = torch.full((R, K, W), -1, dtype=torch.int32)
+        table[:, 1:, 0] = 0                                  # page 0 is the spare one
+        refs = torch.zeros(pages, dtype=torch.int32)
+        for r in range(R):
+            table[r, 0, :held] = torch.arange(1 + r * held, 1 + (r + 1) * held)
+            refs[1 + r * held: 1 + (r + 1) * held] = 2
+        free = torch.full((pages,), -1, dtype=torch.int32)
+        free[:own] = torch.arange(pages - own, pages).flip(0)
+        lengths = torch.ones(R, K, dtype=torch.int32)
+        lengths[:, 0] = prompt
+        scores = torch.full((R, K), NONE)
+        scores[:, 0] = 0.0
+        z = lambda *s: torch.zeros(s, dtype=torch.int32)      # noqa: E731
+        t = dict(logits=torch.randn(R * K, V, generator=g) * 2, scores=scores, stops=torch.tensor([1, 5], dtype=torch.int32), parents=z(R, K),
+                 tokens=z(R, K), ep=z(R, K), et=z(R, K), es=torch.zeros(R, K), lengths=lengths, table=table.view(R * K, W), refs=refs, free=free,
+                 n_free=torch.tensor([own], dtype=torch.int32), positions=z(R, K), dest=z(R, K), src=z(R * K), dst=z(R * K), rows=z(R * K),
+                 shared=z(R), missing=z(1), k=torch.randn(pages, 2, PAGE, hd, generator=g).bfloat16(),
+                 v=torch.randn(pages, 2, PAGE, hd, generator=g).bfloat16(), state=torch.randn(R * K, 24, generator=g), slots=torch.arange(R * K).int(),
+                 q=torch.randn(R * K, 8 * hd, generator=g).bfloat16(), out=torch.zeros(R * K, 8 * hd, dtype=torch.bfloat16))
+        self.t = {name: x.cuda() for name, x in t.items()}
+        self.R, self.K, self.hd, self.workspace = R, K, hd, Workspace(torch.device("cuda"))
+
+    def run(self):
+        t, R, K, hd = self.t, self.R, self.K, self.hd
+        ops.beam_select(t["logits"], t["scores"], t["stops"], parents=t["parents"], tokens=t["tokens"], next_scores=t["scores"],
+                        ended_parents=t["ep"], ended_tokens=t["et"], ended_scores=t["es"], workspace=self.workspace)
+        ops.fork_pages(t["parents"], t["lengths"], t["table"], t["refs"], t["free"], t["n_free"], kv_len=t["lengths"], positions=t["positions"],
+                       dest_rows=t["dest"], new_table=t["table"], new_refs=t["refs"], new_free=t["free"], new_n_free=t["n_free"],
+                       copy_src=t["src"].view(R, K), copy_dst=t["dst"].view(R, K), copy_rows=t["rows"].view(R, K), shared=t["shared"],
+                       missing=t["missing"], spare=0, page_size=PAGE)
+        ops.copy_pages([t["k"], t["v"]], t["src"], t["dst"], t["rows"])
+        ops.reorder_rows([t["state"]], t["slots"], t["parents"])
+        ops.attention_beams(t["q"], t["k"], t["v"], t["out"], t["table"], t["lengths"].view(-1), t["shared"], K, 8, 2, hd, PAGE, 0.125,
+                            self.workspace, 8 * PAGE)
+        t["logits"].mul_(-0.97).add_(0.01)                   # the next step's
+
+    def same(self, other):
+        for name, x in self.t.items():
+            if not torch.equal(x.view(torch.uint8) if name in ("k", "v") else x, other.t[name].view(torch.uint8) if name in ("k", "v") else other.t[name]):
+                return name
+        return None
+
+
+@gpu
+@pytest.mark.parametrize("R, K, V, hd", [(1, 4, 300, 64), (3, 32, 5000, 128), (5, 3, 40000, 256)])
+def test_steps_replayed_on_another_stream(R, K, V, hd):
+    """Ten steps launched one by one, and the same captured once on another stream and replayed."""
+    plain, captured, other = (Step(R, K, V, 3, hd) for _ in range(3))
+    for _ in range(10):
+        plain.run()
+    assert int(plain.t["missing"]) == 0
+    side = torch.cuda.Stream()
+    captured.workspace = other.workspace
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        other.run()                                          # (makes the workspace)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        graph.capture_begin()
+        captured.run()
+        graph.capture_end()
+        for _ in range(10):
+            graph.replay()
+    side.synchronize()
+    assert captured.same(plain) is None
+
+
+@gpu
+def test_steps_of_two_streams_at_once():
+    """Two searches, each with a stream and a workspace of its own."""
+    want = [Step(4, 8, 50000, seed) for seed in (1, 2)]
+    got = [Step(4, 8, 50000, seed) for seed in (1, 2)]
+    for s in want:
+        for _ in range(8):
+            s.run()
+    streams = [torch.cuda.Stream() for _ in got]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for s, stream in zip(got, streams):
+            with torch.cuda.stream(stream):
+                s.run()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert a.same(b) is None
+
+
 # -- refusals --------------------------------------------------------------------------------------------------------------
 def _select_args(R=1, K=2, V=9, S=1, device="cpu"):
     i, f = dict(dtype=torch.int32, device=device), dict(dtype=torch.float32, device=device)
@@ -537,6 +632,37 @@ def test_wrong_types_and_shapes_refused():
     for bad in (torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(3, 8), torch.zeros(8, 2).t()):
         with pytest.raises(ops.KernelError, match="reorder_rows"):
             ops.reorder_rows([torch.zeros(2, 8, device="cuda"), bad.cuda()], i, i.view(1, 2))
+
+
+@gpu
+@pytest.mark.parametrize("name, other", [("parents", "tokens"), ("next_scores", "ended_scores"), ("ended_tokens", "stop_tokens"),
+                                         ("ended_scores", "scores"), ("next_scores", "logits")])
+def test_select_outputs_over_others_refused(name, other):
+    args = _select_args(R=1, K=2, V=2, S=2, device="cuda")
+    args[name] = args[other].view(-1)[:2].view(args[name].shape)
+    args["workspace"] = Workspace(torch.device("cuda"))
+    with pytest.raises(ops.KernelError, match="10004"):
+        ops.beam_select(**args)
+
+
+@gpu
+def test_attention_addresses_refused():
+    args = _attention_args(device="cuda")
+    args["workspace"] = Workspace(torch.device("cuda"))
+    for name in ("q", "out", "k_cache", "v_cache"):
+        t = args[name]
+        odd = torch.zeros(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape)
+        with pytest.raises(ops.KernelError, match="attention_beams"):
+            ops.attention_beams(**{**args, name: odd})
+    with pytest.raises(ops.KernelError, match="10004"):
+        ops.attention_beams(**{**args, "out": args["q"]})
+
+
+@gpu
+def test_reorder_a_matrix_twice_refused():
+    m, i = torch.zeros(2, 8, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(ops.KernelError, match="twice"):
+        ops.reorder_rows([m, m], i, i.view(1, 2))
 
 
 @gpu
