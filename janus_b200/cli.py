@@ -92,12 +92,15 @@ def main(argv=None) -> int:
     from janus_b200.engine.beams import room_for_beams
     from janus_b200.engine.generate import tokens_held
     from janus_b200.engine.shared_prefix import room_for_batch
+    from janus_b200.kernels.ops import MOST_BEAMS
+    if not 0 <= args.beams <= MOST_BEAMS:
+        ap.error(f"--beams takes 1 to {MOST_BEAMS}")
 
     batch = max(1, min(args.batch_size, len(prompts)))
     if prefix:                       # the prefix lies in the cache once, in a slot of its own; its requests take none
         room, slots = room_for_batch(len(prefix), [len(p) for p in prompts], args.max_tokens, max(0, args.drafts), batch), 1
     elif args.beams:                 # a beam takes a slot, and pages of its own behind its prompt's
-        room, slots = room_for_beams([len(p) for p in prompts], args.max_tokens, max(1, args.beams), batch), batch * max(1, args.beams)
+        room, slots = room_for_beams([len(p) for p in prompts], args.max_tokens, args.beams, batch), batch * args.beams
     else:
         room, slots = sum(sorted((tokens_held(len(p), args.max_tokens, 64) for p in prompts), reverse=True)[:batch]), batch
     dtype = {"bf16": "bfloat16", "fp32": "float32"}.get(args.dtype, args.dtype)

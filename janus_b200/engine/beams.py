@@ -263,6 +263,8 @@ class BeamRunner:
             raise ValueError(f"{len(stop)} stop tokens: beam search takes up to {ops.MOST_BEAM_STOPS}")
         if max_tokens < 0 or not math.isfinite(length_penalty) or (batch_size is not None and batch_size < 1):
             raise ValueError(f"max_tokens {max_tokens}, length_penalty {length_penalty}, batch_size {batch_size}")
+        if abs(length_penalty) * math.log(max(2, min(max_tokens, engine.max_seq_len))) > 600.0:      # (scores times that power stay numbers)
+            raise ValueError(f"length_penalty {length_penalty} is too large for {max_tokens} tokens")
         prompts = [np.asarray(p, dtype=np.int64).reshape(-1) for p in prompts]
         for i, p in enumerate(prompts):
             if len(p) == 0:
@@ -361,14 +363,17 @@ class BeamRunner:
             self._search(step, searches, K, length_penalty, early_stopping, stats)
             stats.decode_ms += (time.perf_counter() - t0) * 1e3
         finally:
-            torch.cuda.synchronize(engine.device)
-            for group, pages in zip(cache.groups, mine):
-                for p in reversed(pages):
+            # whatever ended the batch: wait for what is still in flight, then all that it holds comes back
+            try:
+                torch.cuda.synchronize(engine.device)
+            finally:
+                for group, pages in zip(cache.groups, mine):
+                    for p in reversed(pages):
+                        group.pool.give_back(p)
+                for s in slots:
+                    engine.free_slot(s)
+                for group, p in zip(cache.groups, spare):
                     group.pool.give_back(p)
-            for s in slots:
-                engine.free_slot(s)
-            for group, p in zip(cache.groups, spare):
-                group.pool.give_back(p)
 
     def _search(self, step: _BeamStep, searches: List[_Search], K: int, length_penalty: float, early_stopping: bool, stats) -> None:
         """Steps until every request is done.  A step is launched before the host has read what the one before chose; a request that turns out

@@ -328,6 +328,7 @@ def test_refusals():
     model = random_model(LLAMA_C, "float32", max_tokens=64 * 8)
     ok = [[1, 2, 3]]
     for bad, kw in ((ValueError, dict(beams=0)), (ValueError, dict(beams=33)), (ValueError, dict(max_tokens=-1)), (ValueError, dict(length_penalty=math.nan)),
+                    (ValueError, dict(length_penalty=1e3)), (ValueError, dict(length_penalty=-1e3)),
                     (ValueError, dict(stop_token_ids=range(33))), (ValueError, dict(batch_size=0)), (CacheFull, dict(beams=8, max_tokens=200))):
         with pytest.raises(bad):
             model.generate_beams(ok, **kw)
@@ -337,6 +338,41 @@ def test_refusals():
     assert model.generate_beams([], beams=2)[0] == [] and model.generate_beams(ok, max_tokens=0)[0] == [[]]
     model.engine.cache.check()
     assert model.engine.cache.n_free_slots == 64
+
+
+@gpu
+def test_what_ends_a_search_in_the_middle_gives_everything_back(monkeypatch):
+    from janus_b200.engine.beams import BeamRunner
+    model = random_model(LLAMA_C, "float32")
+    prompts = [random_tokens(n, 256, n) for n in (70, 30)]
+    want, _ = model.generate_beams(prompts, beams=3, max_tokens=20, ignore_eos=True)
+    free = model.engine.cache.n_free_slots, [g.pool.n_free for g in model.engine.cache.groups]
+    take, calls = BeamRunner._take, []
+
+    def stops(self, *args):
+        calls.append(1)
+        if len(calls) == 5:
+            raise KeyboardInterrupt
+        return take(self, *args)
+
+    monkeypatch.setattr(BeamRunner, "_take", stops)
+    with pytest.raises(KeyboardInterrupt):
+        model.generate_beams(prompts, beams=3, max_tokens=20, ignore_eos=True)
+    monkeypatch.undo()
+    assert free == (model.engine.cache.n_free_slots, [g.pool.n_free for g in model.engine.cache.groups])
+    model.engine.cache.check()
+    assert model.generate_beams(prompts, beams=3, max_tokens=20, ignore_eos=True)[0] == want
+
+
+@gpu
+def test_on_another_stream_and_with_the_most_beams():
+    model = random_model(LLAMA_C, "float32", max_tokens=64 * 200)
+    prompts = [random_tokens(n, 256, n) for n in (64, 1)]
+    want, _ = model.generate_beams(prompts, beams=32, max_tokens=70, ignore_eos=True)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got, _ = random_model(LLAMA_C, "float32", max_tokens=64 * 200).generate_beams(prompts, beams=32, max_tokens=70, ignore_eos=True)
+    assert got == want
 
 
 @gpu
@@ -350,7 +386,7 @@ def test_command_line(tmp_path, capsys):
 
 def test_command_line_refuses_what_does_not_go_together(capsys):
     from janus_b200.cli import main
-    for more in (["--temperature", "0.5"], ["--shared-prefix", "1,2"], ["--top-k", "3"], ["--repetition-penalty", "1.1"]):
+    for more in (["--temperature", "0.5"], ["--shared-prefix", "1,2"], ["--top-k", "3"], ["--repetition-penalty", "1.1"], ["--beams", "33"], ["--beams=-1"]):
         with pytest.raises(SystemExit):
             main(["nowhere", "1,2", "--beams", "2", *more])
     capsys.readouterr()
