@@ -69,6 +69,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
+__device__ __forceinline__ float low_of(uint32_t two) { return __uint_as_float(two << 16); }
+__device__ __forceinline__ float high_of(uint32_t two) { return __uint_as_float(two & 0xffff0000u); }
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -404,12 +406,11 @@ __global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(c
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[j][e] = fast_exp2(fmaf(s[j][e], a.scale_log2, -use[e >> 1]));
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        l[h] += ((s[0][2 * h] + s[0][2 * h + 1]) + (s[1][2 * h] + s[1][2 * h + 1])) + ((s[2][2 * h] + s[2][2 * h + 1]) + (s[3][2 * h] + s[3][2 * h + 1]));
-#pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         const uint32_t pa[4] = {pack_bf16(s[2 * kk][0], s[2 * kk][1]), pack_bf16(s[2 * kk][2], s[2 * kk][3]),
                                 pack_bf16(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack_bf16(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) l[h] += (low_of(pa[h]) + high_of(pa[h])) + (low_of(pa[2 + h]) + high_of(pa[2 + h]));   // (as they are rounded)
 #pragma unroll
         for (int j = 0; j < HDC / 8; j += 2) {
           uint32_t b[4];
@@ -959,8 +960,8 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
 #pragma unroll
       for (int c = 0; c < C::HALF; c += 2) {
         const float p0 = fast_exp2(s[c]), p1 = fast_exp2(s[c + 1]);
-        l[c] += p0, l[c + 1] += p1;
-        w[c / 2] = pack_bf16(p0, p1);
+        w[c / 2] = pack_bf16(p0, p1);                                  // (summed as they are rounded: a weight that outdoes all others costs nothing)
+        l[c] += low_of(w[c / 2]), l[c + 1] += high_of(w[c / 2]);
       }
       settle();
       uint8_t* p_row = smem + C::AT_P + (c0 / 64) * BLOCK_KEYS * 128 + key * 128;
