@@ -7,10 +7,13 @@
 // head, so that a shared page is read once for all beams; behind it every beam's own pages follow, one beam after another, for
 // the rows of that beam alone.  A softmax over a union of keys joins from (maximum, sum, weighted values), whoever made the parts.
 //
-// Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their units of 32 keys.  Every
-// block of threads (or team of warps) has an even, consecutive share of it, and the copy engine brings its units (128-byte swizzle), ahead
-// across the ends of requests.  Where a share ends inside a block of rows, the sums go out as a partial result; a second launch joins
-// those.
+// Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their units (pages; 32 keys with heads
+// of more than 128 numbers).  Every block of threads (or team of warps) has an even, consecutive share of it, and the copy engine brings
+// its units (128-byte swizzle), ahead across the ends of requests.  Where a share ends inside a block of rows, the sums go out as a partial
+// result; a second launch joins those.
+//
+// 32 heads over 8 of 128 numbers, 16 requests of 8 beams behind 6,000 to 24,000 tokens: 102 us for the 85 that 560 MB take; twice as
+// long 176 for 161, of 16 beams 134 for 94, with heads of 64 numbers 78 for 43; one request of 4 beams behind 300 9.5.
 #include <math_constants.h>
 #include <stdio.h>
 
@@ -482,6 +485,12 @@ __global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(c
 //   warps 4-     two or four groups of four, each with its columns: a thread has one key.  Weights relative to a number a row that is raised
 //                only when a score passes it by RESCALE_LOG2 (then the sums and O' are scaled down); P to shared memory, a row a key
 // A stage's pages may be different beams' own; a mask of rows goes with each.
+//
+// With heads of 128 numbers and 32 rows a stage (64 KB) takes 1.41 us, which is memory's rate for a multiprocessor; 7 us go by before the
+// first scores are there, 10 between the first share's end and the last one's, 4 in the join.  64 rows take 1.6 us a stage, heads of 64 numbers 0.95 (for
+// 0.74): the chain of one stage, of which scores to weights is 1,450 cycles.  Measured on the first case: warp-level products (mma.sync) of
+// the beams' rows padded to 16, 116 us, and 214 for 64 rows, as each of four warps reads all keys from shared memory again; shares of 4 to 8
+// pages at least, no better; weights of two stages in turn, so that a stage need not wait for the products of the one before, level (103).
 // ---------------------------------------------------------------------------
 constexpr int SUB = 2, BLOCK_KEYS = SUB * PAGE;              // pages of a stage
 constexpr float NOTHING = -1e30f;                            // what weights are relative to before a row has seen a key
@@ -1041,7 +1050,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
 // a time.
 constexpr int JOIN_WARPS = 4;
 template <int PER>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) beam_attention_join_kernel(const Args a, int rows) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS) beam_attention_join_kernel(const Args a, int rows, int shares) {
   __shared__ float4 sums[PER > 1 ? PER : 1][PER > 1 ? 64 : 1];
   __shared__ float2 ml_of[PER];
   jb::pdl_launch_dependents();
@@ -1050,7 +1059,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) beam_attention_join_kernel(co
   const int G = a.nh / a.nkv;
   if (item >= a.R * a.K * a.nh) return;
   const int2 parts = a.parts[item];
-  if (parts.y <= 1) return;
+  if (parts.y <= 1 || parts.x < 0 || parts.y > shares - parts.x) return;    // (what a launch whose wait ran out has left is not followed)
   const int head = item % a.nh, beam = item / a.nh % a.K, row = (beam * G + head % G) % rows;
   auto record = [&](int p) { return ((size_t)(parts.x + p) * 2 + (p == 0 ? 1 : 0)) * rows + row; };
   constexpr int AHEAD = 4;
@@ -1130,10 +1139,10 @@ cudaError_t join(const Args& a, int rows, int shares, cudaStream_t stream) {
   const int items = a.R * a.K * a.nh;
   if (shares > 4 * a.R * a.row_blocks * a.nkv) {
     jb::Launch cfg(dim3(items), dim3(32 * JOIN_WARPS), 0, stream);
-    return cudaLaunchKernelEx(&cfg.c, beam_attention_join_kernel<JOIN_WARPS>, a, rows);
+    return cudaLaunchKernelEx(&cfg.c, beam_attention_join_kernel<JOIN_WARPS>, a, rows, shares);
   }
   jb::Launch cfg(dim3((items + JOIN_WARPS - 1) / JOIN_WARPS), dim3(32 * JOIN_WARPS), 0, stream);
-  return cudaLaunchKernelEx(&cfg.c, beam_attention_join_kernel<1>, a, rows);
+  return cudaLaunchKernelEx(&cfg.c, beam_attention_join_kernel<1>, a, rows, shares);
 }
 cudaError_t wide_go(const CUtensorMap* maps, const Args& a, int blocks, int warps, int* status, cudaStream_t stream) {
   static bool ready[64] = {};
