@@ -512,7 +512,7 @@ struct Tc {
   static constexpr int AT_Q = STAGES * STAGE, AT_P = AT_Q + Q, AT_REF = AT_P + P, AT_SWAP = AT_REF + 4 * N, AT_INFO = AT_SWAP + 16 * N,
                        AT_BARS = AT_INFO + STAGES * (int)sizeof(Info), AT_BAD = AT_BARS + (3 * STAGES + 6) * 8 + 16, SMEM = AT_BAD + 128;
   static constexpr int COLS = 3 * N <= 64 ? 64 : 3 * N <= 128 ? 128 : 3 * N <= 256 ? 256 : 512;  // two S', one O'
-  static constexpr int GROUPS = N > 32 ? 4 : 2, HALF = N / GROUPS;      // groups of four warps, columns of each
+  static constexpr int GROUPS = N > 16 ? 4 : 2, HALF = N / GROUPS;      // groups of four warps, columns of each
   static constexpr int WARPS = 4 * GROUPS, THREADS = 128 + 32 * WARPS;
   static_assert(STAGES >= 2 && SMEM <= 232448, "shared memory of a block");
 };
