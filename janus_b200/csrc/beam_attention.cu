@@ -39,6 +39,7 @@ struct Args {
   const int* kv_len;
   const int* shared;
   int R, K, nh, nkv, hd, W, n_pages;
+  int group;                                       // query heads of a key head
   int team, row_blocks, fewest;                    // warps of a team; blocks of rows of a request; units of a share at least
   int block_rows;                                  // rows of a block
   float scale_log2;
@@ -103,27 +104,33 @@ struct Rows {
   int len, first, own, upto;        // of the lane's beam: keys, first page of its own, units of its own, of the beams up to it
 };
 
+// ... from the lane's beam's length and the request's shared pages, as they stand in memory.
 template <int KEYS>
-__device__ __forceinline__ Rows look_up(const Args& a, int block) {
-  const int lane = threadIdx.x & 31, G = a.nh / a.nkv, all = a.block_rows;
+__device__ __forceinline__ Rows rows_of(const Args& a, int block, int len, int shared) {
+  const int lane = threadIdx.x & 31, G = a.group;
   Rows x;
-  x.request = block / a.row_blocks;
-  x.rho0 = block % a.row_blocks * all;
-  x.n_rows = min(all, a.K * G - x.rho0);
-  x.len = lane < a.K ? min(max(a.kv_len[x.request * a.K + lane], 0), a.W * PAGE) : 0;
+  x.request = a.row_blocks == 1 ? block : block / a.row_blocks;
+  x.rho0 = (block - x.request * a.row_blocks) * a.block_rows;
+  x.n_rows = min(a.block_rows, a.K * G - x.rho0);
+  x.len = min(max(len, 0), a.W * PAGE);
   const int most = __reduce_max_sync(0xffffffffu, x.len);
   x.head = __ffs(__ballot_sync(0xffffffffu, lane < a.K && x.len == most)) - 1;
-  x.common = min(max(a.shared[x.request], 0), most / PAGE);
+  x.common = min(max(shared, 0), most / PAGE);
   x.first = x.len < x.common * PAGE ? 0 : x.common;        // shorter beams read all they have by themselves
-  x.own = lane >= x.rho0 / G && lane <= (x.rho0 + x.n_rows - 1) / G ? (x.len - x.first * PAGE + KEYS - 1) / KEYS : 0;
+  x.own = lane < a.K && (lane + 1) * G > x.rho0 && lane * G < x.rho0 + x.n_rows ? (x.len - x.first * PAGE + KEYS - 1) / KEYS : 0;
+  x.units = max(1, x.common * (PAGE / KEYS) + __reduce_add_sync(0xffffffffu, x.own));      // (rows without keys have a unit as well)
   x.upto = x.own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int t = __shfl_up_sync(0xffffffffu, x.upto, o);
     if (lane >= o) x.upto += t;
   }
-  x.units = max(1, x.common * (PAGE / KEYS) + __shfl_sync(0xffffffffu, x.upto, 31));     // (rows without keys have a unit as well)
   return x;
+}
+template <int KEYS>
+__device__ __forceinline__ Rows look_up(const Args& a, int block) {
+  const int lane = threadIdx.x & 31, request = a.row_blocks == 1 ? block : block / a.row_blocks;
+  return rows_of<KEYS>(a, block, lane < a.K ? a.kv_len[request * a.K + lane] : 0, a.shared[request]);
 }
 // The units of a block, by one thread.
 template <int KEYS>
@@ -513,6 +520,7 @@ struct Tc {
                        AT_BARS = AT_INFO + STAGES * (int)sizeof(Info), AT_BAD = AT_BARS + (3 * STAGES + 6) * 8 + 16, SMEM = AT_BAD + 128;
   static constexpr int COLS = 3 * N <= 64 ? 64 : 3 * N <= 128 ? 128 : 3 * N <= 256 ? 256 : 512;  // two S', one O'
   static constexpr int GROUPS = N > 16 ? 4 : 2, HALF = N / GROUPS;      // groups of four warps, columns of each
+  static constexpr int PLACES = 1024;                                   // of the list, whose units are counted
   static constexpr int WARPS = 4 * GROUPS, THREADS = 128 + 32 * WARPS;
   static_assert(STAGES >= 2 && SMEM <= 232448, "shared memory of a block");
 };
@@ -527,6 +535,11 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
       : "r"(bar), "r"(parity)
       : "memory");
   return ok != 0u;
+}
+__device__ __forceinline__ float warp_top(float v) {                 // the largest of a warp's numbers (one that is none is passed over)
+  float top;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(top) : "f"(v));
+  return top;
 }
 __device__ __forceinline__ bool elected() {
   uint32_t yes;
@@ -613,7 +626,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
                                                                         int* __restrict__ status) {
   typedef Tc<HDC, N> C;
   extern __shared__ __align__(1024) uint8_t smem[];
-  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, G = a.nh / a.nkv, hd = a.hd;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, G = a.group, hd = a.hd;
   const uint32_t base = jb::smem_u32(smem), q_at = base + C::AT_Q, p_at = base + C::AT_P;
   float* ref = reinterpret_cast<float*>(smem + C::AT_REF);             // [N] in units of log2
   float* swap = reinterpret_cast<float*>(smem + C::AT_SWAP);           // [4][N]
@@ -632,23 +645,37 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
   if (warp == 1) jb::tmem_alloc<C::COLS>(jb::smem_u32((const void*)tmem_slot));
   jb::pdl_launch_dependents();
   jb::pdl_wait();
-  // ---- the list's length: a thread's blocks of rows, then all threads' ----
-  int* sums = reinterpret_cast<int*>(smem + C::AT_P);                  // (P is not there yet)
-  const int blocks = a.R * a.row_blocks, chunk = (blocks + C::THREADS - 1) / C::THREADS;
-  {
-    int mine = 0;
-    for (int i = tid * chunk; i < min((tid + 1) * chunk, blocks); ++i) mine += count_units<PAGE>(a, i);
-    sums[tid] = mine * a.nkv;
+  // ---- the list's length: every warp has some of its places, several requests' lengths on their way at a time ----
+  int* sums = reinterpret_cast<int*>(smem + C::AT_P);                  // [places] (P is not there yet)
+  const int blocks = a.R * a.row_blocks, chunk = (blocks + C::PLACES - 1) / C::PLACES, places = (blocks + chunk - 1) / chunk;
+  constexpr int AHEAD = 4;
+  for (int p0 = warp; p0 < places; p0 += C::THREADS / 32 * AHEAD) {
+    int units[AHEAD] = {};
+    for (int i = 0; i < chunk; ++i) {
+      int len[AHEAD], shared[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int block = min((p0 + u * (C::THREADS / 32)) * chunk + i, blocks - 1), request = a.row_blocks == 1 ? block : block / a.row_blocks;
+        len[u] = lane < a.K ? a.kv_len[request * a.K + lane] : 0, shared[u] = a.shared[request];
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int block = (p0 + u * (C::THREADS / 32)) * chunk + i;
+        if (block < blocks) units[u] += rows_of<PAGE>(a, block, len[u], shared[u]).units;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (lane == 0 && p0 + u * (C::THREADS / 32) < places) sums[p0 + u * (C::THREADS / 32)] = units[u] * a.nkv;
   }
   jb::tc_fence_before();
   __syncthreads();
   jb::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   if (warp == 0) {
-    constexpr int EACH = C::THREADS / 32;
+    const int each = (places + 31) / 32;
     int mine = 0;
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) mine += sums[lane * EACH + i];
+    for (int i = lane * each; i < min(lane * each + each, places); ++i) mine += sums[i];
     int up = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -670,7 +697,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
         jb::mbar_arrive(kv_full);
       }
     } else {
-      int before = before_owner, t = owner * EACH;
+      int before = before_owner, t = owner * each;
       while (begin >= before + sums[t]) before += sums[t++];
       for (block = t * chunk;; ++block) {
         x = look_up<PAGE>(a, block);
@@ -680,7 +707,6 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       kvh = (begin - before) / x.units;
       unit = begin - before - kvh * x.units;
     }
-    // Lanes 0 and 1 have a page of a stage each.  The next stage's pages are looked up while this one's are asked for.
     unsigned long long joining[2] = {0ull, 0ull}, all[2] = {0ull, 0ull};
     int piece0 = 0, piece1 = 0;
     auto entered = [&]() {                                             // rows that read the shared pages; all rows
@@ -701,22 +727,24 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
     auto begun = [&]() {                                               // the shares that this head's pages lie in
       piece0 = (at - unit) / per, piece1 = (at - unit + x.units - 1) / per;
     };
-    int n = 0, keys = 0, beam = -1, page = -1;                         // units of the next stage; the lane's: keys, beam, page
+    // The lanes look up 32 units at a time; of a stage's, lanes 0 and 1 have one each.
+    int ahead = 0, keys = 0, beam = -1, page = -1;                     // the first one's place; the lane's: keys, beam (-1: all that share it), page
     auto find = [&]() {
-      n = min(min(SUB, x.units - unit), end - at);
+      ahead = unit;
       beam = -1, keys = 0, page = -1;
+      const int mine = unit + lane, j = mine - x.common;
+      const bool there = mine < x.units && at + lane < end;
       const int* entry = nullptr;
-      if (lane < n && unit + lane < x.common) {
+      if (there && j < 0) {
         keys = PAGE;
-        entry = a.table + ((size_t)x.request * a.K + x.head) * a.W + unit + lane;
+        entry = a.table + ((size_t)x.request * a.K + x.head) * a.W + mine;
       }
-      for (int i = max(x.common - unit, 0); i < n; ++i) {              // beams' own
-        const int j = unit + i - x.common;
-        const unsigned behind = __ballot_sync(0xffffffffu, x.upto > j);
-        if (behind == 0u) break;                                       // (rows without keys)
-        const int b = __ffs(behind) - 1;
-        const int first = __shfl_sync(0xffffffffu, x.first, b), before = __shfl_sync(0xffffffffu, x.upto - x.own, b), len = __shfl_sync(0xffffffffu, x.len, b);
-        if (lane == i) {
+      if (unit + 31 >= x.common) {                                     // beams' own
+        int b = 0;
+        for (int k = 0; k < a.K; ++k) b += __shfl_sync(0xffffffffu, x.upto, k) <= j;
+        const int who = min(b, 31), first = __shfl_sync(0xffffffffu, x.first, who), before = __shfl_sync(0xffffffffu, x.upto - x.own, who),
+                  len = __shfl_sync(0xffffffffu, x.len, who);
+        if (there && j >= 0 && b < a.K) {                              // (rows without keys: nobody's)
           const int column = first + j - before;
           beam = b, keys = min(PAGE, len - column * PAGE);
           entry = a.table + ((size_t)x.request * a.K + b) * a.W + column;
@@ -730,44 +758,28 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       find();
     }
     while (at < end) {
-      // ---- this stage, as it was found ----
-      const int n0 = n, keys0 = keys, page0 = page, kvh0 = kvh;
-      const bool first = at == begin || unit == 0, last = unit + n == x.units || at + n == end, final_ = at + n == end;
+      if (unit >= ahead + 32) find();                                  // (stages begin on even units)
+      const int n = min(min(SUB, x.units - unit), end - at), from = unit - ahead + (lane & 1);
+      const int keys0 = __shfl_sync(0xffffffffu, keys, from), beam0 = __shfl_sync(0xffffffffu, beam, from), page0 = __shfl_sync(0xffffffffu, page, from);
       unsigned long long rows[2] = {joining[0], joining[1]};
-      if (beam >= 0) {
+      if (beam0 >= 0) {
         rows[0] = rows[1] = 0ull;
-        add_rows(rows, max(beam * G - x.rho0, 0), min((beam + 1) * G - x.rho0, x.n_rows));
+        add_rows(rows, max(beam0 * G - x.rho0, 0), min((beam0 + 1) * G - x.rho0, x.n_rows));
       }
-      const bool whole_rows = rows[0] == all[0] && rows[1] == all[1];
-      const int4 where = make_int4(x.request, x.rho0, x.n_rows, kvh), pieces = make_int4(piece0, piece1, 0, 0);
-      // ---- the next one's pages are on their way meanwhile ----
-      at += n, unit += n;
-      if (at < end) {
-        if (unit == x.units) {
-          unit = 0;
-          if (++kvh == a.nkv) {
-            kvh = 0;
-            x = look_up<PAGE>(a, ++block);
-            entered();
-          }
-          begun();
-        }
-        find();
-      }
+      const bool there = lane < n && keys0 > 0 && page0 >= 0 && page0 < a.n_pages;    // (no page: no keys)
+      const unsigned loads = __ballot_sync(0xffffffffu, there);
+      const bool whole = __all_sync(0xffffffffu, lane >= SUB || (there && keys0 == PAGE && rows[0] == all[0] && rows[1] == all[1]));
       if (round > 0) {
         ok = __all_sync(0xffffffffu, mbar_wait(kv_empty + 8 * st, (round - 1) & 1, status, 54));
         if (!ok) break;
       }
-      const bool there = lane < n0 && keys0 > 0 && page0 >= 0 && page0 < a.n_pages;   // (no page: no keys)
-      const unsigned loads = __ballot_sync(0xffffffffu, there);
-      const bool whole = __all_sync(0xffffffffu, lane >= SUB || (there && keys0 == PAGE && whole_rows));
       Info& to = info[st];
       if (lane < SUB) to.keys[lane] = there ? keys0 : 0, to.rows[lane][0] = rows[0], to.rows[lane][1] = rows[1];
       const uint32_t full = kv_full + 8 * st, stage = base + st * C::STAGE;
       if (lane == 0) {
-        to.first = first, to.last = last, to.final_ = final_, to.whole = whole;
-        to.request = where.x, to.rho0 = where.y, to.n_rows = where.z, to.kvh = where.w;
-        to.piece0 = pieces.x, to.piece1 = pieces.y;
+        to.first = at == begin || unit == 0, to.last = unit + n == x.units || at + n == end, to.final_ = at + n == end, to.whole = whole;
+        to.request = x.request, to.rho0 = x.rho0, to.n_rows = x.n_rows, to.kvh = kvh;
+        to.piece0 = piece0, to.piece1 = piece1;
       }
       __syncwarp();
       if (lane == 0) {
@@ -777,12 +789,23 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       }
       __syncwarp();
       if (there) {
-        const int row = (page0 * a.nkv + kvh0) * PAGE;
+        const int row = (page0 * a.nkv + kvh) * PAGE;
 #pragma unroll
         for (int h = 0; h < C::SLABS; ++h) {
           jb::tma_load_2d(stage + (C::SLABS + h) * C::SLAB + lane * PAGE * 128, &map_k, full, h * 64, row);
           jb::tma_load_2d(stage + h * C::SLAB + lane * PAGE * 128, &map_v, full, h * 64, row);
         }
+      }
+      at += n, unit += n;
+      if (at < end && unit == x.units) {
+        unit = 0;
+        if (++kvh == a.nkv) {
+          kvh = 0;
+          x = look_up<PAGE>(a, ++block);
+          entered();
+        }
+        begun();
+        find();
       }
       if (++st == C::STAGES) st = 0, ++round;
     }
@@ -933,7 +956,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
         scores();
 #pragma unroll
         for (int c = 0; c < C::HALF; ++c) {
-          const float top = jb::warp_max(s[c]);
+          const float top = warp_top(s[c]);
           if (lane == 0) swap[quarter * N + c0 + c] = top;
         }
         group_any(1 + group, false);
@@ -1199,7 +1222,7 @@ JB_EXPORT int jb_attention_beams(const void* q, const void* k_cache, const void*
   const size_t records = hd <= 128 ? (size_t)blocks * 2 * rows : (size_t)blocks * warps * ROWS * 2;
   a.part_o = (float*)part, a.part_ml = (float2*)(a.part_o + records * hd), a.parts = (int2*)(a.part_ml + records);
   a.R = R, a.K = K, a.nh = nh, a.nkv = nkv, a.hd = hd, a.W = W, a.n_pages = n_pages;
-  a.team = team, a.fewest = fewest, a.scale_log2 = scale * LOG2E, a.block_rows = rows;
+  a.team = team, a.group = nh / nkv, a.fewest = fewest, a.scale_log2 = scale * LOG2E, a.block_rows = rows;
   a.row_blocks = (K * (nh / nkv) + rows - 1) / rows;
   return (int)(hd > 128 ? wide_go(maps, a, blocks, warps, status, stream) : hd > 64 ? tc_for<128>(maps, a, blocks, status, stream)
                                                                                : tc_for<64>(maps, a, blocks, status, stream));
