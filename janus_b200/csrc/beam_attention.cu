@@ -7,13 +7,13 @@
 // head, so that a shared page is read once for all beams; behind it every beam's own pages follow, one beam after another, for
 // the rows of that beam alone.  A softmax over a union of keys joins from (maximum, sum, weighted values), whoever made the parts.
 //
-// Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their units (pages; 32 keys with heads
-// of more than 128 numbers).  Every block of threads (or team of warps) has an even, consecutive share of it, and the copy engine brings
+// Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their units (stages of two pages; 32
+// keys with heads of more than 128 numbers).  Every block of threads (or team of warps) has an even, consecutive share of it, and the copy engine brings
 // its units (128-byte swizzle), ahead across the ends of requests.  Where a share ends inside a block of rows, the sums go out as a partial
 // result; a second launch joins those.
 //
-// 32 heads over 8 of 128 numbers, 16 requests of 8 beams behind 6,000 to 24,000 tokens: 102 us for the 85 that 560 MB take; twice as
-// long 176 for 161, of 16 beams 134 for 94, with heads of 64 numbers 78 for 43; one request of 4 beams behind 300 9.5.
+// 32 heads over 8 of 128 numbers, 16 requests of 8 beams behind 6,000 to 24,000 tokens: 96 us for the 85 that 560 MB take; twice as
+// long 171 for 161, of 16 beams 131 for 94, with heads of 64 numbers 74 for 43; one request of 4 beams behind 300 9.0.
 #include <math_constants.h>
 #include <stdio.h>
 
@@ -24,7 +24,7 @@ namespace {
 typedef __nv_bfloat16 bf16;
 
 constexpr int PAGE = 64;
-constexpr int KEYS = 32;                           // keys of a unit with heads of more than 128 numbers; below that a unit is a page
+constexpr int KEYS = 32;                           // keys of a unit with heads of more than 128 numbers; below that a unit is two pages
 constexpr int MOST_BEAMS = 32;
 constexpr float RESCALE_LOG2 = 8.0f;               // weights may grow to 2^8 before what was summed up is scaled down
 constexpr float LOG2E = 1.4426950408889634f;
@@ -487,17 +487,18 @@ __global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(c
 // ---------------------------------------------------------------------------
 // Heads of up to 128 numbers: the tensor cores of tcgen05, keys on the tile's 128 rows, the beams' queries on its N columns, so that a
 // request's few rows are no padding:  S' = K Q' and O' = V' P', both accumulated in tensor memory.
-//   warp 0       walks the block's share of the list and brings its pages, two (128 keys) a stage, by the copy engine
+//   warp 0       walks the block's share of the list, stages of two pages (128 keys), and brings them by the copy engine
 //   warp 1       one lane issues the products; the next stage's scores before this one's values, where its keys are there
 //   warps 4-     two or four groups of four, each with its columns: a thread has one key.  Weights relative to a number a row that is raised
 //                only when a score passes it by RESCALE_LOG2 (then the sums and O' are scaled down); P to shared memory, a row a key
 // A stage's pages may be different beams' own; a mask of rows goes with each.
 //
-// With heads of 128 numbers and 32 rows a stage (64 KB) takes 1.41 us, which is memory's rate for a multiprocessor; 7 us go by before the
-// first scores are there, 10 between the first share's end and the last one's, 4 in the join.  64 rows take 1.6 us a stage, heads of 64 numbers 0.95 (for
-// 0.74): the chain of one stage, of which scores to weights is 1,450 cycles.  Measured on the first case: warp-level products (mma.sync) of
-// the beams' rows padded to 16, 116 us, and 214 for 64 rows, as each of four warps reads all keys from shared memory again; shares of 4 to 8
-// pages at least, no better; weights of two stages in turn, so that a stage need not wait for the products of the one before, level (103).
+// With heads of 128 numbers and 32 rows a stage (64 KB) takes 1.41 us, which is memory's rate for a multiprocessor; 3.5 us go by before the
+// first copy and 2 more before its scores, 15 between the first share's end and the last one's (multiprocessors are not served alike), 3.5 in
+// the join.  64 rows take 1.6 us a stage.  Measured on the first case: warp-level products (mma.sync) of the beams' rows padded to 16, 116 us,
+// and 214 for 64 rows, as each of four warps reads all keys from shared memory again; two groups of warps for 32 rows 102 for 99.5; lists of
+// single pages, where a share may begin within a stage, 98 for 96, and parted beams, whose shares are one stage, 17 for 13 us; weights of two
+// stages in turn, so that a stage need not wait for the products of the one before, level.
 // ---------------------------------------------------------------------------
 constexpr int SUB = 2, BLOCK_KEYS = SUB * PAGE;              // pages of a stage
 constexpr float NOTHING = -1e30f;                            // what weights are relative to before a row has seen a key
@@ -509,6 +510,8 @@ struct Info {                                                // of a stage
   int keys[SUB];
   unsigned long long rows[SUB][2];                           // that see the unit's keys
 };
+
+__device__ __forceinline__ int stages_of(const Rows& x) { return (x.units + SUB - 1) / SUB; }
 
 template <int HDC, int N>
 struct Tc {
@@ -650,7 +653,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
   const int blocks = a.R * a.row_blocks, chunk = (blocks + C::PLACES - 1) / C::PLACES, places = (blocks + chunk - 1) / chunk;
   constexpr int AHEAD = 4;
   for (int p0 = warp; p0 < places; p0 += C::THREADS / 32 * AHEAD) {
-    int units[AHEAD] = {};
+    int stages[AHEAD] = {};
     for (int i = 0; i < chunk; ++i) {
       int len[AHEAD], shared[AHEAD];
 #pragma unroll
@@ -661,12 +664,12 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         const int block = (p0 + u * (C::THREADS / 32)) * chunk + i;
-        if (block < blocks) units[u] += rows_of<PAGE>(a, block, len[u], shared[u]).units;
+        if (block < blocks) stages[u] += stages_of(rows_of<PAGE>(a, block, len[u], shared[u]));
       }
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
-      if (lane == 0 && p0 + u * (C::THREADS / 32) < places) sums[p0 + u * (C::THREADS / 32)] = units[u] * a.nkv;
+      if (lane == 0 && p0 + u * (C::THREADS / 32) < places) sums[p0 + u * (C::THREADS / 32)] = stages[u] * a.nkv;
   }
   jb::tc_fence_before();
   __syncthreads();
@@ -683,11 +686,10 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       if (lane >= o) up += t;
     }
     const int total = __shfl_sync(0xffffffffu, up, 31);
-    // shares are whole stages, so that where one ends inside a block of rows no stage is cut
-    const int per = max(a.fewest, (total + (int)gridDim.x - 1) / (int)gridDim.x + SUB - 1) / SUB * SUB;
+    const int per = max(a.fewest, (total + (int)gridDim.x - 1) / (int)gridDim.x);      // (a short list: no share with parts of two blocks of rows)
     const int begin = min((int)blockIdx.x * per, total), end = min(begin + per, total);
     const int owner = begin < end ? __ffs(__ballot_sync(0xffffffffu, begin < up)) - 1 : 0, before_owner = __shfl_sync(0xffffffffu, up - mine, owner);
-    int block = 0, kvh = 0, unit = 0, at = begin, st = 0, round = 0;
+    int block = 0, kvh = 0, turn = 0, stages = 1, at = begin, st = 0, round = 0;
     bool ok = true;
     Rows x{};
     if (begin >= end) {                                                // nothing: one stage that says so
@@ -701,11 +703,12 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       while (begin >= before + sums[t]) before += sums[t++];
       for (block = t * chunk;; ++block) {
         x = look_up<PAGE>(a, block);
-        if (begin < before + x.units * a.nkv) break;
-        before += x.units * a.nkv;
+        stages = stages_of(x);
+        if (begin < before + stages * a.nkv) break;
+        before += stages * a.nkv;
       }
-      kvh = (begin - before) / x.units;
-      unit = begin - before - kvh * x.units;
+      kvh = (begin - before) / stages;
+      turn = begin - before - kvh * stages;
     }
     unsigned long long joining[2] = {0ull, 0ull}, all[2] = {0ull, 0ull};
     int piece0 = 0, piece1 = 0;
@@ -725,21 +728,21 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       }
     };
     auto begun = [&]() {                                               // the shares that this head's pages lie in
-      piece0 = (at - unit) / per, piece1 = (at - unit + x.units - 1) / per;
+      piece0 = (at - turn) / per, piece1 = (at - turn + stages - 1) / per;
     };
-    // The lanes look up 32 units at a time; of a stage's, lanes 0 and 1 have one each.
+    // The lanes look up 32 pages at a time; of a stage's, lanes 0 and 1 have one each.
     int ahead = 0, keys = 0, beam = -1, page = -1;                     // the first one's place; the lane's: keys, beam (-1: all that share it), page
     auto find = [&]() {
-      ahead = unit;
+      ahead = turn * SUB;
       beam = -1, keys = 0, page = -1;
-      const int mine = unit + lane, j = mine - x.common;
-      const bool there = mine < x.units && at + lane < end;
+      const int mine = ahead + lane, j = mine - x.common;
+      const bool there = mine < x.units && at + lane / SUB < end;
       const int* entry = nullptr;
       if (there && j < 0) {
         keys = PAGE;
         entry = a.table + ((size_t)x.request * a.K + x.head) * a.W + mine;
       }
-      if (unit + 31 >= x.common) {                                     // beams' own
+      if (ahead + 31 >= x.common) {                                    // beams' own
         int b = 0;
         for (int k = 0; k < a.K; ++k) b += __shfl_sync(0xffffffffu, x.upto, k) <= j;
         const int who = min(b, 31), first = __shfl_sync(0xffffffffu, x.first, who), before = __shfl_sync(0xffffffffu, x.upto - x.own, who),
@@ -753,13 +756,13 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       if (entry != nullptr) page = *entry;
     };
     if (at < end) {
+      find();                                                          // (the rest while the pages' numbers are on their way)
       entered();
       begun();
-      find();
     }
     while (at < end) {
-      if (unit >= ahead + 32) find();                                  // (stages begin on even units)
-      const int n = min(min(SUB, x.units - unit), end - at), from = unit - ahead + (lane & 1);
+      if (turn * SUB >= ahead + 32) find();
+      const int n = min(SUB, x.units - turn * SUB), from = turn * SUB - ahead + (lane & 1);
       const int keys0 = __shfl_sync(0xffffffffu, keys, from), beam0 = __shfl_sync(0xffffffffu, beam, from), page0 = __shfl_sync(0xffffffffu, page, from);
       unsigned long long rows[2] = {joining[0], joining[1]};
       if (beam0 >= 0) {
@@ -777,7 +780,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       if (lane < SUB) to.keys[lane] = there ? keys0 : 0, to.rows[lane][0] = rows[0], to.rows[lane][1] = rows[1];
       const uint32_t full = kv_full + 8 * st, stage = base + st * C::STAGE;
       if (lane == 0) {
-        to.first = at == begin || unit == 0, to.last = unit + n == x.units || at + n == end, to.final_ = at + n == end, to.whole = whole;
+        to.first = at == begin || turn == 0, to.last = turn + 1 == stages || at + 1 == end, to.final_ = at + 1 == end, to.whole = whole;
         to.request = x.request, to.rho0 = x.rho0, to.n_rows = x.n_rows, to.kvh = kvh;
         to.piece0 = piece0, to.piece1 = piece1;
       }
@@ -796,16 +799,14 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
           jb::tma_load_2d(stage + h * C::SLAB + lane * PAGE * 128, &map_v, full, h * 64, row);
         }
       }
-      at += n, unit += n;
-      if (at < end && unit == x.units) {
-        unit = 0;
-        if (++kvh == a.nkv) {
-          kvh = 0;
-          x = look_up<PAGE>(a, ++block);
-          entered();
-        }
-        begun();
+      ++at, ++turn;
+      if (at < end && turn == stages) {
+        turn = 0;
+        const bool enters = ++kvh == a.nkv;
+        if (enters) kvh = 0, x = look_up<PAGE>(a, ++block), stages = stages_of(x);
         find();
+        if (enters) entered();
+        begun();
       }
       if (++st == C::STAGES) st = 0, ++round;
     }
@@ -1157,7 +1158,8 @@ cudaError_t allow(Kernel kernel, int bytes, bool (&ready)[64]) {
   return e;
 }
 // `shares`: of the list, how many.  A block of rows that is cut into many parts has a block of warps a row (6 requests of 5 beams that parted
-// long ago, 12 to a block of rows: 20 us the call, 23 by a warp a row), others a warp (16 of 8 beams behind 6,000 to 24,000: 105 and 109).
+// long ago, 12 to a block of rows: 20 us the call, 23 by a warp a row), others a warp (16 of 8 beams behind 6,000 to 24,000: 105 and 109;
+// both as the kernel before was then).
 cudaError_t join(const Args& a, int rows, int shares, cudaStream_t stream) {
   const int items = a.R * a.K * a.nh;
   if (shares > 4 * a.R * a.row_blocks * a.nkv) {

@@ -2880,11 +2880,11 @@ def beams_pay(rows: int, nkv: int, hd: int, max_kv_len: int) -> bool:
 
 @functools.lru_cache(maxsize=4096)
 def beam_attention_plan(groups: int, beams: int, nh: int, nkv: int, hd: int, max_kv_len: int):
-    """How `attention_beams` runs: (blocks, rows of a block's tile, warps of a block, warps of a team, units (pages; 32 keys) of a share at least)."""
+    """How `attention_beams` runs: (blocks, rows of a block's tile, warps of a block, warps of a team, units (two pages; 32 keys) of a share at least)."""
     rows = beams * (nh // nkv)
     if hd <= 128:
-        tile, unit = next((n for n in (16, 32, 64) if rows <= n), 128), 64
-        warps, team, teams, fewest = 0, 1, 1, 2
+        tile, unit = next((n for n in (16, 32, 64) if rows <= n), 128), 128
+        warps, team, teams, fewest = 0, 1, 1, 1
     else:
         team, warps, fewest = 1 if rows <= 16 else 2 if rows <= 32 else 4, 4, 2
         tile, teams, unit = 16 * team, 2 if team < 4 else 1, 32
