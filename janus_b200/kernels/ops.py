@@ -208,7 +208,7 @@ def _check(code: int, what: str, kernels: int = 1) -> None:
     if code >= 10000:
         names = {10001: "size not supported (see stderr)", 10002: "dtype not supported",
                  10003: "tensor map could not be encoded",
-                 10004: "an output lies over an input or another output"}
+                 10004: "what is made cannot lie where the old tables and lists do, or in each other's place"}
         raise KernelError(f"{what}: {names.get(code, 'error')} (code {code})")
     raise KernelError(f"{what}: CUDA error {code}")
 
