@@ -411,6 +411,57 @@ def test_attention_many_rows(K, group):
 
 
 @gpu
+@pytest.mark.parametrize("R, K, group, hd", [(1300, 2, 1, 64), (40, 32, 5, 72), (70, 3, 2, 160)])
+def test_attention_of_many_groups(R, K, group, hd):
+    """More blocks of rows than places that a block counts them in."""
+    rnd = random.Random(R)
+    kv_len, shared = [], []
+    for _ in range(R):
+        n = [rnd.randrange(0, 150) for _ in range(K)]
+        shared.append(rnd.randrange(0, 1 + min(n) // PAGE))
+        kv_len += n
+    check_attention(R, K, kv_len, shared, 1, group, hd, seed=R)
+
+
+@gpu
+def test_attention_pages_beyond_32_bits():
+    """Numbers of a cache that 32 bits cannot count, rows of 16 bytes up to the last that its rows' number has bits for."""
+    for nkv, hd, pages in ((1, 128, 300000), (8, 8, 2 ** 31 // (8 * PAGE) - 1)):
+        q, k, v, table, nh = attention_case(1, 2, [300, 290], [2], nkv, 2, hd, 4)
+        far = torch.tensor([pages - 1 - 7 * i if i % 2 else 3 * i for i in range(k.shape[0])])
+        big = [torch.empty(pages, nkv, PAGE, hd, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        for to, t in zip(big, (k, v)):
+            to[far.cuda()] = t.cuda()
+        moved = [[int(far[p]) if p >= 0 else -1 for p in row] for row in table]
+        out = empty(2, nh * hd, dtype=torch.bfloat16)
+        ops.attention_beams(q.cuda(), *big, out, ints(moved), ints([300, 290]), ints([2]), 2, nh, nkv, hd, PAGE, 0.3, Workspace(torch.device("cuda")), 300)
+        want, size = P.attention(q, k, v, table, [300, 290], nh, nkv, hd, 0.3)
+        off = (out.cpu().double().view(2, nh, hd) - want).abs()
+        assert float((off / (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -11) * size + 1e-30)).max()) <= 1.0
+        del big
+    with pytest.raises(ops.KernelError, match="attention_beams"):
+        args = _attention_args(K=1, nh=1, nkv=1, hd=8, device="cuda")
+        cache = torch.empty(2 ** 31 // PAGE, 1, PAGE, 8, dtype=torch.bfloat16, device="cuda")
+        ops.attention_beams(**{**args, "k_cache": cache, "v_cache": cache, "workspace": Workspace(torch.device("cuda"))})
+
+
+@gpu
+def test_select_logits_beyond_32_bits():
+    """The last of 2,100 rows of 1,050,000 logits (8.8 GB)."""
+    rows, V = 2100, 1050000
+    logits = torch.full((rows, V), NONE, device="cuda")
+    x, _ = random_logits(3, V, 9)
+    logits[-3:] = x.cuda()
+    scores = torch.full((rows // 3, 3), NONE)
+    scores[-1] = torch.tensor([-1.0, -1.2, -0.7])
+    out = run_select(logits, scores, [5])
+    parents, tokens, nxt, ep, et, es, gap = P.select(x, scores[-1:], [5])
+    assert gap > 2 * LSE_TOL
+    assert out["parents"][-1].tolist() == parents[0] and out["tokens"][-1].tolist() == tokens[0]
+    assert (out["parents"][:-1] == -1).all() and (out["next_scores"][:-1] == NONE).all() and (out["ended_tokens"][:-1] == -1).all()
+
+
+@gpu
 @pytest.mark.parametrize("hd", [40, 64, 128, 256])
 @pytest.mark.parametrize("K, group", [(4, 4), (5, 16), (11, 2)])
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
