@@ -24,7 +24,6 @@ namespace {
 typedef __nv_bfloat16 bf16;
 
 constexpr int PAGE = 64;
-constexpr int KEYS = 32;                           // keys of a unit with heads of more than 128 numbers; below that a unit is two pages
 constexpr int MOST_BEAMS = 32;
 constexpr float RESCALE_LOG2 = 8.0f;               // weights may grow to 2^8 before what was summed up is scaled down
 constexpr float LOG2E = 1.4426950408889634f;
@@ -40,35 +39,11 @@ struct Args {
   const int* shared;
   int R, K, nh, nkv, hd, W, n_pages;
   int group;                                       // query heads of a key head
-  int team, row_blocks, fewest;                    // warps of a team; blocks of rows of a request; units of a share at least
+  int row_blocks;                                  // blocks of rows of a request
   int block_rows;                                  // rows of a block
   float scale_log2;
 };
 
-constexpr int ROWS = 16;                           // of a warp
-
-struct Wide {                                      // heads of more than 128 numbers
-  static constexpr int HDC = 256, SLABS = HDC / 64, SLAB = KEYS * 128;     // 64 numbers of the keys of a unit
-  static constexpr int TILE = SLABS * SLAB, STAGE = 2 * TILE;              // keys, values
-  static constexpr int STAGES = 6, RING = STAGES * STAGE;
-  static constexpr int WARPS = 4, THREADS = 32 * WARPS;                    // at most
-  static constexpr int Q_SLAB = ROWS * 128, Q = SLABS * Q_SLAB;            // a warp's queries
-  static constexpr int SMEM = RING + WARPS * Q + STAGES * 24;              // ... and two barriers and a unit's description a stage
-  static_assert(SMEM <= 227 * 1024, "shared memory of a block");
-};
-
-__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t at) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
-}
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
@@ -100,12 +75,11 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* st
 struct Rows {
   int request, rho0, n_rows;        // rows rho0 .. of the request's beams * group
   int common, head;                 // pages that its beams share; the beam whose table lists them
-  int units;
-  int len, first, own, upto;        // of the lane's beam: keys, first page of its own, units of its own, of the beams up to it
+  int pages;                        // that they read: the shared ones, then each beam's own
+  int len, first, own, upto;        // of the lane's beam: keys, first page of its own, pages of its own, of the beams up to it
 };
 
 // ... from the lane's beam's length and the request's shared pages, as they stand in memory.
-template <int KEYS>
 __device__ __forceinline__ Rows rows_of(const Args& a, int block, int len, int shared) {
   const int lane = threadIdx.x & 31, G = a.group;
   Rows x;
@@ -117,8 +91,8 @@ __device__ __forceinline__ Rows rows_of(const Args& a, int block, int len, int s
   x.head = __ffs(__ballot_sync(0xffffffffu, lane < a.K && x.len == most)) - 1;
   x.common = min(max(shared, 0), most / PAGE);
   x.first = x.len < x.common * PAGE ? 0 : x.common;        // shorter beams read all they have by themselves
-  x.own = lane < a.K && (lane + 1) * G > x.rho0 && lane * G < x.rho0 + x.n_rows ? (x.len - x.first * PAGE + KEYS - 1) / KEYS : 0;
-  x.units = max(1, x.common * (PAGE / KEYS) + __reduce_add_sync(0xffffffffu, x.own));      // (rows without keys have a unit as well)
+  x.own = lane < a.K && (lane + 1) * G > x.rho0 && lane * G < x.rho0 + x.n_rows ? (x.len - x.first * PAGE + PAGE - 1) / PAGE : 0;
+  x.pages = max(1, x.common + __reduce_add_sync(0xffffffffu, x.own));       // (rows without keys have a place as well)
   x.upto = x.own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -127,362 +101,13 @@ __device__ __forceinline__ Rows rows_of(const Args& a, int block, int len, int s
   }
   return x;
 }
-template <int KEYS>
 __device__ __forceinline__ Rows look_up(const Args& a, int block) {
   const int lane = threadIdx.x & 31, request = a.row_blocks == 1 ? block : block / a.row_blocks;
-  return rows_of<KEYS>(a, block, lane < a.K ? a.kv_len[request * a.K + lane] : 0, a.shared[request]);
+  return rows_of(a, block, lane < a.K ? a.kv_len[request * a.K + lane] : 0, a.shared[request]);
 }
-// The units of a block, by one thread.
-template <int KEYS>
-__device__ __forceinline__ int count_units(const Args& a, int block) {
-  const int G = a.nh / a.nkv, all = a.block_rows, r = block / a.row_blocks, rho0 = block % a.row_blocks * all;
-  const int beam0 = rho0 / G, beam1 = (min(rho0 + all, a.K * G) - 1) / G;
-  int most = 0;
-#pragma unroll 8
-  for (int k = 0; k < a.K; ++k) most = max(most, min(max(a.kv_len[r * a.K + k], 0), a.W * PAGE));
-  const int common = min(max(a.shared[r], 0), most / PAGE);
-  int n = common * (PAGE / KEYS);
-#pragma unroll 8
-  for (int k = beam0; k <= beam1; ++k) {
-    const int len = min(max(a.kv_len[r * a.K + k], 0), a.W * PAGE);
-    n += (len - (len < common * PAGE ? 0 : common * PAGE) + KEYS - 1) / KEYS;
-  }
-  return max(1, n);
-}
-
 // Whether one of two numbers is infinite or none (an exponent of ones carries into the sign's place).  A weight of 0 silences neither, so values
 // of pages that not all rows read are looked at: such a value is left out and the rows that read it become no numbers, their neighbours stay.
 __device__ __forceinline__ uint32_t not_finite(uint32_t two) { return ((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
-
-// A place of the list as one thread walks it: the unit's beam (-1: all that share it), its first key, and where its page stands.
-struct Cursor {
-  int block, kvh, unit, units, shared_units;
-  int request, head, common, beam0, beam1, rho0, n_rows;
-  int beam, at, keys;
-  const int* entry;                 // of the table; null: a unit without keys
-
-  __device__ __forceinline__ int length(const Args& a, int b) const { return min(max(a.kv_len[request * a.K + b], 0), a.W * PAGE); }
-  __device__ __forceinline__ int own_from(int len) const { return len < common * PAGE ? 0 : common * PAGE; }
-  __device__ __forceinline__ void enter(const Args& a, int to) {
-    const int G = a.nh / a.nkv, all = a.block_rows;
-    rho0 = to % a.row_blocks * all, n_rows = min(all, a.K * G - rho0);
-    block = to, request = to / a.row_blocks, beam0 = rho0 / G, beam1 = (min(rho0 + all, a.K * G) - 1) / G;
-    int most = -1;
-    head = 0;
-    for (int k = 0; k < a.K; ++k) {
-      const int len = length(a, k);
-      if (len > most) most = len, head = k;
-    }
-    common = min(max(a.shared[request], 0), most / PAGE);
-    units = shared_units = common * (PAGE / KEYS);
-    for (int k = beam0; k <= beam1; ++k) {
-      const int len = length(a, k);
-      units += (len - own_from(len) + KEYS - 1) / KEYS;
-    }
-    units = max(1, units);
-  }
-  __device__ __forceinline__ void find(const Args& a) {      // the unit's keys
-    if (unit < shared_units) {
-      beam = -1, at = unit * KEYS, keys = KEYS;
-      entry = a.table + ((size_t)request * a.K + head) * a.W + at / PAGE;
-      return;
-    }
-    int left = unit - shared_units;
-    for (beam = beam0; beam <= beam1; ++beam) {
-      const int len = length(a, beam), from = own_from(len), own = (len - from + KEYS - 1) / KEYS;
-      if (left < own) {
-        at = from + left * KEYS, keys = min(KEYS, len - at);
-        entry = a.table + ((size_t)request * a.K + beam) * a.W + at / PAGE;
-        return;
-      }
-      left -= own;
-    }
-    beam = -1, at = keys = 0, entry = nullptr;
-  }
-  __device__ __forceinline__ bool step(const Args& a) {      // whether another block of rows has begun
-    bool entered = false;
-    if (++unit == units) {
-      unit = 0;
-      if (++kvh == a.nkv) kvh = 0, enter(a, block + 1), entered = true;
-    } else if (beam >= 0 && at + KEYS < length(a, beam)) {  // the next keys of the same beam
-      entry += (at % PAGE + KEYS) / PAGE;
-      at += KEYS;
-      keys = min(KEYS, length(a, beam) - at);
-      return false;
-    }
-    find(a);
-    return entered;
-  }
-};
-
-// ---------------------------------------------------------------------------
-// Heads of more than 128 numbers: a team of warps has a share of units of 32 keys, each warp 16 rows, by warp-level products (mma.sync); a stage
-// of 128 keys of tcgen05's tile would take half the shared memory.  The team's first warp asks for units, into a ring of the team's own.
-// ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(Wide::THREADS, 1) beam_attention_wide_kernel(const __grid_constant__ CUtensorMap map_k,
-                                                                               const __grid_constant__ CUtensorMap map_v, const Args a,
-                                                                               int* __restrict__ status) {
-  typedef Wide C;
-  constexpr int HDC = Wide::HDC;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, hd = a.hd, G = a.nh / a.nkv;
-  const int T = a.team, here = blockDim.x / 32 / T, team = warp / T, member = warp % T, stages = C::STAGES / here;
-  const uint32_t base = jb::smem_u32(smem), ring = base + team * stages * C::STAGE;
-  const uint32_t bars = base + C::RING + C::WARPS * C::Q + team * stages * 16;   // of a stage: full, empty
-  int2* about = reinterpret_cast<int2*>(smem + C::RING + C::WARPS * C::Q + C::STAGES * 16) + team * stages;   // keys, beam
-  if (member == 0 && lane == 0) {
-    for (int i = 0; i < stages; ++i) jb::mbar_init(bars + 16 * i, 1), jb::mbar_init(bars + 16 * i + 8, T);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncthreads();
-  jb::pdl_launch_dependents();
-  jb::pdl_wait();
-  // ---- the list's length, and this team's share ----
-  const int blocks = a.R * a.row_blocks, chunk = (blocks + 31) / 32, block0 = min(lane * chunk, blocks), block1 = min(block0 + chunk, blocks);
-  int mine = 0;
-  for (int i = block0; i < block1; ++i) mine += count_units<KEYS>(a, i);
-  mine *= a.nkv;
-  int up = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, up, o);
-    if (lane >= o) up += t;
-  }
-  const int total = __shfl_sync(0xffffffffu, up, 31), teams = gridDim.x * here, worker = blockIdx.x * here + team;
-  const int per = max(a.fewest, (total + teams - 1) / teams);
-  const int begin = min(worker * per, total), end = min(begin + per, total);
-  if (begin >= end) return;                                // (a whole team)
-  Rows x;
-  int block, kvh, unit;                                    // the place of the list
-  {
-    const int owner = __ffs(__ballot_sync(0xffffffffu, begin < up)) - 1;
-    int before = __shfl_sync(0xffffffffu, up - mine, owner);
-    for (block = owner * chunk;; ++block) {
-      x = look_up<KEYS>(a, block);
-      if (begin < before + x.units * a.nkv) break;
-      before += x.units * a.nkv;
-    }
-    kvh = (begin - before) / x.units;
-    unit = begin - before - kvh * x.units;
-  }
-  // ---- the team's first warp asks for units, ahead across the ends of rows ----
-  Cursor u{};
-  int page = -1, asked = begin, asked_stage = 0;
-  if (member == 0) {
-    u.enter(a, block);
-    u.kvh = kvh, u.unit = unit;
-    u.find(a);
-    page = u.entry != nullptr ? *u.entry : -1;
-  }
-  auto issue = [&]() {
-    if (lane == 0) {
-      const bool there = page >= 0 && page < a.n_pages;     // (no page: no keys)
-      const int row = ((there ? page : 0) * a.nkv + u.kvh) * PAGE + u.at % PAGE;
-      about[asked_stage] = make_int2(there ? u.keys : 0, u.beam);
-      const uint32_t full = bars + 16 * asked_stage, to = ring + asked_stage * C::STAGE;
-      jb::mbar_expect_tx(full, C::STAGE);                   // (behind the head's numbers the copy engine writes zeroes)
-#pragma unroll
-      for (int h = 0; h < C::SLABS; ++h) jb::tma_load_2d(to + h * C::SLAB, &map_k, full, h * 64, row);
-#pragma unroll
-      for (int h = 0; h < C::SLABS; ++h) jb::tma_load_2d(to + C::TILE + h * C::SLAB, &map_v, full, h * 64, row);
-    }
-    __syncwarp();
-    if (++asked_stage == stages) asked_stage = 0;
-    if (++asked < end) {                                    // (a unit's page is looked up a turn before it is asked for)
-      u.step(a);
-      page = u.entry != nullptr ? *u.entry : -1;
-    }
-  };
-  if (member == 0)
-    for (int i = 0; i < stages && asked < end; ++i) issue();
-  // Places of the operands in swizzled rows: 16 bytes `piece` of row r lie at piece ^ (r % 8), so that a step of 32 bytes is an
-  // exclusive or.
-  const int c = lane & 3, r8 = lane & 7;
-  const uint32_t k_lane = (r8 + ((lane >> 4) << 3)) * 128 + ((((lane >> 3) & 1) ^ r8) << 4);
-  const uint32_t v_lane = (lane & 15) * 128 + (((lane >> 4) ^ r8) << 4);
-  const uint32_t q_at = base + C::RING + warp * C::Q;
-  int beam_of[2] = {-1, -1};         // of this thread's rows; -1: no row
-  bool joins[2] = {false, false};    // whether the row reads the shared pages
-  bool all_join = false;
-  int beam_first = 0, beam_last = -1;     // of the warp's rows
-  float m[2], l[2], o[HDC / 8][4];
-  bool ok = true;
-  int st = 0, st_before = 0;
-  uint32_t phase = 0, phase_before = 0;
-  for (int i = begin; i < end; ++i) {
-    if (i > begin && member == 0 && asked < end) {         // the stage of the turn before, when all warps are done with it
-      ok = __all_sync(0xffffffffu, mbar_wait(bars + 16 * st_before + 8, phase_before, status, 54));
-      if (!ok) break;
-      issue();
-    }
-    if (i == begin || unit == 0) {
-      const int row0 = member * ROWS, rho0 = x.rho0 + row0, n_rows = min(ROWS, x.n_rows - row0);
-      beam_first = rho0 / G, beam_last = n_rows > 0 ? (rho0 + n_rows - 1) / G : -1;
-      bool every = true;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = (lane >> 2) + 8 * h;
-        const bool valid = row < n_rows;
-        beam_of[h] = valid ? (rho0 + row) / G : -1;
-        const int len = __shfl_sync(0xffffffffu, x.len, max(beam_of[h], 0));
-        joins[h] = valid && len >= x.common * PAGE;
-        every = every && (joins[h] || !valid);
-        m[h] = -CUDART_INF_F;
-        l[h] = 0.0f;
-      }
-      for (int ch = lane; ch < ROWS * C::SLABS * 8; ch += 32) {
-        const int row = ch / (C::SLABS * 8), piece = ch % (C::SLABS * 8), rho = rho0 + row;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < n_rows && piece * 8 < hd)
-          v = *reinterpret_cast<const uint4*>(a.q + (((size_t)x.request * a.K + rho / G) * a.nh + kvh * G + rho % G) * hd + piece * 8);
-        *reinterpret_cast<uint4*>(smem + C::RING + warp * C::Q + (piece / 8) * C::Q_SLAB + row * 128 + (((piece % 8) ^ (row & 7)) << 4)) = v;
-      }
-#pragma unroll
-      for (int j = 0; j < HDC / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-      all_join = __all_sync(0xffffffffu, every);           // (rows behind the last may do as they like)
-      __syncwarp();
-    }
-    ok = __all_sync(0xffffffffu, mbar_wait(bars + 16 * st, phase, status, 53));
-    if (!ok) break;
-    const int2 info = about[st];
-    const int keys = info.x, beam = info.y;
-    const uint32_t k_t = ring + st * C::STAGE, v_t = k_t + C::TILE;
-    // (units of another warp's beams are nothing to this one)
-    if (keys > 0 && (beam < 0 ? beam_last >= 0 : beam >= beam_first && beam <= beam_last)) {
-      if (keys < KEYS) {                                   // values behind the last key: a weight of 0 does not silence what is no number
-        for (int p = lane; p < (KEYS - keys) * C::SLABS * 8; p += 32) {
-          const int row = keys + p / (C::SLABS * 8), piece = p % (C::SLABS * 8);
-          *reinterpret_cast<uint4*>(smem + (v_t - base) + (piece / 8) * C::SLAB + row * 128 + ((piece % 8) << 4)) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        __syncwarp();
-      }
-      float s[4][4], s_odd[4][4];                          // (two chains of products, a half as long each)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = s_odd[j][e] = 0.0f;
-#pragma unroll
-      for (int ks = 0; ks < HDC / 16; ++ks) {
-        uint32_t qa[4], b[2][4];
-        const uint32_t at = k_t + (k_lane ^ ((ks % 4) << 5)) + (ks / 4) * C::SLAB;
-        ldmatrix_x4(b[0], at);
-        ldmatrix_x4(b[1], at + 16 * 128);
-        ldmatrix_x4(qa, q_at + (v_lane ^ ((ks % 4) << 5)) + (ks / 4) * C::Q_SLAB);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          mma_bf16(ks & 1 ? s_odd[2 * j] : s[2 * j], qa, b[j][0], b[j][1]);
-          mma_bf16(ks & 1 ? s_odd[2 * j + 1] : s[2 * j + 1], qa, b[j][2], b[j][3]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] += s_odd[j][e];
-      const bool masked = beam >= 0 || keys < KEYS || !all_join;
-      bool bad = false;                                    // some value is no finite number, and rows that do not see it are here
-      if (masked) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int h = e >> 1, key = j * 8 + 2 * c + (e & 1);
-            if (!(key < keys && (beam < 0 ? joins[h] : beam_of[h] == beam))) s[j][e] = -CUDART_INF_F;
-          }
-      }
-      float mx[2], use[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        mx[h] = fmaxf(fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1])),
-                      fmaxf(fmaxf(s[2][2 * h], s[2][2 * h + 1]), fmaxf(s[3][2 * h], s[3][2 * h + 1]))) * a.scale_log2;
-      // what weights are relative to is raised only when a score passes it by RESCALE_LOG2 (also the first number of all)
-      if (__any_sync(0xffffffffu, mx[0] > m[0] + RESCALE_LOG2 || mx[1] > m[1] + RESCALE_LOG2)) {
-        float corr[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-          const float top = fmaxf(m[h], mx[h]);
-          corr[h] = top == -CUDART_INF_F ? 1.0f : fast_exp2(m[h] - top);
-          m[h] = top;
-          l[h] *= corr[h];
-        }
-#pragma unroll
-        for (int j = 0; j < HDC / 8; ++j) o[j][0] *= corr[0], o[j][1] *= corr[0], o[j][2] *= corr[1], o[j][3] *= corr[1];
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) use[h] = m[h] == -CUDART_INF_F ? 0.0f : m[h];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = fast_exp2(fmaf(s[j][e], a.scale_log2, -use[e >> 1]));
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const uint32_t pa[4] = {pack_bf16(s[2 * kk][0], s[2 * kk][1]), pack_bf16(s[2 * kk][2], s[2 * kk][3]),
-                                pack_bf16(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack_bf16(s[2 * kk + 1][2], s[2 * kk + 1][3])};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) l[h] += (low_of(pa[h]) + high_of(pa[h])) + (low_of(pa[2 + h]) + high_of(pa[2 + h]));   // (as they are rounded)
-#pragma unroll
-        for (int j = 0; j < HDC / 8; j += 2) {
-          uint32_t b[4];
-          ldmatrix_x4_trans(b, v_t + (v_lane ^ ((j % 8) << 4)) + (j / 8) * C::SLAB + kk * 16 * 128);
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (not_finite(b[e])) b[e] = 0u, bad = true;
-          }
-          mma_bf16(o[j], pa, b[0], b[1]);
-          mma_bf16(o[j + 1], pa, b[2], b[3]);
-        }
-      }
-      if (masked && __any_sync(0xffffffffu, bad)) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (beam < 0 ? joins[h] : beam_of[h] == beam) l[h] = CUDART_NAN_F;
-      }
-      if (keys < KEYS) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // zeroes, before the copy engine writes there again
-    }
-    __syncwarp();
-    if (lane == 0) jb::mbar_arrive(bars + 16 * st + 8);
-    st_before = st, phase_before = phase;
-    if (++st == stages) st = 0, phase ^= 1;
-    if (unit + 1 == x.units || i + 1 == end) {             // the rows' keys end here, or the share does
-      const int start = i - unit, first = start / per, last = (start + x.units - 1) / per;
-      const bool complete = first == last;
-      const size_t record = ((size_t)worker * 2 + (worker == first ? 1 : 0)) * (ROWS * T) + member * ROWS;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float sum = l[h];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        const int row = (lane >> 2) + 8 * h, rho = x.rho0 + member * ROWS + row;
-        if (beam_of[h] < 0) continue;
-        const size_t item = ((size_t)x.request * a.K + beam_of[h]) * a.nh + kvh * G + rho % G;
-        if (c == 0) {
-          if (worker == first) a.parts[item] = make_int2(first, last - first + 1);
-          if (!complete) a.part_ml[record + row] = make_float2(sum == sum ? m[h] : 0.0f, sum);
-        }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-        for (int j = 0; j < HDC / 8; ++j) {
-          if (j * 8 < hd) {
-            if (complete) *reinterpret_cast<uint32_t*>(a.out + item * hd + j * 8 + 2 * c) = pack_bf16(o[j][2 * h] * inv, o[j][2 * h + 1] * inv);
-            else *reinterpret_cast<float2*>(a.part_o + (record + row) * hd + j * 8 + 2 * c) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
-          }
-        }
-      }
-    }
-    if (++unit == x.units) {
-      unit = 0;
-      if (++kvh == a.nkv) {
-        kvh = 0;
-        if (i + 1 < end) x = look_up<KEYS>(a, ++block);
-      }
-    }
-  }
-  // gave up: what is still on its way arrives before the block ends (or its wait gives up as well)
-  if (!ok && member == 0)
-    for (int turn = max(0, asked - begin - stages); turn < asked - begin; ++turn) mbar_wait(bars + 16 * (turn % stages), (turn / stages) & 1, status, 53);
-}
 
 // ---------------------------------------------------------------------------
 // Heads of up to 128 numbers: the tensor cores of tcgen05, keys on the tile's 128 rows, the beams' queries on its N columns, so that a
@@ -511,21 +136,35 @@ struct Info {                                                // of a stage
   unsigned long long rows[SUB][2];                           // that see the unit's keys
 };
 
-__device__ __forceinline__ int stages_of(const Rows& x) { return (x.units + SUB - 1) / SUB; }
+__device__ __forceinline__ int stages_of(const Rows& x) { return (x.pages + SUB - 1) / SUB; }
 
 template <int HDC, int N>
 struct Tc {
-  static constexpr int SLABS = HDC / 64, SLAB = BLOCK_KEYS * 128, STAGE = 2 * SLABS * SLAB;      // values, then keys
+  static constexpr int SLABS = HDC / 64, SLAB = BLOCK_KEYS * 128, SLOT = SLABS * SLAB;   // 64 numbers of a stage's keys; its keys, or its values
+  static constexpr int TILES = HDC > 128 ? 2 : 1;            // of 128 of the head's numbers in O'
   static constexpr int Q = SLABS * N * 128, P = (N > 64 ? 2 : 1) * BLOCK_KEYS * 128;
   static constexpr int MISC = 4 * N + 16 * N + 1200;         // ref, exchange, barriers and descriptions
-  static constexpr int FIT = (232448 - Q - P - MISC) / STAGE, STAGES = FIT > 6 ? 6 : FIT;
-  static constexpr int AT_Q = STAGES * STAGE, AT_P = AT_Q + Q, AT_REF = AT_P + P, AT_SWAP = AT_REF + 4 * N, AT_INFO = AT_SWAP + 16 * N,
-                       AT_BARS = AT_INFO + STAGES * (int)sizeof(Info), AT_BAD = AT_BARS + (3 * STAGES + 6) * 8 + 16, SMEM = AT_BAD + 128;
-  static constexpr int COLS = 3 * N <= 64 ? 64 : 3 * N <= 128 ? 128 : 3 * N <= 256 ? 256 : 512;  // two S', one O'
+  static constexpr int FIT = (232448 - Q - P - MISC) / SLOT, SLOTS = FIT > 12 ? 12 : FIT, INFOS = SLOTS / 2 + 1;
+  static constexpr int AT_Q = SLOTS * SLOT, AT_P = AT_Q + Q, AT_REF = AT_P + P, AT_SWAP = AT_REF + 4 * N, AT_INFO = AT_SWAP + 16 * N,
+                       AT_BARS = AT_INFO + INFOS * (int)sizeof(Info), BARS = 2 * SLOTS + INFOS + 6, AT_BAD = AT_BARS + BARS * 8 + 16, SMEM = AT_BAD + 128;
+  static constexpr int COLS = (2 + TILES) * N <= 64 ? 64 : (2 + TILES) * N <= 128 ? 128 : (2 + TILES) * N <= 256 ? 256 : 512;    // two S', O'
+  static_assert((2 + TILES) * N <= 512, "tensor memory");
   static constexpr int GROUPS = N > 16 ? 4 : 2, HALF = N / GROUPS;      // groups of four warps, columns of each
   static constexpr int PLACES = 1024;                                   // of the list, whose units are counted
   static constexpr int WARPS = 4 * GROUPS, THREADS = 128 + 32 * WARPS;
-  static_assert(STAGES >= 2 && SMEM <= 232448, "shared memory of a block");
+  static_assert(SLOTS >= 2 && SMEM <= 232448, "shared memory of a block");
+};
+
+// Where a ring's next stage stands: keys take a place, values the next one.
+template <int SLOTS>
+struct Ring {
+  int at;
+  uint32_t phase = 0;
+  __device__ __forceinline__ explicit Ring(int first) : at(first) {}
+  __device__ __forceinline__ void step(int by) {
+    at += by;
+    if (at >= SLOTS) at -= SLOTS, phase ^= 1;
+  }
 };
 
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
@@ -624,7 +263,7 @@ __device__ __forceinline__ void columns_summed(const float (&v)[C], float* out) 
 }
 
 template <int HDC, int N>
-__global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kernel(const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(const __grid_constant__ CUtensorMap map_k,
                                                                         const __grid_constant__ CUtensorMap map_v, const Args a,
                                                                         int* __restrict__ status) {
   typedef Tc<HDC, N> C;
@@ -633,14 +272,15 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
   const uint32_t base = jb::smem_u32(smem), q_at = base + C::AT_Q, p_at = base + C::AT_P;
   float* ref = reinterpret_cast<float*>(smem + C::AT_REF);             // [N] in units of log2
   float* swap = reinterpret_cast<float*>(smem + C::AT_SWAP);           // [4][N]
-  Info* info = reinterpret_cast<Info*>(smem + C::AT_INFO);             // [STAGES]
-  const uint32_t bars = base + C::AT_BARS, kv_full = bars, kv_empty = bars + 8 * C::STAGES, s_full = bars + 16 * C::STAGES, p_full = s_full + 16,
-                 pv_done = p_full + 8, q_full = pv_done + 8, o_full = q_full + 8, told = o_full + 8;
+  Info* info = reinterpret_cast<Info*>(smem + C::AT_INFO);             // [INFOS]
+  const uint32_t full = base + C::AT_BARS, empty = full + 8 * C::SLOTS, told = empty + 8 * C::SLOTS, s_full = told + 8 * C::INFOS, p_full = s_full + 16,
+                 pv_done = p_full + 8, q_full = pv_done + 8, o_full = q_full + 8;
   // [block of rows' parity][group][2]: rows that read a value that is no finite number, as the group has found
   unsigned long long (*bad)[C::GROUPS][2] = reinterpret_cast<unsigned long long (*)[C::GROUPS][2]>(smem + C::AT_BAD);
-  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::AT_BARS + (3 * C::STAGES + 6) * 8);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::AT_BARS + C::BARS * 8);
   if (tid == 0) {
-    for (int i = 0; i < C::STAGES; ++i) jb::mbar_init(kv_full + 8 * i, 1), jb::mbar_init(kv_empty + 8 * i, 1), jb::mbar_init(told + 8 * i, 1);
+    for (int i = 0; i < C::SLOTS; ++i) jb::mbar_init(full + 8 * i, 1), jb::mbar_init(empty + 8 * i, 1);
+    for (int i = 0; i < C::INFOS; ++i) jb::mbar_init(told + 8 * i, 1);
     jb::mbar_init(s_full, 1), jb::mbar_init(s_full + 8, 1), jb::mbar_init(p_full, C::WARPS), jb::mbar_init(pv_done, 1), jb::mbar_init(q_full, C::WARPS);
     jb::mbar_init(o_full, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -664,7 +304,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         const int block = (p0 + u * (C::THREADS / 32)) * chunk + i;
-        if (block < blocks) stages[u] += stages_of(rows_of<PAGE>(a, block, len[u], shared[u]));
+        if (block < blocks) stages[u] += stages_of(rows_of(a, block, len[u], shared[u]));
       }
     }
 #pragma unroll
@@ -686,23 +326,25 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       if (lane >= o) up += t;
     }
     const int total = __shfl_sync(0xffffffffu, up, 31);
-    const int per = max(a.fewest, (total + (int)gridDim.x - 1) / (int)gridDim.x);      // (a short list: no share with parts of two blocks of rows)
+    const int per = max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x);     // (a short list: no share with parts of two blocks of rows)
     const int begin = min((int)blockIdx.x * per, total), end = min(begin + per, total);
     const int owner = begin < end ? __ffs(__ballot_sync(0xffffffffu, begin < up)) - 1 : 0, before_owner = __shfl_sync(0xffffffffu, up - mine, owner);
-    int block = 0, kvh = 0, turn = 0, stages = 1, at = begin, st = 0, round = 0;
+    int block = 0, kvh = 0, turn = 0, stages = 1, at = begin;
+    Ring<C::SLOTS> slot(0);
+    Ring<C::INFOS> note(0);
     bool ok = true;
     Rows x{};
     if (begin >= end) {                                                // nothing: one stage that says so
       if (lane == 0) {
         info[0].final_ = 2;
         jb::mbar_arrive(told);
-        jb::mbar_arrive(kv_full);
+        jb::mbar_arrive(full);
       }
     } else {
       int before = before_owner, t = owner * each;
       while (begin >= before + sums[t]) before += sums[t++];
       for (block = t * chunk;; ++block) {
-        x = look_up<PAGE>(a, block);
+        x = look_up(a, block);
         stages = stages_of(x);
         if (begin < before + stages * a.nkv) break;
         before += stages * a.nkv;
@@ -736,7 +378,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       ahead = turn * SUB;
       beam = -1, keys = 0, page = -1;
       const int mine = ahead + lane, j = mine - x.common;
-      const bool there = mine < x.units && at + lane / SUB < end;
+      const bool there = mine < x.pages && at + lane / SUB < end;
       const int* entry = nullptr;
       if (there && j < 0) {
         keys = PAGE;
@@ -762,7 +404,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
     }
     while (at < end) {
       if (turn * SUB >= ahead + 32) find();
-      const int n = min(SUB, x.units - turn * SUB), from = turn * SUB - ahead + (lane & 1);
+      const int n = min(SUB, x.pages - turn * SUB), from = turn * SUB - ahead + (lane & 1);
       const int keys0 = __shfl_sync(0xffffffffu, keys, from), beam0 = __shfl_sync(0xffffffffu, beam, from), page0 = __shfl_sync(0xffffffffu, page, from);
       unsigned long long rows[2] = {joining[0], joining[1]};
       if (beam0 >= 0) {
@@ -772,94 +414,103 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       const bool there = lane < n && keys0 > 0 && page0 >= 0 && page0 < a.n_pages;    // (no page: no keys)
       const unsigned loads = __ballot_sync(0xffffffffu, there);
       const bool whole = __all_sync(0xffffffffu, lane >= SUB || (there && keys0 == PAGE && rows[0] == all[0] && rows[1] == all[1]));
-      if (round > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(kv_empty + 8 * st, (round - 1) & 1, status, 54));
-        if (!ok) break;
-      }
-      Info& to = info[st];
+      ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot.at, slot.phase ^ 1, status, 54));
+      if (!ok) break;
+      Info& to = info[note.at];
       if (lane < SUB) to.keys[lane] = there ? keys0 : 0, to.rows[lane][0] = rows[0], to.rows[lane][1] = rows[1];
-      const uint32_t full = kv_full + 8 * st, stage = base + st * C::STAGE;
       if (lane == 0) {
         to.first = at == begin || turn == 0, to.last = turn + 1 == stages || at + 1 == end, to.final_ = at + 1 == end, to.whole = whole;
         to.request = x.request, to.rho0 = x.rho0, to.n_rows = x.n_rows, to.kvh = kvh;
         to.piece0 = piece0, to.piece1 = piece1;
       }
       __syncwarp();
-      if (lane == 0) {
-        jb::mbar_arrive(told + 8 * st);
-        if (loads) jb::mbar_expect_tx(full, __popc(loads) * 2 * C::SLABS * PAGE * 128);
-        else jb::mbar_arrive(full);
-      }
-      __syncwarp();
-      if (there) {
-        const int row = (page0 * a.nkv + kvh) * PAGE;
+      if (lane == 0) jb::mbar_arrive(told + 8 * note.at);
+      note.step(1);
+      const int row = (page0 * a.nkv + kvh) * PAGE;
 #pragma unroll
-        for (int h = 0; h < C::SLABS; ++h) {
-          jb::tma_load_2d(stage + (C::SLABS + h) * C::SLAB + lane * PAGE * 128, &map_k, full, h * 64, row);
-          jb::tma_load_2d(stage + h * C::SLAB + lane * PAGE * 128, &map_v, full, h * 64, row);
+      for (int half = 0; half < 2; ++half) {                           // keys, values
+        if (half > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot.at, slot.phase ^ 1, status, 54));
+          if (!ok) break;
         }
+        const uint32_t here = full + 8 * slot.at, place = base + slot.at * C::SLOT + lane * PAGE * 128;
+        if (lane == 0) {
+          if (loads) jb::mbar_expect_tx(here, __popc(loads) * C::SLABS * PAGE * 128);
+          else jb::mbar_arrive(here);
+        }
+        __syncwarp();
+        if (there) {
+#pragma unroll
+          for (int h = 0; h < C::SLABS; ++h) jb::tma_load_2d(place + h * C::SLAB, half ? &map_v : &map_k, here, h * 64, row);
+        }
+        slot.step(1);
       }
+      if (!ok) break;
       ++at, ++turn;
       if (at < end && turn == stages) {
         turn = 0;
         const bool enters = ++kvh == a.nkv;
-        if (enters) kvh = 0, x = look_up<PAGE>(a, ++block), stages = stages_of(x);
+        if (enters) kvh = 0, x = look_up(a, ++block), stages = stages_of(x);
         find();
         if (enters) entered();
         begun();
       }
-      if (++st == C::STAGES) st = 0, ++round;
     }
     // gave up: what is still on its way arrives before the block ends (or its wait gives up as well)
     if (!ok && lane == 0)
-      for (int i = 0; i < C::STAGES; ++i) mbar_wait(kv_full + 8 * i, (i < st ? round : round - 1) & 1, status, 53);
+      for (int i = 0; i < C::SLOTS; ++i) mbar_wait(full + 8 * i, i < slot.at ? slot.phase : slot.phase ^ 1, status, 53);
   } else if (warp == 1) {
     if (elected()) {
       const uint32_t idesc_s = jb::instr_desc_bf16(N), idesc_o = jb::instr_desc_bf16(N) | (1u << 15) | (1u << 16);   // values and weights: MN-major
       const uint32_t o_col = tmem + 2 * N;
-      int st = 0, it = 0, turn = 0;
-      uint32_t phase = 0;
+      Ring<C::SLOTS> ks(0), vs(1);
+      Ring<C::INFOS> note(0);
+      int it = 0, turn = 0;
       bool ok = true, ahead = false;                                   // the stage's scores are under way already
-      auto scores = [&](int stage, int buffer) {
-        const uint32_t k_s = base + stage * C::STAGE + C::SLABS * C::SLAB;
+      auto scores = [&](int buffer) {
+        const uint32_t k_s = base + ks.at * C::SLOT;
         jb::tc_fence_after();
 #pragma unroll
         for (int h = 0; h < C::SLABS; ++h) {
           const uint64_t k = jb::smem_desc_sw128(k_s + h * C::SLAB), q = jb::smem_desc_sw128(q_at + h * N * 128);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) jb::umma_bf16(tmem + buffer * N, k + 2 * ks, q + 2 * ks, idesc_s, (h | ks) ? 1u : 0u);
+          for (int i = 0; i < 4; ++i) jb::umma_bf16(tmem + buffer * N, k + 2 * i, q + 2 * i, idesc_s, (h | i) ? 1u : 0u);
         }
+        jb::umma_commit(empty + 8 * ks.at);
         jb::umma_commit(s_full + 8 * buffer);
+        ks.step(2);
       };
       for (;; ++it) {
+        const Info& x = info[note.at];
         if (!ahead) {
-          ok = mbar_wait(kv_full + 8 * st, phase, status, 53);
-          if (!ok || info[st].final_ == 2) break;
-          if (info[st].first) ok = mbar_wait(q_full, turn++ & 1, status, 55);
+          ok = mbar_wait(full + 8 * ks.at, ks.phase, status, 53) && mbar_wait(told + 8 * note.at, note.phase, status, 53);
+          if (!ok || x.final_ == 2) break;
+          if (x.first) ok = mbar_wait(q_full, turn++ & 1, status, 55);
           if (!ok) break;
-          scores(st, it & 1);
+          scores(it & 1);
         }
-        const bool first = info[st].first, last = info[st].last, final_ = info[st].final_;
-        const int st1 = st + 1 == C::STAGES ? 0 : st + 1;
-        const uint32_t phase1 = st1 == 0 ? phase ^ 1 : phase;
+        const bool first = x.first, last = x.last, final_ = x.final_;
         ahead = false;
-        if (!last && mbar_test(kv_full + 8 * st1, phase1)) {
-          scores(st1, (it + 1) & 1);
+        if (!last && mbar_test(full + 8 * ks.at, ks.phase)) {
+          scores((it + 1) & 1);
           ahead = true;
         }
-        ok = mbar_wait(p_full, it & 1, status, 56);
+        ok = mbar_wait(full + 8 * vs.at, vs.phase, status, 53) && mbar_wait(p_full, it & 1, status, 56);
         if (!ok) break;
         jb::tc_fence_after();
-        const uint32_t v_s = base + st * C::STAGE;
+        const uint32_t v_s = base + vs.at * C::SLOT;
 #pragma unroll
-        for (int ks = 0; ks < BLOCK_KEYS / 16; ++ks)
-          jb::umma_bf16(o_col, desc_mn_sw128(v_s + ks * 2048, C::SLAB, 1024), desc_mn_sw128(p_at + ks * 2048, BLOCK_KEYS * 128, 1024), idesc_o,
-                        first && ks == 0 ? 0u : 1u);
-        jb::umma_commit(kv_empty + 8 * st);
+        for (int m = 0; m < C::TILES; ++m)
+#pragma unroll
+          for (int i = 0; i < BLOCK_KEYS / 16; ++i)
+            jb::umma_bf16(o_col + m * N, desc_mn_sw128(v_s + m * 2 * C::SLAB + i * 2048, C::SLAB, 1024),
+                          desc_mn_sw128(p_at + i * 2048, BLOCK_KEYS * 128, 1024), idesc_o, first && i == 0 ? 0u : 1u);
+        jb::umma_commit(empty + 8 * vs.at);
         jb::umma_commit(pv_done);
         if (last) jb::umma_commit(o_full), jb::mbar_arrive(o_full);    // (by itself as well: what the groups wrote before is seen behind it)
         if (final_) break;
-        st = st1, phase = phase1;
+        vs.step(2);
+        note.step(1);
       }
     }
   } else if (warp >= 4) {
@@ -867,14 +518,15 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     float* my_ref = ref + c0;
     float l[C::HALF];
-    int st = 0, turn = 0, request = 0, rho0 = 0, n_rows = 0, kvh = 0;
-    uint32_t phase = 0;
+    Ring<C::SLOTS> vs(1);
+    Ring<C::INFOS> note(0);
+    int turn = 0, request = 0, rho0 = 0, n_rows = 0, kvh = 0;
     bool ok = true, first = true;
     for (int it = 0;; ++it) {
       // a block of rows begins: its queries, by all groups, while its first keys are on their way
-      const Info* x = info + st;
+      const Info* x = info + note.at;
+      ok = ok && mbar_wait(told + 8 * note.at, note.phase, status, 53);
       if (first) {
-        ok = ok && mbar_wait(told + 8 * st, phase, status, 53);
         if (group_any(1 + group, !ok)) break;                          // (a wait ran out, of one of the group's warps: all leave)
         request = x->request, rho0 = x->rho0, n_rows = x->n_rows, kvh = x->kvh;
         if (x->final_ == 2) break;                                     // (the block has no share)
@@ -893,7 +545,6 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
 #pragma unroll
         for (int c = 0; c < C::HALF; ++c) l[c] = 0.0f;
       }
-      ok = ok && mbar_wait(kv_full + 8 * st, phase, status, 53);
       if (group_any(1 + group, !ok)) break;
       const bool last = x->last;
       const int final_ = x->final_, sub = quarter >> 1, in_page = (quarter & 1) * 32 + lane, keys = x->keys[sub];
@@ -904,7 +555,8 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
         if (in_page >= keys) rows = 0ull;
         // values behind the last key, or that are no finite numbers: a weight of 0 does not silence them (a part of the head's numbers a
         // group; while the scores are made)
-        uint8_t* values = smem + st * C::STAGE + key * 128;
+        ok = ok && mbar_wait(full + 8 * vs.at, vs.phase, status, 53);
+        uint8_t* values = smem + vs.at * C::SLOT + key * 128;
         uint32_t odd = 0u;
 #pragma unroll
         for (int p = 0; p < C::SLABS * 8 / C::GROUPS; ++p) {
@@ -979,12 +631,15 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
             f[e] = swap[c0 + c + e], l[c + e] *= f[e];
           }
           if (!first) {
-            float v[8];
-            jb::tmem_ld8(lanes + 2 * N + c0 + c, v);
-            jb::tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= f[e];
-            tmem_st8(lanes + 2 * N + c0 + c, v);
+            for (int m = 0; m < C::TILES; ++m) {
+              float v[8];
+              jb::tmem_ld8(lanes + (2 + m) * N + c0 + c, v);
+              jb::tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] *= f[e];
+              tmem_st8(lanes + (2 + m) * N + c0 + c, v);
+            }
           }
         }
         tmem_st_wait();
@@ -1039,17 +694,20 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
         group_any(1 + group, false);
 #pragma unroll
         for (int c = 0; c < C::HALF; c += 8) {
-          float v[8];
-          jb::tmem_ld8(lanes + 2 * N + c0 + c, v);
-          jb::tmem_ld_wait();
-          if (key < hd) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int row = c0 + c + e;
-              if (row < n_rows) {
-                const size_t to = (size_t)__float_as_int(swap[N + row]) * hd + key;
-                if (complete) a.out[to] = __float2bfloat16_rn(v[e] * swap[row]);
-                else a.part_o[to] = v[e];
+          for (int m = 0; m < C::TILES; ++m) {
+            float v[8];
+            jb::tmem_ld8(lanes + (2 + m) * N + c0 + c, v);
+            jb::tmem_ld_wait();
+            if (key + 128 * m < hd) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int row = c0 + c + e;
+                if (row < n_rows) {
+                  const size_t to = (size_t)__float_as_int(swap[N + row]) * hd + key + 128 * m;
+                  if (complete) a.out[to] = __float2bfloat16_rn(v[e] * swap[row]);
+                  else a.part_o[to] = v[e];
+                }
               }
             }
           }
@@ -1059,7 +717,8 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_tc_kern
       }
       first = last;
       if (final_) break;
-      if (++st == C::STAGES) st = 0, phase ^= 1;
+      vs.step(2);
+      note.step(1);
     }
   }
   jb::tc_fence_before();
@@ -1169,63 +828,51 @@ cudaError_t join(const Args& a, int rows, int shares, cudaStream_t stream) {
   jb::Launch cfg(dim3((items + JOIN_WARPS - 1) / JOIN_WARPS), dim3(32 * JOIN_WARPS), 0, stream);
   return cudaLaunchKernelEx(&cfg.c, beam_attention_join_kernel<1>, a, rows, shares);
 }
-cudaError_t wide_go(const CUtensorMap* maps, const Args& a, int blocks, int warps, int* status, cudaStream_t stream) {
-  static bool ready[64] = {};
-  cudaError_t e = allow(beam_attention_wide_kernel, Wide::SMEM, ready);
-  if (e != cudaSuccess) return e;
-  jb::Launch cfg(dim3(blocks), dim3(32 * warps), Wide::SMEM, stream);
-  e = cudaLaunchKernelEx(&cfg.c, beam_attention_wide_kernel, maps[0], maps[1], a, status);
-  return e != cudaSuccess ? e : join(a, a.block_rows, blocks * (warps / a.team), stream);
-}
-
 template <int HDC, int N>
 cudaError_t tc_go(const CUtensorMap* maps, Args a, int blocks, int* status, cudaStream_t stream) {
   typedef Tc<HDC, N> C;
   static bool ready[64] = {};
-  cudaError_t e = allow(beam_attention_tc_kernel<HDC, N>, C::SMEM, ready);
+  cudaError_t e = allow(beam_attention_kernel<HDC, N>, C::SMEM, ready);
   if (e != cudaSuccess) return e;
   jb::Launch cfg(dim3(blocks), dim3(C::THREADS), C::SMEM, stream);
-  e = cudaLaunchKernelEx(&cfg.c, beam_attention_tc_kernel<HDC, N>, maps[0], maps[1], a, status);
+  e = cudaLaunchKernelEx(&cfg.c, beam_attention_kernel<HDC, N>, maps[0], maps[1], a, status);
   return e != cudaSuccess ? e : join(a, N, blocks, stream);
 }
 template <int HDC>
 cudaError_t tc_for(const CUtensorMap* maps, const Args& a, int blocks, int* status, cudaStream_t stream) {
-  return a.block_rows == 16 ? tc_go<HDC, 16>(maps, a, blocks, status, stream) : a.block_rows == 32 ? tc_go<HDC, 32>(maps, a, blocks, status, stream)
-         : a.block_rows == 64 ? tc_go<HDC, 64>(maps, a, blocks, status, stream) : tc_go<HDC, 128>(maps, a, blocks, status, stream);
+  if (a.block_rows == 16) return tc_go<HDC, 16>(maps, a, blocks, status, stream);
+  if (a.block_rows == 32) return tc_go<HDC, 32>(maps, a, blocks, status, stream);
+  if constexpr (HDC <= 128)
+    if (a.block_rows == 128) return tc_go<HDC, 128>(maps, a, blocks, status, stream);
+  return tc_go<HDC, 64>(maps, a, blocks, status, stream);
 }
 
 }  // namespace
 
-// part: float32 scratch of `records` * (hd + 2) + 2 R K nh numbers.  rows: of a block.  Heads of up to 128 numbers: rows 16, 32, 64 or 128, warps
-// and team are not used, records blocks * 2 * rows; larger ones: rows 16 * team, team a divisor of warps, records blocks * warps * 2 * 16.
+// part: float32 scratch of 2 * blocks * rows * (hd + 2) + 2 R K nh numbers.  rows: of a block, 16, 32, 64 or (heads of up to 128 numbers) 128.
 JB_EXPORT int jb_attention_beams(const void* q, const void* k_cache, const void* v_cache, void* out, void* part, const int* table,
                                  const int* kv_len, const int* shared, int R, int K, int nh, int nkv, int hd, int W, int n_pages, int blocks,
-                                 int rows, int warps, int team, int fewest, float scale, int* status, cudaStream_t stream) {
+                                 int rows, float scale, int* status, cudaStream_t stream) {
   JB_REFUSE(R < 1 || K < 1 || K > MOST_BEAMS || nkv < 1 || nh < nkv || nh % nkv || hd < 8 || hd > 256 || hd % 8 || W < 1 || W > 0x7fffffff / PAGE ||
-                n_pages < 1 || (long long)R * K * nh > 0x7fffffffLL || (long long)n_pages * nkv * PAGE > 0x7fffffffLL || blocks < 1 || fewest < 1 || !(scale > 0.0f),
+                n_pages < 1 || (long long)R * K * nh > 0x7fffffffLL || (long long)n_pages * nkv * PAGE > 0x7fffffffLL || blocks < 1 || !(scale > 0.0f),
             "attention_beams: %d groups of %d beams, %d heads over %d of %d numbers, %d pages a row of %d, %d blocks, scale %g", R, K, nh, nkv, hd,
             W, n_pages, blocks, scale);
-  if (hd <= 128)
-    JB_REFUSE(rows != 16 && rows != 32 && rows != 64 && rows != 128, "attention_beams: blocks of %d rows", rows);
-  else
-    JB_REFUSE(team < 1 || warps < team || warps % team || warps > Wide::WARPS || warps / team > 3 || rows != ROWS * team,
-              "attention_beams: %d rows for teams of %d of %d warps", rows, team, warps);
+  JB_REFUSE(rows != 16 && rows != 32 && rows != 64 && (rows != 128 || hd > 128), "attention_beams: blocks of %d rows", rows);
   JB_REFUSE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)part) % 16, "attention_beams: q, out or workspace not on a boundary of 16 bytes");
   const size_t row_bytes = (size_t)R * K * nh * hd * 2, cache_bytes = (size_t)n_pages * nkv * PAGE * hd * 2;
   auto over = [&](const void* other, size_t bytes) { return (uintptr_t)out < (uintptr_t)other + bytes && (uintptr_t)other < (uintptr_t)out + row_bytes; };
   if (over(q, row_bytes) || over(k_cache, cache_bytes) || over(v_cache, cache_bytes)) return JB_ERR_OVERLAP;
   CUtensorMap maps[2];
-  const int keys = hd > 128 ? KEYS : PAGE;
-  if (!jb::make_map_64(&maps[0], k_cache, (uint64_t)n_pages * nkv * PAGE, hd, keys, true) ||
-      !jb::make_map_64(&maps[1], v_cache, (uint64_t)n_pages * nkv * PAGE, hd, keys, true))
+  if (!jb::make_map_64(&maps[0], k_cache, (uint64_t)n_pages * nkv * PAGE, hd, PAGE, true) ||
+      !jb::make_map_64(&maps[1], v_cache, (uint64_t)n_pages * nkv * PAGE, hd, PAGE, true))
     return JB_ERR_TENSORMAP;
   Args a{};
   a.q = (const bf16*)q, a.out = (bf16*)out, a.table = table, a.kv_len = kv_len, a.shared = shared;
-  const size_t records = hd <= 128 ? (size_t)blocks * 2 * rows : (size_t)blocks * warps * ROWS * 2;
+  const size_t records = (size_t)blocks * 2 * rows;
   a.part_o = (float*)part, a.part_ml = (float2*)(a.part_o + records * hd), a.parts = (int2*)(a.part_ml + records);
   a.R = R, a.K = K, a.nh = nh, a.nkv = nkv, a.hd = hd, a.W = W, a.n_pages = n_pages;
-  a.team = team, a.group = nh / nkv, a.fewest = fewest, a.scale_log2 = scale * LOG2E, a.block_rows = rows;
+  a.group = nh / nkv, a.scale_log2 = scale * LOG2E, a.block_rows = rows;
   a.row_blocks = (K * (nh / nkv) + rows - 1) / rows;
-  return (int)(hd > 128 ? wide_go(maps, a, blocks, warps, status, stream) : hd > 64 ? tc_for<128>(maps, a, blocks, status, stream)
-                                                                               : tc_for<64>(maps, a, blocks, status, stream));
+  return (int)(hd > 128 ? tc_for<256>(maps, a, blocks, status, stream) : hd > 64 ? tc_for<128>(maps, a, blocks, status, stream)
+                                                                                : tc_for<64>(maps, a, blocks, status, stream));
 }

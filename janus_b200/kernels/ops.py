@@ -103,7 +103,7 @@ _SIGNATURES = {
     "jb_step_tables": "pp", "jb_attention_prefix_f32": "ppp", "jb_attention_prefix_bf16": "pppp",
     "jb_verify_drafts": "pp",
     "jb_beam_select": "pp", "jb_fork_pages": "pp", "jb_copy_pages": "pppipppiiip", "jb_reorder_rows": "ppippiiip",
-    "jb_attention_beams": "ppppppppiiiiiiiiiiiifpp",
+    "jb_attention_beams": "ppppppppiiiiiiiiifpp",
     "jb_gather_rows": "ppiipppiiip", "jb_latent_attention": "ppppppppiiiiiiifiipp", "jb_attention_tc_matrix": "ppppppiiiiiiiifpipp",
 }
 _CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "u": ctypes.c_ulonglong,
@@ -2859,12 +2859,11 @@ def attention_beams(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                   ("block table", "kv_len", "shared pages"))
     if not 0.0 < scale < float("inf"):
         raise KernelError(f"attention_beams: scale {scale}")
-    blocks, rows, warps, team, fewest = beam_attention_plan(N // beams, beams, nh, nkv, hd, min(int(max_kv_len), W * page_size))
-    records = blocks * 2 * (rows if hd <= 128 else 16 * warps)
-    part = workspace.get("beam_parts", (records * (hd + 2) + 2 * N * nh,), torch.float32)
+    blocks, rows = beam_attention_plan(N // beams, beams, nh, nkv, hd, min(int(max_kv_len), W * page_size))
+    part = workspace.get("beam_parts", (2 * blocks * rows * (hd + 2) + 2 * N * nh,), torch.float32)
     _check(_lib("beam_attention").jb_attention_beams(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), part.data_ptr(), block_table.data_ptr(), kv_len.data_ptr(),
-        shared.data_ptr(), N // beams, beams, nh, nkv, hd, W, k_cache.shape[0], blocks, rows, warps, team, fewest, float(scale),
+        shared.data_ptr(), N // beams, beams, nh, nkv, hd, W, k_cache.shape[0], blocks, rows, float(scale),
         kernel_status(q.device).data_ptr(), _stream()), "attention_beams", kernels=2)
 
 
@@ -2880,14 +2879,8 @@ def beams_pay(rows: int, nkv: int, hd: int, max_kv_len: int) -> bool:
 
 @functools.lru_cache(maxsize=4096)
 def beam_attention_plan(groups: int, beams: int, nh: int, nkv: int, hd: int, max_kv_len: int):
-    """How `attention_beams` runs: (blocks, rows of a block's tile, warps of a block, warps of a team, units (two pages; 32 keys) of a share at least)."""
+    """How `attention_beams` runs: (blocks, rows of a block's tile).  Tiles of 128 rows have no room for queries of more than 128 numbers."""
     rows = beams * (nh // nkv)
-    if hd <= 128:
-        tile, unit = next((n for n in (16, 32, 64) if rows <= n), 128), 128
-        warps, team, teams, fewest = 0, 1, 1, 1
-    else:
-        team, warps, fewest = 1 if rows <= 16 else 2 if rows <= 32 else 4, 4, 2
-        tile, teams, unit = 16 * team, 2 if team < 4 else 1, 32
-        warps = team * teams
-    units = groups * -(-rows // tile) * nkv * -(-max_kv_len // unit) * (beams + 1)      # (at most: nothing may be shared)
-    return max(1, min(SM_COUNT_TARGET // 2, -(-units // (fewest * teams)))), tile, warps, team, fewest
+    tile = next((n for n in (16, 32, 64) if rows <= n), 128 if hd <= 128 else 64)
+    stages = groups * -(-rows // tile) * nkv * -(-max_kv_len // 128) * (beams + 1)      # (at most: nothing may be shared)
+    return max(1, min(SM_COUNT_TARGET // 2, stages)), tile
