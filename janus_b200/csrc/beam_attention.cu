@@ -463,6 +463,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
     if (elected()) {
       const uint32_t idesc_s = jb::instr_desc_bf16(N), idesc_o = jb::instr_desc_bf16(N) | (1u << 15) | (1u << 16);   // values and weights: MN-major
       const uint32_t o_col = tmem + 2 * N;
+      const uint64_t p = desc_mn_sw128(p_at, BLOCK_KEYS * 128, 1024);
       Ring<C::SLOTS> ks(0), vs(1);
       Ring<C::INFOS> note(0);
       int it = 0, turn = 0;
@@ -498,15 +499,14 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
         ok = mbar_wait(full + 8 * vs.at, vs.phase, status, 53) && mbar_wait(p_full, it & 1, status, 56);
         if (!ok) break;
         jb::tc_fence_after();
-        const uint32_t v_s = base + vs.at * C::SLOT;
+        const uint64_t v = desc_mn_sw128(base + vs.at * C::SLOT, C::SLAB, 1024);         // (further on by 16 bytes a unit)
 #pragma unroll
         for (int m = 0; m < C::TILES; ++m)
 #pragma unroll
           for (int i = 0; i < BLOCK_KEYS / 16; ++i)
-            jb::umma_bf16(o_col + m * N, desc_mn_sw128(v_s + m * 2 * C::SLAB + i * 2048, C::SLAB, 1024),
-                          desc_mn_sw128(p_at + i * 2048, BLOCK_KEYS * 128, 1024), idesc_o, first && i == 0 ? 0u : 1u);
-        jb::umma_commit(empty + 8 * vs.at);
+            jb::umma_bf16(o_col + m * N, v + (m * 2 * C::SLAB + i * 2048) / 16, p + i * 2048 / 16, idesc_o, first && i == 0 ? 0u : 1u);
         jb::umma_commit(pv_done);
+        jb::umma_commit(empty + 8 * vs.at);
         if (last) jb::umma_commit(o_full), jb::mbar_arrive(o_full);    // (by itself as well: what the groups wrote before is seen behind it)
         if (final_) break;
         vs.step(2);
