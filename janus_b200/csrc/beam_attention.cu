@@ -477,8 +477,8 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
 #pragma unroll
           for (int i = 0; i < 4; ++i) jb::umma_bf16(tmem + buffer * N, k + 2 * i, q + 2 * i, idesc_s, (h | i) ? 1u : 0u);
         }
-        jb::umma_commit(empty + 8 * ks.at);
         jb::umma_commit(s_full + 8 * buffer);
+        jb::umma_commit(empty + 8 * ks.at);
         ks.step(2);
       };
       for (;; ++it) {
