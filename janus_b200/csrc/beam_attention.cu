@@ -7,13 +7,13 @@
 // head, so that a shared page is read once for all beams; behind it every beam's own pages follow, one beam after another, for
 // the rows of that beam alone.  A softmax over a union of keys joins from (maximum, sum, weighted values), whoever made the parts.
 //
-// Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their units (stages of two pages; 32
-// keys with heads of more than 128 numbers).  Every block of threads (or team of warps) has an even, consecutive share of it, and the copy engine brings
-// its units (128-byte swizzle), ahead across the ends of requests.  Where a share ends inside a block of rows, the sums go out as a partial
-// result; a second launch joins those.
+// Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their stages of two pages (128 keys).
+// Every block of threads has an even, consecutive share of it, and the copy engine brings its pages (128-byte swizzle), ahead across the
+// ends of requests.  Where a share ends inside a block of rows, the sums go out as a partial result; a second launch joins those.
 //
-// 32 heads over 8 of 128 numbers, 16 requests of 8 beams behind 6,000 to 24,000 tokens: 96 us for the 85 that 560 MB take; twice as
-// long 171 for 161, of 16 beams 131 for 94, with heads of 64 numbers 74 for 43; one request of 4 beams behind 300 9.0.
+// 32 heads over 8 of 128 numbers, 16 requests of 8 beams behind 6,000 to 24,000 tokens: 97 us for the 85 that 560 MB take; twice as
+// long 172 for 161, of 16 beams 122 for 94, with heads of 64 numbers 78 for 43; 16 heads over 4 of 256 104 for 86, of 16 beams 142
+// for 94; one request of 4 beams behind 300 9.1.
 #include <math_constants.h>
 #include <stdio.h>
 
@@ -31,9 +31,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 struct Args {
   const bf16* q;
   bf16* out;
-  float* part_o;       // [teams][2][rows of a team][hd], not divided by their sums; of a share's first rows (0) and last rows (1)
+  float* part_o;       // [shares][2][rows of a block][hd], not divided by their sums; of a share's first rows (0) and last rows (1)
   float2* part_ml;     // ... maximum (in units of log2), sum
-  int2* parts;         // [beams][heads]: first team with a part of the row, number of teams
+  int2* parts;         // [beams][heads]: first share with a part of the row, number of shares
   const int* table;
   const int* kv_len;
   const int* shared;
@@ -110,20 +110,23 @@ __device__ __forceinline__ Rows look_up(const Args& a, int block) {
 __device__ __forceinline__ uint32_t not_finite(uint32_t two) { return ((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
 
 // ---------------------------------------------------------------------------
-// Heads of up to 128 numbers: the tensor cores of tcgen05, keys on the tile's 128 rows, the beams' queries on its N columns, so that a
-// request's few rows are no padding:  S' = K Q' and O' = V' P', both accumulated in tensor memory.
-//   warp 0       walks the block's share of the list, stages of two pages (128 keys), and brings them by the copy engine
-//   warp 1       one lane issues the products; the next stage's scores before this one's values, where its keys are there
+// The tensor cores of tcgen05, keys on the tile's 128 rows, the beams' queries on its N columns, so that a request's few rows are no padding:
+// S' = K Q' and O' = V' P' (two tiles of it for heads of more than 128 numbers), both accumulated in tensor memory.
+//   warp 0       walks the block's share of the list and brings keys and values, each to the next place of a ring, by the copy engine
+//   warp 1       one lane issues the products; the next stage's scores before this one's values, where its keys are there.  Keys give their place
+//                back with the scores, values with their own product
 //   warps 4-     two or four groups of four, each with its columns: a thread has one key.  Weights relative to a number a row that is raised
 //                only when a score passes it by RESCALE_LOG2 (then the sums and O' are scaled down); P to shared memory, a row a key
 // A stage's pages may be different beams' own; a mask of rows goes with each.
 //
-// With heads of 128 numbers and 32 rows a stage (64 KB) takes 1.41 us, which is memory's rate for a multiprocessor; 3.5 us go by before the
+// With heads of 128 numbers and 32 rows a stage (64 KB) takes 1.3 us, which is memory's rate for a multiprocessor; 3.5 us go by before the
 // first copy and 2 more before its scores, 15 between the first share's end and the last one's (multiprocessors are not served alike), 3.5 in
-// the join.  64 rows take 1.6 us a stage.  Measured on the first case: warp-level products (mma.sync) of the beams' rows padded to 16, 116 us,
-// and 214 for 64 rows, as each of four warps reads all keys from shared memory again; two groups of warps for 32 rows 102 for 99.5; lists of
-// single pages, where a share may begin within a stage, 98 for 96, and parted beams, whose shares are one stage, 17 for 13 us; weights of two
-// stages in turn, so that a stage need not wait for the products of the one before, level.
+// the join.  With heads of 64 the chain of a stage is longer (0.9 us) than its 32 KB take.  Measured on the first case: warp-level products (mma.sync)
+// of the beams' rows padded to 16, 116 us, and 214 for 64 rows, as each of four warps reads all keys from shared memory again; two groups of
+// warps for 32 rows 102 for 99.5; lists of single pages, where a share may begin within a stage, 98 for 96, and parted beams, whose shares are
+// one stage, 17 for 13 us; keys and values in one place, level, with 64 rows 131 for 122, and heads of 64 numbers 74 for 78; weights of two stages in
+// turn, so that a stage need not wait for the products of the one before, level; keys and values asked for by two pairs of lanes at once, level, with
+// 64 rows 130.
 // ---------------------------------------------------------------------------
 constexpr int SUB = 2, BLOCK_KEYS = SUB * PAGE;              // pages of a stage
 constexpr float NOTHING = -1e30f;                            // what weights are relative to before a row has seen a key
@@ -133,7 +136,7 @@ struct Info {                                                // of a stage
   int request, rho0, n_rows, kvh;
   int piece0, piece1;                                        // shares that the block of rows has parts in
   int keys[SUB];
-  unsigned long long rows[SUB][2];                           // that see the unit's keys
+  unsigned long long rows[SUB][2];                           // that see the page's keys
 };
 
 __device__ __forceinline__ int stages_of(const Rows& x) { return (x.pages + SUB - 1) / SUB; }
@@ -150,7 +153,7 @@ struct Tc {
   static constexpr int COLS = (2 + TILES) * N <= 64 ? 64 : (2 + TILES) * N <= 128 ? 128 : (2 + TILES) * N <= 256 ? 256 : 512;    // two S', O'
   static_assert((2 + TILES) * N <= 512, "tensor memory");
   static constexpr int GROUPS = N > 16 ? 4 : 2, HALF = N / GROUPS;      // groups of four warps, columns of each
-  static constexpr int PLACES = 1024;                                   // of the list, whose units are counted
+  static constexpr int PLACES = 1024;                                   // of the list, whose stages are counted
   static constexpr int WARPS = 4 * GROUPS, THREADS = 128 + 32 * WARPS;
   static_assert(SLOTS >= 2 && SMEM <= 232448, "shared memory of a block");
 };

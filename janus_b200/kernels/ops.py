@@ -2870,11 +2870,11 @@ def attention_beams(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 def beams_pay(rows: int, nkv: int, hd: int, max_kv_len: int) -> bool:
     """Whether a step of beam search reads shared pages once (`rope_cache_write`, then `attention_beams`) or lets every row read its own by
     the kernel for single tokens, which rotates and appends in the same launch.  That one's time goes by all rows' bytes, from L2 where rows share
-    them, at 6.5 TB/s; the other's begins at 11 to 14 us a layer, and grows by rows.  32 heads over 8 of 128, both in a graph: 4 requests of 4
-    beams behind 1,000 tokens 16 and 18 us, behind 4,000 42 and 23; 16 of 4 behind 300 19 and 15, behind 16,000 508 and 166; 16 of 16 behind
-    100 46 and 52, behind 16,000 1,739 and 197; one of 8 behind 1,000 10 and 14, behind 4,000 24 and 17.  A step's bound of the lengths is a power of two
-    of pages: rows are taken to be 0.7 of it.  Over 140 shapes the choice costs 0.7 % on average and 34 % at most (16 of 4 behind 300)."""
-    return rows * 0.7 * max_kv_len * nkv * hd * 4 / 6.5e6 > 12 + 0.08 * rows
+    them, at 6.5 TB/s; the other's begins at 11 to 14 us a layer.  32 heads over 8 of 128, both in a graph: 4 requests of 4 beams behind 1,000
+    tokens 15 and 18 us, behind 4,000 42 and 24; 16 of 4 behind 300 19 and 15, behind 16,000 508 and 170; 16 of 16 behind 100 46 and 50, behind
+    16,000 1,741 and 187; one of 8 behind 1,000 10 and 14, behind 4,000 23 and 17.  A step's bound of the lengths is a power of two of pages: rows are
+    taken to be 0.7 of it.  Over 350 shapes (heads of 64 to 256 numbers) the choice costs 1.6 % on average, 57 % at most."""
+    return rows * 0.7 * max_kv_len * nkv * hd * 4 / 6.5e6 > 14 + 0.02 * rows
 
 
 @functools.lru_cache(maxsize=4096)
