@@ -7,12 +7,13 @@
 // head, so that a shared page is read once for all beams; behind it every beam's own pages follow, one beam after another, for
 // the rows of that beam alone.  A softmax over a union of keys joins from (maximum, sum, weighted values), whoever made the parts.
 //
-// Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their stages of two pages (128 keys).
+// Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their stages of two pages (128
+// keys), of four with heads of up to 64 numbers.
 // Every block of threads has an even, consecutive share of it, and the copy engine brings its pages (128-byte swizzle), ahead across the
 // ends of requests.  Where a share ends inside a block of rows, the sums go out as a partial result; a second launch joins those.
 //
 // 32 heads over 8 of 128 numbers, 16 requests of 8 beams behind 6,000 to 24,000 tokens: 97 us for the 85 that 560 MB take; twice as
-// long 172 for 161, of 16 beams 122 for 94, with heads of 64 numbers 78 for 43; 16 heads over 4 of 256 104 for 86, of 16 beams 142
+// long 172 for 161, of 16 beams 122 for 94, with heads of 64 numbers 63 for 43; 16 heads over 4 of 256 104 for 86, of 16 beams 142
 // for 94; one request of 4 beams behind 300 9.1.
 #include <math_constants.h>
 #include <stdio.h>
@@ -121,41 +122,42 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t two) { return ((two & 0x
 //
 // With heads of 128 numbers and 32 rows a stage (64 KB) takes 1.3 us, which is memory's rate for a multiprocessor; 3.5 us go by before the
 // first copy and 2 more before its scores, 15 between the first share's end and the last one's (multiprocessors are not served alike), 3.5 in
-// the join.  With heads of 64 the chain of a stage is longer (0.9 us) than its 32 KB take.  Measured on the first case: warp-level products (mma.sync)
+// the join.  With heads of 64 numbers the chain of a stage is longer than 32 KB take: a thread has two keys there (78 us by one).  Measured on the first case: warp-level products (mma.sync)
 // of the beams' rows padded to 16, 116 us, and 214 for 64 rows, as each of four warps reads all keys from shared memory again; two groups of
 // warps for 32 rows 102 for 99.5; lists of single pages, where a share may begin within a stage, 98 for 96, and parted beams, whose shares are
-// one stage, 17 for 13 us; keys and values in one place, level, with 64 rows 131 for 122, and heads of 64 numbers 74 for 78; weights of two stages in
+// one stage, 17 for 13 us; keys and values in one place, level, with 64 rows 131 for 122; weights of two stages in
 // turn, so that a stage need not wait for the products of the one before, level; keys and values asked for by two pairs of lanes at once, level, with
 // 64 rows 130.
 // ---------------------------------------------------------------------------
-constexpr int SUB = 2, BLOCK_KEYS = SUB * PAGE;              // pages of a stage
 constexpr float NOTHING = -1e30f;                            // what weights are relative to before a row has seen a key
 
 struct Info {                                                // of a stage
   int first, last, final_, whole;                            // of its block of rows' keys in this share; of the share; no mask
   int request, rho0, n_rows, kvh;
   int piece0, piece1;                                        // shares that the block of rows has parts in
-  int keys[SUB];
-  unsigned long long rows[SUB][2];                           // that see the page's keys
+  int keys[4];                                               // of its pages, two or four
+  unsigned long long rows[4][2];                             // that see the page's keys
 };
-
-__device__ __forceinline__ int stages_of(const Rows& x) { return (x.pages + SUB - 1) / SUB; }
 
 template <int HDC, int N>
 struct Tc {
-  static constexpr int SLABS = HDC / 64, SLAB = BLOCK_KEYS * 128, SLOT = SLABS * SLAB;   // 64 numbers of a stage's keys; its keys, or its values
+  static constexpr int HALVES = HDC == 64 && N <= 64 ? 2 : 1;            // of 128 keys, that a thread has one each of
+  static constexpr int KEYS = 128 * HALVES, SUB = KEYS / PAGE;           // keys and pages of a stage
+  static constexpr int SLABS = HDC / 64, SLAB = KEYS * 128, SLOT = SLABS * SLAB;   // 64 numbers of a stage's keys; its keys, or its values
   static constexpr int TILES = HDC > 128 ? 2 : 1;            // of 128 of the head's numbers in O'
-  static constexpr int Q = SLABS * N * 128, P = (N > 64 ? 2 : 1) * BLOCK_KEYS * 128;
-  static constexpr int MISC = 4 * N + 16 * N + 1200;         // ref, exchange, barriers and descriptions
+  static constexpr int Q = SLABS * N * 128, P = (N > 64 ? 2 : 1) * KEYS * 128;
+  static constexpr int MISC = 4 * N + 16 * N + 1300;         // ref, exchange, barriers and descriptions
   static constexpr int FIT = (232448 - Q - P - MISC) / SLOT, SLOTS = FIT > 12 ? 12 : FIT, INFOS = SLOTS / 2 + 1;
   static constexpr int AT_Q = SLOTS * SLOT, AT_P = AT_Q + Q, AT_REF = AT_P + P, AT_SWAP = AT_REF + 4 * N, AT_INFO = AT_SWAP + 16 * N,
                        AT_BARS = AT_INFO + INFOS * (int)sizeof(Info), BARS = 2 * SLOTS + INFOS + 6, AT_BAD = AT_BARS + BARS * 8 + 16, SMEM = AT_BAD + 128;
-  static constexpr int COLS = (2 + TILES) * N <= 64 ? 64 : (2 + TILES) * N <= 128 ? 128 : (2 + TILES) * N <= 256 ? 256 : 512;    // two S', O'
-  static_assert((2 + TILES) * N <= 512, "tensor memory");
+  static constexpr int AT_O = 2 * HALVES * N, COLS_USED = AT_O + TILES * N;     // of tensor memory: two S', O'
+  static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
+  static_assert(COLS_USED <= 512, "tensor memory");
   static constexpr int GROUPS = N > 16 ? 4 : 2, HALF = N / GROUPS;      // groups of four warps, columns of each
   static constexpr int PLACES = 1024;                                   // of the list, whose stages are counted
   static constexpr int WARPS = 4 * GROUPS, THREADS = 128 + 32 * WARPS;
   static_assert(SLOTS >= 2 && SMEM <= 232448, "shared memory of a block");
+  static __device__ __forceinline__ int stages_of(const Rows& x) { return (x.pages + SUB - 1) / SUB; }
 };
 
 // Where a ring's next stage stands: keys take a place, values the next one.
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         const int block = (p0 + u * (C::THREADS / 32)) * chunk + i;
-        if (block < blocks) stages[u] += stages_of(rows_of(a, block, len[u], shared[u]));
+        if (block < blocks) stages[u] += C::stages_of(rows_of(a, block, len[u], shared[u]));
       }
     }
 #pragma unroll
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
       while (begin >= before + sums[t]) before += sums[t++];
       for (block = t * chunk;; ++block) {
         x = look_up(a, block);
-        stages = stages_of(x);
+        stages = C::stages_of(x);
         if (begin < before + stages * a.nkv) break;
         before += stages * a.nkv;
       }
@@ -378,10 +380,10 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
     // The lanes look up 32 pages at a time; of a stage's, lanes 0 and 1 have one each.
     int ahead = 0, keys = 0, beam = -1, page = -1;                     // the first one's place; the lane's: keys, beam (-1: all that share it), page
     auto find = [&]() {
-      ahead = turn * SUB;
+      ahead = turn * C::SUB;
       beam = -1, keys = 0, page = -1;
       const int mine = ahead + lane, j = mine - x.common;
-      const bool there = mine < x.pages && at + lane / SUB < end;
+      const bool there = mine < x.pages && at + lane / C::SUB < end;
       const int* entry = nullptr;
       if (there && j < 0) {
         keys = PAGE;
@@ -406,8 +408,8 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
       begun();
     }
     while (at < end) {
-      if (turn * SUB >= ahead + 32) find();
-      const int n = min(SUB, x.pages - turn * SUB), from = turn * SUB - ahead + (lane & 1);
+      if (turn * C::SUB >= ahead + 32) find();
+      const int n = min(C::SUB, x.pages - turn * C::SUB), from = turn * C::SUB - ahead + (lane & (C::SUB - 1));
       const int keys0 = __shfl_sync(0xffffffffu, keys, from), beam0 = __shfl_sync(0xffffffffu, beam, from), page0 = __shfl_sync(0xffffffffu, page, from);
       unsigned long long rows[2] = {joining[0], joining[1]};
       if (beam0 >= 0) {
@@ -416,11 +418,11 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
       }
       const bool there = lane < n && keys0 > 0 && page0 >= 0 && page0 < a.n_pages;    // (no page: no keys)
       const unsigned loads = __ballot_sync(0xffffffffu, there);
-      const bool whole = __all_sync(0xffffffffu, lane >= SUB || (there && keys0 == PAGE && rows[0] == all[0] && rows[1] == all[1]));
+      const bool whole = __all_sync(0xffffffffu, lane >= C::SUB || (there && keys0 == PAGE && rows[0] == all[0] && rows[1] == all[1]));
       ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot.at, slot.phase ^ 1, status, 54));
       if (!ok) break;
       Info& to = info[note.at];
-      if (lane < SUB) to.keys[lane] = there ? keys0 : 0, to.rows[lane][0] = rows[0], to.rows[lane][1] = rows[1];
+      if (lane < C::SUB) to.keys[lane] = there ? keys0 : 0, to.rows[lane][0] = rows[0], to.rows[lane][1] = rows[1];
       if (lane == 0) {
         to.first = at == begin || turn == 0, to.last = turn + 1 == stages || at + 1 == end, to.final_ = at + 1 == end, to.whole = whole;
         to.request = x.request, to.rho0 = x.rho0, to.n_rows = x.n_rows, to.kvh = kvh;
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
       if (at < end && turn == stages) {
         turn = 0;
         const bool enters = ++kvh == a.nkv;
-        if (enters) kvh = 0, x = look_up(a, ++block), stages = stages_of(x);
+        if (enters) kvh = 0, x = look_up(a, ++block), stages = C::stages_of(x);
         find();
         if (enters) entered();
         begun();
@@ -465,8 +467,8 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
   } else if (warp == 1) {
     if (elected()) {
       const uint32_t idesc_s = jb::instr_desc_bf16(N), idesc_o = jb::instr_desc_bf16(N) | (1u << 15) | (1u << 16);   // values and weights: MN-major
-      const uint32_t o_col = tmem + 2 * N;
-      const uint64_t p = desc_mn_sw128(p_at, BLOCK_KEYS * 128, 1024);
+      const uint32_t o_col = tmem + C::AT_O;
+      const uint64_t p = desc_mn_sw128(p_at, C::KEYS * 128, 1024);
       Ring<C::SLOTS> ks(0), vs(1);
       Ring<C::INFOS> note(0);
       int it = 0, turn = 0;
@@ -475,11 +477,13 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
         const uint32_t k_s = base + ks.at * C::SLOT;
         jb::tc_fence_after();
 #pragma unroll
-        for (int h = 0; h < C::SLABS; ++h) {
-          const uint64_t k = jb::smem_desc_sw128(k_s + h * C::SLAB), q = jb::smem_desc_sw128(q_at + h * N * 128);
+        for (int t = 0; t < C::HALVES; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) jb::umma_bf16(tmem + buffer * N, k + 2 * i, q + 2 * i, idesc_s, (h | i) ? 1u : 0u);
-        }
+          for (int h = 0; h < C::SLABS; ++h) {
+            const uint64_t k = jb::smem_desc_sw128(k_s + h * C::SLAB + t * 128 * 128), q = jb::smem_desc_sw128(q_at + h * N * 128);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) jb::umma_bf16(tmem + (buffer * C::HALVES + t) * N, k + 2 * i, q + 2 * i, idesc_s, (h | i) ? 1u : 0u);
+          }
         jb::umma_commit(s_full + 8 * buffer);
         jb::umma_commit(empty + 8 * ks.at);
         ks.step(2);
@@ -506,7 +510,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
 #pragma unroll
         for (int m = 0; m < C::TILES; ++m)
 #pragma unroll
-          for (int i = 0; i < BLOCK_KEYS / 16; ++i)
+          for (int i = 0; i < C::KEYS / 16; ++i)
             jb::umma_bf16(o_col + m * N, v + (m * 2 * C::SLAB + i * 2048) / 16, p + i * 2048 / 16, idesc_o, first && i == 0 ? 0u : 1u);
         jb::umma_commit(pv_done);
         jb::umma_commit(empty + 8 * vs.at);
@@ -550,27 +554,31 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
       }
       if (group_any(1 + group, !ok)) break;
       const bool last = x->last;
-      const int final_ = x->final_, sub = quarter >> 1, in_page = (quarter & 1) * 32 + lane, keys = x->keys[sub];
+      const int final_ = x->final_, in_page = (quarter & 1) * 32 + lane;
       const bool masked = !x->whole;
-      unsigned long long rows = 0ull;
+      unsigned long long rows[C::HALVES] = {};
       if (masked) {
-        rows = x->rows[sub][c0 / 64] >> (c0 % 64);
-        if (in_page >= keys) rows = 0ull;
         // values behind the last key, or that are no finite numbers: a weight of 0 does not silence them (a part of the head's numbers a
         // group; while the scores are made)
         ok = ok && mbar_wait(full + 8 * vs.at, vs.phase, status, 53);
-        uint8_t* values = smem + vs.at * C::SLOT + key * 128;
-        uint32_t odd = 0u;
 #pragma unroll
-        for (int p = 0; p < C::SLABS * 8 / C::GROUPS; ++p) {
-          const int at = p * C::GROUPS + group;
-          const uint4 v = *reinterpret_cast<const uint4*>(values + (at / 8) * C::SLAB + (((at ^ key) & 7) << 4));
-          odd |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
-        }
-        if (odd != 0u || in_page >= keys) {
-          for (int at = group; at < C::SLABS * 8; at += C::GROUPS)
-            *reinterpret_cast<uint4*>(values + (at / 8) * C::SLAB + (((at ^ key) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
-          if (in_page < keys) atomicOr(&bad[turn & 1][group][0], x->rows[sub][0]), atomicOr(&bad[turn & 1][group][1], x->rows[sub][1]);
+        for (int t = 0; t < C::HALVES; ++t) {
+          const int sub = t * 2 + (quarter >> 1);
+          const bool behind = in_page >= x->keys[sub];
+          rows[t] = behind ? 0ull : x->rows[sub][c0 / 64] >> (c0 % 64);
+          uint8_t* values = smem + vs.at * C::SLOT + (t * 128 + key) * 128;
+          uint32_t odd = 0u;
+#pragma unroll
+          for (int p = 0; p < C::SLABS * 8 / C::GROUPS; ++p) {
+            const int at = p * C::GROUPS + group;
+            const uint4 v = *reinterpret_cast<const uint4*>(values + (at / 8) * C::SLAB + (((at ^ key) & 7) << 4));
+            odd |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
+          }
+          if (odd != 0u || behind) {
+            for (int at = group; at < C::SLABS * 8; at += C::GROUPS)
+              *reinterpret_cast<uint4*>(values + (at / 8) * C::SLAB + (((at ^ key) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+            if (!behind) atomicOr(&bad[turn & 1][group][0], x->rows[sub][0]), atomicOr(&bad[turn & 1][group][1], x->rows[sub][1]);
+          }
         }
       }
       ok = ok && mbar_wait(s_full + 8 * (it & 1), (it >> 1) & 1, status, 57);
@@ -580,20 +588,24 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
         if (!rest) ok = ok && mbar_wait(pv_done, (it - 1) & 1, status, 58), jb::tc_fence_after();
         rest = true;
       };
-      float s[C::HALF];
+      float s[C::HALVES][C::HALF];
       auto scores = [&]() {
 #pragma unroll
-        for (int c = 0; c < C::HALF; c += 8) {
-          float v[8];
-          jb::tmem_ld8(lanes + (it & 1) * N + c0 + c, v);
+        for (int t = 0; t < C::HALVES; ++t)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[c + e] = v[e];
-        }
+          for (int c = 0; c < C::HALF; c += 8) {
+            float v[8];
+            jb::tmem_ld8(lanes + ((it & 1) * C::HALVES + t) * N + c0 + c, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[t][c + e] = v[e];
+          }
         jb::tmem_ld_wait();
         if (masked) {
 #pragma unroll
-          for (int c = 0; c < C::HALF; ++c)
-            if (!((rows >> c) & 1ull)) s[c] = -CUDART_INF_F;
+          for (int t = 0; t < C::HALVES; ++t)
+#pragma unroll
+            for (int c = 0; c < C::HALF; ++c)
+              if (!((rows[t] >> c) & 1ull)) s[t][c] = -CUDART_INF_F;
         }
       };
       scores();
@@ -602,9 +614,13 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
 #pragma unroll
       for (int c = 0; c < C::HALF; c += 4) {
         const float4 r = *reinterpret_cast<const float4*>(my_ref + c);
-        s[c] = fmaf(s[c], a.scale_log2, -r.x), s[c + 1] = fmaf(s[c + 1], a.scale_log2, -r.y);
-        s[c + 2] = fmaf(s[c + 2], a.scale_log2, -r.z), s[c + 3] = fmaf(s[c + 3], a.scale_log2, -r.w);
-        high = fmaxf(high, fmaxf(fmaxf(s[c], s[c + 1]), fmaxf(s[c + 2], s[c + 3])));
+#pragma unroll
+        for (int t = 0; t < C::HALVES; ++t) {
+          float* y = s[t] + c;
+          y[0] = fmaf(y[0], a.scale_log2, -r.x), y[1] = fmaf(y[1], a.scale_log2, -r.y);
+          y[2] = fmaf(y[2], a.scale_log2, -r.z), y[3] = fmaf(y[3], a.scale_log2, -r.w);
+          high = fmaxf(high, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+        }
       }
       if (group_any(1 + group, high > RESCALE_LOG2)) {
         // the rows' largest over the block's keys
@@ -612,7 +628,10 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
         scores();
 #pragma unroll
         for (int c = 0; c < C::HALF; ++c) {
-          const float top = warp_top(s[c]);
+          float most = s[0][c];
+#pragma unroll
+          for (int t = 1; t < C::HALVES; ++t) most = fmaxf(most, s[t][c]);
+          const float top = warp_top(most);
           if (lane == 0) swap[quarter * N + c0 + c] = top;
         }
         group_any(1 + group, false);
@@ -630,36 +649,43 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
           float f[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            s[c + e] = fmaf(s[c + e], a.scale_log2, -my_ref[c + e]);
+#pragma unroll
+            for (int t = 0; t < C::HALVES; ++t) s[t][c + e] = fmaf(s[t][c + e], a.scale_log2, -my_ref[c + e]);
             f[e] = swap[c0 + c + e], l[c + e] *= f[e];
           }
           if (!first) {
 #pragma unroll
             for (int m = 0; m < C::TILES; ++m) {
               float v[8];
-              jb::tmem_ld8(lanes + (2 + m) * N + c0 + c, v);
+              jb::tmem_ld8(lanes + C::AT_O + m * N + c0 + c, v);
               jb::tmem_ld_wait();
 #pragma unroll
               for (int e = 0; e < 8; ++e) v[e] *= f[e];
-              tmem_st8(lanes + (2 + m) * N + c0 + c, v);
+              tmem_st8(lanes + C::AT_O + m * N + c0 + c, v);
             }
           }
         }
         tmem_st_wait();
       }
-      uint32_t w[C::HALF / 2];
+      uint32_t w[C::HALVES][C::HALF / 2];
 #pragma unroll
-      for (int c = 0; c < C::HALF; c += 2) {
-        const float p0 = fast_exp2(s[c]), p1 = fast_exp2(s[c + 1]);
-        w[c / 2] = pack_bf16(p0, p1);                                  // (summed as they are rounded: a weight that outdoes all others costs nothing)
-        l[c] += low_of(w[c / 2]), l[c + 1] += high_of(w[c / 2]);
-      }
+      for (int t = 0; t < C::HALVES; ++t)
+#pragma unroll
+        for (int c = 0; c < C::HALF; c += 2) {
+          const uint32_t two = pack_bf16(fast_exp2(s[t][c]), fast_exp2(s[t][c + 1]));
+          l[c] += low_of(two), l[c + 1] += high_of(two);               // (as they are rounded: a weight that outdoes all others costs nothing)
+          w[t][c / 2] = two;
+        }
       settle();
-      uint8_t* p_row = smem + C::AT_P + (c0 / 64) * BLOCK_KEYS * 128 + key * 128;
 #pragma unroll
-      for (int c = 0; c < C::HALF; c += 8) {
-        const int piece = (c0 % 64 + c) / 8;
-        *reinterpret_cast<uint4*>(p_row + ((piece ^ (key & 7)) << 4)) = make_uint4(w[c / 2], w[c / 2 + 1], w[c / 2 + 2], w[c / 2 + 3]);
+      for (int t = 0; t < C::HALVES; ++t) {
+        uint8_t* p_row = smem + C::AT_P + (c0 / 64) * C::KEYS * 128 + (t * 128 + key) * 128;
+#pragma unroll
+        for (int c = 0; c < C::HALF; c += 8) {
+          const int piece = (c0 % 64 + c) / 8;
+          *reinterpret_cast<uint4*>(p_row + ((piece ^ (key & 7)) << 4)) =
+              make_uint4(w[t][c / 2], w[t][c / 2 + 1], w[t][c / 2 + 2], w[t][c / 2 + 3]);
+        }
       }
       const int piece0 = x->piece0, piece1 = x->piece1;                // (read before the stage is given back)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -700,7 +726,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
 #pragma unroll
           for (int m = 0; m < C::TILES; ++m) {
             float v[8];
-            jb::tmem_ld8(lanes + (2 + m) * N + c0 + c, v);
+            jb::tmem_ld8(lanes + C::AT_O + m * N + c0 + c, v);
             jb::tmem_ld_wait();
             if (key + 128 * m < hd) {
 #pragma unroll

@@ -2882,5 +2882,6 @@ def beam_attention_plan(groups: int, beams: int, nh: int, nkv: int, hd: int, max
     """How `attention_beams` runs: (blocks, rows of a block's tile).  Tiles of 128 rows have no room for queries of more than 128 numbers."""
     rows = beams * (nh // nkv)
     tile = next((n for n in (16, 32, 64) if rows <= n), 128 if hd <= 128 else 64)
-    stages = groups * -(-rows // tile) * nkv * -(-max_kv_len // 128) * (beams + 1)      # (at most: nothing may be shared)
+    keys = 256 if hd <= 64 and tile <= 64 else 128                                       # of a stage
+    stages = groups * -(-rows // tile) * nkv * -(-max_kv_len // keys) * (beams + 1)      # (at most: nothing may be shared)
     return max(1, min(SM_COUNT_TARGET // 2, stages)), tile
