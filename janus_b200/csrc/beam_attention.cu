@@ -7,10 +7,10 @@
 // head, so that a shared page is read once for all beams; behind it every beam's own pages follow, one beam after another, for
 // the rows of that beam alone.  A softmax over a union of keys joins from (maximum, sum, weighted values), whoever made the parts.
 //
-// Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their stages of two pages (128
-// keys), of four with heads of up to 64 numbers.
-// Every block of threads has an even, consecutive share of it, and the copy engine brings its pages (128-byte swizzle), ahead across the
-// ends of requests.  Where a share ends inside a block of rows, the sums go out as a partial result; a second launch joins those.
+// Bound by the bytes of the keys.  The work is a flat list: a request's block of rows, its key heads, their stages of two pages (128 keys),
+// of four with heads of up to 64 numbers. Every block of threads has an even, consecutive share of it, and the copy engine brings its pages
+// (128-byte swizzle), ahead across the ends of requests.  Where a share ends inside a block of rows, the sums go out as a partial result; a
+// second launch joins those.
 //
 // 32 heads over 8 of 128 numbers, 16 requests of 8 beams behind 6,000 to 24,000 tokens: 97 us for the 85 that 560 MB take; twice as
 // long 172 for 161, of 16 beams 122 for 94, with heads of 64 numbers 63 for 43; 16 heads over 4 of 256 104 for 86, of 16 beams 142
@@ -120,14 +120,14 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t two) { return ((two & 0x
 //                only when a score passes it by RESCALE_LOG2 (then the sums and O' are scaled down); P to shared memory, a row a key
 // A stage's pages may be different beams' own; a mask of rows goes with each.
 //
-// With heads of 128 numbers and 32 rows a stage (64 KB) takes 1.3 us, which is memory's rate for a multiprocessor; 3.5 us go by before the
-// first copy and 2 more before its scores, 15 between the first share's end and the last one's (multiprocessors are not served alike), 3.5 in
-// the join.  With heads of 64 numbers the chain of a stage is longer than 32 KB take: a thread has two keys there (78 us by one).  Measured on the first case: warp-level products (mma.sync)
-// of the beams' rows padded to 16, 116 us, and 214 for 64 rows, as each of four warps reads all keys from shared memory again; two groups of
-// warps for 32 rows 102 for 99.5; lists of single pages, where a share may begin within a stage, 98 for 96, and parted beams, whose shares are
-// one stage, 17 for 13 us; keys and values in one place, level, with 64 rows 131 for 122; weights of two stages in
-// turn, so that a stage need not wait for the products of the one before, level; keys and values asked for by two pairs of lanes at once, level, with
-// 64 rows 130.
+// With heads of 128 numbers and 32 rows a stage (64 KB) takes 1.3 us, which is memory's rate for a multiprocessor; 3.5 us go by before the first
+// copy and 2 more before its scores, 15 between the first share's end and the last one's (multiprocessors are not served alike), 3.5 in the join.
+// With heads of 64 numbers the chain of a stage is longer than 32 KB take: a thread has two keys there (78 us by one).  Measured on the first
+// case: warp-level products (mma.sync) of the beams' rows padded to 16, 116 us, and 214 for 64 rows, as each of four warps reads all keys from
+// shared memory again; two groups of warps for 32 rows 102 for 99.5; lists of single pages, where a share may begin within a stage, 98 for 96,
+// and parted beams, whose shares are one stage, 17 for 13 us; keys and values in one place, level, with 64 rows 131 for 122; weights of two
+// stages in turn, so that a stage need not wait for the products of the one before, level; keys and values asked for by two pairs of lanes at
+// once, level, with 64 rows 130.
 // ---------------------------------------------------------------------------
 constexpr float NOTHING = -1e30f;                            // what weights are relative to before a row has seen a key
 
