@@ -230,41 +230,33 @@ __device__ __forceinline__ void add_rows(unsigned long long (&bits)[2], int from
   }
 }
 
-// out[c] = the sum of v[c] over the warp's lanes, for C columns (a power of two from 8 to 64).
+// out[c] = the sum of v[c] over the warp's lanes, for C columns (8, 16 or 32).
 template <int C>
 __device__ __forceinline__ void columns_summed(const float (&v)[C], float* out) {
   const int lane = threadIdx.x & 31;
-  if constexpr (C == 64) {
-    float lo[32], hi[32];
+  float t[C];
 #pragma unroll
-    for (int c = 0; c < 32; ++c) lo[c] = v[c], hi[c] = v[32 + c];
-    columns_summed<32>(lo, out);
-    columns_summed<32>(hi, out + 32);
-  } else {
-    float t[C];
+  for (int c = 0; c < C; ++c) t[c] = v[c];
+  int o = 16, left = C;
 #pragma unroll
-    for (int c = 0; c < C; ++c) t[c] = v[c];
-    int o = 16, left = C;
+  for (int step = 0; step < 5; ++step, o >>= 1) {
+    if (left > 1) {
+      left >>= 1;
+      const bool up = (lane & o) != 0;
 #pragma unroll
-    for (int step = 0; step < 5; ++step, o >>= 1) {
-      if (left > 1) {
-        left >>= 1;
-        const bool up = (lane & o) != 0;
-#pragma unroll
-        for (int c = 0; c < C / 2; ++c) {
-          if (c < left) {
-            const float mine = up ? t[left + c] : t[c], other = up ? t[c] : t[left + c];
-            t[c] = mine + __shfl_xor_sync(0xffffffffu, other, o);
-          }
+      for (int c = 0; c < C / 2; ++c) {
+        if (c < left) {
+          const float mine = up ? t[left + c] : t[c], other = up ? t[c] : t[left + c];
+          t[c] = mine + __shfl_xor_sync(0xffffffffu, other, o);
         }
-      } else {
-        t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
       }
+    } else {
+      t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
     }
-    // lane bits from the top name the column, as far as they were needed
-    constexpr int BITS = C == 8 ? 3 : C == 16 ? 4 : 5;
-    if ((lane & ((1 << (5 - BITS)) - 1)) == 0) out[lane >> (5 - BITS)] = t[0];
   }
+  // lane bits from the top name the column, as far as they were needed
+  constexpr int BITS = C == 8 ? 3 : C == 16 ? 4 : 5;
+  if ((lane & ((1 << (5 - BITS)) - 1)) == 0) out[lane >> (5 - BITS)] = t[0];
 }
 
 template <int HDC, int N>

@@ -5,9 +5,10 @@ float32 terms exp(d), d = x - max: d and its product with log2(e) are each withi
 within 2^-22; weighted by the terms themselves |d| is at most the logarithm of the vocabulary plus 1, below 13 here: 26 / 2^24 + 2^-21 < 2.1e-6.
 Whole numbers are equal; where rankings are compared, the smallest distance of two neighbours of different beams is above twice that.
 
-Attention: the result's own rounding, 2^-8 of it; the weights' rounding to bfloat16, 2^-8 of the weighted sum of the values'
-magnitudes S; scores are float32 sums over a head's numbers, whose errors (d 2^-24 of their terms, below 2^-12 for scores below 30) and the
-rounding of the power change weights by less than 2^-11 of S.
+Attention is sum(p v) / sum(p) with weights p (1 + d), |d| <= 2^-8 (their rounding to bfloat16), above and below: off by sum(p d (v - result)) /
+sum(p), at most 2^-8 of the weighted mean of |v - result|, which is at most S + |result|, S the weighted mean of the values' magnitudes.  The
+result's own rounding is 2^-8 of it: 2^-7 |result| + 2^-8 S together.  Scores are float32 sums over a head's numbers, whose errors (d 2^-24 of their
+terms, below 2^-12 for scores below 30) and the rounding of the power change weights by less than 2^-11 of S.
 """
 import math
 import random
@@ -365,6 +366,10 @@ def attention_case(R, K, kv_len, shared, nkv, group, hd, seed, extra=1):
     return q, k, v, table, nh
 
 
+def attention_bound(want, size):
+    return 2.0 ** -7 * want.abs() + (2.0 ** -8 + 2.0 ** -11) * size + 1e-30
+
+
 def check_attention(R, K, kv_len, shared, nkv, group, hd, seed=1, extra=1, bound=None):
     q, k, v, table, nh = attention_case(R, K, kv_len, shared, nkv, group, hd, seed, extra)
     out = empty(R * K, nh * hd, dtype=torch.bfloat16)
@@ -373,7 +378,7 @@ def check_attention(R, K, kv_len, shared, nkv, group, hd, seed=1, extra=1, bound
                         Workspace(torch.device("cuda")), bound or max(kv_len))
     want, size = P.attention(q, k, v, table, kv_len, nh, nkv, hd, scale)
     off = (out.cpu().double().view(R * K, nh, hd) - want).abs()
-    worst = (off / (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -11) * size + 1e-30)).max()
+    worst = (off / attention_bound(want, size)).max()
     assert worst <= 1.0, float(worst)
 
 
@@ -437,7 +442,7 @@ def test_attention_pages_beyond_32_bits():
         ops.attention_beams(q.cuda(), *big, out, ints(moved), ints([300, 290]), ints([2]), 2, nh, nkv, hd, PAGE, 0.3, Workspace(torch.device("cuda")), 300)
         want, size = P.attention(q, k, v, table, [300, 290], nh, nkv, hd, 0.3)
         off = (out.cpu().double().view(2, nh, hd) - want).abs()
-        assert float((off / (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -11) * size + 1e-30)).max()) <= 1.0
+        assert float((off / attention_bound(want, size)).max()) <= 1.0
         del big
     with pytest.raises(ops.KernelError, match="attention_beams"):
         args = _attention_args(K=1, nh=1, nkv=1, hd=8, device="cuda")
@@ -481,7 +486,7 @@ def test_attention_numbers_that_are_not_finite_stay_with_their_readers(hd, K, gr
     want, size = want.view(2 * K, 2, group, hd), size.view(2 * K, 2, group, -1)
     clean = torch.ones(2 * K, 2, dtype=torch.bool)
     clean[1:K, 1] = clean[2, 0] = clean[K - 1, 0] = False
-    off = (got - want).abs() / (2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -11) * size + 1e-30)
+    off = (got - want).abs() / attention_bound(want, size)
     assert float(off[clean].max()) <= 1.0
     bad = ~torch.isfinite(want)
     assert bad[1, 1, :, hd - 3].all() and bad[K - 1, 0, :, 0].all() and not torch.isfinite(got[bad]).any()
