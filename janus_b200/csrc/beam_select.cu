@@ -5,13 +5,13 @@
 // The K best that are no stop token go on; a stop token among the K best of all ends its beam's text.  A beam's best continuation
 // stays in the beam's row, so that cache rows and states move only where a beam is lost; the others take the rows left, in order.
 //
-// Three launches.  The first reads every logit once and does nothing but keep, in registers, each thread's largest one and its sum of
-// exponentials.  In the second a block a beam finds the beam's K best: the K-th largest of the threads' maxima bounds the K-th largest
-// logit of the row from below, and only the few threads' numbers at or above it are looked at again (from L2).  The third, a block a
-// request, joins its beams.  64 requests of 8 beams over 128,256 tokens: 59 us, the first 45.  (With the second step done by each block
-// of the first launch 63 us: memory stood still meanwhile; with a warp a beam in the third 76.  With fewer launches, the last block of a
-// row or of a request going on by a ticket: 61 by two, 65 by one, whose blocks that only read are fewer at a time; one request 12.8
-// and 13.6 us, by three 11.8.)
+// Three launches.  The first reads every logit once and does nothing but keep, in registers, each thread's largest one and its sum
+// of exponentials.  In the second a block a beam finds the beam's K best: the K-th largest of the threads' maxima bounds the K-th
+// largest logit of the row from below, and only the few threads' numbers at or above it are looked at again (from L2).  The third,
+// a block a request, joins its beams.  64 requests of 8 beams over 128,256 tokens: 58 us, the first 44.  (With vectors of 16 bytes,
+// of which the second fetches twice the memory, 60.  With the second step done by each block of the first launch 63 us: memory
+// stood still meanwhile; with a warp a beam in the third 76.  With fewer launches, the last block of a row or of a request going on
+// by a ticket: 61 by two, 65 by one, whose blocks that only read are fewer at a time; one request 12.8 and 13.6 us, by three 11.8.)
 // Within a beam the order is that of the logits (equal ones: the lowest token first), which no rounding touches; between beams it is
 // that of the totals, whose sum of exponentials is taken to 64 bits where threads meet: 32 bits would turn two beams round now and
 // then.
@@ -28,9 +28,11 @@ typedef unsigned long long Key;      // a logit that sorts as a whole number, ab
 
 constexpr int THREADS = 256;
 constexpr int WARPS = THREADS / 32;
-constexpr int VECTORS = 4;                                // of 16 bytes that a thread has on its way at a time
+constexpr int WIDE_LOAD = 8;                              // numbers of a vector, 32 bytes
+constexpr int VECTORS = 2;                                // that a thread has on its way at a time
 constexpr int MOST_BEAMS = 32, MOST_STOPS = 32, MOST_RANGES = 8;
-constexpr int ROOM = THREADS * 4 + MOST_BEAMS;            // candidates of a beam at a time
+constexpr int AGAIN = 2;                                  // halves of vectors that a thread looks at again at a time
+constexpr int ROOM = THREADS * 4 * AGAIN + MOST_BEAMS;            // candidates of a beam at a time
 constexpr float FAR = 40.0f;                              // how far a power may lie above what a thread's sum is relative to
 constexpr float WIDE = 1e8f;                              // powers beyond are made by 64-bit arithmetic
 
@@ -100,25 +102,42 @@ __device__ __forceinline__ double warp_max(double v) {
   return v;
 }
 
-// A row of logits in vectors of 16 bytes; vector i holds numbers 4 i - lead .., of which the first and the last may lie outside the row.
+struct Eight {
+  float x[WIDE_LOAD];
+};
+__device__ __forceinline__ Eight load_eight(const float* at) {
+  Eight v;
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v.x[0]), "=f"(v.x[1]), "=f"(v.x[2]), "=f"(v.x[3]), "=f"(v.x[4]), "=f"(v.x[5]), "=f"(v.x[6]), "=f"(v.x[7])
+               : "l"(at));
+  return v;
+}
+
+// A row of logits in vectors of 32 bytes; vector i holds numbers 8 i - lead .., of which the first and the last may lie outside the row.
 // Range r of the row has vectors begin(r) .. begin(r + 1), its thread t those at begin(r) + t, + THREADS, ...
 struct Row {
   const float* x;
   int lead, vectors, V, ranges;
   __device__ __forceinline__ Row(const Args& a, int row) : x(a.logits + (size_t)row * a.V), V(a.V), ranges(a.ranges) {
-    lead = (int)(((uintptr_t)x >> 2) & 3);
-    vectors = (V + lead + 3) / 4;
+    lead = (int)(((uintptr_t)x >> 2) & (WIDE_LOAD - 1));
+    vectors = (V + lead + WIDE_LOAD - 1) / WIDE_LOAD;
   }
   __device__ __forceinline__ int begin(int range) const { return (int)((long long)range * vectors / ranges); }
-  __device__ __forceinline__ float4 load(int i) const {
+  __device__ __forceinline__ Eight load(int i) const {
+    const int at = WIDE_LOAD * i - lead;
+    if (at >= 0 && at + WIDE_LOAD <= V) return load_eight(x + at);
+    Eight v;
+#pragma unroll
+    for (int e = 0; e < WIDE_LOAD; ++e) v.x[e] = at + e >= 0 && at + e < V ? x[at + e] : -CUDART_INF_F;
+    return v;
+  }
+  __device__ __forceinline__ float4 load_half(int i) const {      // half i of the vectors
     const int at = 4 * i - lead;
     if (at >= 0 && at + 4 <= V) return *reinterpret_cast<const float4*>(x + at);
-    float4 v = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
-    if (at >= 0 && at < V) v.x = x[at];
-    if (at + 1 >= 0 && at + 1 < V) v.y = x[at + 1];
-    if (at + 2 >= 0 && at + 2 < V) v.z = x[at + 2];
-    if (at + 3 >= 0 && at + 3 < V) v.w = x[at + 3];
-    return v;
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = at + e >= 0 && at + e < V ? x[at + e] : -CUDART_INF_F;
+    return make_float4(y[0], y[1], y[2], y[3]);
   }
 };
 
@@ -138,11 +157,12 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
   float top = -CUDART_INF_F, scale = -CUDART_INF_F;
   bool wide = false;
   double sum = 0.0;
-  const float4 none = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
-  auto take = [&](const float4 (&v)[VECTORS]) {
+  auto take = [&](const Eight (&v)[VECTORS]) {
     float high = -CUDART_INF_F;                           // (what is no number is never the larger)
 #pragma unroll
-    for (int u = 0; u < VECTORS; ++u) high = max3(max3(high, v[u].x, v[u].y), v[u].z, v[u].w);
+    for (int u = 0; u < VECTORS; ++u)
+#pragma unroll
+      for (int e = 0; e < WIDE_LOAD; e += 2) high = max3(high, v[u].x[e], v[u].x[e + 1]);
     top = fmaxf(top, high);
     const float power = high * (float)LOG2E;
     if (!(power >= -WIDE)) return;
@@ -156,21 +176,28 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
     const jb::Pair minus = jb::pair(-scale, -scale), one = jb::pair(1.0f, 1.0f);
 #pragma unroll
     for (int u = 0; u < VECTORS; ++u) {
-      s = jb::fma2(powers(jb::pair(v[u].x, v[u].y), minus), one, s);
-      t = jb::fma2(powers(jb::pair(v[u].z, v[u].w), minus), one, t);
+#pragma unroll
+      for (int e = 0; e < WIDE_LOAD; e += 4) {
+        s = jb::fma2(powers(jb::pair(v[u].x[e], v[u].x[e + 1]), minus), one, s);
+        t = jb::fma2(powers(jb::pair(v[u].x[e + 2], v[u].x[e + 3]), minus), one, t);
+      }
     }
     sum += (double)((jb::lo(s) + jb::hi(s)) + (jb::lo(t) + jb::hi(t)));
   };
-  const int whole0 = x.lead > 0 ? 1 : 0, whole1 = min(last, (x.V + x.lead) / 4);     // vectors that lie inside the row
+  const int whole0 = x.lead > 0 ? 1 : 0, whole1 = min(last, (x.V + x.lead) / WIDE_LOAD);     // vectors that lie inside the row
   for (int i0 = first + tid; i0 < last; i0 += THREADS * VECTORS) {
-    float4 v[VECTORS];
+    Eight v[VECTORS];
     if (i0 >= whole0 && i0 + (VECTORS - 1) * THREADS < whole1) {
-      const float4* at = reinterpret_cast<const float4*>(x.x - x.lead) + i0;
+      const float* at = x.x - x.lead + (size_t)i0 * WIDE_LOAD;
 #pragma unroll
-      for (int u = 0; u < VECTORS; ++u) v[u] = at[u * THREADS];
+      for (int u = 0; u < VECTORS; ++u) v[u] = load_eight(at + u * THREADS * WIDE_LOAD);
     } else {
 #pragma unroll
-      for (int u = 0; u < VECTORS; ++u) v[u] = i0 + u * THREADS < last ? x.load(i0 + u * THREADS) : none;
+      for (int u = 0; u < VECTORS; ++u) {
+#pragma unroll
+        for (int e = 0; e < WIDE_LOAD; ++e) v[u].x[e] = -CUDART_INF_F;
+        if (i0 + u * THREADS < last) v[u] = x.load(i0 + u * THREADS);
+      }
     }
     take(v);
   }
@@ -178,10 +205,10 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
   if (wide || sum != sum || (scale == -CUDART_INF_F && top > -CUDART_INF_F)) {
     mine.sum = 0.0, mine.scale = power_of(mine.top);
     for (int i = first + tid; i < last; i += THREADS) {
-      const float4 v = x.load(i);
-      const float y[4] = {v.x, v.y, v.z, v.w};
+      const Eight v = x.load(i);
+      const float* y = v.x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < WIDE_LOAD; ++e)
         if (y[e] > -CUDART_INF_F) mine.sum += top == CUDART_INF_F ? (y[e] == top ? 1.0 : 0.0) : exp((double)y[e] - mine.top);
     }
   }
@@ -283,20 +310,29 @@ __global__ void __launch_bounds__(THREADS) beam_best_kernel(const Args a) {
   for (int r = 0; r < MOST_RANGES; ++r)
     if (maxima[r] >= least && maxima[r] > -CUDART_INF_F) chosen[atomicAdd(&n_chosen, 1)] = (unsigned short)(r * THREADS + tid);
   __syncthreads();
-  // ---- their numbers at or above it, in rounds of a vector a thread (two or three, unless many maxima are equal) ----
-  const int each = (x.vectors + a.ranges - 1) / a.ranges / THREADS + 1, n = n_chosen * each;       // vectors of a thread, at most
+  // ---- their numbers at or above it, in rounds of two halves of vectors a thread (one or two, unless many maxima are equal) ----
+  const int each = 2 * ((x.vectors + a.ranges - 1) / a.ranges / THREADS + 1), n = n_chosen * each;  // halves of a thread's vectors, at most
   Key bound = 0;                       // the K-th best so far, 0 while there are fewer
-  for (int j0 = 0; j0 < n; j0 += THREADS) {
-    const int j = j0 + tid;
-    if (j < n) {
-      const int slot = chosen[j / each], range = slot / THREADS, i = x.begin(range) + slot % THREADS + j % each * THREADS;
-      if (i < x.begin(range + 1)) {
-        const float4 v = x.load(i);
-        const float y[4] = {v.x, v.y, v.z, v.w};
+  for (int j0 = 0; j0 < n; j0 += THREADS * AGAIN) {
+    float4 v[AGAIN];
+    int half[AGAIN];                   // its number in the row; -1: none
+#pragma unroll
+    for (int u = 0; u < AGAIN; ++u) {
+      const int j = j0 + u * THREADS + tid;
+      half[u] = -1;
+      if (j < n) {
+        const int slot = chosen[j / each], range = slot / THREADS, i = x.begin(range) + slot % THREADS + j % each / 2 * THREADS;
+        if (i < x.begin(range + 1)) half[u] = 2 * i + j % each % 2, v[u] = x.load_half(half[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AGAIN; ++u) {
+      if (half[u] >= 0) {
+        const float y[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (y[e] >= least && y[e] > -CUDART_INF_F) {
-            const int token = 4 * i - x.lead + e;
+            const int token = 4 * half[u] - x.lead + e;
             const Key k = key_of(y[e], token);
             bool stop = false;
             for (int s = 0; s < a.S; ++s) stop |= stops[s] == token;
@@ -306,7 +342,7 @@ __global__ void __launch_bounds__(THREADS) beam_best_kernel(const Args a) {
       }
     }
     // (rounds whose numbers leave room for the next one's are put in order later)
-    const bool last = j0 + THREADS >= n, full = __syncthreads_or(n_found > ROOM - 4 * THREADS) != 0;
+    const bool last = j0 + THREADS * AGAIN >= n, full = __syncthreads_or(n_found > ROOM - 4 * AGAIN * THREADS) != 0;
     if (!full && !last) continue;
     // the K best of what was there and what came, in order: a key's place is the number of larger ones
     const int m = n_found;
@@ -315,6 +351,7 @@ __global__ void __launch_bounds__(THREADS) beam_best_kernel(const Args a) {
 #pragma unroll
     for (int u = 0; u < (ROOM + THREADS - 1) / THREADS; ++u) {
       place[u] = K;
+      if (u * THREADS >= m) continue;
       if (tid + u * THREADS < m) {
         k[u] = found[tid + u * THREADS];
         int above = 0;
