@@ -163,6 +163,45 @@ def test_select_sums_against_64_bits():
     assert torch.all((got - want).abs() <= LSE_TOL + 2.0 ** -24 * want.abs())
 
 
+def log_weight_of_the_largest(x):
+    """log softmax(x) of each row's largest number, from the distances to it (far from 0 their difference is all that 64 bits hold)."""
+    return -(x.double() - x.double().max(1, keepdim=True).values).exp().sum(1).log()
+
+
+@gpu
+@pytest.mark.parametrize("edge", [1e4, 1e6, 6.9314716e7, 1e8, 1e12, 3e38])
+def test_select_sums_of_far_logits(edge):
+    """Numbers on both sides of -edge and of edge, as near to one another as float32 has them, in every thread's share of a row; beside them rows with a
+    few such numbers among ordinary ones, and among masked ones."""
+    V = 16 * 4096 + 700
+    g = torch.Generator().manual_seed(11)
+    near = torch.tensor([float(torch.nextafter(torch.tensor(edge), torch.tensor(math.inf if up else 0.0))) for up in (True, False)] + [edge])
+    pick = near[torch.randint(0, 3, (2, V), generator=g)]
+    few = torch.where(torch.arange(V) % 176 == 5, near.max(), near.min())          # one of a thread's largest, all others a step below
+    masked = torch.full((2, V), torch.finfo(torch.float32).min)
+    masked[:, ::7] = torch.randn(2, len(range(0, V, 7)), generator=g)
+    masked[0, ::11] = -edge
+    x = torch.cat([-pick, pick[:1], -few[None], few[None], masked])
+    rows, want = x.shape[0], log_weight_of_the_largest(x)
+    out = run_select(x.cuda(), torch.zeros(rows, 1), [])
+    got = out["next_scores"].cpu().double()[:, 0]
+    assert torch.all((got - want).abs() <= LSE_TOL + 2.0 ** -24 * want.abs()), (got - want).tolist()
+
+
+@gpu
+def test_select_a_thread_with_numbers_on_both_sides_of_a_power():
+    """Some of a thread's vectors have numbers only below -1e8 in powers of two, others a number above; 8 apart, float32's spacing there."""
+    V, step = 32 * 4096, 8.0
+    for top in (-69314720.0, -69314712.0, -69314728.0):
+        x = torch.full((3, V), top - step)
+        x[0, ::176] = top
+        x[1, V // 2:] = top
+        x[2, :4096] = top
+        out = run_select(x.cuda(), torch.zeros(3, 1), [])
+        want = log_weight_of_the_largest(x)
+        assert torch.all((out["next_scores"].cpu().double()[:, 0] - want).abs() <= LSE_TOL + 2.0 ** -24 * want.abs())
+
+
 # -- tables ----------------------------------------------------------------------------------------------------------------
 def run_fork(parents, lengths, table, refs, free, F=None, spare=0, page=PAGE, in_place=False):
     (R, K), (N, W), Pn = (len(parents), len(parents[0])), (len(table), len(table[0])), len(refs)
