@@ -239,9 +239,6 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
   a.maxima[list * THREADS + tid] = top;
 }
 
-// Whether continuation (x, i) comes in front of (y, j): by total, then by beam and token.
-__device__ __forceinline__ bool in_front(double x, long long i, double y, long long j) { return x > y || (x == y && i < j); }
-
 // A logit's distance from its row's largest; beside entries at +inf, 0 for those and -inf for others.
 __device__ __forceinline__ double worth(float x, double top) {
   return top == CUDART_INF ? (x == CUDART_INF_F ? 0.0 : -CUDART_INF) : (double)x - top;
@@ -377,44 +374,46 @@ __global__ void __launch_bounds__(THREADS) beam_best_kernel(const Args a) {
 
 constexpr int JOIN_THREADS = 256;
 
-// One block a request.  Dynamic memory: K * K continuations (total, place), their shortened list, and for K * S stop tokens the same.
+// One block a request.  Dynamic memory: K * K continuations (total, key), their shortened list, and a list of K * S stop tokens.
 __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t memory[];
   __shared__ double base[MOST_BEAMS], top_of[MOST_BEAMS];  // see Best
   __shared__ double kth[MOST_BEAMS], head[MOST_BEAMS];
   __shared__ double on[MOST_BEAMS];
-  __shared__ long long on_at[MOST_BEAMS];
+  __shared__ int on_at[MOST_BEAMS];                        // beam * K + place
   __shared__ int n_list, n_stop;
   const int r = blockIdx.x, K = a.K, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, KK = K * K;
   double* totals = reinterpret_cast<double*>(memory);                    // [K][K]
   double* short_total = totals + KK;
-  double* stop_total = short_total + KK;                                 // [K * S]
-  int* token = reinterpret_cast<int*>(stop_total + K * a.S);             // [K][K]
-  int* short_at = token + KK;                                            // beam * K + place
-  int* stop_at = short_at + KK;                                          // beam * S + stop
+  Key* keys = reinterpret_cast<Key*>(short_total + KK);                  // [K][K]
+  Key* stop_key = keys + KK;                                             // [K * S]
+  int* short_at = reinterpret_cast<int*>(stop_key + K * a.S);            // beam * K + place
+  int* stop_at = short_at + KK;                                          // beam
   jb::pdl_launch_dependents();
   jb::pdl_wait();
+  if (tid < K) {
+    const Best best = a.best[r * K + tid];
+    base[tid] = best.base, top_of[tid] = best.top;
+  }
+  for (int i = tid; i < KK; i += JOIN_THREADS) keys[i] = a.keys[(size_t)r * KK + i];
+  // (a stop token's logit is on its way meanwhile)
+  const int b0 = a.S > 0 ? tid / a.S : K, stop0 = b0 < K ? a.stops[tid % a.S] : -1;
+  const float x0 = b0 < K && stop0 >= 0 && stop0 < a.V ? a.logits[((size_t)r * K + b0) * a.V + stop0] : -CUDART_INF_F;
+  auto total_of = [&](Key k, int b) { return base[b] + worth(logit_of(k), top_of[b]); };
   if (tid == 0) n_list = n_stop = 0;
   if (tid < K) {
     a.ended_parents[r * K + tid] = a.ended_tokens[r * K + tid] = -1;
     a.ended_scores[r * K + tid] = -CUDART_INF_F;
     on[tid] = -CUDART_INF;
     on_at[tid] = 0;
-    const Best best = a.best[r * K + tid];
-    base[tid] = best.base, top_of[tid] = best.top;
   }
+  __syncthreads();
   for (int i = tid; i < KK; i += JOIN_THREADS) {
-    const Best best = a.best[r * K + i / K];
-    const Key k = a.keys[(size_t)r * KK + i];
-    const double total = k > 0 ? best.base + worth(logit_of(k), best.top) : -CUDART_INF;
+    const double total = keys[i] > 0 ? total_of(keys[i], i / K) : -CUDART_INF;
     totals[i] = total;
-    token[i] = k > 0 ? token_of(k) : 0;
     if (i % K == 0) head[i / K] = total;
     if (i % K == K - 1) kth[i / K] = total;
   }
-  // (a stop token's logit is on its way meanwhile)
-  const int b0 = a.S > 0 ? tid / a.S : K, stop0 = b0 < K ? a.stops[tid % a.S] : -1;
-  const float x0 = b0 < K && stop0 >= 0 && stop0 < a.V ? a.logits[((size_t)r * K + b0) * a.V + stop0] : -CUDART_INF_F;
   __syncthreads();
   // ---- the K best of all beams: at least K lie at or above the largest K-th of a beam, and above the least of the beams' best ----
   double edge = -CUDART_INF, least = CUDART_INF;
@@ -428,46 +427,54 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const Args a) {
     }
   }
   __syncthreads();
-  const long long V = a.V;
   for (int i = tid; i < n_list; i += JOIN_THREADS) {
     const double t = short_total[i];
-    const long long at = short_at[i] / K * V + token[short_at[i]];
+    const int at = short_at[i];
     int before = 0;
-    for (int j = 0; j < n_list; ++j) before += in_front(short_total[j], short_at[j] / K * V + token[short_at[j]], t, at);
+    for (int j = 0; j < n_list; ++j) {                    // (a beam's keys are in order)
+      const double u = short_total[j];
+      before += u > t || (u == t && short_at[j] < at);
+    }
     if (before < K) on[before] = t, on_at[before] = at;
   }
   __syncthreads();
   // ---- stop tokens that stand among the K best ----
   for (int i = tid; i < K * a.S; i += JOIN_THREADS) {
     const int b = i / a.S, stop = a.stops[i % a.S];
-    bool again = false;
-    for (int s = 0; s < i % a.S; ++s) again |= a.stops[s] == stop;
-    if (stop < 0 || stop >= a.V || again || !(base[b] > -CUDART_INF)) continue;
+    bool twice = false;
+    for (int s = 0; s < i % a.S; ++s) twice |= a.stops[s] == stop;
+    if (stop < 0 || stop >= a.V || twice || !(base[b] > -CUDART_INF)) continue;
     const float x = i == tid ? x0 : a.logits[((size_t)r * K + b) * a.V + stop];
     if (!(x > -CUDART_INF_F)) continue;
-    const double t = base[b] + worth(x, top_of[b]);
-    if (!(t > -CUDART_INF) || !in_front(t, b * V + stop, on[K - 1], on[K - 1] > -CUDART_INF ? on_at[K - 1] : K * V)) continue;
+    const Key k = key_of(x, stop);
+    const double t = total_of(k, b);
+    if (!(t > -CUDART_INF) || t < on[K - 1]) continue;
     const int at = atomicAdd(&n_stop, 1);
-    stop_total[at] = t;
-    stop_at[at] = i;
+    stop_key[at] = k;
+    stop_at[at] = b;
   }
   __syncthreads();
   for (int i = tid; i < n_stop; i += JOIN_THREADS) {
-    const double t = stop_total[i];
-    const int b = stop_at[i] / a.S, stop = a.stops[stop_at[i] % a.S];
+    const Key k = stop_key[i];
+    const int b = stop_at[i];
+    const double t = total_of(k, b);
+    auto in_front = [&](Key other, int c) {
+      const double u = total_of(other, c);
+      return u > t || (u == t && (c < b || (c == b && other > k)));
+    };
     int place = 0, before = 0;
-    for (int j = 0; j < n_stop; ++j) place += in_front(stop_total[j], stop_at[j] / a.S * V + a.stops[stop_at[j] % a.S], t, b * V + stop);
-    for (int j = 0; j < K; ++j) before += on[j] > -CUDART_INF && in_front(on[j], on_at[j], t, b * V + stop);
+    for (int j = 0; j < n_stop; ++j) place += in_front(stop_key[j], stop_at[j]);
+    for (int j = 0; j < K; ++j) before += on[j] > -CUDART_INF && in_front(keys[on_at[j]], on_at[j] / K);
     if (place + before < K) {
       a.ended_parents[r * K + place] = b;
-      a.ended_tokens[r * K + place] = stop;
+      a.ended_tokens[r * K + place] = token_of(k);
       a.ended_scores[r * K + place] = (float)t;
     }
   }
   // ---- rows: a beam's best continuation stays in the beam's row ----
   if (warp == 0) {
     const bool live = lane < K && on[lane] > -CUDART_INF;
-    const int parent = live ? (int)(on_at[lane] / V) : -1 - lane;
+    const int parent = live ? on_at[lane] / K : -1 - lane;
     const unsigned same = __match_any_sync(0xffffffffu, parent);
     const bool stays = live && (same & ((1u << lane) - 1u)) == 0;
     const unsigned kept = __reduce_or_sync(0xffffffffu, stays ? 1u << parent : 0u);
@@ -480,14 +487,14 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const Args a) {
         row = __ffs(left) - 1;
       }
       a.parents[r * K + row] = live ? parent : -1;
-      a.tokens[r * K + row] = live ? (int)(on_at[lane] % V) : 0;
+      a.tokens[r * K + row] = live ? token_of(keys[on_at[lane]]) : 0;
       a.next_scores[r * K + row] = (float)on[lane];
     }
   }
 }
 
-size_t join_memory(int K, int S) { return (size_t)K * K * (8 + 8 + 4 + 4) + (size_t)K * S * (8 + 4); }
-static_assert(MOST_BEAMS * (MOST_BEAMS * 24 + MOST_STOPS * 12) <= 40 * 1024, "the third launch's memory");
+size_t join_memory(int K, int S) { return (size_t)K * K * (8 + 8 + 8 + 4) + (size_t)K * S * (8 + 4); }
+static_assert(MOST_BEAMS * (MOST_BEAMS * 28 + MOST_STOPS * 12) <= 40 * 1024, "the third launch's memory");
 
 }  // namespace
 

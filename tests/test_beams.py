@@ -163,6 +163,22 @@ def test_select_sums_against_64_bits():
     assert torch.all((got - want).abs() <= LSE_TOL + 2.0 ** -24 * want.abs())
 
 
+@gpu
+def test_select_within_a_beam_the_logits_decide():
+    """Scores so large that 64 bits hold no logarithm beside them: totals of a beam are equal, its logits are not."""
+    V = 9000
+    x = torch.zeros(4, V)
+    for row, best in enumerate(([70, 20, 8999], [5, 4, 3], [8000, 12, 13], [1, 2, 0])):
+        x[row, best] = torch.tensor([9.0, 8.0, 7.0])
+    out = run_select(x.cuda(), torch.tensor([[-1e17, NONE], [-1e30, -2e30]]), [])
+    assert out["parents"].tolist() == [[0, 0], [0, 0]] and out["tokens"].tolist() == [[70, 20], [8000, 12]]
+    # a stop token in front of others, and behind one, of its beam
+    out = run_select(x[:2].cuda(), torch.tensor([[-1e17, NONE]]), [20])
+    assert out["tokens"].tolist() == [[70, 8999]] and out["ended_tokens"].tolist() == [[20, -1]] and out["ended_parents"].tolist() == [[0, -1]]
+    out = run_select(x[:2].cuda(), torch.tensor([[-1e17, NONE]]), [8999])
+    assert out["tokens"].tolist() == [[70, 20]] and out["ended_tokens"].tolist() == [[-1, -1]]
+
+
 def log_weight_of_the_largest(x):
     """log softmax(x) of each row's largest number, from the distances to it (far from 0 their difference is all that 64 bits hold)."""
     return -(x.double() - x.double().max(1, keepdim=True).values).exp().sum(1).log()
