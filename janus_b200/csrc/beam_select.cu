@@ -35,7 +35,7 @@ constexpr int AGAIN = 2;                                  // halves of vectors t
 constexpr int ROOM = THREADS * 4 * AGAIN + MOST_BEAMS;            // candidates of a beam at a time
 constexpr float FAR = 40.0f;                              // how far a power may lie above what a thread's sum is relative to
 constexpr float WIDE = 1e8f;                              // powers beyond are made by 64-bit arithmetic
-constexpr float NEAR = 128.0f;                            // exp of as much less adds nothing that 64 bits hold, however many there are
+constexpr float NEAR = 256.0f;                            // powers of two as much below add nothing that 64 bits hold, however many there are
 
 __device__ __forceinline__ unsigned sortable(float x) {   // of numbers, -0 taken as 0
   const unsigned u = __float_as_uint(x + 0.0f);
@@ -153,10 +153,10 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
   if (dead(a.scores[row])) return;                        // (the second launch asks for nothing of it)
   // ---- maximum and sum of the thread's numbers: vectors first + tid, + THREADS, ... ----
   // The sum is relative to a power of two near the first numbers' maximum, which is left where it is until one lies FAR above: what changes
-  // with every new maximum would cost a warp as much as the numbers themselves.  Vectors whose powers all lie below -WIDE are passed over; where
-  // one of their numbers is worth something beside the largest of all (the only ones, or logits of some -7e7 on both sides of that edge),
-  // where a power lies beyond WIDE, and where something is no number, the thread goes over its numbers once more.
-  float top = -CUDART_INF_F, scale = -CUDART_INF_F, passed = -CUDART_INF_F;
+  // with every new maximum would cost a warp as much as the numbers themselves.  Powers beyond WIDE below that are 0; where they are
+  // all there is, where one lies just below -WIDE (beside larger ones it is worth something) or beyond WIDE, and where something is no
+  // number, the thread goes over its numbers once more.
+  float top = -CUDART_INF_F, scale = -CUDART_INF_F;
   bool wide = false;
   double sum = 0.0;
   auto take = [&](const Eight (&v)[VECTORS]) {
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
     top = fmaxf(top, high);
     const float power = high * (float)LOG2E;
     if (!(power >= -WIDE)) {
-      passed = fmaxf(passed, high);
+      wide |= power >= -WIDE - NEAR;
       return;
     }
     if (power > scale + FAR) {
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(THREADS) beam_rows_kernel(const Args a) {
     take(v);
   }
   Stat mine{sum, (double)scale, (double)top};
-  if (wide || sum != sum || (passed > -CUDART_INF_F && passed >= top - NEAR)) {
+  if (wide || sum != sum || (scale == -CUDART_INF_F && top > -CUDART_INF_F)) {
     mine.sum = 0.0, mine.scale = power_of(mine.top);
     for (int i = first + tid; i < last; i += THREADS) {
       const Eight v = x.load(i);
