@@ -13,8 +13,9 @@
 // stood still meanwhile; with a warp a beam in the third 76.  With fewer launches, the last block of a row or of a request going on
 // by a ticket: 61 by two, 65 by one, whose blocks that only read are fewer at a time; one request 12.8 and 13.6 us, by three 11.8.)
 // Within a beam the order is that of the logits (equal ones: the lowest token first), which no rounding touches; between beams it is
-// that of the totals, whose sum of exponentials is taken to 64 bits where threads meet: 32 bits would turn two beams round now and
-// then.
+// that of the totals.  The first launch makes each power, and adds up to 16 of them, in 32 bits: a power's exponent is within 2^6 and rounded
+// twice, so that a logarithm is off by 2 * 2^-19 log(2) + 2^-21 < 3.3e-6 (in practice some 5e-8), and differently for equal rows that begin at
+// different places of a vector.  Scores are given with that.  Where it could decide between two beams, the third launch sums their rows again in 64 bits.
 #include <math_constants.h>
 #include <stdio.h>
 #include <stddef.h>
@@ -373,108 +374,139 @@ __global__ void __launch_bounds__(THREADS) beam_best_kernel(const Args a) {
 }
 
 constexpr int JOIN_THREADS = 256;
+constexpr double DOUBT = 1e-5;                            // more than the totals of two beams may be off together
 
-// One block a request.  Dynamic memory: K * K continuations (total, key), their shortened list, and a list of K * S stop tokens.
-__global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const Args a) {
-  extern __shared__ __align__(16) uint8_t memory[];
-  __shared__ double base[MOST_BEAMS], top_of[MOST_BEAMS];  // see Best
-  __shared__ double kth[MOST_BEAMS], head[MOST_BEAMS];
-  __shared__ double on[MOST_BEAMS];
-  __shared__ int on_at[MOST_BEAMS];                        // beam * K + place
-  __shared__ int n_list, n_stop;
-  const int r = blockIdx.x, K = a.K, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, KK = K * K;
-  double* totals = reinterpret_cast<double*>(memory);                    // [K][K]
-  double* short_total = totals + KK;
-  Key* keys = reinterpret_cast<Key*>(short_total + KK);                  // [K][K]
-  Key* stop_key = keys + KK;                                             // [K * S]
-  int* short_at = reinterpret_cast<int*>(stop_key + K * a.S);            // beam * K + place
-  int* stop_at = short_at + KK;                                          // beam
-  jb::pdl_launch_dependents();
-  jb::pdl_wait();
-  if (tid < K) {
-    const Best best = a.best[r * K + tid];
-    base[tid] = best.base, top_of[tid] = best.top;
+// What a block of the third launch has in shared memory, by beam and place (of a beam's continuations, in order; of the stop tokens): beam * 32 +
+// place.  Behind it, of as many numbers as beams ask for: see Lists.
+struct Join {
+  double base[MOST_BEAMS], top[MOST_BEAMS];               // see Best
+  double score[MOST_BEAMS];
+  double kth[MOST_BEAMS], head[MOST_BEAMS];
+  double scratch[JOIN_THREADS / 32];
+  int n_list, n_stop;
+  unsigned doubtful;                                      // beams
+};
+struct Lists {
+  double* totals;         // then the short list's in order
+  double* short_total;
+  Key* keys;
+  Key* stop_key;
+  int* short_at;
+  int* on_at;             // the short list in order
+  int* stop_at;
+  __device__ __forceinline__ Lists(uint8_t* memory, int K) {
+    const int n = 32 * K;
+    totals = reinterpret_cast<double*>(memory), short_total = totals + n, keys = reinterpret_cast<Key*>(short_total + n), stop_key = keys + n;
+    short_at = reinterpret_cast<int*>(stop_key + n), on_at = short_at + n, stop_at = on_at + n;
   }
-  for (int i = tid; i < KK; i += JOIN_THREADS) keys[i] = a.keys[(size_t)r * KK + i];
-  // (a stop token's logit is on its way meanwhile)
-  const int b0 = a.S > 0 ? tid / a.S : K, stop0 = b0 < K ? a.stops[tid % a.S] : -1;
-  const float x0 = b0 < K && stop0 >= 0 && stop0 < a.V ? a.logits[((size_t)r * K + b0) * a.V + stop0] : -CUDART_INF_F;
-  auto total_of = [&](Key k, int b) { return base[b] + worth(logit_of(k), top_of[b]); };
-  if (tid == 0) n_list = n_stop = 0;
+};
+constexpr int JOIN_BYTES = 32 * (8 + 8 + 8 + 8 + 4 + 4 + 4);              // a beam
+static_assert(MOST_BEAMS * JOIN_BYTES + sizeof(Join) <= 48 * 1024, "the third launch's memory");
+
+// A continuation's total in its beam's list.
+__device__ __forceinline__ void put_total(Join& m, const Lists& l, int K, int b, int place, Key key, double base, double top) {
+  const double total = key > 0 ? base + worth(logit_of(key), top) : -CUDART_INF;
+  l.totals[b * 32 + place] = total;
+  if (place == 0) m.head[b] = total;
+  if (place == K - 1) m.kth[b] = total;
+}
+
+// From a request's continuations to what goes on and ends.  FIRST: beams are marked whose totals lie too near to one another's.
+// (Its code comes from memory, as the logits have passed through the L2 cache since: loops stay loops, and beams and places are told apart
+// without a division.  With loops unrolled and divisions 64 requests of 8 beams over 128,256 tokens took 63 to 65 us.)
+template <bool FIRST>
+__device__ __forceinline__ void join_beams(const Args& a, Join& m, uint8_t* memory, float x0) {
+  const int r = blockIdx.x, K = a.K, S = a.S, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, back = JOIN_THREADS - 1 - tid;
+  constexpr double doubt = FIRST ? DOUBT : 0.0;
+  const Lists l(memory, K);
+  const double* on = l.totals;
+  if (tid == 0) m.n_list = m.n_stop = 0, m.doubtful = 0u;
   if (tid < K) {
     a.ended_parents[r * K + tid] = a.ended_tokens[r * K + tid] = -1;
     a.ended_scores[r * K + tid] = -CUDART_INF_F;
-    on[tid] = -CUDART_INF;
-    on_at[tid] = 0;
-  }
-  __syncthreads();
-  for (int i = tid; i < KK; i += JOIN_THREADS) {
-    const double total = keys[i] > 0 ? total_of(keys[i], i / K) : -CUDART_INF;
-    totals[i] = total;
-    if (i % K == 0) head[i / K] = total;
-    if (i % K == K - 1) kth[i / K] = total;
   }
   __syncthreads();
   // ---- the K best of all beams: at least K lie at or above the largest K-th of a beam, and above the least of the beams' best ----
   double edge = -CUDART_INF, least = CUDART_INF;
-  for (int b = 0; b < K; ++b) edge = fmax(edge, kth[b]), least = fmin(least, head[b]);
-  edge = fmax(edge, least);
-  for (int i = tid; i < KK; i += JOIN_THREADS) {
-    if (totals[i] > -CUDART_INF && totals[i] >= edge) {
-      const int at = atomicAdd(&n_list, 1);
-      short_total[at] = totals[i];
-      short_at[at] = i;
+#pragma unroll 1
+  for (int b = 0; b < K; ++b) edge = fmax(edge, m.kth[b]), least = fmin(least, m.head[b]);
+  edge = fmax(edge, least) - doubt;
+#pragma unroll 1
+  for (int i = tid; i < 32 * K; i += JOIN_THREADS) {
+    const double t = l.totals[i];
+    if (lane < K && t > -CUDART_INF && t >= edge) {
+      const int at = atomicAdd(&m.n_list, 1);
+      l.short_total[at] = t;
+      l.short_at[at] = i;
     }
   }
   __syncthreads();
-  for (int i = tid; i < n_list; i += JOIN_THREADS) {
-    const double t = short_total[i];
-    const int at = short_at[i];
+#pragma unroll 1
+  for (int i = tid; i < m.n_list; i += JOIN_THREADS) {
+    const double t = l.short_total[i];
+    const int at = l.short_at[i];
     int before = 0;
-    for (int j = 0; j < n_list; ++j) {                    // (a beam's keys are in order)
-      const double u = short_total[j];
-      before += u > t || (u == t && short_at[j] < at);
+#pragma unroll 2
+    for (int j = 0; j < m.n_list; ++j) {                    // (a beam's keys are in order)
+      const double u = l.short_total[j];
+      before += u > t || (u == t && l.short_at[j] < at);
     }
-    if (before < K) on[before] = t, on_at[before] = at;
+    l.totals[before] = t, l.on_at[before] = at;
   }
+  if (tid < K && tid >= m.n_list) l.totals[tid] = -CUDART_INF, l.on_at[tid] = 0;
   __syncthreads();
+  const double last = on[K - 1] - doubt;
+  if (FIRST) {                                              // (by the last warps; of near ones in a row, every beam has a neighbour of another)
+#pragma unroll 1
+    for (int i = back; i + 1 < m.n_list; i += JOIN_THREADS) {
+      const double u = on[i + 1];
+      const int b = l.on_at[i] >> 5, c = l.on_at[i + 1] >> 5;
+      if (on[i] - u <= doubt && u >= last && b != c) atomicOr(&m.doubtful, 1u << b | 1u << c);
+    }
+  }
   // ---- stop tokens that stand among the K best ----
-  for (int i = tid; i < K * a.S; i += JOIN_THREADS) {
-    const int b = i / a.S, stop = a.stops[i % a.S];
+#pragma unroll 1
+  for (int b = warp; b < K; b += JOIN_THREADS / 32) {
+    if (lane >= S || !(m.base[b] > -CUDART_INF)) continue;
+    const int stop = a.stops[lane];
     bool twice = false;
-    for (int s = 0; s < i % a.S; ++s) twice |= a.stops[s] == stop;
-    if (stop < 0 || stop >= a.V || twice || !(base[b] > -CUDART_INF)) continue;
-    const float x = i == tid ? x0 : a.logits[((size_t)r * K + b) * a.V + stop];
-    if (!(x > -CUDART_INF_F)) continue;
-    const Key k = key_of(x, stop);
-    const double t = total_of(k, b);
-    if (!(t > -CUDART_INF) || t < on[K - 1]) continue;
-    const int at = atomicAdd(&n_stop, 1);
-    stop_key[at] = k;
-    stop_at[at] = b;
+#pragma unroll 1
+    for (int s = 0; s < lane; ++s) twice |= a.stops[s] == stop;
+    if (stop < 0 || stop >= a.V || twice) continue;
+    const float x = FIRST && b == warp ? x0 : a.logits[((size_t)r * K + b) * a.V + stop];
+    const double t = m.base[b] + worth(x, m.top[b]);
+    if (!(x > -CUDART_INF_F) || !(t > -CUDART_INF) || t < last) continue;
+    const int at = atomicAdd(&m.n_stop, 1);
+    l.stop_key[at] = key_of(x, stop);
+    l.stop_at[at] = b;
   }
   __syncthreads();
-  for (int i = tid; i < n_stop; i += JOIN_THREADS) {
-    const Key k = stop_key[i];
-    const int b = stop_at[i];
-    const double t = total_of(k, b);
-    auto in_front = [&](Key other, int c) {
-      const double u = total_of(other, c);
-      return u > t || (u == t && (c < b || (c == b && other > k)));
-    };
+  auto stop_total = [&](int i) { return m.base[l.stop_at[i]] + worth(logit_of(l.stop_key[i]), m.top[l.stop_at[i]]); };
+#pragma unroll 1
+  for (int i = tid; i < m.n_stop; i += JOIN_THREADS) {
+    const Key key = l.stop_key[i];
+    const int b = l.stop_at[i];
+    const double t = stop_total(i);
     int place = 0, before = 0;
-    for (int j = 0; j < n_stop; ++j) place += in_front(stop_key[j], stop_at[j]);
-    for (int j = 0; j < K; ++j) before += on[j] > -CUDART_INF && in_front(keys[on_at[j]], on_at[j] / K);
-    if (place + before < K) {
+#pragma unroll 1
+    for (int j = -K; j < m.n_stop; ++j) {                   // continuations, then stop tokens
+      const double u = j < 0 ? on[j + K] : stop_total(j);
+      const int c = j < 0 ? l.on_at[j + K] >> 5 : l.stop_at[j];
+      const Key other = j < 0 ? l.keys[l.on_at[j + K]] : l.stop_key[j];
+      const bool front = u > t || (u == t && (c < b || (c == b && other > key)));
+      before += front, place += front && j >= 0;
+      if (FIRST && fabs(u - t) <= doubt && c != b) atomicOr(&m.doubtful, 1u << b | 1u << c);
+    }
+    if (before < K) {
       a.ended_parents[r * K + place] = b;
-      a.ended_tokens[r * K + place] = token_of(k);
+      a.ended_tokens[r * K + place] = token_of(key);
       a.ended_scores[r * K + place] = (float)t;
     }
   }
   // ---- rows: a beam's best continuation stays in the beam's row ----
   if (warp == 0) {
     const bool live = lane < K && on[lane] > -CUDART_INF;
-    const int parent = live ? on_at[lane] / K : -1 - lane;
+    const int at = lane < K ? l.on_at[lane] : 0, parent = live ? at >> 5 : -1 - lane;
     const unsigned same = __match_any_sync(0xffffffffu, parent);
     const bool stays = live && (same & ((1u << lane) - 1u)) == 0;
     const unsigned kept = __reduce_or_sync(0xffffffffu, stays ? 1u << parent : 0u);
@@ -483,18 +515,90 @@ __global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const Args a) {
       int row = parent;
       if (!stays) {
         unsigned left = ~kept;
+#pragma unroll 1
         for (int n = __popc(moves & ((1u << lane) - 1u)); n > 0; --n) left &= left - 1;
         row = __ffs(left) - 1;
       }
       a.parents[r * K + row] = live ? parent : -1;
-      a.tokens[r * K + row] = live ? token_of(keys[on_at[lane]]) : 0;
+      a.tokens[r * K + row] = live ? token_of(l.keys[at]) : 0;
       a.next_scores[r * K + row] = (float)on[lane];
     }
   }
 }
 
-size_t join_memory(int K, int S) { return (size_t)K * K * (8 + 8 + 8 + 4) + (size_t)K * S * (8 + 4); }
-static_assert(MOST_BEAMS * (MOST_BEAMS * 28 + MOST_STOPS * 12) <= 40 * 1024, "the third launch's memory");
+// The sum of exp(x - top) over a row, in 64 bits and in one order whatever the row's address.
+__device__ __forceinline__ double row_sum(const float* x, int V, double top, double* scratch) {
+  constexpr int AHEAD = 16;
+  const int tid = threadIdx.x;
+  double part[AHEAD] = {}, sum = 0.0;
+#pragma unroll 1
+  for (int i0 = 0; i0 < V; i0 += JOIN_THREADS * AHEAD) {
+    float y[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) y[u] = i0 + u * JOIN_THREADS + tid < V ? x[i0 + u * JOIN_THREADS + tid] : -CUDART_INF_F;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const double d = worth(y[u], top);                  // (no number: nothing)
+      part[u] += exp(y[u] > -CUDART_INF_F ? d : -CUDART_INF);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) sum += part[u];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __syncthreads();
+  if ((tid & 31) == 0) scratch[tid >> 5] = sum;
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < JOIN_THREADS / 32; ++w) sum += scratch[w];
+  return sum;
+}
+
+// Where totals of two beams lie within DOUBT of one another and that may decide what goes on or ends, the first launch's sums do not tell them
+// apart: those beams' rows are summed once more by the definition, and everything is ranked again.  (A call of its own, behind what has been
+// written, so that nothing waits for it otherwise.)  Logits of the benchmark's distribution: no request of 768 with 8 beams over 128,256 tokens;
+// where all 8 beams of 64 requests are equal 715 us for 58.
+__device__ __noinline__ void join_again(const Args& a, Join& m, uint8_t* memory) {
+  const int r = blockIdx.x, K = a.K, tid = threadIdx.x;
+  for (unsigned left = m.doubtful; left != 0u; left &= left - 1) {
+    const int b = __ffs(left) - 1;
+    const double sum = row_sum(a.logits + ((size_t)r * K + b) * a.V, a.V, m.top[b], m.scratch);
+    if (tid == 0) m.base[b] = m.score[b] - log(sum);
+  }
+  __syncthreads();
+  const Lists l(memory, K);
+  for (int b = tid >> 5, place = tid & 31; b < K; b += JOIN_THREADS / 32)
+    if (place < K) put_total(m, l, K, b, place, l.keys[b * 32 + place], m.base[b], m.top[b]);
+  join_beams<false>(a, m, memory, 0.0f);
+}
+
+// One block a request.
+__global__ void __launch_bounds__(JOIN_THREADS) beam_join_kernel(const __grid_constant__ Args a) {
+  extern __shared__ __align__(16) uint8_t memory[];
+  __shared__ Join m;
+  const int r = blockIdx.x, K = a.K, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Lists l(memory, K);
+  jb::pdl_launch_dependents();
+  jb::pdl_wait();
+  if (tid < K) m.score[tid] = (double)a.scores[r * K + tid];          // (next_scores may be the same tensor)
+#pragma unroll 1
+  for (int b = warp; b < K; b += JOIN_THREADS / 32) {
+    const Best best = a.best[r * K + b];
+    if (lane == 0) m.base[b] = best.base, m.top[b] = best.top;
+    if (lane < K) {
+      const Key key = a.keys[((size_t)r * K + b) * K + lane];
+      l.keys[b * 32 + lane] = key;
+      put_total(m, l, K, b, lane, key, best.base, best.top);
+    }
+  }
+  // (a stop token's logit is on its way meanwhile)
+  const int stop = warp < K && lane < a.S ? a.stops[lane] : -1;
+  const float x0 = stop >= 0 && stop < a.V ? a.logits[((size_t)r * K + warp) * a.V + stop] : -CUDART_INF_F;
+  join_beams<true>(a, m, memory, x0);
+  __syncthreads();
+  if (m.doubtful != 0u) join_again(a, m, memory);
+}
 
 }  // namespace
 
@@ -526,7 +630,7 @@ JB_EXPORT int jb_beam_select(const void* given, cudaStream_t stream) {
   jb::Launch best(dim3(R * K), dim3(THREADS), 0, stream);
   e = cudaLaunchKernelEx(&best.c, beam_best_kernel, a);
   if (e != cudaSuccess) return (int)e;
-  const size_t memory = join_memory(K, S);
+  const size_t memory = (size_t)K * JOIN_BYTES;
   jb::Launch join(dim3(R), dim3(JOIN_THREADS), memory, stream);
   return (int)cudaLaunchKernelEx(&join.c, beam_join_kernel, a);
 }

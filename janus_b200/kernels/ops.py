@@ -2691,6 +2691,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, stop_tokens: torch.T
     score scores[r, b] (float32; -inf, or not a number: no beam) and the logits of row r K + b (float32 [R K, V]).  A continuation by
     token v is worth the score plus the log-probability log softmax(logits)[v]; continuations are ordered by that, taken to 64 bits, equal ones by
     beam and token (within a beam by logit and token).  Logits that are -inf or not numbers have no weight and are never chosen.
+    Scores come out as float32; their log-probabilities are off by 3.3e-6 at most beside that.
 
     Out, [R, K]: the K best continuations whose token is none of `stop_tokens` (int32, up to MOST_BEAM_STOPS; ids outside the vocabulary
     mean nothing) as parents (the beam that is continued), tokens and next_scores.  A beam's best continuation stands in the beam's own place, the

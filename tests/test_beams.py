@@ -179,6 +179,62 @@ def test_select_within_a_beam_the_logits_decide():
     assert out["tokens"].tolist() == [[70, 20]] and out["ended_tokens"].tolist() == [[-1, -1]]
 
 
+@gpu
+@pytest.mark.parametrize("V", [130, 4099, 50001, 50257, 128257])
+def test_select_equal_beams_at_any_address(V):
+    """Rows of the same logits begin at different places of a vector where the vocabulary is no multiple of 8, or where the tensor begins off one;
+    totals are equal all the same, and the lowest beam comes first."""
+    x, g = random_logits(3, V, V)
+    x = x.repeat_interleave(4, 0)
+    flat = torch.zeros(12 * V + 8, device="cuda")
+    order = x[::4].sort(dim=1, descending=True, stable=True).indices[:, :4].tolist()
+    for shift in (0, 1, 6):
+        view = flat[shift: shift + 12 * V].view(12, V)
+        view.copy_(x)
+        # the four beams' best, which are equal: every beam goes on with its own
+        out = run_select(view, torch.full((3, 4), -2.0), [])
+        assert out["parents"].tolist() == [[0, 1, 2, 3]] * 3 and out["tokens"].tolist() == [[o[0]] * 4 for o in order]
+        assert all(len(set(row)) == 1 for row in out["next_scores"].tolist())
+        # ... which all end: then their second ones; of eight equal beams' two best tokens each the first four stand in front
+        out = run_select(view, torch.full((3, 4), -2.0), [o[0] for o in order])
+        for r, o in enumerate(order):
+            others = [t for t in o if t not in [p[0] for p in order]]
+            assert out["ended_parents"][r].tolist() == [0, 1, 2, 3] and out["ended_tokens"][r].tolist() == [o[0]] * 4
+            assert out["parents"][r].tolist() == [0, 1, 2, 3] and out["tokens"][r].tolist() == [others[0]] * 4
+
+
+def near_beams(R, K, V, seed):
+    """Logits and scores whose rows' sums of exponentials are the same number: the beams of a request have the same logits at other places, above
+    one another by what float32 holds exactly.  Totals of the best tokens differ by the scores alone: steps of 2^-23."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.empty(R * K, V)
+    scores = torch.empty(R, K)
+    for r in range(R):
+        one = (torch.randn(V, generator=g) * 2.5 * 4096).round() / 4096
+        if r % 3 == 0:
+            one[:] = 0.0                                # one number stands out of a flat row
+            one[0], one[1] = 27.0, 26.5
+        elif r % 3 == 1:
+            one = 26.9921875 + (one / 64 * 4096).round() / 4096
+            one[::9] = 0.0
+        for b in range(K):
+            x[r * K + b] = one[torch.randperm(V, generator=g)] + [0.0, 64.0, -777.0, 3.5][(b + r) % 4]
+        scores[r] = -1.0 - torch.randperm(K, generator=g) * 2.0 ** -23
+    return x, scores
+
+
+@gpu
+@pytest.mark.parametrize("R, K, V", [(12, 4, 9001), (30, 2, 40000), (6, 8, 50257), (3, 32, 4100)])
+def test_select_beams_that_float32_sums_do_not_tell_apart(R, K, V):
+    """Totals 2^-23 apart, less than sums of float32 terms are off (2.1e-6): the order is that of 64 bits, among stop tokens as well."""
+    x, scores = near_beams(R, K, V, R + V)
+    for stops in ([], [int(t) for t in x[::K].argmax(1)[:16]] + [int(t) for t in x[1::K].argmax(1)[:16]]):
+        gap = P.select(x, scores, stops)[-1]
+        assert gap > 2.0 ** -24
+        for in_place in (False, True):
+            check_select(x, scores, stops, in_place, gap_needed=False)
+
+
 def log_weight_of_the_largest(x):
     """log softmax(x) of each row's largest number, from the distances to it (far from 0 their difference is all that 64 bits hold)."""
     return -(x.double() - x.double().max(1, keepdim=True).values).exp().sum(1).log()
