@@ -99,6 +99,20 @@ def room_for_beams(prompt_lens: Sequence[int], max_tokens: int, beams: int, batc
     return (sum(pages[:batch_size]) + 1) * PAGE_SIZE
 
 
+def table_width(pages: int) -> int:
+    """Pages that a step's tables have room for a row: a power of two, so that a captured step serves texts of about as many."""
+    W = 1
+    while W < pages:
+        W *= 2
+    return W
+
+
+def stateless_pages(R: int, K: int, W: int) -> Tuple[int, int]:
+    """(tokens of a page, pages) of the table of a model whose mixers keep only states.  Nobody stores anything in its pages: they carry positions
+    and lengths, and one is as long as the longest text.  Page 0 for rows without a beam, one a prompt, one a beam."""
+    return W * PAGE_SIZE, 1 + R + R * K
+
+
 class _Tables:
     """One cache group's tables on the device."""
 
@@ -124,9 +138,11 @@ class _BeamStep:
         self.scores, self.ended_scores = part(4).view(torch.float32), part(5).view(torch.float32)
         self.missing = [self.result[6 * N + g: 6 * N + g + 1] for g in range(G)]
         self.stops = torch.full((stops,), -1, **i32)
-        # a model whose mixers keep only states has tables of pages that nobody stores anything in: they carry positions and lengths
-        self.pages = [g.pool.n_pages for g in cache.groups] or [N * W + R + 2]
-        self.tables = [_Tables(R, K, W, n, device) for n in self.pages]
+        self.page_size, self.pages = PAGE_SIZE, [g.pool.n_pages for g in cache.groups]
+        if not cache.groups:
+            self.page_size, n = stateless_pages(R, K, W)
+            self.pages = [n]
+        self.tables = [_Tables(R, K, W if cache.groups else 1, n, device) for n in self.pages]
         self.lengths = torch.zeros((R, K), **i32)
         self.other_lengths = torch.zeros((R, K), **i32)
         self.spares = torch.zeros(G, **i32)
@@ -162,7 +178,7 @@ class _BeamStep:
                                kv_len=self.lengths if last else self.other_lengths, positions=t.positions, dest_rows=t.dest_rows,
                                new_table=t.table, new_refs=t.refs, new_free=t.free, new_n_free=t.n_free, copy_src=t.copy_src,
                                copy_dst=t.copy_dst, copy_rows=t.copy_rows, shared=t.shared, missing=self.missing[i], spare=self.spare[i],
-                               page_size=PAGE_SIZE)
+                               page_size=self.page_size)
                 if i < len(self.storage):
                     N = self.R * self.K
                     ops.copy_pages(self.storage[i], t.copy_src.view(N), t.copy_dst.view(N), t.copy_rows.view(N))
@@ -176,7 +192,7 @@ class _BeamStep:
               stops: List[int]) -> None:
         """A batch's first tables: row 0 of each request holds its prompt (pages[group][request]), which its slot keeps as well; mine[group]
         are the pages that beams may take, spare[group] the one that rows without a beam use."""
-        R, K, W = self.R, self.K, self.W
+        R, K = self.R, self.K
         if spare != self.spare:
             self.spare, self.graph = list(spare), None       # a captured launch knows it by number
         copy = lambda t, values: t.copy_(torch.from_numpy(np.asarray(values, dtype=np.int32).reshape(t.shape)))      # noqa: E731
@@ -187,7 +203,7 @@ class _BeamStep:
         copy(self.lengths, lengths)
         self.scores.copy_(torch.tensor([[0.0] + [-math.inf] * (K - 1)] * R))
         for g, t in enumerate(self.tables):
-            table, refs = np.full((R, K, W), -1, dtype=np.int32), np.zeros(self.pages[g], dtype=np.int32)
+            table, refs = np.full((R, K, t.table.shape[1]), -1, dtype=np.int32), np.zeros(self.pages[g], dtype=np.int32)
             table[:, 1:, 0] = spare[g]
             for r, held in enumerate(pages[g]):
                 table[r, 0, : len(held)] = held
@@ -208,7 +224,7 @@ class _BeamStep:
             rows.fill_(-1)
             rows[:, 0].fill_(self.spare[g])
             t.positions[r].zero_()
-            t.dest_rows[r].fill_(self.spare[g] * PAGE_SIZE)
+            t.dest_rows[r].fill_(self.spare[g] * self.page_size)
             t.shared[r].zero_()
 
     def run(self) -> None:
@@ -273,6 +289,9 @@ class BeamRunner:
                 raise ValueError(f"prompt {i} has {len(p)} tokens, the longest sequence allowed is {engine.max_seq_len}")
             if p.min() < 0 or p.max() >= V:
                 raise StepError(f"a token id of prompt {i} is outside the vocabulary of {V}")
+        for g in engine.cache.groups:
+            if g.pool.n_pages > ops.MOST_FORK_PAGES:
+                raise ValueError(f"beam search takes caches of up to {ops.MOST_FORK_PAGES} pages of {PAGE_SIZE} tokens, this one has {g.pool.n_pages}")
         stats = GenerationStats(requests=len(prompts))
         if max_tokens == 0:
             return [[BeamText([], 0.0, 0.0, "length")] for _ in prompts], stats
@@ -293,23 +312,32 @@ class BeamRunner:
     def _batch_size(self, prompts, searches, first: int, beams: int, most: int) -> int:
         """Requests of the next batch: as many as slots and every group's free pages have room for."""
         cache = self.engine.cache
-        free = min((g.pool.n_free for g in cache.groups), default=1 << 30) - 1            # one for rows without a beam
-        n = pages = 0
+        free = min((g.pool.n_free for g in cache.groups), default=0) - 1                  # one for rows without a beam
+        n = pages = longest = 0
         for q in searches[first: first + most]:
             length = len(prompts[q.index])
             pages += -(-length // PAGE_SIZE) + beams * beam_pages(length, q.limit)
-            if pages > free or (n + 1) * beams > cache.n_free_slots:
+            longest = max(longest, -(-(length + q.limit) // PAGE_SIZE))
+            if (n + 1) * beams > cache.n_free_slots:
                 break
+            if cache.groups:
+                if pages > free:
+                    break
+            else:
+                size, count = stateless_pages(n + 1, beams, table_width(longest))
+                if count > ops.MOST_FORK_PAGES or size * count > ops.MOST_FORK_TOKENS:
+                    break
             n += 1
         if n == 0:
-            raise CacheFull(f"request {searches[first].index} needs {pages + 1} pages of {PAGE_SIZE} tokens and {beams} slots for {beams} beams; the "
-                            f"cache has {free + 1} free pages and {cache.n_free_slots} slots")
+            what = f"request {searches[first].index} with {beams} beams needs {beams} slots"
+            if cache.groups:
+                raise CacheFull(f"{what} and {pages + 1} pages of {PAGE_SIZE} tokens; the cache has {cache.n_free_slots} free slots and {free + 1} pages")
+            raise CacheFull(f"{what} and texts of {longest * PAGE_SIZE} tokens; the cache has {cache.n_free_slots} free slots, tables of positions "
+                            f"count {ops.MOST_FORK_TOKENS} tokens")
         return n
 
     def _step_for(self, R: int, K: int, pages: int, stops: int) -> _BeamStep:
-        W = 1
-        while W < pages:
-            W *= 2
+        W = table_width(pages)
         key = (R, K, W, stops)
         step = self.steps.pop(key, None)
         logits, _ = self.engine._graph_output_buffers(R * K)
@@ -352,10 +380,7 @@ class BeamRunner:
             if cache.groups:
                 step.begin(slots, [len(p) for p in prompts], pages, mine, spare, stop)
             else:                                            # pages of no storage: 0 spare, then the prompts', then the beams'
-                counts = [-(-len(p) // PAGE_SIZE) for p in prompts]
-                at = np.concatenate([[1], 1 + np.cumsum(counts)])
-                step.begin(slots, [len(p) for p in prompts], [[list(range(a, a + n)) for a, n in zip(at, counts)]],
-                           [list(range(at[-1], at[-1] + own))], [0], stop)
+                step.begin(slots, [len(p) for p in prompts], [[[1 + r] for r in range(R)]], [list(range(1 + R, 1 + R + R * K))], [0], stop)
             torch.cuda.synchronize(engine.device)
             stats.prefill_tokens += sum(len(p) for p in prompts)
             stats.prefill_ms += (time.perf_counter() - t0) * 1e3

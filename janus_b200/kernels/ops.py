@@ -2728,6 +2728,10 @@ def beam_ranges(rows: int, vocab: int) -> int:
     return max(1, min(8, -(-vocab // 4096), -(-10 * SM_COUNT_TARGET // 2 // rows)))
 
 
+MOST_FORK_PAGES = 512 * 1024     # pages whose holders `fork_pages` counts
+MOST_FORK_TOKENS = 2 ** 31 - 1   # ... and their tokens
+
+
 def fork_pages(parents: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, free_pages: torch.Tensor,
                n_free: torch.Tensor, *, kv_len: torch.Tensor, positions: torch.Tensor, dest_rows: torch.Tensor, new_table: torch.Tensor,
                new_refs: torch.Tensor, new_free: torch.Tensor, new_n_free: torch.Tensor, copy_src: torch.Tensor, copy_dst: torch.Tensor,
@@ -2735,8 +2739,8 @@ def fork_pages(parents: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
     """The block tables of the next step's rows, which go on with rows of this one; all int32, in one launch.
 
     Rows come in R groups of K (up to MOST_BEAMS).  Row r K + k goes on with what row r K + parents[r, k] holds: lengths[r, parents[r, k]]
-    tokens in the pages that `table` [R K, W] lists for it; a parent outside 0 .. K - 1 means that the row does not go on.  refs [P] counts who
-    holds a page: rows of the table, and anybody else (a page that is to stay has a holder outside).  free_pages[:n_free] are pages
+    tokens in the pages that `table` [R K, W] lists for it; a parent outside 0 .. K - 1 means that the row does not go on.  refs [P] (up to
+    MOST_FORK_PAGES, of MOST_FORK_TOKENS tokens) counts who holds a page: rows of the table, and anybody else (a page that is to stay has a holder outside).  free_pages[:n_free] are pages
     that nobody holds.  Each row that goes on is made ready for one more token.  Whole pages are held by all rows that go on with
     them.  The page that the token goes to stays with the lowest row of the group that holds it, if nobody else does; any other row
     takes a page of its own from the back of the free list, with a copy to be made where the page is partly filled (a partly filled page is
@@ -2753,7 +2757,8 @@ def fork_pages(parents: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
     kv_len, new_table, new_refs, new_free and new_n_free may be lengths, table, refs, free_pages and n_free themselves, which are
     then changed in place; other outputs are tensors of their own."""
     (R, K), (N, W), P, F = parents.shape, table.shape, refs.shape[0], free_pages.shape[0]
-    if not 1 <= K <= MOST_BEAMS or R < 1 or W < 1 or not 0 <= spare < P or page_size < 1:
+    if (not 1 <= K <= MOST_BEAMS or R < 1 or W < 1 or not 0 <= spare < P or page_size < 1 or P > MOST_FORK_PAGES
+            or P * page_size > MOST_FORK_TOKENS):
         raise KernelError(f"fork_pages: {R} groups of {K} rows (1 to {MOST_BEAMS}) of {W} pages, spare page {spare} of {P}, pages of {page_size}")
     tensors = (parents, lengths, table, refs, free_pages, n_free, kv_len, positions, dest_rows, new_table, new_refs, new_free, new_n_free,
                copy_src, copy_dst, copy_rows, shared, missing)

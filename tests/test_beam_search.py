@@ -113,6 +113,49 @@ def test_host_search_finds_the_best_text_of_all():
     assert got[0].tokens == best[0] and abs(got[0].value - best[1] / best[2]) < 1e-6
 
 
+def _cache(slots, groups=()):
+    from types import SimpleNamespace
+    groups = [SimpleNamespace(pool=SimpleNamespace(n_free=n, n_pages=n)) for n in groups]
+    return SimpleNamespace(n_free_slots=slots, groups=groups)
+
+
+def _runner(cache):
+    from types import SimpleNamespace
+    from janus_b200.engine.beams import BeamRunner
+    return BeamRunner(SimpleNamespace(cache=cache, max_seq_len=1 << 30, model=SimpleNamespace(vocab_size=100)))
+
+
+@pytest.mark.parametrize("requests, beams, length, limit", [(64, 4, 40, 66000), (1024, 1, 3, 70), (32, 32, 1000, 130000), (1, 32, 1, (1 << 25) - 64)])
+def test_batches_of_models_that_keep_only_states(requests, beams, length, limit):
+    """Their tables are of pages that hold nothing; whatever a batch's slots have room for, they are what `ops.fork_pages` takes."""
+    from janus_b200.engine.beams import stateless_pages, table_width
+    from janus_b200.kernels import ops
+    prompts, searches = [[1] * length] * requests, [_Search(i, limit) for i in range(requests)]
+    n = _runner(_cache(1024))._batch_size(prompts, searches, 0, beams, requests)
+    assert n == requests
+    size, pages = stateless_pages(n, beams, table_width(-(-(length + limit) // 64)))
+    assert size >= length + limit and pages <= ops.MOST_FORK_PAGES and size * pages <= ops.MOST_FORK_TOKENS
+
+
+def test_batches_stop_where_tables_end():
+    """Texts so long that their tokens pass what tables count: fewer requests a batch; one that is alone too long is refused."""
+    from janus_b200.cache import CacheFull
+    limit = 1 << 22
+    prompts, searches = [[1]] * 300, [_Search(i, limit) for i in range(300)]
+    n = _runner(_cache(4096))._batch_size(prompts, searches, 0, 4, 300)
+    assert n == 50                                          # pages of 2^23 tokens, 255 of them: 1 + 5 n
+    with pytest.raises(CacheFull, match="tables"):
+        _runner(_cache(4096))._batch_size(prompts, [_Search(0, 1 << 29)], 0, 4, 1)
+    with pytest.raises(CacheFull, match="1 pages"):
+        _runner(_cache(4096, [1]))._batch_size(prompts, searches[:1], 0, 1, 1)
+
+
+def test_a_cache_of_more_pages_than_tables_count_is_refused_before_the_prompts():
+    from janus_b200.kernels import ops
+    with pytest.raises(ValueError, match="pages"):
+        _runner(_cache(64, [10, ops.MOST_FORK_PAGES + 1])).generate([[1, 2]], 2, 10)
+
+
 def test_room_for_beams():
     assert beam_pages(64, 1) == 1 and beam_pages(63, 1) == 1 and beam_pages(63, 2) == 2 and beam_pages(130, 70) == 2
     assert room_for_beams([10, 64], 1, 3, 2) == (1 + 3 + 1 + 3 + 1) * 64
@@ -181,6 +224,63 @@ def test_every_architecture_searches_as_the_plain_search(name):
     assert stats.requests == 3 and stats.batches == 1
     model.engine.cache.check()
     assert model.engine.cache.n_free_slots == 64 and all(g.pool.n_held == 0 for g in model.engine.cache.groups)
+
+
+STATES_ONLY = {
+    "lightning": dict(architecture="Zivitar", vocab=120, width=64, norm=dict(eps=1e-5), streams=2,
+                      layers=[test_zivitar.layer("lightning", dict(heads=2, dim=16, vdim=40, decay=[0.9, 0.999]), 96, 1.0),
+                              test_zivitar.layer("lightning", dict(heads=4, dim=8, vdim=16, decay=[0.5, 0.8, 0.95, 0.99]), 72, 0.5)]),
+    "mamba2": test_ramolix.config(140, 96, 1e-6, 1.0, 1.0, [test_ramolix.layer("mamba2", test_ramolix.mamba(3, 16, 24, 3, 4, 3), 40),
+                                                            test_ramolix.layer("mamba2", test_ramolix.mamba(2, 24, 8, 1, 2, 1), 72)])}
+
+
+@gpu
+@pytest.mark.parametrize("name", list(STATES_ONLY))
+def test_models_that_keep_only_states(name):
+    """No pages at all: states move with their beams, positions and lengths with tables that hold nothing."""
+    model = random_model(STATES_ONLY[name], "float32")
+    assert not model.engine.cache.groups
+    stops = [7, 11]
+    cases = clear_cases(model, model.engine.model.vocab_size, [66, 5, 31], 4, 9, stops, 1.0, False, 3, 100, 1e-3)
+    for _ in range(2):                                       # (the second time from the captured step)
+        got, stats = model.generate_beams([c[0] for c in cases], beams=4, max_tokens=9, stop_token_ids=stops, ignore_eos=True, return_all=True)
+        for texts, (_, want) in zip(got, cases):
+            assert [(t.tokens, t.reason) for t in texts] == [(w[0], w[3]) for w in want]
+    assert stats.graph_captures == 0
+    # texts across what would be pages of 64 tokens, alone and in a batch
+    whole, _ = model.generate_beams([c[0] for c in cases], beams=3, max_tokens=100, ignore_eos=True, return_all=True)
+    for (prompt, _), texts in zip(cases, whole):
+        alone, _ = model.generate_beams([prompt], beams=3, max_tokens=100, ignore_eos=True, return_all=True)
+        assert [t.tokens for t in alone[0]] == [t.tokens for t in texts] and all(len(t.tokens) == 100 for t in texts)
+    model.engine.cache.check()
+    assert model.engine.cache.n_free_slots == 64
+
+
+@gpu
+def test_many_long_requests_of_a_model_that_keeps_only_states(monkeypatch):
+    """64 requests of 4 beams with tables for texts of 70,000 tokens, more than 2^19 pages of 64: the first 30 tokens of them."""
+    import janus_b200
+    from janus_b200.engine.beams import BeamRunner
+    model = janus_b200.load_random(STATES_ONLY["mamba2"], 3, dtype="float32", max_tokens=1 << 20, max_slots=256, std=0.15)
+    prompts = [random_tokens(2 + n % 5, 140, n) for n in range(64)]
+    want, _ = model.generate_beams(prompts, beams=4, max_tokens=30, ignore_eos=True, return_all=True)
+    run_batch, step_for, widths = BeamRunner._run_batch, BeamRunner._step_for, []
+
+    def shortened(self, prompts, searches, *args):
+        def cut(self, *sizes):
+            step = step_for(self, *sizes)
+            widths.append(step.W)
+            for q in searches:
+                q.limit = 30
+            return step
+
+        monkeypatch.setattr(BeamRunner, "_step_for", cut)
+        return run_batch(self, prompts, searches, *args)
+
+    monkeypatch.setattr(BeamRunner, "_run_batch", shortened)
+    got, stats = model.generate_beams(prompts, beams=4, max_tokens=70000, ignore_eos=True, return_all=True)
+    assert stats.batches == 1 and widths == [2048]
+    assert [[t.tokens for t in row] for row in got] == [[t.tokens for t in row] for row in want]
 
 
 @gpu

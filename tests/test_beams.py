@@ -763,6 +763,13 @@ def test_fork_spare_page_refused(change):
         ops.fork_pages(**{**_fork_args(), **change})
 
 
+def test_fork_more_pages_than_are_counted_refused():
+    with pytest.raises(ops.KernelError, match="fork_pages"):
+        ops.fork_pages(**_fork_args(n=ops.MOST_FORK_PAGES + 1))
+    with pytest.raises(ops.KernelError, match="fork_pages"):
+        ops.fork_pages(**{**_fork_args(n=8), "page_size": 1 << 28})
+
+
 @pytest.mark.parametrize("change", [dict(beams=33), dict(beams=3), dict(page_size=32), dict(hd=60), dict(hd=264), dict(nh=3), dict(nkv=0)])
 def test_attention_sizes_refused(change):
     with pytest.raises(ops.KernelError, match="attention_beams"):
