@@ -106,9 +106,29 @@ __device__ __forceinline__ Rows look_up(const Args& a, int block) {
   const int lane = threadIdx.x & 31, request = a.row_blocks == 1 ? block : block / a.row_blocks;
   return rows_of(a, block, lane < a.K ? a.kv_len[request * a.K + lane] : 0, a.shared[request]);
 }
-// Whether one of two numbers is infinite or none (an exponent of ones carries into the sign's place).  A weight of 0 silences neither, so values
-// of pages that not all rows read are looked at: such a value is left out and the rows that read it become no numbers, their neighbours stay.
+// Whether one of two numbers is infinite or none (an exponent of ones carries into the sign's place); the bits say which.  A weight of 0 silences
+// neither, so values of pages that not all rows read are looked at: such a value is left out, and that number of the rows that read it becomes no
+// number; their other numbers, and other rows, stay what they are.
 __device__ __forceinline__ uint32_t not_finite(uint32_t two) { return ((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+
+// Eight values of one key, some of them not finite: those are made 0 and noted for the beams that read the page.  (A call: inlined, what is hardly
+// ever done costs the warps registers, 102 us for 97 on the first case, 131 for 119 with 64 rows.)
+__device__ __noinline__ void note_values(uint4& place, uint32_t* bad, const unsigned long long* rows, int K, int G, int rho0, int n_rows) {
+  uint32_t readers = 0u;
+#pragma unroll 1
+  for (int b = 0; b < K; ++b) {
+    const int row = max(b * G - rho0, 0);
+    if (row < min((b + 1) * G - rho0, n_rows)) readers |= (uint32_t)(rows[row / 64] >> (row % 64) & 1ull) << b;
+  }
+  uint32_t v[4] = {place.x, place.y, place.z, place.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t two = not_finite(v[e]);
+    if (two & 0x00008000u) v[e] &= 0xffff0000u, atomicOr(bad + 2 * e, readers);
+    if (two & 0x80000000u) v[e] &= 0x0000ffffu, atomicOr(bad + 2 * e + 1, readers);
+  }
+  place = make_uint4(v[0], v[1], v[2], v[3]);
+}
 
 // ---------------------------------------------------------------------------
 // The tensor cores of tcgen05, keys on the tile's 128 rows, the beams' queries on its N columns, so that a request's few rows are no padding:
@@ -146,17 +166,27 @@ struct Tc {
   static constexpr int SLABS = HDC / 64, SLAB = KEYS * 128, SLOT = SLABS * SLAB;   // 64 numbers of a stage's keys; its keys, or its values
   static constexpr int TILES = HDC > 128 ? 2 : 1;            // of 128 of the head's numbers in O'
   static constexpr int Q = SLABS * N * 128, P = (N > 64 ? 2 : 1) * KEYS * 128;
-  static constexpr int MISC = 4 * N + 16 * N + 1300;         // ref, exchange, barriers and descriptions
-  static constexpr int FIT = (232448 - Q - P - MISC) / SLOT, SLOTS = FIT > 12 ? 12 : FIT, INFOS = SLOTS / 2 + 1;
+  // keys' and values' places, as many as fit beside queries, weights, ref, exchange, descriptions, barriers and notes of values
+  static constexpr int infos(int slots) { return slots / 2 + 1; }
+  static constexpr int barriers(int slots) { return 2 * slots + infos(slots) + 6; }
+  static constexpr int bytes(int slots) {
+    return slots * SLOT + Q + P + 4 * N + 16 * N + infos(slots) * (int)sizeof(Info) + barriers(slots) * 8 + 16 + 8 * HDC;
+  }
+  static constexpr int fit() {
+    int slots = 12;
+    while (bytes(slots) > 232448) --slots;
+    return slots;
+  }
+  static constexpr int SLOTS = fit(), INFOS = infos(SLOTS);
   static constexpr int AT_Q = SLOTS * SLOT, AT_P = AT_Q + Q, AT_REF = AT_P + P, AT_SWAP = AT_REF + 4 * N, AT_INFO = AT_SWAP + 16 * N,
-                       AT_BARS = AT_INFO + INFOS * (int)sizeof(Info), BARS = 2 * SLOTS + INFOS + 6, AT_BAD = AT_BARS + BARS * 8 + 16, SMEM = AT_BAD + 128;
+                       AT_BARS = AT_INFO + INFOS * (int)sizeof(Info), BARS = barriers(SLOTS), AT_BAD = AT_BARS + BARS * 8 + 16, SMEM = AT_BAD + 8 * HDC;
   static constexpr int AT_O = 2 * HALVES * N, COLS_USED = AT_O + TILES * N;     // of tensor memory: two S', O'
   static constexpr int COLS = COLS_USED <= 64 ? 64 : COLS_USED <= 128 ? 128 : COLS_USED <= 256 ? 256 : 512;
   static_assert(COLS_USED <= 512, "tensor memory");
   static constexpr int GROUPS = N > 16 ? 4 : 2, HALF = N / GROUPS;      // groups of four warps, columns of each
   static constexpr int PLACES = 1024;                                   // of the list, whose stages are counted
   static constexpr int WARPS = 4 * GROUPS, THREADS = 128 + 32 * WARPS;
-  static_assert(SLOTS >= 2 && SMEM <= 232448, "shared memory of a block");
+  static_assert(SLOTS >= 2 && SMEM == bytes(SLOTS) && SMEM <= 232448, "shared memory of a block");
   static __device__ __forceinline__ int stages_of(const Rows& x) { return (x.pages + SUB - 1) / SUB; }
 };
 
@@ -272,8 +302,8 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
   Info* info = reinterpret_cast<Info*>(smem + C::AT_INFO);             // [INFOS]
   const uint32_t full = base + C::AT_BARS, empty = full + 8 * C::SLOTS, told = empty + 8 * C::SLOTS, s_full = told + 8 * C::INFOS, p_full = s_full + 16,
                  pv_done = p_full + 8, q_full = pv_done + 8, o_full = q_full + 8;
-  // [block of rows' parity][group][2]: rows that read a value that is no finite number, as the group has found
-  unsigned long long (*bad)[C::GROUPS][2] = reinterpret_cast<unsigned long long (*)[C::GROUPS][2]>(smem + C::AT_BAD);
+  // [block of rows' parity][number of the head]: beams that read a value there that is not finite, as the group that looks there has found
+  uint32_t (*bad)[HDC] = reinterpret_cast<uint32_t (*)[HDC]>(smem + C::AT_BAD);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::AT_BARS + C::BARS * 8);
   if (tid == 0) {
     for (int i = 0; i < C::SLOTS; ++i) jb::mbar_init(full + 8 * i, 1), jb::mbar_init(empty + 8 * i, 1);
@@ -540,7 +570,8 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
         __syncwarp();
         if (lane == 0) jb::mbar_arrive(q_full);
         if (key < C::HALF) my_ref[key] = NOTHING;
-        if (key < 2) bad[turn & 1][group][key] = 0ull;
+        for (int d = key; d < HDC; d += 128)
+          if (d / 8 % C::GROUPS == group) bad[turn & 1][d] = 0u;
 #pragma unroll
         for (int c = 0; c < C::HALF; ++c) l[c] = 0.0f;
       }
@@ -567,9 +598,12 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
             odd |= not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
           }
           if (odd != 0u || behind) {
-            for (int at = group; at < C::SLABS * 8; at += C::GROUPS)
-              *reinterpret_cast<uint4*>(values + (at / 8) * C::SLAB + (((at ^ key) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
-            if (!behind) atomicOr(&bad[turn & 1][group][0], x->rows[sub][0]), atomicOr(&bad[turn & 1][group][1], x->rows[sub][1]);
+#pragma unroll 1
+            for (int at = group; at < C::SLABS * 8; at += C::GROUPS) {
+              uint4* place = reinterpret_cast<uint4*>(values + (at / 8) * C::SLAB + (((at ^ key) & 7) << 4));
+              if (odd != 0u && !behind) note_values(*place, bad[turn & 1] + at * 8, x->rows[sub], a.K, G, rho0, n_rows);
+              else *place = make_uint4(0u, 0u, 0u, 0u);
+            }
           }
         }
       }
@@ -699,11 +733,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
         if (key < C::HALF) {
           const int row = c0 + key, rho = rho0 + row;
           float* t = swap + c0 + key;
-          float sum = (t[0] + t[N]) + (t[2 * N] + t[3 * N]);
-          unsigned long long spoilt = 0ull;
-#pragma unroll
-          for (int g = 0; g < C::GROUPS; ++g) spoilt |= bad[spoil][g][row / 64];
-          if ((spoilt >> (row % 64)) & 1ull) sum = CUDART_NAN_F;
+          const float sum = (t[0] + t[N]) + (t[2 * N] + t[3 * N]);
           t[0] = complete ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
           if (row < n_rows) {
             const int item = (request * a.K + rho / G) * a.nh + kvh * G + rho % G;
@@ -721,6 +751,12 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
             jb::tmem_ld8(lanes + C::AT_O + m * N + c0 + c, v);
             jb::tmem_ld_wait();
             if (key + 128 * m < hd) {
+              const uint32_t spoilt = bad[spoil][key + 128 * m];
+              if (spoilt != 0u) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (spoilt >> ((rho0 + c0 + c + e) / G & 31) & 1u) v[e] = CUDART_NAN_F;
+              }
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const int row = c0 + c + e;

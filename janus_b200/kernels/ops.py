@@ -2851,8 +2851,9 @@ def attention_beams(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """Attention of one query token a row over the row's first kv_len[row] keys.  Rows come in groups of `beams` (up to MOST_BEAMS); the
     first shared[r] pages of the rows of group r are the same and are read once for all of them (a row of fewer tokens reads its
     own).  bfloat16: q and out [rows, nh hd], caches [pages, nkv, page_size, hd]; int32: block_table [rows, W], kv_len [rows] (up to W
-    pages), shared [rows / beams].  Heads of up to 256 numbers, multiples of 8; pages of 64 tokens.  A row without keys is 0.  max_kv_len: at least the
-    longest row's keys."""
+    pages), shared [rows / beams].  Heads of up to 256 numbers, multiples of 8; pages of 64 tokens.  A row without keys is 0.  A value that is
+    not finite makes that number of the rows that read it infinite or no number, and nothing else.  max_kv_len: at least the longest row's
+    keys."""
     N, W = block_table.shape
     if not 1 <= beams <= MOST_BEAMS or N < 1 or N % beams or page_size != 64 or W < 1:
         raise KernelError(f"attention_beams: {N} rows of {W} pages in groups of {beams} (1 to {MOST_BEAMS}), pages of {page_size} (64)")

@@ -604,6 +604,33 @@ def test_attention_numbers_that_are_not_finite_stay_with_their_readers(hd, K, gr
 
 
 @gpu
+@pytest.mark.parametrize("hd", [40, 64, 128, 136, 256])
+@pytest.mark.parametrize("K, group", [(4, 4), (5, 6), (5, 12), (11, 2)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_attention_a_value_that_is_not_finite_is_one_number_of_a_row(hd, K, group, what):
+    """Whether a stage is read by all rows of a tile or by some: the other numbers of the rows that read the value are those of the definition, and so
+    are the rows that do not."""
+    kv_len = [130] + [700] * (K - 2) + [650] + [700] * K
+    q, k, v, table, nh = attention_case(2, K, kv_len, [9, 9], 2, group, hd, 7)
+    v[table[1][5], 1, 17, hd - 3] = what                    # a page that all but the first beam share
+    v[table[1][5], 1, 18, 2] = v[table[1][6], 1, 40, 2] = what
+    v[table[2][10], 0, 3, 5] = what                         # own pages
+    v[table[2][10], 0, 3, 6] = v[table[2][10], 0, 59, 7] = what
+    v[table[K - 1][9], 0, 60, 0] = what
+    v[table[K + 1][3], 0, 11, 9] = what                     # a page that all of a request share
+    out = empty(2 * K, nh * hd, dtype=torch.bfloat16)
+    scale = 1.0 / math.sqrt(hd)
+    ops.attention_beams(q.cuda(), k.cuda(), v.cuda(), out, ints(table), ints(kv_len), ints([9, 9]), K, nh, 2, hd, PAGE, scale,
+                        Workspace(torch.device("cuda")), 700)
+    got = out.cpu().double().view(2 * K, nh, hd)
+    want, size = P.attention(q, k, v, table, kv_len, nh, 2, hd, scale)
+    bad = ~torch.isfinite(want)
+    assert int(bad.sum()) == group * (2 * (K - 1) + 3 + 1 + K) and not torch.isfinite(got[bad]).any()
+    off = (got - want).abs() / attention_bound(want, size)
+    assert float(off[~bad].max()) <= 1.0
+
+
+@gpu
 def test_attention_shared_pages_said_too_many():
     """More pages said to be shared than the rows have."""
     q, k, v, table, nh = attention_case(1, 2, [100, 100], [2], 1, 4, 64, 3)
