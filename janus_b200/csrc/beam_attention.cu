@@ -149,7 +149,7 @@ __device__ __noinline__ void note_values(uint4& place, uint32_t* bad, const unsi
 // stages in turn, so that a stage need not wait for the products of the one before, level; keys and values asked for by two pairs of lanes at
 // once, level, with 64 rows 130.
 // ---------------------------------------------------------------------------
-constexpr float NOTHING = -1e30f;                            // what weights are relative to before a row has seen a key
+constexpr float NOTHING = -3.402823466e38f;                  // what weights are relative to before a row has seen a key: no number is below
 
 struct Info {                                                // of a stage
   int first, last, final_, whole;                            // of its block of rows' keys in this share; of the share; no mask
@@ -626,6 +626,11 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
             for (int e = 0; e < 8; ++e) s[t][c + e] = v[e];
           }
         jb::tmem_ld_wait();
+        // (rounded by itself: a fused product less the row's number, which is rounded, would leave 2^-24 of a large score as a power)
+#pragma unroll
+        for (int t = 0; t < C::HALVES; ++t)
+#pragma unroll
+          for (int c = 0; c < C::HALF; ++c) s[t][c] = __fmul_rn(s[t][c], a.scale_log2);
         if (masked) {
 #pragma unroll
           for (int t = 0; t < C::HALVES; ++t)
@@ -643,8 +648,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
 #pragma unroll
         for (int t = 0; t < C::HALVES; ++t) {
           float* y = s[t] + c;
-          y[0] = fmaf(y[0], a.scale_log2, -r.x), y[1] = fmaf(y[1], a.scale_log2, -r.y);
-          y[2] = fmaf(y[2], a.scale_log2, -r.z), y[3] = fmaf(y[3], a.scale_log2, -r.w);
+          y[0] -= r.x, y[1] -= r.y, y[2] -= r.z, y[3] -= r.w;
           high = fmaxf(high, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
         }
       }
@@ -665,7 +669,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
         if (key < C::HALF) {
           const float* t = swap + c0 + key;
           old = my_ref[key];
-          now = fmaxf(old, fmaxf(fmaxf(t[0], t[N]), fmaxf(t[2 * N], t[3 * N])) * a.scale_log2);
+          now = fmaxf(old, fmaxf(fmaxf(t[0], t[N]), fmaxf(t[2 * N], t[3 * N])));
         }
         group_any(1 + group, false);
         if (key < C::HALF) my_ref[key] = now, swap[c0 + key] = fast_exp2(old - now);
@@ -676,7 +680,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
 #pragma unroll
-            for (int t = 0; t < C::HALVES; ++t) s[t][c + e] = fmaf(s[t][c + e], a.scale_log2, -my_ref[c + e]);
+            for (int t = 0; t < C::HALVES; ++t) s[t][c + e] -= my_ref[c + e];
             f[e] = swap[c0 + c + e], l[c + e] *= f[e];
           }
           if (!first) {
@@ -739,7 +743,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
             const int item = (request * a.K + rho / G) * a.nh + kvh * G + rho % G;
             t[N] = __int_as_float(complete ? item : (int)record + row);
             if (piece == piece0) a.parts[item] = make_int2(piece0, piece1 - piece0 + 1);
-            if (!complete) a.part_ml[record + row] = make_float2(sum != sum ? 0.0f : my_ref[key] > 0.5f * NOTHING ? my_ref[key] : -CUDART_INF_F, sum);
+            if (!complete) a.part_ml[record + row] = make_float2(sum != sum ? 0.0f : sum == 0.0f ? -CUDART_INF_F : my_ref[key], sum);
           }
         }
         group_any(1 + group, false);

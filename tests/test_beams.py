@@ -631,6 +631,32 @@ def test_attention_a_value_that_is_not_finite_is_one_number_of_a_row(hd, K, grou
 
 
 @gpu
+@pytest.mark.parametrize("size", [1e3, 1e15, 1e18])
+@pytest.mark.parametrize("K, group, hd", [(4, 4, 128), (5, 2, 64), (16, 4, 64), (3, 2, 256)])
+def test_attention_scores_far_below_zero(K, group, hd, size):
+    """All scores of some rows lie at -size^2 and below, of some at size^2 and above: the largest of them share the weight, in one part and in several."""
+    R = 2
+    kv_len = [130] * K + [1500] * K
+    q, k, v, table, nh = attention_case(R, K, kv_len, [1, 9], 2, group, hd, 5)
+    sign = torch.where(torch.arange(R * K * nh) % 3 == 0, 1.0, -1.0).view(R * K, nh, 1)
+    q = torch.zeros(R * K, nh, hd)
+    q[:, :, 1:2] = sign * size
+    q = q.view(R * K, nh * hd).bfloat16()
+    fine = torch.isfinite(k)
+    k = torch.where(fine, torch.zeros(()), k.float())
+    # a key in seven has the least, one in five the most: numbers that bfloat16 holds
+    step = torch.arange(k.shape[0] * PAGE).view(k.shape[0], 1, PAGE)
+    k[..., 1] = torch.where(fine[..., 1], torch.where(step % 7 == 0, 0.5, torch.where(step % 5 == 0, 2.0, 1.0)) * size, k[..., 1])
+    k = k.bfloat16()
+    out = empty(R * K, nh * hd, dtype=torch.bfloat16)
+    ops.attention_beams(q.cuda(), k.cuda(), v.cuda(), out, ints(table), ints(kv_len), ints([1, 9]), K, nh, 2, hd, PAGE, 0.25,
+                        Workspace(torch.device("cuda")), 1500)
+    want, weight = P.attention(q, k, v, table, kv_len, nh, 2, hd, 0.25)
+    off = (out.cpu().double().view(R * K, nh, hd) - want).abs()
+    assert float((off / attention_bound(want, weight)).max()) <= 1.0
+
+
+@gpu
 def test_attention_shared_pages_said_too_many():
     """More pages said to be shared than the rows have."""
     q, k, v, table, nh = attention_case(1, 2, [100, 100], [2], 1, 4, 64, 3)
