@@ -57,7 +57,9 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
-// Bounded wait: false (and *status = code) if the phase did not complete in 4e9 cycles, about two seconds.
+// Bounded wait: false (and *status = code) if the phase did not complete in 4e9 cycles, about two seconds.  Codes are 5, what was waited for
+// (1 a place of the ring, 2 keys or values, 3 a stage's description, 4 queries, 5 weights, 6 scores, 7 the products of the stage before, 8 a
+// block of rows' sums), and who waited (1 the loads, 2 the products' issuer, 3 the weights and the results).
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* status, int code) {
   if (jb::mbar_try(bar, parity)) return true;
   const long long t0 = clock64();
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
       const bool there = lane < n && keys0 > 0 && page0 >= 0 && page0 < a.n_pages;    // (no page: no keys)
       const unsigned loads = __ballot_sync(0xffffffffu, there);
       const bool whole = __all_sync(0xffffffffu, lane >= C::SUB || (there && keys0 == PAGE && rows[0] == all[0] && rows[1] == all[1]));
-      ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot.at, slot.phase ^ 1, status, 54));
+      ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot.at, slot.phase ^ 1, status, 511));
       if (!ok) break;
       Info& to = info[note.at];
       if (lane < C::SUB) to.keys[lane] = there ? keys0 : 0, to.rows[lane][0] = rows[0], to.rows[lane][1] = rows[1];
@@ -457,7 +459,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
 #pragma unroll
       for (int half = 0; half < 2; ++half) {                           // keys, values
         if (half > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot.at, slot.phase ^ 1, status, 54));
+          ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * slot.at, slot.phase ^ 1, status, 511));
           if (!ok) break;
         }
         const uint32_t here = full + 8 * slot.at, place = base + slot.at * C::SLOT + lane * PAGE * 128;
@@ -485,7 +487,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
     }
     // gave up: what is still on its way arrives before the block ends (or its wait gives up as well)
     if (!ok && lane == 0)
-      for (int i = 0; i < C::SLOTS; ++i) mbar_wait(full + 8 * i, i < slot.at ? slot.phase : slot.phase ^ 1, status, 53);
+      for (int i = 0; i < C::SLOTS; ++i) mbar_wait(full + 8 * i, i < slot.at ? slot.phase : slot.phase ^ 1, status, 521);
   } else if (warp == 1) {
     if (elected()) {
       const uint32_t idesc_s = jb::instr_desc_bf16(N), idesc_o = jb::instr_desc_bf16(N) | (1u << 15) | (1u << 16);   // values and weights: MN-major
@@ -513,9 +515,9 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
       for (;; ++it) {
         const Info& x = info[note.at];
         if (!ahead) {
-          ok = mbar_wait(full + 8 * ks.at, ks.phase, status, 53) && mbar_wait(told + 8 * note.at, note.phase, status, 53);
+          ok = mbar_wait(full + 8 * ks.at, ks.phase, status, 522) && mbar_wait(told + 8 * note.at, note.phase, status, 532);
           if (!ok || x.final_ == 2) break;
-          if (x.first) ok = mbar_wait(q_full, turn++ & 1, status, 55);
+          if (x.first) ok = mbar_wait(q_full, turn++ & 1, status, 542);
           if (!ok) break;
           scores(it & 1);
         }
@@ -525,7 +527,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
           scores((it + 1) & 1);
           ahead = true;
         }
-        ok = mbar_wait(full + 8 * vs.at, vs.phase, status, 53) && mbar_wait(p_full, it & 1, status, 56);
+        ok = mbar_wait(full + 8 * vs.at, vs.phase, status, 522) && mbar_wait(p_full, it & 1, status, 552);
         if (!ok) break;
         jb::tc_fence_after();
         const uint64_t v = desc_mn_sw128(base + vs.at * C::SLOT, C::SLAB, 1024);         // (further on by 16 bytes a unit)
@@ -554,7 +556,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
     for (int it = 0;; ++it) {
       // a block of rows begins: its queries, by all groups, while its first keys are on their way
       const Info* x = info + note.at;
-      ok = ok && mbar_wait(told + 8 * note.at, note.phase, status, 53);
+      ok = ok && mbar_wait(told + 8 * note.at, note.phase, status, 533);
       if (first) {
         if (group_any(1 + group, !ok)) break;                          // (a wait ran out, of one of the group's warps: all leave)
         request = x->request, rho0 = x->rho0, n_rows = x->n_rows, kvh = x->kvh;
@@ -583,7 +585,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
       if (masked) {
         // values behind the last key, or that are no finite numbers: a weight of 0 does not silence them (a part of the head's numbers a
         // group; while the scores are made)
-        ok = ok && mbar_wait(full + 8 * vs.at, vs.phase, status, 53);
+        ok = ok && mbar_wait(full + 8 * vs.at, vs.phase, status, 523);
 #pragma unroll
         for (int t = 0; t < C::HALVES; ++t) {
           const int sub = t * 2 + (quarter >> 1);
@@ -607,11 +609,11 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
           }
         }
       }
-      ok = ok && mbar_wait(s_full + 8 * (it & 1), (it >> 1) & 1, status, 57);
+      ok = ok && mbar_wait(s_full + 8 * (it & 1), (it >> 1) & 1, status, 563);
       jb::tc_fence_after();
       bool rest = it == 0;                                             // P is free, and O' at rest
       auto settle = [&]() {
-        if (!rest) ok = ok && mbar_wait(pv_done, (it - 1) & 1, status, 58), jb::tc_fence_after();
+        if (!rest) ok = ok && mbar_wait(pv_done, (it - 1) & 1, status, 573), jb::tc_fence_after();
         rest = true;
       };
       float s[C::HALVES][C::HALF];
@@ -727,7 +729,7 @@ __global__ void __launch_bounds__(Tc<HDC, N>::THREADS, 1) beam_attention_kernel(
         // the sums over the keys: half the columns go to the other half of the lanes, and so on, until a lane has one
         columns_summed<C::HALF>(l, swap + quarter * N + c0);
         const int spoil = turn & 1;
-        ok = ok && mbar_wait(o_full, turn++ & 1, status, 59);
+        ok = ok && mbar_wait(o_full, turn++ & 1, status, 583);
         jb::tc_fence_after();
         group_any(1 + group, false);
         const int piece = (int)blockIdx.x;

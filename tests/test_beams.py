@@ -784,6 +784,30 @@ def _attention_args(K=2, R=1, nh=4, nkv=2, hd=64, W=2, device="cpu"):
                 shared=torch.zeros(R, **i), beams=K, nh=nh, nkv=nkv, hd=hd, page_size=64, scale=1.0, workspace=None, max_kv_len=64)
 
 
+def test_a_wait_that_ran_out_names_who_waited():
+    """Every code that a bounded wait of the kernels gives ends in the digit of one of the three that a message names, and in attention of beams in
+    that of the warp it stands in."""
+    import os
+    import re
+    folder = os.path.join(os.path.dirname(ops.__file__), "..", "csrc")
+    for name in sorted(os.listdir(folder)):
+        if name.endswith((".cu", ".cuh")):
+            text = open(os.path.join(folder, name)).read()
+            codes = [int(c) for c in re.findall(r"mbar_wait\([^;]*?status, (\d+)\)", text)]
+            assert all(c % 10 in (1, 2, 3) for c in codes), (name, codes)
+    text = open(os.path.join(folder, "beam_attention.cu")).read()
+    text = text[text.index("beam_attention_kernel"):]
+    roles = [text.index(s) for s in ("if (warp == 0) {", "} else if (warp == 1) {", "} else if (warp >= 4) {", "// The parts of a (beam, head)")]
+    for role, (begin, end) in enumerate(zip(roles, roles[1:]), 1):
+        codes = [int(c) for c in re.findall(r"status, (\d+)\)", text[begin:end])]
+        assert codes and all(c % 10 == role for c in codes), (role, codes)
+    for code, who in ((511, "TMA producer"), (552, "MMA issuer"), (583, "epilogue")):
+        ops.kernel_status(torch.device("cpu")).fill_(code)
+        with pytest.raises(ops.KernelError, match=f"{who}, code {code}"):
+            ops.check_kernel_status(torch.device("cpu"))
+        ops.check_kernel_status(torch.device("cpu"))            # told once
+
+
 def test_refused_off_the_device():
     with pytest.raises(ops.KernelError, match="CUDA"):
         ops.beam_select(**_select_args())
