@@ -356,6 +356,48 @@ def test_one_beam_is_greedy_generation(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("lengths", [(70, 1, 33), (64, 128, 5)])
+def test_one_beam_in_bfloat16_takes_what_a_prompt_prefers(lengths):
+    """Every token of the one text is within the engine's tolerance (3e-2 of the largest logit, for the step and for the prompt) of the best, and the
+    score is the sum of those log-probabilities."""
+    model = random_model(LLAMA_C, "bfloat16")
+    prompts = [random_tokens(n, 256, n) for n in lengths]
+    got, _ = model.generate_beams(prompts, beams=1, max_tokens=40, ignore_eos=True, return_all=True)
+    for prompt, (text,) in zip(prompts, got):
+        assert len(text.tokens) == 40 and text.reason == "length"
+        rows = torch.cat([by_prompts(model, prompt)([text.tokens[:i]]) for i in range(40)]).double()
+        taken = rows.gather(1, torch.tensor(text.tokens)[:, None])[:, 0]
+        tolerance = 2 * 3e-2 * rows.abs().max(1).values
+        assert torch.all(taken >= rows.max(1).values - tolerance)
+        assert abs(float((taken - rows.logsumexp(1)).sum()) - text.score) <= float(tolerance.sum())
+
+
+@gpu
+@pytest.mark.parametrize("name, beams, lengths", [("llama A", 4, (200, 64, 9)), ("llama A", 16, (130, 63)), ("llama B", 7, (128, 1, 100))])
+def test_attention_within_a_search_is_each_rows_own(name, beams, lengths, monkeypatch):
+    """Every call of `attention_beams` that a search makes, in every layer of every step, against the definition over the rows' own pages in 64 bits: pages
+    said to be shared that are not, tables or copies a step behind would show in it."""
+    import plain_beams
+    from janus_b200.kernels import ops
+    from test_beams import attention_bound
+    calls, attention = [], ops.attention_beams
+    monkeypatch.setattr(ops, "beams_pay", lambda *sizes: True)
+
+    def compared(q, k, v, out, table, kv_len, shared, K, nh, nkv, hd, page_size, scale, workspace, bound):
+        attention(q, k, v, out, table, kv_len, shared, K, nh, nkv, hd, page_size, scale, workspace, bound)
+        want, size = plain_beams.attention(q, k, v, table.tolist(), kv_len.tolist(), nh, nkv, hd, scale)
+        off = (out.cpu().double().view(want.shape) - want).abs()
+        calls.append((float((off / attention_bound(want, size)).max()), int(shared.max())))
+
+    monkeypatch.setattr(ops, "attention_beams", compared)
+    model = random_model(DESIGNS[name], "bfloat16", use_graphs=False)
+    prompts = [random_tokens(n, model.engine.model.vocab_size, n) for n in lengths]
+    model.generate_beams(prompts, beams=beams, max_tokens=24, ignore_eos=True)
+    layers = DESIGNS[name]["num_hidden_layers"]
+    assert len(calls) == 23 * layers and max(c[0] for c in calls) <= 1.0 and max(c[1] for c in calls) == max(lengths) // 64
+
+
+@gpu
 def test_with_and_without_graphs():
     out = []
     for graphs in (True, False):

@@ -630,6 +630,49 @@ def test_attention_a_value_that_is_not_finite_is_one_number_of_a_row(hd, K, grou
     assert float(off[~bad].max()) <= 1.0
 
 
+def climbing_case(R, K, kv_len, shared, nkv, group, hd, seed):
+    """Scores that climb (or fall, or stay) along the keys, each beam's and head's by a slope of its own: -48 to 48 from the first key to the last,
+    69 powers of two.  A query has 16 numbers that are not 0."""
+    q, k, v, table, nh = attention_case(R, K, kv_len, shared, nkv, group, hd, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    longest = max(kv_len)
+    fine = torch.isfinite(k[:, 0, :, 0])
+    place = torch.zeros(k.shape[0], PAGE)                    # of a key in its row, as far as rows agree
+    for row, n in zip(table, kv_len):
+        for i in range(-(-n // PAGE)):
+            place[row[i]] = torch.arange(i * PAGE, (i + 1) * PAGE) / longest
+    slope = (torch.arange(R * K * nh).view(R * K, nh) % 7 - 3) * 16.0
+    q = torch.zeros(R * K, nh, hd)
+    q[:, :, 8:16] = torch.randn(R * K, nh, 8, generator=g) * 0.3
+    q[:, :, :8] = slope[:, :, None] / 8 * math.sqrt(hd)
+    k = torch.where(fine[:, None, :, None], torch.randn(k.shape, generator=g), k.float())
+    k[..., :8] = torch.where(fine[:, None, :, None], place[:, None, :, None] + torch.randn(*k.shape[:-1], 8, generator=g) * 0.01, k[..., :8])
+    return q.view(R * K, nh * hd).bfloat16(), k.bfloat16(), v, table, nh
+
+
+@gpu
+@pytest.mark.parametrize("blocks", [2, 7, 74])
+@pytest.mark.parametrize("K, group, hd", [(4, 4, 64), (4, 4, 128), (4, 4, 256), (4, 7, 64), (4, 7, 128), (4, 7, 256), (8, 8, 64), (8, 8, 128), (8, 8, 256),
+                                          (16, 8, 64), (16, 8, 128), (16, 8, 256)])
+def test_attention_scores_that_climb(K, group, hd, blocks, monkeypatch):
+    """Sums and results are scaled down in the middle of a run of keys again and again, by factors between 0 and 1 that differ from row to row; tiles of 16 to
+    128 rows, the list cut into few shares (runs of many stages) and many.  Errors: 16 products of a query, |q k| scale below 64 together, summed
+    in float32 within 16 * 64 / 2^24 = 2^-14; scaled by log2(e) and rounded below 128, 2^-18, and once more as a distance: with the power's 2^-22
+    less than 2^-11 of a weight."""
+    plan = ops.beam_attention_plan
+    monkeypatch.setattr(ops, "beam_attention_plan", lambda *sizes: (blocks, plan(*sizes)[1]))
+    kv_len = [1300 - 20 * (k % 3) for k in range(K)] + [1700] * K
+    shared = [14, 26]
+    q, k, v, table, nh = climbing_case(2, K, kv_len, shared, 2, group, hd, K + hd)
+    out = empty(2 * K, nh * hd, dtype=torch.bfloat16)
+    scale = 1.0 / math.sqrt(hd)
+    ops.attention_beams(q.cuda(), k.cuda(), v.cuda(), out, ints(table), ints(kv_len), ints(shared), K, nh, 2, hd, PAGE, scale,
+                        Workspace(torch.device("cuda")), max(kv_len))
+    want, size = P.attention(q, k, v, table, kv_len, nh, 2, hd, scale)
+    off = (out.cpu().double().view(2 * K, nh, hd) - want).abs()
+    assert float((off / attention_bound(want, size)).max()) <= 1.0
+
+
 @gpu
 @pytest.mark.parametrize("size", [1e3, 1e15, 1e18])
 @pytest.mark.parametrize("K, group, hd", [(4, 4, 128), (5, 2, 64), (16, 4, 64), (3, 2, 256)])
