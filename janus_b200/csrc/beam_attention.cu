@@ -924,7 +924,9 @@ JB_EXPORT int jb_attention_beams(const void* q, const void* k_cache, const void*
   JB_REFUSE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)part) % 16, "attention_beams: q, out or workspace not on a boundary of 16 bytes");
   const size_t row_bytes = (size_t)R * K * nh * hd * 2, cache_bytes = (size_t)n_pages * nkv * PAGE * hd * 2;
   auto over = [&](const void* other, size_t bytes) { return (uintptr_t)out < (uintptr_t)other + bytes && (uintptr_t)other < (uintptr_t)out + row_bytes; };
-  if (over(q, row_bytes) || over(k_cache, cache_bytes) || over(v_cache, cache_bytes)) return JB_ERR_OVERLAP;
+  if (over(q, row_bytes) || over(k_cache, cache_bytes) || over(v_cache, cache_bytes) || over(table, (size_t)R * K * W * 4) ||
+      over(kv_len, (size_t)R * K * 4) || over(shared, (size_t)R * 4))
+    return JB_ERR_OVERLAP;
   CUtensorMap maps[2];
   if (!jb::make_map_64(&maps[0], k_cache, (uint64_t)n_pages * nkv * PAGE, hd, PAGE, true) ||
       !jb::make_map_64(&maps[1], v_cache, (uint64_t)n_pages * nkv * PAGE, hd, PAGE, true))

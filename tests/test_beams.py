@@ -953,6 +953,17 @@ def test_attention_addresses_refused():
 
 
 @gpu
+@pytest.mark.parametrize("name", ["block_table", "kv_len", "shared"])
+def test_attention_output_over_the_tables_refused(name):
+    args = _attention_args(device="cuda")
+    args["workspace"] = Workspace(torch.device("cuda"))
+    words = args["out"].view(torch.int32).view(-1)
+    args[name] = words[128: 128 + args[name].numel()].view(args[name].shape)
+    with pytest.raises(ops.KernelError, match="10004"):
+        ops.attention_beams(**args)
+
+
+@gpu
 def test_reorder_a_matrix_twice_refused():
     m, i = torch.zeros(2, 8, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
     with pytest.raises(ops.KernelError, match="twice"):
