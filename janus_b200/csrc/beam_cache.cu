@@ -7,6 +7,7 @@
 // All three work in place: a thread has one column (of a group's tables, of its states) for all K rows, so that it has read what
 // goes elsewhere before it writes, without a second buffer or a barrier.
 #include <cooperative_groups.h>
+#include <algorithm>
 #include <stddef.h>
 #include <stdio.h>
 #include <string.h>
@@ -266,6 +267,21 @@ bool fork_overlaps(const Fork& a) {
   return false;
 }
 
+// A stretch of memory that is written.  Whether any two of n share a byte, or one with a list of `words` numbers that is read (sorts them).
+// `same_twice`: the very same stretch may be there again.
+struct Span {
+  uintptr_t at, end;
+};
+bool spans_overlap(Span* spans, int n, bool same_twice, const int* const* lists, int n_lists, size_t words) {
+  std::sort(spans, spans + n, [](const Span& x, const Span& y) { return x.at < y.at || (x.at == y.at && x.end < y.end); });
+  for (int i = 1; i < n; ++i)
+    if (spans[i].at < spans[i - 1].end && !(same_twice && spans[i].at == spans[i - 1].at && spans[i].end == spans[i - 1].end)) return true;
+  for (int l = 0; l < n_lists; ++l)
+    for (int i = 0; i < n; ++i)
+      if ((uintptr_t)lists[l] < spans[i].end && spans[i].at < (uintptr_t)lists[l] + 4 * words) return true;
+  return false;
+}
+
 template <int KM, int THREADS>
 cudaError_t fork_launch(const Fork& a, cudaStream_t stream) {
   const size_t memory = (size_t)((a.P + 31) / 32) * 8;
@@ -427,6 +443,7 @@ JB_EXPORT int jb_copy_pages(const void* pages, const void* heads, const void* ro
   a.src = src, a.dst = dst, a.rows = rows, a.n_pages = n_pages, a.page_size = page_size;
   uintptr_t all = 0;
   long long most = 0;
+  Span spans[MOST_TENSORS];
   for (int i = 0; i < n_tensors; ++i) {
     CopyTensor& t = a.tensors[i];
     t.pages = ((char* const*)pages)[i];
@@ -437,7 +454,10 @@ JB_EXPORT int jb_copy_pages(const void* pages, const void* heads, const void* ro
               t.row_bytes);
     all |= (uintptr_t)t.pages | (uintptr_t)t.row_bytes;
     if (bytes > most) most = bytes;
+    spans[i] = Span{(uintptr_t)t.pages, (uintptr_t)t.pages + (uintptr_t)bytes * n_pages};
   }
+  const int* lists[3] = {src, dst, rows};
+  if (spans_overlap(spans, n_tensors, true, lists, 3, (size_t)n)) return JB_ERR_OVERLAP;
   // A block for a whole page where that gives every multiprocessor some, else a block for each of the page's parts of eight vectors a thread.
   const long long blocks = (long long)n * n_tensors, most_parts = (most + COPY_THREADS * 128 - 1) / (COPY_THREADS * 128);
   a.parts = (int)(blocks >= 148 * 16 ? 1 : most_parts < 1 ? 1 : most_parts > 64 ? 64 : most_parts);
@@ -457,12 +477,16 @@ JB_EXPORT int jb_reorder_rows(const void* matrices, const void* numbers, int n_m
   a.slots = slots, a.parents = parents, a.K = K, a.n_slots = n_slots;
   bool wide = true;
   long long most = 0;
+  Span spans[MOST_MATRICES];
   for (int i = 0; i < n_matrices; ++i) {
     a.matrices[i] = ((char* const*)matrices)[i];
     a.row_words[i] = ((const long long*)numbers)[i];
     wide &= (uintptr_t)a.matrices[i] % 16 == 0 && a.row_words[i] % 4 == 0;
     if (a.row_words[i] > most) most = a.row_words[i];
+    spans[i] = Span{(uintptr_t)a.matrices[i], (uintptr_t)a.matrices[i] + 4 * (uintptr_t)a.row_words[i] * n_slots};
   }
+  const int* lists[2] = {slots, parents};
+  if (spans_overlap(spans, n_matrices, false, lists, 2, (size_t)groups * K)) return JB_ERR_OVERLAP;
   if (!wide) return (int)move_for<float>(a, n_matrices, groups, most, stream);
   for (int i = 0; i < n_matrices; ++i) a.row_words[i] /= 4;
   return (int)move_for<float4>(a, n_matrices, groups, most / 4, stream);

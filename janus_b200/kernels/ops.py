@@ -2782,8 +2782,8 @@ COPY_PAGES = 128        # tensors that one launch of `copy_pages` takes
 def copy_pages(tensors: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor, rows: torch.Tensor) -> None:
     """For every i with src[i] and dst[i] among the pages: the first rows[i] tokens of each head of page src[i] are copied to page dst[i], in
     every tensor ([pages, heads, page size, numbers], 2 or 4 bytes a number; heads and numbers may differ).  src, dst, rows: int32
-    [n].  Pages that are copied to differ from one another and from those that are copied from.  Up to COPY_PAGES tensors go in
-    one launch."""
+    [n].  Pages that are copied to differ from one another and from those that are copied from.  Tensors share no memory, but for one
+    that is given twice.  Up to COPY_PAGES tensors go in one launch."""
     n = src.shape[0]
     if not tensors or n == 0:
         return
@@ -2819,7 +2819,7 @@ REORDER_ROWS = 64       # matrices that one launch of `reorder_rows` takes
 def reorder_rows(matrices: Sequence[torch.Tensor], slots: torch.Tensor, parents: torch.Tensor) -> None:
     """In every float32 tensor (its first axis: slots), in place: row slots[r K + k] becomes what row slots[r K + parents[r, k]] was.
     parents [R, K] (up to MOST_BEAMS), slots [R K], int32, no slot twice; a parent outside 0 .. K - 1, or a slot outside the tensor, leaves
-    the row as it was.  Up to REORDER_ROWS tensors go in one launch."""
+    the row as it was.  Tensors share no memory.  Up to REORDER_ROWS of them go in one launch."""
     R, K = parents.shape
     if not 1 <= K <= MOST_BEAMS:
         raise KernelError(f"reorder_rows: groups of {K} rows (1 to {MOST_BEAMS})")

@@ -964,6 +964,32 @@ def test_attention_output_over_the_tables_refused(name):
 
 
 @gpu
+def test_copies_and_moves_over_one_another_refused():
+    """Views that share some of their memory; a tensor of pages given twice, of which both copies are the same, is taken."""
+    i = torch.zeros(2, dtype=torch.int32, device="cuda")
+    some = torch.arange(4 * 64 * 8, dtype=torch.float32, device="cuda")
+    a, b = some[: 2 * 64 * 8].view(2, 1, 64, 8), some[64 * 8: 3 * 64 * 8].view(2, 1, 64, 8)
+    lists = [torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0], [1], [3])]
+    with pytest.raises(ops.KernelError, match="10004"):
+        ops.copy_pages([a, b], *lists)
+    with pytest.raises(ops.KernelError, match="10004"):
+        ops.copy_pages([a], some[:1].view(torch.int32), lists[1], lists[2])
+    before = a.clone()
+    ops.copy_pages([a, a], *lists)
+    assert torch.equal(a[1, :, :3], before[0, :, :3]) and torch.equal(a[1, :, 3:], before[1, :, 3:])
+    m, n = some[:32].view(4, 8), some[8:40].view(4, 8)
+    with pytest.raises(ops.KernelError, match="10004"):
+        ops.reorder_rows([m, n], i, i.view(1, 2))
+    with pytest.raises(ops.KernelError, match="10004"):
+        ops.reorder_rows([m], m.view(-1)[4:6].view(torch.int32), i.view(1, 2))
+    # lists are read: they may be one another
+    slots = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    before = m.clone()
+    ops.reorder_rows([m], slots, slots.view(1, 2))              # row 1 becomes row 0, and row 0 row 1
+    assert torch.equal(m[:2], before[:2].flip(0)) and torch.equal(m[2:], before[2:])
+
+
+@gpu
 def test_reorder_a_matrix_twice_refused():
     m, i = torch.zeros(2, 8, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
     with pytest.raises(ops.KernelError, match="twice"):
