@@ -13,7 +13,7 @@
 // second launch joins those.
 //
 // 32 heads over 8 of 128 numbers, 16 requests of 8 beams behind 6,000 to 24,000 tokens: 97 us for the 85 that 560 MB take; twice as
-// long 172 for 161, of 16 beams 122 for 94, with heads of 64 numbers 63 for 43; 16 heads over 4 of 256 104 for 86, of 16 beams 142
+// long 166 for 161, of 16 beams 120 for 94, with heads of 64 numbers 60 for 43; 16 heads over 4 of 256 100 for 86, of 16 beams 140
 // for 94; one request of 4 beams behind 300 9.1.
 #include <math_constants.h>
 #include <stdio.h>
@@ -879,9 +879,10 @@ cudaError_t allow(Kernel kernel, int bytes, bool (&ready)[64]) {
   if (e == cudaSuccess && device < 64) ready[device] = true;
   return e;
 }
-// `shares`: of the list, how many.  A block of rows that is cut into many parts has a block of warps a row (6 requests of 5 beams that parted
-// long ago, 12 to a block of rows: 20 us the call, 23 by a warp a row), others a warp (16 of 8 beams behind 6,000 to 24,000: 105 and 109;
-// both as the kernel before was then).
+// `shares`: of the list, how many.  A block of rows that is cut into many parts has a block of warps a row, others a warp.  Both sides over 180
+// shapes (4 and 8 beams of 1 to 64 requests, three kinds of heads, 300 to 16,000 tokens), by shares a block of rows: at 0.3 53 us by a warp and 66
+// by a block, at 2.3 13.9 and 15.0, at 4.6 level, at 9 32 and 30, at 18 16.2 and 13.7, at 37 27.5 and 20.3.  From 4 on costs 0.9 % on average, 15 %
+// at most (from 6 or 8 on 0.5 %).
 cudaError_t join(const Args& a, int rows, int shares, cudaStream_t stream) {
   const int items = a.R * a.K * a.nh;
   if (shares > 4 * a.R * a.row_blocks * a.nkv) {

@@ -295,7 +295,8 @@ cudaError_t fork_launch(const Fork& a, cudaStream_t stream) {
 
 // ------------------------------------------------------------ copies ------------------------------------------------------------
 // Bound by bytes.  A block has one page of one tensor (or a part of it); a head's first tokens lie in one piece.  512 rows' copies in 32
-// tensors, 0.9 GB to and fro, 121 us (7.5 TB/s: several beams copy the same page, which L2 serves again); 4 rows' in as many 3.4.
+// tensors, 0.9 GB to and fro, 121 us (7.5 TB/s: several beams copy the same page, which L2 serves again; a page read once, 113 us at the copy
+// rate); 4 rows' in as many 3.2.
 constexpr int COPY_THREADS = 256;
 constexpr int MOST_TENSORS = 128;
 
@@ -342,8 +343,8 @@ __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const __grid_c
 
 // ------------------------------------------------------------ states ------------------------------------------------------------
 // Bound by bytes: every state that goes elsewhere is read once for all the rows it goes to (again from the block's own cache), rows
-// that stay are not touched.  40 requests of 5 beams, 12 matrices of 0.5 MB a slot: 150 us for 0.9 GB (92 % of the copy rate); one of 4 beams
-// 2.9.  A thread has four columns for 4 rows, two for 8, one beyond: as much as its registers hold on the way.
+// that stay are not touched.  40 requests of 5 beams, 12 matrices of 0.5 MB a slot: 150 us for 0.83 GB (85 % of the copy rate; what
+// beams are lost makes it 0.77 to 0.87); one of 4 beams 2.9.  A thread has four columns for 4 rows, two for 8, one beyond: as much as its registers hold on the way.
 constexpr int MOVE_THREADS = 256;
 constexpr int MOST_MATRICES = 64;
 
