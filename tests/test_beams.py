@@ -235,6 +235,40 @@ def test_select_beams_that_float32_sums_do_not_tell_apart(R, K, V):
             check_select(x, scores, stops, in_place, gap_needed=False)
 
 
+@gpu
+def test_select_beams_that_float32_sums_do_not_tell_apart_replayed():
+    """The same from a graph on another stream, scores changed in place from step to step: rows are summed again in some replays and not in others."""
+    x, scores = near_beams(6, 8, 50257, 6 + 50257)
+    R, K = scores.shape
+    logits, stops, far = x.cuda(), ints([int(t) for t in x[::K].argmax(1)]), -torch.rand(R, K, generator=torch.Generator().manual_seed(3))
+
+    def outputs():
+        return dict(parents=empty(R, K), tokens=empty(R, K), ended_parents=empty(R, K), ended_tokens=empty(R, K),
+                    ended_scores=empty(R, K, dtype=torch.float32))
+
+    want, given = [], (scores, far, scores - 1.0, far - 3.0)
+    for start in given:
+        held, out = start.cuda(), outputs()
+        for _ in range(2):
+            ops.beam_select(logits, held, stops, next_scores=held, **out, workspace=Workspace(torch.device("cuda")))
+        want.append([held] + list(out.values()))
+    torch.cuda.synchronize()
+    side, workspace, held, out = torch.cuda.Stream(), Workspace(torch.device("cuda")), scores.cuda(), outputs()
+    with torch.cuda.stream(side):
+        ops.beam_select(logits, held, stops, next_scores=held, **out, workspace=workspace)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        graph.capture_begin()
+        ops.beam_select(logits, held, stops, next_scores=held, **out, workspace=workspace)
+        graph.capture_end()
+        for start, w in zip(given, want):
+            held.copy_(start)
+            graph.replay()
+            graph.replay()
+            side.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip([held] + list(out.values()), w))
+
+
 def log_weight_of_the_largest(x):
     """log softmax(x) of each row's largest number, from the distances to it (far from 0 their difference is all that 64 bits hold)."""
     return -(x.double() - x.double().max(1, keepdim=True).values).exp().sum(1).log()
