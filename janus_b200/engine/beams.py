@@ -107,7 +107,7 @@ def table_width(pages: int) -> int:
     return W
 
 
-def stateless_pages(R: int, K: int, W: int) -> Tuple[int, int]:
+def position_pages(R: int, K: int, W: int) -> Tuple[int, int]:
     """(tokens of a page, pages) of the table of a model whose mixers keep only states.  Nobody stores anything in its pages: they carry positions
     and lengths, and one is as long as the longest text.  Page 0 for rows without a beam, one a prompt, one a beam."""
     return W * PAGE_SIZE, 1 + R + R * K
@@ -140,7 +140,7 @@ class _BeamStep:
         self.stops = torch.full((stops,), -1, **i32)
         self.page_size, self.pages = PAGE_SIZE, [g.pool.n_pages for g in cache.groups]
         if not cache.groups:
-            self.page_size, n = stateless_pages(R, K, W)
+            self.page_size, n = position_pages(R, K, W)
             self.pages = [n]
         self.tables = [_Tables(R, K, W if cache.groups else 1, n, device) for n in self.pages]
         self.lengths = torch.zeros((R, K), **i32)
@@ -324,7 +324,7 @@ class BeamRunner:
                 if pages > free:
                     break
             else:
-                size, count = stateless_pages(n + 1, beams, table_width(longest))
+                size, count = position_pages(n + 1, beams, table_width(longest))
                 if count > ops.MOST_FORK_PAGES or size * count > ops.MOST_FORK_TOKENS:
                     break
             n += 1

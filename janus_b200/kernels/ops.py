@@ -2740,12 +2740,12 @@ def fork_pages(parents: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor
 
     Rows come in R groups of K (up to MOST_BEAMS).  Row r K + k goes on with what row r K + parents[r, k] holds: lengths[r, parents[r, k]]
     tokens in the pages that `table` [R K, W] lists for it; a parent outside 0 .. K - 1 means that the row does not go on.  refs [P] (up to
-    MOST_FORK_PAGES, of MOST_FORK_TOKENS tokens) counts who holds a page: rows of the table, and anybody else (a page that is to stay has a holder outside).  free_pages[:n_free] are pages
-    that nobody holds.  Each row that goes on is made ready for one more token.  Whole pages are held by all rows that go on with
-    them.  The page that the token goes to stays with the lowest row of the group that holds it, if nobody else does; any other row
-    takes a page of its own from the back of the free list, with a copy to be made where the page is partly filled (a partly filled page is
-    held by the rows of one group only, or by holders outside).  Pages that nobody holds any longer come back first, behind the free
-    ones, in order of number.
+    MOST_FORK_PAGES, of MOST_FORK_TOKENS tokens) counts who holds a page: rows of the table, and anybody else (a page that is to stay has a
+    holder outside).  free_pages[:n_free] are pages that nobody holds.  Each row that goes on is made ready for one more token.  Whole pages
+    are held by all rows that go on with them.  The page that the token goes to stays with the lowest row of the group that holds it, if
+    nobody else does; any other row takes a page of its own from the back of the free list, with a copy to be made where the page is partly
+    filled (a partly filled page is held by the rows of one group only, or by holders outside).  Pages that nobody holds any longer come
+    back first, behind the free ones, in order of number.
 
     Made: new_table, new_refs, new_free (-1 behind new_n_free); kv_len, positions and dest_rows [R, K], the length with the token, its
     position and its cache row; copy_src, copy_dst and copy_rows [R, K], what `copy_pages` has to copy (-1, -1, 0: nothing);

@@ -128,12 +128,12 @@ def _runner(cache):
 @pytest.mark.parametrize("requests, beams, length, limit", [(64, 4, 40, 66000), (1024, 1, 3, 70), (32, 32, 1000, 130000), (1, 32, 1, (1 << 25) - 64)])
 def test_batches_of_models_that_keep_only_states(requests, beams, length, limit):
     """Their tables are of pages that hold nothing; whatever a batch's slots have room for, they are what `ops.fork_pages` takes."""
-    from janus_b200.engine.beams import stateless_pages, table_width
+    from janus_b200.engine.beams import position_pages, table_width
     from janus_b200.kernels import ops
     prompts, searches = [[1] * length] * requests, [_Search(i, limit) for i in range(requests)]
     n = _runner(_cache(1024))._batch_size(prompts, searches, 0, beams, requests)
     assert n == requests
-    size, pages = stateless_pages(n, beams, table_width(-(-(length + limit) // 64)))
+    size, pages = position_pages(n, beams, table_width(-(-(length + limit) // 64)))
     assert size >= length + limit and pages <= ops.MOST_FORK_PAGES and size * pages <= ops.MOST_FORK_TOKENS
 
 
